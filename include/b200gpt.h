@@ -282,6 +282,31 @@ int b200_attn_decode_tune(int force_scalar);
 size_t b200_attn_decode_noalloc_max_bytes(void);
 int b200_attn_decode_noalloc(const b200_attn_decode_args* args, b200_stream_t stream);
 
+/* One decode step of `batch` rows that share a prefix (several answers to one prompt): as b200_attn_decode, but keys and values 0 .. n - 1 are the prefix's,
+ * held once, and position p >= n of row b is at p - n of the row's own cache, where the step appends its rotated k and its v.
+ *   qkv        (batch, (n_head + 2 n_groups) * head_size) bf16, interleaved per group as in b200_attn_decode
+ *   pos        one position for all rows or one per row (pos_count), on the device.  A row at a negative position takes no part: its cache stays as it is, its
+ *              result is zero.  A position whose place lies outside the own cache uses the cache's nearest row.
+ *   prefix_len on the device, clamped to 0 .. prefix_rows; NULL: prefix_rows.  (Captured launches follow both as they change.)
+ *   k_cache, v_cache   (batch, n_groups, own_rows, head_size) bf16, rows head_size apart, batches and groups at the given distances (elements)
+ *   k_prefix, v_prefix (n_groups, prefix_rows, head_size) bf16 likewise; not read where prefix_rows is 0
+ *   cos, sin   (table_rows, rope_n_elem), row = position (clamped); table_preselected: row = index of the position in pos
+ * head_size 64 or 128.  Caches, prefix and workspace on 16-byte boundaries, distances multiples of 8.  The workspace needs no initial contents; two calls that
+ * run at the same time need one each. */
+typedef struct b200_attn_decode_shared_args {
+  const void* qkv;
+  const void* cos; const void* sin; int table_dtype, table_rows, table_preselected, rope_n_elem;
+  const void* pos; int pos_is_int64, pos_count;
+  const void* prefix_len; int prefix_len_is_int64;
+  void* k_cache; void* v_cache; int64_t k_batch_stride, k_group_stride, v_batch_stride, v_group_stride;
+  const void* k_prefix; const void* v_prefix; int64_t k_prefix_stride, v_prefix_stride;
+  void* out;                  /* (batch, n_head * head_size) bf16 */
+  int batch, n_head, n_groups, head_size, own_rows, prefix_rows;
+  void* workspace; size_t workspace_bytes;
+} b200_attn_decode_shared_args;
+size_t b200_attn_decode_shared_workspace_bytes(int batch, int n_head, int n_groups, int head_size, int prefix_rows, int own_rows);
+int b200_attn_decode_shared(const b200_attn_decode_shared_args* args, b200_stream_t stream);
+
 /* ---- prefill helper: RoPE + KV-cache write for T > 1 tokens at positions pos[0..T) (lit_gpt/model.py:624-649).
  * table_preselected = 1: cos/sin are (T, rope_n_elem) rows already gathered by input_pos; 0: full tables.
  * Writes roped q to q_out (batch, n_head, T, head_size) and the roped k / v rows into the GQA-native caches. */
@@ -734,6 +759,47 @@ int b200_attn_prefill_mixed(const void* q, int64_t ldq, const void* k_cache, int
                             int n_kv_head, int head_size, float scale, float* sbuf, int64_t s_ld, b200_stream_t stream);
 size_t b200_talk_attn_workspace_bytes(int64_t rows, int n_head, int dv, int n_split);
 int b200_talk_attn(const b200_talk_attn_args* args, b200_stream_t stream);
+
+/* ---- several rows of logits ---------------------------------------------------------------------------------------------------- */
+/* Rules that change logits before a draw, fp32 with every step rounded by itself.  With n = counts[b, v] (NULL: none; below zero counts as zero), where n > 0:
+ * l = l > 0 ? l / repetition : l * repetition; l = l - frequency * n; l = l - presence.  Then l = l + bias[v] (NULL: none), and -inf for tokens whose bit
+ * (v % 32 of word v / 32) in `allowed` (NULL: all allowed) is 0.  logits (rows, vocab) bf16 or fp32, rows `ld` elements apart (0: one row for all); counts, bias
+ * and allowed likewise with their own distances.  repetition, frequency, presence: one number per row on the device, or NULL for the number in *_all. */
+typedef struct b200_logit_rules {
+  const void* logits; int logits_dtype; int64_t ld;
+  int64_t rows, vocab;
+  const int32_t* counts; int64_t counts_ld;
+  const float* repetition; const float* frequency; const float* presence;
+  float repetition_all, frequency_all, presence_all;
+  const float* bias; int64_t bias_ld;
+  const int32_t* allowed; int64_t allowed_ld;
+} b200_logit_rules;
+/* out (rows, vocab) bf16 or fp32, rows out_ld apart; may be the logits themselves (same type and distance). */
+int b200_adjust_logits(const b200_logit_rules* rules, void* out, int out_dtype, int64_t out_ld, b200_stream_t stream);
+/* One draw per row from softmax(top_k(adjusted logits) / temperature), as b200_sample draws for one: kept are the top_k largest (<= 0 or >= vocab: all; equal
+ * ones in the order of the tokens), the token is the argmax over them of (l - max) / T - ln e with e from noise (rows, vocab; Exp(1) values) or from the row's Philox
+ * state rng_state[b] = (seed, offset), whose offset moves on by one; temperature <= 0: argmax, the lowest token of equal ones.  NaN logits are never drawn.  A row
+ * that allows nothing gives token -1 and log-probability -inf.  logprob_out[b] (optional): ln of the token's probability among those kept (temperature <= 0: among
+ * all, at temperature 1).  count: rules->counts[b, token] += 1.  pos_inout[b] (optional) += 1, and history[b, pos] = token where pos < history_len.
+ * temperature, top_k: one per row on the device, or NULL for the number in *_all.  The result does not depend on how rows are cut or which run with them. */
+typedef struct b200_draw_args {
+  const float* temperature; float temperature_all;
+  const int32_t* top_k; int top_k_all;
+  int64_t* rng_state; const float* noise; int64_t noise_ld;
+  void* token_out; int token_is_int64;
+  float* logprob_out;
+  int count;
+  void* pos_inout; int pos_is_int64;
+  void* history; int64_t history_ld, history_len;
+} b200_draw_args;
+int b200_sample_rows(const b200_logit_rules* rules, const b200_draw_args* args, b200_stream_t stream);
+
+/* ---- copies between cache slots -------------------------------------------------------------------------------------------------- */
+/* For every copy and every tensor (slots, rows, row_bytes contiguous bytes each): slot dst = slot src, the leading `rows` rows of it, or all where copy.rows < 0.
+ * Tables are host memory, read before the call returns.  A slot that is written is read by no copy and written by no other: anything else is refused. */
+typedef struct b200_slot_tensor { void* base; int64_t rows, row_bytes; } b200_slot_tensor;
+typedef struct b200_slot_copy { int32_t src, dst; int64_t rows; } b200_slot_copy;
+int b200_copy_slots(const b200_slot_tensor* tensors, int n_tensors, int slots, const b200_slot_copy* copies, int n_copies, b200_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -151,6 +151,35 @@ class LinearAttnArgs(ctypes.Structure):  # mirrors b200_linear_attn_args
                 ("workspace_bytes", c_size_t), ("qk_f32", c_int)]
 
 
+class AttnDecodeSharedArgs(ctypes.Structure):  # mirrors b200_attn_decode_shared_args
+    _fields_ = [("qkv", c_void_p), ("cos", c_void_p), ("sin", c_void_p), ("table_dtype", c_int), ("table_rows", c_int), ("table_preselected", c_int),
+                ("rope_n_elem", c_int), ("pos", c_void_p), ("pos_is_int64", c_int), ("pos_count", c_int), ("prefix_len", c_void_p), ("prefix_len_is_int64", c_int),
+                ("k_cache", c_void_p), ("v_cache", c_void_p), ("k_batch_stride", c_int64), ("k_group_stride", c_int64), ("v_batch_stride", c_int64),
+                ("v_group_stride", c_int64), ("k_prefix", c_void_p), ("v_prefix", c_void_p), ("k_prefix_stride", c_int64), ("v_prefix_stride", c_int64),
+                ("out", c_void_p), ("batch", c_int), ("n_head", c_int), ("n_groups", c_int), ("head_size", c_int), ("own_rows", c_int), ("prefix_rows", c_int),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class LogitRules(ctypes.Structure):  # mirrors b200_logit_rules
+    _fields_ = [("logits", c_void_p), ("logits_dtype", c_int), ("ld", c_int64), ("rows", c_int64), ("vocab", c_int64), ("counts", c_void_p), ("counts_ld", c_int64),
+                ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p), ("repetition_all", c_float), ("frequency_all", c_float),
+                ("presence_all", c_float), ("bias", c_void_p), ("bias_ld", c_int64), ("allowed", c_void_p), ("allowed_ld", c_int64)]
+
+
+class DrawArgs(ctypes.Structure):  # mirrors b200_draw_args
+    _fields_ = [("temperature", c_void_p), ("temperature_all", c_float), ("top_k", c_void_p), ("top_k_all", c_int), ("rng_state", c_void_p), ("noise", c_void_p),
+                ("noise_ld", c_int64), ("token_out", c_void_p), ("token_is_int64", c_int), ("logprob_out", c_void_p), ("count", c_int), ("pos_inout", c_void_p),
+                ("pos_is_int64", c_int), ("history", c_void_p), ("history_ld", c_int64), ("history_len", c_int64)]
+
+
+class SlotTensor(ctypes.Structure):  # mirrors b200_slot_tensor
+    _fields_ = [("base", c_void_p), ("rows", c_int64), ("row_bytes", c_int64)]
+
+
+class SlotPair(ctypes.Structure):  # mirrors b200_slot_copy
+    _fields_ = [("src", ctypes.c_int32), ("dst", ctypes.c_int32), ("rows", c_int64)]
+
+
 class GatedResidualArgs(ctypes.Structure):  # mirrors b200_gated_residual_args
     _fields_ = [("y0", c_void_p), ("slot_of", c_void_p), ("wts", c_void_p), ("top", c_int), ("y1", c_void_p), ("gate", c_void_p), ("scale", c_void_p),
                 ("mult", c_float), ("x", c_void_p), ("w", c_void_p), ("plus_one", c_int), ("act", c_void_p), ("rows", c_int64), ("d", c_int), ("eps", c_float),
@@ -170,7 +199,7 @@ ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_RELU2 = 0, 1, 2, 3
 # expert kernels: `load_core()` can serve them from a library built from those sources alone.
 _CORE_SOURCES = ("api.cu", "norm.cu", "sample.cu", "resid.cu", "latent.cu", "moe.cu", "attn_prefill.cu", "attn_tc05.cu", "shortconv.cu", "delta.cu",
                  "delta_chunk.cu", "window_attn.cu",
-                 "linear_attn.cu", "depth.cu", "rope.cu", "talk_attn.cu")
+                 "linear_attn.cu", "depth.cu", "rope.cu", "talk_attn.cu", "logits.cu", "slots.cu")
 _CORE_SIGNATURES = {
     "b200_embed_pos": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "b200_rms_rows": (c_int, [ctypes.POINTER(RmsRowsSeg), c_int, c_int64, c_float, c_int, c_int, c_void_p]),
@@ -237,6 +266,9 @@ _CORE_SIGNATURES = {
                                             c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "b200_ring_store": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_int,
                                 c_void_p]),
+    "b200_adjust_logits": (c_int, [ctypes.POINTER(LogitRules), c_void_p, c_int, c_int64, c_void_p]),
+    "b200_sample_rows": (c_int, [ctypes.POINTER(LogitRules), ctypes.POINTER(DrawArgs), c_void_p]),
+    "b200_copy_slots": (c_int, [ctypes.POINTER(SlotTensor), c_int, c_int, ctypes.POINTER(SlotPair), c_int, c_void_p]),
 }
 _CORE_SHARED = ("b200_abi_version", "b200_last_error", "b200_device_info", "b200_set_pdl", "b200_launch_count", "b200_rmsnorm", "b200_swiglu",
                 "b200_embedding", "b200_argmax", "b200_sample", "b200_attn_prefill", "b200_wait_error", "b200_wait_errors_take", "b200_wait_probe")
@@ -281,6 +313,8 @@ _SIGNATURES = {
     "b200_attn_decode_tune": (c_int, [c_int]),
     "b200_attn_decode_noalloc": (c_int, [ctypes.POINTER(AttnDecodeArgs), c_void_p]),
     "b200_attn_decode_noalloc_max_bytes": (c_size_t, []),
+    "b200_attn_decode_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "b200_attn_decode_shared": (c_int, [ctypes.POINTER(AttnDecodeSharedArgs), c_void_p]),
     "b200_rope_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "b200_attn_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -10,27 +10,11 @@
 //   T <= 0     : greedy (argmax of the logits, lowest index on ties)
 // One CTA of 1024 threads; thread t owns the contiguous index range [t * chunk, (t + 1) * chunk) so that tie ranks follow
 // index order; the threshold is found by an 8-bit radix select over order-preserving keys (4 histogram passes).
-#include "common.cuh"
+#include "philox.cuh"
 
 namespace b200 {
 
 namespace {
-
-__device__ __forceinline__ uint32_t order_key(float v) {   // ascending float order == ascending unsigned order
-  const uint32_t u = __float_as_uint(v);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-
-__device__ __forceinline__ void philox4x32_10(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1, uint32_t (&out)[4]) {
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
-    const uint32_t hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-    c0 = hi1 ^ c1 ^ k0; c1 = lo1; c2 = hi0 ^ c3 ^ k1; c3 = lo0;
-    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
-  }
-  out[0] = c0; out[1] = c1; out[2] = c2; out[3] = c3;
-}
 
 template <typename LT>
 __device__ __forceinline__ float ld_logit(const LT* p, int64_t i) { return load_as_float<LT>(p, i); }

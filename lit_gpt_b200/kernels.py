@@ -5,9 +5,10 @@ graph.  CUDA tensors only — no CPU path exists (``B200Error`` is raised instea
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 import torch._dynamo
@@ -555,10 +556,12 @@ def argmax_(logits: torch.Tensor, token_out: torch.Tensor, pos_inout: Optional[t
                                  C.stream_ptr(logits.device)), "argmax")
 
 
-def new_rng_state(device: torch.device, seed: Optional[int] = None) -> torch.Tensor:
+def new_rng_state(device: torch.device, seed: Optional[int] = None, rows: Optional[int] = None) -> torch.Tensor:
     """Device-side Philox state for ``sample_``: int64[2] = (seed, offset).  The seed defaults to torch's current seed, so
-    ``seed_everything`` (generate/base.py:140) makes the draws reproducible."""
+    ``seed_everything`` (generate/base.py:140) makes the draws reproducible.  ``rows``: int64 (rows, 2), a state for each row of ``sample_rows_``; row i has seed + i."""
     seed = (torch.initial_seed() if seed is None else int(seed)) & 0x7FFFFFFFFFFFFFFF  # torch's default seed is a full uint64
+    if rows is not None:
+        return torch.tensor([[(seed + i) & 0x7FFFFFFFFFFFFFFF, 0] for i in range(rows)], dtype=torch.int64, device=device).view(rows, 2)
     return torch.tensor([seed, 0], dtype=torch.int64, device=device)
 
 
@@ -586,6 +589,164 @@ def sample_(logits: torch.Tensor, token_out: torch.Tensor, temperature: float = 
                                  token_out.data_ptr(), int(token_out.dtype == torch.int64), C.ptr(pos_inout),
                                  int(pos_inout is not None and pos_inout.dtype == torch.int64), C.ptr(history),
                                  0 if history is None else history.numel(), C.stream_ptr(logits.device)), "sample")
+
+
+# ---------------------------------------------------------------------------------------------------------
+# several rows of logits (csrc/logits.cu), copies between cache slots (csrc/slots.cu)
+# ---------------------------------------------------------------------------------------------------------
+PerRow = Union[float, torch.Tensor]
+
+
+def _current(device: torch.device):
+    """`device` made current for a launch where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _one_device(what: str, device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            C.require_cuda(t)
+            raise C.B200Error(f"{what}: tensors on {device} and {t.device}")
+
+
+def _per_row(value: PerRow, rows: int, dtype: torch.dtype, name: str) -> Tuple[Optional[torch.Tensor], float]:
+    """A setting that is one number for all rows or a tensor with one per row -> (tensor or None, number)."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.dim() != 1 or value.shape[0] != rows:
+        raise C.B200Error(f"{name} must be a number or a {dtype} tensor of one per row (got {value.dtype}, {tuple(value.shape)} for {rows} rows)")
+    return value.contiguous(), 0
+
+
+def _rows_of(t: Optional[torch.Tensor], rows: int, cols: int, dtype: torch.dtype, name: str) -> int:
+    """Distance of the rows of a (rows, cols) tensor, 0 for a (cols,) one that all rows share."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.shape[-1] != cols or t.dim() not in (1, 2) or (t.dim() == 2 and t.shape[0] != rows):
+        raise C.B200Error(f"{name} must be {dtype}, ({cols},) or ({rows}, {cols}) (got {t.dtype}, {tuple(t.shape)})")
+    if (cols > 1 and t.stride(-1) != 1) or t.stride(0) < 0:
+        raise C.B200Error(f"{name}: the numbers of a row must lie next to each other")
+    return t.stride(0) if t.dim() == 2 else 0
+
+
+def _logit_rules(what: str, logits: torch.Tensor, counts: Optional[torch.Tensor], repetition: PerRow, frequency: PerRow, presence: PerRow,
+                 bias: Optional[torch.Tensor], allowed: Optional[torch.Tensor]) -> Tuple["C.LogitRules", tuple]:
+    """-> the rules and the tensors they point into."""
+    C.require_cuda(logits)
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise C.B200Error(f"{what}: logits must be bf16 or fp32 (rows, vocabulary) (got {logits.dtype}, {tuple(logits.shape)})")
+    B, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    rep, rep_all = _per_row(repetition, B, torch.float32, f"{what}: repetition")
+    freq, freq_all = _per_row(frequency, B, torch.float32, f"{what}: frequency")
+    pres, pres_all = _per_row(presence, B, torch.float32, f"{what}: presence")
+    if rep is None and not rep_all > 0.0:
+        raise C.B200Error(f"{what}: repetition must be above zero (got {rep_all})")
+    if counts is not None and counts.dim() != 2:
+        raise C.B200Error(f"{what}: counts must be int32 (rows, vocabulary)")
+    _one_device(what, logits.device, counts, rep, freq, pres, bias, allowed)
+    rules = C.LogitRules(logits.data_ptr(), C.DTYPE_CODE[logits.dtype], logits.stride(0), B, V, C.ptr(counts), _rows_of(counts, B, V, torch.int32, f"{what}: counts"),
+                         C.ptr(rep), C.ptr(freq), C.ptr(pres), rep_all, freq_all, pres_all, C.ptr(bias), _rows_of(bias, B, V, torch.float32, f"{what}: bias"),
+                         C.ptr(allowed), _rows_of(allowed, B, (V + 31) // 32, torch.int32, f"{what}: allowed"))
+    return rules, (logits, rep, freq, pres)
+
+
+def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
+    """Truth values (..., V), true for a token that may be drawn -> int32 (..., ceil(V / 32)), the form that ``adjust_logits`` and ``sample_rows_`` take: token v
+    is bit v % 32 of word v // 32."""
+    V = allowed.shape[-1]
+    words = torch.nn.functional.pad(allowed.bool(), (0, -V % 32)).view(*allowed.shape[:-1], -1, 32)
+    words = (words.long() << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+def adjust_logits(logits: torch.Tensor, *, counts: Optional[torch.Tensor] = None, repetition: PerRow = 1.0, frequency: PerRow = 0.0, presence: PerRow = 0.0,
+                  bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and a mask on logits (rows, V), bf16 or fp32 -> fp32 (rows, V), or into ``out`` (bf16 or fp32; the logits themselves for
+    a change in place).  Where a token was counted n > 0 times: l = l > 0 ? l / repetition : l * repetition, then l -= frequency * n, then l -= presence; then
+    l += bias; tokens that are not allowed: -inf.
+
+    counts int32 (rows, V); repetition (> 0), frequency, presence: a number or fp32 (rows,); bias fp32 (V,) or (rows, V); allowed int32 (ceil(V / 32),) or
+    (rows, ceil(V / 32)) as ``pack_allowed`` makes it."""
+    rules, kept = _logit_rules("adjust_logits", logits, counts, repetition, frequency, presence, bias, allowed)
+    B, V = logits.shape
+    if out is None:
+        out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
+    elif out.shape != logits.shape or out.dtype not in (torch.bfloat16, torch.float32) or out.device != logits.device or (V > 1 and out.stride(1) != 1):
+        raise C.B200Error(f"adjust_logits: out must be bf16 or fp32 {tuple(logits.shape)} on {logits.device}, the numbers of a row next to each other")
+    elif kept[0] is not logits and out.data_ptr() == logits.data_ptr():
+        raise C.B200Error("adjust_logits: in place the numbers of a row must lie next to each other")
+    with _current(logits.device):
+        C.check(C.load_core().b200_adjust_logits(ctypes.byref(rules), out.data_ptr(), C.DTYPE_CODE[out.dtype], out.stride(0), C.stream_ptr(logits.device)), "adjust_logits")
+    return out
+
+
+def sample_rows_(logits: torch.Tensor, token_out: torch.Tensor, temperature: PerRow = 1.0, top_k: Union[None, int, torch.Tensor] = None,
+                 rng_state: Optional[torch.Tensor] = None, *, noise: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, repetition: PerRow = 1.0,
+                 frequency: PerRow = 0.0, presence: PerRow = 0.0, bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None, count: bool = False,
+                 logprob_out: Optional[torch.Tensor] = None, pos_inout: Optional[torch.Tensor] = None, history: Optional[torch.Tensor] = None) -> None:
+    """token_out[b] = one draw from softmax(top_k(l[b]) / temperature) for every row of logits (rows, V), l the logits as ``adjust_logits`` changes them; ``sample_`` for
+    a batch.  A row's token depends on its own numbers alone.  -1 where a row allows nothing.
+
+    temperature: a number or fp32 (rows,), <= 0 for the largest (the lowest token of equal ones); top_k: a number or int32 (rows,), None or <= 0 for all;
+    rng_state: int64 (rows, 2) (``new_rng_state(rows=...)``), every row's offset moves on by one; noise: fp32 (V,) or (rows, V) Exp(1) values to use instead.
+    logprob_out fp32 (rows,): ln of the token's probability among those kept.  count: counts[b, token] += 1.  pos_inout (rows,): += 1, and then
+    history[b, pos] = token where that lies inside ``history`` (rows, length)."""
+    rules, kept = _logit_rules("sample_rows_", logits, counts, repetition, frequency, presence, bias, allowed)
+    B, V = logits.shape
+    temp, temp_all = _per_row(temperature, B, torch.float32, "sample_rows_: temperature")
+    top, top_all = _per_row(0 if top_k is None else top_k, B, torch.int32, "sample_rows_: top_k")
+    if token_out.dtype not in (torch.int32, torch.int64) or token_out.shape != (B,) or not token_out.is_contiguous():
+        raise C.B200Error(f"sample_rows_: token_out must be a contiguous int32 / int64 ({B},) tensor")
+    if rng_state is None and noise is None and (temp is not None or temp_all > 0.0):
+        raise C.B200Error("sample_rows_: temperature > 0 needs rng_state (K.new_rng_state(rows=...)) or noise")
+    if rng_state is not None and (rng_state.dtype != torch.int64 or rng_state.shape != (B, 2) or not rng_state.is_contiguous()):
+        raise C.B200Error(f"sample_rows_: rng_state must be a contiguous int64 ({B}, 2) tensor, a state per row")
+    if logprob_out is not None and (logprob_out.dtype != torch.float32 or logprob_out.shape != (B,) or not logprob_out.is_contiguous()):
+        raise C.B200Error(f"sample_rows_: logprob_out must be a contiguous fp32 ({B},) tensor")
+    if pos_inout is not None and (pos_inout.dtype not in (torch.int32, torch.int64) or pos_inout.shape != (B,) or not pos_inout.is_contiguous()):
+        raise C.B200Error(f"sample_rows_: pos_inout must be a contiguous int32 / int64 ({B},) tensor, a position per row")
+    if history is not None and (pos_inout is None or history.dtype != token_out.dtype or history.dim() != 2 or history.shape[0] != B
+                                or (history.shape[1] > 1 and history.stride(1) != 1) or (B > 1 and history.stride(0) < history.shape[1])):
+        raise C.B200Error(f"sample_rows_: history must be ({B}, length) of token_out's dtype, with pos_inout")
+    if count and (counts is None or (B > 1 and counts.stride(0) < V)):
+        raise C.B200Error("sample_rows_: nothing to count in")
+    _one_device("sample_rows_", logits.device, token_out, temp, top, rng_state, noise, logprob_out, pos_inout, history)
+    args = C.DrawArgs(C.ptr(temp), temp_all, C.ptr(top), min(int(top_all), 2 ** 31 - 1), C.ptr(rng_state), C.ptr(noise), _rows_of(noise, B, V, torch.float32, "sample_rows_: noise"),
+                      token_out.data_ptr(), token_out.dtype == torch.int64, C.ptr(logprob_out), count, C.ptr(pos_inout),
+                      pos_inout is not None and pos_inout.dtype == torch.int64, C.ptr(history), 0 if history is None else history.stride(0),
+                      0 if history is None else history.shape[1])
+    with _current(logits.device):
+        C.check(C.load_core().b200_sample_rows(ctypes.byref(rules), ctypes.byref(args), C.stream_ptr(logits.device)), "sample_rows_")
+
+
+def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], lengths: Optional[Sequence[int]] = None) -> None:
+    """t[dst[i]] = t[src[i]] for every i and every tensor t (slots, ...) of caches and states, in one launch for all of them: a live sequence forked, or moved to another slot.
+    ``lengths``: copy i takes only the leading lengths[i] positions (the second dimension) of caches by position.  A slot may be the source of several copies;
+    one that is written may be neither the source nor the destination of another."""
+    if len(src) != len(dst) or (lengths is not None and len(lengths) != len(src)):
+        raise C.B200Error("copy_slots: as many destinations (and lengths) as sources")
+    if not tensors:
+        return
+    device, slots = tensors[0].device, tensors[0].shape[0] if tensors[0].dim() else 0
+    table = (C.SlotTensor * len(tensors))()
+    for i, t in enumerate(tensors):
+        if t.dim() < 2 or not t.is_contiguous() or t.shape[0] != slots:
+            raise C.B200Error(f"copy_slots: tensor {i} must be contiguous (slots, ...) with {slots} slots (got {tuple(t.shape)})")
+        if t.numel() == 0:
+            raise C.B200Error(f"copy_slots: tensor {i} is empty")
+        table[i].base, table[i].rows, table[i].row_bytes = t.data_ptr(), t.shape[1], t.stride(0) // t.shape[1] * t.element_size()
+    C.require_cuda(*tensors)
+    _one_device("copy_slots", device, *tensors)
+    pairs = (C.SlotPair * max(len(src), 1))()
+    for i in range(len(src)):
+        n = -1 if lengths is None else int(lengths[i])
+        if lengths is not None and n < 0:
+            raise C.B200Error(f"copy_slots: copy {i} of {n} positions")
+        pairs[i].src, pairs[i].dst, pairs[i].rows = int(src[i]), int(dst[i]), n
+    with _current(device):
+        C.check(C.load_core().b200_copy_slots(table, len(tensors), slots, pairs, len(src), C.stream_ptr(device)), "copy_slots")
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -627,6 +788,56 @@ def attn_decode(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: to
         out=out.data_ptr(), batch=B, n_head=n_head, n_groups=n_groups, head_size=head_size, max_seq=max_seq,
         num_splits=num_splits, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
     C.check(lib.b200_attn_decode(ctypes.byref(args), C.stream_ptr(qkv.device)), "attn_decode")
+    return out
+
+
+def attn_decode_shared(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       k_prefix: torch.Tensor, v_prefix: torch.Tensor, prefix_len: Optional[torch.Tensor], n_head: int, n_groups: int, head_size: int, rope_n_elem: int,
+                       table_preselected: bool = False) -> torch.Tensor:
+    """``attn_decode`` for rows that share a prefix (several answers to one prompt): one token per row, whose keys are the prefix's, held and read once for all rows,
+    and those of the row's own cache.
+
+    qkv (B, 1, (H+2G)*hs) or (B, (H+2G)*hs) bf16; pos: the new tokens' positions, one device int for all rows or (B,); a row at a negative position takes no part (cache
+    untouched, result zero).  k_prefix / v_prefix (G, P, hs) bf16 hold positions 0 .. n - 1, n = prefix_len (device int, at most P; None: P); k_cache / v_cache
+    (B, G, rows, hs) bf16 hold row b's position p at p - n and are updated in place.  Any distance between groups and rows of a batch that is a multiple of 8
+    numbers; rows of hs numbers next to each other.  Returns (B, H*hs)."""
+    C.require_cuda(qkv, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len)
+    qkv = _bf16c(qkv, "qkv")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != n_groups or k_cache.shape[3] != head_size:
+        raise C.B200Error(f"attn_decode_shared: caches must be (rows, {n_groups}, length, {head_size}) (got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
+    if k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != n_groups or k_prefix.shape[2] != head_size:
+        raise C.B200Error(f"attn_decode_shared: prefix must be ({n_groups}, length, {head_size}) (got {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)})")
+    for t in (k_cache, v_cache, k_prefix, v_prefix):
+        if t.dtype != torch.bfloat16 or t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) != head_size):
+            raise C.B200Error("attn_decode_shared: caches and prefix must be bfloat16, rows of head_size numbers next to each other")
+    apart = [tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 2)) for t in (k_cache, v_cache, k_prefix, v_prefix)]
+    if any(n > 1 and step < k_cache.shape[2] * head_size for t in apart[:2] for n, step in zip(k_cache.shape, t)):
+        raise C.B200Error("attn_decode_shared: the caches of two rows or groups overlap")
+    B, _, S, _ = k_cache.shape
+    if qkv.numel() != B * (n_head + 2 * n_groups) * head_size:
+        raise C.B200Error("attn_decode_shared: qkv does not hold exactly one token per row of the caches")
+    for t, n, name in ((pos, (1, B), "pos"), (prefix_len, (1,), "prefix_len")):
+        if t is not None and (t.dtype not in (torch.int64, torch.int32) or t.numel() not in n):
+            raise C.B200Error(f"attn_decode_shared: {name} must be an int32/int64 device tensor of {' or '.join(map(str, n))}")
+    if cos.dtype != sin.dtype or cos.shape != sin.shape or cos.shape[-1] != rope_n_elem:
+        raise C.B200Error(f"attn_decode_shared: cos and sin must be (positions, {rope_n_elem}) of one dtype")
+    _one_device("attn_decode_shared", qkv.device, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len)
+    cos, sin, pos = cos.contiguous(), sin.contiguous(), pos.contiguous()
+    table_rows = cos.numel() // max(rope_n_elem, 1)
+    if table_preselected and table_rows != pos.numel():
+        raise C.B200Error(f"attn_decode_shared: {table_rows} preselected table rows for {pos.numel()} positions")
+    P = k_prefix.shape[1]
+    out = torch.empty((B, n_head * head_size), dtype=torch.bfloat16, device=qkv.device)
+    lib = C.load()
+    with _current(qkv.device):
+        nbytes = lib.b200_attn_decode_shared_workspace_bytes(B, n_head, n_groups, head_size, P, S)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=qkv.device)   # of this call: calls on two streams, or in two graphs, have one each
+        args = C.AttnDecodeSharedArgs(
+            qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, pos.data_ptr(), pos.dtype == torch.int64,
+            pos.numel(), C.ptr(prefix_len), prefix_len is not None and prefix_len.dtype == torch.int64, k_cache.data_ptr(), v_cache.data_ptr(), *apart[0], *apart[1],
+            k_prefix.data_ptr(), v_prefix.data_ptr(), *apart[2], *apart[3], out.data_ptr(),
+            B, n_head, n_groups, head_size, S, P, ws.data_ptr(), nbytes)
+        C.check(lib.b200_attn_decode_shared(ctypes.byref(args), C.stream_ptr(qkv.device)), "attn_decode_shared")
     return out
 
 
