@@ -8,16 +8,18 @@ output sequence all stay on the device, and the EOS test is polled every ``EOS_P
 """
 from __future__ import annotations
 
+import contextlib
 import sys
 import time
 from pathlib import Path
-from typing import Any, Dict, Literal, Optional, Tuple
+from typing import Any, Dict, List, Literal, Optional, Tuple
 
 import torch
 
 from lit_gpt_b200 import GPT, Config, QuantPrecision
 from lit_gpt_b200 import kernels as K
 from lit_gpt_b200.fabric import Fabric, seed_everything
+from lit_gpt_b200.model import SharedKVCache
 from lit_gpt_b200.quant import weight_epoch
 from lit_gpt_b200.utils import check_valid_checkpoint_dir, get_default_supported_precision, load_checkpoint
 
@@ -266,6 +268,172 @@ def generate(model: GPT, prompt: torch.Tensor, max_returned_tokens: int, *, temp
     return out
 
 
+SAMPLE_ROWS = 16          # rows that the fused decode step takes at once
+SAMPLE_CACHE_STEP = 64    # own caches grow in steps of this many tokens, so that calls of similar lengths use one captured step
+
+
+def row_rng_states(device: torch.device, rows: int) -> torch.Tensor:
+    """A Philox state per row, different from call to call and reproduced by the seed: taken from the device's one sampler state, which moves on by one."""
+    state = _rng_for(device)
+    seed, offset = state.tolist()
+    state[1] += 1
+    return K.new_rng_state(device, (seed + 0x9E3779B97F4A7C15 * (offset + 1)) % 2 ** 63, rows=rows)
+
+
+class SampleGraph:
+    """A decode step of several rows that continue one prompt, with the draw of a token for each: tokens, positions, counts, sampler states and history live on the
+    device.  Captured where the model's step is (``fused_decode_ready``), else run as it is."""
+
+    def __init__(self, model: GPT, rows: int, length: int, temperature: float, top_k: Optional[int], penalties: Tuple[float, float, float], biased: bool,
+                 logprobs: bool, dtype: torch.dtype) -> None:
+        dev, V = model.transformer.wte.weight.device, model.config.padded_vocab_size
+        self.model, self.temperature, self.top_k, self.penalties = model, temperature, top_k, penalties
+        self.token = torch.zeros(rows, dtype=dtype, device=dev)
+        self.pos = torch.zeros(rows, dtype=torch.int64, device=dev)
+        self.history = torch.zeros(rows, model.max_seq_length + 1, dtype=dtype, device=dev)
+        self.logprobs = torch.zeros(rows, model.max_seq_length + 1, device=dev) if logprobs else None
+        self.logprob = torch.zeros(rows, device=dev) if logprobs else None
+        self.rng = torch.zeros(rows, 2, dtype=torch.int64, device=dev)
+        self.counts = torch.zeros(rows, V, dtype=torch.int32, device=dev) if penalties != (1.0, 0.0, 0.0) else None
+        self.bias = torch.zeros(V, device=dev) if biased else None
+        self.prefix_len = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.caches = [SharedKVCache(b.attn.kv_cache, self.prefix_len, rows, length) for b in model.transformer.h]
+        self.graph: Optional[torch.cuda.CUDAGraph] = None
+
+    def draw(self, logits: torch.Tensor) -> None:
+        """A token for every row from logits (rows, V); the rows' positions move on by one."""
+        rep, freq, pres = self.penalties
+        K.sample_rows_(logits, self.token, self.temperature, self.top_k, None if self.temperature <= 0.0 else self.rng, counts=self.counts, repetition=rep, frequency=freq,
+                       presence=pres, bias=self.bias, count=self.counts is not None, logprob_out=self.logprob, pos_inout=self.pos, history=self.history)
+        if self.logprobs is not None:
+            self.logprobs.index_copy_(1, self.pos[:1], self.logprob[:, None])
+
+    def _step(self) -> None:
+        self.draw(self.model(self.token.view(-1, 1), self.pos[:1])[:, -1])   # (all rows are at one position)
+
+    def capture(self) -> None:
+        held = [t for t in (self.token, self.pos, self.rng, self.counts) if t is not None]
+        state = [t.clone() for t in held]
+
+        def put_back() -> None:
+            for t, saved in zip(held, state):
+                t.copy_(saved)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):   # warm-up outside capture (DecodeGraph.capture)
+            for _ in range(2):
+                put_back()
+                self._step()
+        torch.cuda.current_stream().wait_stream(side)
+        put_back()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self._step()
+
+    def step(self) -> None:
+        if self.graph is not None:
+            self.graph.replay()
+        else:
+            self._step()
+
+    @contextlib.contextmanager
+    def in_place(self):
+        """The model over these rows' caches."""
+        blocks = self.model.transformer.h
+        before = [b.attn.kv_cache for b in blocks]
+        try:
+            for b, cache in zip(blocks, self.caches):
+                b.attn.kv_cache = cache
+            yield
+        finally:
+            for b, cache in zip(blocks, before):
+                b.attn.kv_cache = cache
+
+
+def _sample_graph_for(model: GPT, *key: Any) -> SampleGraph:
+    cache: Dict[Tuple, SampleGraph] = model.__dict__.setdefault("_sample_graphs", {})
+    full = key + _graph_key(model)
+    sg = cache.get(full)
+    if sg is None:
+        if cache and next(iter(cache))[len(key):] != full[len(key):] or len(cache) >= 2:
+            cache.clear()   # (a call's last group of rows may be smaller than the others: two)
+        sg = cache[full] = SampleGraph(model, *key)
+    return sg
+
+
+@torch.inference_mode()
+def generate_samples(model: GPT, prompt: torch.Tensor, max_returned_tokens: int, num_samples: int, *, temperature: float = 1.0, top_k: Optional[int] = None,
+                     eos_id: Optional[int] = None, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0, presence_penalty: float = 0.0,
+                     count_prompt: bool = False, logit_bias: Optional[Dict[int, float]] = None, logprobs: bool = False) -> Any:
+    """Several answers to one prompt, ``generate`` for `num_samples` at once: the prompt runs once, its keys and values are held once and read once per step for all
+    answers (``kernels.attn_decode_shared``), and every answer draws from a sampler state of its own.
+
+    prompt (T,) token ids on the GPU.  Returns a list of prompt + answer, each at most `max_returned_tokens` long and ending with its `eos_id`; with `logprobs` also the
+    list of the answers' log-probabilities (fp32, one per generated token, of the distribution that it was drawn from).  Penalties count the answer's own
+    tokens, with `count_prompt` the prompt's too (``kernels.adjust_logits``); `logit_bias`: token -> what is added to its logit.  Needs the GQA-native cache
+    (CUDA, bf16, head size 64 or 128) on one device."""
+    T = prompt.size(0)
+    assert max_returned_tokens > T
+    if model.max_seq_length < max_returned_tokens - 1:
+        raise NotImplementedError(f"max_seq_length {model.max_seq_length} needs to be >= {max_returned_tokens - 1}")
+    if num_samples < 1:
+        raise ValueError(f"num_samples must be at least 1 (got {num_samples})")
+    caches = [b.attn.kv_cache for b in model.transformer.h]
+    if any(c is None for c in caches):
+        raise TypeError("You need to call `gpt.set_kv_cache()`")
+    if not prompt.is_cuda or model.tp_world_size != 1 or model.spans_devices() or not all(c.gqa_native for c in caches):
+        raise NotImplementedError("answers that share their prompt run on one GPU over the GQA-native cache (bf16, head size 64 or 128)")
+    V = model.config.padded_vocab_size
+    if logit_bias and not all(0 <= t < V for t in logit_bias):
+        raise ValueError(f"logit_bias names tokens outside 0 .. {V - 1}")
+    device, penalties = prompt.device, (float(repetition_penalty), float(frequency_penalty), float(presence_penalty))
+    rng = row_rng_states(device, num_samples) if temperature > 0.0 else None
+    first = model(prompt.view(1, -1), torch.arange(0, T, device=device))[:, -1]
+    fused = model.fused_decode_ready(prompt.view(1, -1))
+    length = -(-(max_returned_tokens - T) // SAMPLE_CACHE_STEP) * SAMPLE_CACHE_STEP
+    each = min(num_samples, SAMPLE_ROWS) if fused else num_samples
+    tokens: List[torch.Tensor] = []
+    scores: List[torch.Tensor] = []
+    for begin in range(0, num_samples, each):
+        rows = min(each, num_samples - begin)
+        sg = _sample_graph_for(model, rows, length, temperature, top_k, penalties, bool(logit_bias), logprobs, prompt.dtype)
+        sg.prefix_len.fill_(T)
+        sg.pos.fill_(T - 1)
+        if rng is not None:
+            sg.rng.copy_(rng[begin : begin + rows])
+        if sg.counts is not None:
+            sg.counts.zero_()
+            if count_prompt:
+                sg.counts.scatter_add_(1, prompt.long().expand(rows, -1), torch.ones_like(prompt, dtype=torch.int32).expand(rows, -1))
+        if sg.bias is not None:
+            sg.bias.zero_()
+            sg.bias[torch.tensor(list(logit_bias), device=device)] = torch.tensor(list(logit_bias.values()), dtype=torch.float32, device=device)
+        sg.draw(first.expand(rows, -1))
+        done = 1
+        with sg.in_place():
+            if fused and sg.graph is None and max_returned_tokens - T > 1:
+                sg.capture()
+            while done < max_returned_tokens - T:
+                burst = max_returned_tokens - T - done if eos_id is None else min(EOS_POLL, max_returned_tokens - T - done)
+                for _ in range(burst):
+                    sg.step()
+                done += burst
+                if eos_id is not None and bool((sg.history[:, T : T + done] == eos_id).any(1).all()):   # the only host sync of the loop
+                    break
+        answers = sg.history[:, T : T + done].clone()
+        ends = [done] * rows
+        if eos_id is not None:
+            hit = answers == eos_id
+            ends = torch.where(hit.any(1), hit.int().argmax(1) + 1, done).tolist()
+        tokens += [torch.cat((prompt, answers[i, :n])) for i, n in enumerate(ends)]
+        if logprobs:
+            given = sg.logprobs[:, T : T + done].clone()
+            scores += [given[i, :n] for i, n in enumerate(ends)]
+    K.check_gemv_errors(device)
+    return (tokens, scores) if logprobs else tokens
+
+
 @torch.inference_mode()
 def main(
     prompt: str = "What food do llamas eat?",
@@ -278,18 +446,27 @@ def main(
     quantize: Optional[Literal["bnb.nf4", "bnb.nf4-dq", "bnb.fp4", "bnb.fp4-dq", "bnb.int8", "gptq.int4"]] = None,
     precision: Optional[str] = None,
     compile: bool = False,
+    batch_samples: bool = False,
+    repetition_penalty: float = 1.0,
+    frequency_penalty: float = 0.0,
+    presence_penalty: float = 0.0,
 ) -> None:
     """Generates text samples based on a pre-trained model and tokenizer.
 
     Args mirror the reference CLI (generate/base.py:97-124).  ``quantize``: bnb.nf4 / bnb.fp4 are the bitsandbytes
     block-64 4-bit formats, gptq.int4 is this project's int4 group-128 format.  ``compile`` is accepted for parity;
     the decode loop is a CUDA graph of hand-written kernels, there is no tracing compiler on this path.
+    ``batch_samples``: the ``num_samples`` answers as one batch that shares the prompt (``generate_samples``) instead of one after the other; the penalties
+    for repeated tokens apply to that path, which they switch on.
     """
+    repetition_penalty, frequency_penalty, presence_penalty = float(repetition_penalty), float(frequency_penalty), float(presence_penalty)
+    batch_samples = batch_samples or (repetition_penalty, frequency_penalty, presence_penalty) != (1.0, 0.0, 0.0)
+    penalties = dict(repetition_penalty=repetition_penalty, frequency_penalty=frequency_penalty, presence_penalty=presence_penalty) if batch_samples else None
     from lit_gpt_b200.tokenizer import Tokenizer
 
     precision = precision or get_default_supported_precision(training=False)
     if (checkpoint_dir / "config.json").is_file() and not (checkpoint_dir / "lit_config.json").is_file():
-        return _main_registered(prompt, num_samples, max_new_tokens, top_k, temperature, checkpoint_dir, quantize, precision)
+        return _main_registered(prompt, num_samples, max_new_tokens, top_k, temperature, checkpoint_dir, quantize, precision, penalties)
 
     plugins = None
     if quantize is not None:
@@ -327,6 +504,11 @@ def main(
     fabric.print(f"Time to load the model weights: {time.perf_counter() - t0:.02f} seconds.", file=sys.stderr)
 
     seed_everything(1234)
+    if penalties is not None:
+        t0 = time.perf_counter()
+        ys = generate_samples(model, encoded, max_returned_tokens, num_samples, temperature=temperature, top_k=top_k, eos_id=tokenizer.eos_id, **penalties)
+        _print_batch(fabric, [tokenizer.decode(y) for y in ys], sum(y.size(0) - prompt_length for y in ys), time.perf_counter() - t0)
+        return
     for i in range(num_samples):
         t0 = time.perf_counter()
         y = generate(model, encoded, max_returned_tokens, temperature=temperature, top_k=top_k, eos_id=tokenizer.eos_id)
@@ -342,8 +524,16 @@ def main(
         fabric.print(f"Memory used: {torch.cuda.max_memory_allocated() / 1e9:.02f} GB", file=sys.stderr)
 
 
+def _print_batch(fabric: Fabric, texts: List[str], tokens_generated: int, t: float) -> None:
+    for text in texts:
+        fabric.print(text)
+    fabric.print(f"Time for inference of {len(texts)}: {t:.02f} sec total, {tokens_generated / t:.02f} tokens/sec", file=sys.stderr)
+    if fabric.device.type == "cuda":
+        fabric.print(f"Memory used: {torch.cuda.max_memory_allocated() / 1e9:.02f} GB", file=sys.stderr)
+
+
 def _main_registered(prompt: str, num_samples: int, max_new_tokens: int, top_k: Optional[int], temperature: float, checkpoint_dir: Path,
-                     quantize: Optional[str], precision: str) -> None:
+                     quantize: Optional[str], precision: str, penalties: Optional[Dict[str, float]] = None) -> None:
     """`main` for a checkpoint directory with a ``config.json`` whose architecture is registered in ``lit_gpt_b200.config``
     (``model.safetensors`` weights).  Without tokenizer files the prompt is a list of token ids ("3 17 250" or "3,17,250") and
     ids are printed."""
@@ -376,6 +566,14 @@ def _main_registered(prompt: str, num_samples: int, max_new_tokens: int, top_k: 
     model.set_kv_cache(batch_size=1)
     fabric.print(f"Time to load the model weights: {time.perf_counter() - t0:.02f} seconds.", file=sys.stderr)
     seed_everything(1234)
+    if penalties is not None:
+        from lit_gpt_b200.generate.serve import generate_batch
+
+        t0 = time.perf_counter()
+        ys = generate_batch(model, [encoded.tolist()], max_new_tokens, temperature=temperature, top_k=top_k, eos_id=eos_id, num_samples=num_samples, **penalties)
+        texts = [tokenizer.decode(torch.tensor(y)) if tokenizer is not None else " ".join(map(str, y)) for y in ys]
+        _print_batch(fabric, texts, sum(len(y) - encoded.size(0) for y in ys), time.perf_counter() - t0)
+        return
     for i in range(num_samples):
         t0 = time.perf_counter()
         y = generate(model, encoded, max_returned_tokens, temperature=temperature, top_k=top_k, eos_id=eos_id)

@@ -89,6 +89,8 @@ class GPT(nn.Module):
         if input_pos is not None:
             if self.mask_cache is None:
                 raise TypeError("You need to call `gpt.set_kv_cache()`")
+            if T > 1 and isinstance(self.transformer.h[0].attn.kv_cache, SharedKVCache):
+                raise RuntimeError("rows that share a prefix take one token each per step")
             # (a traced forward takes the module path: its kernels are registered custom ops, the fused chain is raw C-ABI calls)
             if T == 1 and input_pos.numel() == 1 and not torch.compiler.is_compiling() and self.fused_decode_ready(idx):
                 return self._fused_decode(idx, input_pos)
@@ -134,6 +136,7 @@ class GPT(nn.Module):
         self._fused_plan = None
         self.__dict__.pop("_decode_graphs", None)  # captured graphs pin the kv / table / weight buffers
         self.__dict__.pop("_prefill_graphs", None)
+        self.__dict__.pop("_sample_graphs", None)
 
     def clear_kv_cache(self) -> None:
         self.mask_cache = None
@@ -142,6 +145,7 @@ class GPT(nn.Module):
         self._fused_plan = None
         self.__dict__.pop("_decode_graphs", None)  # captured graphs pin the kv / table / weight buffers
         self.__dict__.pop("_prefill_graphs", None)
+        self.__dict__.pop("_sample_graphs", None)
 
     # ------------------------------------------------------------------------------------------------------
     # fused decode step
@@ -155,6 +159,7 @@ class GPT(nn.Module):
         self.__dict__.pop("_p2p", None)
         self.__dict__.pop("_decode_graphs", None)  # captured graphs pin the kv / table / weight buffers
         self.__dict__.pop("_prefill_graphs", None)
+        self.__dict__.pop("_sample_graphs", None)
         return super()._apply(fn, recurse)
 
     def fused_decode_ready(self, idx: Optional[torch.Tensor] = None) -> bool:
@@ -353,7 +358,7 @@ class GPT(nn.Module):
                     qkv = a.attn.gemv(K.rmsnorm(x, block.norm_1.weight, eps), kv_hint=(cache.k, cache.v, pos))
                 else:
                     qkv = a.attn.gemv(x, norm_weight=block.norm_1.weight, norm_eps=eps, kv_hint=(cache.k, cache.v, pos))
-                y = K.attn_decode(qkv, cos, sin, pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem)
+                y = _decode_attention(c, cache, qkv, cos, sin, pos)
                 x = a.proj.gemv(y, residual=x)
                 if B > SPLIT_NORM_ROWS:
                     act = m.fc_1.gemv(K.rmsnorm(x, block.norm_2.weight, eps), other=m.fc_2)
@@ -417,8 +422,7 @@ class GPT(nn.Module):
                     else:
                         qkv = lin(a.attn, x, delta=pending, x_out=x_new, norm_weight=block.norm_1.weight, norm_eps=eps)
                     x = x_new
-                y = K.attn_decode(qkv, self.cos, self.sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups,
-                                  c.head_size, c.rope_n_elem)
+                y = _decode_attention(c, cache, qkv, self.cos, self.sin, input_pos)
                 tlin(a.proj, y, send=0)
                 x_new = torch.empty_like(x)
                 act = tlin(m.fc_1, x, other=m.fc_2, recv=0, x_out=x_new, norm_weight=block.norm_2.weight, norm_eps=eps)
@@ -454,7 +458,7 @@ class GPT(nn.Module):
         # launches per token fewer, but measured SLOWER on B200 (632 vs 676 tok/s): in-kernel the
         # attention tail runs on one SM per head at the GEMV's register budget, 5.5 - 7.5 us against ~6 us for the stand-alone
         # cluster kernel INCLUDING its launch boundary
-        fuse_attn = (not tp and B == 1 and a0 is not None and self.max_seq_length <= int(os.environ.get("B200_FUSE_ATTN_MAX_SEQ", "0"))
+        fuse_attn = (not tp and B == 1 and a0 is not None and not isinstance(blocks[0].attn.kv_cache, SharedKVCache) and self.max_seq_length <= int(os.environ.get("B200_FUSE_ATTN_MAX_SEQ", "0"))
                      and a0.fold == 1 and a0.streams(1) and input_pos.numel() == 1
                      and K.qgemv_attn_fusable(a0.out_features, a0.in_features, a0.quant_type, c.n_head, c.n_query_groups, c.head_size,
                                               c.rope_n_elem, self.max_seq_length))
@@ -464,7 +468,8 @@ class GPT(nn.Module):
         for li, block in enumerate(blocks):
             a, m, cache = block.attn, block.mlp, block.attn.kv_cache
             nxt_qkv = blocks[li + 1].attn.attn if li + 1 < len(blocks) else self.lm_head
-            hint = (cache.k, cache.v, input_pos)  # L2 hint: the filled K / V rows this block's attention reads next
+            # L2 hint: the filled K / V rows this block's attention reads next (positions of a row's own cache behind a shared prefix count from another zero)
+            hint = None if isinstance(cache, SharedKVCache) else (cache.k, cache.v, input_pos)
             if fuse_attn:
                 # the attention step runs inside the QKV GEMV's kernel (b200_qgemv_tiled_args::attn): one launch boundary less
                 y = torch.empty((B, c.n_head * c.head_size), dtype=torch.bfloat16, device=x.device)
@@ -480,8 +485,7 @@ class GPT(nn.Module):
             else:
                 qkv = lin(a.attn, x, a.proj, norm_weight=block.norm_1.weight, norm_eps=eps, kv_hint=hint)
             if not fuse_attn:
-                y = K.attn_decode(qkv, self.cos, self.sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups,
-                                  c.head_size, c.rope_n_elem)
+                y = _decode_attention(c, cache, qkv, self.cos, self.sin, input_pos)
             if tp:
                 h = self._all_reduce(lin(a.proj, y, m.fc_1))
                 x_new = torch.empty_like(x)
@@ -590,13 +594,16 @@ class CausalSelfAttention(nn.Module):
 
             o = torch.ops.b200gpt
             if T == 1:
-                y = o.attn_decode(qkv, cos, sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem, True)
+                if isinstance(cache, SharedKVCache):
+                    y = o.attn_decode_shared(qkv, cos, sin, input_pos, cache.k, cache.v, cache.k_prefix, cache.v_prefix, cache.prefix_len, c.n_head, c.n_query_groups,
+                                             c.head_size, c.rope_n_elem, True)
+                else:
+                    y = o.attn_decode(qkv, cos, sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem, True)
                 return y.view(B, 1, c.n_head * c.head_size)
             q = o.rope_kv_append(qkv, cos, sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem, True)
             return o.attn_prefill(q, cache.k, cache.v, input_pos, 1.0 / math.sqrt(c.head_size))
         if T == 1:
-            y = K.attn_decode(qkv, cos, sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size,
-                              c.rope_n_elem, table_preselected=True)
+            y = _decode_attention(c, cache, qkv, cos, sin, input_pos, table_preselected=True)
             return y.view(B, 1, c.n_head * c.head_size)
         q = K.rope_kv_append(qkv, cos, sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size,
                              c.rope_n_elem, table_preselected=True)
@@ -724,6 +731,27 @@ class KVCache(nn.Module):
     def reset_parameters(self) -> None:
         torch.nn.init.zeros_(self.k)
         torch.nn.init.zeros_(self.v)
+
+
+class SharedKVCache(KVCache):
+    """Cache of rows that continue one prompt: the prompt's keys and values, held once -- row 0 of the GQA-native cache that its prefill filled --, and a cache of its own
+    for every row's tokens behind it."""
+
+    def __init__(self, prompt: KVCache, prefix_len: torch.Tensor, rows: int, length: int) -> None:
+        if not prompt.gqa_native:
+            raise RuntimeError("a shared prefix needs the GQA-native cache of the CUDA bf16 kernels (head size 64 or 128)")
+        _, G, _, hs = prompt.k.shape
+        super().__init__((rows, G, length, hs), (rows, G, length, hs), device=prompt.k.device, dtype=prompt.k.dtype, gqa_native=True)
+        self.k_prefix, self.v_prefix = prompt.k[0], prompt.v[0]
+        self.prefix_len = prefix_len   # int32 (1,) on the device: how much of the prompt's cache is the prompt
+
+
+def _decode_attention(c: Config, cache: KVCache, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, table_preselected: bool = False) -> torch.Tensor:
+    """Rotation, cache append and attention of one token per row, over the kind of cache that there is."""
+    if isinstance(cache, SharedKVCache):
+        return K.attn_decode_shared(qkv, cos, sin, pos, cache.k, cache.v, cache.k_prefix, cache.v_prefix, cache.prefix_len, c.n_head, c.n_query_groups, c.head_size,
+                                    c.rope_n_elem, table_preselected=table_preselected)
+    return K.attn_decode(qkv, cos, sin, pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem, table_preselected=table_preselected)
 
 
 def build_mask_cache(max_seq_length: int, device: Optional[torch.device] = None) -> torch.Tensor:

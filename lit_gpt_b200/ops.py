@@ -71,6 +71,20 @@ def _(qkv, cos, sin, pos, k_cache, v_cache, n_head, n_groups, head_size, rope_n_
     return qkv.new_empty((k_cache.shape[0], n_head * head_size), dtype=torch.bfloat16)
 
 
+# ---- the same for rows that share a prefix ------------------------------------------------------------------------
+@torch.library.custom_op(f"{NS}::attn_decode_shared", mutates_args=("k_cache", "v_cache"))
+def attn_decode_shared(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, prefix_len: Optional[torch.Tensor], n_head: int,
+                       n_groups: int, head_size: int, rope_n_elem: int, table_preselected: bool = False) -> torch.Tensor:
+    return K.attn_decode_shared(qkv, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len, n_head, n_groups, head_size, rope_n_elem,
+                                table_preselected=table_preselected)
+
+
+@attn_decode_shared.register_fake
+def _(qkv, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len, n_head, n_groups, head_size, rope_n_elem, table_preselected=False):
+    return qkv.new_empty((k_cache.shape[0], n_head * head_size), dtype=torch.bfloat16)
+
+
 # ---- prefill: RoPE + cache write, then causal attention over the cache (model.py:624-665) -------------------------
 @torch.library.custom_op(f"{NS}::rope_kv_append", mutates_args=("k_cache", "v_cache"))
 def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,

@@ -83,6 +83,7 @@ class SlotServed:
 
     supports_prefill_graph = False   # a prompt's extent is read on the host
     repeatable_steps = True          # running a step twice at the same position leaves the same cache (false for recurrent states)
+    positional_states = True         # the second dimension of every state tensor is the position (false for states of constant size)
     tp_world_size = 1
 
     @property
@@ -140,6 +141,7 @@ class StateServed(SlotServed):
     ``build_state``), ``head`` and ``_run(tokens, batch, want_rows)``."""
 
     needs_positions = True           # the rows' positions are part of the step's description
+    positional_states = False
 
     def init_serving(self, runs: Sequence[Tuple]) -> None:
         self.runs = list(runs)

@@ -1,0 +1,270 @@
+"""Several answers to one prompt through the public entry points: generate.base.generate_samples (shared prefix, a draw per row), Session.fork / compact / shrink and
+generate_batch with several samples and rules on the logits."""
+import pytest
+import torch
+
+from oracle import model_ref as M
+
+pytestmark = pytest.mark.gpu
+
+
+def toy(golden, mode="nf4", max_seq=200, name="llama_gqa_hs64", batch=1):
+    from test_gpu_model import build_cuda_model, cfg_from_golden, oracle_weights
+
+    g = golden(name)
+    cfgd, kw = cfg_from_golden(g)
+    kw["block_size"] = max(kw["block_size"], max_seq)
+    rc = M.RefConfig.from_any(cfgd)
+    p = M.init_weights(rc, seed=1234)
+    if mode is None:
+        from lit_gpt_b200 import GPT, Config
+        from lit_gpt_b200.fabric import Fabric
+
+        fabric = Fabric(devices=1, precision="bf16-true")
+        with fabric.init_module(empty_init=True):
+            model = GPT(Config(**kw))
+        with fabric.init_tensor():
+            model.max_seq_length = max_seq
+            model.set_kv_cache(batch_size=batch)
+        model = fabric.setup_module(model.eval())
+        model.load_state_dict({k: v.to(torch.bfloat16) for k, v in p.items()}, strict=True)
+        pw = {k: v.to(torch.bfloat16).float() for k, v in p.items()}
+    else:
+        model, pw = build_cuda_model(kw, p, mode, max_seq, batch), oracle_weights(p, mode)
+    return model, rc, pw, torch.from_numpy(g["gen_prompt"])
+
+
+def along(model, rc, pw, seq, T):
+    """The oracle's logits at the steps that chose seq[T:], and the tolerance of test_gpu_model.check_rollout."""
+    from test_gpu_model import run_oracle
+
+    cos, sin = model.cos.cpu(), model.sin.cpu()
+    _, l32 = run_oracle(rc, pw, cos.float(), sin.float(), seq[:T], len(seq), torch.float32, forced=seq)
+    _, l16 = run_oracle(rc, pw, cos, sin, seq[:T], len(seq), torch.bfloat16, forced=seq)
+    return l32, 2.0 * (l16 - l32).abs().max().item() + 1e-3 * l32.abs().max().item()
+
+
+@pytest.mark.parametrize("mode,name", [("nf4", "llama_gqa_hs64"), ("int4", "llama_mha_hs128"), (None, "llama_gqa_hs64")])
+@torch.inference_mode()
+def test_greedy_answers_follow_the_oracle(golden, mode, name):
+    import lit_gpt_b200.generate.base as gb
+
+    model, rc, pw, prompt = toy(golden, mode, name=name)
+    assert model.fused_decode_ready() == (mode is not None)
+    T = len(prompt)
+    ys = gb.generate_samples(model, prompt.cuda(), T + 20, 19, temperature=0.0)    # two groups of rows where the step is fused
+    assert len(ys) == 19 and all(torch.equal(y[:T].cpu(), prompt) and len(y) == T + 20 for y in ys)
+    for y in {tuple(y.tolist()) for y in ys}:    # (rows of one group are the same numbers; groups of other sizes run other kernels)
+        l32, tol = along(model, rc, pw, torch.tensor(y), T)
+        chosen = l32.gather(1, torch.tensor(y[T:])[:, None])[:, 0]
+        assert (l32.amax(-1) - chosen <= 2 * tol).all()
+    assert len({tuple(y.tolist()) for y in ys[:16]}) == 1
+
+
+@torch.inference_mode()
+def test_drawn_answers_and_their_log_probabilities(golden):
+    import lit_gpt_b200.generate.base as gb
+
+    model, rc, pw, prompt = toy(golden)
+    T = len(prompt)
+
+    def answers(seed):
+        torch.manual_seed(seed)
+        gb._RNG.clear()
+        return gb.generate_samples(model, prompt.cuda(), T + 30, 6, temperature=0.8, logprobs=True)
+
+    ys, lps = answers(5)
+    again, _ = answers(5)
+    other, _ = answers(6)
+    assert all(torch.equal(a, b) for a, b in zip(ys, again)) and not all(torch.equal(a, b) for a, b in zip(ys, other))
+    assert len({tuple(y.tolist()) for y in ys}) == 6
+    ys2 = gb.generate_samples(model, prompt.cuda(), T + 30, 6, temperature=0.8)    # the next call draws on
+    assert not all(torch.equal(a, b) for a, b in zip(other, ys2))
+    for y, lp in zip(ys, lps):
+        l32, tol = along(model, rc, pw, y.cpu(), T)
+        want = torch.log_softmax(l32 / 0.8, -1).gather(1, y[T:].cpu()[:, None])[:, 0]
+        assert lp.shape == want.shape and ((lp.cpu() - want).abs() <= 2 * tol / 0.8).all()    # a logit off by tol moves its probability's logarithm by 2 tol / T at most
+
+
+@torch.inference_mode()
+def test_answers_end_at_eos_and_obey_their_rules(golden):
+    import lit_gpt_b200.generate.base as gb
+
+    model, rc, pw, prompt = toy(golden)
+    T, p = len(prompt), prompt.cuda()
+    ys = gb.generate_samples(model, p, T + 40, 9, temperature=1.0)
+    eos = ys[0][T + 3].item()
+    torch.manual_seed(3)
+    for y in gb.generate_samples(model, p, T + 40, 9, temperature=1.0, eos_id=eos):
+        body = y[T:].tolist()
+        assert eos not in body[:-1] and (body[-1] == eos or len(body) == 40)
+    for y in gb.generate_samples(model, p, T + 40, 5, temperature=0.7, frequency_penalty=1e4):
+        assert len(set(y[T:].tolist())) == 40
+    for y in gb.generate_samples(model, p, T + 40, 5, temperature=0.7, presence_penalty=1e4, count_prompt=True):
+        assert len(set(y[T:].tolist())) == 40 and not set(y[T:].tolist()) & set(prompt.tolist())
+    for y in gb.generate_samples(model, p, T + 20, 3, temperature=0.0, logit_bias={7: 1e6}):
+        assert y[T:].tolist() == [7] * 20
+    for y in gb.generate_samples(model, p, T + 20, 3, logit_bias={t: float("-inf") for t in range(50)}):
+        assert min(y[T:].tolist()) >= 50
+    one = gb.generate_samples(model, p, T + 1, 4, temperature=0.0)    # the first token alone
+    assert len(one) == 4 and all(len(y) == T + 1 for y in one)
+
+
+@torch.inference_mode()
+def test_one_captured_step_serves_prompts_of_all_lengths(golden):
+    import lit_gpt_b200.generate.base as gb
+
+    model, *_ = toy(golden)
+    fresh, *_ = toy(golden)
+    g = torch.Generator().manual_seed(8)
+    alone = torch.randint(0, 100, (11,), generator=g).cuda()
+    before = gb.generate(model, alone, 40, temperature=0.0)
+    for T in (9, 60, 3, 100):
+        prompt = torch.randint(0, 100, (T,), generator=g).cuda()
+        ys = gb.generate_samples(model, prompt, T + 25, 4, temperature=0.0)
+        fresh.__dict__.pop("_sample_graphs", None)
+        for blk in fresh.transformer.h:
+            blk.attn.kv_cache.reset_parameters()
+        assert all(torch.equal(a, b) for a, b in zip(ys, gb.generate_samples(fresh, prompt, T + 25, 4, temperature=0.0)))
+    assert len(model._sample_graphs) == 1 and next(iter(model._sample_graphs.values())).graph is not None
+    assert torch.equal(before, gb.generate(model, alone, 40, temperature=0.0))    # the model's own caches and captured step
+    model.max_seq_length = 150
+    model.set_kv_cache(batch_size=2, device="cuda", dtype=torch.bfloat16)
+    assert "_sample_graphs" not in model.__dict__
+    ys = gb.generate_samples(model, alone, 40, 3, temperature=0.0)
+    assert all(torch.equal(ys[0], y) for y in ys)
+
+
+@torch.inference_mode()
+def test_refusals(golden):
+    import lit_gpt_b200.generate.base as gb
+
+    model, _, _, prompt = toy(golden)
+    p, T = prompt.cuda(), len(prompt)
+    for kw, error in ((dict(num_samples=0), ValueError), (dict(num_samples=2, logit_bias={-1: 1.0}), ValueError), (dict(num_samples=2, logit_bias={10 ** 6: 1.0}), ValueError)):
+        with pytest.raises(error):
+            gb.generate_samples(model, p, T + 5, **kw)
+    with pytest.raises(NotImplementedError):
+        gb.generate_samples(model, p, 1000, 2)
+    sg = gb._sample_graph_for(model, 2, 64, 0.0, None, (1.0, 0.0, 0.0), False, False, p.dtype)
+    with sg.in_place(), pytest.raises(RuntimeError, match="one token each"):
+        model(p.view(1, -1).expand(2, -1).contiguous(), torch.arange(T, device="cuda"))
+    model.clear_kv_cache()
+    with pytest.raises(TypeError):
+        gb.generate_samples(model, p, T + 5, 2)
+
+
+@torch.inference_mode()
+def test_traced_step_over_a_shared_prefix(golden):
+    import torch._dynamo
+
+    import lit_gpt_b200.generate.base as gb
+
+    model, _, _, prompt = toy(golden)
+    p, T = prompt.cuda(), len(prompt)
+    model(p.view(1, -1), torch.arange(T, device="cuda"))
+    sg = gb._sample_graph_for(model, 3, 64, 0.0, None, (1.0, 0.0, 0.0), False, False, p.dtype)
+    sg.prefix_len.fill_(T)
+    tok, pos = torch.tensor([[1], [2], [3]], device="cuda"), torch.tensor([T], device="cuda")
+    with sg.in_place():
+        want = model(tok, pos).float()
+        torch._dynamo.reset()
+        with torch.inference_mode(False), torch.no_grad():
+            got = torch.compile(model, backend="eager", fullgraph=True)(tok, pos).float()
+    # another order of the same roundings to bf16 (norms and products are not fused): the rounding points differ by a few steps of 2^-8
+    assert (got - want).abs().max() <= 2 ** -5 * want.abs().max()
+
+
+# ---- models that serve sequences from slots -----------------------------------------------------------------------------------------
+def _kinds():
+    import test_gpu_fizadra as F
+    import test_gpu_lefalix as L
+    import test_gpu_pomipel as P
+
+    return {"lefalix": (L, L.CFG_ODD, {}), "pomipel": (P, P.CFG_ODD, dict(max_seq=200)), "fizadra": (F, F.CFG_ODD, dict(max_seq=200))}
+
+
+@pytest.mark.parametrize("kind", ["lefalix", "pomipel", "fizadra"])
+def test_forked_requests_go_their_own_ways(kind):
+    from lit_gpt_b200.generate.serve import Session
+
+    mod, cfg, kw = _kinds()[kind]
+    w = mod.checkpoint(cfg, 21)
+    model = mod.build(cfg, w, torch.float32, slots=2, **kw)
+    session = Session(model, slots=2)
+    prompt, other = mod.tokens_for(cfg, 23, 1), mod.tokens_for(cfg, 9, 2)
+    session.step([("p", prompt, []), ("q", other, [])])
+    session.fork("p", ["a", "b", "c"])                   # grows
+    assert model.slots.in_use == 5 and session.live["b"][1] == 23
+    with pytest.raises(KeyError):
+        session.fork("nobody", ["x"])
+    for new in (["a"], ["x", "x"], ["q"]):
+        with pytest.raises(ValueError):
+            session.fork("p", new)
+    follow = {r: mod.tokens_for(cfg, 12, 30 + i) for i, r in enumerate("pabcq")}
+    seq = {r: (other if r == "q" else prompt) + follow[r] for r in follow}
+    alone = {r: mod.O.forward(cfg, w, t) for r, t in seq.items()}
+    start = {r: len(seq[r]) - 12 for r in seq}
+
+    def steps(live, first, last, end=()):
+        for i in range(first, last):
+            out = session.step([(r, [follow[r][i]], [0]) for r in live], end=end if i == last - 1 else ())
+            for j, r in enumerate(live):
+                assert mod.rel_err(out[j], alone[r][start[r] + i]) < 1e-4, (r, i)
+
+    steps("pabcq", 0, 4, end=["p", "b"])
+    session.compact()
+    assert sorted(s for s, _ in session.live.values()) == [0, 1, 2] and model.slots.in_use == 3
+    steps("acq", 4, 7)
+    session.shrink()
+    assert model.slots.capacity == 3 and model.slots.in_use == 3
+    steps("acq", 7, 9, end=["q"])
+    session.fork("a", ["d"])
+    follow["d"], alone["d"], start["d"] = follow["a"], alone["a"], start["a"]
+    steps("acd", 9, 12)
+    session.step([], end=["a", "c", "d"])
+    session.shrink()
+    assert model.slots.capacity == 1 and model.slots.in_use == 0
+
+
+@pytest.mark.parametrize("kind", ["lefalix", "pomipel"])
+def test_batches_of_samples_and_rules(kind):
+    import lit_gpt_b200.generate.base as gb
+    from lit_gpt_b200.generate.serve import Session, generate_batch
+
+    mod, cfg, kw = _kinds()[kind]
+    model = mod.build(cfg, mod.checkpoint(cfg, 22), torch.float32, **kw)
+    V = cfg["vocab"]
+    prompts = [mod.tokens_for(cfg, 9, 3), mod.tokens_for(cfg, 4, 4)]
+    plain = generate_batch(model, prompts, 11)
+    ys = generate_batch(model, prompts, 11, num_samples=3)
+    assert ys == [plain[0]] * 3 + [plain[1]] * 3 and model.slots.in_use == 0
+    session = Session(model, slots=1)
+
+    def drawn(seed):
+        torch.manual_seed(seed)
+        gb._RNG.clear()
+        return generate_batch(model, prompts, 11, num_samples=4, temperature=1.0, top_k=30, session=session)
+
+    a, b = drawn(1), drawn(1)
+    assert a == b and a != drawn(2) and len({tuple(y) for y in a}) == 8 and not session.live
+    eos = a[0][len(prompts[0]) + 2]
+    for y, p in zip(generate_batch(model, prompts, 30, num_samples=4, temperature=1.0, eos_id=eos), [prompts[0]] * 4 + [prompts[1]] * 4):
+        assert y[: len(p)] == p and eos not in y[len(p) : -1] and (y[-1] == eos or len(y) == len(p) + 30)
+    for y, p in zip(generate_batch(model, prompts, 30, temperature=0.5, presence_penalty=1e4, count_prompt=True, num_samples=2), [prompts[0]] * 2 + [prompts[1]] * 2):
+        assert len(set(y)) == len(set(p)) + 30
+    even = torch.arange(V) % 2 == 0
+    calls = []
+
+    def grammar(i, tokens):
+        calls.append((i, len(tokens)))
+        if i == 1 and len(tokens) == len(prompts[1]) + 5:
+            return torch.zeros(V, dtype=torch.bool)
+        return even if i == 0 else None
+
+    y0, y1 = generate_batch(model, prompts, 11, allowed=grammar)
+    assert len(y0) == 20 and all(t % 2 == 0 for t in y0[9:]) and len(y1) == 9 and y1 == plain[1][:9] and (0, 9) in calls
+    assert generate_batch(model, prompts, 5, logit_bias={3: 1e6})[0][9:] == [3] * 5
+    with pytest.raises(ValueError):
+        generate_batch(model, prompts, 5, logit_bias={V: 1.0})
+    assert generate_batch(model, [], 5, num_samples=2) == [] and generate_batch(model, prompts, 0, num_samples=2) == [prompts[0]] * 2 + [prompts[1]] * 2
