@@ -4,13 +4,14 @@
 // fp32 with a running maximum, the result is rounded once.
 //
 // The prefix is read once for all rows: the B * (heads per group) query rows of a key-value group are the left operand of its products, a key tile serves them all.
-// Launch 1 computes partial results (maximum, sum, unscaled output) of key ranges, of the prefix for 16 * MT rows of a group and of a row's own keys for
-// its heads of a group; launch 2 joins a row's partial results.  Both kinds of range run side by side in launch 1, so the step has no third launch, and neither has a
-// counter that two calls at a time could share.
+// Three launches: the queries and new keys are turned and the new rows stored; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys of the
+// prefix for up to 32 query rows of a group, and of a row's own keys for its heads of a group; a head's partial results are joined.  No counter or flag is left
+// between calls, and two calls at a time share nothing.
 //
-// A CTA has four warps; warp w takes the key tiles w, w + 4, .. of the CTA's range, double-buffered in its own shared-memory stages by cp.async.  S = Q K^T and
-// O += P V on mma.sync.m16n8k16.  P enters as two bf16 numbers, its leading bits and the rest, so that its rounding does not add to the result's own (with the nearest
-// bf16 number alone the error against 64 bits is a fifth larger than that of the final rounding).  The rest is kept above zero, so that an infinite value
+// All tiles, of the prefix and of all rows' own keys, are one list that is cut evenly over the warps of all SMs, so that neither few rows over a long prefix nor many
+// rows of unequal lengths leave SMs without work.  A warp keeps a ring of units of 32 keys or values, two of them on their way, and the queries of its next item behind them.
+// S = Q K^T and O += P V on mma.sync.m16n8k16.  P enters as two bf16 numbers, its leading bits and the rest, so that its rounding does not add to the result's own (with the
+// nearest bf16 number alone the error against 64 bits is a fifth larger than that of the final rounding).  The rest is kept above zero, so that an infinite value
 // times it is infinite and not NaN.
 #include <math.h>
 
@@ -21,21 +22,25 @@ namespace b200 {
 
 namespace {
 
-constexpr int kShThreads = 128, kShTile = 32;
+constexpr int kShTile = 32;                 // keys of a tile
+constexpr int kShUnits = 3;                 // a warp's ring: units of 32 keys or 32 values
 
 struct SharedParams {
   const __nv_bfloat16* qkv;
   const void* cos; const void* sin;
-  int table_bf16, table_rows, table_presel, rope_n;
+  int table_bf16, table_rows, table_presel, rope_n, wide;   // wide: rows of heads and tables allow accesses of HS / 32 numbers
   const void* pos; int pos64, pos_each;      // pos_each: one position per row
   const void* plen; int plen64;              // null: prefix_rows
   __nv_bfloat16* kc; __nv_bfloat16* vc; int64_t kc_b, kc_g, vc_b, vc_g;
   const __nv_bfloat16* kp; const __nv_bfloat16* vp; int64_t kp_g, vp_g;
   __nv_bfloat16* out;
   int batch, n_head, n_groups, per, own_rows, prefix_rows;
-  int tiles, prefix_splits, own_splits, head_tiles;   // query-row tiles of a group; key ranges; tiles of 16 heads of one row
-  float* acc;                                // [batch][n_head][splits][HS]
-  float2* ml;                                // [batch][n_head][splits]: maximum (log2 units), sum
+  int head_tiles, row_tiles;                 // tiles of 16 heads of a row's group; tiles of a group's query rows over the prefix
+  __nv_bfloat16* q;                          // the queries, turned: [n_groups][batch * per][HS]
+  int workers, sms;                          // warps that share the tiles, at most
+  float* own_acc; float2* own_ml;            // results of key ranges of own items: slots of min(16, per) rows
+  float* pre_acc; float2* pre_ml;            // of prefix items: slots of 16 * MT rows
+  int ways;                                  // warps that join a head's results
   float scale_log2;
 };
 
@@ -48,314 +53,620 @@ __device__ __forceinline__ int prefix_len(const SharedParams& p) {
   const int64_t n = index_at(p.plen, p.plen64, 0);
   return (int)(n < 0 ? 0 : (n > p.prefix_rows ? p.prefix_rows : n));
 }
-// index of a row's new key in its own cache (pos >= 0)
+// index of a row's new key in its own cache; -1: the row takes no part
 __device__ __forceinline__ int own_index(const SharedParams& p, int64_t pos, int plen) {
+  if (pos < 0) return -1;
   const int64_t i = pos - plen;
   return (int)(i < 0 ? 0 : (i >= p.own_rows ? p.own_rows - 1 : i));
 }
-__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-
-// apply_rope (lit_gpt/model.py:767-773) on element d of a head, for a position's table row
-__device__ __forceinline__ __nv_bfloat16 turned(const SharedParams& p, const __nv_bfloat16* x, int d, int64_t row) {
-  const int n = p.rope_n;
-  if (d >= n) return x[d];
-  const int half = n >> 1;
-  const float a = __bfloat162float(x[d]), o = __bfloat162float(d < half ? x[d + half] : x[d - half]), rot = d < half ? -o : o;
-  const float c = table_at(p.cos, p.table_bf16, row * n + d), s = table_at(p.sin, p.table_bf16, row * n + d);
-  if (p.table_bf16) return __float2bfloat16_rn(__fadd_rn(round_bf16(__fmul_rn(a, c)), round_bf16(__fmul_rn(rot, s))));
-  return __float2bfloat16_rn(__fadd_rn(__fmul_rn(a, c), __fmul_rn(rot, s)));
-}
+__device__ __forceinline__ int own_tiles(const SharedParams& p, int b, int plen) { return (own_index(p, row_pos(p, b), plen) + kShTile) / kShTile; }
 __device__ __forceinline__ int64_t table_row(const SharedParams& p, int b, int64_t pos) {
   const int64_t r = p.table_presel ? (p.pos_each ? b : 0) : pos;
   return r < 0 ? 0 : (r >= p.table_rows ? p.table_rows - 1 : r);
 }
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// Shared memory: four warps' key and value stages, then the query tile.
+// apply_rope (lit_gpt/model.py:767-773)
+__device__ __forceinline__ float turned(float a, float other, bool low, float c, float s, int table_bf16) {
+  const float rot = low ? -other : other;
+  if (table_bf16) return __fadd_rn(round_bf16(__fmul_rn(a, c)), round_bf16(__fmul_rn(rot, s)));
+  return __fadd_rn(__fmul_rn(a, c), __fmul_rn(rot, s));
+}
+// HS / 32 numbers of a head from lane * HS / 32 on, after the rotation
+template <int HS>
+__device__ __forceinline__ void turned_part(const SharedParams& p, const __nv_bfloat16* x, int64_t trow, int lane, uint32_t (&out)[HS / 64]) {
+  constexpr int V = HS / 32;
+  const int n = p.rope_n, half = n >> 1, d0 = lane * V;
+  if (p.wide) {
+    auto get = [&](int d, float (&f)[V]) {
+      if constexpr (V == 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(x + d);
+        f[0] = bf16lo(w.x); f[1] = bf16hi(w.x); f[2] = bf16lo(w.y); f[3] = bf16hi(w.y);
+      } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(x + d);
+        f[0] = bf16lo(w); f[1] = bf16hi(w);
+      }
+    };
+    auto table = [&](const void* t, float (&f)[V]) {
+      const int64_t at = trow * n + d0;
+      if (p.table_bf16) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(t)[at + i]);
+      } else if constexpr (V == 4) {
+        const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(t) + at);
+        f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
+      } else {
+        const float2 w = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(t) + at);
+        f[0] = w.x; f[1] = w.y;
+      }
+    };
+    float a[V];
+    get(d0, a);
+    if (d0 < n) {
+      const bool low = d0 < half;
+      float o[V], c[V], s[V];
+      get(low ? d0 + half : d0 - half, o);
+      table(p.cos, c);
+      table(p.sin, s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = turned(a[i], o[i], low, c[i], s[i], p.table_bf16);
+    }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) out[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
+  } else {
+    float a[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int d = d0 + i;
+      a[i] = __bfloat162float(x[d]);
+      if (d < n) {
+        const bool low = d < half;
+        a[i] = turned(a[i], __bfloat162float(x[low ? d + half : d - half]), low, table_at(p.cos, p.table_bf16, trow * n + d), table_at(p.sin, p.table_bf16, trow * n + d),
+                      p.table_bf16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) out[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
+  }
+}
+
+// The tiles of a step, one after the other: rows' own keys, row after row, there group after group and tile of heads after tile of heads, then the prefix, group after
+// group and tile of query rows after tile of query rows.  An item is what one query tile sees of one of them.  Workers take runs of tiles; the result of item i by worker w goes to
+// slot i + w, which no other pair has, since either grows with the tiles.
+struct Split {
+  int own, all;          // tiles of own keys; all tiles
+  int prefix, workers;   // tiles of the prefix for one item; workers
+  int each, more;        // every worker has `each` tiles, the first `more` of them one more
+};
+__device__ __forceinline__ int worker_of(int tile, const Split& s) {
+  const int wide = s.more * (s.each + 1);
+  return tile < wide ? tile / (s.each + 1) : s.more + (tile - wide) / s.each;
+}
+__device__ __forceinline__ int first_tile(int w, const Split& s) { return w * s.each + min(w, s.more); }
+
+// Rows are summed in runs of one per thread: sums[t] = own tiles (of one group and tile of heads) of the rows before run t; sums[THREADS] of all.
+template <int THREADS>
+__device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int* sums, int* s_warp) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = (p.batch + THREADS - 1) / THREADS;
+  int mine = 0;
+  for (int b = tid * run; b < min(p.batch, (tid + 1) * run); ++b) mine += own_tiles(p, b, plen);
+  int inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int before = inc - mine;
+  for (int w = 0; w < warp; ++w) before += s_warp[w];
+  sums[tid] = before;
+  if (tid == THREADS - 1) sums[THREADS] = before + mine;
+  __syncthreads();
+  Split s;
+  s.own = sums[THREADS] * p.n_groups * p.head_tiles;
+  s.prefix = (plen + kShTile - 1) / kShTile;
+  s.all = s.own + s.prefix * p.n_groups * p.row_tiles;
+  // two tiles a worker at least, unless that leaves SMs without one
+  s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
+  s.each = s.workers ? s.all / s.workers : 0;
+  s.more = s.all - s.each * s.workers;
+  return s;
+}
+
+// A warp's shared memory: a ring of units, the queries of two items.  One CTA an SM.
 template <int HS, int MT>
 struct ShSmem {
-  static constexpr int kStage = 2 * kShTile * HS * 2, kWarp = 2 * kStage;     // K + V tile; two stages
-  static constexpr int kQ = 16 * MT * HS * 2;
-  static constexpr int kBytes = 4 * kWarp + kQ + 2 * HS * 2;
+  static constexpr int kUnit = kShTile * HS * 2, kQ = 16 * MT * HS * 2;
+  static constexpr int kWarp = kShUnits * kUnit + 2 * kQ;
+  static constexpr int kWarps = HS == 64 ? (MT == 2 ? 10 : 12) : (MT == 2 ? 5 : 7);
+  static constexpr int kBytes = kWarps * kWarp;
 };
 
-// The CTA's query tile against the keys [kbeg, kend) of one matrix of keys and values (rows HS apart), and the four warps' results joined.  `fresh` >= 0: that key's row
-// and its value are in shared memory (nk, nv) and not yet in the matrix.  Results of row r go to slot(r); slot(r) < 0: nowhere.
-template <int HS, int MT, typename Slot>
-__device__ __forceinline__ void attend(const SharedParams& p, uint8_t* smem, uint8_t* sQ, const __nv_bfloat16* kg, const __nv_bfloat16* vg, int kbeg, int kend,
-                                       int fresh, const __nv_bfloat16* nk, const __nv_bfloat16* nv, float (*s_m)[16 * MT], float (*s_l)[16 * MT], Slot slot) {
-  constexpr int CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
-  const uint32_t wbase = pf_smem(smem) + warp * ShSmem<HS, MT>::kWarp;
-  const int ntiles = kend > kbeg ? (kend - kbeg + kShTile - 1) / kShTile : 0;
+// ---- the queries and the new keys turned, the new rows stored: a head a warp ----
+template <int HS>
+__global__ void __launch_bounds__(256) attn_shared_turn_kernel(const SharedParams p) {
+  constexpr int V = HS / 32;
+  griddep_wait();     // (before the launch of what follows: the kernels behind read positions, lengths and the prefix ahead of their own wait)
+  griddep_launch();
+  const int lane = threadIdx.x & 31, heads = p.n_groups * (p.per + 2);
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int b = (int)(at / heads), i = (int)(at - (int64_t)b * heads), gi = i / (p.per + 2), h = i - gi * (p.per + 2);
+  if (b >= p.batch) return;
+  const int64_t pos = row_pos(p, b);
+  const __nv_bfloat16* const x = p.qkv + at * HS;
+  uint32_t v[HS / 64];
+  if (h <= p.per) {
+    turned_part<HS>(p, x, table_row(p, b, pos), lane, v);
+  } else {
+    const uint16_t* const u = reinterpret_cast<const uint16_t*>(x + lane * V);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = (uint32_t)u[2 * j] | ((uint32_t)u[2 * j + 1] << 16);
+  }
+  __nv_bfloat16* to;
+  if (h < p.per) {
+    to = p.q + ((int64_t)gi * p.batch * p.per + (int64_t)b * p.per + h) * HS;
+    if (pos < 0)
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) v[j] = 0u;
+  } else {
+    const int mine = own_index(p, pos, prefix_len(p));
+    if (mine < 0) return;
+    to = (h == p.per ? p.kc + (int64_t)b * p.kc_b + (int64_t)gi * p.kc_g : p.vc + (int64_t)b * p.vc_b + (int64_t)gi * p.vc_g) + (int64_t)mine * HS;
+  }
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(to + lane * V) = make_uint2(v[0], v[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t*>(to + lane * V) = v[0];
+}
 
-  auto load_tile = [&](int tile, int buf) {
-    const int j0 = kbeg + tile * kShTile;
-    const uint32_t kb = wbase + buf * ShSmem<HS, MT>::kStage, vb = kb + kShTile * HS * 2;
+// A tile of a worker's range, and the item that it belongs to.
+struct Tile {
+  int index;                         // in the order of all tiles
+  const __nv_bfloat16* k; const __nv_bfloat16* v;   // its first rows
+  int valid;                         // rows of it
+  int left;                          // tiles of the item behind this one
+  int own;                           // an own item?
+  int b, gi, part;                   // row, group, tile of heads (own); -, group, tile of query rows
+  int at;                            // own: index of the new key
+};
+
+template <int HS, int MT>
+struct Walk {
+  const SharedParams& p;
+  const Split& s;
+  const int* sums;
+  int plen, run;
+
+  __device__ __forceinline__ void own_item(Tile& t, int mine, int tile) const {
+    const int tiles = mine / kShTile + 1;
+    t.own = 1;
+    t.at = mine;
+    t.left = tiles - 1 - tile;
+    t.k = p.kc + (int64_t)t.b * p.kc_b + (int64_t)t.gi * p.kc_g + (int64_t)tile * kShTile * HS;
+    t.v = p.vc + (int64_t)t.b * p.vc_b + (int64_t)t.gi * p.vc_g + (int64_t)tile * kShTile * HS;
+    t.valid = min(kShTile, mine + 1 - tile * kShTile);
+  }
+  __device__ __forceinline__ void prefix_item(Tile& t, int tile) const {
+    t.own = 0;
+    t.left = s.prefix - 1 - tile;
+    t.k = p.kp + (int64_t)t.gi * p.kp_g + (int64_t)tile * kShTile * HS;
+    t.v = p.vp + (int64_t)t.gi * p.vp_g + (int64_t)tile * kShTile * HS;
+    t.valid = min(kShTile, plen - tile * kShTile);
+  }
+  __device__ __forceinline__ Tile find(int index, int threads) const {
+    Tile t;
+    t.index = index;
+    if (index < s.own) {
+      const int each = p.n_groups * p.head_tiles;
+      int lo = 0, hi = threads;      // the run whose rows hold it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (sums[mid] * each <= index) lo = mid; else hi = mid;
+      }
+      int rest = index - sums[lo] * each;
+      int b = lo * run, mine = own_index(p, row_pos(p, b), plen);
+      for (;;) {                     // (one row a run unless the batch is large)
+        const int here = (mine + kShTile) / kShTile * each;
+        if (rest < here) break;
+        rest -= here;
+        ++b;
+        mine = own_index(p, row_pos(p, b), plen);
+      }
+      const int tiles = mine / kShTile + 1, item = rest / tiles;
+      t.b = b;
+      t.gi = item / p.head_tiles;
+      t.part = item - t.gi * p.head_tiles;
+      own_item(t, mine, rest - item * tiles);
+    } else {
+      const int rest = index - s.own, item = rest / s.prefix;
+      t.b = 0;
+      t.gi = item / p.row_tiles;
+      t.part = item - t.gi * p.row_tiles;
+      t.at = 0;
+      prefix_item(t, rest - item * s.prefix);
+    }
+    return t;
+  }
+  // the tile behind it (there is one)
+  __device__ __forceinline__ void next(Tile& t) const {
+    ++t.index;
+    if (t.left > 0) {
+      --t.left;
+      t.k += kShTile * HS;
+      t.v += kShTile * HS;
+      if (t.own) {
+        const int done = t.at / kShTile - t.left;
+        t.valid = min(kShTile, t.at + 1 - done * kShTile);
+      } else {
+        t.valid = min(kShTile, plen - (s.prefix - 1 - t.left) * kShTile);
+      }
+      return;
+    }
+    if (t.index == s.own) {
+      t.gi = t.part = 0;
+      prefix_item(t, 0);
+    } else if (t.own) {
+      int mine = t.at;
+      if (++t.part == p.head_tiles) {
+        t.part = 0;
+        if (++t.gi == p.n_groups) {
+          t.gi = 0;
+          do { ++t.b; mine = own_index(p, row_pos(p, t.b), plen); } while (mine < 0);
+        }
+      }
+      own_item(t, mine, 0);
+    } else {
+      if (++t.part == p.row_tiles) { t.part = 0; ++t.gi; }
+      prefix_item(t, 0);
+    }
+  }
+  __device__ __forceinline__ int64_t query_row(const Tile& t) const {
+    return (int64_t)t.gi * p.batch * p.per + (t.own ? (int64_t)t.b * p.per + t.part * 16 : (int64_t)t.part * 16 * MT);
+  }
+  __device__ __forceinline__ int queries(const Tile& t) const { return t.own ? min(16, p.per - t.part * 16) : min(16 * MT, p.batch * p.per - t.part * 16 * MT); }
+  __device__ __forceinline__ int64_t item(const Tile& t) const {   // own items count with rows that take no part
+    return t.own ? ((int64_t)t.b * p.n_groups + t.gi) * p.head_tiles + t.part : (int64_t)t.gi * p.row_tiles + t.part;
+  }
+};
+
+template <int HS, int M>
+struct Sums {
+  float o[M][HS / 8][4], m[M][2], l[M][2];
+};
+
+// S = Q K^T of 16 * M rows and a tile, and the tile's weights; `vb` is waited for by `values`
+template <int HS, int MT, int M, typename Values>
+__device__ __forceinline__ void attend_tile(Sums<HS, MT>& a, uint32_t q, uint32_t kb, int valid, float scale_log2, int lane, Values values) {
+  const int tq = lane & 3;
+  float s[M][kShTile / 8][4];
+#pragma unroll
+  for (int t = 0; t < M; ++t)
+#pragma unroll
+    for (int i = 0; i < kShTile / 8; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < HS / 16; ++ks) {
+    uint32_t qf[M][4];
+#pragma unroll
+    for (int t = 0; t < M; ++t) ldsm_x4(qf[t], q + sw<HS>(t * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+#pragma unroll
+    for (int np = 0; np < kShTile / 16; ++np) {
+      uint32_t kf[4];
+      ldsm_x4(kf, kb + sw<HS>(np * 16 + ((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+      for (int t = 0; t < M; ++t) {
+        pf_mma(s[t][2 * np], qf[t], kf[0], kf[1]);
+        pf_mma(s[t][2 * np + 1], qf[t], kf[2], kf[3]);
+      }
+    }
+  }
+  uint32_t hi[M][kShTile / 16][4], lo[M][kShTile / 16][4];
+#pragma unroll
+  for (int t = 0; t < M; ++t) {
+    float top[2] = {a.m[t][0], a.m[t][1]};
+#pragma unroll
+    for (int i = 0; i < kShTile / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[t][i][e] = i * 8 + 2 * tq + (e & 1) < valid ? s[t][i][e] * scale_log2 : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[t][i][e]);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      const float org = top[h] == -INFINITY ? 0.f : top[h];   // (scores that are all -inf: weights of zero)
+      const float shrink = ex2(a.m[t][h] - org);
+      a.m[t][h] = top[h];
+      a.l[t][h] *= shrink;
+#pragma unroll
+      for (int i = 0; i < HS / 8; ++i) { a.o[t][i][2 * h] *= shrink; a.o[t][i][2 * h + 1] *= shrink; }
+#pragma unroll
+      for (int i = 0; i < kShTile / 8; ++i) {
+        const float x = ex2(s[t][i][2 * h] - org), y = ex2(s[t][i][2 * h + 1] - org);
+        a.l[t][h] += x + y;
+        const uint32_t w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);   // the leading 16 bits of both
+        hi[t][i >> 1][(i & 1) * 2 + h] = w;
+        lo[t][i >> 1][(i & 1) * 2 + h] = pack_bf16(fmaxf(x - bf16lo(w), 1e-36f), fmaxf(y - bf16hi(w), 1e-36f));
+      }
+    }
+  }
+  const uint32_t vb = values();
+#pragma unroll
+  for (int ks = 0; ks < kShTile / 16; ++ks) {
+#pragma unroll
+    for (int dp = 0; dp < HS / 16; ++dp) {
+      uint32_t vf[4];
+      ldsm_x4_t(vf, vb + sw<HS>(ks * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), dp * 2 + (lane >> 4)));
+#pragma unroll
+      for (int t = 0; t < M; ++t) {
+        pf_mma(a.o[t][2 * dp], hi[t][ks], vf[0], vf[1]);
+        pf_mma(a.o[t][2 * dp + 1], hi[t][ks], vf[2], vf[3]);
+        pf_mma(a.o[t][2 * dp], lo[t][ks], vf[0], vf[1]);
+        pf_mma(a.o[t][2 * dp + 1], lo[t][ks], vf[2], vf[3]);
+      }
+    }
+  }
+}
+
+template <int HS, int MT>
+__global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_kernel(const SharedParams p) {
+  using C = ShSmem<HS, MT>;
+  constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
+  extern __shared__ __align__(128) uint8_t sh_smem[];
+  __shared__ int s_sums[T + 1], s_warp[C::kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
+  griddep_launch();
+  const int plen = prefix_len(p);
+  const Split s = make_split<T>(p, plen, s_sums, s_warp);
+  const int w = warp * (int)gridDim.x + (int)blockIdx.x;   // (workers beside each other on different SMs)
+  if (w >= s.workers) {
+    griddep_wait();
+    return;
+  }
+  const Walk<HS, MT> walk{p, s, s_sums, plen, (p.batch + T - 1) / T};
+  const uint32_t ring = pf_smem(sh_smem) + warp * C::kWarp, sq = ring + kShUnits * C::kUnit;
+
+  auto load = [&](uint32_t dst, const __nv_bfloat16* src, int valid) {   // 32 rows, zeros from `valid` on: a weight of zero times whatever lies there must be zero
 #pragma unroll
     for (int j = 0; j < kShTile / RP; ++j) {
       const int r = j * RP + lane / CH, c = lane % CH;
-      const bool ok = j0 + r < kend && j0 + r != fresh;   // (zeros behind the range: a weight of zero times whatever lies there must be zero)
-      const int64_t off = (int64_t)(ok ? j0 + r : kbeg) * HS + c * 8;
-      pf_cp16(kb + sw<HS>(r, c), kg + off, ok);
-      pf_cp16(vb + sw<HS>(r, c), vg + off, ok);
+      const bool ok = r < valid;
+      pf_cp16(dst + sw<HS>(r, c), src + (ok ? r * HS : 0) + c * 8, ok);
     }
-    pf_commit();
   };
-
-  float o[MT][HS / 8][4], m[MT][2], l[MT][2];
+  auto load_queries = [&](uint32_t dst, const Tile& t) {
+    const __nv_bfloat16* const src = p.q + walk.query_row(t) * HS;
+    const int valid = walk.queries(t);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-#pragma unroll
-    for (int i = 0; i < HS / 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
-    m[t][0] = m[t][1] = -INFINITY;
-    l[t][0] = l[t][1] = 0.f;
+    for (int j = 0; j < 16 * MT / RP; ++j) {
+      const int r = j * RP + lane / CH, c = lane % CH;
+      const bool ok = r < valid;
+      pf_cp16(dst + sw<HS>(r, c), src + (ok ? r * HS : 0) + c * 8, ok);
+    }
+  };
+  const int end = first_tile(w + 1, s);
+  Tile cur = walk.find(first_tile(w, s), T);
+  // What the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before.
+  if (!cur.own) load(ring, cur.k, cur.valid);
+  griddep_wait();
+  if (cur.own) load(ring, cur.k, cur.valid);
+  load_queries(sq, cur);
+  pf_commit();
+  load(ring + C::kUnit, cur.v, cur.valid);
+  pf_commit();
+  Tile coming = cur;                                       // the tile behind it: its values are loaded next
+  int qb = 0, next_qb = 0;                                 // the query buffers of either
+  if (cur.index + 1 < end) {
+    walk.next(coming);
+    load(ring + 2 * C::kUnit, coming.k, coming.valid);
+    if (cur.left == 0) load_queries(sq + (next_qb = 1) * C::kQ, coming);
   }
-  if (warp < ntiles) load_tile(warp, 0);
-  int it = 0;
-  for (int tile = warp; tile < ntiles; tile += 4, ++it) {
-    const int buf = it & 1;
-    if (tile + 4 < ntiles) { load_tile(tile + 4, buf ^ 1); pf_wait<1>(); } else { pf_wait<0>(); }
-    __syncwarp();
-    const int j0 = kbeg + tile * kShTile;
-    const uint32_t kb = wbase + buf * ShSmem<HS, MT>::kStage, vb = kb + kShTile * HS * 2;
-    if (fresh >= j0 && fresh < j0 + kShTile) {
-      if (lane < 2 * CH) {
-        const int r = fresh - j0, c = lane % CH;
-        const uint4 val = *reinterpret_cast<const uint4*>((lane < CH ? nk : nv) + c * 8);
-        const uint32_t dst = (lane < CH ? kb : vb) + sw<HS>(r, c);
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(val.x), "r"(val.y), "r"(val.z), "r"(val.w) : "memory");
-      }
-      __syncwarp();
-    }
-    float s[MT][kShTile / 8][4];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int i = 0; i < kShTile / 8; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < HS / 16; ++ks) {
-      uint32_t qf[MT][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) ldsm_x4(qf[t], pf_smem(sQ) + sw<HS>(t * 16 + (lane & 15), ks * 2 + (lane >> 4)));
-#pragma unroll
-      for (int np = 0; np < kShTile / 16; ++np) {
-        uint32_t kf[4];
-        ldsm_x4(kf, kb + sw<HS>(np * 16 + ((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          pf_mma(s[t][2 * np], qf[t], kf[0], kf[1]);
-          pf_mma(s[t][2 * np + 1], qf[t], kf[2], kf[3]);
-        }
-      }
-    }
-    uint32_t hi[MT][kShTile / 16][4], lo[MT][kShTile / 16][4];
+  pf_commit();
+
+  Sums<HS, MT> a;
+  auto clear = [&]() {
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float top[2] = {m[t][0], m[t][1]};
 #pragma unroll
-      for (int i = 0; i < kShTile / 8; ++i) {
-        const int j = j0 + i * 8 + 2 * tq;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[t][i][e] = (j + (e & 1) < kend) ? s[t][i][e] * p.scale_log2 : -INFINITY;
-          top[e >> 1] = fmaxf(top[e >> 1], s[t][i][e]);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        const float org = top[h] == -INFINITY ? 0.f : top[h];   // (scores that are all -inf: weights of zero)
-        const float shrink = ex2(m[t][h] - org);
-        m[t][h] = top[h];
-        l[t][h] *= shrink;
-#pragma unroll
-        for (int i = 0; i < HS / 8; ++i) { o[t][i][2 * h] *= shrink; o[t][i][2 * h + 1] *= shrink; }
-#pragma unroll
-        for (int i = 0; i < kShTile / 8; ++i) {
-          const float a = ex2(s[t][i][2 * h] - org), b = ex2(s[t][i][2 * h + 1] - org);
-          l[t][h] += a + b;
-          const uint32_t w = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);   // the leading 16 bits of both
-          hi[t][i >> 1][(i & 1) * 2 + h] = w;
-          lo[t][i >> 1][(i & 1) * 2 + h] = pack_bf16(fmaxf(a - bf16lo(w), 1e-36f), fmaxf(b - bf16hi(w), 1e-36f));
-        }
-      }
+      for (int i = 0; i < HS / 8; ++i) a.o[t][i][0] = a.o[t][i][1] = a.o[t][i][2] = a.o[t][i][3] = 0.f;
+      a.m[t][0] = a.m[t][1] = -INFINITY;
+      a.l[t][0] = a.l[t][1] = 0.f;
     }
-#pragma unroll
-    for (int ks = 0; ks < kShTile / 16; ++ks) {
-#pragma unroll
-      for (int dp = 0; dp < HS / 16; ++dp) {
-        uint32_t vf[4];
-        ldsm_x4_t(vf, vb + sw<HS>(ks * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), dp * 2 + (lane >> 4)));
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          pf_mma(o[t][2 * dp], hi[t][ks], vf[0], vf[1]);
-          pf_mma(o[t][2 * dp + 1], hi[t][ks], vf[2], vf[3]);
-          pf_mma(o[t][2 * dp], lo[t][ks], vf[0], vf[1]);
-          pf_mma(o[t][2 * dp + 1], lo[t][ks], vf[2], vf[3]);
-        }
-      }
-    }
-    __syncwarp();   // the stage just read is filled again by this warp's own copies
-  }
-
-  // the warp's result into its own stages, then all four joined
-  float* const mine = reinterpret_cast<float*>(smem + warp * ShSmem<HS, MT>::kWarp);   // [16 * MT][HS]
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 1);
-      l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 2);
-      const int r = t * 16 + h * 8 + g;
-#pragma unroll
-      for (int i = 0; i < HS / 8; ++i) *reinterpret_cast<float2*>(mine + r * HS + i * 8 + 2 * tq) = make_float2(o[t][i][2 * h], o[t][i][2 * h + 1]);
-      if (tq == 0) { s_m[warp][r] = m[t][h]; s_l[warp][r] = l[t][h]; }
-    }
-  __syncthreads();
-  for (int i = tid; i < 16 * MT * (HS / 4); i += kShThreads) {
-    const int r = i / (HS / 4), d = (i % (HS / 4)) * 4;
-    const int64_t at = slot(r);
-    if (at < 0) continue;
-    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])), org = top == -INFINITY ? 0.f : top;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (s_m[w][r] == -INFINITY && !(s_l[w][r] != 0.f)) continue;   // (nothing there)
-      const float c = ex2(s_m[w][r] - org);
-      const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * ShSmem<HS, MT>::kWarp) + r * HS + d);
-      a.x += v.x * c; a.y += v.y * c; a.z += v.z * c; a.w += v.w * c;
-      sum += s_l[w][r] * c;
-    }
-    __stcg(reinterpret_cast<float4*>(p.acc + at * HS + d), a);
-    if (d == 0) __stcg(p.ml + at, make_float2(top, sum));
-  }
-}
-
-template <int HS, int MT>
-__global__ void __launch_bounds__(kShThreads, 1) attn_shared_kernel(const SharedParams p) {
-  extern __shared__ __align__(128) uint8_t sh_smem[];
-  __shared__ float s_m[4][16 * MT], s_l[4][16 * MT];
-  uint8_t* const sQ = sh_smem + 4 * ShSmem<HS, MT>::kWarp;
-  const int tid = threadIdx.x;
-  griddep_launch();
-  griddep_wait();
-  const int plen = prefix_len(p), splits = p.prefix_splits + p.own_splits;
-  int unit = blockIdx.x;
-  const int own_units = p.batch * p.n_groups * p.head_tiles * p.own_splits;
-  if (unit >= own_units) {
-    // ---- rows of a group against a range of the prefix ----
-    unit -= own_units;
-    const int split = unit % p.prefix_splits, tile = (unit / p.prefix_splits) % p.tiles, gi = unit / (p.prefix_splits * p.tiles);
-    const int per_range = (plen + p.prefix_splits - 1) / p.prefix_splits;
-    const int kbeg = min(plen, split * per_range), kend = min(plen, kbeg + per_range);
-    const int rows = p.batch * p.per;
-    for (int i = tid; i < 16 * MT * HS; i += kShThreads) {
-      const int r = i / HS, d = i % HS, row = tile * 16 * MT + r, b = row / p.per, h = row - b * p.per;
-      __nv_bfloat16 v = __float2bfloat16_rn(0.f);
-      if (row < rows) {
-        const int64_t pos = row_pos(p, b);
-        if (pos >= 0) v = turned(p, p.qkv + (((int64_t)b * p.n_groups + gi) * (p.per + 2) + h) * HS, d, table_row(p, b, pos));
-      }
-      *reinterpret_cast<__nv_bfloat16*>(sQ + sw<HS>(r, d >> 3) + (d & 7) * 2) = v;
-    }
-    __syncthreads();
-    attend<HS, MT>(p, sh_smem, sQ, p.kp + (int64_t)gi * p.kp_g, p.vp + (int64_t)gi * p.vp_g, kbeg, kend, -1, nullptr, nullptr, s_m, s_l, [&](int r) -> int64_t {
-      const int row = tile * 16 * MT + r, b = row / p.per;
-      return row < rows ? ((int64_t)b * p.n_head + gi * p.per + (row - b * p.per)) * splits + split : (int64_t)-1;
-    });
-    return;
-  }
-  // ---- a row's heads of a group against a range of its own keys ----
-  const int split = unit % p.own_splits;
-  unit /= p.own_splits;
-  const int ht = unit % p.head_tiles;
-  unit /= p.head_tiles;
-  const int gi = unit % p.n_groups, b = unit / p.n_groups;
-  const int64_t pos = row_pos(p, b);
-  if (pos < 0) return;
-  const int mine = own_index(p, pos, plen), keys = mine + 1, per_range = (keys + p.own_splits - 1) / p.own_splits;
-  const int kbeg = min(keys, split * per_range), kend = min(keys, kbeg + per_range);
-  const bool fresh = mine >= kbeg && mine < kend;
-  __nv_bfloat16* const nk = reinterpret_cast<__nv_bfloat16*>(sQ + ShSmem<HS, MT>::kQ);
-  __nv_bfloat16* const nv = nk + HS;
-  const __nv_bfloat16* const grp = p.qkv + ((int64_t)b * p.n_groups + gi) * (p.per + 2) * HS;
-  const int64_t trow = table_row(p, b, pos);
-  const int heads = min(16, p.per - ht * 16);
-  for (int i = tid; i < 16 * HS; i += kShThreads) {
-    const int r = i / HS, d = i % HS;
-    *reinterpret_cast<__nv_bfloat16*>(sQ + sw<HS>(r, d >> 3) + (d & 7) * 2) = r < heads ? turned(p, grp + (int64_t)(ht * 16 + r) * HS, d, trow) : __float2bfloat16_rn(0.f);
-  }
-  if (fresh && tid < HS) {
-    const __nv_bfloat16 k = turned(p, grp + (int64_t)p.per * HS, tid, trow), v = grp[(int64_t)(p.per + 1) * HS + tid];
-    nk[tid] = k;
-    nv[tid] = v;
-    if (ht == 0) {   // (the other tiles of heads take the row from their own shared memory)
-      p.kc[(int64_t)b * p.kc_b + (int64_t)gi * p.kc_g + (int64_t)mine * HS + tid] = k;
-      p.vc[(int64_t)b * p.vc_b + (int64_t)gi * p.vc_g + (int64_t)mine * HS + tid] = v;
-    }
-  }
-  __syncthreads();
-  attend<HS, 1>(p, sh_smem, sQ, p.kc + (int64_t)b * p.kc_b + (int64_t)gi * p.kc_g, p.vc + (int64_t)b * p.vc_b + (int64_t)gi * p.vc_g, kbeg, kend, fresh ? mine : -1, nk, nv,
-                reinterpret_cast<float (*)[16]>(s_m), reinterpret_cast<float (*)[16]>(s_l), [&](int r) -> int64_t {
-                  return r < heads ? ((int64_t)b * p.n_head + gi * p.per + ht * 16 + r) * splits + p.prefix_splits + split : (int64_t)-1;
-                });
-}
-
-// a (row, head) per HS / 4 threads
-template <int HS>
-__global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParams p) {
-  griddep_launch();
-  griddep_wait();
-  constexpr int T = HS / 4;
-  const int64_t rh = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T;
-  if (rh >= (int64_t)p.batch * p.n_head) return;
-  const int d = (threadIdx.x % T) * 4;
-  __nv_bfloat16* const out = p.out + rh * HS + d;
-  if (row_pos(p, (int)(rh / p.n_head)) < 0) {
-    *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
-    return;
-  }
-  const int splits = p.prefix_splits + p.own_splits;
-  const float2* const ml = p.ml + rh * splits;
-  float top = -INFINITY;
-  for (int i = 0; i < splits; ++i) top = fmaxf(top, __ldcg(ml + i).x);
-  const float org = top == -INFINITY ? 0.f : top;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  for (int i = 0; i < splits; ++i) {
-    const float2 e = __ldcg(ml + i);
-    if (e.x == -INFINITY && e.y == 0.f) continue;
-    const float c = ex2(e.x - org);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.acc + (rh * splits + i) * HS + d));
-    a.x += v.x * c; a.y += v.y * c; a.z += v.z * c; a.w += v.w * c;
-    sum += e.y * c;
-  }
-  const float inv = 1.f / sum;
-  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
-}
-
-struct SharedPlan { int mt, tiles, prefix_splits, own_splits, head_tiles; };
-
-SharedPlan shared_plan(int batch, int n_groups, int per, int prefix_rows, int own_rows) {
-  SharedPlan s;
-  const int rows = batch * per, fill = 2 * sm_count();
-  s.mt = rows > 16 ? 2 : 1;
-  s.tiles = (rows + 16 * s.mt - 1) / (16 * s.mt);
-  s.head_tiles = (per + 15) / 16;
-  auto ranges = [&](int units, int keys) {
-    const int want = (fill + units - 1) / units, most = keys / 256;
-    const int n = want < most ? want : most;
-    return n < 1 ? 1 : (n > 64 ? 64 : n);
   };
-  s.prefix_splits = prefix_rows > 0 ? ranges(s.tiles * n_groups, prefix_rows) : 0;
-  s.own_splits = ranges(batch * n_groups * s.head_tiles, own_rows);
+  clear();
+  int unit = 0;                                            // of the current tile's keys
+  for (;;) {
+    const uint32_t kb = ring + unit * C::kUnit;
+    unit = unit == kShUnits - 1 ? 0 : unit + 1;
+    const uint32_t vb = ring + unit * C::kUnit;
+    unit = unit == kShUnits - 1 ? 0 : unit + 1;
+    const bool more = cur.index + 1 < end;
+    pf_wait<2>();
+    __syncwarp();
+    auto values = [&]() {
+      __syncwarp();                                        // the keys have been read: the values of the next tile take their place
+      if (more) load(kb, coming.v, coming.valid);
+      pf_commit();
+      pf_wait<2>();
+      __syncwarp();
+      return vb;
+    };
+    if (MT == 1 || cur.own) attend_tile<HS, MT, 1>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
+    else attend_tile<HS, MT, MT>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
+    __syncwarp();                                          // the values have been read: the keys of the tile after the next take their place
+    const bool ends = cur.left == 0 || !more;
+    Tile was = cur;
+    cur = coming;
+    qb = next_qb;
+    if (cur.index + 1 < end) {
+      walk.next(coming);
+      load(vb, coming.k, coming.valid);
+      if (cur.left == 0) load_queries(sq + (next_qb = qb ^ 1) * C::kQ, coming);
+    }
+    pf_commit();
+    if (ends) {
+      // ---- the item, or this worker's part of it, ends ----
+      const int64_t slot = walk.item(was) + w;
+      const int rows = was.own ? min(16, p.per) : 16 * MT, valid = walk.queries(was);
+      float* const acc = (was.own ? p.own_acc : p.pre_acc) + slot * rows * HS;
+      float2* const ml = (was.own ? p.own_ml : p.pre_ml) + slot * rows;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float l = a.l[t][h];
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          const int r = t * 16 + h * 8 + g;
+          if (r < valid) {
+#pragma unroll
+            for (int i = 0; i < HS / 8; ++i) __stcg(reinterpret_cast<float2*>(acc + r * HS + i * 8 + 2 * tq), make_float2(a.o[t][i][2 * h], a.o[t][i][2 * h + 1]));
+            if (tq == 0) __stcg(ml + r, make_float2(a.m[t][h], l));
+          }
+        }
+      if (!more) break;
+      clear();
+    }
+  }
+  pf_wait<0>();
+}
+
+// A head's results joined: `ways` warps a head, HS / 32 numbers a lane.
+template <int HS, int MT>
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParams p) {
+  constexpr int V = HS / 32;
+  __shared__ int s_sums[257], s_warp[8];
+  __shared__ float s_acc[8][HS];
+  __shared__ float2 s_ml[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = 8 / p.ways, blocks = (p.n_head + heads - 1) / heads;
+  const int b = blockIdx.x / blocks, h = (blockIdx.x - b * blocks) * heads + warp / p.ways, way = warp % p.ways;
+  griddep_launch();
+  const int plen = prefix_len(p);
+  const int mine = own_index(p, row_pos(p, b), plen);
+  if (mine < 0) {
+    griddep_wait();
+    if (h < p.n_head && way == 0)
+#pragma unroll
+      for (int i = 0; i < V; ++i) p.out[((int64_t)b * p.n_head + h) * HS + lane * V + i] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  const Split s = make_split<256>(p, plen, s_sums, s_warp);
+  float top = -INFINITY, sum = 0.f, a[V] = {};
+  if (h < p.n_head) {
+    const int gi = h / p.per, hh = h - gi * p.per, run = (p.batch + 255) / 256, tiles = mine / kShTile + 1;
+    // own: the item's tiles, the workers that had them, their slots
+    int before = s_sums[b / run];
+    for (int i = b / run * run; i < b; ++i) before += own_tiles(p, i, plen);
+    const int own_first = (before * p.n_groups + gi * tiles) * p.head_tiles + hh / 16 * tiles;
+    const int own_rows = min(16, p.per);
+    const int ow0 = worker_of(own_first, s), own_n = worker_of(own_first + tiles - 1, s) - ow0 + 1;
+    const int64_t own_at = ((((int64_t)b * p.n_groups + gi) * p.head_tiles + hh / 16) + ow0) * own_rows + hh % 16;
+    // prefix
+    const int row = b * p.per + hh, item = gi * p.row_tiles + row / (16 * MT);
+    int pre_n = 0;
+    int64_t pre_at = 0;
+    if (s.prefix > 0) {
+      const int t0 = s.own + item * s.prefix;
+      const int pw0 = worker_of(t0, s);
+      pre_n = worker_of(t0 + s.prefix - 1, s) - pw0 + 1;
+      pre_at = ((int64_t)item + pw0) * (16 * MT) + row % (16 * MT);
+    }
+    const int n = own_n + pre_n;
+    griddep_wait();
+    for (int i0 = way; i0 < n; i0 += 4 * p.ways) {
+      float2 e[4];
+      float v[4][V];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * p.ways;
+        e[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[u][j] = 0.f;
+        if (i < n) {
+          const bool own = i < own_n;
+          const int64_t at = own ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * (16 * MT);
+          e[u] = __ldcg((own ? p.own_ml : p.pre_ml) + at);
+          const float* const src = (own ? p.own_acc : p.pre_acc) + at * HS + lane * V;
+          if constexpr (V == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+            v[u][0] = x.x; v[u][1] = x.y; v[u][V - 2] = x.z; v[u][V - 1] = x.w;
+          } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+            v[u][0] = x.x; v[u][1] = x.y;
+          }
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) now = fmaxf(now, e[u].x);
+      const float org = now == -INFINITY ? 0.f : now, shrink = ex2(top - org);
+      top = now;
+      sum *= shrink;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] *= shrink;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float c = ex2(e[u].x - org);   // (a range that saw nothing: 0 times 0)
+        sum += e[u].y * c;
+#pragma unroll
+        for (int j = 0; j < V; ++j) a[j] += v[u][j] * c;
+      }
+    }
+  }
+  if (h >= p.n_head) griddep_wait();
+  if (p.ways > 1) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) s_acc[warp][lane * V + j] = a[j];
+    if (lane == 0) s_ml[warp] = make_float2(top, sum);
+    __syncthreads();
+    if (way != 0) return;
+    float now = top;
+    for (int u = 1; u < p.ways; ++u) now = fmaxf(now, s_ml[warp + u].x);
+    const float org = now == -INFINITY ? 0.f : now, c0 = ex2(top - org);
+    sum *= c0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] *= c0;
+    for (int u = 1; u < p.ways; ++u) {
+      const float c = ex2(s_ml[warp + u].x - org);
+      sum += s_ml[warp + u].y * c;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] += s_acc[warp + u][lane * V + j] * c;
+    }
+  }
+  if (h >= p.n_head) return;
+  const float inv = 1.f / sum;
+  __nv_bfloat16* const out = p.out + ((int64_t)b * p.n_head + h) * HS + lane * V;
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[V - 2] * inv, a[V - 1] * inv));
+  else *reinterpret_cast<uint32_t*>(out) = pack_bf16(a[0] * inv, a[1] * inv);
+}
+
+struct SharedPlan {
+  int mt, head_tiles, row_tiles, ctas, workers, ways;
+  int64_t own_slots, pre_slots;   // rows
+  int64_t tiles, q;               // tiles at most; numbers of the turned queries
+  size_t bytes;
+};
+
+SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows, int own_rows) {
+  SharedPlan s;
+  const int64_t rows = (int64_t)batch * per;
+  s.mt = prefix_rows > 0 && rows > 16 ? 2 : 1;
+  s.head_tiles = (per + 15) / 16;
+  s.row_tiles = prefix_rows > 0 ? (int)((rows + 16 * s.mt - 1) / (16 * s.mt)) : 0;
+  const int64_t own_items = (int64_t)batch * n_groups * s.head_tiles, pre_items = (int64_t)n_groups * s.row_tiles;
+  const int64_t tiles = own_items * ((own_rows + kShTile - 1) / kShTile) + pre_items * ((prefix_rows + kShTile - 1) / kShTile);
+  const int warps = hs == 64 ? (s.mt == 2 ? ShSmem<64, 2>::kWarps : ShSmem<64, 1>::kWarps) : (s.mt == 2 ? ShSmem<128, 2>::kWarps : ShSmem<128, 1>::kWarps);
+  s.tiles = tiles;
+  s.ctas = sm_count() < tiles ? sm_count() : (int)tiles;
+  s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
+  s.own_slots = (own_items + s.workers) * (per < 16 ? per : 16);
+  s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 16 * s.mt : 0;
+  s.q = rows * n_groups * hs;
+  s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2;
+  // results of a head: about those of a prefix item and of an own one
+  const int64_t results = 2 + (int64_t)s.workers / (pre_items > 0 ? pre_items : own_items);
+  s.ways = results > 32 ? 8 : results > 16 ? 4 : results > 8 ? 2 : 1;
   return s;
 }
 
 template <int HS, int MT>
-cudaError_t launch_shared(const SharedParams& p, cudaStream_t st) {
+cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
   constexpr int smem = ShSmem<HS, MT>::kBytes;
   static PerDeviceOnce once;
   if (once.need()) {
@@ -363,12 +674,13 @@ cudaError_t launch_shared(const SharedParams& p, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     once.done();
   }
-  const int64_t units = (int64_t)p.batch * p.n_groups * p.head_tiles * p.own_splits + (int64_t)p.n_groups * p.tiles * p.prefix_splits;
-  const cudaError_t e = launch(attn_shared_kernel<HS, MT>, dim3((unsigned)units), dim3(kShThreads), (size_t)smem, st, p);
+  const int64_t warps = (int64_t)p.batch * p.n_groups * (p.per + 2);
+  cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
-  const int64_t heads = (int64_t)p.batch * p.n_head;
-  constexpr int each = 256 / (HS / 4);
-  return launch(attn_shared_join_kernel<HS>, dim3((unsigned)((heads + each - 1) / each)), dim3(256), 0, st, p);
+  e = launch(attn_shared_kernel<HS, MT>, dim3((unsigned)s.ctas), dim3(ShSmem<HS, MT>::kWarps * 32), (size_t)smem, st, p);
+  if (e != cudaSuccess) return e;
+  const int heads = 8 / s.ways;
+  return launch(attn_shared_join_kernel<HS, MT>, dim3((unsigned)(p.batch * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -380,8 +692,8 @@ extern "C" {
 
 size_t b200_attn_decode_shared_workspace_bytes(int batch, int n_head, int n_groups, int head_size, int prefix_rows, int own_rows) {
   if (batch <= 0 || n_groups <= 0 || n_head <= 0 || n_head % n_groups || prefix_rows < 0 || own_rows <= 0 || (head_size != 64 && head_size != 128)) return 0;
-  const SharedPlan s = shared_plan(batch, n_groups, n_head / n_groups, prefix_rows, own_rows);
-  return (size_t)batch * n_head * (s.prefix_splits + s.own_splits) * (head_size + 2) * sizeof(float);
+  const SharedPlan s = shared_plan(batch, n_groups, n_head / n_groups, head_size, prefix_rows, own_rows);
+  return s.bytes;
 }
 
 int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t stream) {
@@ -400,9 +712,9 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   const uintptr_t at = (uintptr_t)a->k_cache | (uintptr_t)a->v_cache | (uintptr_t)a->k_prefix | (uintptr_t)a->v_prefix | (uintptr_t)a->workspace;
   const int64_t strides = a->k_batch_stride | a->k_group_stride | a->v_batch_stride | a->v_group_stride | a->k_prefix_stride | a->v_prefix_stride;
   B200_CHECK_ARG((at & 15) == 0 && (strides & 7) == 0 && ((uintptr_t)a->out & 7) == 0, "b200_attn_decode_shared: caches and prefix must lie on 16-byte boundaries");
-  const SharedPlan s = shared_plan(a->batch, a->n_groups, a->n_head / a->n_groups, a->prefix_rows, a->own_rows);
-  const size_t slots = (size_t)a->batch * a->n_head * (s.prefix_splits + s.own_splits);
-  B200_CHECK_ARG(a->workspace_bytes >= slots * (a->head_size + 2) * sizeof(float), "b200_attn_decode_shared: workspace too small");
+  const SharedPlan s = shared_plan(a->batch, a->n_groups, a->n_head / a->n_groups, a->head_size, a->prefix_rows, a->own_rows);
+  B200_CHECK_ARG(s.tiles < (1 << 30), "b200_attn_decode_shared: caches of too many keys");
+  B200_CHECK_ARG(a->workspace_bytes >= s.bytes, "b200_attn_decode_shared: workspace too small");
   SharedParams p = {};
   p.qkv = (const __nv_bfloat16*)a->qkv;
   p.cos = a->cos; p.sin = a->sin; p.table_bf16 = a->table_dtype == B200_BF16; p.table_rows = a->table_rows; p.table_presel = a->table_preselected; p.rope_n = a->rope_n_elem;
@@ -413,13 +725,19 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   p.kp = (const __nv_bfloat16*)a->k_prefix; p.vp = (const __nv_bfloat16*)a->v_prefix; p.kp_g = a->k_prefix_stride; p.vp_g = a->v_prefix_stride;
   p.out = (__nv_bfloat16*)a->out;
   p.batch = a->batch; p.n_head = a->n_head; p.n_groups = a->n_groups; p.per = a->n_head / a->n_groups; p.own_rows = a->own_rows; p.prefix_rows = a->prefix_rows;
-  p.tiles = s.tiles; p.prefix_splits = s.prefix_splits; p.own_splits = s.own_splits; p.head_tiles = s.head_tiles;
-  p.acc = (float*)a->workspace;
-  p.ml = (float2*)(p.acc + slots * a->head_size);
+  p.head_tiles = s.head_tiles; p.row_tiles = s.row_tiles; p.workers = s.workers; p.sms = sm_count(); p.ways = s.ways;
+  const int n = a->rope_n_elem, part = a->head_size / 32;
+  p.wide = ((uintptr_t)a->qkv & 15) == 0 && n % (2 * part) == 0 && (a->table_dtype == B200_BF16 || (((uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0);
+  // (every part begins on a 16-byte boundary but the last, of pairs of floats)
+  p.q = (__nv_bfloat16*)a->workspace;
+  p.own_acc = (float*)(p.q + s.q);
+  p.pre_acc = p.own_acc + s.own_slots * a->head_size;
+  p.own_ml = (float2*)(p.pre_acc + s.pre_slots * a->head_size);
+  p.pre_ml = p.own_ml + s.own_slots;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (a->head_size == 128) B200_CUDA((s.mt == 2 ? launch_shared<128, 2>(p, st) : launch_shared<128, 1>(p, st)));
-  else B200_CUDA((s.mt == 2 ? launch_shared<64, 2>(p, st) : launch_shared<64, 1>(p, st)));
+  if (a->head_size == 128) B200_CUDA((s.mt == 2 ? launch_shared<128, 2>(p, s, st) : launch_shared<128, 1>(p, s, st)));
+  else B200_CUDA((s.mt == 2 ? launch_shared<64, 2>(p, s, st) : launch_shared<64, 1>(p, s, st)));
   return B200_OK;
 }
 
