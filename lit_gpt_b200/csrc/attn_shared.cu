@@ -11,48 +11,23 @@
 // All tiles, of the prefix and of all rows' own keys, are one list that is cut evenly over the warps of all SMs, so that neither few rows over a long prefix nor many
 // rows of unequal lengths leave SMs without work.  A warp keeps a ring of units of 32 keys or values, two of them on their way, and the queries of its next item behind them.
 // S = Q K^T and O += P V on mma.sync.m16n8k16.  P enters as two bf16 numbers, its leading bits and the rest, so that its rounding does not add to the result's own (with the
-// nearest bf16 number alone the error against 64 bits is a fifth larger than that of the final rounding).  The rest is kept above zero, so that an infinite value
-// times it is infinite and not NaN.
+// nearest bf16 number alone the error against 64 bits is a fifth larger than that of the final rounding).  The rest is taken of the number above the weight: it is
+// not zero, and an infinite value times it is infinite and not NaN.
 #include <math.h>
 
 #include "attn_body.cuh"
+#include "attn_shared.cuh"
 #include "mma_tile.cuh"
+#include "tc05.cuh"
 
 namespace b200 {
 
 namespace {
 
 constexpr int kShTile = 32;                 // keys of a tile
+constexpr float kAbove = 1.00000012f;       // 1 + 2^-23: a weight's second number is never zero
 constexpr int kShUnits = 3;                 // a warp's ring: units of 32 keys or 32 values
 
-struct SharedParams {
-  const __nv_bfloat16* qkv;
-  const void* cos; const void* sin;
-  int table_bf16, table_rows, table_presel, rope_n, wide;   // wide: rows of heads and tables allow accesses of HS / 32 numbers
-  const void* pos; int pos64, pos_each;      // pos_each: one position per row
-  const void* plen; int plen64;              // null: prefix_rows
-  __nv_bfloat16* kc; __nv_bfloat16* vc; int64_t kc_b, kc_g, vc_b, vc_g;
-  const __nv_bfloat16* kp; const __nv_bfloat16* vp; int64_t kp_g, vp_g;
-  __nv_bfloat16* out;
-  int batch, n_head, n_groups, per, own_rows, prefix_rows;
-  int head_tiles, row_tiles;                 // tiles of 16 heads of a row's group; tiles of a group's query rows over the prefix
-  __nv_bfloat16* q;                          // the queries, turned: [n_groups][batch * per][HS]
-  int workers, sms;                          // warps that share the tiles, at most
-  float* own_acc; float2* own_ml;            // results of key ranges of own items: slots of min(16, per) rows
-  float* pre_acc; float2* pre_ml;            // of prefix items: slots of 16 * MT rows
-  int ways;                                  // warps that join a head's results
-  float scale_log2;
-};
-
-__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
-  return is64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
-}
-__device__ __forceinline__ int64_t row_pos(const SharedParams& p, int b) { return index_at(p.pos, p.pos64, p.pos_each ? b : 0); }
-__device__ __forceinline__ int prefix_len(const SharedParams& p) {
-  if (!p.plen) return p.prefix_rows;
-  const int64_t n = index_at(p.plen, p.plen64, 0);
-  return (int)(n < 0 ? 0 : (n > p.prefix_rows ? p.prefix_rows : n));
-}
 // index of a row's new key in its own cache; -1: the row takes no part
 __device__ __forceinline__ int own_index(const SharedParams& p, int64_t pos, int plen) {
   if (pos < 0) return -1;
@@ -162,7 +137,7 @@ __device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int
   __syncthreads();
   Split s;
   s.own = sums[THREADS] * p.n_groups * p.head_tiles;
-  s.prefix = (plen + kShTile - 1) / kShTile;
+  s.prefix = p.row_tiles ? (plen + kShTile - 1) / kShTile : 0;
   s.all = s.own + s.prefix * p.n_groups * p.row_tiles;
   // two tiles a worker at least, unless that leaves SMs without one
   s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
@@ -382,7 +357,7 @@ __device__ __forceinline__ void attend_tile(Sums<HS, MT>& a, uint32_t q, uint32_
         a.l[t][h] += x + y;
         const uint32_t w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);   // the leading 16 bits of both
         hi[t][i >> 1][(i & 1) * 2 + h] = w;
-        lo[t][i >> 1][(i & 1) * 2 + h] = pack_bf16(fmaxf(x - bf16lo(w), 1e-36f), fmaxf(y - bf16hi(w), 1e-36f));
+        lo[t][i >> 1][(i & 1) * 2 + h] = pack_bf16(fmaf(x, kAbove, -bf16lo(w)), fmaf(y, kAbove, -bf16hi(w)));
       }
     }
   }
@@ -442,9 +417,10 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
   };
   const int end = first_tile(w + 1, s);
   Tile cur = walk.find(first_tile(w, s), T);
-  // What the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before.
+  // What the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before.  Where the prefix's own kernel ran in between, the
+  // turning kernel ended before that one let this one begin: then the wait, for that kernel, is at the end.
   if (!cur.own) load(ring, cur.k, cur.valid);
-  griddep_wait();
+  if (p.pre_parts == 0) griddep_wait();
   if (cur.own) load(ring, cur.k, cur.valid);
   load_queries(sq, cur);
   pf_commit();
@@ -525,6 +501,7 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
     }
   }
   pf_wait<0>();
+  if (p.pre_parts > 0) griddep_wait();
 }
 
 // A head's results joined: `ways` warps a head, HS / 32 numbers a lane.
@@ -559,9 +536,10 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
     const int64_t own_at = ((((int64_t)b * p.n_groups + gi) * p.head_tiles + hh / 16) + ow0) * own_rows + hh % 16;
     // prefix
     const int row = b * p.per + hh, item = gi * p.row_tiles + row / (16 * MT);
-    int pre_n = 0;
-    int64_t pre_at = 0;
-    if (s.prefix > 0) {
+    int pre_n = p.pre_parts;
+    int64_t pre_at = ((int64_t)gi * p.pre_tiles + (pre_n ? row / p.pre_rows : 0)) * pre_n * p.pre_rows + (pre_n ? row % p.pre_rows : 0);
+    const int pre_step = pre_n ? p.pre_rows : 16 * MT;
+    if (pre_n == 0 && s.prefix > 0) {
       const int t0 = s.own + item * s.prefix;
       const int pw0 = worker_of(t0, s);
       pre_n = worker_of(t0 + s.prefix - 1, s) - pw0 + 1;
@@ -580,8 +558,9 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
         for (int j = 0; j < V; ++j) v[u][j] = 0.f;
         if (i < n) {
           const bool own = i < own_n;
-          const int64_t at = own ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * (16 * MT);
+          const int64_t at = own ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * pre_step;
           e[u] = __ldcg((own ? p.own_ml : p.pre_ml) + at);
+          if (e[u].y == 0.f) continue;   // (a range that saw nothing has no result)
           const float* const src = (own ? p.own_acc : p.pre_acc) + at * HS + lane * V;
           if constexpr (V == 4) {
             const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
@@ -602,7 +581,7 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
       for (int j = 0; j < V; ++j) a[j] *= shrink;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float c = ex2(e[u].x - org);   // (a range that saw nothing: 0 times 0)
+        const float c = ex2(e[u].x - org);
         sum += e[u].y * c;
 #pragma unroll
         for (int j = 0; j < V; ++j) a[j] += v[u][j] * c;
@@ -641,11 +620,26 @@ struct SharedPlan {
   int64_t own_slots, pre_slots;   // rows
   int64_t tiles, q;               // tiles at most; numbers of the turned queries
   size_t bytes;
+  bool tensor, pair;              // the prefix on the tensor memory; 256 query rows a CTA instead of 128
+  int splits;                     // its key ranges
+  int pre_rows, pre_tiles, pre_parts;
 };
 
 SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows, int own_rows) {
   SharedPlan s;
   const int64_t rows = (int64_t)batch * per;
+  s.tensor = prefix_rows > 0 && rows > 32;
+  s.pair = rows > 128;
+  s.splits = s.pre_rows = s.pre_tiles = s.pre_parts = 0;
+  if (s.tensor) {
+    s.pre_rows = s.pair ? 256 : 128;
+    s.pre_tiles = (int)((rows + s.pre_rows - 1) / s.pre_rows);
+    const int64_t items = (int64_t)n_groups * s.pre_tiles, ranges = ((int64_t)prefix_rows + 127) / 128;
+    s.splits = (int)(sm_count() / items < ranges ? sm_count() / items : ranges);
+    if (s.splits < 1) s.splits = 1;
+    s.pre_parts = s.pair ? s.splits : 2 * s.splits;
+    prefix_rows = 0;               // not in the list of tiles
+  }
   s.mt = prefix_rows > 0 && rows > 16 ? 2 : 1;
   s.head_tiles = (per + 15) / 16;
   s.row_tiles = prefix_rows > 0 ? (int)((rows + 16 * s.mt - 1) / (16 * s.mt)) : 0;
@@ -656,11 +650,11 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   s.ctas = sm_count() < tiles ? sm_count() : (int)tiles;
   s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
   s.own_slots = (own_items + s.workers) * (per < 16 ? per : 16);
-  s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 16 * s.mt : 0;
+  s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 16 * s.mt : (int64_t)n_groups * s.pre_tiles * s.pre_parts * s.pre_rows;
   s.q = rows * n_groups * hs;
   s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2;
   // results of a head: about those of a prefix item and of an own one
-  const int64_t results = 2 + (int64_t)s.workers / (pre_items > 0 ? pre_items : own_items);
+  const int64_t results = 2 + s.pre_parts + (int64_t)s.workers / (pre_items > 0 ? pre_items : own_items);
   s.ways = results > 32 ? 8 : results > 16 ? 4 : results > 8 ? 2 : 1;
   return s;
 }
@@ -677,6 +671,7 @@ cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream
   const int64_t warps = (int64_t)p.batch * p.n_groups * (p.per + 2);
   cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
+  if (s.tensor && (e = launch_attn_shared_prefix(p, HS, s.pair, s.splits, st)) != cudaSuccess) return e;
   e = launch(attn_shared_kernel<HS, MT>, dim3((unsigned)s.ctas), dim3(ShSmem<HS, MT>::kWarps * 32), (size_t)smem, st, p);
   if (e != cudaSuccess) return e;
   const int heads = 8 / s.ways;
@@ -715,6 +710,7 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   const SharedPlan s = shared_plan(a->batch, a->n_groups, a->n_head / a->n_groups, a->head_size, a->prefix_rows, a->own_rows);
   B200_CHECK_ARG(s.tiles < (1 << 30), "b200_attn_decode_shared: caches of too many keys");
   B200_CHECK_ARG(a->workspace_bytes >= s.bytes, "b200_attn_decode_shared: workspace too small");
+  if (s.tensor) B200_CHECK_WAITS("b200_attn_decode_shared");
   SharedParams p = {};
   p.qkv = (const __nv_bfloat16*)a->qkv;
   p.cos = a->cos; p.sin = a->sin; p.table_bf16 = a->table_dtype == B200_BF16; p.table_rows = a->table_rows; p.table_presel = a->table_preselected; p.rope_n = a->rope_n_elem;
@@ -726,6 +722,7 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   p.out = (__nv_bfloat16*)a->out;
   p.batch = a->batch; p.n_head = a->n_head; p.n_groups = a->n_groups; p.per = a->n_head / a->n_groups; p.own_rows = a->own_rows; p.prefix_rows = a->prefix_rows;
   p.head_tiles = s.head_tiles; p.row_tiles = s.row_tiles; p.workers = s.workers; p.sms = sm_count(); p.ways = s.ways;
+  p.pre_parts = s.pre_parts; p.pre_rows = s.pre_rows; p.pre_tiles = s.pre_tiles;
   const int n = a->rope_n_elem, part = a->head_size / 32;
   p.wide = ((uintptr_t)a->qkv & 15) == 0 && n % (2 * part) == 0 && (a->table_dtype == B200_BF16 || (((uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0);
   // (every part begins on a 16-byte boundary but the last, of pairs of floats)

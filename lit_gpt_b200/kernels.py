@@ -813,6 +813,8 @@ def attn_decode_shared(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     apart = [tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 2)) for t in (k_cache, v_cache, k_prefix, v_prefix)]
     if any(n > 1 and step < k_cache.shape[2] * head_size for t in apart[:2] for n, step in zip(k_cache.shape, t)):
         raise C.B200Error("attn_decode_shared: the caches of two rows or groups overlap")
+    if n_groups > 1 and min(apart[2][0], apart[3][0]) < k_prefix.shape[1] * head_size:
+        raise C.B200Error("attn_decode_shared: the prefixes of two groups overlap")
     B, _, S, _ = k_cache.shape
     if qkv.numel() != B * (n_head + 2 * n_groups) * head_size:
         raise C.B200Error("attn_decode_shared: qkv does not hold exactly one token per row of the caches")
