@@ -119,6 +119,18 @@ __device__ __forceinline__ int worker_of(int tile, const Split& s) {
 }
 __device__ __forceinline__ int first_tile(int w, const Split& s) { return w * s.each + min(w, s.more); }
 
+__device__ __forceinline__ Split split_of(const SharedParams& p, int plen, int own_tiles_of_all) {
+  Split s;
+  s.own = own_tiles_of_all * p.n_groups * p.head_tiles;
+  s.prefix = p.row_tiles ? (plen + kShTile - 1) / kShTile : 0;
+  s.all = s.own + s.prefix * p.n_groups * p.row_tiles;
+  // two tiles a worker at least, unless that leaves SMs without one
+  s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
+  s.each = s.workers ? s.all / s.workers : 0;
+  s.more = s.all - s.each * s.workers;
+  return s;
+}
+
 // Rows are summed in runs of one per thread: sums[t] = own tiles (of one group and tile of heads) of the rows before run t; sums[THREADS] of all.
 template <int THREADS>
 __device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int* sums, int* s_warp) {
@@ -135,15 +147,7 @@ __device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int
   sums[tid] = before;
   if (tid == THREADS - 1) sums[THREADS] = before + mine;
   __syncthreads();
-  Split s;
-  s.own = sums[THREADS] * p.n_groups * p.head_tiles;
-  s.prefix = p.row_tiles ? (plen + kShTile - 1) / kShTile : 0;
-  s.all = s.own + s.prefix * p.n_groups * p.row_tiles;
-  // two tiles a worker at least, unless that leaves SMs without one
-  s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
-  s.each = s.workers ? s.all / s.workers : 0;
-  s.more = s.all - s.each * s.workers;
-  return s;
+  return split_of(p, plen, sums[THREADS]);
 }
 
 // A warp's shared memory: a ring of units, the queries of two items.  One CTA an SM.
@@ -161,6 +165,19 @@ __global__ void __launch_bounds__(256) attn_shared_turn_kernel(const SharedParam
   constexpr int V = HS / 32;
   griddep_wait();     // (before the launch of what follows: the kernels behind read positions, lengths and the prefix ahead of their own wait)
   griddep_launch();
+  if (blockIdx.x == gridDim.x - 1) {   // own tiles (of one group and tile of heads) of the rows before each
+    __shared__ int s_sums[257], s_warp[8];
+    const int plen = prefix_len(p);
+    make_split<256>(p, plen, s_sums, s_warp);
+    const int run = (p.batch + 255) / 256;
+    int sum = s_sums[threadIdx.x];
+    for (int b = threadIdx.x * run; b < min(p.batch, ((int)threadIdx.x + 1) * run); ++b) {
+      p.before[b] = sum;
+      sum += own_tiles(p, b, plen);
+    }
+    if (threadIdx.x == 0) p.before[p.batch] = s_sums[256];
+    return;
+  }
   const int lane = threadIdx.x & 31, heads = p.n_groups * (p.per + 2);
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int b = (int)(at / heads), i = (int)(at - (int64_t)b * heads), gi = i / (p.per + 2), h = i - gi * (p.per + 2);
@@ -508,7 +525,6 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
 template <int HS, int MT>
 __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParams p) {
   constexpr int V = HS / 32;
-  __shared__ int s_sums[257], s_warp[8];
   __shared__ float s_acc[8][HS];
   __shared__ float2 s_ml[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = 8 / p.ways, blocks = (p.n_head + heads - 1) / heads;
@@ -516,20 +532,19 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
   griddep_launch();
   const int plen = prefix_len(p);
   const int mine = own_index(p, row_pos(p, b), plen);
+  griddep_wait();
   if (mine < 0) {
-    griddep_wait();
     if (h < p.n_head && way == 0)
 #pragma unroll
       for (int i = 0; i < V; ++i) p.out[((int64_t)b * p.n_head + h) * HS + lane * V + i] = __float2bfloat16_rn(0.f);
     return;
   }
-  const Split s = make_split<256>(p, plen, s_sums, s_warp);
+  const int before = p.before[b];
+  const Split s = split_of(p, plen, p.before[p.batch]);
   float top = -INFINITY, sum = 0.f, a[V] = {};
   if (h < p.n_head) {
-    const int gi = h / p.per, hh = h - gi * p.per, run = (p.batch + 255) / 256, tiles = mine / kShTile + 1;
+    const int gi = h / p.per, hh = h - gi * p.per, tiles = mine / kShTile + 1;
     // own: the item's tiles, the workers that had them, their slots
-    int before = s_sums[b / run];
-    for (int i = b / run * run; i < b; ++i) before += own_tiles(p, i, plen);
     const int own_first = (before * p.n_groups + gi * tiles) * p.head_tiles + hh / 16 * tiles;
     const int own_rows = min(16, p.per);
     const int ow0 = worker_of(own_first, s), own_n = worker_of(own_first + tiles - 1, s) - ow0 + 1;
@@ -546,7 +561,6 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
       pre_at = ((int64_t)item + pw0) * (16 * MT) + row % (16 * MT);
     }
     const int n = own_n + pre_n;
-    griddep_wait();
     for (int i0 = way; i0 < n; i0 += 4 * p.ways) {
       float2 e[4];
       float v[4][V];
@@ -588,7 +602,6 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
       }
     }
   }
-  if (h >= p.n_head) griddep_wait();
   if (p.ways > 1) {
 #pragma unroll
     for (int j = 0; j < V; ++j) s_acc[warp][lane * V + j] = a[j];
@@ -652,10 +665,10 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   s.own_slots = (own_items + s.workers) * (per < 16 ? per : 16);
   s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 16 * s.mt : (int64_t)n_groups * s.pre_tiles * s.pre_parts * s.pre_rows;
   s.q = rows * n_groups * hs;
-  s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2;
+  s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)(batch + 1) * sizeof(int);
   // results of a head: about those of a prefix item and of an own one
   const int64_t results = 2 + s.pre_parts + (int64_t)s.workers / (pre_items > 0 ? pre_items : own_items);
-  s.ways = results > 32 ? 8 : results > 16 ? 4 : results > 8 ? 2 : 1;
+  s.ways = results > 16 ? 8 : results > 8 ? 4 : results > 4 ? 2 : 1;   // four results a warp in one round
   return s;
 }
 
@@ -669,7 +682,7 @@ cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream
     once.done();
   }
   const int64_t warps = (int64_t)p.batch * p.n_groups * (p.per + 2);
-  cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
+  cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8 + 1)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
   if (s.tensor && (e = launch_attn_shared_prefix(p, HS, s.pair, s.splits, st)) != cudaSuccess) return e;
   e = launch(attn_shared_kernel<HS, MT>, dim3((unsigned)s.ctas), dim3(ShSmem<HS, MT>::kWarps * 32), (size_t)smem, st, p);
@@ -725,12 +738,13 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   p.pre_parts = s.pre_parts; p.pre_rows = s.pre_rows; p.pre_tiles = s.pre_tiles;
   const int n = a->rope_n_elem, part = a->head_size / 32;
   p.wide = ((uintptr_t)a->qkv & 15) == 0 && n % (2 * part) == 0 && (a->table_dtype == B200_BF16 || (((uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0);
-  // (every part begins on a 16-byte boundary but the last, of pairs of floats)
+  // (every part of wide accesses begins on a 16-byte boundary: they come first)
   p.q = (__nv_bfloat16*)a->workspace;
   p.own_acc = (float*)(p.q + s.q);
   p.pre_acc = p.own_acc + s.own_slots * a->head_size;
   p.own_ml = (float2*)(p.pre_acc + s.pre_slots * a->head_size);
   p.pre_ml = p.own_ml + s.own_slots;
+  p.before = (int*)(p.pre_ml + s.pre_slots);
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
   const cudaStream_t st = (cudaStream_t)stream;
   if (a->head_size == 128) B200_CUDA((s.mt == 2 ? launch_shared<128, 2>(p, s, st) : launch_shared<128, 1>(p, s, st)));

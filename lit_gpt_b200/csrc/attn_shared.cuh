@@ -19,6 +19,7 @@ struct SharedParams {
   int workers, sms;                          // warps that share the tiles, at most
   float* own_acc; float2* own_ml;            // results of key ranges of own items: slots of min(16, per) rows
   float* pre_acc; float2* pre_ml;            // of prefix items: slots of 16 * MT rows
+  int* before;                               // [batch + 1]: tiles of the rows' own keys, of one group and tile of heads, before each row
   int ways;                                  // warps that join a head's results
   // On the tensor memory (attn_shared_tc05.cu) prefix items are 128 or 256 query rows of a group, with `pre_parts` results each, in slots of `pre_rows` rows, item after item;
   // row_tiles is 0 then.  pre_parts 0: the prefix is in the list of tiles.

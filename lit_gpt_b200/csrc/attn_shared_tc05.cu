@@ -4,8 +4,9 @@
 // One CTA = 128 or 256 query rows of a group (rows of the batch times heads of the group) against a range of the prefix's keys, in tiles of 128 keys.  Two streams of products
 // and softmax, each with its scores and its output in tensor memory, fill each other's gaps: with 256 rows the halves of the rows, with 128 the even and the odd key tiles,
 // whose results are joined as those of two ranges.
-//   * warps 0-3 and 4-7: a stream's softmax, a row per thread: 128 scores are read into registers, the weights go back over them as two bf16 numbers, the leading bits and
-//     the rest (attn_shared.cu says why).  A row's maximum moves, and its output shrinks, only when the maximum grew by 2^8: with the rest a weight of 256 is as exact as one of 1.
+//   * warps 0-3 and 4-7: a stream's softmax, a row per thread: scores are read for their maximum and, 32 at a time, for the weights, which go back over them as two bf16
+//     numbers, the leading bits and the rest (attn_shared.cu says why).  In loops of 32, which read the scores twice: unrolled over a tile the code was 15 KB, and
+//     a launch spent 10000 clocks, as long as three tiles, on fetching it once.  A row's maximum moves, and its output shrinks, only when the maximum grew by 2^8: with the rest a weight of 256 is as exact as one of 1.
 //   * warp 8: S = Q K^T (operands in shared memory) and O += P V (P from tensor memory, V as it lies), 128 x 128 x 16 each
 //   * warps 9 and 10 bring keys and values, two stages each: whole tiles by TMA, the prefix's last one row by row, zeros behind it.
 // Bound: the prefix's bytes with up to 128 rows (a tile of 128 keys, 64 KB, is 2800 clocks of an SM's share of the memory's rate, its products 1536), with 256 rows the
@@ -39,7 +40,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int splits, unsigned* err) {
   using C = SpTile<HS>;
   extern __shared__ __align__(1024) uint8_t sp_smem[];
-  __shared__ __align__(8) uint64_t s_bars[16];
+  __shared__ __align__(8) uint64_t s_bars[18];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, tile_of_rows = item % p.pre_tiles, gi = item / p.pre_tiles;
@@ -48,7 +49,7 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
   const uint32_t sq_ = smem, sk_ = smem + 2 * C::kBytes, sv_ = smem + 4 * C::kBytes;
   const uint32_t bars = tc::smem_u32(s_bars);
   const uint32_t k_full = bars, v_full = bars + 16, k_empty = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 80, o_done = bars + 96, q_full = bars + 112,
-                 idle = bars + 120;   // idle: products that gave up
+                 idle = bars + 120, p_half = bars + 128;   // idle: products that gave up
   const int plen = prefix_len(p), tiles = (plen + 127) / 128, each = (tiles + splits - 1) / splits;
   const int first = min(tiles, split * each), n = min(tiles, first + each) - first;   // this CTA's key tiles
   if (tid == 0) {
@@ -58,6 +59,7 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
       tc::mbar_init(k_empty + 8 * i, 1);
       tc::mbar_init(v_empty + 8 * i, 1);
       tc::mbar_init(s_full + 8 * i, 1);
+      tc::mbar_init(p_half + 8 * i, 4);
       tc::mbar_init(p_full + 8 * i, 4);
       tc::mbar_init(o_done + 8 * i, 1);
     }
@@ -65,13 +67,19 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
     tc::mbar_init(idle, 1);
     tc::mbar_init_fence();
   }
-  griddep_wait();
-  griddep_launch();   // (behind the wait: attn_shared_kernel, which comes next, counts on it)
-  if (warp == 8) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
-  tc::fence_before();
   __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = s_tmem;
+  // The prefix was there before the turning kernel: its copies begin ahead of the wait for that one.  Only behind its wait a CTA lets attn_shared_kernel begin, which
+  // counts on the turning kernel's end.
+  uint32_t tmem = 0;
+  if (warp < 9) {
+    griddep_wait();
+    griddep_launch();
+    if (warp == 8) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+    tc::fence_before();
+    asm volatile("bar.sync 1, 288;" ::: "memory");
+    tc::fence_after();
+    tmem = s_tmem;
+  }
   bool ok = true;
 
   if (warp >= 9) {
@@ -79,8 +87,10 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
     const bool keys = warp == 9;
     const __nv_bfloat16* const src = keys ? p.kp + (int64_t)gi * p.kp_g : p.vp + (int64_t)gi * p.vp_g;
     const uint32_t dst = keys ? sk_ : sv_, full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
+    if (lane == 0) tc::prefetch_map(keys ? &map_k : &map_v);
     int j = 0;
     for (; j < n; ++j) {
+      if (j == 2) { griddep_wait(); griddep_launch(); }
       const int s = j & 1, row = (first + j) * 128;
       ok = __all_sync(0xffffffffu, tc::mbar_wait(empty + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u));
       if (!ok) break;
@@ -98,6 +108,8 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
         if (lane == 0) tc::mbar_arrive(full + 8 * s);
       }
     }
+    griddep_wait();
+    griddep_launch();
     // no copy may land after the CTA has left
     for (int i = max(j - 2, 0); i < j; ++i) ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * (i & 1), (uint32_t)(i >> 1) & 1u)) && ok;
   } else if (warp == 8) {
@@ -113,12 +125,14 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
         }
         tc::commit(s_full + 8 * t);
       };
-      auto outputs = [&](int t, int s, bool begins) {      // O of stream t with the values of stage s
+      auto outputs = [&](int t, int s, int half, bool begins) {   // O of stream t with half of the values of stage s
         const uint32_t dv = v_low + s * (C::kBytes >> 4), d = tmem + C::kO + t * HS, pp = tmem + C::kS + t * 128;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mma_ts(d, pp + e * 8, tc::desc_of(dv + 128 * e, tc::kDescSw128High), C::kIdescO, !(begins && e == 0));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mma_ts(d, pp + 64 + e * 8, tc::desc_of(dv + 128 * e, tc::kDescSw128High), C::kIdescO, 1u);
+        for (int e = 4 * half; e < 4 * half + 4; ++e) {          // 16 keys: their leading bits, their rests
+          const uint64_t v = tc::desc_of(dv + 128 * e, tc::kDescSw128High);
+          mma_ts(d, pp + (e >> 1) * 32 + (e & 1) * 8, v, C::kIdescO, !(begins && e == 0));
+          mma_ts(d, pp + (e >> 1) * 32 + 16 + (e & 1) * 8, v, C::kIdescO, 1u);
+        }
       };
       auto arrived = [&](uint32_t bar, int j) { return tc::mbar_wait_here(bar + 8 * (j & 1), (uint32_t)(j >> 1) & 1u); };   // the copies of tile j
       ok = tc::mbar_wait_here(q_full, 0) && arrived(k_full, 0);
@@ -144,10 +158,14 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
 #pragma unroll
         for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
           const int t = PAIR ? u : s;
-          ok = ok && tc::mbar_wait_here(p_full + 8 * t, (uint32_t)(PAIR ? j : j >> 1) & 1u);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            ok = ok && tc::mbar_wait_here((half ? p_full : p_half) + 8 * t, (uint32_t)(PAIR ? j : j >> 1) & 1u);
+            if (!ok) break;
+            tc::fence_after();
+            outputs(t, s, half, PAIR ? j == 0 : j < 2);
+          }
           if (!ok) break;
-          tc::fence_after();
-          outputs(t, s, PAIR ? j == 0 : j < 2);
           if (next < n) scores(t, next & 1);
           else tc::commit(o_done + 8 * t);
         }
@@ -180,25 +198,34 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
       ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * t, steps & 1u));
       if (!ok) break;
       tc::fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tc::ld32(s[i], ts + 32 * i);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tc::wait_ld(s[i]);
       const int valid = plen - (first + j) * 128;
-      if (valid < 128) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
+      auto mask = [&](uint32_t (&v)[32], int i) {
+        if (32 * i + 32 > valid) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (32 * i + e >= valid) s[i][e] = 0xff800000u;
-      }
+            if (32 * i + e >= valid) v[e] = 0xff800000u;
+        }
+      };
+      auto most = [](const uint32_t (&v)[32], float mx) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        return mx;
+      };
+      uint32_t v[2][32];
       float mx[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mx[i] = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) mx[i] = max3(mx[i], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+#pragma unroll 1
+      for (int h = 1; h >= 0; --h) {                       // the second half is read again below
+        tc::ld32(v[0], ts + 64 * h);
+        tc::ld32(v[1], ts + 64 * h + 32);
+        tc::wait_ld(v[0]);
+        tc::wait_ld(v[1]);
+        mask(v[0], 2 * h);
+        mask(v[1], 2 * h + 1);
+        const float a = most(v[0], -INFINITY), b = most(v[1], -INFINITY);
+        mx[2] = h ? a : mx[2];
+        mx[3] = h ? b : mx[3];
+        mx[0] = a;
+        mx[1] = b;
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool grew = top > m + room || (m == -INFINITY && top > m);
@@ -225,42 +252,56 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
       if (grew) m = top;
       const float org = m == -INFINITY ? 0.f : m * sl;
       const f2 sl2 = pk2(sl, sl), org2 = pk2(-org, -org);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t hi[16], lo[16];
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi[16], lo[16];
+          if (h) {
+            tc::wait_ld(v[i]);
+            mask(v[i], 2 + i);
+          }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float a, b;
-          un2(fma2(pk2(__uint_as_float(s[i][2 * e]), __uint_as_float(s[i][2 * e + 1])), sl2, org2), a, b);
-          a = ex2(a);
-          b = ex2(b);
-          l2[e & 1] = add2(l2[e & 1], pk2(a, b));
-          hi[e] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-          un2(fma2(pk2(a, b), pk2(kAbove, kAbove), pk2(-bf16lo(hi[e]), -bf16hi(hi[e]))), a, b);
-          lo[e] = pack_bf16(a, b);
+          for (int e = 0; e < 16; ++e) {
+            float a, b;
+            un2(fma2(pk2(__uint_as_float(v[i][2 * e]), __uint_as_float(v[i][2 * e + 1])), sl2, org2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            l2[e & 1] = add2(l2[e & 1], pk2(a, b));
+            hi[e] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+            un2(fma2(pk2(a, b), pk2(kAbove, kAbove), pk2(-bf16lo(hi[e]), -bf16hi(hi[e]))), a, b);
+            lo[e] = pack_bf16(a, b);
+          }
+          if (h == 0) tc::ld32(v[i], ts + 64 + 32 * i);
+          st16(ts + h * 64 + i * 32, hi);        // over their own scores: leading bits, rests
+          st16(ts + h * 64 + i * 32 + 16, lo);
         }
-        st16(ts + i * 16, hi);
-        st16(ts + 64 + i * 16, lo);
+        wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive((h == 0 ? p_half : p_full) + 8 * t);
       }
-      wait_st();
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(p_full + 8 * t);
     }
     const int64_t slot = PAIR ? ((int64_t)item * splits + split) * 256 + tid : (((int64_t)item * splits + split) * 2 + t) * 128 + r;
     if (steps > 0 && ok) {
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * t, 0));
+      // the row goes through shared memory, where nothing is read any more once both streams are done, and from there in one copy of the thread's own: stored from
+      // registers, a warp's 16 bytes of 32 rows take 32 sectors each
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, 0) && (!(PAIR || n > 1) || tc::mbar_wait(o_done + 8, 0)));
       tc::fence_after();
-      float* const acc = p.pre_acc + slot * HS;
+      const uint32_t mine = smem + (uint32_t)tid * (HS * 4 + 16);
 #pragma unroll 1
-      for (int c = 0; c < HS; c += 32) {
+      for (int c = 0; c < HS && ok; c += 32) {
         uint32_t o[32];
         tc::ld32(o, to + c);
         tc::wait_ld(o);
-        if (row < rows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) __stcg(reinterpret_cast<uint4*>(acc + c + e), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
-        }
+        for (int e = 0; e < 32; e += 4)
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(mine + (c + e) * 4), "r"(o[e]), "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3]) : "memory");
+      }
+      tc::fence_smem_async();
+      if (row < rows && ok) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.pre_acc + slot * HS), "r"(mine), "n"(HS * 4) : "memory");
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       }
     }
     if (row < rows) {

@@ -5,7 +5,6 @@ graph.  CUDA tensors only — no CPU path exists (``B200Error`` is raised instea
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import Dict, Optional, Sequence, Tuple, Union
@@ -597,58 +596,80 @@ def sample_(logits: torch.Tensor, token_out: torch.Tensor, temperature: float = 
 PerRow = Union[float, torch.Tensor]
 
 
-def _current(device: torch.device):
-    """`device` made current for a launch where it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+class _Device:
+    """A device made current for a launch, and the one before again behind it."""
+
+    def __init__(self, index: int, before: int) -> None:
+        self.index, self.before = index, before
+
+    def __enter__(self) -> None:
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc: object) -> None:
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
 
 
-def _one_device(what: str, device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+def _on(device: int) -> _Device:
+    return _Device(device, torch.cuda.current_device())
+
+
+def _one_device(what: str, device: int, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != device:
             C.require_cuda(t)
-            raise C.B200Error(f"{what}: tensors on {device} and {t.device}")
+            raise C.B200Error(f"{what}: tensors on GPU {device} and {t.device}")
 
 
-def _per_row(value: PerRow, rows: int, dtype: torch.dtype, name: str) -> Tuple[Optional[torch.Tensor], float]:
+def _per_row(value: PerRow, rows: int, dtype: torch.dtype, device: int, name: str) -> Tuple[Optional[torch.Tensor], float]:
     """A setting that is one number for all rows or a tensor with one per row -> (tensor or None, number)."""
     if not isinstance(value, torch.Tensor):
         return None, value
-    if value.dtype != dtype or value.dim() != 1 or value.shape[0] != rows:
+    if value.dtype is not dtype or value.shape != (rows,):
         raise C.B200Error(f"{name} must be a number or a {dtype} tensor of one per row (got {value.dtype}, {tuple(value.shape)} for {rows} rows)")
-    return value.contiguous(), 0
+    if value.get_device() != device:
+        _one_device(name, device, value)
+    return value if value.is_contiguous() else value.contiguous(), 0
 
 
-def _rows_of(t: Optional[torch.Tensor], rows: int, cols: int, dtype: torch.dtype, name: str) -> int:
+def _rows_of(t: Optional[torch.Tensor], rows: int, cols: int, dtype: torch.dtype, device: int, name: str) -> int:
     """Distance of the rows of a (rows, cols) tensor, 0 for a (cols,) one that all rows share."""
     if t is None:
         return 0
-    if t.dtype != dtype or t.shape[-1] != cols or t.dim() not in (1, 2) or (t.dim() == 2 and t.shape[0] != rows):
-        raise C.B200Error(f"{name} must be {dtype}, ({cols},) or ({rows}, {cols}) (got {t.dtype}, {tuple(t.shape)})")
-    if (cols > 1 and t.stride(-1) != 1) or t.stride(0) < 0:
+    shape, step = t.shape, t.stride()
+    if t.dtype is not dtype or (shape != (rows, cols) and shape != (cols,)):
+        raise C.B200Error(f"{name} must be {dtype}, ({cols},) or ({rows}, {cols}) (got {t.dtype}, {tuple(shape)})")
+    if cols > 1 and step[-1] != 1:
         raise C.B200Error(f"{name}: the numbers of a row must lie next to each other")
-    return t.stride(0) if t.dim() == 2 else 0
+    if t.get_device() != device:
+        _one_device(name, device, t)
+    return step[0] if len(step) == 2 else 0
 
 
-def _logit_rules(what: str, logits: torch.Tensor, counts: Optional[torch.Tensor], repetition: PerRow, frequency: PerRow, presence: PerRow,
+def _logit_rules(what: str, logits: torch.Tensor, device: int, counts: Optional[torch.Tensor], repetition: PerRow, frequency: PerRow, presence: PerRow,
                  bias: Optional[torch.Tensor], allowed: Optional[torch.Tensor]) -> Tuple["C.LogitRules", tuple]:
     """-> the rules and the tensors they point into."""
-    C.require_cuda(logits)
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
-        raise C.B200Error(f"{what}: logits must be bf16 or fp32 (rows, vocabulary) (got {logits.dtype}, {tuple(logits.shape)})")
+    if device < 0:
+        C.require_cuda(logits)
+    dtype = logits.dtype
+    if logits.dim() != 2 or (dtype is not torch.bfloat16 and dtype is not torch.float32):
+        raise C.B200Error(f"{what}: logits must be bf16 or fp32 (rows, vocabulary) (got {dtype}, {tuple(logits.shape)})")
     B, V = logits.shape
-    if V > 1 and logits.stride(1) != 1:
+    ld, step = logits.stride()
+    if V > 1 and step != 1:
         logits = logits.contiguous()
-    rep, rep_all = _per_row(repetition, B, torch.float32, f"{what}: repetition")
-    freq, freq_all = _per_row(frequency, B, torch.float32, f"{what}: frequency")
-    pres, pres_all = _per_row(presence, B, torch.float32, f"{what}: presence")
+        ld = V
+    rep, rep_all = _per_row(repetition, B, torch.float32, device, "repetition")
+    freq, freq_all = _per_row(frequency, B, torch.float32, device, "frequency")
+    pres, pres_all = _per_row(presence, B, torch.float32, device, "presence")
     if rep is None and not rep_all > 0.0:
         raise C.B200Error(f"{what}: repetition must be above zero (got {rep_all})")
     if counts is not None and counts.dim() != 2:
         raise C.B200Error(f"{what}: counts must be int32 (rows, vocabulary)")
-    _one_device(what, logits.device, counts, rep, freq, pres, bias, allowed)
-    rules = C.LogitRules(logits.data_ptr(), C.DTYPE_CODE[logits.dtype], logits.stride(0), B, V, C.ptr(counts), _rows_of(counts, B, V, torch.int32, f"{what}: counts"),
-                         C.ptr(rep), C.ptr(freq), C.ptr(pres), rep_all, freq_all, pres_all, C.ptr(bias), _rows_of(bias, B, V, torch.float32, f"{what}: bias"),
-                         C.ptr(allowed), _rows_of(allowed, B, (V + 31) // 32, torch.int32, f"{what}: allowed"))
+    rules = C.LogitRules(logits.data_ptr(), C.BF16 if dtype is torch.bfloat16 else C.F32, ld, B, V, C.ptr(counts), _rows_of(counts, B, V, torch.int32, device, "counts"),
+                         C.ptr(rep), C.ptr(freq), C.ptr(pres), rep_all, freq_all, pres_all, C.ptr(bias), _rows_of(bias, B, V, torch.float32, device, "bias"),
+                         C.ptr(allowed), _rows_of(allowed, B, (V + 31) // 32, torch.int32, device, "allowed"))
     return rules, (logits, rep, freq, pres)
 
 
@@ -669,16 +690,17 @@ def adjust_logits(logits: torch.Tensor, *, counts: Optional[torch.Tensor] = None
 
     counts int32 (rows, V); repetition (> 0), frequency, presence: a number or fp32 (rows,); bias fp32 (V,) or (rows, V); allowed int32 (ceil(V / 32),) or
     (rows, ceil(V / 32)) as ``pack_allowed`` makes it."""
-    rules, kept = _logit_rules("adjust_logits", logits, counts, repetition, frequency, presence, bias, allowed)
-    B, V = logits.shape
+    device = logits.get_device()
+    rules, kept = _logit_rules("adjust_logits", logits, device, counts, repetition, frequency, presence, bias, allowed)
     if out is None:
-        out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
-    elif out.shape != logits.shape or out.dtype not in (torch.bfloat16, torch.float32) or out.device != logits.device or (V > 1 and out.stride(1) != 1):
+        out = logits.new_empty(logits.shape, dtype=torch.float32)
+    elif out.shape != logits.shape or out.dtype not in (torch.bfloat16, torch.float32) or out.get_device() != device or (out.shape[1] > 1 and out.stride(1) != 1):
         raise C.B200Error(f"adjust_logits: out must be bf16 or fp32 {tuple(logits.shape)} on {logits.device}, the numbers of a row next to each other")
     elif kept[0] is not logits and out.data_ptr() == logits.data_ptr():
         raise C.B200Error("adjust_logits: in place the numbers of a row must lie next to each other")
-    with _current(logits.device):
-        C.check(C.load_core().b200_adjust_logits(ctypes.byref(rules), out.data_ptr(), C.DTYPE_CODE[out.dtype], out.stride(0), C.stream_ptr(logits.device)), "adjust_logits")
+    with _on(device):
+        C.check(C.load_core().b200_adjust_logits(ctypes.byref(rules), out.data_ptr(), C.BF16 if out.dtype is torch.bfloat16 else C.F32, out.stride(0),
+                                                 torch._C._cuda_getCurrentRawStream(device)), "adjust_logits")
     return out
 
 
@@ -693,32 +715,35 @@ def sample_rows_(logits: torch.Tensor, token_out: torch.Tensor, temperature: Per
     rng_state: int64 (rows, 2) (``new_rng_state(rows=...)``), every row's offset moves on by one; noise: fp32 (V,) or (rows, V) Exp(1) values to use instead.
     logprob_out fp32 (rows,): ln of the token's probability among those kept.  count: counts[b, token] += 1.  pos_inout (rows,): += 1, and then
     history[b, pos] = token where that lies inside ``history`` (rows, length)."""
-    rules, kept = _logit_rules("sample_rows_", logits, counts, repetition, frequency, presence, bias, allowed)
+    device = logits.get_device()
+    rules, kept = _logit_rules("sample_rows_", logits, device, counts, repetition, frequency, presence, bias, allowed)
     B, V = logits.shape
-    temp, temp_all = _per_row(temperature, B, torch.float32, "sample_rows_: temperature")
-    top, top_all = _per_row(0 if top_k is None else top_k, B, torch.int32, "sample_rows_: top_k")
-    if token_out.dtype not in (torch.int32, torch.int64) or token_out.shape != (B,) or not token_out.is_contiguous():
+    temp, temp_all = _per_row(temperature, B, torch.float32, device, "temperature")
+    top, top_all = _per_row(0 if top_k is None else top_k, B, torch.int32, device, "top_k")
+    kind = token_out.dtype
+    if (kind is not torch.int64 and kind is not torch.int32) or token_out.shape != (B,) or not token_out.is_contiguous():
         raise C.B200Error(f"sample_rows_: token_out must be a contiguous int32 / int64 ({B},) tensor")
-    if rng_state is None and noise is None and (temp is not None or temp_all > 0.0):
-        raise C.B200Error("sample_rows_: temperature > 0 needs rng_state (K.new_rng_state(rows=...)) or noise")
-    if rng_state is not None and (rng_state.dtype != torch.int64 or rng_state.shape != (B, 2) or not rng_state.is_contiguous()):
+    if rng_state is None:
+        if noise is None and (temp is not None or temp_all > 0.0):
+            raise C.B200Error("sample_rows_: temperature > 0 needs rng_state (K.new_rng_state(rows=...)) or noise")
+    elif rng_state.dtype is not torch.int64 or rng_state.shape != (B, 2) or not rng_state.is_contiguous():
         raise C.B200Error(f"sample_rows_: rng_state must be a contiguous int64 ({B}, 2) tensor, a state per row")
-    if logprob_out is not None and (logprob_out.dtype != torch.float32 or logprob_out.shape != (B,) or not logprob_out.is_contiguous()):
+    if logprob_out is not None and (logprob_out.dtype is not torch.float32 or logprob_out.shape != (B,) or not logprob_out.is_contiguous()):
         raise C.B200Error(f"sample_rows_: logprob_out must be a contiguous fp32 ({B},) tensor")
     if pos_inout is not None and (pos_inout.dtype not in (torch.int32, torch.int64) or pos_inout.shape != (B,) or not pos_inout.is_contiguous()):
         raise C.B200Error(f"sample_rows_: pos_inout must be a contiguous int32 / int64 ({B},) tensor, a position per row")
-    if history is not None and (pos_inout is None or history.dtype != token_out.dtype or history.dim() != 2 or history.shape[0] != B
+    if history is not None and (pos_inout is None or history.dtype is not kind or history.dim() != 2 or history.shape[0] != B
                                 or (history.shape[1] > 1 and history.stride(1) != 1) or (B > 1 and history.stride(0) < history.shape[1])):
         raise C.B200Error(f"sample_rows_: history must be ({B}, length) of token_out's dtype, with pos_inout")
     if count and (counts is None or (B > 1 and counts.stride(0) < V)):
         raise C.B200Error("sample_rows_: nothing to count in")
-    _one_device("sample_rows_", logits.device, token_out, temp, top, rng_state, noise, logprob_out, pos_inout, history)
-    args = C.DrawArgs(C.ptr(temp), temp_all, C.ptr(top), min(int(top_all), 2 ** 31 - 1), C.ptr(rng_state), C.ptr(noise), _rows_of(noise, B, V, torch.float32, "sample_rows_: noise"),
-                      token_out.data_ptr(), token_out.dtype == torch.int64, C.ptr(logprob_out), count, C.ptr(pos_inout),
-                      pos_inout is not None and pos_inout.dtype == torch.int64, C.ptr(history), 0 if history is None else history.stride(0),
+    _one_device("sample_rows_", device, token_out, rng_state, logprob_out, pos_inout, history)
+    args = C.DrawArgs(C.ptr(temp), temp_all, C.ptr(top), min(int(top_all), 2 ** 31 - 1), C.ptr(rng_state), C.ptr(noise),
+                      _rows_of(noise, B, V, torch.float32, device, "noise"), token_out.data_ptr(), kind is torch.int64, C.ptr(logprob_out), count, C.ptr(pos_inout),
+                      pos_inout is not None and pos_inout.dtype is torch.int64, C.ptr(history), 0 if history is None else history.stride(0),
                       0 if history is None else history.shape[1])
-    with _current(logits.device):
-        C.check(C.load_core().b200_sample_rows(ctypes.byref(rules), ctypes.byref(args), C.stream_ptr(logits.device)), "sample_rows_")
+    with _on(device):
+        C.check(C.load_core().b200_sample_rows(ctypes.byref(rules), ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), "sample_rows_")
 
 
 def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], lengths: Optional[Sequence[int]] = None) -> None:
@@ -729,24 +754,28 @@ def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
         raise C.B200Error("copy_slots: as many destinations (and lengths) as sources")
     if not tensors:
         return
-    device, slots = tensors[0].device, tensors[0].shape[0] if tensors[0].dim() else 0
-    table = (C.SlotTensor * len(tensors))()
+    device, slots = tensors[0].get_device(), tensors[0].shape[0] if tensors[0].dim() else 0
+    table = []
     for i, t in enumerate(tensors):
-        if t.dim() < 2 or not t.is_contiguous() or t.shape[0] != slots:
-            raise C.B200Error(f"copy_slots: tensor {i} must be contiguous (slots, ...) with {slots} slots (got {tuple(t.shape)})")
-        if t.numel() == 0:
+        shape = t.shape
+        if len(shape) < 2 or shape[0] != slots or not t.is_contiguous():
+            raise C.B200Error(f"copy_slots: tensor {i} must be contiguous (slots, ...) with {slots} slots (got {tuple(shape)})")
+        nbytes = t.nbytes
+        if nbytes == 0:
             raise C.B200Error(f"copy_slots: tensor {i} is empty")
-        table[i].base, table[i].rows, table[i].row_bytes = t.data_ptr(), t.shape[1], t.stride(0) // t.shape[1] * t.element_size()
-    C.require_cuda(*tensors)
-    _one_device("copy_slots", device, *tensors)
-    pairs = (C.SlotPair * max(len(src), 1))()
-    for i in range(len(src)):
-        n = -1 if lengths is None else int(lengths[i])
-        if lengths is not None and n < 0:
-            raise C.B200Error(f"copy_slots: copy {i} of {n} positions")
-        pairs[i].src, pairs[i].dst, pairs[i].rows = int(src[i]), int(dst[i]), n
-    with _current(device):
-        C.check(C.load_core().b200_copy_slots(table, len(tensors), slots, pairs, len(src), C.stream_ptr(device)), "copy_slots")
+        if device < 0 or t.get_device() != device:
+            _one_device("copy_slots", max(device, 0), t)
+        table.append((t.data_ptr(), shape[1], nbytes // (slots * shape[1])))
+    n = len(src)
+    if lengths is None:
+        pairs = [(int(a), int(b), -1) for a, b in zip(src, dst)]
+    elif n and min(lengths) < 0:
+        raise C.B200Error(f"copy_slots: a copy of {min(lengths)} positions")
+    else:
+        pairs = [(int(a), int(b), int(c)) for a, b, c in zip(src, dst, lengths)]
+    with _on(device):
+        C.check(C.load_core().b200_copy_slots((C.SlotTensor * len(table))(*table), len(table), slots, (C.SlotPair * max(n, 1))(*pairs), n,
+                                              torch._C._cuda_getCurrentRawStream(device)), "copy_slots")
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -801,46 +830,63 @@ def attn_decode_shared(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     untouched, result zero).  k_prefix / v_prefix (G, P, hs) bf16 hold positions 0 .. n - 1, n = prefix_len (device int, at most P; None: P); k_cache / v_cache
     (B, G, rows, hs) bf16 hold row b's position p at p - n and are updated in place.  Any distance between groups and rows of a batch that is a multiple of 8
     numbers; rows of hs numbers next to each other.  Returns (B, H*hs)."""
-    C.require_cuda(qkv, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len)
-    qkv = _bf16c(qkv, "qkv")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != n_groups or k_cache.shape[3] != head_size:
-        raise C.B200Error(f"attn_decode_shared: caches must be (rows, {n_groups}, length, {head_size}) (got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
-    if k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != n_groups or k_prefix.shape[2] != head_size:
-        raise C.B200Error(f"attn_decode_shared: prefix must be ({n_groups}, length, {head_size}) (got {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)})")
-    for t in (k_cache, v_cache, k_prefix, v_prefix):
-        if t.dtype != torch.bfloat16 or t.stride(-1) != 1 or (t.shape[-2] > 1 and t.stride(-2) != head_size):
-            raise C.B200Error("attn_decode_shared: caches and prefix must be bfloat16, rows of head_size numbers next to each other")
-    apart = [tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 2)) for t in (k_cache, v_cache, k_prefix, v_prefix)]
-    if any(n > 1 and step < k_cache.shape[2] * head_size for t in apart[:2] for n, step in zip(k_cache.shape, t)):
-        raise C.B200Error("attn_decode_shared: the caches of two rows or groups overlap")
-    if n_groups > 1 and min(apart[2][0], apart[3][0]) < k_prefix.shape[1] * head_size:
-        raise C.B200Error("attn_decode_shared: the prefixes of two groups overlap")
-    B, _, S, _ = k_cache.shape
-    if qkv.numel() != B * (n_head + 2 * n_groups) * head_size:
+    device, bf16 = qkv.get_device(), torch.bfloat16
+    if device < 0 or any(t.get_device() != device for t in (cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix)) or (prefix_len is not None and prefix_len.get_device() != device):
+        C.require_cuda(qkv)
+        _one_device("attn_decode_shared", device, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len)
+    if qkv.dtype is not bf16 or not qkv.is_contiguous():
+        qkv = _bf16c(qkv, "qkv")
+    own, pre = k_cache.shape, k_prefix.shape
+    if len(own) != 4 or own != v_cache.shape or own[1] != n_groups or own[3] != head_size:
+        raise C.B200Error(f"attn_decode_shared: caches must be (rows, {n_groups}, length, {head_size}) (got {tuple(own)}, {tuple(v_cache.shape)})")
+    if len(pre) != 3 or pre != v_prefix.shape or pre[0] != n_groups or pre[2] != head_size:
+        raise C.B200Error(f"attn_decode_shared: prefix must be ({n_groups}, length, {head_size}) (got {tuple(pre)}, {tuple(v_prefix.shape)})")
+    B, G, S, hs = own
+    P = pre[1]
+    kb, kg, kr, ke = k_cache.stride()
+    vb, vg, vr, ve = v_cache.stride()
+    pkg, pkr, pke = k_prefix.stride()
+    pvg, pvr, pve = v_prefix.stride()
+    if not (k_cache.dtype is bf16 and v_cache.dtype is bf16 and k_prefix.dtype is bf16 and v_prefix.dtype is bf16 and ke == ve == pke == pve == 1
+            and (S <= 1 or kr == vr == hs) and (P <= 1 or pkr == pvr == hs)):
+        raise C.B200Error("attn_decode_shared: caches and prefix must be bfloat16, rows of head_size numbers next to each other")
+    if B == 1:
+        kb = vb = 0
+    elif min(kb, vb) < S * hs:
+        raise C.B200Error("attn_decode_shared: the caches of two rows overlap")
+    if G == 1:
+        kg = vg = pkg = pvg = 0
+    elif min(kg, vg) < S * hs or min(pkg, pvg) < P * hs:
+        raise C.B200Error("attn_decode_shared: the caches or the prefixes of two groups overlap")
+    if qkv.numel() != B * (n_head + 2 * n_groups) * hs:
         raise C.B200Error("attn_decode_shared: qkv does not hold exactly one token per row of the caches")
-    for t, n, name in ((pos, (1, B), "pos"), (prefix_len, (1,), "prefix_len")):
-        if t is not None and (t.dtype not in (torch.int64, torch.int32) or t.numel() not in n):
-            raise C.B200Error(f"attn_decode_shared: {name} must be an int32/int64 device tensor of {' or '.join(map(str, n))}")
-    if cos.dtype != sin.dtype or cos.shape != sin.shape or cos.shape[-1] != rope_n_elem:
+    positions, kind = pos.numel(), pos.dtype
+    if (kind is not torch.int64 and kind is not torch.int32) or (positions != 1 and positions != B):
+        raise C.B200Error(f"attn_decode_shared: pos must be an int32/int64 device tensor of 1 or {B}")
+    if prefix_len is not None and (prefix_len.dtype not in (torch.int64, torch.int32) or prefix_len.numel() != 1):
+        raise C.B200Error("attn_decode_shared: prefix_len must be a single int32/int64 device scalar")
+    table = cos.shape
+    if table != sin.shape or table[-1] != rope_n_elem or cos.dtype is not sin.dtype:
         raise C.B200Error(f"attn_decode_shared: cos and sin must be (positions, {rope_n_elem}) of one dtype")
-    _one_device("attn_decode_shared", qkv.device, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len)
     cos, sin, pos = cos.contiguous(), sin.contiguous(), pos.contiguous()
     table_rows = cos.numel() // max(rope_n_elem, 1)
-    if table_preselected and table_rows != pos.numel():
-        raise C.B200Error(f"attn_decode_shared: {table_rows} preselected table rows for {pos.numel()} positions")
-    P = k_prefix.shape[1]
-    out = torch.empty((B, n_head * head_size), dtype=torch.bfloat16, device=qkv.device)
-    lib = C.load()
-    with _current(qkv.device):
-        nbytes = lib.b200_attn_decode_shared_workspace_bytes(B, n_head, n_groups, head_size, P, S)
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=qkv.device)   # of this call: calls on two streams, or in two graphs, have one each
+    if table_preselected and table_rows != positions:
+        raise C.B200Error(f"attn_decode_shared: {table_rows} preselected table rows for {positions} positions")
+    out = qkv.new_empty((B, n_head * hs))
+    with _on(device):
+        nbytes = _shared_workspace_bytes(device, B, n_head, n_groups, hs, P, S)
+        ws = qkv.new_empty(max(nbytes // 2, 8))   # of this call: calls on two streams, or in two graphs, have one each
         args = C.AttnDecodeSharedArgs(
-            qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, pos.data_ptr(), pos.dtype == torch.int64,
-            pos.numel(), C.ptr(prefix_len), prefix_len is not None and prefix_len.dtype == torch.int64, k_cache.data_ptr(), v_cache.data_ptr(), *apart[0], *apart[1],
-            k_prefix.data_ptr(), v_prefix.data_ptr(), *apart[2], *apart[3], out.data_ptr(),
-            B, n_head, n_groups, head_size, S, P, ws.data_ptr(), nbytes)
-        C.check(lib.b200_attn_decode_shared(ctypes.byref(args), C.stream_ptr(qkv.device)), "attn_decode_shared")
+            qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, pos.data_ptr(), kind is torch.int64, positions,
+            None if prefix_len is None else prefix_len.data_ptr(), prefix_len is not None and prefix_len.dtype is torch.int64, k_cache.data_ptr(), v_cache.data_ptr(), kb, kg, vb, vg,
+            k_prefix.data_ptr(), v_prefix.data_ptr(), pkg, pvg, out.data_ptr(), B, n_head, n_groups, hs, S, P, ws.data_ptr(), nbytes)
+        C.check(C.load().b200_attn_decode_shared(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), "attn_decode_shared")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_workspace_bytes(device: int, batch: int, n_head: int, n_groups: int, head_size: int, prefix_rows: int, own_rows: int) -> int:
+    return int(C.load().b200_attn_decode_shared_workspace_bytes(batch, n_head, n_groups, head_size, prefix_rows, own_rows))
 
 
 def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,
