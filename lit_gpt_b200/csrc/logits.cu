@@ -76,6 +76,28 @@ struct RowRules {
         if (!((w >> e) & 1u)) l[e] = -INFINITY;
     }
   }
+  // N tokens first, first + step, .., those below `end`; everything is on its way before any of it is used
+  template <int N>
+  __device__ __forceinline__ void some(int first, int step, int end, float (&l)[N]) const {
+    int n[N];
+    float add[N];
+    uint32_t word[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int v = first + i * step;
+      const bool in = v < end;
+      l[i] = in ? load_as_float<LT>(logits, v) : -INFINITY;
+      n[i] = in && counts ? counts[v] : 0;
+      add[i] = in && bias ? bias[v] : 0.f;
+      word[i] = in && allowed ? allowed[v >> 5] >> (v & 31) : 1u;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      l[i] = penalised(l[i], n[i]);
+      if (bias) l[i] = __fadd_rn(l[i], add[i]);
+      if (!(word[i] & 1u)) l[i] = -INFINITY;
+    }
+  }
   __device__ __forceinline__ bool wide() const {
     return ((reinterpret_cast<uintptr_t>(logits) & (4 * sizeof(LT) - 1)) | ((reinterpret_cast<uintptr_t>(counts) | reinterpret_cast<uintptr_t>(bias)) & 15)) == 0;
   }
@@ -115,8 +137,10 @@ __global__ void __launch_bounds__(kAdjThreads) adjust_kernel(const Rules r, OT* 
 }
 
 // ---- the draw -----------------------------------------------------------------------------------------------------------------------
-// A row's tokens are cut into the slices of a cluster's CTAs; a slice's adjusted logits stay in shared memory (CACHED) and are read again by every later step.
-constexpr int kSaThreads = 512, kSaBins = 2048;
+// A row's tokens are cut into the slices of a cluster's CTAs; a slice's adjusted logits stay in shared memory (CACHED) and are read again by the later steps.
+constexpr int kSaThreads = 512, kSaWarps = kSaThreads / 32, kSaBins = 2 * kSaThreads, kSaDigit = 10, kSaCtas = 8;
+constexpr int kSaGather = 2048;   // tokens that one CTA goes on with alone
+constexpr float kNear = 1e-3f;    // scores this close to the best are compared in 64 bits
 
 struct DrawArgs {
   const float* temperature; float temperature_all;
@@ -138,72 +162,96 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float remote_f32(const float* p, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(p, rank)) : "memory");
+__device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ double remote_f64(const double* p, uint32_t rank) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote(p, rank)) : "memory");
+__device__ __forceinline__ uint2 remote_u2(const void* p, uint32_t rank) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(remote(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ uint4 remote_u4(const void* p, uint32_t rank) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote(p, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void remote_store(const void* p, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t remote_add(const void* p, uint32_t rank, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(remote(p, rank)), "r"(v) : "memory");
+  return old;
 }
 
-template <typename LT, bool CACHED>
-__global__ void __launch_bounds__(kSaThreads) sample_rows_kernel(const Rules r, const DrawArgs a) {
-  extern __shared__ __align__(16) float s_l[];                       // the slice's adjusted logits, then its scores
+// Where counts, from bin 0 on or with DOWN from the last bin on, come to `left`: the bin, what is left of `left` in it, what it holds (0xffffffff: nowhere).  n: the
+// counts of bins 2 i and 2 i + 1, DOWN counted from the last, with i the thread.  All threads call it; true in the one whose bin it is.
+template <bool DOWN>
+__device__ __forceinline__ bool find_bin(const uint2& n, uint32_t left, uint32_t* s_warp, uint32_t (&s_found)[3]) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t c0 = DOWN ? n.y : n.x, c1 = DOWN ? n.x : n.y, total = c0 + c1;
+  uint32_t inc = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+  if (lane == 31) s_warp[warp] = inc;
+  if (tid == 0) s_found[0] = 0xffffffffu;
+  __syncthreads();
+  uint32_t sum = lane < kSaWarps && lane < warp ? s_warp[lane] : 0u;
+  sum = __reduce_add_sync(0xffffffffu, sum) + inc - total;
+  const bool mine = sum < left && sum + total >= left;   // one thread at most
+  if (mine) {
+    const bool second = sum + c0 < left;
+    const int bin = 2 * tid + second;
+    s_found[0] = (uint32_t)(DOWN ? kSaBins - 1 - bin : bin);
+    s_found[1] = left - sum - (second ? c0 : 0u);
+    s_found[2] = second ? c1 : c0;
+  }
+  __syncthreads();
+  return mine;
+}
+
+template <typename LT, bool CACHED, bool WIDE>
+__global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules r, const DrawArgs a) {
+  extern __shared__ __align__(16) float s_l[];                       // the slice's adjusted logits
   __shared__ __align__(16) uint32_t s_hist[2][kSaBins];
-  __shared__ uint32_t s_warp[16], s_bin, s_left, s_in_bin;
-  __shared__ float s_red[16];
-  __shared__ double s_redd[16], s_weights[16];
-  __shared__ int s_redi[16];
-  __shared__ float s_max;
-  __shared__ double s_score, s_weight, s_sum;
-  __shared__ int s_index;
+  __shared__ uint32_t s_warp[kSaWarps], s_found[3], s_ties[kSaCtas], s_gathered;
+  __shared__ float s_gl[kSaGather], s_ge[kSaGather];                  // gathered in the first CTA: logits, their e, their tokens
+  __shared__ int s_gv[kSaGather];
+  __shared__ float s_top[kSaWarps], s_l_of[kSaWarps], s_max;
+  __shared__ uint64_t s_sum[kSaWarps];
+  __shared__ int s_index[kSaWarps], s_close;
+  __shared__ double s_exact[kSaWarps];
+  __shared__ uint32_t s_all[kSaCtas][5];                              // of every CTA, in the first one: best score, its token, its logit, sum
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cta_rank(), ctas = cta_count();
   const int b = blockIdx.x / ctas;
+  *reinterpret_cast<uint2*>(s_hist[0] + 2 * tid) = make_uint2(0u, 0u);
+  if (tid == 0) { s_close = 0; s_gathered = 0u; }
   griddep_launch();
   griddep_wait();
   const RowRules<LT> row(r, b);
-  const int V = r.vocab, v0 = (int)rank * a.slice, v1 = min(V, v0 + a.slice), quads = v1 > v0 ? (v1 - v0 + 3) / 4 : 0;
+  const int V = r.vocab, v0 = (int)rank * a.slice, n = max(0, min(V - v0, a.slice)), quads = (n + 3) / 4;
   const float T = a.temperature ? a.temperature[b] : a.temperature_all;
   const bool greedy = !(T > 0.f);
   const int k = a.top_k ? a.top_k[b] : a.top_k_all;
+  const bool select = !greedy && k > 0 && k < V;
   const float* const noise = a.noise ? a.noise + (int64_t)b * a.noise_ld : nullptr;
   const uint64_t seed = a.rng ? (uint64_t)a.rng[2 * b] : 0ull, offset = a.rng ? (uint64_t)a.rng[2 * b + 1] : 0ull;
-  const bool wide = row.wide(), noise_wide = noise && (reinterpret_cast<uintptr_t>(noise) & 15) == 0;
+  __syncthreads();
 
-  // a NaN logit counts as -inf, a zero has no sign; tokens past the vocabulary are -inf
-  auto fetch = [&](int q, float (&l)[4]) {
-    const int v = v0 + 4 * q;
-    if (wide && v + 3 < V) {
-      row.at4(v, l);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) l[e] = v + e < V ? row.at(v + e) : -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) l[e] = l[e] == l[e] ? l[e] + 0.f : -INFINITY;
-  };
+  // a NaN logit counts as -inf, a zero has no sign; tokens past the slice are -inf
+  auto clean = [](float l) { return l == l ? l + 0.f : -INFINITY; };
   auto logits4 = [&](int q, float (&l)[4]) {
     if constexpr (CACHED) {
       const float4 w = *reinterpret_cast<const float4*>(s_l + 4 * q);
       l[0] = w.x; l[1] = w.y; l[2] = w.z; l[3] = w.w;
     } else {
-      fetch(q, l);
+      row.some(v0 + 4 * q, 1, v0 + n, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[e] = clean(l[e]);
     }
   };
   // e of four tokens: between 0 and the largest number
-  auto exponentials = [&](int q, float (&e)[4]) {
-    const int v = v0 + 4 * q;
+  auto exponentials = [&](int v, float (&e)[4]) {
     if (noise) {
-      if (noise_wide && v + 3 < V) {
+      if (WIDE && v + 3 < V) {
         const float4 w = *reinterpret_cast<const float4*>(noise + v);
         e[0] = w.x; e[1] = w.y; e[2] = w.z; e[3] = w.w;
       } else {
@@ -219,214 +267,394 @@ __global__ void __launch_bounds__(kSaThreads) sample_rows_kernel(const Rules r, 
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = fmaxf(fminf(e[i], 3.4028234e38f), 0.f);
   };
+  auto exponential = [&](int v) {
+    float e[4];
+    exponentials(v & ~3, e);
+    const float lo = v & 1 ? e[1] : e[0], hi = v & 1 ? e[3] : e[2];
+    return v & 2 ? hi : lo;
+  };
 
-  // ---- adjusted logits and their maximum ----
+  // ---- adjusted logits, their maximum, the first digit's histogram ----
   float top = -INFINITY;
-  for (int q = tid; q < quads; q += kSaThreads) {
-    float l[4];
-    fetch(q, l);
-    if constexpr (CACHED) *reinterpret_cast<float4*>(s_l + 4 * q) = make_float4(l[0], l[1], l[2], l[3]);
-    top = fmaxf(fmaxf(top, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
+  auto see = [&](float l) {
+    top = fmaxf(top, l);
+    if (select && l > -INFINITY) atomicAdd(&s_hist[0][order_key(l) >> (32 - kSaDigit)], 1u);
+  };
+  if constexpr (CACHED && WIDE) {
+#pragma unroll 2
+    for (int q = tid; q < quads; q += kSaThreads) {
+      float l[4];
+      if (v0 + 4 * q + 3 < V) row.at4(v0 + 4 * q, l);
+      else row.some(v0 + 4 * q, 1, v0 + n, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[e] = clean(l[e]);
+      *reinterpret_cast<float4*>(s_l + 4 * q) = make_float4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) see(l[e]);
+    }
+  } else {
+    constexpr int N = 8;
+    for (int i0 = tid; i0 < 4 * quads; i0 += N * kSaThreads) {
+      float l[N];
+      row.some(v0 + i0, kSaThreads, v0 + n, l);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int i = i0 + e * kSaThreads;
+        l[e] = clean(l[e]);
+        if (CACHED && i < 4 * quads) s_l[i] = l[e];
+        see(l[e]);
+      }
+    }
   }
-  for (int i = tid; i < kSaBins; i += kSaThreads) s_hist[0][i] = 0u;
   top = warp_max(top);
-  if (lane == 0) s_red[warp] = top;
+  if (lane == 0) s_top[warp] = top;
   __syncthreads();
   if (warp == 0) {
-    top = warp_max(lane < 16 ? s_red[lane] : -INFINITY);
+    top = warp_max(lane < kSaWarps ? s_top[lane] : -INFINITY);
     if (lane == 0) s_max = top;
   }
   cluster_barrier();
-  float M = -INFINITY;
-  for (uint32_t c = 0; c < ctas; ++c) M = fmaxf(M, remote_f32(&s_max, c));
+  float M = __uint_as_float(remote_u32(&s_max, min((uint32_t)lane, ctas - 1)));   // (its warp's maximum is taken below)
 
-  // ---- the k-th largest (logit, lowest token): a digit of the 62-bit key a pass, from the highest ----
-  uint64_t bound = 0ull;   // kept: keys from here on
-  auto key_of = [](float l, int v) { return ((uint64_t)order_key(l) << 30) | (uint64_t)((1u << 30) - 1u - (uint32_t)v); };
-  if (!greedy && k > 0 && k < V && M > -INFINITY) {
+  // ---- the k-th largest logit, a digit of its key a pass; of those equal to it the lowest tokens ----
+  uint32_t bound = 0u;      // kept: keys above it, and those equal to it, from bit `low` on, up to token `cut`
+  int low = 0, cut = 0x7fffffff;
+  bool alone = false;       // the first CTA goes on with what was gathered
+  uint32_t gathered = 0u;
+  if (select) {
     uint32_t left = (uint32_t)k;
-    int pass = 0;
-    for (int shift = 51, bits = 11; shift >= 0; ++pass) {
+    const bool short_keys = sizeof(LT) == 2 && !row.counts && !row.bias;   // bf16 numbers: bits 15 .. 0 of a key say nothing
+#pragma unroll 1
+    for (int pass = 0, shift = 32 - kSaDigit, bits = kSaDigit;; ++pass) {
       uint32_t* const hist = s_hist[pass & 1];
-      for (int q = tid; q < quads; q += kSaThreads) {
-        float l[4];
-        logits4(q, l);
+      if (pass > 0) {
+        if (alone) {
+#pragma unroll 1
+          for (uint32_t i = tid; i < gathered; i += kSaThreads) {
+            const uint32_t key = order_key(s_gl[i]);
+            if (((key ^ bound) >> (shift + bits)) == 0u) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+          }
+          __syncthreads();
+        } else {
+#pragma unroll 1
+          for (int q = tid; q < quads; q += kSaThreads) {
+            float l[4];
+            logits4(q, l);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint64_t key = key_of(l[e], v0 + 4 * q + e);
-          if ((key >> (shift + bits)) == (bound >> (shift + bits)) && l[e] > -INFINITY) atomicAdd(&hist[(uint32_t)(key >> shift) & ((1u << bits) - 1u)], 1u);
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t key = order_key(l[e]);
+              if (((key ^ bound) >> (shift + bits)) == 0u && l[e] > -INFINITY) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+            }
+          }
+          cluster_barrier();
         }
       }
-      cluster_barrier();
-      // every CTA adds the histograms up: four bins a thread, the highest bins first
-      const int first = kSaBins - 4 * (tid + 1);
-      uint4 n = make_uint4(0u, 0u, 0u, 0u);
-      for (uint32_t c = 0; c < ctas; ++c) {
-        const uint4 m = remote_u4(hist + first, c);
-        n.x += m.x; n.y += m.y; n.z += m.z; n.w += m.w;
-      }
-      uint32_t* const other = s_hist[(pass & 1) ^ 1];   // (read by all before they came to the barrier)
-      *reinterpret_cast<uint4*>(other + first) = make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t total = n.x + n.y + n.z + n.w;
-      uint32_t inc = total;
+      // every CTA adds the histograms up, the highest bins first
+      const int first = kSaBins - 2 * (tid + 1);
+      uint2 m[kSaCtas], sum = make_uint2(0u, 0u);
+      if (alone) {
+        sum = *reinterpret_cast<const uint2*>(hist + first);
+      } else {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
-      if (lane == 31) s_warp[warp] = inc;
-      if (tid == 0) s_bin = 0xffffffffu;
-      __syncthreads();
-      uint32_t before = inc - total;
-      for (int w = 0; w < warp; ++w) before += s_warp[w];
-      if (before < left && before + total >= left) {   // one thread at most
-        uint32_t cum = before, bin = (uint32_t)first + 3u, here = n.w;
-        if (cum + here < left) { cum += here; here = n.z; --bin; }
-        if (bin == (uint32_t)first + 2u && cum + here < left) { cum += here; here = n.y; --bin; }
-        if (bin == (uint32_t)first + 1u && cum + here < left) { cum += here; here = n.x; --bin; }
-        s_bin = bin;
-        s_left = left - cum;
-        s_in_bin = here;
+        for (uint32_t c = 0; c < kSaCtas; ++c) m[c] = c < ctas ? remote_u2(hist + first, c) : make_uint2(0u, 0u);
+#pragma unroll
+        for (uint32_t c = 0; c < kSaCtas; ++c) { sum.x += m[c].x; sum.y += m[c].y; }
+      }
+      *reinterpret_cast<uint2*>(s_hist[(pass & 1) ^ 1] + first) = make_uint2(0u, 0u);   // (read by all before they came to the barrier)
+      if (find_bin<true>(sum, left, s_warp, s_found) && !alone) {
+#pragma unroll
+        for (uint32_t c = 0; c < kSaCtas; ++c) s_ties[c] = s_found[0] & 1u ? m[c].y : m[c].x;
       }
       __syncthreads();
-      if (s_bin == 0xffffffffu) break;   // fewer than k are above -inf: all of them (first pass only)
-      bound |= (uint64_t)s_bin << shift;
-      left = s_left;
-      if (s_in_bin == left) break;       // the bin's are all kept
-      if (shift == 0) break;
-      const int next = shift == 51 ? 11 : 10;
+      const uint32_t bin = s_found[0], in_bin = s_found[2];
+      if (bin == 0xffffffffu) break;           // fewer than k are above -inf: all of them (in the first pass)
+      const uint32_t above = left - s_found[1];   // in higher bins
+      bound |= bin << shift;
+      left = s_found[1];
+      low = shift;
+      if (in_bin == left && (alone || pass > 0)) break;           // the bin's are all kept
+      if (pass == 0 && above + in_bin <= (uint32_t)kSaGather) {
+        // few: the first CTA takes them all
+#pragma unroll 1
+        for (int q = tid; q < quads; q += kSaThreads) {
+          float l[4];
+          logits4(q, l);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (l[e] > -INFINITY && order_key(l[e]) >> shift >= bin) {
+              const int v = v0 + 4 * q + e;
+              const uint32_t at = remote_add(&s_gathered, 0, 1u);
+              const float x = exponential(v);
+              remote_store(s_gl + at, 0, __float_as_uint(l[e]));
+              remote_store(s_ge + at, 0, __float_as_uint(x));
+              remote_store(s_gv + at, 0, (uint32_t)v);
+            }
+        }
+        M = warp_max(M);
+        cluster_barrier();   // (behind it no CTA reads or writes another's shared memory)
+        if (rank != 0) return;
+        alone = true;
+        gathered = above + in_bin;
+        if (in_bin == left) break;
+      } else if (in_bin == left) {
+        break;
+      }
+      if (shift == 0 || (short_keys && shift <= 16)) {
+        // equal logits: those of the first CTAs, then of one CTA those of the lowest tokens
+        uint32_t have = in_bin, keep = left;
+        if (!alone) {
+          uint32_t before = 0u;
+          for (uint32_t c = 0; c < rank; ++c) before += s_ties[c];
+          have = s_ties[rank];
+          keep = left <= before ? 0u : min(left - before, have);
+        }
+        if (keep < have) {
+          cut = -1;
+          if (keep > 0u) {
+            uint32_t want = keep;
+            uint32_t* const local = s_hist[(pass & 1) ^ 1];    // (empty, and no other CTA's business)
+            int token = 0;
+#pragma unroll 1
+            for (int at = 2 * kSaDigit; at >= 0; at -= kSaDigit) {   // digits of the token
+              if (V >> at == 0) continue;
+              auto look = [&](float l, int v) {
+                if (((order_key(l) ^ bound) >> low) == 0u && l > -INFINITY && (at == 2 * kSaDigit || v >> (at + kSaDigit) == token >> (at + kSaDigit)))
+                  atomicAdd(&local[(v >> at) & (kSaBins - 1)], 1u);
+              };
+              if (alone) {
+#pragma unroll 1
+                for (uint32_t i = tid; i < gathered; i += kSaThreads) look(s_gl[i], s_gv[i]);
+              } else {
+#pragma unroll 1
+                for (int q = tid; q < quads; q += kSaThreads) {
+                  float l[4];
+                  logits4(q, l);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) look(l[e], v0 + 4 * q + e);
+                }
+              }
+              __syncthreads();
+              const uint2 h = *reinterpret_cast<const uint2*>(local + 2 * tid);
+              *reinterpret_cast<uint2*>(local + 2 * tid) = make_uint2(0u, 0u);
+              find_bin<false>(h, want, s_warp, s_found);
+              token |= (int)(s_found[0] << at);
+              want = s_found[1];
+              __syncthreads();
+            }
+            cut = token;
+          }
+        }
+        break;
+      }
+      const int next = min(shift, kSaDigit);
       shift -= next;
       bits = next;
       __syncthreads();
     }
   }
+  if (!alone) M = warp_max(M);
+  auto kept = [&](float l, int v) {
+    const uint32_t key = order_key(l) >> low, edge = bound >> low;
+    return l > -INFINITY && (key > edge || (key == edge && v <= cut));
+  };
 
-  // ---- weights, scores in fp32 ----
-  const float inv = greedy ? 1.f : 1.f / T, inv2 = inv * 1.4426950408889634f;
-  float sum = 0.f, best = -INFINITY;
-  if (M > -INFINITY) {
-    for (int q = tid; q < quads; q += kSaThreads) {
-      float l[4], e[4], s[4];
-      logits4(q, l);
-      if (!greedy) exponentials(q, e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i] = -INFINITY;
-        if (l[i] > -INFINITY && key_of(l[i], v0 + 4 * q + i) >= bound) {
-          const float gap = l[i] == M ? 0.f : l[i] - M;
-          sum += gap == 0.f ? 1.f : exp2f(gap * inv2);
-          s[i] = greedy ? l[i] : (gap == 0.f ? 0.f : gap * inv) - __logf(e[i]);
-          best = fmaxf(best, s[i]);
-        }
-      }
-      if constexpr (CACHED) *reinterpret_cast<float4*>(s_l + 4 * q) = make_float4(s[0], s[1], s[2], s[3]);
-    }
-  }
-  sum = warp_sum(sum);
-  best = warp_max(best);
-  __syncthreads();
-  if (lane == 0) { s_red[warp] = best; s_redd[warp] = (double)sum; }
-  __syncthreads();
-  best = warp_max(lane < 16 ? s_red[lane] : -INFINITY);
-  double all = 0.0;
-  if (tid == 0)
-    for (int w = 0; w < 16; ++w) all += s_redd[w];
-
-  // ---- the best of the slice in 64 bits, of equal ones the lowest token ----
-  double score = -INFINITY, weight = 0.0;
+  // ---- weights and scores; a thread's best and whether another of its own comes close ----
+  // Weights are added as whole numbers, so that the sum does not depend on the order that tokens were gathered in.
+  const float inv = greedy ? 1.f : 1.f / T, inv2 = inv * 1.4426950408889634f, unit = __int_as_float((127 + __clz(V)  + 30) << 23);   // 2^(30 + leading zeros): V of them stay below 2^63
+  auto score_of = [&](float l, float e) {
+    const float w = l == M ? 0.f : (l - M) * inv;
+    return greedy ? l : w > -INFINITY ? w - __logf(e) : -INFINITY;
+  };
+  uint64_t sum = 0ull;
+  float best = -INFINITY, second = -INFINITY, best_l = 0.f;
   int index = 0x7fffffff;
-  if (best > -INFINITY) {
-    const float near = greedy ? best : best - 1e-3f;
+  auto weigh = [&](float l, float e, int v) {
+    const float gap = l == M ? 0.f : l - M;
+    sum += __float2ull_rz((gap == 0.f ? 1.f : exp2f(gap * inv2)) * unit);
+    const float s = score_of(l, e);
+    if (s > best || index == 0x7fffffff || (s == best && v < index)) {
+      second = best;
+      best = s;
+      best_l = l;
+      index = v;
+    } else {
+      second = fmaxf(second, s);
+    }
+  };
+  if (alone) {
+#pragma unroll 1
+    for (uint32_t i = tid; i < gathered; i += kSaThreads) {
+      const float l = s_gl[i];
+      if (kept(l, s_gv[i])) weigh(l, s_ge[i], s_gv[i]);
+    }
+  } else if (M > -INFINITY) {
+#pragma unroll 2
     for (int q = tid; q < quads; q += kSaThreads) {
-      float s[4], l[4], e[4];
-      bool any;
-      if constexpr (CACHED) {
-        const float4 w = *reinterpret_cast<const float4*>(s_l + 4 * q);
-        s[0] = w.x; s[1] = w.y; s[2] = w.z; s[3] = w.w;
-        any = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) >= near;
-        if (!any) continue;
-        fetch(q, l);
-        if (!greedy) exponentials(q, e);
-      } else {
-        fetch(q, l);
-        if (!greedy) exponentials(q, e);
+      float l[4], e[4] = {1.f, 1.f, 1.f, 1.f};
+      logits4(q, l);
+      if (!greedy) exponentials(v0 + 4 * q, e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float gap = l[i] == M ? 0.f : l[i] - M;
-          s[i] = !(l[i] > -INFINITY) || key_of(l[i], v0 + 4 * q + i) < bound ? -INFINITY : greedy ? l[i] : (gap == 0.f ? 0.f : gap * inv) - __logf(e[i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!(s[i] >= near)) continue;
-        const double w = l[i] == M ? 0.0 : ((double)l[i] - (double)M) / (greedy ? 1.0 : (double)T);
-        const double exact = greedy ? w : w - log((double)e[i]);
-        const int v = v0 + 4 * q + i;
-        if (index == 0x7fffffff || exact > score || (exact == score && v < index)) { score = exact; weight = w; index = v; }
-      }
+      for (int i = 0; i < 4; ++i)
+        if (kept(l[i], v0 + 4 * q + i)) weigh(l[i], e[i], v0 + 4 * q + i);
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double os = __shfl_xor_sync(0xffffffffu, score, o), ow = __shfl_xor_sync(0xffffffffu, weight, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, index, o);
-    if (oi != 0x7fffffff && (index == 0x7fffffff || os > score || (os == score && oi < index))) { score = os; weight = ow; index = oi; }
+  const float mine = best;
+  // the warp's, then the warps'
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) {
+      const float ob = __shfl_xor_sync(0xffffffffu, best, o), ol = __shfl_xor_sync(0xffffffffu, best_l, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, index, o);
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (ob > best || (ob == best && oi < index)) { best = ob; best_l = ol; index = oi; }
+    }
+    if (half == 0) {
+      if (lane == 0) { s_top[warp] = best; s_l_of[warp] = best_l; s_index[warp] = index; s_sum[warp] = sum; }
+      __syncthreads();
+      const bool there = lane < kSaWarps;
+      best = there ? s_top[lane] : -INFINITY;
+      best_l = there ? s_l_of[lane] : 0.f;
+      index = there ? s_index[lane] : 0x7fffffff;
+      sum = there ? s_sum[lane] : 0ull;
+    }
+  }
+  // ---- others that come close to the slice's best: in 64 bits, of equal ones the lowest token ----
+  auto exact_score = [&](float l, float e) { return (l == M ? 0.0 : ((double)l - (double)M) / (double)T) - log((double)e); };
+  const float near = best - kNear;
+  if (!greedy && best > -INFINITY) {
+    const int close = (mine >= near) + (second >= near);
+    if (close) atomicAdd(&s_close, close);
   }
   __syncthreads();
-  if (lane == 0) { s_redd[warp] = score; s_redi[warp] = index; s_weights[warp] = weight; }
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 16; ++w)
-      if (s_redi[w] != 0x7fffffff && (index == 0x7fffffff || s_redd[w] > score || (s_redd[w] == score && s_redi[w] < index))) {
-        score = s_redd[w]; weight = s_weights[w]; index = s_redi[w];
-      }
-    s_score = score; s_weight = weight; s_index = index; s_sum = all;
-  }
-  cluster_barrier();
-  if (rank == 0 && tid == 0) {
-    for (uint32_t c = 1; c < ctas; ++c) {
-      int oi;
-      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(oi) : "r"(remote(&s_index, c)) : "memory");
-      const double os = remote_f64(&s_score, c);
-      all += remote_f64(&s_sum, c);
-      if (oi != 0x7fffffff && (index == 0x7fffffff || os > score || (os == score && oi < index))) { score = os; weight = remote_f64(&s_weight, c); index = oi; }
-    }
-    const bool none = index == 0x7fffffff;   // nothing is allowed
-    const int64_t tok = none ? -1 : index;
-    if (a.token64) reinterpret_cast<int64_t*>(a.token)[b] = tok;
-    else reinterpret_cast<int32_t*>(a.token)[b] = (int32_t)tok;
-    if (a.logprob) a.logprob[b] = none ? -INFINITY : (float)(weight - log(all));
-    if (a.rng) a.rng[2 * b + 1] = (int64_t)(offset + 1ull);
-    if (a.count && !none) a.count[(int64_t)b * r.counts_ld + tok] += 1;
-    if (a.pos) {
-      const int64_t np = (a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[b] : (int64_t)reinterpret_cast<const int32_t*>(a.pos)[b]) + 1;
-      if (a.pos64) reinterpret_cast<int64_t*>(a.pos)[b] = np;
-      else reinterpret_cast<int32_t*>(a.pos)[b] = (int32_t)np;
-      if (a.history && np >= 0 && np < a.history_len) {
-        if (a.token64) reinterpret_cast<int64_t*>(a.history)[(int64_t)b * a.history_ld + np] = tok;
-        else reinterpret_cast<int32_t*>(a.history)[(int64_t)b * a.history_ld + np] = (int32_t)tok;
+  if (s_close > 1) {
+    double score = -INFINITY;
+    best_l = 0.f;
+    index = 0x7fffffff;
+    auto rival = [&](float l, float e, int v) {
+      if (!kept(l, v) || !(score_of(l, e) >= near)) return;
+      const double x = exact_score(l, e);
+      if (x > score || index == 0x7fffffff || (x == score && v < index)) { score = x; best_l = l; index = v; }
+    };
+    if (alone) {
+#pragma unroll 1
+      for (uint32_t i = tid; i < gathered; i += kSaThreads) rival(s_gl[i], s_ge[i], s_gv[i]);
+    } else {
+#pragma unroll 1
+      for (int q = tid; q < quads; q += kSaThreads) {
+        float l[4], e[4];
+        logits4(q, l);
+        exponentials(v0 + 4 * q, e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rival(l[i], e[i], v0 + 4 * q + i);
       }
     }
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll 1
+      for (int o = 16; o > 0; o >>= 1) {
+        const double ox = __shfl_xor_sync(0xffffffffu, score, o);
+        const float ol = __shfl_xor_sync(0xffffffffu, best_l, o);
+        const int oi = __shfl_xor_sync(0xffffffffu, index, o);
+        if (oi != 0x7fffffff && (index == 0x7fffffff || ox > score || (ox == score && oi < index))) { score = ox; best_l = ol; index = oi; }
+      }
+      if (half == 0) {
+        if (lane == 0) { s_exact[warp] = score; s_l_of[warp] = best_l; s_index[warp] = index; }
+        __syncthreads();
+        score = lane < kSaWarps ? s_exact[lane] : -INFINITY;
+        best_l = lane < kSaWarps ? s_l_of[lane] : 0.f;
+        index = lane < kSaWarps ? s_index[lane] : 0x7fffffff;
+      }
+    }
   }
-  cluster_barrier();   // no CTA leaves before its shared memory was read
+
+  // ---- the first CTA's first warp takes the slices' results ----
+  if (!alone && ctas > 1) {
+    if (tid == 0) {
+      remote_store(&s_all[rank][0], 0, __float_as_uint(best));
+      remote_store(&s_all[rank][1], 0, (uint32_t)index);
+      remote_store(&s_all[rank][2], 0, __float_as_uint(best_l));
+      remote_store(&s_all[rank][3], 0, (uint32_t)sum);
+      remote_store(&s_all[rank][4], 0, (uint32_t)(sum >> 32));
+    }
+    cluster_barrier();   // (behind it no CTA reads or writes another's shared memory)
+    if (rank != 0 || warp != 0) return;
+    const bool there = lane < (int)ctas;
+    best = there ? __uint_as_float(s_all[lane & 7][0]) : -INFINITY;
+    index = there ? (int)s_all[lane & 7][1] : 0x7fffffff;
+    best_l = there ? __uint_as_float(s_all[lane & 7][2]) : 0.f;
+    sum = there ? (uint64_t)s_all[lane & 7][3] | (uint64_t)s_all[lane & 7][4] << 32 : 0ull;
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float most = warp_max(best);
+    const unsigned rivals = __ballot_sync(0xffffffffu, index != 0x7fffffff && (greedy ? best == most : best >= most - kNear));
+    bool wins = rivals >> lane & 1u;
+    if (rivals & (rivals - 1u)) {
+      double score = -INFINITY;
+      if (wins) score = greedy ? 0.0 : exact_score(best_l, exponential(index));
+      double highest = score;
+#pragma unroll 1
+      for (int o = 16; o > 0; o >>= 1) {
+        const double ox = __shfl_xor_sync(0xffffffffu, highest, o);
+        highest = ox > highest ? ox : highest;
+      }
+      wins = wins && score == highest;
+      const int lowest = __reduce_min_sync(0xffffffffu, wins ? index : 0x7fffffff);
+      wins = wins && index == lowest;
+    }
+    const unsigned winner = __ballot_sync(0xffffffffu, wins);
+    const int from = winner ? __ffs(winner) - 1 : 0;
+    index = __shfl_sync(0xffffffffu, index, from);
+    best_l = __shfl_sync(0xffffffffu, best_l, from);
+  }
+  if (tid != 0) return;
+  const bool none = index == 0x7fffffff;   // nothing is allowed
+  const int64_t tok = none ? -1 : index;
+  if (a.token64) reinterpret_cast<int64_t*>(a.token)[b] = tok;
+  else reinterpret_cast<int32_t*>(a.token)[b] = (int32_t)tok;
+  if (a.logprob) a.logprob[b] = none ? -INFINITY : (best_l == M ? 0.f : (greedy ? best_l - M : (best_l - M) / T)) - logf(__ull2float_rn(sum) / unit);
+  if (a.rng) a.rng[2 * b + 1] = (int64_t)(offset + 1ull);
+  if (a.count && !none) a.count[(int64_t)b * r.counts_ld + tok] += 1;
+  if (a.pos) {
+    const int64_t np = (a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[b] : (int64_t)reinterpret_cast<const int32_t*>(a.pos)[b]) + 1;
+    if (a.pos64) reinterpret_cast<int64_t*>(a.pos)[b] = np;
+    else reinterpret_cast<int32_t*>(a.pos)[b] = (int32_t)np;
+    if (a.history && np >= 0 && np < a.history_len) {
+      if (a.token64) reinterpret_cast<int64_t*>(a.history)[(int64_t)b * a.history_ld + np] = tok;
+      else reinterpret_cast<int32_t*>(a.history)[(int64_t)b * a.history_ld + np] = (int32_t)tok;
+    }
+  }
 }
 
-constexpr int kSaMaxSlice = 48 * 1024;   // floats: 192 KB beside 17 KB of histograms
+constexpr int kSaMaxSlice = 47 * 1024;   // floats: 188 KB beside 33 KB of histograms and gathered tokens
 
-template <typename LT>
-cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
-  int ctas = 1;
-  while (ctas < 8 && (r.rows * ctas < 2 * sm_count() || (r.vocab + ctas - 1) / ctas > kSaMaxSlice) && r.vocab / ctas > 2048) ctas *= 2;
-  a.slice = ((r.vocab + ctas - 1) / ctas + 3) & ~3;
-  const bool cached = a.slice <= kSaMaxSlice;
-  const size_t smem = cached ? (size_t)a.slice * sizeof(float) : 0;
-  if (cached) {
+template <typename LT, bool CACHED, bool WIDE>
+cudaError_t launch_draw_as(const Rules& r, const DrawArgs& a, int ctas, cudaStream_t st) {
+  if (CACHED) {
     static PerDeviceOnce once;
     if (once.need()) {
-      const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<LT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSaMaxSlice * (int)sizeof(float));
+      const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<LT, CACHED, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSaMaxSlice * (int)sizeof(float));
       if (e != cudaSuccess) return e;
       once.done();
     }
-    return launch_cluster(sample_rows_kernel<LT, true>, dim3((unsigned)(r.rows * ctas)), dim3(kSaThreads), ctas, smem, st, r, a);
   }
-  return launch_cluster(sample_rows_kernel<LT, false>, dim3((unsigned)(r.rows * ctas)), dim3(kSaThreads), ctas, smem, st, r, a);
+  return launch_cluster(sample_rows_kernel<LT, CACHED, WIDE>, dim3((unsigned)(r.rows * ctas)), dim3(kSaThreads), ctas, CACHED ? (size_t)a.slice * sizeof(float) : 0, st, r, a);
+}
+
+template <typename LT>
+cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
+  // two CTAs an SM, as far as a cluster and slices of 2048 tokens allow; more where the slices would not fit shared memory
+  int ctas = 2 * sm_count() / r.rows;
+  ctas = ctas < r.vocab / 2048 ? ctas : r.vocab / 2048;
+  const int least = (r.vocab + kSaMaxSlice - 1) / kSaMaxSlice;
+  ctas = ctas > least ? ctas : least;
+  ctas = ctas < 1 ? 1 : ctas > kSaCtas ? kSaCtas : ctas;
+  a.slice = ((r.vocab + ctas - 1) / ctas + 3) & ~3;
+  // four tokens an access where every row of everything that is there begins on such a boundary
+  auto whole = [&](const void* p, int64_t ld, int bytes) { return !p || (((uintptr_t)p & (4 * bytes - 1)) == 0 && (r.rows == 1 || (ld & 3) == 0)); };
+  const bool wide = whole(r.logits, r.ld, (int)sizeof(LT)) && whole(r.counts, r.counts_ld, 4) && whole(r.bias, r.bias_ld, 4) && whole(a.noise, a.noise_ld, 4);
+  if (a.slice > kSaMaxSlice) return launch_draw_as<LT, false, false>(r, a, ctas, st);
+  return wide ? launch_draw_as<LT, true, true>(r, a, ctas, st) : launch_draw_as<LT, true, false>(r, a, ctas, st);
 }
 
 int check_rules(const b200_logit_rules* a, const char* what, Rules* out) {
