@@ -6,7 +6,7 @@
 //   kept   : the top_k largest l of a row, equal ones in the order of the tokens; never one of -inf
 //   token  : argmax over the kept ones of (l - max) / T - ln e,  e ~ Exp(1) from the row's own Philox state or a caller-given row;  T <= 0: argmax of l
 //   logprob: (l_token - max) / T - ln sum over the kept ones of exp((l - max) / T)      (T <= 0: over all, as with T = 1)
-// The adjusted logits are compared as the fp32 numbers that they are.  The winner is found in fp32 and, among those within 1e-3 of it (rounding of a score
+// The adjusted logits are compared as the fp32 numbers that they are.  The winner is found in fp32 and, among those that come within 1e-3 of it (rounding of a score
 // near the top: 4e-5 at most), in 64 bits, so that it is the argmax of the formula, the lowest token of equal ones.
 #include "philox.cuh"
 
@@ -76,27 +76,42 @@ struct RowRules {
         if (!((w >> e) & 1u)) l[e] = -INFINITY;
     }
   }
-  // N tokens first, first + step, .., those below `end`; everything is on its way before any of it is used
-  template <int N>
-  __device__ __forceinline__ void some(int first, int step, int end, float (&l)[N]) const {
+  // N tokens v, v + STEP, ..; with FULL all of them are there, else those below `end`.  Everything is on its way before any of it is used.
+  template <int N, int STEP, bool FULL>
+  __device__ __forceinline__ void some(int v, int end, float (&l)[N]) const {
     int n[N];
     float add[N];
-    uint32_t word[N];
+    bool out[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int v = first + i * step;
-      const bool in = v < end;
-      l[i] = in ? load_as_float<LT>(logits, v) : -INFINITY;
-      n[i] = in && counts ? counts[v] : 0;
-      add[i] = in && bias ? bias[v] : 0.f;
-      word[i] = in && allowed ? allowed[v >> 5] >> (v & 31) : 1u;
+      l[i] = FULL || v + i * STEP < end ? load_as_float<LT>(logits + v, i * STEP) : -INFINITY;
+      n[i] = 0;
+      add[i] = 0.f;
+      out[i] = false;
+    }
+    if (counts) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || v + i * STEP < end) n[i] = (counts + v)[i * STEP];
+    }
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || v + i * STEP < end) add[i] = (bias + v)[i * STEP];
+    }
+    if (allowed) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || v + i * STEP < end) out[i] = STEP % 32 == 0 ? !((allowed + (v >> 5))[i * (STEP / 32)] >> (v & 31) & 1u) : !(allowed[(v + i * STEP) >> 5] >> ((v + i * STEP) & 31) & 1u);
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      l[i] = penalised(l[i], n[i]);
-      if (bias) l[i] = __fadd_rn(l[i], add[i]);
-      if (!(word[i] & 1u)) l[i] = -INFINITY;
+    for (int i = 0; i < N; ++i) l[i] = penalised(l[i], n[i]);
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) l[i] = __fadd_rn(l[i], add[i]);
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) l[i] = out[i] ? -INFINITY : l[i];
   }
   __device__ __forceinline__ bool wide() const {
     return ((reinterpret_cast<uintptr_t>(logits) & (4 * sizeof(LT) - 1)) | ((reinterpret_cast<uintptr_t>(counts) | reinterpret_cast<uintptr_t>(bias)) & 15)) == 0;
@@ -138,9 +153,13 @@ __global__ void __launch_bounds__(kAdjThreads) adjust_kernel(const Rules r, OT* 
 
 // ---- the draw -----------------------------------------------------------------------------------------------------------------------
 // A row's tokens are cut into the slices of a cluster's CTAs; a slice's adjusted logits stay in shared memory (CACHED) and are read again by the later steps.
-constexpr int kSaThreads = 512, kSaWarps = kSaThreads / 32, kSaBins = 2 * kSaThreads, kSaDigit = 10, kSaCtas = 8;
-constexpr int kSaGather = 2048;   // tokens that one CTA goes on with alone
-constexpr float kNear = 1e-3f;    // scores this close to the best are compared in 64 bits
+// NT threads a CTA: 512 while rows are few, 256, of which three CTAs fit an SM, where they fill the GPU.
+constexpr int kSaDigit = 10, kSaBins = 1 << kSaDigit, kSaCtas = 8;
+constexpr int kSaGather = 1024;   // tokens that one CTA goes on with alone
+constexpr float kNear = 1.5e-3f;  // scores, in powers of two, this close to the best are compared in 64 bits
+
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float lg2(float x) { float r; asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
 struct DrawArgs {
   const float* temperature; float temperature_all;
@@ -167,10 +186,10 @@ __device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 remote_u2(const void* p, uint32_t rank) {
-  uint2 v;
-  asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(remote(p, rank)) : "memory");
-  return v;
+template <int N>
+__device__ __forceinline__ void remote_bins(const uint32_t* p, uint32_t rank, uint32_t (&v)[N]) {
+  if constexpr (N == 4) asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[N - 1]) : "r"(remote(p, rank)) : "memory");
+  else asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(remote(p, rank)) : "memory");
 }
 __device__ __forceinline__ void remote_store(const void* p, uint32_t rank, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
@@ -182,33 +201,44 @@ __device__ __forceinline__ uint32_t remote_add(const void* p, uint32_t rank, uin
 }
 
 // Where counts, from bin 0 on or with DOWN from the last bin on, come to `left`: the bin, what is left of `left` in it, what it holds (0xffffffff: nowhere).  n: the
-// counts of bins 2 i and 2 i + 1, DOWN counted from the last, with i the thread.  All threads call it; true in the one whose bin it is.
-template <bool DOWN>
-__device__ __forceinline__ bool find_bin(const uint2& n, uint32_t left, uint32_t* s_warp, uint32_t (&s_found)[3]) {
+// counts of the thread's own bins, of as many neighbours a thread.  All threads call it; true in the one whose bin it is.
+template <int NT, bool DOWN>
+__device__ __forceinline__ bool find_bin(const uint32_t (&n)[kSaBins / NT], uint32_t left, uint32_t* s_warp, uint32_t (&s_found)[3]) {
+  constexpr int N = kSaBins / NT;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t c0 = DOWN ? n.y : n.x, c1 = DOWN ? n.x : n.y, total = c0 + c1;
+  uint32_t total = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) total += n[i];
   uint32_t inc = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
   if (lane == 31) s_warp[warp] = inc;
   if (tid == 0) s_found[0] = 0xffffffffu;
   __syncthreads();
-  uint32_t sum = lane < kSaWarps && lane < warp ? s_warp[lane] : 0u;
+  uint32_t sum = lane < NT / 32 && lane < warp ? s_warp[lane] : 0u;
   sum = __reduce_add_sync(0xffffffffu, sum) + inc - total;
   const bool mine = sum < left && sum + total >= left;   // one thread at most
   if (mine) {
-    const bool second = sum + c0 < left;
-    const int bin = 2 * tid + second;
-    s_found[0] = (uint32_t)(DOWN ? kSaBins - 1 - bin : bin);
-    s_found[1] = left - sum - (second ? c0 : 0u);
-    s_found[2] = second ? c1 : c0;
+    int at = -1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t c = n[DOWN ? N - 1 - i : i];
+      if (at < 0 && sum + c >= left) {
+        at = i;
+        s_found[1] = left - sum;
+        s_found[2] = c;
+      }
+      sum += at < 0 ? c : 0u;
+    }
+    s_found[0] = (uint32_t)(DOWN ? kSaBins - 1 - (N * tid + at) : N * tid + at);
   }
   __syncthreads();
   return mine;
 }
 
-template <typename LT, bool CACHED, bool WIDE>
-__global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules r, const DrawArgs a) {
+template <typename LT, bool CACHED, bool WIDE, int NT>
+__global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(const Rules r, const DrawArgs a) {
+  constexpr int kSaThreads = NT, kSaWarps = NT / 32, N = kSaBins / NT;
   extern __shared__ __align__(16) float s_l[];                       // the slice's adjusted logits
   __shared__ __align__(16) uint32_t s_hist[2][kSaBins];
   __shared__ uint32_t s_warp[kSaWarps], s_found[3], s_ties[kSaCtas], s_gathered;
@@ -222,7 +252,8 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cta_rank(), ctas = cta_count();
   const int b = blockIdx.x / ctas;
-  *reinterpret_cast<uint2*>(s_hist[0] + 2 * tid) = make_uint2(0u, 0u);
+#pragma unroll
+  for (int i = 0; i < N; ++i) s_hist[0][N * tid + i] = 0u;
   if (tid == 0) { s_close = 0; s_gathered = 0u; }
   griddep_launch();
   griddep_wait();
@@ -243,17 +274,22 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
       const float4 w = *reinterpret_cast<const float4*>(s_l + 4 * q);
       l[0] = w.x; l[1] = w.y; l[2] = w.z; l[3] = w.w;
     } else {
-      row.some(v0 + 4 * q, 1, v0 + n, l);
+      row.template some<4, 1, false>(v0 + 4 * q, v0 + n, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) l[e] = clean(l[e]);
     }
   };
-  // e of four tokens: between 0 and the largest number
+  // e of four tokens: at most the largest number
   auto exponentials = [&](int v, float (&e)[4]) {
     if (noise) {
-      if (WIDE && v + 3 < V) {
-        const float4 w = *reinterpret_cast<const float4*>(noise + v);
-        e[0] = w.x; e[1] = w.y; e[2] = w.z; e[3] = w.w;
+      if (v + 3 < V) {
+        if constexpr (WIDE) {
+          const float4 w = *reinterpret_cast<const float4*>(noise + v);
+          e[0] = w.x; e[1] = w.y; e[2] = w.z; e[3] = w.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = (noise + v)[i];
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = v + i < V ? noise[v + i] : 1.f;
@@ -265,7 +301,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
       for (int i = 0; i < 4; ++i) e[i] = -__logf(((float)(rnd[i] >> 8) + 0.5f) * (1.0f / 16777216.0f));
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = fmaxf(fminf(e[i], 3.4028234e38f), 0.f);
+    for (int i = 0; i < 4; ++i) e[i] = fminf(e[i], 3.4028234e38f);
   };
   auto exponential = [&](int v) {
     float e[4];
@@ -276,34 +312,38 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
 
   // ---- adjusted logits, their maximum, the first digit's histogram ----
   float top = -INFINITY;
-  auto see = [&](float l) {
-    top = fmaxf(top, l);
-    if (select && l > -INFINITY) atomicAdd(&s_hist[0][order_key(l) >> (32 - kSaDigit)], 1u);
+  auto see = [&](const auto& l) {
+    if (select) {
+      for (const float x : l)
+        if (x > -INFINITY) atomicAdd(&s_hist[0][order_key(x) >> (32 - kSaDigit)], 1u);
+    }
   };
   if constexpr (CACHED && WIDE) {
 #pragma unroll 2
     for (int q = tid; q < quads; q += kSaThreads) {
       float l[4];
       if (v0 + 4 * q + 3 < V) row.at4(v0 + 4 * q, l);
-      else row.some(v0 + 4 * q, 1, v0 + n, l);
+      else row.template some<4, 1, false>(v0 + 4 * q, v0 + n, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) l[e] = clean(l[e]);
       *reinterpret_cast<float4*>(s_l + 4 * q) = make_float4(l[0], l[1], l[2], l[3]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) see(l[e]);
+      top = fmaxf(fmaxf(top, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
+      see(l);
     }
   } else {
-    constexpr int N = 8;
-    for (int i0 = tid; i0 < 4 * quads; i0 += N * kSaThreads) {
-      float l[N];
-      row.some(v0 + i0, kSaThreads, v0 + n, l);
+    constexpr int E = 8;
+    for (int i0 = tid; i0 < 4 * quads; i0 += E * NT) {
+      float l[E];
+      if (i0 + (E - 1) * NT < n) row.template some<E, NT, true>(v0 + i0, v0 + n, l);
+      else row.template some<E, NT, false>(v0 + i0, v0 + n, l);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int i = i0 + e * kSaThreads;
+      for (int e = 0; e < E; ++e) {
+        const int i = i0 + e * NT;
         l[e] = clean(l[e]);
         if (CACHED && i < 4 * quads) s_l[i] = l[e];
-        see(l[e]);
+        top = fmaxf(top, l[e]);
       }
+      see(l);
     }
   }
   top = warp_max(top);
@@ -350,20 +390,29 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
         }
       }
       // every CTA adds the histograms up, the highest bins first
-      const int first = kSaBins - 2 * (tid + 1);
-      uint2 m[kSaCtas], sum = make_uint2(0u, 0u);
+      const int first = kSaBins - N * (tid + 1);
+      uint32_t m[kSaCtas][N], sum[N] = {};
       if (alone) {
-        sum = *reinterpret_cast<const uint2*>(hist + first);
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = hist[first + i];
       } else {
 #pragma unroll
-        for (uint32_t c = 0; c < kSaCtas; ++c) m[c] = c < ctas ? remote_u2(hist + first, c) : make_uint2(0u, 0u);
+        for (uint32_t c = 0; c < kSaCtas; ++c)
+          if (c < ctas) remote_bins(hist + first, c, m[c]);
 #pragma unroll
-        for (uint32_t c = 0; c < kSaCtas; ++c) { sum.x += m[c].x; sum.y += m[c].y; }
+        for (uint32_t c = 0; c < kSaCtas; ++c)
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[i] += c < ctas ? m[c][i] : 0u;
       }
-      *reinterpret_cast<uint2*>(s_hist[(pass & 1) ^ 1] + first) = make_uint2(0u, 0u);   // (read by all before they came to the barrier)
-      if (find_bin<true>(sum, left, s_warp, s_found) && !alone) {
 #pragma unroll
-        for (uint32_t c = 0; c < kSaCtas; ++c) s_ties[c] = s_found[0] & 1u ? m[c].y : m[c].x;
+      for (int i = 0; i < N; ++i) s_hist[(pass & 1) ^ 1][first + i] = 0u;   // (read by all before they came to the barrier)
+      if (find_bin<NT, true>(sum, left, s_warp, s_found) && !alone) {
+        const int at = (int)s_found[0] - first;
+#pragma unroll
+        for (uint32_t c = 0; c < kSaCtas; ++c)
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (i == at && c < ctas) s_ties[c] = m[c][i];
       }
       __syncthreads();
       const uint32_t bin = s_found[0], in_bin = s_found[2];
@@ -374,20 +423,34 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
       low = shift;
       if (in_bin == left && (alone || pass > 0)) break;           // the bin's are all kept
       if (pass == 0 && above + in_bin <= (uint32_t)kSaGather) {
-        // few: the first CTA takes them all
+        // few: the first CTA takes them all; a warp finds out how many it has and asks for as many places
+        auto goes = [&](float l) { return l > -INFINITY && order_key(l) >> shift >= bin; };
+        int have = 0;
 #pragma unroll 1
-        for (int q = tid; q < quads; q += kSaThreads) {
+        for (int q = tid; q < quads; q += NT) {
+          float l[4];
+          logits4(q, l);
+          have += goes(l[0]) + goes(l[1]) + goes(l[2]) + goes(l[3]);
+        }
+        int upto = have;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += t; }
+        uint32_t at = 0u;
+        if (lane == 31 && upto > 0) at = remote_add(&s_gathered, 0, (uint32_t)upto);
+        at = __shfl_sync(0xffffffffu, at, 31) + (uint32_t)(upto - have);
+#pragma unroll 1
+        for (int q = tid; have > 0 && q < quads; q += NT) {
           float l[4];
           logits4(q, l);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (l[e] > -INFINITY && order_key(l[e]) >> shift >= bin) {
+            if (goes(l[e])) {
               const int v = v0 + 4 * q + e;
-              const uint32_t at = remote_add(&s_gathered, 0, 1u);
-              const float x = exponential(v);
               remote_store(s_gl + at, 0, __float_as_uint(l[e]));
-              remote_store(s_ge + at, 0, __float_as_uint(x));
               remote_store(s_gv + at, 0, (uint32_t)v);
+              remote_store(s_ge + at, 0, __float_as_uint(exponential(v)));
+              ++at;
+              --have;
             }
         }
         M = warp_max(M);
@@ -434,9 +497,10 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
                 }
               }
               __syncthreads();
-              const uint2 h = *reinterpret_cast<const uint2*>(local + 2 * tid);
-              *reinterpret_cast<uint2*>(local + 2 * tid) = make_uint2(0u, 0u);
-              find_bin<false>(h, want, s_warp, s_found);
+              uint32_t h[N];
+#pragma unroll
+              for (int i = 0; i < N; ++i) { h[i] = local[N * tid + i]; local[N * tid + i] = 0u; }
+              find_bin<NT, false>(h, want, s_warp, s_found);
               token |= (int)(s_found[0] << at);
               want = s_found[1];
               __syncthreads();
@@ -455,39 +519,35 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
   if (!alone) M = warp_max(M);
   auto kept = [&](float l, int v) {
     const uint32_t key = order_key(l) >> low, edge = bound >> low;
-    return l > -INFINITY && (key > edge || (key == edge && v <= cut));
+    return l > -INFINITY && (!select || key > edge || (key == edge && v <= cut));
   };
 
   // ---- weights and scores; a thread's best and whether another of its own comes close ----
-  // Weights are added as whole numbers, so that the sum does not depend on the order that tokens were gathered in.
-  const float inv = greedy ? 1.f : 1.f / T, inv2 = inv * 1.4426950408889634f, unit = __int_as_float((127 + __clz(V)  + 30) << 23);   // 2^(30 + leading zeros): V of them stay below 2^63
-  auto score_of = [&](float l, float e) {
-    const float w = l == M ? 0.f : (l - M) * inv;
-    return greedy ? l : w > -INFINITY ? w - __logf(e) : -INFINITY;
-  };
+  // What threads have is added as whole numbers, and gathered tokens each: the sum does not depend on the order that they were gathered in.
+  const float inv2 = fminf((greedy ? 1.f : 1.f / T) * 1.4426950408889634f, 3.4028234e38f);
+  const float unit = __int_as_float((127 + __clz(V) + 30) << 23);   // 2^(30 + leading zeros): V of them stay below 2^63
+  auto power_of = [&](float l) { return (l == M ? 0.f : l - M) * inv2; };
+  auto score_of = [&](float l, float e) { return greedy ? l : power_of(l) - lg2(e); };
   uint64_t sum = 0ull;
   float best = -INFINITY, second = -INFINITY, best_l = 0.f;
   int index = 0x7fffffff;
   auto weigh = [&](float l, float e, int v) {
-    const float gap = l == M ? 0.f : l - M;
-    sum += __float2ull_rz((gap == 0.f ? 1.f : exp2f(gap * inv2)) * unit);
-    const float s = score_of(l, e);
-    if (s > best || index == 0x7fffffff || (s == best && v < index)) {
-      second = best;
-      best = s;
-      best_l = l;
-      index = v;
-    } else {
-      second = fmaxf(second, s);
-    }
+    const float power = power_of(l), s = greedy ? l : power - lg2(e);
+    const bool first = s > best;      // (the tokens of a slice come to a thread in their order)
+    second = fmaxf(second, first ? best : s);
+    best = first ? s : best;
+    best_l = first ? l : best_l;
+    index = first ? v : index;
+    return ex2(power);
   };
   if (alone) {
 #pragma unroll 1
     for (uint32_t i = tid; i < gathered; i += kSaThreads) {
       const float l = s_gl[i];
-      if (kept(l, s_gv[i])) weigh(l, s_ge[i], s_gv[i]);
+      if (kept(l, s_gv[i])) sum += __float2ull_rz(weigh(l, s_ge[i], s_gv[i]) * unit);
     }
   } else if (M > -INFINITY) {
+    float part = 0.f;
 #pragma unroll 2
     for (int q = tid; q < quads; q += kSaThreads) {
       float l[4], e[4] = {1.f, 1.f, 1.f, 1.f};
@@ -495,8 +555,9 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
       if (!greedy) exponentials(v0 + 4 * q, e);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (kept(l[i], v0 + 4 * q + i)) weigh(l[i], e[i], v0 + 4 * q + i);
+        if (select ? kept(l[i], v0 + 4 * q + i) : l[i] > -INFINITY) part += weigh(l[i], e[i], v0 + 4 * q + i);
     }
+    sum = __float2ull_rz(part * unit);
   }
   const float mine = best;
   // the warp's, then the warps'
@@ -521,7 +582,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
   }
   // ---- others that come close to the slice's best: in 64 bits, of equal ones the lowest token ----
   auto exact_score = [&](float l, float e) { return (l == M ? 0.0 : ((double)l - (double)M) / (double)T) - log((double)e); };
-  const float near = best - kNear;
+  const float near = greedy ? best : best - kNear;
   if (!greedy && best > -INFINITY) {
     const int close = (mine >= near) + (second >= near);
     if (close) atomicAdd(&s_close, close);
@@ -626,25 +687,26 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Rules 
   }
 }
 
-constexpr int kSaMaxSlice = 47 * 1024;   // floats: 188 KB beside 33 KB of histograms and gathered tokens
+constexpr int kSaMaxSlice = 48 * 1024;   // floats: 192 KB beside 21 KB of histograms and gathered tokens
 
-template <typename LT, bool CACHED, bool WIDE>
+template <typename LT, bool CACHED, bool WIDE, int NT>
 cudaError_t launch_draw_as(const Rules& r, const DrawArgs& a, int ctas, cudaStream_t st) {
   if (CACHED) {
     static PerDeviceOnce once;
     if (once.need()) {
-      const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<LT, CACHED, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSaMaxSlice * (int)sizeof(float));
+      const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<LT, CACHED, WIDE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSaMaxSlice * (int)sizeof(float));
       if (e != cudaSuccess) return e;
       once.done();
     }
   }
-  return launch_cluster(sample_rows_kernel<LT, CACHED, WIDE>, dim3((unsigned)(r.rows * ctas)), dim3(kSaThreads), ctas, CACHED ? (size_t)a.slice * sizeof(float) : 0, st, r, a);
+  return launch_cluster(sample_rows_kernel<LT, CACHED, WIDE, NT>, dim3((unsigned)(r.rows * ctas)), dim3(NT), ctas, CACHED ? (size_t)a.slice * sizeof(float) : 0, st, r, a);
 }
 
 template <typename LT>
 cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
-  // two CTAs an SM, as far as a cluster and slices of 2048 tokens allow; more where the slices would not fit shared memory
-  int ctas = 2 * sm_count() / r.rows;
+  // few rows: clusters of eight CTAs of 512 threads, as far as slices of 2048 tokens allow.  Rows that fill the GPU: CTAs of 256 threads, three an SM
+  const bool few = r.rows * kSaCtas <= 2 * sm_count();
+  int ctas = few ? kSaCtas : 3 * sm_count() / r.rows;
   ctas = ctas < r.vocab / 2048 ? ctas : r.vocab / 2048;
   const int least = (r.vocab + kSaMaxSlice - 1) / kSaMaxSlice;
   ctas = ctas > least ? ctas : least;
@@ -653,8 +715,9 @@ cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
   // four tokens an access where every row of everything that is there begins on such a boundary
   auto whole = [&](const void* p, int64_t ld, int bytes) { return !p || (((uintptr_t)p & (4 * bytes - 1)) == 0 && (r.rows == 1 || (ld & 3) == 0)); };
   const bool wide = whole(r.logits, r.ld, (int)sizeof(LT)) && whole(r.counts, r.counts_ld, 4) && whole(r.bias, r.bias_ld, 4) && whole(a.noise, a.noise_ld, 4);
-  if (a.slice > kSaMaxSlice) return launch_draw_as<LT, false, false>(r, a, ctas, st);
-  return wide ? launch_draw_as<LT, true, true>(r, a, ctas, st) : launch_draw_as<LT, true, false>(r, a, ctas, st);
+  if (a.slice > kSaMaxSlice) return launch_draw_as<LT, false, false, 512>(r, a, ctas, st);
+  if (few) return wide ? launch_draw_as<LT, true, true, 512>(r, a, ctas, st) : launch_draw_as<LT, true, false, 512>(r, a, ctas, st);
+  return wide ? launch_draw_as<LT, true, true, 256>(r, a, ctas, st) : launch_draw_as<LT, true, false, 256>(r, a, ctas, st);
 }
 
 int check_rules(const b200_logit_rules* a, const char* what, Rules* out) {
