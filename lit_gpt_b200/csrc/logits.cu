@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
     for (int i = 0; i < 4; ++i) e[i] = fminf(e[i], 3.4028234e38f);
   };
   auto exponential = [&](int v) {
+    if (noise) return fminf(noise[v], 3.4028234e38f);
     float e[4];
     exponentials(v & ~3, e);
     const float lo = v & 1 ? e[1] : e[0], hi = v & 1 ? e[3] : e[2];
@@ -548,14 +549,44 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
     }
   } else if (M > -INFINITY) {
     float part = 0.f;
-#pragma unroll 2
-    for (int q = tid; q < quads; q += kSaThreads) {
-      float l[4], e[4] = {1.f, 1.f, 1.f, 1.f};
-      logits4(q, l);
-      if (!greedy) exponentials(v0 + 4 * q, e);
+    constexpr int G = 4;   // quads of a thread whose noise is on its way together
+#pragma unroll 1
+    for (int q0 = tid; q0 < quads; q0 += G * NT) {
+      float e[G][4];
+      const int last = q0 + (G - 1) * NT;
+      if (noise && !greedy && last < quads && v0 + 4 * last + 3 < V) {
+        const float* const from = noise + v0 + 4 * q0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (select ? kept(l[i], v0 + 4 * q + i) : l[i] > -INFINITY) part += weigh(l[i], e[i], v0 + 4 * q + i);
+        for (int g = 0; g < G; ++g) {
+          if constexpr (WIDE) {
+            const float4 w = *reinterpret_cast<const float4*>(from + g * 4 * NT);
+            e[g][0] = w.x; e[g][1] = w.y; e[g][2] = w.z; e[g][3] = w.w;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[g][i] = from[g * 4 * NT + i];
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[g][i] = fminf(e[g][i], 3.4028234e38f);
+      } else {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          e[g][0] = e[g][1] = e[g][2] = e[g][3] = 1.f;
+          if (!greedy && q0 + g * NT < quads) exponentials(v0 + 4 * (q0 + g * NT), e[g]);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int q = q0 + g * NT;
+        if (q >= quads) break;
+        float l[4];
+        logits4(q, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (select ? kept(l[i], v0 + 4 * q + i) : l[i] > -INFINITY) part += weigh(l[i], e[g][i], v0 + 4 * q + i);
+      }
     }
     sum = __float2ull_rz(part * unit);
   }
