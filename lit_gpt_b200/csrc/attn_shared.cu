@@ -648,8 +648,12 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
     s.pre_rows = s.pair ? 256 : 128;
     s.pre_tiles = (int)((rows + s.pre_rows - 1) / s.pre_rows);
     const int64_t items = (int64_t)n_groups * s.pre_tiles, ranges = ((int64_t)prefix_rows + 127) / 128;
-    s.splits = (int)(sm_count() / items < ranges ? sm_count() / items : ranges);
-    if (s.splits < 1) s.splits = 1;
+    // SMs for the prefix's kernel: the kernel of the own keys begins beside it on the others, so each has the share of SMs that its work asks for (own caches half full): a tile
+    // of 128 keys takes 2.15 us with 256 rows and @@ with 128, own keys come at 90 GB/s an SM.
+    const double prefix_work = (double)items * ranges * (s.pair ? 2.15 : 1.3), own_work = (double)batch * n_groups * own_rows * hs * 2 / 90e3;
+    const double share = sm_count() * prefix_work / (prefix_work + own_work) / items;
+    s.splits = share < 1.0 ? 1 : share < (double)ranges ? (int)(share + 0.5) : (int)ranges;
+    while (s.splits > 1 && s.splits * items > sm_count()) --s.splits;
     s.pre_parts = s.pair ? s.splits : 2 * s.splits;
     prefix_rows = 0;               // not in the list of tiles
   }
@@ -668,7 +672,8 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)(batch + 1) * sizeof(int);
   // results of a head: about those of a prefix item and of an own one
   const int64_t results = 2 + s.pre_parts + (int64_t)s.workers / (pre_items > 0 ? pre_items : own_items);
-  s.ways = results > 16 ? 8 : results > 8 ? 4 : results > 4 ? 2 : 1;   // four results a warp in one round
+  s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
+  while (s.ways < 8 && results > 4 * s.ways && (int64_t)batch * n_groups * per * s.ways < 24 * sm_count()) s.ways *= 2;
   return s;
 }
 

@@ -37,7 +37,8 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
 
 template <int HS, bool PAIR>
 __global__ void __launch_bounds__(kSpThreads, 1)
-attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int splits, unsigned* err) {
+attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                          int splits, unsigned* err) {
   using C = SpTile<HS>;
   extern __shared__ __align__(1024) uint8_t sp_smem[];
   __shared__ __align__(8) uint64_t s_bars[18];
@@ -63,7 +64,7 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
       tc::mbar_init(p_full + 8 * i, 4);
       tc::mbar_init(o_done + 8 * i, 1);
     }
-    tc::mbar_init(q_full, PAIR ? 8 : 4);
+    tc::mbar_init(q_full, 1);
     tc::mbar_init(idle, 1);
     tc::mbar_init_fence();
   }
@@ -88,9 +89,18 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
     const __nv_bfloat16* const src = keys ? p.kp + (int64_t)gi * p.kp_g : p.vp + (int64_t)gi * p.vp_g;
     const uint32_t dst = keys ? sk_ : sv_, full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
     if (lane == 0) tc::prefetch_map(keys ? &map_k : &map_v);
+    auto behind_the_wait = [&]() {
+      griddep_wait();
+      griddep_launch();
+      if (keys && n > 0 && tc::elect()) {
+        tc::mbar_expect_tx(q_full, (PAIR ? 2 : 1) * C::kBytes);
+#pragma unroll
+        for (int e = 0; e < (PAIR ? 2 : 1) * C::kPanels; ++e) load_box(sq_ + e * 16384u, &map_q, e % C::kPanels * 64, r0 + e / C::kPanels * 128, gi, q_full);
+      }
+    };
     int j = 0;
     for (; j < n; ++j) {
-      if (j == 2) { griddep_wait(); griddep_launch(); }
+      if (j == 1) behind_the_wait();
       const int s = j & 1, row = (first + j) * 128;
       ok = __all_sync(0xffffffffu, tc::mbar_wait(empty + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u));
       if (!ok) break;
@@ -108,9 +118,9 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
         if (lane == 0) tc::mbar_arrive(full + 8 * s);
       }
     }
-    griddep_wait();
-    griddep_launch();
+    if (n <= 1) behind_the_wait();
     // no copy may land after the CTA has left
+    if (keys && n > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(q_full, 0)) && ok;
     for (int i = max(j - 2, 0); i < j; ++i) ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * (i & 1), (uint32_t)(i >> 1) & 1u)) && ok;
   } else if (warp == 8) {
     // ================================ products ================================
@@ -181,13 +191,6 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
   } else {
     // ================================ softmax: a row per thread ================================
     const int t = warp >> 2, r = tid & 127, row = r0 + (PAIR ? tid : r);
-    if ((PAIR || t == 0) && n > 0) {
-      copy_tile<HS, 128>(sq_ + t * C::kBytes, p.q + (int64_t)gi * rows * HS, HS, r0 + t * 128, rows, r);
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      tc::fence_smem_async();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(q_full);
-    }
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + C::kS + t * 128, to = tmem + lanes + C::kO + t * HS;
     const float sl = p.scale_log2, room = 8.f / sl;
@@ -284,11 +287,12 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
     }
     const int64_t slot = PAIR ? ((int64_t)item * splits + split) * 256 + tid : (((int64_t)item * splits + split) * 2 + t) * 128 + r;
     if (steps > 0 && ok) {
-      // the row goes through shared memory, where nothing is read any more once both streams are done, and from there in one copy of the thread's own: stored from
-      // registers, a warp's 16 bytes of 32 rows take 32 sectors each
+      // The rows go through shared memory, where nothing is read any more once both streams are done, and from there a row at a time: stored from registers, a warp's
+      // 16 bytes of 32 rows take 32 sectors each; by a bulk copy of every thread's own row, 256 copies took 4500 clocks.
       ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, 0) && (!(PAIR || n > 1) || tc::mbar_wait(o_done + 8, 0)));
       tc::fence_after();
-      const uint32_t mine = smem + (uint32_t)tid * (HS * 4 + 16);
+      constexpr uint32_t LD = HS * 4 + 16;
+      const uint32_t mine = smem + (uint32_t)tid * LD;
 #pragma unroll 1
       for (int c = 0; c < HS && ok; c += 32) {
         uint32_t o[32];
@@ -298,10 +302,16 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
         for (int e = 0; e < 32; e += 4)
           asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(mine + (c + e) * 4), "r"(o[e]), "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3]) : "memory");
       }
-      tc::fence_smem_async();
-      if (row < rows && ok) {
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.pre_acc + slot * HS), "r"(mine), "n"(HS * 4) : "memory");
-        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+      constexpr int LR = HS / 4, R = 32 / LR;   // lanes a row, rows at once
+      const uint32_t from = smem + (uint32_t)(tid - lane + lane / LR) * LD + lane % LR * 16;
+      float* const acc = p.pre_acc + (slot - lane + lane / LR) * HS + lane % LR * 4;
+      const int there = ok ? rows - (row - lane) - lane / LR : 0;
+#pragma unroll 8
+      for (int i = 0; i < 32; i += R) {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from + i * LD));
+        if (i < there) __stcg(reinterpret_cast<uint4*>(acc + i * HS), v);
       }
     }
     if (row < rows) {
@@ -320,11 +330,11 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
   }
 }
 
-// [groups][rows][HS] in boxes of 128 rows x 64 numbers, 128-byte swizzle, zeros outside
+// [groups][rows][HS] in boxes of 128 rows x 64 numbers, 128-byte swizzle, zeros outside.  (Prefixes of fewer than 128 rows are not read through it.)
 bool prefix_map(CUtensorMap* map, const void* base, int hs, int rows, int groups, int64_t group_stride) {
   const TensorMapEncodeFn enc = tensor_map_encoder();
   if (!enc) return false;
-  const cuuint64_t dim[3] = {(cuuint64_t)hs, (cuuint64_t)(rows > 128 ? rows : 128), (cuuint64_t)groups};   // (shorter prefixes are not read through it)
+  const cuuint64_t dim[3] = {(cuuint64_t)hs, (cuuint64_t)rows, (cuuint64_t)groups};
   const cuuint64_t stride[2] = {(cuuint64_t)hs * 2, (cuuint64_t)(groups > 1 ? group_stride : (int64_t)rows * hs) * 2};
   const cuuint32_t box[3] = {64u, 128u, 1u}, step[3] = {1u, 1u, 1u};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -340,11 +350,11 @@ cudaError_t launch_prefix(const SharedParams& p, int splits, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     once.done();
   }
-  alignas(64) CUtensorMap mk, mv;
-  if (!prefix_map(&mk, p.kp, HS, p.prefix_rows, p.n_groups, p.kp_g) || !prefix_map(&mv, p.vp, HS, p.prefix_rows, p.n_groups, p.vp_g)) return cudaErrorInvalidValue;
+  alignas(64) CUtensorMap mq, mk, mv;
+  if (!prefix_map(&mq, p.q, HS, p.batch * p.per, p.n_groups, (int64_t)p.batch * p.per * HS) || !prefix_map(&mk, p.kp, HS, p.prefix_rows, p.n_groups, p.kp_g) || !prefix_map(&mv, p.vp, HS, p.prefix_rows, p.n_groups, p.vp_g)) return cudaErrorInvalidValue;
   unsigned* const err = wait_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  return launch(attn_shared_prefix_kernel<HS, PAIR>, dim3((unsigned)(p.n_groups * p.pre_tiles * splits)), dim3(kSpThreads), (size_t)smem, st, p, mk, mv, splits, err);
+  return launch(attn_shared_prefix_kernel<HS, PAIR>, dim3((unsigned)(p.n_groups * p.pre_tiles * splits)), dim3(kSpThreads), (size_t)smem, st, p, mq, mk, mv, splits, err);
 }
 
 }  // namespace
