@@ -5,12 +5,12 @@
 //
 // The prefix is read once for all rows: the B * (heads per group) query rows of a key-value group are the left operand of its products, a key tile serves them all.
 // Three launches: the queries and new keys are turned and the new rows stored; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys of the
-// prefix for up to 32 query rows of a group, and of a row's own keys for its heads of a group; a head's partial results are joined.  No counter or flag is left
+// prefix for up to 32 query rows of a group (more: attn_shared_tc05.cu), and of a row's own keys for its heads of a group; a head's partial results are joined.  No counter or flag is left
 // between calls, and two calls at a time share nothing.
 //
 // All tiles, of the prefix and of all rows' own keys, are one list that is cut evenly over the warps of all SMs, so that neither few rows over a long prefix nor many
 // rows of unequal lengths leave SMs without work.  A warp keeps a ring of units of 32 keys or values, two of them on their way, and the queries of its next item behind them.
-// S = Q K^T and O += P V on mma.sync.m16n8k16.  P enters as two bf16 numbers, its leading bits and the rest, so that its rounding does not add to the result's own (with the
+// S^T = K Q^T and O^T += V^T P^T on mma.sync.m16n8k16, eight queries a product.  P enters as two bf16 numbers, its leading bits and the rest, so that its rounding does not add to the result's own (with the
 // nearest bf16 number alone the error against 64 bits is a fifth larger than that of the final rounding).  The rest is taken of the number above the weight: it is
 // not zero, and an infinite value times it is infinite and not NaN.
 #include <math.h>
@@ -150,12 +150,12 @@ __device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int
   return split_of(p, plen, sums[THREADS]);
 }
 
-// A warp's shared memory: a ring of units, the queries of two items.  One CTA an SM.
-template <int HS, int MT>
+// A warp's shared memory: a ring of units, the queries of two items.  One CTA an SM.  Queries come in eights: NP of them over the prefix, NO over a row's own keys.
+template <int HS, int NP>
 struct ShSmem {
-  static constexpr int kUnit = kShTile * HS * 2, kQ = 16 * MT * HS * 2;
+  static constexpr int kUnit = kShTile * HS * 2, kQ = 8 * (NP > 2 ? NP : 2) * HS * 2;
   static constexpr int kWarp = kShUnits * kUnit + 2 * kQ;
-  static constexpr int kWarps = HS == 64 ? (MT == 2 ? 10 : 12) : (MT == 2 ? 5 : 7);
+  static constexpr int kWarps = HS == 64 ? (NP == 4 ? 10 : 12) : (NP == 4 ? 5 : 7);
   static constexpr int kBytes = kWarps * kWarp;
 };
 
@@ -218,7 +218,7 @@ struct Tile {
   int at;                            // own: index of the new key
 };
 
-template <int HS, int MT>
+template <int HS, int NP>
 struct Walk {
   const SharedParams& p;
   const Split& s;
@@ -309,96 +309,105 @@ struct Walk {
     }
   }
   __device__ __forceinline__ int64_t query_row(const Tile& t) const {
-    return (int64_t)t.gi * p.batch * p.per + (t.own ? (int64_t)t.b * p.per + t.part * 16 : (int64_t)t.part * 16 * MT);
+    return (int64_t)t.gi * p.batch * p.per + (t.own ? (int64_t)t.b * p.per + t.part * 16 : (int64_t)t.part * 8 * NP);
   }
-  __device__ __forceinline__ int queries(const Tile& t) const { return t.own ? min(16, p.per - t.part * 16) : min(16 * MT, p.batch * p.per - t.part * 16 * MT); }
+  __device__ __forceinline__ int queries(const Tile& t) const { return t.own ? min(16, p.per - t.part * 16) : min(8 * NP, p.batch * p.per - t.part * 8 * NP); }
   __device__ __forceinline__ int64_t item(const Tile& t) const {   // own items count with rows that take no part
     return t.own ? ((int64_t)t.b * p.n_groups + t.gi) * p.head_tiles + t.part : (int64_t)t.gi * p.row_tiles + t.part;
   }
 };
 
-template <int HS, int M>
+// O^T: dimensions 16 i + g and 16 i + g + 8 of queries 8 t + 2 tq and 8 t + 2 tq + 1 (g = lane / 4, tq = lane % 4), and those queries' maxima and this lane's part of their sums
+template <int HS, int NQ>
 struct Sums {
-  float o[M][HS / 8][4], m[M][2], l[M][2];
+  float o[HS / 16][NQ][4], m[NQ][2], l[NQ][2];
 };
 
-// S = Q K^T of 16 * M rows and a tile, and the tile's weights; `vb` is waited for by `values`
-template <int HS, int MT, int M, typename Values>
-__device__ __forceinline__ void attend_tile(Sums<HS, MT>& a, uint32_t q, uint32_t kb, int valid, float scale_log2, int lane, Values values) {
-  const int tq = lane & 3;
-  float s[M][kShTile / 8][4];
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8 x 8 matrix of 16-bit numbers over a warp
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// 8 N queries and a tile of keys: S^T = K Q^T and O^T += V^T P^T, keys and dimensions as the rows of the products, so that few queries cost few of them.  `vb` of the
+// values is what `values` gives, which waits for them.
+template <int HS, int NQ, int N, typename Values>
+__device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, uint32_t kb, int valid, float scale_log2, int lane, Values values) {
+  const int g = lane >> 2;
+  float s[kShTile / 16][N][4];
 #pragma unroll
-  for (int t = 0; t < M; ++t)
+  for (int i = 0; i < kShTile / 16; ++i)
 #pragma unroll
-    for (int i = 0; i < kShTile / 8; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
+    for (int t = 0; t < N; ++t) s[i][t][0] = s[i][t][1] = s[i][t][2] = s[i][t][3] = 0.f;
 #pragma unroll
-  for (int ks = 0; ks < HS / 16; ++ks) {
-    uint32_t qf[M][4];
+  for (int kp = 0; kp < HS / 32; ++kp) {
+    uint32_t qf[N][4];
 #pragma unroll
-    for (int t = 0; t < M; ++t) ldsm_x4(qf[t], q + sw<HS>(t * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+    for (int t = 0; t < N; ++t) ldsm_x4(qf[t], q + sw<HS>(t * 8 + (lane & 7), kp * 4 + (lane >> 3)));
 #pragma unroll
-    for (int np = 0; np < kShTile / 16; ++np) {
-      uint32_t kf[4];
-      ldsm_x4(kf, kb + sw<HS>(np * 16 + ((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int t = 0; t < M; ++t) {
-        pf_mma(s[t][2 * np], qf[t], kf[0], kf[1]);
-        pf_mma(s[t][2 * np + 1], qf[t], kf[2], kf[3]);
+      for (int i = 0; i < kShTile / 16; ++i) {
+        uint32_t kf[4];
+        ldsm_x4(kf, kb + sw<HS>(i * 16 + (lane & 15), kp * 4 + h * 2 + (lane >> 4)));
+#pragma unroll
+        for (int t = 0; t < N; ++t) pf_mma(s[i][t], kf, qf[t][2 * h], qf[t][2 * h + 1]);
       }
-    }
   }
-  uint32_t hi[M][kShTile / 16][4], lo[M][kShTile / 16][4];
+  uint32_t hi[kShTile / 16][N][2], lo[kShTile / 16][N][2];
 #pragma unroll
-  for (int t = 0; t < M; ++t) {
-    float top[2] = {a.m[t][0], a.m[t][1]};
+  for (int t = 0; t < N; ++t) {
+    float top[2] = {a.m[t][0], a.m[t][1]}, org[2];
 #pragma unroll
-    for (int i = 0; i < kShTile / 8; ++i)
+    for (int i = 0; i < kShTile / 16; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[t][i][e] = i * 8 + 2 * tq + (e & 1) < valid ? s[t][i][e] * scale_log2 : -INFINITY;
-        top[e >> 1] = fmaxf(top[e >> 1], s[t][i][e]);
+        s[i][t][e] = i * 16 + (e >> 1) * 8 + g < valid ? s[i][t][e] * scale_log2 : -INFINITY;
+        top[e & 1] = fmaxf(top[e & 1], s[i][t][e]);
       }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      const float org = top[h] == -INFINITY ? 0.f : top[h];   // (scores that are all -inf: weights of zero)
-      const float shrink = ex2(a.m[t][h] - org);
-      a.m[t][h] = top[h];
-      a.l[t][h] *= shrink;
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int i = 0; i < HS / 8; ++i) { a.o[t][i][2 * h] *= shrink; a.o[t][i][2 * h + 1] *= shrink; }
+      for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+      org[c] = top[c] == -INFINITY ? 0.f : top[c];   // (scores that are all -inf: weights of zero)
+      const float shrink = ex2(a.m[t][c] - org[c]);
+      a.m[t][c] = top[c];
+      a.l[t][c] *= shrink;
 #pragma unroll
-      for (int i = 0; i < kShTile / 8; ++i) {
-        const float x = ex2(s[t][i][2 * h] - org), y = ex2(s[t][i][2 * h + 1] - org);
-        a.l[t][h] += x + y;
-        const uint32_t w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);   // the leading 16 bits of both
-        hi[t][i >> 1][(i & 1) * 2 + h] = w;
-        lo[t][i >> 1][(i & 1) * 2 + h] = pack_bf16(fmaf(x, kAbove, -bf16lo(w)), fmaf(y, kAbove, -bf16hi(w)));
-      }
+      for (int i = 0; i < HS / 16; ++i) { a.o[i][t][c] *= shrink; a.o[i][t][2 + c] *= shrink; }
     }
+#pragma unroll
+    for (int i = 0; i < kShTile / 16; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = ex2(s[i][t][2 * h] - org[0]), y = ex2(s[i][t][2 * h + 1] - org[1]);
+        a.l[t][0] += x;
+        a.l[t][1] += y;
+        const uint32_t w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);   // the leading 16 bits of both
+        hi[i][t][h] = transposed(w);
+        lo[i][t][h] = transposed(pack_bf16(fmaf(x, kAbove, -bf16lo(w)), fmaf(y, kAbove, -bf16hi(w))));
+      }
   }
   const uint32_t vb = values();
 #pragma unroll
-  for (int ks = 0; ks < kShTile / 16; ++ks) {
+  for (int i = 0; i < kShTile / 16; ++i) {
 #pragma unroll
-    for (int dp = 0; dp < HS / 16; ++dp) {
+    for (int d = 0; d < HS / 16; ++d) {
       uint32_t vf[4];
-      ldsm_x4_t(vf, vb + sw<HS>(ks * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), dp * 2 + (lane >> 4)));
+      ldsm_x4_t(vf, vb + sw<HS>(i * 16 + ((lane >> 4) << 3) + (lane & 7), d * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-      for (int t = 0; t < M; ++t) {
-        pf_mma(a.o[t][2 * dp], hi[t][ks], vf[0], vf[1]);
-        pf_mma(a.o[t][2 * dp + 1], hi[t][ks], vf[2], vf[3]);
-        pf_mma(a.o[t][2 * dp], lo[t][ks], vf[0], vf[1]);
-        pf_mma(a.o[t][2 * dp + 1], lo[t][ks], vf[2], vf[3]);
+      for (int t = 0; t < N; ++t) {
+        pf_mma(a.o[d][t], vf, hi[i][t][0], hi[i][t][1]);
+        pf_mma(a.o[d][t], vf, lo[i][t][0], lo[i][t][1]);
       }
     }
   }
 }
 
-template <int HS, int MT>
-__global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_kernel(const SharedParams p) {
-  using C = ShSmem<HS, MT>;
+template <int HS, int NP, int NO>
+__global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_kernel(const SharedParams p) {
+  using C = ShSmem<HS, NP>;
+  constexpr int NQ = NP > NO ? NP : NO;
   constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
   extern __shared__ __align__(128) uint8_t sh_smem[];
   __shared__ int s_sums[T + 1], s_warp[C::kWarps];
@@ -407,11 +416,14 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
   const int plen = prefix_len(p);
   const Split s = make_split<T>(p, plen, s_sums, s_warp);
   const int w = warp * (int)gridDim.x + (int)blockIdx.x;   // (workers beside each other on different SMs)
+  // Where the prefix's own kernel ran in between, the turning kernel ended before that one let this one begin: then the wait is for that kernel, so that what comes next
+  // finds both done; one CTA waits for all.
+  const bool late = p.pre_parts > 0;
   if (w >= s.workers) {
-    griddep_wait();
+    if (!late || blockIdx.x == gridDim.x - 1) griddep_wait();
     return;
   }
-  const Walk<HS, MT> walk{p, s, s_sums, plen, (p.batch + T - 1) / T};
+  const Walk<HS, NP> walk{p, s, s_sums, plen, (p.batch + T - 1) / T};
   const uint32_t ring = pf_smem(sh_smem) + warp * C::kWarp, sq = ring + kShUnits * C::kUnit;
 
   auto load = [&](uint32_t dst, const __nv_bfloat16* src, int valid) {   // 32 rows, zeros from `valid` on: a weight of zero times whatever lies there must be zero
@@ -426,18 +438,18 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
     const __nv_bfloat16* const src = p.q + walk.query_row(t) * HS;
     const int valid = walk.queries(t);
 #pragma unroll
-    for (int j = 0; j < 16 * MT / RP; ++j) {
+    for (int j = 0; j < 8 * NQ / RP; ++j) {
       const int r = j * RP + lane / CH, c = lane % CH;
+      if (8 * NQ % RP && r >= 8 * NQ) break;
       const bool ok = r < valid;
       pf_cp16(dst + sw<HS>(r, c), src + (ok ? r * HS : 0) + c * 8, ok);
     }
   };
   const int end = first_tile(w + 1, s);
   Tile cur = walk.find(first_tile(w, s), T);
-  // What the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before.  Where the prefix's own kernel ran in between, the
-  // turning kernel ended before that one let this one begin: then the wait, for that kernel, is at the end.
+  // what the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before
   if (!cur.own) load(ring, cur.k, cur.valid);
-  if (p.pre_parts == 0) griddep_wait();
+  if (!late) griddep_wait();
   if (cur.own) load(ring, cur.k, cur.valid);
   load_queries(sq, cur);
   pf_commit();
@@ -452,12 +464,12 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
   }
   pf_commit();
 
-  Sums<HS, MT> a;
+  Sums<HS, NQ> a;
   auto clear = [&]() {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-      for (int i = 0; i < HS / 8; ++i) a.o[t][i][0] = a.o[t][i][1] = a.o[t][i][2] = a.o[t][i][3] = 0.f;
+      for (int i = 0; i < HS / 16; ++i) a.o[i][t][0] = a.o[i][t][1] = a.o[i][t][2] = a.o[i][t][3] = 0.f;
       a.m[t][0] = a.m[t][1] = -INFINITY;
       a.l[t][0] = a.l[t][1] = 0.f;
     }
@@ -480,8 +492,8 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
       __syncwarp();
       return vb;
     };
-    if (MT == 1 || cur.own) attend_tile<HS, MT, 1>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
-    else attend_tile<HS, MT, MT>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
+    if (NP == NO || cur.own) attend_tile<HS, NQ, NO>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
+    else attend_tile<HS, NQ, NP>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
     __syncwarp();                                          // the values have been read: the keys of the tile after the next take their place
     const bool ends = cur.left == 0 || !more;
     Tile was = cur;
@@ -496,21 +508,24 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
     if (ends) {
       // ---- the item, or this worker's part of it, ends ----
       const int64_t slot = walk.item(was) + w;
-      const int rows = was.own ? min(16, p.per) : 16 * MT, valid = walk.queries(was);
+      const int rows = was.own ? min(16, p.per) : 8 * NP, valid = walk.queries(was);
       float* const acc = (was.own ? p.own_acc : p.pre_acc) + slot * rows * HS;
       float2* const ml = (was.own ? p.own_ml : p.pre_ml) + slot * rows;
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < NQ; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float l = a.l[t][h];
-          l += __shfl_xor_sync(0xffffffffu, l, 1);
-          l += __shfl_xor_sync(0xffffffffu, l, 2);
-          const int r = t * 16 + h * 8 + g;
+        for (int c = 0; c < 2; ++c) {
+          float l = a.l[t][c];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          const int r = t * 8 + 2 * tq + c;
           if (r < valid) {
 #pragma unroll
-            for (int i = 0; i < HS / 8; ++i) __stcg(reinterpret_cast<float2*>(acc + r * HS + i * 8 + 2 * tq), make_float2(a.o[t][i][2 * h], a.o[t][i][2 * h + 1]));
-            if (tq == 0) __stcg(ml + r, make_float2(a.m[t][h], l));
+            for (int i = 0; i < HS / 16; ++i) {
+              __stcg(acc + r * HS + i * 16 + g, a.o[i][t][c]);
+              __stcg(acc + r * HS + i * 16 + 8 + g, a.o[i][t][2 + c]);
+            }
+            if (g == 0) __stcg(ml + r, make_float2(a.m[t][c], l));
           }
         }
       if (!more) break;
@@ -518,11 +533,11 @@ __global__ void __launch_bounds__(ShSmem<HS, MT>::kWarps * 32, 1) attn_shared_ke
     }
   }
   pf_wait<0>();
-  if (p.pre_parts > 0) griddep_wait();
+  if (late && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
 // A head's results joined: `ways` warps a head, HS / 32 numbers a lane.
-template <int HS, int MT>
+template <int HS>
 __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParams p) {
   constexpr int V = HS / 32;
   __shared__ float s_acc[8][HS];
@@ -550,15 +565,15 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
     const int ow0 = worker_of(own_first, s), own_n = worker_of(own_first + tiles - 1, s) - ow0 + 1;
     const int64_t own_at = ((((int64_t)b * p.n_groups + gi) * p.head_tiles + hh / 16) + ow0) * own_rows + hh % 16;
     // prefix
-    const int row = b * p.per + hh, item = gi * p.row_tiles + row / (16 * MT);
+    const int row = b * p.per + hh, item = gi * p.row_tiles + row / p.tile_rows;
     int pre_n = p.pre_parts;
     int64_t pre_at = ((int64_t)gi * p.pre_tiles + (pre_n ? row / p.pre_rows : 0)) * pre_n * p.pre_rows + (pre_n ? row % p.pre_rows : 0);
-    const int pre_step = pre_n ? p.pre_rows : 16 * MT;
+    const int pre_step = pre_n ? p.pre_rows : p.tile_rows;
     if (pre_n == 0 && s.prefix > 0) {
       const int t0 = s.own + item * s.prefix;
       const int pw0 = worker_of(t0, s);
       pre_n = worker_of(t0 + s.prefix - 1, s) - pw0 + 1;
-      pre_at = ((int64_t)item + pw0) * (16 * MT) + row % (16 * MT);
+      pre_at = ((int64_t)item + pw0) * p.tile_rows + row % p.tile_rows;
     }
     const int n = own_n + pre_n;
     for (int i0 = way; i0 < n; i0 += 4 * p.ways) {
@@ -629,7 +644,7 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
 }
 
 struct SharedPlan {
-  int mt, head_tiles, row_tiles, ctas, workers, ways;
+  int np, no, head_tiles, row_tiles, ctas, workers, ways;   // np, no: eights of queries of a prefix's item and of an own one
   int64_t own_slots, pre_slots;   // rows
   int64_t tiles, q;               // tiles at most; numbers of the turned queries
   size_t bytes;
@@ -657,17 +672,18 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
     s.pre_parts = s.pair ? s.splits : 2 * s.splits;
     prefix_rows = 0;               // not in the list of tiles
   }
-  s.mt = prefix_rows > 0 && rows > 16 ? 2 : 1;
+  s.no = per > 8 ? 2 : 1;
+  s.np = prefix_rows == 0 ? s.no : rows > 16 ? 4 : rows > 8 ? 2 : 1;
   s.head_tiles = (per + 15) / 16;
-  s.row_tiles = prefix_rows > 0 ? (int)((rows + 16 * s.mt - 1) / (16 * s.mt)) : 0;
+  s.row_tiles = prefix_rows > 0 ? (int)((rows + 8 * s.np - 1) / (8 * s.np)) : 0;
   const int64_t own_items = (int64_t)batch * n_groups * s.head_tiles, pre_items = (int64_t)n_groups * s.row_tiles;
   const int64_t tiles = own_items * ((own_rows + kShTile - 1) / kShTile) + pre_items * ((prefix_rows + kShTile - 1) / kShTile);
-  const int warps = hs == 64 ? (s.mt == 2 ? ShSmem<64, 2>::kWarps : ShSmem<64, 1>::kWarps) : (s.mt == 2 ? ShSmem<128, 2>::kWarps : ShSmem<128, 1>::kWarps);
+  const int warps = hs == 64 ? (s.np == 4 ? ShSmem<64, 4>::kWarps : ShSmem<64, 1>::kWarps) : (s.np == 4 ? ShSmem<128, 4>::kWarps : ShSmem<128, 1>::kWarps);
   s.tiles = tiles;
   s.ctas = sm_count() < tiles ? sm_count() : (int)tiles;
   s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
   s.own_slots = (own_items + s.workers) * (per < 16 ? per : 16);
-  s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 16 * s.mt : (int64_t)n_groups * s.pre_tiles * s.pre_parts * s.pre_rows;
+  s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 8 * s.np : (int64_t)n_groups * s.pre_tiles * s.pre_parts * s.pre_rows;
   s.q = rows * n_groups * hs;
   s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)(batch + 1) * sizeof(int);
   // results of a head: about those of a prefix item and of an own one
@@ -677,23 +693,30 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   return s;
 }
 
-template <int HS, int MT>
-cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
-  constexpr int smem = ShSmem<HS, MT>::kBytes;
+template <int HS, int NP, int NO>
+cudaError_t launch_tiles(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
+  using C = ShSmem<HS, NP>;
   static PerDeviceOnce once;
   if (once.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_shared_kernel<HS, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(attn_shared_kernel<HS, NP, NO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
     if (e != cudaSuccess) return e;
     once.done();
   }
+  return launch(attn_shared_kernel<HS, NP, NO>, dim3((unsigned)s.ctas), dim3(C::kWarps * 32), (size_t)C::kBytes, st, p);
+}
+
+template <int HS>
+cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
   const int64_t warps = (int64_t)p.batch * p.n_groups * (p.per + 2);
   cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8 + 1)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
   if (s.tensor && (e = launch_attn_shared_prefix(p, HS, s.pair, s.splits, st)) != cudaSuccess) return e;
-  e = launch(attn_shared_kernel<HS, MT>, dim3((unsigned)s.ctas), dim3(ShSmem<HS, MT>::kWarps * 32), (size_t)smem, st, p);
+  if (s.np == 4) e = s.no == 2 ? launch_tiles<HS, 4, 2>(p, s, st) : launch_tiles<HS, 4, 1>(p, s, st);
+  else if (s.np == 2) e = s.no == 2 ? launch_tiles<HS, 2, 2>(p, s, st) : launch_tiles<HS, 2, 1>(p, s, st);
+  else e = launch_tiles<HS, 1, 1>(p, s, st);
   if (e != cudaSuccess) return e;
   const int heads = 8 / s.ways;
-  return launch(attn_shared_join_kernel<HS, MT>, dim3((unsigned)(p.batch * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
+  return launch(attn_shared_join_kernel<HS>, dim3((unsigned)(p.batch * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -739,7 +762,7 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   p.kp = (const __nv_bfloat16*)a->k_prefix; p.vp = (const __nv_bfloat16*)a->v_prefix; p.kp_g = a->k_prefix_stride; p.vp_g = a->v_prefix_stride;
   p.out = (__nv_bfloat16*)a->out;
   p.batch = a->batch; p.n_head = a->n_head; p.n_groups = a->n_groups; p.per = a->n_head / a->n_groups; p.own_rows = a->own_rows; p.prefix_rows = a->prefix_rows;
-  p.head_tiles = s.head_tiles; p.row_tiles = s.row_tiles; p.workers = s.workers; p.sms = sm_count(); p.ways = s.ways;
+  p.head_tiles = s.head_tiles; p.row_tiles = s.row_tiles; p.tile_rows = 8 * s.np; p.workers = s.workers; p.sms = sm_count(); p.ways = s.ways;
   p.pre_parts = s.pre_parts; p.pre_rows = s.pre_rows; p.pre_tiles = s.pre_tiles;
   const int n = a->rope_n_elem, part = a->head_size / 32;
   p.wide = ((uintptr_t)a->qkv & 15) == 0 && n % (2 * part) == 0 && (a->table_dtype == B200_BF16 || (((uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0);
@@ -752,8 +775,7 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   p.before = (int*)(p.pre_ml + s.pre_slots);
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (a->head_size == 128) B200_CUDA((s.mt == 2 ? launch_shared<128, 2>(p, s, st) : launch_shared<128, 1>(p, s, st)));
-  else B200_CUDA((s.mt == 2 ? launch_shared<64, 2>(p, s, st) : launch_shared<64, 1>(p, s, st)));
+  B200_CUDA((a->head_size == 128 ? launch_shared<128>(p, s, st) : launch_shared<64>(p, s, st)));
   return B200_OK;
 }
 

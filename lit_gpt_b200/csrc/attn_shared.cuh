@@ -14,11 +14,11 @@ struct SharedParams {
   const __nv_bfloat16* kp; const __nv_bfloat16* vp; int64_t kp_g, vp_g;
   __nv_bfloat16* out;
   int batch, n_head, n_groups, per, own_rows, prefix_rows;
-  int head_tiles, row_tiles;                 // tiles of 16 heads of a row's group; tiles of a group's query rows over the prefix
+  int head_tiles, row_tiles, tile_rows;      // tiles of 16 heads of a row's group; tiles of a group's query rows over the prefix, of so many rows
   __nv_bfloat16* q;                          // the queries, turned: [n_groups][batch * per][HS]
   int workers, sms;                          // warps that share the tiles, at most
   float* own_acc; float2* own_ml;            // results of key ranges of own items: slots of min(16, per) rows
-  float* pre_acc; float2* pre_ml;            // of prefix items: slots of 16 * MT rows
+  float* pre_acc; float2* pre_ml;            // of prefix items: slots of tile_rows rows
   int* before;                               // [batch + 1]: tiles of the rows' own keys, of one group and tile of heads, before each row
   int ways;                                  // warps that join a head's results
   // On the tensor memory (attn_shared_tc05.cu) prefix items are 128 or 256 query rows of a group, with `pre_parts` results each, in slots of `pre_rows` rows, item after item;
