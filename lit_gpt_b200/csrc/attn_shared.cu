@@ -680,7 +680,9 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   const int64_t tiles = own_items * ((own_rows + kShTile - 1) / kShTile) + pre_items * ((prefix_rows + kShTile - 1) / kShTile);
   const int warps = hs == 64 ? (s.np == 4 ? ShSmem<64, 4>::kWarps : ShSmem<64, 1>::kWarps) : (s.np == 4 ? ShSmem<128, 4>::kWarps : ShSmem<128, 1>::kWarps);
   s.tiles = tiles;
-  s.ctas = sm_count() < tiles ? sm_count() : (int)tiles;
+  // a CTA an SM; beside the prefix's own kernel, which leaves SMs one by one, two shorter ones
+  s.ctas = sm_count() * (s.tensor ? 2 : 1);
+  if (s.ctas > tiles) s.ctas = (int)tiles;
   s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
   s.own_slots = (own_items + s.workers) * (per < 16 ? per : 16);
   s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 8 * s.np : (int64_t)n_groups * s.pre_tiles * s.pre_parts * s.pre_rows;
