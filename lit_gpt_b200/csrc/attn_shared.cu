@@ -34,7 +34,6 @@ __device__ __forceinline__ int own_index(const SharedParams& p, int64_t pos, int
   const int64_t i = pos - plen;
   return (int)(i < 0 ? 0 : (i >= p.own_rows ? p.own_rows - 1 : i));
 }
-__device__ __forceinline__ int own_tiles(const SharedParams& p, int b, int plen) { return (own_index(p, row_pos(p, b), plen) + kShTile) / kShTile; }
 __device__ __forceinline__ int64_t table_row(const SharedParams& p, int b, int64_t pos) {
   const int64_t r = p.table_presel ? (p.pos_each ? b : 0) : pos;
   return r < 0 ? 0 : (r >= p.table_rows ? p.table_rows - 1 : r);
@@ -119,9 +118,29 @@ __device__ __forceinline__ int worker_of(int tile, const Split& s) {
 }
 __device__ __forceinline__ int first_tile(int w, const Split& s) { return w * s.each + min(w, s.more); }
 
-__device__ __forceinline__ Split split_of(const SharedParams& p, int plen, int own_tiles_of_all) {
+// Rows are summed in runs of one per thread: sums[t] = own tiles (of one group and tile of heads) of the rows before run t, sums[THREADS] of all.  mine[b]: own_index of the
+// rows there is place for.
+template <int THREADS>
+__device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int* sums, int* mine, int* s_warp) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = (p.batch + THREADS - 1) / THREADS;
+  int here = 0;
+  for (int b = tid * run; b < min(p.batch, (tid + 1) * run); ++b) {
+    const int at = own_index(p, row_pos(p, b), plen);
+    if (b < THREADS) mine[b] = at;
+    here += (at + kShTile) / kShTile;
+  }
+  int inc = here;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int before = inc - here;
+  for (int w = 0; w < warp; ++w) before += s_warp[w];
+  sums[tid] = before;
+  if (tid == THREADS - 1) sums[THREADS] = before + here;
+  __syncthreads();
   Split s;
-  s.own = own_tiles_of_all * p.n_groups * p.head_tiles;
+  s.own = sums[THREADS] * p.n_groups * p.head_tiles;
   s.prefix = p.row_tiles ? (plen + kShTile - 1) / kShTile : 0;
   s.all = s.own + s.prefix * p.n_groups * p.row_tiles;
   // two tiles a worker at least, unless that leaves SMs without one
@@ -129,25 +148,6 @@ __device__ __forceinline__ Split split_of(const SharedParams& p, int plen, int o
   s.each = s.workers ? s.all / s.workers : 0;
   s.more = s.all - s.each * s.workers;
   return s;
-}
-
-// Rows are summed in runs of one per thread: sums[t] = own tiles (of one group and tile of heads) of the rows before run t; sums[THREADS] of all.
-template <int THREADS>
-__device__ __forceinline__ Split make_split(const SharedParams& p, int plen, int* sums, int* s_warp) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = (p.batch + THREADS - 1) / THREADS;
-  int mine = 0;
-  for (int b = tid * run; b < min(p.batch, (tid + 1) * run); ++b) mine += own_tiles(p, b, plen);
-  int inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
-  if (lane == 31) s_warp[warp] = inc;
-  __syncthreads();
-  int before = inc - mine;
-  for (int w = 0; w < warp; ++w) before += s_warp[w];
-  sums[tid] = before;
-  if (tid == THREADS - 1) sums[THREADS] = before + mine;
-  __syncthreads();
-  return split_of(p, plen, sums[THREADS]);
 }
 
 // A warp's shared memory: a ring of units, the queries of two items.  One CTA an SM.  Queries come in eights: NP of them over the prefix, NO over a row's own keys.
@@ -165,19 +165,6 @@ __global__ void __launch_bounds__(256) attn_shared_turn_kernel(const SharedParam
   constexpr int V = HS / 32;
   griddep_wait();     // (before the launch of what follows: the kernels behind read positions, lengths and the prefix ahead of their own wait)
   griddep_launch();
-  if (blockIdx.x == gridDim.x - 1) {   // own tiles (of one group and tile of heads) of the rows before each
-    __shared__ int s_sums[257], s_warp[8];
-    const int plen = prefix_len(p);
-    make_split<256>(p, plen, s_sums, s_warp);
-    const int run = (p.batch + 255) / 256;
-    int sum = s_sums[threadIdx.x];
-    for (int b = threadIdx.x * run; b < min(p.batch, ((int)threadIdx.x + 1) * run); ++b) {
-      p.before[b] = sum;
-      sum += own_tiles(p, b, plen);
-    }
-    if (threadIdx.x == 0) p.before[p.batch] = s_sums[256];
-    return;
-  }
   const int lane = threadIdx.x & 31, heads = p.n_groups * (p.per + 2);
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int b = (int)(at / heads), i = (int)(at - (int64_t)b * heads), gi = i / (p.per + 2), h = i - gi * (p.per + 2);
@@ -223,7 +210,10 @@ struct Walk {
   const SharedParams& p;
   const Split& s;
   const int* sums;
-  int plen, run;
+  const int* mine_of;                // of the first `threads` rows
+  int plen, run, threads;
+
+  __device__ __forceinline__ int mine(int b) const { return b < threads ? mine_of[b] : own_index(p, row_pos(p, b), plen); }
 
   __device__ __forceinline__ void own_item(Tile& t, int mine, int tile) const {
     const int tiles = mine / kShTile + 1;
@@ -241,7 +231,7 @@ struct Walk {
     t.v = p.vp + (int64_t)t.gi * p.vp_g + (int64_t)tile * kShTile * HS;
     t.valid = min(kShTile, plen - tile * kShTile);
   }
-  __device__ __forceinline__ Tile find(int index, int threads) const {
+  __device__ __forceinline__ Tile find(int index) const {
     Tile t;
     t.index = index;
     if (index < s.own) {
@@ -252,19 +242,18 @@ struct Walk {
         if (sums[mid] * each <= index) lo = mid; else hi = mid;
       }
       int rest = index - sums[lo] * each;
-      int b = lo * run, mine = own_index(p, row_pos(p, b), plen);
+      int b = lo * run, at = mine(b);
       for (;;) {                     // (one row a run unless the batch is large)
-        const int here = (mine + kShTile) / kShTile * each;
+        const int here = (at + kShTile) / kShTile * each;
         if (rest < here) break;
         rest -= here;
-        ++b;
-        mine = own_index(p, row_pos(p, b), plen);
+        at = mine(++b);
       }
-      const int tiles = mine / kShTile + 1, item = rest / tiles;
+      const int tiles = at / kShTile + 1, item = rest / tiles;
       t.b = b;
       t.gi = item / p.head_tiles;
       t.part = item - t.gi * p.head_tiles;
-      own_item(t, mine, rest - item * tiles);
+      own_item(t, at, rest - item * tiles);
     } else {
       const int rest = index - s.own, item = rest / s.prefix;
       t.b = 0;
@@ -294,15 +283,15 @@ struct Walk {
       t.gi = t.part = 0;
       prefix_item(t, 0);
     } else if (t.own) {
-      int mine = t.at;
+      int at = t.at;
       if (++t.part == p.head_tiles) {
         t.part = 0;
         if (++t.gi == p.n_groups) {
           t.gi = 0;
-          do { ++t.b; mine = own_index(p, row_pos(p, t.b), plen); } while (mine < 0);
+          do at = mine(++t.b); while (at < 0);
         }
       }
-      own_item(t, mine, 0);
+      own_item(t, at, 0);
     } else {
       if (++t.part == p.row_tiles) { t.part = 0; ++t.gi; }
       prefix_item(t, 0);
@@ -312,6 +301,7 @@ struct Walk {
     return (int64_t)t.gi * p.batch * p.per + (t.own ? (int64_t)t.b * p.per + t.part * 16 : (int64_t)t.part * 8 * NP);
   }
   __device__ __forceinline__ int queries(const Tile& t) const { return t.own ? min(16, p.per - t.part * 16) : min(8 * NP, p.batch * p.per - t.part * 8 * NP); }
+  __device__ __forceinline__ int tiles(const Tile& t) const { return t.own ? t.at / kShTile + 1 : s.prefix; }
   __device__ __forceinline__ int64_t item(const Tile& t) const {   // own items count with rows that take no part
     return t.own ? ((int64_t)t.b * p.n_groups + t.gi) * p.head_tiles + t.part : (int64_t)t.gi * p.row_tiles + t.part;
   }
@@ -410,11 +400,11 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
   constexpr int NQ = NP > NO ? NP : NO;
   constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
   extern __shared__ __align__(128) uint8_t sh_smem[];
-  __shared__ int s_sums[T + 1], s_warp[C::kWarps];
+  __shared__ int s_sums[T + 1], s_mine[T], s_warp[C::kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
   griddep_launch();
   const int plen = prefix_len(p);
-  const Split s = make_split<T>(p, plen, s_sums, s_warp);
+  const Split s = make_split<T>(p, plen, s_sums, s_mine, s_warp);
   const int w = warp * (int)gridDim.x + (int)blockIdx.x;   // (workers beside each other on different SMs)
   // Where the prefix's own kernel ran in between, the turning kernel ended before that one let this one begin: then the wait is for that kernel, so that what comes next
   // finds both done; one CTA waits for all.
@@ -423,7 +413,7 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
     if (!late || blockIdx.x == gridDim.x - 1) griddep_wait();
     return;
   }
-  const Walk<HS, NP> walk{p, s, s_sums, plen, (p.batch + T - 1) / T};
+  const Walk<HS, NP> walk{p, s, s_sums, s_mine, plen, (p.batch + T - 1) / T, T};
   const uint32_t ring = pf_smem(sh_smem) + warp * C::kWarp, sq = ring + kShUnits * C::kUnit;
 
   auto load = [&](uint32_t dst, const __nv_bfloat16* src, int valid) {   // 32 rows, zeros from `valid` on: a weight of zero times whatever lies there must be zero
@@ -445,8 +435,8 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
       pf_cp16(dst + sw<HS>(r, c), src + (ok ? r * HS : 0) + c * 8, ok);
     }
   };
-  const int end = first_tile(w + 1, s);
-  Tile cur = walk.find(first_tile(w, s), T);
+  const int first = first_tile(w, s), end = first_tile(w + 1, s);
+  Tile cur = walk.find(first);
   // what the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before
   if (!cur.own) load(ring, cur.k, cur.valid);
   if (!late) griddep_wait();
@@ -507,7 +497,12 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
     pf_commit();
     if (ends) {
       // ---- the item, or this worker's part of it, ends ----
-      const int64_t slot = walk.item(was) + w;
+      const int64_t item = walk.item(was), slot = item + w;
+      const int begun = walk.tiles(was) - 1 - was.left;   // the item's tiles before the last one here
+      if (lane == 0 && was.index - begun >= first) {       // it began here: who joins its results learns where they are
+        int2* const where = was.own ? p.own_where : p.pre_where;
+        __stcg(where + item, make_int2(w, worker_of(was.index + was.left, s) - w + 1));
+      }
       const int rows = was.own ? min(16, p.per) : 8 * NP, valid = walk.queries(was);
       float* const acc = (was.own ? p.own_acc : p.pre_acc) + slot * rows * HS;
       float2* const ml = (was.own ? p.own_ml : p.pre_ml) + slot * rows;
@@ -545,37 +540,24 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = 8 / p.ways, blocks = (p.n_head + heads - 1) / heads;
   const int b = blockIdx.x / blocks, h = (blockIdx.x - b * blocks) * heads + warp / p.ways, way = warp % p.ways;
   griddep_launch();
-  const int plen = prefix_len(p);
-  const int mine = own_index(p, row_pos(p, b), plen);
+  const bool idle = row_pos(p, b) < 0;
+  const int gi = h / p.per, hh = h - gi * p.per, row = b * p.per + hh, own_rows = min(16, p.per);
+  const int64_t own_item = ((int64_t)b * p.n_groups + gi) * p.head_tiles + hh / 16, pre_item = (int64_t)gi * p.row_tiles + row / p.tile_rows;
+  int2 pre = make_int2(0, p.pre_parts);
+  int64_t pre_at = 0;
+  if (p.pre_parts) pre_at = ((int64_t)gi * p.pre_tiles + row / p.pre_rows) * p.pre_parts * p.pre_rows + row % p.pre_rows;
+  const int pre_step = p.pre_parts ? p.pre_rows : p.tile_rows;
+  const bool listed = p.row_tiles > 0 && prefix_len(p) > 0;   // the prefix is in the list of tiles
   griddep_wait();
-  if (mine < 0) {
-    if (h < p.n_head && way == 0)
-#pragma unroll
-      for (int i = 0; i < V; ++i) p.out[((int64_t)b * p.n_head + h) * HS + lane * V + i] = __float2bfloat16_rn(0.f);
-    return;
-  }
-  const int before = p.before[b];
-  const Split s = split_of(p, plen, p.before[p.batch]);
   float top = -INFINITY, sum = 0.f, a[V] = {};
-  if (h < p.n_head) {
-    const int gi = h / p.per, hh = h - gi * p.per, tiles = mine / kShTile + 1;
-    // own: the item's tiles, the workers that had them, their slots
-    const int own_first = (before * p.n_groups + gi * tiles) * p.head_tiles + hh / 16 * tiles;
-    const int own_rows = min(16, p.per);
-    const int ow0 = worker_of(own_first, s), own_n = worker_of(own_first + tiles - 1, s) - ow0 + 1;
-    const int64_t own_at = ((((int64_t)b * p.n_groups + gi) * p.head_tiles + hh / 16) + ow0) * own_rows + hh % 16;
-    // prefix
-    const int row = b * p.per + hh, item = gi * p.row_tiles + row / p.tile_rows;
-    int pre_n = p.pre_parts;
-    int64_t pre_at = ((int64_t)gi * p.pre_tiles + (pre_n ? row / p.pre_rows : 0)) * pre_n * p.pre_rows + (pre_n ? row % p.pre_rows : 0);
-    const int pre_step = pre_n ? p.pre_rows : p.tile_rows;
-    if (pre_n == 0 && s.prefix > 0) {
-      const int t0 = s.own + item * s.prefix;
-      const int pw0 = worker_of(t0, s);
-      pre_n = worker_of(t0 + s.prefix - 1, s) - pw0 + 1;
-      pre_at = ((int64_t)item + pw0) * p.tile_rows + row % p.tile_rows;
+  if (h < p.n_head && !idle) {
+    const int2 own = __ldcg(p.own_where + own_item);
+    if (listed) {
+      pre = __ldcg(p.pre_where + pre_item);
+      pre_at = (pre_item + pre.x) * p.tile_rows + row % p.tile_rows;
     }
-    const int n = own_n + pre_n;
+    const int64_t own_at = (own_item + own.x) * own_rows + hh % 16;
+    const int own_n = own.y, n = own_n + pre.y;
     for (int i0 = way; i0 < n; i0 += 4 * p.ways) {
       float2 e[4];
       float v[4][V];
@@ -586,11 +568,10 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
 #pragma unroll
         for (int j = 0; j < V; ++j) v[u][j] = 0.f;
         if (i < n) {
-          const bool own = i < own_n;
-          const int64_t at = own ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * pre_step;
-          e[u] = __ldcg((own ? p.own_ml : p.pre_ml) + at);
-          if (e[u].y == 0.f) continue;   // (a range that saw nothing has no result)
-          const float* const src = (own ? p.own_acc : p.pre_acc) + at * HS + lane * V;
+          const bool mine = i < own_n;
+          const int64_t at = mine ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * pre_step;
+          e[u] = __ldcg((mine ? p.own_ml : p.pre_ml) + at);
+          const float* const src = (mine ? p.own_acc : p.pre_acc) + at * HS + lane * V;
           if constexpr (V == 4) {
             const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
             v[u][0] = x.x; v[u][1] = x.y; v[u][V - 2] = x.z; v[u][V - 1] = x.w;
@@ -613,7 +594,7 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
         const float c = ex2(e[u].x - org);
         sum += e[u].y * c;
 #pragma unroll
-        for (int j = 0; j < V; ++j) a[j] += v[u][j] * c;
+        for (int j = 0; j < V; ++j) a[j] += e[u].y == 0.f ? 0.f : v[u][j] * c;   // (a range that saw nothing has no result)
       }
     }
   }
@@ -637,7 +618,7 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
     }
   }
   if (h >= p.n_head) return;
-  const float inv = 1.f / sum;
+  const float inv = idle ? 0.f : 1.f / sum;
   __nv_bfloat16* const out = p.out + ((int64_t)b * p.n_head + h) * HS + lane * V;
   if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[V - 2] * inv, a[V - 1] * inv));
   else *reinterpret_cast<uint32_t*>(out) = pack_bf16(a[0] * inv, a[1] * inv);
@@ -646,6 +627,7 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
 struct SharedPlan {
   int np, no, head_tiles, row_tiles, ctas, workers, ways;   // np, no: eights of queries of a prefix's item and of an own one
   int64_t own_slots, pre_slots;   // rows
+  int64_t own_items, pre_items;   // in the list of tiles
   int64_t tiles, q;               // tiles at most; numbers of the turned queries
   size_t bytes;
   bool tensor, pair;              // the prefix on the tensor memory; 256 query rows a CTA instead of 128
@@ -687,7 +669,9 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   s.own_slots = (own_items + s.workers) * (per < 16 ? per : 16);
   s.pre_slots = prefix_rows > 0 ? (pre_items + s.workers) * 8 * s.np : (int64_t)n_groups * s.pre_tiles * s.pre_parts * s.pre_rows;
   s.q = rows * n_groups * hs;
-  s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)(batch + 1) * sizeof(int);
+  s.own_items = own_items;
+  s.pre_items = pre_items;
+  s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)(own_items + pre_items) * sizeof(int2);
   // results of a head: about those of a prefix item and of an own one
   const int64_t results = 2 + s.pre_parts + (int64_t)s.workers / (pre_items > 0 ? pre_items : own_items);
   s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
@@ -710,7 +694,7 @@ cudaError_t launch_tiles(const SharedParams& p, const SharedPlan& s, cudaStream_
 template <int HS>
 cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
   const int64_t warps = (int64_t)p.batch * p.n_groups * (p.per + 2);
-  cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8 + 1)), dim3(256), 0, st, p);
+  cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
   if (s.tensor && (e = launch_attn_shared_prefix(p, HS, s.pair, s.splits, st)) != cudaSuccess) return e;
   if (s.np == 4) e = s.no == 2 ? launch_tiles<HS, 4, 2>(p, s, st) : launch_tiles<HS, 4, 1>(p, s, st);
@@ -774,7 +758,8 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t
   p.pre_acc = p.own_acc + s.own_slots * a->head_size;
   p.own_ml = (float2*)(p.pre_acc + s.pre_slots * a->head_size);
   p.pre_ml = p.own_ml + s.own_slots;
-  p.before = (int*)(p.pre_ml + s.pre_slots);
+  p.own_where = (int2*)(p.pre_ml + s.pre_slots);
+  p.pre_where = p.own_where + s.own_items;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
   const cudaStream_t st = (cudaStream_t)stream;
   B200_CUDA((a->head_size == 128 ? launch_shared<128>(p, s, st) : launch_shared<64>(p, s, st)));

@@ -19,7 +19,7 @@ struct SharedParams {
   int workers, sms;                          // warps that share the tiles, at most
   float* own_acc; float2* own_ml;            // results of key ranges of own items: slots of min(16, per) rows
   float* pre_acc; float2* pre_ml;            // of prefix items: slots of tile_rows rows
-  int* before;                               // [batch + 1]: tiles of the rows' own keys, of one group and tile of heads, before each row
+  int2* own_where; int2* pre_where;          // per item of the list: the first worker that has tiles of it, and how many workers have
   int ways;                                  // warps that join a head's results
   // On the tensor memory (attn_shared_tc05.cu) prefix items are 128 or 256 query rows of a group, with `pre_parts` results each, in slots of `pre_rows` rows, item after item;
   // row_tiles is 0 then.  pre_parts 0: the prefix is in the list of tiles.
