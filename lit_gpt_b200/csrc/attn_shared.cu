@@ -437,21 +437,26 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
   };
   const int first = first_tile(w, s), end = first_tile(w + 1, s);
   Tile cur = walk.find(first);
-  // what the turning kernel wrote, queries and the newest own rows, is read behind the wait; a prefix was there before
-  if (!cur.own) load(ring, cur.k, cur.valid);
-  if (!late) griddep_wait();
-  if (cur.own) load(ring, cur.k, cur.valid);
-  load_queries(sq, cur);
-  pf_commit();
-  load(ring + C::kUnit, cur.v, cur.valid);
-  pf_commit();
   Tile coming = cur;                                       // the tile behind it: its values are loaded next
+  const bool two = cur.index + 1 < end;
+  if (two) walk.next(coming);
+  // What the turning kernel writes, queries and the newest own row, the last of an item's, is read behind the wait; everything else was there before.
+  auto early = [&](bool now) {
+    const bool c = now == (!cur.own || cur.left > 0), n = two && now == (!coming.own || coming.left > 0);
+    if (c) {
+      load(ring, cur.k, cur.valid);
+      load(ring + C::kUnit, cur.v, cur.valid);
+    }
+    if (n) load(ring + 2 * C::kUnit, coming.k, coming.valid);
+  };
+  early(true);
+  if (!late) griddep_wait();
+  early(false);
+  load_queries(sq, cur);
   int qb = 0, next_qb = 0;                                 // the query buffers of either
-  if (cur.index + 1 < end) {
-    walk.next(coming);
-    load(ring + 2 * C::kUnit, coming.k, coming.valid);
-    if (cur.left == 0) load_queries(sq + (next_qb = 1) * C::kQ, coming);
-  }
+  if (two && cur.left == 0) load_queries(sq + (next_qb = 1) * C::kQ, coming);
+  pf_commit();
+  pf_commit();
   pf_commit();
 
   Sums<HS, NQ> a;

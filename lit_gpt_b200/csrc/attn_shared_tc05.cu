@@ -4,11 +4,12 @@
 // One CTA = 128 or 256 query rows of a group (rows of the batch times heads of the group) against a range of the prefix's keys, in tiles of 128 keys.  Two streams of products
 // and softmax, each with its scores and its output in tensor memory, fill each other's gaps: with 256 rows the halves of the rows, with 128 the even and the odd key tiles,
 // whose results are joined as those of two ranges.
-//   * warps 0-3 and 4-7: a stream's softmax, a row per thread: scores are read for their maximum and, 32 at a time, for the weights, which go back over them as two bf16
-//     numbers, the leading bits and the rest (attn_shared.cu says why).  In loops of 32, which read the scores twice: unrolled over a tile the code was 15 KB, and
-//     a launch spent 10000 clocks, as long as three tiles, on fetching it once.  A row's maximum moves, and its output shrinks, only when the maximum grew by 2^8: with the rest a weight of 256 is as exact as one of 1.
-//   * warp 8: S = Q K^T (operands in shared memory) and O += P V (P from tensor memory, V as it lies), 128 x 128 x 16 each
-//   * warps 9 and 10 bring keys and values, two stages each: whole tiles by TMA, the prefix's last one row by row, zeros behind it.
+//   * warps 0-7 and 8-15: a stream's softmax, half of a row's 128 keys per thread: its 64 scores are read into registers, the row's maximum is joined through shared memory,
+//     and the weights go back over the scores as two bf16 numbers, the leading bits and the rest (attn_shared.cu says why).  A row's maximum moves, and its output shrinks,
+//     only when the maximum grew by 2^8: with the rest a weight of 256 is as exact as one of 1.  With a whole row per thread, four warps a stream, a tile took 4600
+//     clocks: a warp a scheduler does not fill the exponentials' 1024 clocks.  Unrolled over a row the code was 15 KB, and a launch spent 10000 clocks on fetching it once.
+//   * warp 16: S = Q K^T (operands in shared memory) and O += P V (P from tensor memory, V as it lies), 128 x 128 x 16 each
+//   * warps 17 and 18 bring keys and values, two stages each: whole tiles by TMA, the prefix's last one row by row, zeros behind it.
 // Bound: the prefix's bytes with up to 128 rows (a tile of 128 keys, 64 KB, is 2800 clocks of an SM's share of the memory's rate, its products 1536), with 256 rows the
 // products: 3072 clocks a tile, 1024 of them for the weights' second numbers.
 #include "attn_shared.cuh"
@@ -18,7 +19,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kSpThreads = 352;
+constexpr int kSpThreads = 608;
 constexpr float kAbove = 1.00000012f;   // 1 + 2^-23 (attn_shared.cu)
 
 template <int HS>
@@ -43,6 +44,7 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
   extern __shared__ __align__(1024) uint8_t sp_smem[];
   __shared__ __align__(8) uint64_t s_bars[18];
   __shared__ uint32_t s_tmem;
+  __shared__ float s_both[2][2][2][128];   // step, stream, half: a row's maximum over half of a tile; at the end its sum
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, tile_of_rows = item % p.pre_tiles, gi = item / p.pre_tiles;
   const int rows = p.batch * p.per, r0 = tile_of_rows * p.pre_rows;
@@ -60,7 +62,7 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
       tc::mbar_init(k_empty + 8 * i, 1);
       tc::mbar_init(v_empty + 8 * i, 1);
       tc::mbar_init(s_full + 8 * i, 1);
-      tc::mbar_init(p_half + 8 * i, 4);
+      tc::mbar_init(p_half + 8 * i, 8);
       tc::mbar_init(p_full + 8 * i, 4);
       tc::mbar_init(o_done + 8 * i, 1);
     }
@@ -72,20 +74,20 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
   // The prefix was there before the turning kernel: its copies begin ahead of the wait for that one.  Only behind its wait a CTA lets attn_shared_kernel begin, which
   // counts on the turning kernel's end.
   uint32_t tmem = 0;
-  if (warp < 9) {
+  if (warp < 17) {
     griddep_wait();
     griddep_launch();
-    if (warp == 8) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+    if (warp == 16) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
     tc::fence_before();
-    asm volatile("bar.sync 1, 288;" ::: "memory");
+    asm volatile("bar.sync 1, 544;" ::: "memory");
     tc::fence_after();
     tmem = s_tmem;
   }
   bool ok = true;
 
-  if (warp >= 9) {
+  if (warp >= 17) {
     // ================================ loads ================================
-    const bool keys = warp == 9;
+    const bool keys = warp == 17;
     const __nv_bfloat16* const src = keys ? p.kp + (int64_t)gi * p.kp_g : p.vp + (int64_t)gi * p.vp_g;
     const uint32_t dst = keys ? sk_ : sv_, full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
     if (lane == 0) tc::prefetch_map(keys ? &map_k : &map_v);
@@ -122,7 +124,7 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
     // no copy may land after the CTA has left
     if (keys && n > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(q_full, 0)) && ok;
     for (int i = max(j - 2, 0); i < j; ++i) ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * (i & 1), (uint32_t)(i >> 1) & 1u)) && ok;
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ================================ products ================================
     if (tc::elect() && n > 0) {
       const uint32_t q_low = tc::desc_sw128_low(sq_), k_low = tc::desc_sw128_low(sk_), v_low = desc_v_low(sv_);
@@ -189,48 +191,44 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
       }
     }
   } else {
-    // ================================ softmax: a row per thread ================================
-    const int t = warp >> 2, r = tid & 127, row = r0 + (PAIR ? tid : r);
+    // ================================ softmax: half of a row's keys per thread ================================
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, row = r0 + (PAIR ? t * 128 : 0) + r;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + C::kS + t * 128, to = tmem + lanes + C::kO + t * HS;
+    const uint32_t ts = tmem + lanes + C::kS + t * 128 + half * 64, to = tmem + lanes + C::kO + t * HS + half * (HS / 2);
     const float sl = p.scale_log2, room = 8.f / sl;
+    auto both = [&](float mine, int step) {                // the other half's number of the row
+      s_both[step][t][half][r] = mine;
+      asm volatile("bar.sync %0, 64;" ::"r"(2 + t * 4 + (warp & 3)) : "memory");
+      return s_both[step][t][half ^ 1][r];
+    };
     float m = -INFINITY;
     f2 l2[2] = {0ull, 0ull};
     uint32_t steps = 0;
     for (int j = PAIR ? 0 : t; j < n; j += PAIR ? 1 : 2, ++steps) {
       ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * t, steps & 1u));
-      if (!ok) break;
+      if (!ok) {       // (a warp that gave up a wait still meets the one that has the rows' other half)
+        both(0.f, steps & 1);
+        continue;
+      }
       tc::fence_after();
-      const int valid = plen - (first + j) * 128;
-      auto mask = [&](uint32_t (&v)[32], int i) {
+      uint32_t v[2][32];
+      tc::ld32(v[0], ts);
+      tc::ld32(v[1], ts + 32);
+      const int valid = plen - (first + j) * 128 - half * 64;
+      float mx[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        tc::wait_ld(v[i]);
         if (32 * i + 32 > valid) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (32 * i + e >= valid) v[e] = 0xff800000u;
+            if (32 * i + e >= valid) v[i][e] = 0xff800000u;
         }
-      };
-      auto most = [](const uint32_t (&v)[32], float mx) {
+        mx[i] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-        return mx;
-      };
-      uint32_t v[2][32];
-      float mx[4];
-#pragma unroll 1
-      for (int h = 1; h >= 0; --h) {                       // the second half is read again below
-        tc::ld32(v[0], ts + 64 * h);
-        tc::ld32(v[1], ts + 64 * h + 32);
-        tc::wait_ld(v[0]);
-        tc::wait_ld(v[1]);
-        mask(v[0], 2 * h);
-        mask(v[1], 2 * h + 1);
-        const float a = most(v[0], -INFINITY), b = most(v[1], -INFINITY);
-        mx[2] = h ? a : mx[2];
-        mx[3] = h ? b : mx[3];
-        mx[0] = a;
-        mx[1] = b;
+        for (int e = 0; e < 32; e += 2) mx[i] = max3(mx[i], __uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1]));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const float here = fmaxf(mx[0], mx[1]), top = fmaxf(here, both(here, steps & 1));
       const bool grew = top > m + room || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grew && steps > 0)) {   // (S of this step is there, so P V of the last one is done)
         const float f = !grew ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * sl);
@@ -238,63 +236,56 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
         l2[0] = fma2(l2[0], ff, 0ull);
         l2[1] = fma2(l2[1], ff, 0ull);
 #pragma unroll 1
-        for (int c = 0; c < HS; c += 32) {
-          uint32_t o[32];
-          tc::ld32(o, to + c);
+        for (int c = 0; c < HS / 2; c += 16) {
+          uint32_t o[16];
+          tc::ld16(o, to + c);
           tc::wait_ld(o);
-          uint32_t a[16], b[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            a[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            b[e] = __float_as_uint(__uint_as_float(o[16 + e]) * f);
-          }
-          st16(to + c, a);
-          st16(to + c + 16, b);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          st16(to + c, o);
         }
+        wait_st();
+      }
+      if (half) {      // both halves' outputs have shrunk before any product
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_half + 8 * t);
       }
       if (grew) m = top;
       const float org = m == -INFINITY ? 0.f : m * sl;
       const f2 sl2 = pk2(sl, sl), org2 = pk2(-org, -org);
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t hi[16], lo[16];
-          if (h) {
-            tc::wait_ld(v[i]);
-            mask(v[i], 2 + i);
-          }
+      for (int i = 0; i < 2; ++i) {
+        uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float a, b;
-            un2(fma2(pk2(__uint_as_float(v[i][2 * e]), __uint_as_float(v[i][2 * e + 1])), sl2, org2), a, b);
-            a = ex2(a);
-            b = ex2(b);
-            l2[e & 1] = add2(l2[e & 1], pk2(a, b));
-            hi[e] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-            un2(fma2(pk2(a, b), pk2(kAbove, kAbove), pk2(-bf16lo(hi[e]), -bf16hi(hi[e]))), a, b);
-            lo[e] = pack_bf16(a, b);
-          }
-          if (h == 0) tc::ld32(v[i], ts + 64 + 32 * i);
-          st16(ts + h * 64 + i * 32, hi);        // over their own scores: leading bits, rests
-          st16(ts + h * 64 + i * 32 + 16, lo);
+        for (int e = 0; e < 16; ++e) {
+          float a, b;
+          un2(fma2(pk2(__uint_as_float(v[i][2 * e]), __uint_as_float(v[i][2 * e + 1])), sl2, org2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          l2[e & 1] = add2(l2[e & 1], pk2(a, b));
+          hi[e] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+          un2(fma2(pk2(a, b), pk2(kAbove, kAbove), pk2(-bf16lo(hi[e]), -bf16hi(hi[e]))), a, b);
+          lo[e] = pack_bf16(a, b);
         }
-        wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive((h == 0 ? p_half : p_full) + 8 * t);
+        st16(ts + i * 32, hi);        // over their own scores: leading bits, rests
+        st16(ts + i * 32 + 16, lo);
       }
+      wait_st();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive((half ? p_full : p_half) + 8 * t);
     }
-    const int64_t slot = PAIR ? ((int64_t)item * splits + split) * 256 + tid : (((int64_t)item * splits + split) * 2 + t) * 128 + r;
+    const int64_t slot = PAIR ? ((int64_t)item * splits + split) * 256 + t * 128 + r : (((int64_t)item * splits + split) * 2 + t) * 128 + r;
     if (steps > 0 && ok) {
       // The rows go through shared memory, where nothing is read any more once both streams are done, and from there a row at a time: stored from registers, a warp's
       // 16 bytes of 32 rows take 32 sectors each; by a bulk copy of every thread's own row, 256 copies took 4500 clocks.
       ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, 0) && (!(PAIR || n > 1) || tc::mbar_wait(o_done + 8, 0)));
       tc::fence_after();
-      constexpr uint32_t LD = HS * 4 + 16;
+      constexpr uint32_t LD = HS * 2 + 16;      // half a row
       const uint32_t mine = smem + (uint32_t)tid * LD;
 #pragma unroll 1
-      for (int c = 0; c < HS && ok; c += 32) {
+      for (int c = 0; c < HS / 2 && ok; c += 32) {
         uint32_t o[32];
         tc::ld32(o, to + c);
         tc::wait_ld(o);
@@ -303,28 +294,27 @@ attn_shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensor
           asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(mine + (c + e) * 4), "r"(o[e]), "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3]) : "memory");
       }
       __syncwarp();
-      constexpr int LR = HS / 4, R = 32 / LR;   // lanes a row, rows at once
+      constexpr int LR = HS / 8, R = 32 / LR;   // lanes half a row, rows at once
       const uint32_t from = smem + (uint32_t)(tid - lane + lane / LR) * LD + lane % LR * 16;
-      float* const acc = p.pre_acc + (slot - lane + lane / LR) * HS + lane % LR * 4;
+      float* const acc = p.pre_acc + (slot - lane + lane / LR) * HS + half * (HS / 2) + lane % LR * 4;
       const int there = ok ? rows - (row - lane) - lane / LR : 0;
-#pragma unroll 8
+#pragma unroll 4
       for (int i = 0; i < 32; i += R) {
-        uint4 v;
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from + i * LD));
-        if (i < there) __stcg(reinterpret_cast<uint4*>(acc + i * HS), v);
+        uint4 x;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(from + i * LD));
+        if (i < there) __stcg(reinterpret_cast<uint4*>(acc + i * HS), x);
       }
     }
-    if (row < rows) {
-      float a, b, c, d;
-      un2(l2[0], a, b);
-      un2(l2[1], c, d);
-      __stcg(p.pre_ml + slot, make_float2(m == -INFINITY ? m : m * sl, (a + b) + (c + d)));
-    }
+    float a, b, c, d;
+    un2(l2[0], a, b);
+    un2(l2[1], c, d);
+    const float l = (a + b) + (c + d), all = l + both(l, steps & 1);   // (a step's buffer that no half still reads: the last one's was the other)
+    if (row < rows && half == 0) __stcg(p.pre_ml + slot, make_float2(m == -INFINITY ? m : m * sl, all));
   }
   if (!ok) *err = 1u;
   tc::fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     __syncwarp();
     tc::tmem_free<512>(tmem);
   }
