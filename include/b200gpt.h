@@ -306,6 +306,9 @@ typedef struct b200_attn_decode_shared_args {
 } b200_attn_decode_shared_args;
 size_t b200_attn_decode_shared_workspace_bytes(int batch, int n_head, int n_groups, int head_size, int prefix_rows, int own_rows);
 int b200_attn_decode_shared(const b200_attn_decode_shared_args* args, b200_stream_t stream);
+/* development / test knob: the prefix always in the list of tiles (1), always on the tensor memory (2), by size (0); returns the previous setting.  Workspaces are sized for
+ * the setting at the time. */
+int b200_attn_decode_shared_tune(int path);
 
 /* ---- prefill helper: RoPE + KV-cache write for T > 1 tokens at positions pos[0..T) (lit_gpt/model.py:624-649).
  * table_preselected = 1: cos/sin are (T, rope_n_elem) rows already gathered by input_pos; 0: full tables.

@@ -5,7 +5,7 @@
 //
 // The prefix is read once for all rows: the B * (heads per group) query rows of a key-value group are the left operand of its products, a key tile serves them all.
 // Three launches: the queries and new keys are turned and the new rows stored; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys of the
-// prefix for up to 32 query rows of a group (more: attn_shared_tc05.cu), and of a row's own keys for its heads of a group; a head's partial results are joined.  No counter or flag is left
+// prefix for up to 32 query rows of a group (the prefix's larger products: attn_shared_tc05.cu), and of a row's own keys for its heads of a group; a head's partial results are joined.  No counter or flag is left
 // between calls, and two calls at a time share nothing.
 //
 // All tiles, of the prefix and of all rows' own keys, are one list that is cut evenly over the warps of all SMs, so that neither few rows over a long prefix nor many
@@ -629,6 +629,8 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
   else *reinterpret_cast<uint32_t*>(out) = pack_bf16(a[0] * inv, a[1] * inv);
 }
 
+std::atomic<int> g_shared_path{0};   // b200_attn_decode_shared_tune
+
 struct SharedPlan {
   int np, no, head_tiles, row_tiles, ctas, workers, ways;   // np, no: eights of queries of a prefix's item and of an own one
   int64_t own_slots, pre_slots;   // rows
@@ -643,7 +645,11 @@ struct SharedPlan {
 SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows, int own_rows) {
   SharedPlan s;
   const int64_t rows = (int64_t)batch * per;
-  s.tensor = prefix_rows > 0 && rows > 32;
+  // The prefix on the tensor memory from so much work on: its kernel reads a key once for 256 rows, the list once for 32, but it is a launch more.  List and tensor memory, us:
+  // 48 rows of 8 groups x 2048 16.5, 19.5; 32 rows of 32 groups x 2048 26.3, 29.9; 24 rows of 8 groups x 8000 23.4, 23.5; 64 x 8000 34.1, 30.4; 32 x 16000 33.1, 29.2;
+  // up to 16 rows a tile of the list has no more products than eights: 16 rows of 8 groups x 8000 20.0, 22.3.
+  const int path = g_shared_path.load(std::memory_order_relaxed);
+  s.tensor = prefix_rows > 0 && (path ? path == 2 : rows > 16 && (int64_t)prefix_rows * n_groups * ((rows + 31) / 32) > 100000);
   s.pair = rows > 128;
   s.splits = s.pre_rows = s.pre_tiles = s.pre_parts = 0;
   if (s.tensor) {
@@ -651,8 +657,9 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
     s.pre_tiles = (int)((rows + s.pre_rows - 1) / s.pre_rows);
     const int64_t items = (int64_t)n_groups * s.pre_tiles, ranges = ((int64_t)prefix_rows + 127) / 128;
     // SMs for the prefix's kernel: the kernel of the own keys begins beside it on the others, so each has the share of SMs that its work asks for (own caches half full): a tile
-    // of 128 keys takes 2.15 us with 256 rows and @@ with 128, own keys come at 90 GB/s an SM.
-    const double prefix_work = (double)items * ranges * (s.pair ? 2.15 : 1.3), own_work = (double)batch * n_groups * own_rows * hs * 2 / 90e3;
+    // of 128 keys takes 2.15 us with 256 rows and 1.3 with 128, own keys come at 58 GB/s an SM.  64 rows x 16001 in 8 groups of 4 heads, up to 1000 own tokens, in 6, 9, 12, 18
+    // ranges 69, 54, 55, 64 us; 10 own tokens 63, 50, 43, 46; 4000 shared and up to 1000 own ones 42, 43, 47, 51 (3 ranges 46).
+    const double prefix_work = (double)items * ranges * (s.pair ? 2.15 : 1.3), own_work = (double)batch * n_groups * own_rows * hs * 2 / 58e3;
     const double share = sm_count() * prefix_work / (prefix_work + own_work) / items;
     s.splits = share < 1.0 ? 1 : share < (double)ranges ? (int)(share + 0.5) : (int)ranges;
     while (s.splits > 1 && s.splits * items > sm_count()) --s.splits;
@@ -722,6 +729,8 @@ size_t b200_attn_decode_shared_workspace_bytes(int batch, int n_head, int n_grou
   const SharedPlan s = shared_plan(batch, n_groups, n_head / n_groups, head_size, prefix_rows, own_rows);
   return s.bytes;
 }
+
+int b200_attn_decode_shared_tune(int path) { return g_shared_path.exchange(path == 1 || path == 2 ? path : 0); }
 
 int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a, "b200_attn_decode_shared: null argument");

@@ -1,5 +1,4 @@
-// Partial results of a decode step's query rows over the prefix that they share, more than 32 rows a key-value group, on the 5th-generation tensor cores
-// (attn_shared.cu has the step, and the path of fewer rows).
+// Partial results of a decode step's query rows over the prefix that they share, on the 5th-generation tensor cores (attn_shared.cu has the step, and says from where on).
 //
 // One CTA = 128 or 256 query rows of a group (rows of the batch times heads of the group) against a range of the prefix's keys, in tiles of 128 keys.  Two streams of products
 // and softmax, each with its scores and its output in tensor memory, fill each other's gaps: with 256 rows the halves of the rows, with 128 the even and the odd key tiles,

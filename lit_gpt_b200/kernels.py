@@ -927,6 +927,12 @@ def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     return y
 
 
+def attn_decode_shared_tune(path: int = 0) -> int:
+    """Test knob: the prefix of ``attn_decode_shared`` always in the list of tiles (1), always on the tensor memory (2), by size (0); returns the previous setting."""
+    _shared_workspace_bytes.cache_clear()
+    return int(C.load().b200_attn_decode_shared_tune(int(path)))
+
+
 def attn_decode_tune(force_scalar: bool = False) -> bool:
     """Test knob: route grouped-query shapes through the scalar decode-attention kernel; returns the previous setting."""
     return bool(C.load().b200_attn_decode_tune(int(force_scalar)))

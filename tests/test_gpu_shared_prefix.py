@@ -16,13 +16,16 @@ pytestmark = pytest.mark.gpu
 F64 = torch.float64
 
 
-@pytest.fixture(scope="module")
-def K():
+@pytest.fixture(params=["list", "tensor memory"])
+def K(request):
+    """The kernels with the prefix on either of its two ways, whatever the sizes say."""
     if not torch.cuda.is_available():
         pytest.skip("needs a CUDA device")
     from lit_gpt_b200 import kernels
 
-    return kernels
+    before = kernels.attn_decode_shared_tune(1 + (request.param != "list"))
+    yield kernels
+    kernels.attn_decode_shared_tune(before)
 
 
 def make(rows, groups, per, hs, prefix, cap, own, rope=None, table=torch.float32, seed=0):
@@ -243,3 +246,12 @@ def test_refusals(K):
             call(K, d, **change)
     with pytest.raises(K.C.B200Error):
         K.attn_decode_shared(t["qkv"], t["cos"], t["sin"], t["pos"], t["kc"], t["vc"], t["kp"], t["vp"], t["n"], 4, 2, 64, 64, table_preselected=True)
+
+
+@pytest.mark.parametrize("rows,groups,per,prefix", [(64, 8, 4, 1700), (64, 8, 4, 1500), (20, 8, 1, 13000), (16, 8, 1, 13000)])
+def test_either_way_by_size(rows, groups, per, prefix):
+    """Sizes on both sides of the rule: 64 x 4 rows of 8 groups over 1700 and 1500 keys, 20 and 16 rows over 13000."""
+    from lit_gpt_b200 import kernels
+
+    d = make(rows, groups, per, 128, prefix, 33, [i % 33 for i in range(rows)], seed=prefix)
+    check(call(kernels, d), formula(d))
