@@ -172,14 +172,6 @@ class DrawArgs(ctypes.Structure):  # mirrors b200_draw_args
                 ("pos_is_int64", c_int), ("history", c_void_p), ("history_ld", c_int64), ("history_len", c_int64)]
 
 
-class SlotTensor(ctypes.Structure):  # mirrors b200_slot_tensor
-    _fields_ = [("base", c_void_p), ("rows", c_int64), ("row_bytes", c_int64)]
-
-
-class SlotPair(ctypes.Structure):  # mirrors b200_slot_copy
-    _fields_ = [("src", ctypes.c_int32), ("dst", ctypes.c_int32), ("rows", c_int64)]
-
-
 class GatedResidualArgs(ctypes.Structure):  # mirrors b200_gated_residual_args
     _fields_ = [("y0", c_void_p), ("slot_of", c_void_p), ("wts", c_void_p), ("top", c_int), ("y1", c_void_p), ("gate", c_void_p), ("scale", c_void_p),
                 ("mult", c_float), ("x", c_void_p), ("w", c_void_p), ("plus_one", c_int), ("act", c_void_p), ("rows", c_int64), ("d", c_int), ("eps", c_float),
@@ -268,7 +260,7 @@ _CORE_SIGNATURES = {
                                 c_void_p]),
     "b200_adjust_logits": (c_int, [ctypes.POINTER(LogitRules), c_void_p, c_int, c_int64, c_void_p]),
     "b200_sample_rows": (c_int, [ctypes.POINTER(LogitRules), ctypes.POINTER(DrawArgs), c_void_p]),
-    "b200_copy_slots": (c_int, [ctypes.POINTER(SlotTensor), c_int, c_int, ctypes.POINTER(SlotPair), c_int, c_void_p]),
+    "b200_copy_slots": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),   # tables of b200_slot_tensor and b200_slot_copy, packed
 }
 _CORE_SHARED = ("b200_abi_version", "b200_last_error", "b200_device_info", "b200_set_pdl", "b200_launch_count", "b200_rmsnorm", "b200_swiglu",
                 "b200_embedding", "b200_argmax", "b200_sample", "b200_attn_prefill", "b200_wait_error", "b200_wait_errors_take", "b200_wait_probe")

@@ -7,7 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Dict, Optional, Sequence, Tuple, Union
+import struct
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 import torch._dynamo
@@ -596,23 +597,8 @@ def sample_(logits: torch.Tensor, token_out: torch.Tensor, temperature: float = 
 PerRow = Union[float, torch.Tensor]
 
 
-class _Device:
-    """A device made current for a launch, and the one before again behind it."""
-
-    def __init__(self, index: int, before: int) -> None:
-        self.index, self.before = index, before
-
-    def __enter__(self) -> None:
-        if self.index != self.before:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc: object) -> None:
-        if self.index != self.before:
-            torch.cuda.set_device(self.before)
-
-
-def _on(device: int) -> _Device:
-    return _Device(device, torch.cuda.current_device())
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device   # (no lazy initialisation: there is a CUDA tensor)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", C.stream_ptr)
 
 
 def _one_device(what: str, device: int, *tensors: Optional[torch.Tensor]) -> None:
@@ -626,19 +612,17 @@ def _per_row(value: PerRow, rows: int, dtype: torch.dtype, device: int, name: st
     """A setting that is one number for all rows or a tensor with one per row -> (tensor or None, number)."""
     if not isinstance(value, torch.Tensor):
         return None, value
-    if value.dtype is not dtype or value.shape != (rows,):
+    if value.dtype is not dtype or value.dim() != 1 or value.numel() != rows:
         raise C.B200Error(f"{name} must be a number or a {dtype} tensor of one per row (got {value.dtype}, {tuple(value.shape)} for {rows} rows)")
     if value.get_device() != device:
         _one_device(name, device, value)
     return value if value.is_contiguous() else value.contiguous(), 0
 
 
-def _rows_of(t: Optional[torch.Tensor], rows: int, cols: int, dtype: torch.dtype, device: int, name: str) -> int:
+def _rows_of(t: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, device: int, name: str) -> int:
     """Distance of the rows of a (rows, cols) tensor, 0 for a (cols,) one that all rows share."""
-    if t is None:
-        return 0
     shape, step = t.shape, t.stride()
-    if t.dtype is not dtype or (shape != (rows, cols) and shape != (cols,)):
+    if t.dtype is not dtype or shape[-1:] != (cols,) or len(shape) > 2 or (len(shape) == 2 and shape[0] != rows):
         raise C.B200Error(f"{name} must be {dtype}, ({cols},) or ({rows}, {cols}) (got {t.dtype}, {tuple(shape)})")
     if cols > 1 and step[-1] != 1:
         raise C.B200Error(f"{name}: the numbers of a row must lie next to each other")
@@ -652,24 +636,27 @@ def _logit_rules(what: str, logits: torch.Tensor, device: int, counts: Optional[
     """-> the rules and the tensors they point into."""
     if device < 0:
         C.require_cuda(logits)
-    dtype = logits.dtype
-    if logits.dim() != 2 or (dtype is not torch.bfloat16 and dtype is not torch.float32):
-        raise C.B200Error(f"{what}: logits must be bf16 or fp32 (rows, vocabulary) (got {dtype}, {tuple(logits.shape)})")
-    B, V = logits.shape
+    dtype, shape = logits.dtype, logits.shape
+    if len(shape) != 2 or (dtype is not torch.bfloat16 and dtype is not torch.float32):
+        raise C.B200Error(f"{what}: logits must be bf16 or fp32 (rows, vocabulary) (got {dtype}, {tuple(shape)})")
+    B, V = shape
     ld, step = logits.stride()
     if V > 1 and step != 1:
         logits = logits.contiguous()
         ld = V
-    rep, rep_all = _per_row(repetition, B, torch.float32, device, "repetition")
-    freq, freq_all = _per_row(frequency, B, torch.float32, device, "frequency")
-    pres, pres_all = _per_row(presence, B, torch.float32, device, "presence")
+    f32 = torch.float32
+    rep, rep_all = _per_row(repetition, B, f32, device, "repetition")
+    freq, freq_all = _per_row(frequency, B, f32, device, "frequency")
+    pres, pres_all = _per_row(presence, B, f32, device, "presence")
     if rep is None and not rep_all > 0.0:
         raise C.B200Error(f"{what}: repetition must be above zero (got {rep_all})")
     if counts is not None and counts.dim() != 2:
         raise C.B200Error(f"{what}: counts must be int32 (rows, vocabulary)")
-    rules = C.LogitRules(logits.data_ptr(), C.BF16 if dtype is torch.bfloat16 else C.F32, ld, B, V, C.ptr(counts), _rows_of(counts, B, V, torch.int32, device, "counts"),
-                         C.ptr(rep), C.ptr(freq), C.ptr(pres), rep_all, freq_all, pres_all, C.ptr(bias), _rows_of(bias, B, V, torch.float32, device, "bias"),
-                         C.ptr(allowed), _rows_of(allowed, B, (V + 31) // 32, torch.int32, device, "allowed"))
+    rules = C.LogitRules(logits.data_ptr(), C.BF16 if dtype is torch.bfloat16 else C.F32, ld, B, V,
+                         None if counts is None else counts.data_ptr(), 0 if counts is None else _rows_of(counts, B, V, torch.int32, device, "counts"),
+                         None if rep is None else rep.data_ptr(), None if freq is None else freq.data_ptr(), None if pres is None else pres.data_ptr(), rep_all, freq_all, pres_all,
+                         None if bias is None else bias.data_ptr(), 0 if bias is None else _rows_of(bias, B, V, f32, device, "bias"),
+                         None if allowed is None else allowed.data_ptr(), 0 if allowed is None else _rows_of(allowed, B, (V + 31) // 32, torch.int32, device, "allowed"))
     return rules, (logits, rep, freq, pres)
 
 
@@ -691,6 +678,9 @@ def adjust_logits(logits: torch.Tensor, *, counts: Optional[torch.Tensor] = None
     counts int32 (rows, V); repetition (> 0), frequency, presence: a number or fp32 (rows,); bias fp32 (V,) or (rows, V); allowed int32 (ceil(V / 32),) or
     (rows, ceil(V / 32)) as ``pack_allowed`` makes it."""
     device = logits.get_device()
+    if device >= 0 and device != _current_device():
+        with torch.cuda.device(device):
+            return adjust_logits(logits, counts=counts, repetition=repetition, frequency=frequency, presence=presence, bias=bias, allowed=allowed, out=out)
     rules, kept = _logit_rules("adjust_logits", logits, device, counts, repetition, frequency, presence, bias, allowed)
     if out is None:
         out = logits.new_empty(logits.shape, dtype=torch.float32)
@@ -698,9 +688,8 @@ def adjust_logits(logits: torch.Tensor, *, counts: Optional[torch.Tensor] = None
         raise C.B200Error(f"adjust_logits: out must be bf16 or fp32 {tuple(logits.shape)} on {logits.device}, the numbers of a row next to each other")
     elif kept[0] is not logits and out.data_ptr() == logits.data_ptr():
         raise C.B200Error("adjust_logits: in place the numbers of a row must lie next to each other")
-    with _on(device):
-        C.check(C.load_core().b200_adjust_logits(ctypes.byref(rules), out.data_ptr(), C.BF16 if out.dtype is torch.bfloat16 else C.F32, out.stride(0),
-                                                 torch._C._cuda_getCurrentRawStream(device)), "adjust_logits")
+    C.check(C.load_core().b200_adjust_logits(ctypes.byref(rules), out.data_ptr(), C.BF16 if out.dtype is torch.bfloat16 else C.F32, out.stride(0), _raw_stream(device)),
+            "adjust_logits")
     return out
 
 
@@ -716,6 +705,10 @@ def sample_rows_(logits: torch.Tensor, token_out: torch.Tensor, temperature: Per
     logprob_out fp32 (rows,): ln of the token's probability among those kept.  count: counts[b, token] += 1.  pos_inout (rows,): += 1, and then
     history[b, pos] = token where that lies inside ``history`` (rows, length)."""
     device = logits.get_device()
+    if device >= 0 and device != _current_device():
+        with torch.cuda.device(device):
+            return sample_rows_(logits, token_out, temperature, top_k, rng_state, noise=noise, counts=counts, repetition=repetition, frequency=frequency, presence=presence,
+                                bias=bias, allowed=allowed, count=count, logprob_out=logprob_out, pos_inout=pos_inout, history=history)
     rules, kept = _logit_rules("sample_rows_", logits, device, counts, repetition, frequency, presence, bias, allowed)
     B, V = logits.shape
     temp, temp_all = _per_row(temperature, B, torch.float32, device, "temperature")
@@ -738,12 +731,12 @@ def sample_rows_(logits: torch.Tensor, token_out: torch.Tensor, temperature: Per
     if count and (counts is None or (B > 1 and counts.stride(0) < V)):
         raise C.B200Error("sample_rows_: nothing to count in")
     _one_device("sample_rows_", device, token_out, rng_state, logprob_out, pos_inout, history)
-    args = C.DrawArgs(C.ptr(temp), temp_all, C.ptr(top), min(int(top_all), 2 ** 31 - 1), C.ptr(rng_state), C.ptr(noise),
-                      _rows_of(noise, B, V, torch.float32, device, "noise"), token_out.data_ptr(), kind is torch.int64, C.ptr(logprob_out), count, C.ptr(pos_inout),
+    args = C.DrawArgs(None if temp is None else temp.data_ptr(), temp_all, None if top is None else top.data_ptr(), min(int(top_all), 2 ** 31 - 1), C.ptr(rng_state),
+                      None if noise is None else noise.data_ptr(), 0 if noise is None else _rows_of(noise, B, V, torch.float32, device, "noise"), token_out.data_ptr(),
+                      kind is torch.int64, None if logprob_out is None else logprob_out.data_ptr(), count, C.ptr(pos_inout),
                       pos_inout is not None and pos_inout.dtype is torch.int64, C.ptr(history), 0 if history is None else history.stride(0),
                       0 if history is None else history.shape[1])
-    with _on(device):
-        C.check(C.load_core().b200_sample_rows(ctypes.byref(rules), ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), "sample_rows_")
+    C.check(C.load_core().b200_sample_rows(ctypes.byref(rules), ctypes.byref(args), _raw_stream(device)), "sample_rows_")
 
 
 def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], lengths: Optional[Sequence[int]] = None) -> None:
@@ -755,27 +748,27 @@ def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     if not tensors:
         return
     device, slots = tensors[0].get_device(), tensors[0].shape[0] if tensors[0].dim() else 0
-    table = []
-    for i, t in enumerate(tensors):
-        shape = t.shape
-        if len(shape) < 2 or shape[0] != slots or not t.is_contiguous():
-            raise C.B200Error(f"copy_slots: tensor {i} must be contiguous (slots, ...) with {slots} slots (got {tuple(shape)})")
-        nbytes = t.nbytes
-        if nbytes == 0:
-            raise C.B200Error(f"copy_slots: tensor {i} is empty")
+    if device >= 0 and device != _current_device():
+        with torch.cuda.device(device):
+            return copy_slots(tensors, src, dst, lengths)
+    table: List[int] = []
+    for t in tensors:
+        shape, numbers = t.shape, t.numel()
+        if len(shape) < 2 or shape[0] != slots or numbers == 0 or not t.is_contiguous():
+            raise C.B200Error(f"copy_slots: tensors must be contiguous (slots, ...) with {slots} slots and something in them (got {tuple(shape)})")
         if device < 0 or t.get_device() != device:
             _one_device("copy_slots", max(device, 0), t)
-        table.append((t.data_ptr(), shape[1], nbytes // (slots * shape[1])))
+        table += (t.data_ptr(), shape[1], numbers * t.element_size() // (slots * shape[1]))
     n = len(src)
     if lengths is None:
-        pairs = [(int(a), int(b), -1) for a, b in zip(src, dst)]
-    elif n and min(lengths) < 0:
-        raise C.B200Error(f"copy_slots: a copy of {min(lengths)} positions")
-    else:
-        pairs = [(int(a), int(b), int(c)) for a, b, c in zip(src, dst, lengths)]
-    with _on(device):
-        C.check(C.load_core().b200_copy_slots((C.SlotTensor * len(table))(*table), len(table), slots, (C.SlotPair * max(n, 1))(*pairs), n,
-                                              torch._C._cuda_getCurrentRawStream(device)), "copy_slots")
+        lengths = (-1,) * n
+    elif n and not (0 <= min(lengths) and max(lengths) < 2 ** 62):
+        raise C.B200Error(f"copy_slots: a copy of {min(lengths)} to {max(lengths)} positions")
+    if n and not (0 <= min(src) and max(src) < slots and 0 <= min(dst) and max(dst) < slots):
+        raise C.B200Error(f"copy_slots: copies from {list(src)} to {list(dst)}, of {slots} slots")
+    pairs = [int(v) for pair in zip(src, dst, lengths) for v in pair]
+    # b200_slot_tensor is three 64-bit numbers, b200_slot_copy two of 32 bits and one of 64
+    C.check(C.load_core().b200_copy_slots(struct.pack(f"@{len(table)}q", *table), len(tensors), slots, struct.pack("@" + "iiq" * n, *pairs), n, _raw_stream(device)), "copy_slots")
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -831,9 +824,13 @@ def attn_decode_shared(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     (B, G, rows, hs) bf16 hold row b's position p at p - n and are updated in place.  Any distance between groups and rows of a batch that is a multiple of 8
     numbers; rows of hs numbers next to each other.  Returns (B, H*hs)."""
     device, bf16 = qkv.get_device(), torch.bfloat16
-    if device < 0 or any(t.get_device() != device for t in (cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix)) or (prefix_len is not None and prefix_len.get_device() != device):
+    if (device < 0 or cos.get_device() != device or sin.get_device() != device or pos.get_device() != device or k_cache.get_device() != device or v_cache.get_device() != device
+            or k_prefix.get_device() != device or v_prefix.get_device() != device or (prefix_len is not None and prefix_len.get_device() != device)):
         C.require_cuda(qkv)
         _one_device("attn_decode_shared", device, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return attn_decode_shared(qkv, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len, n_head, n_groups, head_size, rope_n_elem, table_preselected)
     if qkv.dtype is not bf16 or not qkv.is_contiguous():
         qkv = _bf16c(qkv, "qkv")
     own, pre = k_cache.shape, k_prefix.shape
@@ -868,19 +865,19 @@ def attn_decode_shared(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     table = cos.shape
     if table != sin.shape or table[-1] != rope_n_elem or cos.dtype is not sin.dtype:
         raise C.B200Error(f"attn_decode_shared: cos and sin must be (positions, {rope_n_elem}) of one dtype")
-    cos, sin, pos = cos.contiguous(), sin.contiguous(), pos.contiguous()
+    if not (cos.is_contiguous() and sin.is_contiguous() and pos.is_contiguous()):
+        cos, sin, pos = cos.contiguous(), sin.contiguous(), pos.contiguous()
     table_rows = cos.numel() // max(rope_n_elem, 1)
     if table_preselected and table_rows != positions:
         raise C.B200Error(f"attn_decode_shared: {table_rows} preselected table rows for {positions} positions")
     out = qkv.new_empty((B, n_head * hs))
-    with _on(device):
-        nbytes = _shared_workspace_bytes(device, B, n_head, n_groups, hs, P, S)
-        ws = qkv.new_empty(max(nbytes // 2, 8))   # of this call: calls on two streams, or in two graphs, have one each
-        args = C.AttnDecodeSharedArgs(
-            qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, pos.data_ptr(), kind is torch.int64, positions,
-            None if prefix_len is None else prefix_len.data_ptr(), prefix_len is not None and prefix_len.dtype is torch.int64, k_cache.data_ptr(), v_cache.data_ptr(), kb, kg, vb, vg,
-            k_prefix.data_ptr(), v_prefix.data_ptr(), pkg, pvg, out.data_ptr(), B, n_head, n_groups, hs, S, P, ws.data_ptr(), nbytes)
-        C.check(C.load().b200_attn_decode_shared(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), "attn_decode_shared")
+    nbytes = _shared_workspace_bytes(device, B, n_head, n_groups, hs, P, S)
+    ws = qkv.new_empty(max(nbytes // 2, 8))   # of this call: calls on two streams, or in two graphs, have one each
+    args = C.AttnDecodeSharedArgs(
+        qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, pos.data_ptr(), kind is torch.int64, positions,
+        None if prefix_len is None else prefix_len.data_ptr(), prefix_len is not None and prefix_len.dtype is torch.int64, k_cache.data_ptr(), v_cache.data_ptr(), kb, kg, vb, vg,
+        k_prefix.data_ptr(), v_prefix.data_ptr(), pkg, pvg, out.data_ptr(), B, n_head, n_groups, hs, S, P, ws.data_ptr(), nbytes)
+    C.check(C.load().b200_attn_decode_shared(ctypes.byref(args), _raw_stream(device)), "attn_decode_shared")
     return out
 
 

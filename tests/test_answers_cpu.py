@@ -1,5 +1,6 @@
 """Several answers to one prompt, what needs no GPU: refusals of the C entry points before any launch, the bookkeeping of forked and compacted requests."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -18,8 +19,8 @@ def refused(rc, text):
 
 
 def copies(tensors, slots, pairs):
-    table = (C.SlotTensor * max(len(tensors), 1))(*[C.SlotTensor(*t) for t in tensors])
-    pair = (C.SlotPair * max(len(pairs), 1))(*[C.SlotPair(*p) for p in pairs])
+    table = struct.pack("@" + "qqq" * len(tensors), *[v or 0 for t in tensors for v in t])
+    pair = struct.pack("@" + "iiq" * len(pairs), *[v for p in pairs for v in p])
     return C.load().b200_copy_slots(table, len(tensors), slots, pair, len(pairs), None)
 
 
