@@ -784,7 +784,7 @@ int b200_adjust_logits(const b200_logit_rules* rules, void* out, int out_dtype, 
  * state rng_state[b] = (seed, offset), whose offset moves on by one; temperature <= 0: argmax, the lowest token of equal ones.  NaN logits are never drawn.  A row
  * that allows nothing gives token -1 and log-probability -inf.  logprob_out[b] (optional): ln of the token's probability among those kept (temperature <= 0: among
  * all, at temperature 1).  count: rules->counts[b, token] += 1.  pos_inout[b] (optional) += 1, and history[b, pos] = token where pos < history_len.
- * temperature, top_k: one per row on the device, or NULL for the number in *_all.  The result does not depend on how rows are cut or which run with them. */
+ * temperature, top_k: one per row on the device, or NULL for the number in *_all.  A row's token depends on its own numbers alone. */
 typedef struct b200_draw_args {
   const float* temperature; float temperature_all;
   const int32_t* top_k; int top_k_all;

@@ -525,10 +525,13 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
 
   // ---- weights and scores; a thread's best and whether another of its own comes close ----
   // What threads have is added as whole numbers, and gathered tokens each: the sum does not depend on the order that they were gathered in.
-  const float inv2 = fminf((greedy ? 1.f : 1.f / T) * 1.4426950408889634f, 3.4028234e38f);
+  // powers of two: gap * log2(e) / T, and what the product and the quotient were rounded by, which a weight of 2^-20 would otherwise have 2e-6 of its own of
+  const float t = greedy ? 1.f : T, inv2 = fminf(1.44269502f / t, 3.4028234e38f);
+  const float inv2_rest = inv2 < 1e30f && t < 1e30f ? (fmaf(-inv2, t, 1.44269502f) + 1.925963e-8f) / t : 0.f;
   const float unit = __int_as_float((127 + __clz(V) + 30) << 23);   // 2^(30 + leading zeros): V of them stay below 2^63
   auto power_of = [&](float l) { return (l == M ? 0.f : l - M) * inv2; };
   auto score_of = [&](float l, float e) { return greedy ? l : power_of(l) - lg2(e); };
+  const uint64_t one = __float2ull_rz(unit);                        // the largest logit's weight; beside it what is small keeps its digits
   uint64_t sum = 0ull;
   float best = -INFINITY, second = -INFINITY, best_l = 0.f;
   int index = 0x7fffffff;
@@ -539,7 +542,8 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
     best = first ? s : best;
     best_l = first ? l : best_l;
     index = first ? v : index;
-    return ex2(power);
+    const float gap = l == M ? 0.f : l - M, w = ex2(power), rest = fmaf(gap, inv2, -power) + gap * inv2_rest;
+    return power > -126.f ? fmaf(w, rest * 0.693147181f, w) : 0.f;
   };
   if (alone) {
 #pragma unroll 1
@@ -549,6 +553,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
     }
   } else if (M > -INFINITY) {
     float part = 0.f;
+    int tops = 0;
     constexpr int G = 4;   // quads of a thread whose noise is on its way together
 #pragma unroll 1
     for (int q0 = tid; q0 < quads; q0 += G * NT) {
@@ -585,10 +590,14 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
         logits4(q, l);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (select ? kept(l[i], v0 + 4 * q + i) : l[i] > -INFINITY) part += weigh(l[i], e[g][i], v0 + 4 * q + i);
+          if (select ? kept(l[i], v0 + 4 * q + i) : l[i] > -INFINITY) {
+            const float w = weigh(l[i], e[g][i], v0 + 4 * q + i);
+            tops += l[i] == M;
+            part += l[i] == M ? 0.f : w;
+          }
       }
     }
-    sum = __float2ull_rz(part * unit);
+    sum = __float2ull_rz(part * unit) + (uint64_t)tops * one;
   }
   const float mine = best;
   // the warp's, then the warps'
@@ -704,7 +713,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
   const int64_t tok = none ? -1 : index;
   if (a.token64) reinterpret_cast<int64_t*>(a.token)[b] = tok;
   else reinterpret_cast<int32_t*>(a.token)[b] = (int32_t)tok;
-  if (a.logprob) a.logprob[b] = none ? -INFINITY : (best_l == M ? 0.f : (greedy ? best_l - M : (best_l - M) / T)) - logf(__ull2float_rn(sum) / unit);
+  if (a.logprob) a.logprob[b] = none ? -INFINITY : (best_l == M ? 0.f : (greedy ? best_l - M : (best_l - M) / T)) - log1pf(__ull2float_rn(sum > one ? sum - one : 0ull) / unit);
   if (a.rng) a.rng[2 * b + 1] = (int64_t)(offset + 1ull);
   if (a.count && !none) a.count[(int64_t)b * r.counts_ld + tok] += 1;
   if (a.pos) {

@@ -158,6 +158,24 @@ def test_draw_large_vocabularies(K):
         check_draw(K, d, 0.0, 0, None)
 
 
+def test_log_probabilities_of_near_certain_tokens(K):
+    """One logit far above the others: ln p = -ln(1 + d), d the others' weights, of which each is off by 2^-22 (ex2), its exponent's rounding being carried along, and the gap's own
+    rounding of 2^-24, times the exponent (at most 30) and ln 2: 2e-6 at the worst, for the last bit of gaps that are no fp32 numbers.  Weights are added as multiples of
+    2^-(30 + leading zeros of V as a 32-bit number), 2^-50 for V = 3000, cut off below: every weight above 2^-50 (two here, those of -60 are nothing) by that much."""
+    V = 3000
+    for gap in (2.0, 8.0, 16.0, 20.0):
+        logits = torch.full((1, V), -60.0)
+        logits[0, 7], logits[0, 2000], logits[0, 2500] = gap, 0.0, 0.25
+        for k, T in ((0, 1.0), (2, 1.0), (3, 0.7), (500, 1.3)):
+            tok, lp = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, device="cuda")
+            K.sample_rows_(logits.cuda(), tok, T, k, noise=torch.ones(V, device="cuda"), logprob_out=lp)
+            want = drawn(logits[0].numpy(), np.float32(T), k, np.ones(V, dtype=np.float32))
+            assert tok.item() == want[0] == 7
+            rest = np.sort((logits[0].double().numpy() - gap) / float(np.float32(T)))[::-1][1 : k if k else V]
+            exact = -np.log1p(np.exp(rest).sum())
+            assert abs(lp.item() - exact) <= 2e-6 * abs(exact) + 2 * 2 ** -50, (gap, k, T, lp.item(), exact)
+
+
 def test_draw_equal_logits(K):
     """Equal logits at the threshold are kept in the order of the tokens; of equal largest ones the lowest token."""
     V = 9000

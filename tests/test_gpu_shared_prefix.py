@@ -185,6 +185,70 @@ def test_infinite_values_and_keys(K, rows):
     check(got, formula(d))
 
 
+def test_more_rows_than_a_cta_has_threads(K):
+    rows = 900
+    d = make(rows, 1, 1, 64, 40, 70, [-1 if i % 7 == 3 or 300 <= i < 340 else i % 70 for i in range(rows)], seed=4)
+    check(call(K, d), formula(d))
+
+
+def test_offsets_past_32_bits(K):
+    """The third row's cache and the third group's prefix begin behind 2^31 numbers."""
+    d = make(3, 3, 2, 128, 50, 20, [7, 0, 19], seed=6)
+    long = 9_000_000
+
+    caches = []
+    for t in (d["kc"], d["vc"]):
+        flat = torch.empty(2 * long * 128 + 3 * 20 * 128, dtype=torch.bfloat16, device="cuda")
+        view = flat.as_strided((3, 3, 20, 128), (long * 128, 20 * 128, 128, 1))
+        view.copy_(t)
+        caches.append(view)
+    prefixes = []
+    for t in (d["kp"], d["vp"]):
+        flat = torch.empty(2 * long * 128 + 50 * 128, dtype=torch.bfloat16, device="cuda")
+        view = flat.as_strided((3, 50, 128), (long * 128, 128, 1))
+        view.copy_(t)
+        prefixes.append(view)
+    check(call(K, d, kc=caches[0], vc=caches[1], kp=prefixes[0], vp=prefixes[1]), formula(d))
+
+
+def test_another_stream(K):
+    d = make(20, 2, 4, 128, 300, 40, [i % 40 for i in range(20)], seed=9)
+    t = {k: v.cuda() if torch.is_tensor(v) else v for k, v in d.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = K.attn_decode_shared(t["qkv"], t["cos"], t["sin"], t["pos"], t["kc"], t["vc"], t["kp"], t["vp"], t["n"], 8, 2, 128, 128)
+    side.synchronize()
+    check((got, t["kc"], t["vc"]), formula(d))
+
+
+def test_same_result_every_time(K):
+    d = make(48, 4, 2, 128, 2100, 200, [(i * 29) % 200 for i in range(48)], seed=10)
+    first = call(K, d)[0]
+    for _ in range(5):
+        assert torch.equal(first, call(K, d)[0])
+
+
+def test_every_kernel_launch_waits_for_the_one_before(K):
+    """Steps one behind the other, each on what the step before left, with and without launches that begin early."""
+    for early in (True, False):
+        before = K.set_pdl(early)
+        try:
+            d = make(6, 2, 4, 128, 200, 40, [0] * 6, seed=11)
+            t = {k: v.cuda() if torch.is_tensor(v) else v for k, v in d.items()}
+            for i in range(12):
+                t["pos"].fill_(200 + i)
+                t["qkv"].copy_(d["qkv"].roll(i, 0))
+                out = K.attn_decode_shared(t["qkv"], t["cos"], t["sin"], t["pos"], t["kc"], t["vc"], t["kp"], t["vp"], t["n"], 8, 2, 128, 128)
+            for i in range(12):
+                e = dict(d, qkv=d["qkv"].roll(i, 0), pos=torch.full((6,), 200 + i))
+                want = formula(e)
+                d["kc"], d["vc"] = want[2], want[3]
+            check((out, t["kc"], t["vc"]), want)
+        finally:
+            K.set_pdl(before)
+
+
 def test_scores_of_hundreds(K):
     d = make(20, 1, 2, 128, 333, 12, [i % 12 for i in range(20)])
     d["qkv"] *= 16
