@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
       uint32_t rnd[4];
       philox4x32_10((uint32_t)(v >> 2), 0u, (uint32_t)offset, (uint32_t)(offset >> 32), (uint32_t)seed, (uint32_t)(seed >> 32), rnd);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = -__logf(((float)(rnd[i] >> 8) + 0.5f) * (1.0f / 16777216.0f));
+      for (int i = 0; i < 4; ++i) e[i] = fmaxf(-__logf(((float)(rnd[i] >> 8) + 0.5f) * (1.0f / 16777216.0f)), 2.98023224e-8f);   // (the last of 2^24 numbers is rounded to 1: not 0 but 2^-25)
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = fminf(e[i], 3.4028234e38f);

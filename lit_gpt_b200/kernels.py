@@ -731,7 +731,7 @@ def sample_rows_(logits: torch.Tensor, token_out: torch.Tensor, temperature: Per
     if count and (counts is None or (B > 1 and counts.stride(0) < V)):
         raise C.B200Error("sample_rows_: nothing to count in")
     _one_device("sample_rows_", device, token_out, rng_state, logprob_out, pos_inout, history)
-    args = C.DrawArgs(None if temp is None else temp.data_ptr(), temp_all, None if top is None else top.data_ptr(), min(int(top_all), 2 ** 31 - 1), C.ptr(rng_state),
+    args = C.DrawArgs(None if temp is None else temp.data_ptr(), temp_all, None if top is None else top.data_ptr(), max(min(int(top_all), 2 ** 31 - 1), 0), C.ptr(rng_state),
                       None if noise is None else noise.data_ptr(), 0 if noise is None else _rows_of(noise, B, V, torch.float32, device, "noise"), token_out.data_ptr(),
                       kind is torch.int64, None if logprob_out is None else logprob_out.data_ptr(), count, C.ptr(pos_inout),
                       pos_inout is not None and pos_inout.dtype is torch.int64, C.ptr(history), 0 if history is None else history.stride(0),

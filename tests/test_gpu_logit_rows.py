@@ -290,6 +290,26 @@ def test_random_states(K):
         assert freq[p == 0].sum() == 0 and (freq - p).abs().max() < 0.04
 
 
+@pytest.mark.parametrize("seed,token", [(207, 39758), (836, 28258), (909, 20637)])
+def test_the_last_random_number_draws_nothing_by_itself(K, seed, token):
+    """The states at whose offset 0 `token`'s 24 random bits are all ones: its u is rounded to 1, and an e of 0 would win over any logit.  Another token's lead of 40 is more than
+    -ln of the smallest e (17.4) and ln of the largest (ln 17.4 = 2.9) together."""
+    c, M = [token // 4, 0, 0, 0], 0xFFFFFFFF
+    k0, k1 = seed, 0
+    for _ in range(10):
+        a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [b >> 32 ^ c[1] ^ k0, b & M, a >> 32 ^ c[3] ^ k1, a & M]
+        k0, k1 = k0 + 0x9E3779B9 & M, k1 + 0xBB67AE85 & M
+    assert c[token % 4] >> 8 == 0xFFFFFF
+    logits = torch.zeros(2, 50257)
+    logits[:, 11] = 40.0
+    tok = torch.zeros(2, dtype=torch.int64, device="cuda")
+    K.sample_rows_(logits.cuda(), tok, 1.0, None, torch.tensor([[seed, 0], [seed, 0]], device="cuda"))
+    assert tok.tolist() == [11, 11]
+    K.sample_rows_(logits.cuda(), tok, 1.0, 50256, torch.tensor([[seed, 0], [seed, 0]], device="cuda"))
+    assert tok.tolist() == [11, 11]
+
+
 def test_no_rows(K):
     empty = torch.empty(0, 50, device="cuda")
     assert K.adjust_logits(empty).shape == (0, 50)
