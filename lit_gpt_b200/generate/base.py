@@ -308,8 +308,8 @@ class SampleGraph:
         if self.logprobs is not None:
             self.logprobs.index_copy_(1, self.pos[:1], self.logprob[:, None])
 
-    def _step(self) -> None:
-        self.draw(self.model(self.token.view(-1, 1), self.pos[:1])[:, -1])   # (all rows are at one position)
+    def _step(self, token: torch.Tensor) -> None:
+        self.draw(self.model(token.view(-1, 1), self.pos[:1])[:, -1])   # (all rows are at one position)
 
     def capture(self) -> None:
         held = [t for t in (self.token, self.pos, self.rng, self.counts) if t is not None]
@@ -324,18 +324,18 @@ class SampleGraph:
         with torch.cuda.stream(side):   # warm-up outside capture (DecodeGraph.capture)
             for _ in range(2):
                 put_back()
-                self._step()
+                self._step(self.token)
         torch.cuda.current_stream().wait_stream(side)
         put_back()
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
-            self._step()
+            self._step(self.token)
 
     def step(self) -> None:
         if self.graph is not None:
             self.graph.replay()
         else:
-            self._step()
+            self._step(self.token.clamp(min=0))   # (-1 of a row that has ended without a token: the fused step's embedding reads row 0 for it by itself)
 
     @contextlib.contextmanager
     def in_place(self):
@@ -422,10 +422,12 @@ def generate_samples(model: GPT, prompt: torch.Tensor, max_returned_tokens: int,
                 if eos_id is not None and bool((sg.history[:, T : T + done] == eos_id).any(1).all()):   # the only host sync of the loop
                     break
         answers = sg.history[:, T : T + done].clone()
-        ends = [done] * rows
+        none = answers < 0
+        last = torch.where(none.any(1), none.int().argmax(1), done)
         if eos_id is not None:
             hit = answers == eos_id
-            ends = torch.where(hit.any(1), hit.int().argmax(1) + 1, done).tolist()
+            last = torch.where(hit.any(1), torch.minimum(hit.int().argmax(1) + 1, last), last)
+        ends = last.tolist()
         tokens += [torch.cat((prompt, answers[i, :n])) for i, n in enumerate(ends)]
         if logprobs:
             given = sg.logprobs[:, T : T + done].clone()

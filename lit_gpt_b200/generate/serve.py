@@ -173,6 +173,8 @@ def _generate_ruled(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens
     out = [list(p) for p in prompts for _ in range(num_samples)]
     if N == 0 or max_new_tokens <= 0:
         return out
+    if not all(out):
+        raise ValueError("a prompt has one token at least")
     if logit_bias and not all(0 <= t < V for t in logit_bias):
         raise ValueError(f"logit_bias names tokens outside 0 .. {V - 1}")
     rng = row_rng_states(dev, N) if temperature > 0.0 else None
@@ -207,25 +209,26 @@ def _generate_ruled(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens
 
     ids = [("gen", i) for i in range(N)]
     live, budget = list(range(N)), [max_new_tokens] * N
-    first = session.step([(ids[p * num_samples], prompts[p], [len(prompts[p]) - 1]) for p in range(len(prompts))])
-    for p in range(len(prompts)):
-        session.fork(ids[p * num_samples], ids[p * num_samples + 1 : (p + 1) * num_samples])
-    nxt = draw(first.repeat_interleave(num_samples, 0), live)
-    while live:
-        done = []
-        for i, t in zip(live, nxt):
-            if t >= 0:
-                out[i].append(t)
-            budget[i] -= 1
-            if t < 0 or budget[i] <= 0 or t == eos_id or len(out[i]) >= model.max_seq_length:
-                done.append(i)
-        live = [i for i in live if i not in done]
-        if not live:
-            session.step([], end=[ids[i] for i in done])
-            break
-        logits = session.step([(ids[i], [out[i][-1]], None) for i in live], end=[ids[i] for i in done])
-        nxt = draw(logits, live)
-    return out
+    try:
+        first = session.step([(ids[p * num_samples], prompts[p], [len(prompts[p]) - 1]) for p in range(len(prompts))])
+        for p in range(len(prompts)):
+            session.fork(ids[p * num_samples], ids[p * num_samples + 1 : (p + 1) * num_samples])
+        nxt = draw(first.repeat_interleave(num_samples, 0), live)
+        while True:
+            done = []
+            for i, t in zip(live, nxt):
+                if t >= 0:
+                    out[i].append(t)
+                budget[i] -= 1
+                if t < 0 or budget[i] <= 0 or t == eos_id or len(out[i]) >= model.max_seq_length:
+                    done.append(i)
+            live = [i for i in live if i not in done]
+            if not live:
+                return out
+            logits = session.step([(ids[i], [out[i][-1]], None) for i in live], end=[ids[i] for i in done])
+            nxt = draw(logits, live)
+    finally:
+        session.step([], end=ids)   # (also when the grammar raises: the slots are the session's again)
 
 
 class Replayer:

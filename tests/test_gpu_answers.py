@@ -110,6 +110,21 @@ def test_answers_end_at_eos_and_obey_their_rules(golden):
     assert len(one) == 4 and all(len(y) == T + 1 for y in one)
 
 
+@pytest.mark.parametrize("mode", ["nf4", None])
+@torch.inference_mode()
+def test_an_answer_ends_where_nothing_can_be_drawn(golden, mode):
+    import lit_gpt_b200.generate.base as gb
+
+    model, *_, prompt = toy(golden, mode)
+    p, T = prompt.cuda(), len(prompt)
+    nothing = {t: float("-inf") for t in range(model.config.padded_vocab_size)}
+    ys, lps = gb.generate_samples(model, p, T + 12, 3, temperature=0.9, logit_bias=nothing, logprobs=True)
+    assert all(torch.equal(y.cpu(), prompt) for y in ys) and all(lp.numel() == 0 for lp in lps)
+    ys = gb.generate_samples(model, p, T + 12, 3, temperature=0.9, logit_bias=nothing, eos_id=5)
+    assert all(torch.equal(y.cpu(), prompt) for y in ys)
+    assert all(len(y) == T + 12 for y in gb.generate_samples(model, p, T + 12, 3, temperature=0.9))
+
+
 @torch.inference_mode()
 def test_one_captured_step_serves_prompts_of_all_lengths(golden):
     import lit_gpt_b200.generate.base as gb
@@ -178,13 +193,17 @@ def test_traced_step_over_a_shared_prefix(golden):
 # ---- models that serve sequences from slots -----------------------------------------------------------------------------------------
 def _kinds():
     import test_gpu_fizadra as F
+    import test_gpu_fovirax as X
     import test_gpu_lefalix as L
+    import test_gpu_nulezen as N
     import test_gpu_pomipel as P
+    import test_gpu_votavik as V
 
-    return {"lefalix": (L, L.CFG_ODD, {}), "pomipel": (P, P.CFG_ODD, dict(max_seq=200)), "fizadra": (F, F.CFG_ODD, dict(max_seq=200))}
+    return {"lefalix": (L, L.CFG_ODD, {}), "pomipel": (P, P.CFG_ODD, dict(max_seq=200)), "fizadra": (F, F.CFG_ODD, dict(max_seq=200)), "nulezen": (N, N.CFG_ODD, {}),
+            "votavik": (V, V.CFG_ODD, {}), "fovirax": (X, X.CFG_ODD, {})}
 
 
-@pytest.mark.parametrize("kind", ["lefalix", "pomipel", "fizadra"])
+@pytest.mark.parametrize("kind", ["lefalix", "pomipel", "fizadra", "nulezen", "votavik", "fovirax"])
 def test_forked_requests_go_their_own_ways(kind):
     from lit_gpt_b200.generate.serve import Session
 
@@ -203,7 +222,7 @@ def test_forked_requests_go_their_own_ways(kind):
             session.fork("p", new)
     follow = {r: mod.tokens_for(cfg, 12, 30 + i) for i, r in enumerate("pabcq")}
     seq = {r: (other if r == "q" else prompt) + follow[r] for r in follow}
-    alone = {r: mod.O.forward(cfg, w, t) for r, t in seq.items()}
+    alone = {r: mod.O.forward(cfg[0] if isinstance(cfg, tuple) else cfg, w, t) for r, t in seq.items()}
     start = {r: len(seq[r]) - 12 for r in seq}
 
     def steps(live, first, last, end=()):
@@ -268,3 +287,15 @@ def test_batches_of_samples_and_rules(kind):
     with pytest.raises(ValueError):
         generate_batch(model, prompts, 5, logit_bias={V: 1.0})
     assert generate_batch(model, [], 5, num_samples=2) == [] and generate_batch(model, prompts, 0, num_samples=2) == [prompts[0]] * 2 + [prompts[1]] * 2
+
+    def broken(i, tokens):
+        if len(tokens) == len(prompts[i // 2]) + 3:
+            raise RuntimeError("no such rule")
+
+    with pytest.raises(RuntimeError, match="no such rule"):
+        generate_batch(model, prompts, 8, num_samples=2, allowed=broken, session=session)
+    assert not session.live and model.slots.in_use == 0
+    assert generate_batch(model, prompts, 8, num_samples=2, session=session) == [plain[0][:17]] * 2 + [plain[1][:12]] * 2
+    with pytest.raises(ValueError, match="one token at least"):
+        generate_batch(model, [[], prompts[0]], 5, num_samples=2, session=session)
+    assert not session.live
