@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kAdjThreads) adjust_kernel(const Rules r, OT* 
 
 // ---- the draw -----------------------------------------------------------------------------------------------------------------------
 // A row's tokens are cut into the slices of a cluster's CTAs; a slice's adjusted logits stay in shared memory (CACHED) and are read again by the later steps.
-// NT threads a CTA: 512 while rows are few, 256, of which three CTAs fit an SM, where they fill the GPU.
+// NT threads a CTA: 512, or 256, of which three CTAs fit an SM.
 constexpr int kSaDigit = 10, kSaBins = 1 << kSaDigit, kSaCtas = 8;
 constexpr int kSaGather = 1024;   // tokens that one CTA goes on with alone
 constexpr float kNear = 1.5e-3f;  // scores, in powers of two, this close to the best are compared in 64 bits
@@ -727,31 +727,89 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 3) sample_rows_kernel(cons
   }
 }
 
-constexpr int kSaMaxSlice = 48 * 1024;   // floats: 192 KB beside 21 KB of histograms and gathered tokens
+constexpr int kSaMaxSlice = 48 * 1024;   // floats: 192 KB beside the histograms and gathered tokens
+constexpr int kSaOwnBytes = 22 * 1024;   // those, rounded up
+
+template <typename LT, bool CACHED, bool WIDE, int NT>
+cudaError_t allow_slices() {
+  static PerDeviceOnce once;
+  if (!once.need()) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<LT, CACHED, WIDE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSaMaxSlice * (int)sizeof(float));
+  if (e == cudaSuccess) once.done();
+  return e;
+}
+
+// CTAs of NT threads that an SM has place for beside each other, by their slices
+template <int NT>
+int ctas_an_sm(int slice) {
+  const int by_memory = 228 * 1024 / (slice * (int)sizeof(float) + kSaOwnBytes + 1024), most = NT == 512 ? 2 : 3;
+  return by_memory < most ? by_memory : most;
+}
+// Clusters that the GPU has at once (a cluster's SMs are neighbours: of 8 CTAs, two an SM, 148 SMs have 33, not 37).  Asked once per device.
+template <int NT>
+int clusters_at_once(int ctas, int an_sm) {
+  static std::atomic<int> known[64][kSaCtas + 1][4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  std::atomic<int>& here = known[dev & 63][ctas][an_sm];
+  int n = here.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (allow_slices<float, true, true, NT>() == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = an_sm == 1 ? kSaMaxSlice * sizeof(float) : 228 * 1024 / an_sm - kSaOwnBytes - 1024;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_rows_kernel<float, true, true, NT>, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+  }
+  if (n <= 0) n = sm_count() * an_sm / ctas > 1 ? sm_count() * an_sm / ctas : 1;
+  here.store(n, std::memory_order_relaxed);
+  return n;
+}
+// What a draw takes, us, but for what all of them take: 3.5 for each further round of clusters, and per round by the SM that has most of it: 0.5 per 1000 tokens, 0.58 with CTAs
+// of 256 threads, 0.7 and 1.1 if it has one CTA only; more CTAs of a cluster or of an SM wait for one another a little longer.  Against 34 sizes, 1 to 600 rows of 1000 to 150000
+// tokens with and without a top-k, the CTAs chosen take 1.035 times the time of the best ones on average, 1.22 at worst (48 x 32000).
+template <int NT>
+float draw_time(int rows, int ctas, int slice) {
+  const int an_sm = ctas_an_sm<NT>(slice), once = clusters_at_once<NT>(ctas, an_sm), full = (rows - 1) / once, rest = rows - full * once;
+  const int last = (rest * ctas + sm_count() - 1) / sm_count();
+  auto tokens = [&](int n) { return (n == 1 ? (NT == 512 ? 0.7f : 1.1f) : (NT == 512 ? 0.5f : 0.58f) * (float)n) * 1e-3f * (float)slice; };
+  return 3.5f * (float)full + (float)full * tokens(an_sm) + tokens(last < an_sm ? last : an_sm) + (float)ctas * (0.15f + 0.5f * (float)rows / (float)sm_count());
+}
 
 template <typename LT, bool CACHED, bool WIDE, int NT>
 cudaError_t launch_draw_as(const Rules& r, const DrawArgs& a, int ctas, cudaStream_t st) {
   if (CACHED) {
-    static PerDeviceOnce once;
-    if (once.need()) {
-      const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<LT, CACHED, WIDE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSaMaxSlice * (int)sizeof(float));
-      if (e != cudaSuccess) return e;
-      once.done();
-    }
+    const cudaError_t e = allow_slices<LT, CACHED, WIDE, NT>();
+    if (e != cudaSuccess) return e;
   }
   return launch_cluster(sample_rows_kernel<LT, CACHED, WIDE, NT>, dim3((unsigned)(r.rows * ctas)), dim3(NT), ctas, CACHED ? (size_t)a.slice * sizeof(float) : 0, st, r, a);
 }
 
 template <typename LT>
 cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
-  // few rows: clusters of eight CTAs of 512 threads, as far as slices of 2048 tokens allow.  Rows that fill the GPU: CTAs of 256 threads, three an SM
-  const bool few = r.rows * kSaCtas <= 2 * sm_count();
-  int ctas = few ? kSaCtas : 3 * sm_count() / r.rows;
-  ctas = ctas < r.vocab / 2048 ? ctas : r.vocab / 2048;
-  const int least = (r.vocab + kSaMaxSlice - 1) / kSaMaxSlice;
-  ctas = ctas > least ? ctas : least;
-  ctas = ctas < 1 ? 1 : ctas > kSaCtas ? kSaCtas : ctas;
-  a.slice = ((r.vocab + ctas - 1) / ctas + 3) & ~3;
+  // The cluster's CTAs, each with 1024 tokens at least, and their threads: the shortest of draw_time.  us, k = 50, of clusters of 1, 2, 3, 4, 6, 8 CTAs of 512 threads, of 256:
+  //   1 x 32000   25.5 17.7 15.6 14.3 13.1 12.7, 37.4 23.2 18.7 17.0 15.4 14.1;     38 x 50304   25.6 25.5 24.2 21.9 19.6 27.9, 35.8 35.8 28.5 26.1 23.4 22.1
+  //   96 x 50257  47.2 47.4 38.0 38.6 42.6 47.8, 65.9 65.8 49.7 30.3 39.9 42.0;     200 x 32000  51.7 38.5 46.7 47.4 59.1 72.8, 77.1 51.6 42.9 41.9 52.7 62.5
+  const int sizes = r.vocab / 1024, most = sizes < 1 ? 1 : sizes < kSaCtas ? sizes : kSaCtas, least = (r.vocab + kSaMaxSlice - 1) / kSaMaxSlice;
+  auto slice_of = [&](int ctas) { return ((r.vocab + ctas - 1) / ctas + 3) & ~3; };
+  int ctas = kSaCtas;
+  bool few = true;
+  float best = INFINITY;
+  for (int c = least; c <= most; ++c) {
+    const float wide_cta = draw_time<512>(r.rows, c, slice_of(c)), narrow = draw_time<256>(r.rows, c, slice_of(c));
+    if (wide_cta <= best) { best = wide_cta; ctas = c; few = true; }
+    if (narrow < best) { best = narrow; ctas = c; few = false; }
+  }
+  a.slice = slice_of(ctas);
   // four tokens an access where every row of everything that is there begins on such a boundary
   auto whole = [&](const void* p, int64_t ld, int bytes) { return !p || (((uintptr_t)p & (4 * bytes - 1)) == 0 && (r.rows == 1 || (ld & 3) == 0)); };
   const bool wide = whole(r.logits, r.ld, (int)sizeof(LT)) && whole(r.counts, r.counts_ld, 4) && whole(r.bias, r.bias_ld, 4) && whole(a.noise, a.noise_ld, 4);
@@ -789,6 +847,7 @@ int b200_adjust_logits(const b200_logit_rules* rules, void* out, int out_dtype, 
   if (const int rc = check_rules(rules, "b200_adjust_logits", &r)) return rc;
   B200_CHECK_ARG((out || r.rows == 0) && (out_dtype == B200_BF16 || out_dtype == B200_F32), "b200_adjust_logits: the result is bf16 or fp32");
   B200_CHECK_ARG(out_ld >= r.vocab || r.rows <= 1, "b200_adjust_logits: result rows overlap");
+  B200_CHECK_ARG(out != r.logits || (out_dtype == rules->logits_dtype && (out_ld == r.ld || r.rows <= 1)), "b200_adjust_logits: in place the result has the logits' type and distance");
   if (r.rows == 0) return B200_OK;
   const int each = kAdjThreads * kAdjQuads * 4, chunks = (r.vocab + each - 1) / each;
   B200_CHECK_ARG((int64_t)chunks * r.rows < 0x7fffffff, "b200_adjust_logits: too many logits");

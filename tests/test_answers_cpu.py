@@ -50,6 +50,8 @@ def test_logit_rules_are_checked():
     refused(adjust(out=None), "result")
     refused(adjust(dtype=C.F16), "result")
     refused(adjust(apart=7), "overlap")
+    refused(adjust(dtype=C.BF16), "in place")
+    refused(adjust(apart=16), "in place")
     refused(lib.b200_adjust_logits(None, FAKE, C.F32, 8, None), "null")
     draw = lambda **kw: lib.b200_sample_rows(ctypes.byref(C.LogitRules(**ok)), ctypes.byref(C.DrawArgs(**{**dict(token_out=FAKE, noise=FAKE), **kw})), None)
     refused(draw(token_out=None), "null")
