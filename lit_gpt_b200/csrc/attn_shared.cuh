@@ -37,7 +37,7 @@ __device__ __forceinline__ int prefix_len(const SharedParams& p) {
   return (int)(n < 0 ? 0 : (n > p.prefix_rows ? p.prefix_rows : n));
 }
 
-// Partial results of a group's query rows over the prefix, on the tensor memory.  splits: key ranges of an item; two items' worth of rows a CTA where `pair`
+// Partial results of a group's query rows over the prefix, on the tensor memory.  splits: key ranges of an item; pair: 256 query rows a CTA, else 128
 cudaError_t launch_attn_shared_prefix(const SharedParams& p, int head_size, bool pair, int splits, cudaStream_t st);
 
 }  // namespace b200
