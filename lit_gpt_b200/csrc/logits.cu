@@ -753,10 +753,8 @@ int ctas_an_sm(int slice) {
 }
 // Clusters that the GPU has at once (a cluster's SMs are neighbours: of 8 CTAs, two an SM, 148 SMs have 33, not 37).  Asked once per device.
 template <int NT>
-int clusters_at_once(int ctas, int an_sm) {
+int clusters_at_once(int dev, int sms, int ctas, int an_sm) {
   static std::atomic<int> known[64][kSaCtas + 1][4];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
   std::atomic<int>& here = known[dev & 63][ctas][an_sm];
   int n = here.load(std::memory_order_relaxed);
   if (n > 0) return n;
@@ -776,7 +774,7 @@ int clusters_at_once(int ctas, int an_sm) {
       n = 0;
     }
   }
-  if (n <= 0) n = sm_count() * an_sm / ctas > 1 ? sm_count() * an_sm / ctas : 1;
+  if (n <= 0) n = sms * an_sm / ctas > 1 ? sms * an_sm / ctas : 1;
   here.store(n, std::memory_order_relaxed);
   return n;
 }
@@ -784,11 +782,11 @@ int clusters_at_once(int ctas, int an_sm) {
 // of 256 threads, 0.7 and 1.1 if it has one CTA only; more CTAs of a cluster or of an SM wait for one another a little longer.  Against 34 sizes, 1 to 600 rows of 1000 to 150000
 // tokens with and without a top-k, the CTAs chosen take 1.035 times the time of the best ones on average, 1.22 at worst (48 x 32000).
 template <int NT>
-float draw_time(int rows, int ctas, int slice) {
-  const int an_sm = ctas_an_sm<NT>(slice), once = clusters_at_once<NT>(ctas, an_sm), full = (rows - 1) / once, rest = rows - full * once;
-  const int last = (rest * ctas + sm_count() - 1) / sm_count();
+float draw_time(int dev, int sms, int rows, int ctas, int slice) {
+  const int an_sm = ctas_an_sm<NT>(slice), once = clusters_at_once<NT>(dev, sms, ctas, an_sm), full = (rows - 1) / once, rest = rows - full * once;
+  const int last = (rest * ctas + sms - 1) / sms;
   auto tokens = [&](int n) { return (n == 1 ? (NT == 512 ? 0.7f : 1.1f) : (NT == 512 ? 0.5f : 0.58f) * (float)n) * 1e-3f * (float)slice; };
-  return 3.5f * (float)full + (float)full * tokens(an_sm) + tokens(last < an_sm ? last : an_sm) + (float)ctas * (0.15f + 0.5f * (float)rows / (float)sm_count());
+  return 3.5f * (float)full + (float)full * tokens(an_sm) + tokens(last < an_sm ? last : an_sm) + (float)ctas * (0.15f + 0.5f * (float)rows / (float)sms);
 }
 
 template <typename LT, bool CACHED, bool WIDE, int NT>
@@ -807,11 +805,13 @@ cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
   //   96 x 50257  47.2 47.4 38.0 38.6 42.6 47.8, 65.9 65.8 49.7 30.3 39.9 42.0;     200 x 32000  51.7 38.5 46.7 47.4 59.1 72.8, 77.1 51.6 42.9 41.9 52.7 62.5
   const int sizes = r.vocab / 1024, most = sizes < 1 ? 1 : sizes < kSaCtas ? sizes : kSaCtas, least = (r.vocab + kSaMaxSlice - 1) / kSaMaxSlice;
   auto slice_of = [&](int ctas) { return ((r.vocab + ctas - 1) / ctas + 3) & ~3; };
-  int ctas = kSaCtas;
+  int ctas = kSaCtas, dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  const int sms = sm_count();
   bool few = true;
   float best = INFINITY;
   for (int c = least; c <= most; ++c) {
-    const float wide_cta = draw_time<512>(r.rows, c, slice_of(c)), narrow = draw_time<256>(r.rows, c, slice_of(c));
+    const float wide_cta = draw_time<512>(dev, sms, r.rows, c, slice_of(c)), narrow = draw_time<256>(dev, sms, r.rows, c, slice_of(c));
     if (wide_cta <= best) { best = wide_cta; ctas = c; few = true; }
     if (narrow < best) { best = narrow; ctas = c; few = false; }
   }
