@@ -306,7 +306,8 @@ typedef struct b200_attn_decode_shared_args {
 } b200_attn_decode_shared_args;
 size_t b200_attn_decode_shared_workspace_bytes(int batch, int n_head, int n_groups, int head_size, int prefix_rows, int own_rows);
 int b200_attn_decode_shared(const b200_attn_decode_shared_args* args, b200_stream_t stream);
-/* development / test knob: the prefix always in the list of tiles (1), always on the tensor memory (2), by size (0); returns the previous setting.  Workspaces are sized for
+/* development / test knob: the prefix always in the list of tiles (1), always on the tensor memory (2), a group's step always by a cluster where
+ * its rows are few enough (3), by size (0); returns the previous setting.  Workspaces are sized for
  * the setting at the time. */
 int b200_attn_decode_shared_tune(int path);
 

@@ -6,9 +6,9 @@
 // The prefix is read once for all rows: the B * (heads per group) query rows of a key-value group are the left operand of its products, a key tile serves them all.
 // Three launches: the queries and new keys are turned and the new rows stored; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys of the
 // prefix for up to 32 query rows of a group (the prefix's larger products: attn_shared_tc05.cu), and of a row's own keys for its heads of a group; a head's partial
-// results are joined.  No counter or flag is left between calls, and two calls at a time share nothing.
+// results are joined.  Few rows a group: the whole of it in one launch, a cluster of CTAs a group.  No counter or flag is left between calls, and two calls at a time share nothing.
 //
-// Bound: a few short rows by latency: 2 rows of 32 heads over 96 shared keys take 9.7 us, 1.8 MB.  Else by bytes: 16 rows of 32 heads over 2048 shared and 200 own
+// Bound: a few short rows by latency: 2 rows of 32 heads over 96 shared keys take 7.2 us, 1.8 MB (10.0 in three launches).  Else by bytes: 16 rows of 32 heads over 2048 shared and 200 own
 // keys, 87 MB, take 25 us (3.5 TB/s): 13 at the memory's rate, the rest the way to the first tile, the queries' launch before it and the join behind it.
 //
 // All tiles, of the prefix and of all rows' own keys, are one list that is cut evenly over the warps of all SMs, so that neither few rows over a long prefix nor many
@@ -323,10 +323,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8 x 8 matri
   return r;
 }
 
-// 8 N queries and a tile of keys: S^T = K Q^T and O^T += V^T P^T, keys and dimensions as the rows of the products, so that few queries cost few of them.  `vb` of the
+// 8 N queries, from row q0 of `q` on, and a tile of keys: S^T = K Q^T and O^T += V^T P^T, keys and dimensions as the rows of the products, so that few queries cost few of them.  `vb` of the
 // values is what `values` gives, which waits for them.
 template <int HS, int NQ, int N, typename Values>
-__device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, uint32_t kb, int valid, float scale_log2, int lane, Values values) {
+__device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, int q0, uint32_t kb, int valid, float scale_log2, int lane, Values values) {
   const int g = lane >> 2;
   float s[kShTile / 16][N][4];
 #pragma unroll
@@ -337,7 +337,7 @@ __device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, uint32_
   for (int kp = 0; kp < HS / 32; ++kp) {
     uint32_t qf[N][4];
 #pragma unroll
-    for (int t = 0; t < N; ++t) ldsm_x4(qf[t], q + sw<HS>(t * 8 + (lane & 7), kp * 4 + (lane >> 3)));
+    for (int t = 0; t < N; ++t) ldsm_x4(qf[t], q + sw<HS>(q0 + t * 8 + (lane & 7), kp * 4 + (lane >> 3)));
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -398,6 +398,29 @@ __device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, uint32_
   }
 }
 
+// The first `valid` queries' results to a slot
+template <int HS, int NQ>
+__device__ __forceinline__ void store_sums(const Sums<HS, NQ>& a, float* acc, float2* ml, int valid, int lane) {
+  const int g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int t = 0; t < NQ; ++t)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = a.l[t][c];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const int r = t * 8 + 2 * tq + c;
+      if (r < valid) {
+#pragma unroll
+        for (int i = 0; i < HS / 16; ++i) {
+          __stcg(acc + r * HS + i * 16 + g, a.o[i][t][c]);
+          __stcg(acc + r * HS + i * 16 + 8 + g, a.o[i][t][2 + c]);
+        }
+        if (g == 0) __stcg(ml + r, make_float2(a.m[t][c], l));
+      }
+    }
+}
+
 template <int HS, int NP, int NO>
 __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_kernel(const SharedParams p) {
   using C = ShSmem<HS, NP>;
@@ -405,7 +428,7 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
   constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
   extern __shared__ __align__(128) uint8_t sh_smem[];
   __shared__ int s_sums[T + 1], s_mine[T], s_warp[C::kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_launch();
   const int plen = prefix_len(p);
   const Split s = make_split<T>(p, plen, s_sums, s_mine, s_warp);
@@ -491,8 +514,8 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
       __syncwarp();
       return vb;
     };
-    if (NP == NO || cur.own) attend_tile<HS, NQ, NO>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
-    else attend_tile<HS, NQ, NP>(a, sq + qb * C::kQ, kb, cur.valid, p.scale_log2, lane, values);
+    if (NP == NO || cur.own) attend_tile<HS, NQ, NO>(a, sq + qb * C::kQ, 0, kb, cur.valid, p.scale_log2, lane, values);
+    else attend_tile<HS, NQ, NP>(a, sq + qb * C::kQ, 0, kb, cur.valid, p.scale_log2, lane, values);
     __syncwarp();                                          // the values have been read: the keys of the tile after the next take their place
     const bool ends = cur.left == 0 || !more;
     Tile was = cur;
@@ -512,32 +535,82 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
         int2* const where = was.own ? p.own_where : p.pre_where;
         __stcg(where + item, make_int2(w, worker_of(was.index + was.left, s) - w + 1));
       }
-      const int rows = was.own ? min(16, p.per) : 8 * NP, valid = walk.queries(was);
-      float* const acc = (was.own ? p.own_acc : p.pre_acc) + slot * rows * HS;
-      float2* const ml = (was.own ? p.own_ml : p.pre_ml) + slot * rows;
-#pragma unroll
-      for (int t = 0; t < NQ; ++t)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float l = a.l[t][c];
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-          const int r = t * 8 + 2 * tq + c;
-          if (r < valid) {
-#pragma unroll
-            for (int i = 0; i < HS / 16; ++i) {
-              __stcg(acc + r * HS + i * 16 + g, a.o[i][t][c]);
-              __stcg(acc + r * HS + i * 16 + 8 + g, a.o[i][t][2 + c]);
-            }
-            if (g == 0) __stcg(ml + r, make_float2(a.m[t][c], l));
-          }
-        }
+      const int rows = was.own ? min(16, p.per) : 8 * NP;
+      store_sums<HS, NQ>(a, (was.own ? p.own_acc : p.pre_acc) + slot * rows * HS, (was.own ? p.own_ml : p.pre_ml) + slot * rows, walk.queries(was), lane);
       if (!more) break;
       clear();
     }
   }
   pf_wait<0>();
   if (late && blockIdx.x == gridDim.x - 1) griddep_wait();
+}
+
+// Results first, first + step, .. of n, V numbers a lane, four on their way at a time; where(i): the i-th result's maximum and sum, and its numbers
+template <int V, typename Where>
+__device__ __forceinline__ void join_results(int first, int step, int n, int lane, float& top, float& sum, float (&a)[V], Where where) {
+  for (int i0 = first; i0 < n; i0 += 4 * step) {
+    float2 e[4];
+    float v[4][V];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * step;
+      e[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[u][j] = 0.f;
+      if (i < n) {
+        const float2* ml;
+        const float* acc;
+        where(i, ml, acc);
+        e[u] = __ldcg(ml);
+        if constexpr (V == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(acc + lane * V));
+          v[u][0] = x.x; v[u][1] = x.y; v[u][V - 2] = x.z; v[u][V - 1] = x.w;
+        } else {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(acc + lane * V));
+          v[u][0] = x.x; v[u][1] = x.y;
+        }
+      }
+    }
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) now = fmaxf(now, e[u].x);
+    const float org = now == -INFINITY ? 0.f : now, shrink = ex2(top - org);
+    top = now;
+    sum *= shrink;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] *= shrink;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float c = ex2(e[u].x - org);
+      sum += e[u].y * c;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] += e[u].y == 0.f ? 0.f : v[u][j] * c;   // (a range that saw nothing has no result)
+    }
+  }
+}
+
+// What the next ways - 1 warps left in shared memory, to the first one's
+template <int HS>
+__device__ __forceinline__ void join_warps(const float* acc, const float2* ml, int ways, int lane, float& top, float& sum, float (&a)[HS / 32]) {
+  constexpr int V = HS / 32;
+  float now = top;
+  for (int u = 1; u < ways; ++u) now = fmaxf(now, ml[u].x);
+  const float org = now == -INFINITY ? 0.f : now, c0 = ex2(top - org);
+  sum *= c0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) a[j] *= c0;
+  for (int u = 1; u < ways; ++u) {
+    const float c = ex2(ml[u].x - org);
+    sum += ml[u].y * c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] += acc[u * HS + lane * V + j] * c;
+  }
+}
+template <int HS>
+__device__ __forceinline__ void store_result(__nv_bfloat16* out, const float (&a)[HS / 32], float inv, int lane) {
+  constexpr int V = HS / 32;
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(out + lane * V) = make_uint2(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[V - 2] * inv, a[V - 1] * inv));
+  else *reinterpret_cast<uint32_t*>(out + lane * V) = pack_bf16(a[0] * inv, a[1] * inv);
 }
 
 // A head's results joined: `ways` warps a head, HS / 32 numbers a lane.
@@ -567,45 +640,12 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
     }
     const int64_t own_at = (own_item + own.x) * own_rows + hh % 16;
     const int own_n = own.y, n = own_n + pre.y;
-    for (int i0 = way; i0 < n; i0 += 4 * p.ways) {
-      float2 e[4];
-      float v[4][V];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * p.ways;
-        e[u] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[u][j] = 0.f;
-        if (i < n) {
-          const bool mine = i < own_n;
-          const int64_t at = mine ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * pre_step;
-          e[u] = __ldcg((mine ? p.own_ml : p.pre_ml) + at);
-          const float* const src = (mine ? p.own_acc : p.pre_acc) + at * HS + lane * V;
-          if constexpr (V == 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-            v[u][0] = x.x; v[u][1] = x.y; v[u][V - 2] = x.z; v[u][V - 1] = x.w;
-          } else {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-            v[u][0] = x.x; v[u][1] = x.y;
-          }
-        }
-      }
-      float now = top;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) now = fmaxf(now, e[u].x);
-      const float org = now == -INFINITY ? 0.f : now, shrink = ex2(top - org);
-      top = now;
-      sum *= shrink;
-#pragma unroll
-      for (int j = 0; j < V; ++j) a[j] *= shrink;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float c = ex2(e[u].x - org);
-        sum += e[u].y * c;
-#pragma unroll
-        for (int j = 0; j < V; ++j) a[j] += e[u].y == 0.f ? 0.f : v[u][j] * c;   // (a range that saw nothing has no result)
-      }
-    }
+    join_results<V>(way, p.ways, n, lane, top, sum, a, [&](int i, const float2*& ml, const float*& acc) {
+      const bool mine = i < own_n;
+      const int64_t at = mine ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * pre_step;
+      ml = (mine ? p.own_ml : p.pre_ml) + at;
+      acc = (mine ? p.own_acc : p.pre_acc) + at * HS;
+    });
   }
   if (p.ways > 1) {
 #pragma unroll
@@ -613,24 +653,230 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(const SharedParam
     if (lane == 0) s_ml[warp] = make_float2(top, sum);
     __syncthreads();
     if (way != 0) return;
-    float now = top;
-    for (int u = 1; u < p.ways; ++u) now = fmaxf(now, s_ml[warp + u].x);
-    const float org = now == -INFINITY ? 0.f : now, c0 = ex2(top - org);
-    sum *= c0;
+    join_warps<HS>(s_acc[warp], s_ml + warp, p.ways, lane, top, sum, a);
+  }
+  if (h < p.n_head) store_result<HS>(p.out + ((int64_t)b * p.n_head + h) * HS, a, idle ? 0.f : 1.f / sum, lane);
+}
+
+// ---- few query rows a group: the step of a group by a cluster, in one launch ----
+// The three launches above wait for one another, which is most of a short step's time.  Here each CTA of a group's cluster turns the group's few queries and new keys itself, its
+// warps share the group's key tiles with those of the others, and behind the cluster's barrier they join the results.
+constexpr int kClHeads = 32;   // heads that a CTA turns, queries, keys and values of all rows
+constexpr int kClCtas = 8;
+
+template <int HS, int NP>
+struct ClSmem {
+  static constexpr int kUnit = kShTile * HS * 2, kWarps = HS == 64 ? 12 : 7, kQRows = 16 * NP, kNew = kClHeads / 3;
+  static constexpr int kQ = kWarps * kShUnits * kUnit, kNewKeys = kQ + kQRows * HS * 2, kNewValues = kNewKeys + kNew * HS * 2, kBytes = kNewValues + kNew * HS * 2;
+};
+
+template <int HS, int NP>
+__global__ void __launch_bounds__(ClSmem<HS, NP>::kWarps * 32, 1) attn_shared_cluster_kernel(const SharedParams p, int ctas) {
+  using C = ClSmem<HS, NP>;
+  constexpr int W = C::kWarps, V = HS / 32, CH = HS / 8, RP = 32 / CH;
+  extern __shared__ __align__(128) uint8_t sh_smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gi = blockIdx.x / ctas, rank = blockIdx.x - gi * ctas;
+  const uint32_t smem = pf_smem(sh_smem), ring = smem + warp * kShUnits * C::kUnit, sq = smem + C::kQ;
+  griddep_wait();
+  griddep_launch();
+  // lane b: row b's newest own key, the first of its tiles
+  const int plen = prefix_len(p), rows = p.batch * p.per;
+  const int64_t pos_of = lane < p.batch ? row_pos(p, lane) : -1;
+  const int at = own_index(p, pos_of, plen), here = (at + kShTile) / kShTile;
+  int inc = here;
 #pragma unroll
-    for (int j = 0; j < V; ++j) a[j] *= c0;
-    for (int u = 1; u < p.ways; ++u) {
-      const float c = ex2(s_ml[warp + u].x - org);
-      sum += s_ml[warp + u].y * c;
+  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+  const int first = inc - here;
+  Split s;
+  s.own = __shfl_sync(0xffffffffu, inc, 31);
+  s.prefix = (plen + kShTile - 1) / kShTile;
+  s.all = s.own + s.prefix;
+  s.workers = min(s.all, ctas * W);
+  s.each = s.workers ? s.all / s.workers : 0;
+  s.more = s.all - s.each * s.workers;
+  const int w = warp * ctas + rank;
+  const int begin = w < s.workers ? first_tile(w, s) : s.all, end = w < s.workers ? first_tile(w + 1, s) : s.all;
+
+  struct Place { const __nv_bfloat16* k; const __nv_bfloat16* v; int stored, valid, own, b, last; };   // stored: rows that lie in the cache already; the newest one comes behind them
+  auto find = [&](int t) {
+    Place x;
+    x.own = t < s.own;
+    if (x.own) {
+      x.b = __popc(__ballot_sync(0xffffffffu, lane < p.batch && first <= t)) - 1;
+      const int newest = __shfl_sync(0xffffffffu, at, x.b), tile = t - __shfl_sync(0xffffffffu, first, x.b);
+      x.k = p.kc + (int64_t)x.b * p.kc_b + (int64_t)gi * p.kc_g + (int64_t)tile * kShTile * HS;
+      x.v = p.vc + (int64_t)x.b * p.vc_b + (int64_t)gi * p.vc_g + (int64_t)tile * kShTile * HS;
+      x.last = tile == newest / kShTile;
+      x.stored = x.last ? newest % kShTile : kShTile;
+      x.valid = x.stored + x.last;
+    } else {
+      const int tile = t - s.own;
+      x.b = 0;
+      x.k = p.kp + (int64_t)gi * p.kp_g + (int64_t)tile * kShTile * HS;
+      x.v = p.vp + (int64_t)gi * p.vp_g + (int64_t)tile * kShTile * HS;
+      x.last = tile == s.prefix - 1;
+      x.stored = x.valid = min(kShTile, plen - tile * kShTile);
+    }
+    return x;
+  };
+  auto load = [&](uint32_t dst, const __nv_bfloat16* src, int valid) {   // zeros from `valid` on
 #pragma unroll
-      for (int j = 0; j < V; ++j) a[j] += s_acc[warp + u][lane * V + j] * c;
+    for (int j = 0; j < kShTile / RP; ++j) {
+      const int r = j * RP + lane / CH, c = lane % CH;
+      const bool ok = r < valid;
+      pf_cp16(dst + sw<HS>(r, c), src + (ok ? r * HS : 0) + c * 8, ok);
+    }
+  };
+  Place cur = {}, coming = {};
+  if (begin < end) {
+    cur = find(begin);
+    load(ring, cur.k, cur.stored);
+    pf_commit();
+    load(ring + C::kUnit, cur.v, cur.stored);
+    pf_commit();
+    if (begin + 1 < end) {
+      coming = find(begin + 1);
+      load(ring + 2 * C::kUnit, coming.k, coming.stored);
+    }
+    pf_commit();
+  }
+
+  // ---- the group's queries, keys and values of this step ----
+  auto put = [&](uint32_t dst, const uint32_t (&v)[HS / 64]) {
+    if constexpr (V == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(dst), "r"(v[0]), "r"(v[V / 2 - 1]) : "memory");
+    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v[0]) : "memory");
+  };
+  auto row_of = [&](uint32_t base, int r) { return base + sw<HS>(r, lane * V * 2 / 16) + lane * V * 2 % 16; };
+  const int heads = p.batch * (p.per + 2);
+#pragma unroll 1
+  for (int i = warp; i < heads; i += W) {
+    const int b = i / (p.per + 2), h = i - b * (p.per + 2), mine = __shfl_sync(0xffffffffu, at, b);
+    const int64_t pos = __shfl_sync(0xffffffffu, pos_of, b);
+    const __nv_bfloat16* const x = p.qkv + (((int64_t)b * p.n_groups + gi) * (p.per + 2) + h) * HS;
+    uint32_t v[HS / 64];
+    if (h <= p.per) {
+      turned_part<HS>(p, x, table_row(p, b, pos), lane, v);
+    } else {
+      const uint16_t* const n = reinterpret_cast<const uint16_t*>(x + lane * V);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) v[j] = (uint32_t)n[2 * j] | ((uint32_t)n[2 * j + 1] << 16);
+    }
+    if (h < p.per) {
+      if (pos < 0)
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) v[j] = 0u;
+      put(row_of(sq, b * p.per + h), v);
+    } else {
+      put(smem + (h == p.per ? C::kNewKeys : C::kNewValues) + (b * HS + lane * V) * 2, v);
+      if (rank == 0 && mine >= 0) {
+        __nv_bfloat16* const to = (h == p.per ? p.kc + (int64_t)b * p.kc_b + (int64_t)gi * p.kc_g : p.vc + (int64_t)b * p.vc_b + (int64_t)gi * p.vc_g) + (int64_t)mine * HS + lane * V;
+        if constexpr (V == 4) *reinterpret_cast<uint2*>(to) = make_uint2(v[0], v[V / 2 - 1]);
+        else *reinterpret_cast<uint32_t*>(to) = v[0];
+      }
     }
   }
-  if (h >= p.n_head) return;
-  const float inv = idle ? 0.f : 1.f / sum;
-  __nv_bfloat16* const out = p.out + ((int64_t)b * p.n_head + h) * HS + lane * V;
-  if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[V - 2] * inv, a[V - 1] * inv));
-  else *reinterpret_cast<uint32_t*>(out) = pack_bf16(a[0] * inv, a[1] * inv);
+  for (int r = rows + warp; r < C::kQRows; r += W) {
+    const uint32_t none[HS / 64] = {};
+    put(row_of(sq, r), none);
+  }
+  __syncthreads();
+
+  // ---- the key tiles ----
+  const int own_rows = p.per, slots = p.batch + p.workers;   // (workers: the most of a cluster)
+  if (begin < end) {
+    auto newest = [&](uint32_t unit, uint32_t news) {   // the row that the caches do not hold yet
+      if (cur.own && cur.last) {
+        uint32_t v[HS / 64];
+        const uint32_t src = smem + news + (cur.b * HS + lane * V) * 2;
+        if constexpr (V == 4) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[V / 2 - 1]) : "r"(src) : "memory");
+        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(src) : "memory");
+        put(row_of(unit, cur.stored), v);
+      }
+      __syncwarp();
+    };
+    Sums<HS, NP> a;
+    auto clear = [&]() {
+#pragma unroll
+      for (int t = 0; t < NP; ++t) {
+#pragma unroll
+        for (int i = 0; i < HS / 16; ++i) a.o[i][t][0] = a.o[i][t][1] = a.o[i][t][2] = a.o[i][t][3] = 0.f;
+        a.m[t][0] = a.m[t][1] = -INFINITY;
+        a.l[t][0] = a.l[t][1] = 0.f;
+      }
+    };
+    clear();
+    int unit = 0;                                          // of the current tile's keys
+    for (int t = begin;; ++t) {
+      const uint32_t kb = ring + unit * C::kUnit;
+      unit = unit == kShUnits - 1 ? 0 : unit + 1;
+      const uint32_t vb = ring + unit * C::kUnit;
+      unit = unit == kShUnits - 1 ? 0 : unit + 1;
+      const bool more = t + 1 < end;
+      pf_wait<2>();
+      __syncwarp();
+      newest(kb, C::kNewKeys);
+      auto values = [&]() {
+        __syncwarp();                                      // the keys have been read: the values of the next tile take their place
+        if (more) load(kb, coming.v, coming.stored);
+        pf_commit();
+        pf_wait<2>();
+        __syncwarp();
+        newest(vb, C::kNewValues);
+        return vb;
+      };
+      attend_tile<HS, NP, NP>(a, sq, cur.own ? cur.b * p.per : 0, kb, cur.valid, p.scale_log2, lane, values);   // (own keys with as many columns: the code of fewer is fetched, too)
+      __syncwarp();                                        // the values have been read: the keys of the tile after the next take their place
+      const bool ends = cur.last || !more;
+      const int own = cur.own, b = cur.b;
+      cur = coming;
+      if (t + 2 < end) {
+        coming = find(t + 2);
+        load(vb, coming.k, coming.stored);
+      }
+      pf_commit();
+      if (ends) {
+        const int64_t slot = own ? (int64_t)gi * slots + b + w : (int64_t)gi * p.workers + w;
+        const int size = own ? own_rows : 8 * NP;
+        store_sums<HS, NP>(a, (own ? p.own_acc : p.pre_acc) + slot * size * HS, (own ? p.own_ml : p.pre_ml) + slot * size, own ? p.per : rows, lane);
+        if (!more) break;
+        clear();
+      }
+    }
+    pf_wait<0>();
+  }
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+
+  // ---- the results joined: heads in turn to the CTAs, there as many warps a head as there are for it ----
+  const int joined = (rows + ctas - 1) / ctas, ways = joined < W ? W / joined : 1, once = W / ways, way = warp % ways;
+  float* const s_acc = reinterpret_cast<float*>(sh_smem) + warp * HS;      // (over the ring, which nothing reads any more)
+  float2* const s_ml = reinterpret_cast<float2*>(sh_smem + W * HS * sizeof(float)) + warp;
+  for (int h0 = 0; h0 < joined; h0 += once) {
+    const int r = rank + ctas * (h0 + warp / ways);
+    const bool here = warp / ways < once && r < rows;
+    const int b = here ? r / p.per : 0, newest = __shfl_sync(0xffffffffu, at, b), t0 = __shfl_sync(0xffffffffu, first, b);
+    float top = -INFINITY, sum = 0.f, a[V] = {};
+    if (here && newest >= 0) {
+      const int own_w = worker_of(t0, s), own_n = worker_of(t0 + newest / kShTile, s) - own_w + 1;
+      const int pre_w = s.prefix ? worker_of(s.own, s) : 0, n = own_n + (s.prefix ? worker_of(s.all - 1, s) - pre_w + 1 : 0);
+      const int64_t own_at = ((int64_t)gi * slots + b + own_w) * own_rows + r - b * p.per, pre_at = ((int64_t)gi * p.workers + pre_w) * 8 * NP + r;
+      join_results<V>(way, ways, n, lane, top, sum, a, [&](int i, const float2*& ml, const float*& acc) {
+        const bool mine = i < own_n;
+        const int64_t at = mine ? own_at + (int64_t)i * own_rows : pre_at + (int64_t)(i - own_n) * 8 * NP;
+        ml = (mine ? p.own_ml : p.pre_ml) + at;
+        acc = (mine ? p.own_acc : p.pre_acc) + at * HS;
+      });
+    }
+    if (ways > 1) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) s_acc[lane * V + j] = a[j];
+      if (lane == 0) *s_ml = make_float2(top, sum);
+      __syncthreads();
+      if (here && way == 0) {
+        join_warps<HS>(s_acc, s_ml, ways, lane, top, sum, a);
+      }
+    }
+    if (here && way == 0) store_result<HS>(p.out + ((int64_t)b * p.n_head + gi * p.per + r - b * p.per) * HS, a, newest < 0 ? 0.f : 1.f / sum, lane);
+  }
 }
 
 std::atomic<int> g_shared_path{0};   // b200_attn_decode_shared_tune
@@ -644,7 +890,21 @@ struct SharedPlan {
   bool tensor, pair;              // the prefix on the tensor memory; 256 query rows a CTA instead of 128
   int splits;                     // its key ranges
   int pre_rows, pre_tiles, pre_parts;
+  bool cluster;                   // a cluster a group, in one launch
 };
+
+// Whether a group's step goes to a cluster: it saves two launches, but a cluster's few CTAs turn all of the group's heads each, and have a group's tiles to themselves while
+// others' SMs idle.  us of list and cluster, in a graph (call after call a cluster is 5 us of the host shorter):
+//   rows x groups x heads of 128 each, prefix 96 to 200, 500, 1500, 2500 to 4000:  1 x 32 x 1  9.6 10.2 12.9 16.3, 8.1 8.4 11.9 15.1;  4 x 32 x 1  10.7 10.7 13.8 16.8, 8.3 9.3 13.6 16.4;
+//   2 x 8 x 4  8.7 10.0 10.6 12.5, 7.9 8.7 9.6 12.8;  4 x 8 x 2  8.6 10.2 10.6 12.7, 7.9 9.2 10.1 12.9;  8 x 32 x 1  10.8 11.3 14.6 17.7, 10.0 12.0 16.5 18.8;
+//   5 x 8 x 4 over 100 10.9, 14.3;  4 x 2 x 4 over 8000 15.4, 20.2;  of 64: 7 x 12 x 1 over 1001 11.0, 8.7;  8 x 24 x 2 over 300 11.6, 9.7
+// So: no more than 16 heads of 128 or 32 of 64 to turn, and at most 1.25 tiles a warp more than in the list (own caches half full).
+bool few_rows(int batch, int n_groups, int per, int hs, int prefix_rows, int own_rows) {
+  if (batch * (per + 2) * hs > 2048) return false;
+  const int sms = sm_count(), ctas = sms / n_groups < 1 ? 1 : sms / n_groups < kClCtas ? sms / n_groups : kClCtas;
+  const double tiles = (prefix_rows + 0.5 * batch * own_rows) / kShTile, warps = hs == 64 ? ClSmem<64, 1>::kWarps : ClSmem<128, 1>::kWarps;
+  return tiles * (1.0 / ctas - (double)n_groups / sms) <= 1.25 * warps;
+}
 
 SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows, int own_rows) {
   SharedPlan s;
@@ -653,6 +913,23 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
   // 48 rows of 8 groups x 2048 16.5, 19.5; 32 rows of 32 groups x 2048 26.3, 29.9; 24 rows of 8 groups x 8000 23.4, 23.5; 64 x 8000 34.1, 30.4; 32 x 16000 33.1, 29.2;
   // up to 16 rows a tile of the list has no more products than eights: 16 rows of 8 groups x 8000 20.0, 22.3.
   const int path = g_shared_path.load(std::memory_order_relaxed);
+  s.cluster = per <= 16 && (int64_t)batch * (per + 2) <= kClHeads && (path == 3 || (path == 0 && few_rows(batch, n_groups, per, hs, prefix_rows, own_rows)));
+  if (s.cluster) {
+    s.np = rows > 16 ? 4 : rows > 8 ? 2 : 1;
+    s.no = per > 8 ? 2 : 1;
+    s.tensor = s.pair = false;
+    s.splits = s.pre_rows = s.pre_tiles = s.pre_parts = s.head_tiles = s.row_tiles = s.ctas = 0;
+    s.ways = 1;
+    s.q = s.own_items = s.pre_items = 0;
+    const int64_t tiles = (int64_t)batch * ((own_rows + kShTile - 1) / kShTile) + (prefix_rows + kShTile - 1) / kShTile;
+    const int warps = hs == 64 ? ClSmem<64, 1>::kWarps : ClSmem<128, 1>::kWarps;
+    s.tiles = tiles * n_groups;
+    s.workers = kClCtas * warps < tiles ? kClCtas * warps : (int)tiles;
+    s.own_slots = (int64_t)n_groups * (batch + s.workers) * per;
+    s.pre_slots = prefix_rows > 0 ? (int64_t)n_groups * s.workers * 8 * s.np : 0;
+    s.bytes = (size_t)(s.own_slots + s.pre_slots) * (hs + 2) * sizeof(float);
+    return s;
+  }
   s.tensor = prefix_rows > 0 && (path ? path == 2 : rows > 16 && (int64_t)prefix_rows * n_groups * ((rows + 31) / 32) > 100000);
   s.pair = rows > 128;
   s.splits = s.pre_rows = s.pre_tiles = s.pre_parts = 0;
@@ -707,8 +984,51 @@ cudaError_t launch_tiles(const SharedParams& p, const SharedPlan& s, cudaStream_
   return launch(attn_shared_kernel<HS, NP, NO>, dim3((unsigned)s.ctas), dim3(C::kWarps * 32), (size_t)C::kBytes, st, p);
 }
 
+// As many CTAs a cluster as let all groups' clusters run at once, no more than there are tiles for their warps.
+template <int HS, int NP>
+cudaError_t launch_clusters(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
+  using C = ClSmem<HS, NP>;
+  static std::atomic<int> known[64][kClCtas + 1];   // clusters at once
+  static PerDeviceOnce once;
+  if (once.need()) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_shared_cluster_kernel<HS, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (e != cudaSuccess) return e;
+    once.done();
+  }
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  int ctas = (s.workers + C::kWarps - 1) / C::kWarps;
+  for (; ctas > 1; --ctas) {
+    if (ctas * p.n_groups > p.sms) continue;
+    std::atomic<int>& n = known[dev & 63][ctas];
+    int have = n.load(std::memory_order_relaxed);
+    if (have == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)ctas);
+      cfg.blockDim = dim3(C::kWarps * 32);
+      cfg.dynamicSmemBytes = C::kBytes;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)ctas;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&have, attn_shared_cluster_kernel<HS, NP>, &cfg) != cudaSuccess || have <= 0) {
+        (void)cudaGetLastError();
+        have = 1;
+      }
+      n.store(have, std::memory_order_relaxed);
+    }
+    if (have >= p.n_groups) break;
+  }
+  return launch_cluster(attn_shared_cluster_kernel<HS, NP>, dim3((unsigned)(p.n_groups * ctas)), dim3(C::kWarps * 32), ctas, (size_t)C::kBytes, st, p, ctas);
+}
+
 template <int HS>
 cudaError_t launch_shared(const SharedParams& p, const SharedPlan& s, cudaStream_t st) {
+  if (s.cluster) {
+    return s.np == 4 ? launch_clusters<HS, 4>(p, s, st) : s.np == 2 ? launch_clusters<HS, 2>(p, s, st) : launch_clusters<HS, 1>(p, s, st);
+  }
   const int64_t warps = (int64_t)p.batch * p.n_groups * (p.per + 2);
   cudaError_t e = launch(attn_shared_turn_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
@@ -734,7 +1054,7 @@ size_t b200_attn_decode_shared_workspace_bytes(int batch, int n_head, int n_grou
   return s.bytes;
 }
 
-int b200_attn_decode_shared_tune(int path) { return g_shared_path.exchange(path == 1 || path == 2 ? path : 0); }
+int b200_attn_decode_shared_tune(int path) { return g_shared_path.exchange(path >= 1 && path <= 3 ? path : 0); }
 
 int b200_attn_decode_shared(const b200_attn_decode_shared_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a, "b200_attn_decode_shared: null argument");

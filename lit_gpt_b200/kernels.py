@@ -925,7 +925,8 @@ def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
 
 def attn_decode_shared_tune(path: int = 0) -> int:
-    """Test knob: the prefix of ``attn_decode_shared`` always in the list of tiles (1), always on the tensor memory (2), by size (0); returns the previous setting."""
+    """Test knob: the prefix of ``attn_decode_shared`` always in the list of tiles (1), always on the tensor memory (2), a group's step by a cluster wherever its rows are few
+    enough (3), by size (0); returns the previous setting."""
     _shared_workspace_bytes.cache_clear()
     return int(C.load().b200_attn_decode_shared_tune(int(path)))
 

@@ -16,14 +16,14 @@ pytestmark = pytest.mark.gpu
 F64 = torch.float64
 
 
-@pytest.fixture(params=["list", "tensor memory"])
+@pytest.fixture(params=["list", "tensor memory", "cluster"])
 def K(request):
-    """The kernels with the prefix on either of its two ways, whatever the sizes say."""
+    """The kernels with the step on one of its ways, whatever the sizes say (a cluster a group: where the group's rows are few enough)."""
     if not torch.cuda.is_available():
         pytest.skip("needs a CUDA device")
     from lit_gpt_b200 import kernels
 
-    before = kernels.attn_decode_shared_tune(1 + (request.param != "list"))
+    before = kernels.attn_decode_shared_tune({"list": 1, "tensor memory": 2, "cluster": 3}[request.param])
     yield kernels
     kernels.attn_decode_shared_tune(before)
 
@@ -92,6 +92,15 @@ def check(got, want):
 @pytest.mark.parametrize("prefix,cap", [(1, 1), (31, 7), (128, 40), (300, 130)])
 def test_formula(K, hs, rows, groups, per, prefix, cap):
     own = [(5 * i + 2) % cap for i in range(rows)]
+    d = make(rows, groups, per, hs, prefix, cap, own, seed=rows + prefix)
+    check(call(K, d), formula(d))
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("rows,groups,per", [(10, 3, 1), (8, 2, 2), (6, 40, 3), (5, 5, 4), (4, 33, 6), (3, 148, 8), (2, 7, 14), (1, 300, 16), (1, 1, 16)])
+@pytest.mark.parametrize("prefix,cap", [(0, 70), (33, 33), (700, 200)])
+def test_few_rows(K, hs, rows, groups, per, prefix, cap):
+    own = [-1 if i % 4 == 1 else (41 * i + cap - 1) % cap for i in range(rows)]
     d = make(rows, groups, per, hs, prefix, cap, own, seed=rows + prefix)
     check(call(K, d), formula(d))
 
@@ -267,9 +276,10 @@ def test_same_as_the_ordinary_step(K):
     assert torch.equal(kc, full[0][:, :, 300:]) and torch.equal(vc, full[1][:, :, 300:])
 
 
-def test_captured_steps_follow_position_and_length(K):
+@pytest.mark.parametrize("rows", [20, 5])
+def test_captured_steps_follow_position_and_length(K, rows):
     """Two graphs that are replayed on two streams at once, each with lengths that change between replays."""
-    ds = [make(20, 2, 4, 128, 600, 40, [0] * 20, seed=s) for s in (1, 2)]
+    ds = [make(rows, 2, 4, 128, 600, 40, [0] * rows, seed=s) for s in (1, 2)]
     ts, graphs, outs, streams = [], [], [], [torch.cuda.Stream() for _ in ds]
     for d in ds:
         t = {k: v.cuda() if torch.is_tensor(v) else v for k, v in d.items()}
@@ -285,7 +295,7 @@ def test_captured_steps_follow_position_and_length(K):
     for n, p in ((600, 600), (77, 78), (599, 638)):
         torch.cuda.synchronize()
         for d, t in zip(ds, ts):
-            d["n"], d["pos"] = torch.tensor([n]), torch.full((20,), p)
+            d["n"], d["pos"] = torch.tensor([n]), torch.full((rows,), p)
             t["n"].fill_(n), t["pos"].fill_(p)
             t["kc"].copy_(d["kc"]), t["vc"].copy_(d["vc"])
         torch.cuda.synchronize()
@@ -312,9 +322,11 @@ def test_refusals(K):
         K.attn_decode_shared(t["qkv"], t["cos"], t["sin"], t["pos"], t["kc"], t["vc"], t["kp"], t["vp"], t["n"], 4, 2, 64, 64, table_preselected=True)
 
 
-@pytest.mark.parametrize("rows,groups,per,prefix", [(64, 8, 4, 1700), (64, 8, 4, 1500), (20, 8, 1, 13000), (16, 8, 1, 13000)])
+@pytest.mark.parametrize("rows,groups,per,prefix", [(64, 8, 4, 1700), (64, 8, 4, 1500), (20, 8, 1, 13000), (16, 8, 1, 13000), (5, 32, 1, 900), (6, 32, 1, 900), (2, 2, 4, 2000),
+                                                     (2, 2, 4, 3000)])
 def test_either_way_by_size(rows, groups, per, prefix):
-    """Sizes on both sides of the rule: 64 x 4 rows of 8 groups over 1700 and 1500 keys, 20 and 16 rows over 13000."""
+    """Sizes on both sides of the rule: 64 x 4 rows of 8 groups over 1700 and 1500 keys, 20 and 16 rows over 13000, 5 and 6 rows, 2 x 4 rows of 2 groups
+    over 2000 and 3000 keys."""
     from lit_gpt_b200 import kernels
 
     d = make(rows, groups, per, 128, prefix, 33, [i % 33 for i in range(rows)], seed=prefix)
