@@ -753,12 +753,12 @@ def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
             return copy_slots(tensors, src, dst, lengths)
     table: List[int] = []
     for t in tensors:
-        shape, numbers = t.shape, t.numel()
-        if len(shape) < 2 or shape[0] != slots or numbers == 0 or not t.is_contiguous():
+        shape, nbytes = t.shape, t.nbytes
+        if len(shape) < 2 or shape[0] != slots or nbytes == 0 or not t.is_contiguous():
             raise C.B200Error(f"copy_slots: tensors must be contiguous (slots, ...) with {slots} slots and something in them (got {tuple(shape)})")
         if device < 0 or t.get_device() != device:
             _one_device("copy_slots", max(device, 0), t)
-        table += (t.data_ptr(), shape[1], numbers * t.element_size() // (slots * shape[1]))
+        table += (t.data_ptr(), shape[1], nbytes // (slots * shape[1]))
     n = len(src)
     if lengths is None:
         lengths = (-1,) * n
