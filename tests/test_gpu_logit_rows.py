@@ -194,6 +194,34 @@ def test_draw_equal_logits(K):
     check_draw(K, d, 0.0, 4, None)
 
 
+@pytest.mark.parametrize("V", [300, 9000, 40000])
+@pytest.mark.parametrize("step", [None, 0.25, 2.0 ** -6])
+def test_the_last_one_kept(K, V, step):
+    """The k-th largest logit, equal ones in the order of their tokens, wins by its noise; the next one's noise is smaller still, but it is not kept.  step: logits are multiples of it."""
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn(14, V, generator=g) * 2
+    if step:
+        logits = (logits / step).round() * step
+    ks = [1, 2, 31, 100, 200, 255, 257, 299, 300, 500, 511, 512, 513, 1000]
+    order = torch.sort(logits, dim=-1, descending=True, stable=True).indices
+    e, want = torch.ones(14, V), []
+    for b, k in enumerate(ks):
+        k = min(k, V)
+        want.append(order[b, k - 1].item())
+        e[b, want[-1]] = 1e-20
+        if k < V:
+            e[b, order[b, k]] = 1e-30
+    for l in (logits, logits.bfloat16()) if step else (logits,):
+        if l.dtype == torch.bfloat16 and not torch.equal(l.float(), logits):
+            continue
+        tok = torch.zeros(14, dtype=torch.int64, device="cuda")
+        K.sample_rows_(l.cuda(), tok, 1.0, torch.tensor(ks, dtype=torch.int32, device="cuda"), noise=e.cuda())
+        assert tok.tolist() == want
+        for b, k in enumerate(ks):    # a row at a time, by CTAs of other sizes
+            K.sample_rows_(l[b : b + 1].cuda(), tok[:1], 1.0, k, noise=e[b : b + 1].cuda())
+            assert tok[0].item() == want[b]
+
+
 def test_draw_near_ties_go_by_64_bits(K):
     """Scores that 32 bits cannot tell apart."""
     V = 5000
