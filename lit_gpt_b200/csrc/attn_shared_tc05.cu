@@ -10,7 +10,7 @@
 //   * warp 16: S = Q K^T (operands in shared memory) and O += P V (P from tensor memory, V as it lies), 128 x 128 x 16 each
 //   * warps 17 and 18 bring keys and values, two stages each: whole tiles by TMA, the prefix's last one row by row, zeros behind it.
 // Bound: the prefix's bytes with up to 128 rows (a tile of 128 keys, 64 KB, is 2800 clocks of an SM's share of the memory's rate, its products 1536), with 256 rows the
-// products: 3072 clocks a tile, 1024 of them for the weights' second numbers.  A tile of 256 rows takes 4100: a stream's chain of scores, maximum, weights and output, which
+// products: 3 x 1024 clocks a tile, a third of them for the weights' second numbers.  A tile of 256 rows takes 4100: a stream's chain of scores, maximum, weights and output, which
 // the other stream fills in part.  64 rows of 8 groups of 4 heads over 16001 shared and up to 1000 own keys, 193 MB: 54 us the whole step, 3.6 TB/s.
 #include "attn_shared.cuh"
 #include "attn_tmem.cuh"
