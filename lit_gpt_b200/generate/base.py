@@ -419,8 +419,10 @@ def generate_samples(model: GPT, prompt: torch.Tensor, max_returned_tokens: int,
                 for _ in range(burst):
                     sg.step()
                 done += burst
-                if eos_id is not None and bool((sg.history[:, T : T + done] == eos_id).any(1).all()):   # the only host sync of the loop
-                    break
+                if eos_id is not None:   # the only host sync of the loop
+                    answers = sg.history[:, T : T + done]
+                    if bool(((answers == eos_id) | (answers < 0)).any(1).all()):   # (-1: a row that nothing could be drawn for)
+                        break
         answers = sg.history[:, T : T + done].clone()
         none = answers < 0
         last = torch.where(none.any(1), none.int().argmax(1), done)

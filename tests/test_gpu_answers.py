@@ -125,6 +125,31 @@ def test_an_answer_ends_where_nothing_can_be_drawn(golden, mode):
     assert all(len(y) == T + 12 for y in gb.generate_samples(model, p, T + 12, 3, temperature=0.9))
 
 
+@pytest.mark.parametrize("mode", ["nf4", None])
+@torch.inference_mode()
+def test_answers_that_can_draw_nothing_end_the_steps(golden, mode, monkeypatch):
+    """Rows that ended without a token count as ended where an eos_id is looked for: the steps stop at the next look."""
+    import lit_gpt_b200.generate.base as gb
+
+    model, *_, prompt = toy(golden, mode)
+    p, T, V = prompt.cuda(), len(prompt), model.config.padded_vocab_size
+    steps, step = [], gb.SampleGraph.step
+    monkeypatch.setattr(gb.SampleGraph, "step", lambda self: (steps.append(1), step(self))[1])
+    nothing = {t: float("-inf") for t in range(V)}
+    ys = gb.generate_samples(model, p, T + 100, 3, temperature=0.9, logit_bias=nothing, eos_id=5)
+    assert all(torch.equal(y, p) for y in ys) and len(steps) == gb.EOS_POLL
+    # two tokens may follow, each once: an answer holds both, or ends with the one that ends it
+    steps.clear()
+    two = {t: float("-inf") for t in range(V) if t not in (7, 9)}
+    for y in gb.generate_samples(model, p, T + 100, 6, temperature=1.5, logit_bias=two, presence_penalty=float("inf"), eos_id=8):
+        assert sorted(y[T:].tolist()) == [7, 9]
+    assert len(steps) == gb.EOS_POLL
+    steps.clear()
+    for y in gb.generate_samples(model, p, T + 100, 6, temperature=1.5, logit_bias=two, presence_penalty=float("inf"), eos_id=9):
+        assert y[T:].tolist() in ([9], [7, 9])
+    assert len(steps) == gb.EOS_POLL
+
+
 @torch.inference_mode()
 def test_one_captured_step_serves_prompts_of_all_lengths(golden):
     import lit_gpt_b200.generate.base as gb
