@@ -117,9 +117,10 @@ class DecodeGraph:
         if keep is not None:
             for t, saved in zip(self.model.state_tensors(), keep):
                 t.copy_(saved)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self._step()
+        self.graph = graph   # (an exception ends the capture with the launches there were)
         self.token.copy_(state[0]); self.pos.copy_(state[1])
         self.rng.copy_(rng0)
 
@@ -156,9 +157,10 @@ class PrefillGraph:
             for _ in range(2):
                 self._run()
         torch.cuda.current_stream().wait_stream(side)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self._run()
+        self.graph = graph
         self.rng.copy_(rng0)
 
 
@@ -327,9 +329,10 @@ class SampleGraph:
                 self._step(self.token)
         torch.cuda.current_stream().wait_stream(side)
         put_back()
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self._step(self.token)
+        self.graph = graph
 
     def step(self) -> None:
         if self.graph is not None:

@@ -150,6 +150,31 @@ def test_answers_that_can_draw_nothing_end_the_steps(golden, mode, monkeypatch):
     assert len(steps) == gb.EOS_POLL
 
 
+@pytest.mark.parametrize("draw", ["sample_rows_", "argmax_", "sample_"])
+@torch.inference_mode()
+def test_a_capture_that_fails_leaves_no_graph(golden, monkeypatch, draw):
+    """An exception behind most of a captured step's launches (of several answers, of one, of a prompt): the next call captures anew and does not replay what there is of it."""
+    import lit_gpt_b200.generate.base as gb
+
+    model, *_, prompt = toy(golden)
+    first, then = prompt.cuda()[:8], prompt.flip(0).cuda()[:8]
+    call = (lambda p: gb.generate_samples(model, p, 28, 3, temperature=0.0)) if draw == "sample_rows_" else lambda p: [gb.generate(model, p, 28, temperature=0.0)]
+    want = call(then)
+    model.set_kv_cache(batch_size=1, device="cuda", dtype=torch.bfloat16)    # (lets the captured steps go)
+    whole = getattr(gb.K, draw)
+
+    def fails(*args, **kw):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("no more")
+        return whole(*args, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(gb.K, draw, fails)
+        with pytest.raises(RuntimeError, match="no more"):
+            call(first)
+    assert all(torch.equal(a, b) for a, b in zip(call(then), want))
+
+
 @torch.inference_mode()
 def test_one_captured_step_serves_prompts_of_all_lengths(golden):
     import lit_gpt_b200.generate.base as gb
