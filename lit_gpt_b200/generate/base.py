@@ -361,7 +361,15 @@ def _sample_graph_for(model: GPT, *key: Any) -> SampleGraph:
     if sg is None:
         if cache and next(iter(cache))[len(key):] != full[len(key):] or len(cache) >= 2:
             cache.clear()   # (a call's last group of rows may be smaller than the others: two)
-        sg = cache[full] = SampleGraph(model, *key)
+        try:
+            sg = SampleGraph(model, *key)
+        except torch.OutOfMemoryError:
+            if not cache:
+                raise
+        if sg is None:
+            cache.clear()   # what is kept from earlier calls gives its place (behind the exception, which held what there was of the new one)
+            sg = SampleGraph(model, *key)
+        cache[full] = sg
     return sg
 
 
@@ -400,6 +408,7 @@ def generate_samples(model: GPT, prompt: torch.Tensor, max_returned_tokens: int,
     scores: List[torch.Tensor] = []
     for begin in range(0, num_samples, each):
         rows = min(each, num_samples - begin)
+        sg = None   # (the group before: kept by the model alone, which may let it go)
         sg = _sample_graph_for(model, rows, length, temperature, top_k, penalties, bool(logit_bias), logprobs, prompt.dtype)
         sg.prefix_len.fill_(T)
         sg.pos.fill_(T - 1)

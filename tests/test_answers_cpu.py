@@ -90,6 +90,44 @@ def test_samples_need_the_gpu_cache():
         gb.generate_samples(model, torch.tensor([1, 2]), 8, 2)
 
 
+def test_kept_steps_make_place_for_a_new_one(monkeypatch):
+    """Where a step's caches find no place, the steps kept from earlier calls go first; where they find none even so, the call is refused."""
+    import weakref
+
+    import lit_gpt_b200.generate.base as gb
+
+    class Step:
+        full, asked = 0, []    # how many more find no place; how many steps were alive beside each
+
+        def __init__(self, model, *key):
+            Step.asked.append(sum(kept() is not None for kept in seen))
+            if Step.full:
+                Step.full -= 1
+                raise torch.OutOfMemoryError("full")
+            seen.append(weakref.ref(self))
+
+    class Model:
+        device = torch.device("cpu")
+
+        def graph_key(self):
+            return ("buffers",)
+
+    monkeypatch.setattr(gb, "SampleGraph", Step)
+    model, seen = Model(), []
+    step = lambda rows: gb._sample_graph_for(model, rows, 64)
+    assert step(16) is step(16) and Step.asked == [0]
+    Step.full = 1
+    assert step(3) is step(3) and Step.asked == [0, 1, 0] and len(model._sample_graphs) == 1
+    Step.full = 2
+    with pytest.raises(torch.OutOfMemoryError):
+        step(5)
+    assert Step.asked == [0, 1, 0, 1, 0] and not model._sample_graphs
+    Step.full = 1
+    with pytest.raises(torch.OutOfMemoryError):    # nothing was kept: not tried again
+        step(5)
+    assert Step.asked == [0, 1, 0, 1, 0, 0] and step(5) is step(5)
+
+
 class Slots(nn.Module):
     """A model whose state of a slot is the tokens that it was fed."""
 
