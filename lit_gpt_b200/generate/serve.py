@@ -193,6 +193,9 @@ def _generate_ruled(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens
         words = None
         if allowed is not None:
             masks = [allowed(i, out[i]) for i in live]
+            for i, m in zip(live, masks):
+                if m is not None and m.shape != (V,):
+                    raise ValueError(f"allowed gives truth values for {V} tokens (got {tuple(m.shape)} for request {i})")
             if any(m is not None for m in masks):
                 words = K.pack_allowed(torch.stack([torch.ones(V, dtype=torch.bool) if m is None else m.to("cpu", torch.bool) for m in masks])).to(dev)
         token = torch.empty(len(live), dtype=torch.int64, device=dev)

@@ -198,3 +198,26 @@ def test_fork_compact_and_shrink(monkeypatch, positional):
     session.shrink()
     check()
     assert model.slots.capacity == 1
+
+
+@pytest.mark.parametrize("shape", [(39,), (41,), (1, 40), ()])
+def test_a_grammar_speaks_about_every_token(monkeypatch, shape):
+    """Truth values for more or fewer tokens than there are: refused, also where they pack into as many words."""
+    from types import SimpleNamespace
+
+    from lit_gpt_b200.generate import serve
+
+    class Model(Slots):
+        device, max_seq_length, config = torch.device("cpu"), 40, SimpleNamespace(vocab_size=40)
+
+    drawn = []
+    monkeypatch.setattr(K, "copy_slots", lambda *args: None)
+    monkeypatch.setattr(K, "sample_rows_", lambda logits, token, *args, **kw: (drawn.append(kw["allowed"]), token.fill_(3)))
+    model = Model(True)
+    session = Session(model, slots=2)
+    ask = lambda mask: serve.generate_batch(model, [[1, 2], [4]], 3, session=session, allowed=lambda i, tokens: mask)
+    assert ask(torch.ones(40, dtype=torch.bool)) == [[1, 2, 3, 3, 3], [4, 3, 3, 3]] and all(w.shape == (2, 2) for w in drawn)
+    drawn.clear()
+    with pytest.raises(ValueError, match="40 tokens"):
+        ask(torch.ones(shape, dtype=torch.bool))
+    assert not drawn and not session.live
