@@ -390,15 +390,17 @@ def generate_samples(model: GPT, prompt: torch.Tensor, max_returned_tokens: int,
         raise NotImplementedError(f"max_seq_length {model.max_seq_length} needs to be >= {max_returned_tokens - 1}")
     if num_samples < 1:
         raise ValueError(f"num_samples must be at least 1 (got {num_samples})")
+    V, penalties = model.config.padded_vocab_size, (float(repetition_penalty), float(frequency_penalty), float(presence_penalty))
+    if count_prompt and penalties != (1.0, 0.0, 0.0) and bool(((prompt < 0) | (prompt >= V)).any()):
+        raise ValueError(f"the prompt has tokens outside 0 .. {V - 1}, which cannot be counted")
     caches = [b.attn.kv_cache for b in model.transformer.h]
     if any(c is None for c in caches):
         raise TypeError("You need to call `gpt.set_kv_cache()`")
     if not prompt.is_cuda or model.tp_world_size != 1 or model.spans_devices() or not all(c.gqa_native for c in caches):
         raise NotImplementedError("answers that share their prompt run on one GPU over the GQA-native cache (bf16, head size 64 or 128)")
-    V = model.config.padded_vocab_size
     if logit_bias and not all(0 <= t < V for t in logit_bias):
         raise ValueError(f"logit_bias names tokens outside 0 .. {V - 1}")
-    device, penalties = prompt.device, (float(repetition_penalty), float(frequency_penalty), float(presence_penalty))
+    device = prompt.device
     rng = row_rng_states(device, num_samples) if temperature > 0.0 else None
     first = model(prompt.view(1, -1), torch.arange(0, T, device=device))[:, -1]
     fused = model.fused_decode_ready(prompt.view(1, -1))

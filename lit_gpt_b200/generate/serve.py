@@ -177,9 +177,12 @@ def _generate_ruled(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens
         raise ValueError("a prompt has one token at least")
     if logit_bias and not all(0 <= t < V for t in logit_bias):
         raise ValueError(f"logit_bias names tokens outside 0 .. {V - 1}")
+    counted = penalties != (1.0, 0.0, 0.0)
+    if counted and count_prompt and not all(0 <= t < V for p in prompts for t in p):
+        raise ValueError(f"a prompt has tokens outside 0 .. {V - 1}, which cannot be counted")
     rng = row_rng_states(dev, N) if temperature > 0.0 else None
     counts = bias = None
-    if penalties != (1.0, 0.0, 0.0):
+    if counted:
         counts = torch.zeros(N, V, dtype=torch.int32, device=dev)
         if count_prompt:
             for i, p in enumerate(out):

@@ -90,6 +90,33 @@ def test_samples_need_the_gpu_cache():
         gb.generate_samples(model, torch.tensor([1, 2]), 8, 2)
 
 
+@pytest.mark.parametrize("token", [-1, 50, 2 ** 40])
+def test_prompts_that_are_counted_have_tokens_of_the_vocabulary(token):
+    """A token outside has no place among the counts: refused on the host, before anything runs."""
+    from types import SimpleNamespace
+
+    import lit_gpt_b200.generate.base as gb
+    from lit_gpt_b200 import GPT, Config
+    from lit_gpt_b200.generate import serve
+
+    model = GPT(Config(name="t", block_size=32, vocab_size=50, padded_vocab_size=50, n_layer=1, n_head=2, n_embd=16))
+    model.set_kv_cache(batch_size=1)
+    with pytest.raises(ValueError, match="outside 0 .. 49"):
+        gb.generate_samples(model, torch.tensor([1, token]), 8, 2, presence_penalty=0.5, count_prompt=True)
+    for kw in (dict(count_prompt=True), dict(presence_penalty=0.5)):    # nothing is counted in the prompt: as far as the refusal of this cache
+        with pytest.raises(NotImplementedError, match="GQA-native"):
+            gb.generate_samples(model, torch.tensor([1, token]), 8, 2, **kw)
+
+    class Model(Slots):
+        device, max_seq_length, config = torch.device("cpu"), 40, SimpleNamespace(vocab_size=50)
+
+    model = Model(True)
+    session = Session(model, slots=2)
+    with pytest.raises(ValueError, match="outside 0 .. 49"):
+        serve.generate_batch(model, [[1, 2], [4, token]], 3, session=session, presence_penalty=0.5, count_prompt=True)
+    assert not session.live and (model.fed == -1).all()
+
+
 def test_kept_steps_make_place_for_a_new_one(monkeypatch):
     """Where a step's caches find no place, the steps kept from earlier calls go first; where they find none even so, the call is refused."""
     import weakref
