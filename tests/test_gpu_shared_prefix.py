@@ -331,3 +331,30 @@ def test_either_way_by_size(rows, groups, per, prefix):
 
     d = make(rows, groups, per, 128, prefix, 33, [i % 33 for i in range(rows)], seed=prefix)
     check(call(kernels, d), formula(d))
+
+
+@pytest.mark.parametrize("rows,groups,per,prefix,launches", [(64, 8, 4, 1700, 4), (64, 8, 4, 1500, 3), (20, 8, 1, 13000, 4), (16, 8, 1, 13000, 3), (5, 32, 1, 900, 1), (6, 32, 1, 900, 3),
+                                                              (2, 2, 4, 2000, 1), (2, 2, 4, 3000, 3)])
+def test_which_way_by_size(rows, groups, per, prefix, launches):
+    """The sizes of test_either_way_by_size take the way that the rule says: a cluster a group is one launch, the list three, tensor memory beside the list four."""
+    from lit_gpt_b200 import kernels
+
+    d = make(rows, groups, per, 128, prefix, 33, [i % 33 for i in range(rows)], seed=prefix)
+    t = {k: v.cuda() if torch.is_tensor(v) else v for k, v in d.items()}
+    before = kernels.launch_count()
+    kernels.attn_decode_shared(t["qkv"], t["cos"], t["sin"], t["pos"], t["kc"], t["vc"], t["kp"], t["vp"], t["n"], groups * per, groups, 128, 128)
+    assert kernels.launch_count() - before == launches
+
+
+@pytest.mark.parametrize("hs,rope", [(64, 64), (64, 16), (128, 128), (128, 6)])
+@pytest.mark.parametrize("table", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_tables_by_position_in_the_call(K, hs, rope, table, rows):
+    """Rows of the tables already picked, in the order of pos: one per row, rows that take no part among them, or one for all."""
+    d = make(rows, 2, 2, hs, 70, 30, [-1 if i % 5 == 3 else (7 * i + 4) % 30 for i in range(rows)], rope=rope, table=table, seed=rows + rope)
+    for pos in (d["pos"], torch.tensor([83])):
+        d["pos"] = pos
+        at = pos.clamp(min=0)
+        t = {k: v.cuda() if torch.is_tensor(v) else v for k, v in d.items()}
+        out = K.attn_decode_shared(t["qkv"], d["cos"][at].cuda(), d["sin"][at].cuda(), t["pos"], t["kc"], t["vc"], t["kp"], t["vp"], t["n"], 4, 2, hs, rope, table_preselected=True)
+        check((out, t["kc"], t["vc"]), formula(d))
