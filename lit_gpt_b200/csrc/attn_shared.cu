@@ -899,6 +899,9 @@ struct SharedPlan {
 //   2 x 8 x 4  8.7 10.0 10.6 12.5, 7.9 8.7 9.6 12.8;  4 x 8 x 2  8.6 10.2 10.6 12.7, 7.9 9.2 10.1 12.9;  8 x 32 x 1  10.8 11.3 14.6 17.7, 10.0 12.0 16.5 18.8;
 //   5 x 8 x 4 over 100 10.9, 14.3;  4 x 2 x 4 over 8000 15.4, 20.2;  of 64: 7 x 12 x 1 over 1001 11.0, 8.7;  8 x 24 x 2 over 300 11.6, 9.7
 // So: no more than 16 heads of 128 or 32 of 64 to turn, and at most 1.25 tiles a warp more than in the list (own caches half full).
+// The plan goes by prefix_rows, what the buffer has room for, since the length is on the device; these times and those at shared_plan are of prefixes that fill it.  In a buffer
+// of 8192, rows x groups x heads over 500 and 2000 keys:  2 x 32 x 1  10.0 14.8 (filled 7.9 13.5);  16 x 32 x 1  15.0 19.9 (15.2 20.0);  16 x 8 x 4  19.0 22.7 (16.2 18.6);
+// 64 x 8 x 4  26.8 28.0 (22.3 26.8).
 bool few_rows(int batch, int n_groups, int per, int hs, int prefix_rows, int own_rows) {
   if (batch * (per + 2) * hs > 2048) return false;
   const int sms = sm_count(), ctas = sms / n_groups < 1 ? 1 : sms / n_groups < kClCtas ? sms / n_groups : kClCtas;
@@ -939,7 +942,8 @@ SharedPlan shared_plan(int batch, int n_groups, int per, int hs, int prefix_rows
     const int64_t items = (int64_t)n_groups * s.pre_tiles, ranges = ((int64_t)prefix_rows + 127) / 128;
     // SMs for the prefix's kernel: the kernel of the own keys begins beside it on the others, so each has the share of SMs that its work asks for (own caches half full): a tile
     // of 128 keys takes 2.15 us with 256 rows and 1.3 with 128, own keys come at 58 GB/s an SM.  64 rows x 16001 in 8 groups of 4 heads, up to 1000 own tokens, in 6, 9, 12, 18
-    // ranges 69, 54, 55, 64 us; 10 own tokens 63, 50, 43, 46; 4000 shared and up to 1000 own ones 42, 43, 47, 51 (3 ranges 46).
+    // ranges 69, 54, 55, 64 us; 10 own tokens 63, 50, 43, 46; 4000 shared and up to 1000 own ones 42, 43, 47, 51 (3 ranges 46).  (All of heads of 128; a tile of heads of 64,
+    // half as large, is counted as much.)
     const double prefix_work = (double)items * ranges * (s.pair ? 2.15 : 1.3), own_work = (double)batch * n_groups * own_rows * hs * 2 / 58e3;
     const double share = sm_count() * prefix_work / (prefix_work + own_work) / items;
     s.splits = share < 1.0 ? 1 : share < (double)ranges ? (int)(share + 0.5) : (int)ranges;

@@ -11,10 +11,13 @@
 //
 // Bound: adjusting by bytes, 64 x 50304 fp32 with counts, a bias and a mask per row 52 MB in 9.6 us (5.4 TB/s).  The draw reads what the rules need once.  Of a few rows it is
 // a chain of waits: 32000 bf16 logits 8 us, 14.5 with a top-k of 200: a histogram of the first ten bits of the keys over the cluster, then one CTA goes on with the 1024 tokens
-// at most that are left (29 with every digit by a pass over the cluster; up to 512 of them ranked one by one instead of digit by digit: 11.6 against 11.0 for fp32, 16.0 against 12.7
-// for bf16 with its equal logits, k = 50).  Of many rows it is what a token takes, its rules, weight and score, 96 instructions that wait
+// at most that are left (up to 512 of them ranked one by one instead of digit by digit: 11.6 against 11.0 for fp32, 16.0 against 12.7 for bf16 with its equal logits, k = 50).
+// Two bins a power of two leave more than 1024 where the vocabulary is large; every digit is then a pass over the cluster.  us, 1 row, k = 200, normal logits of standard
+// deviation 2, 3, 4: of 32000 bf16 tokens 13.8 14.0 14.7, of 50257 16.6 14.7 16.6 (at 3 some rows leave few), of 128256 21.3 19.3 23.9; 16 rows 19.0 18.9 19.1, 21.9 21.1 21.4, 31.5 25.3 31.4.
+// Of many rows it is what a token takes, its rules, weight and score, 96 instructions that wait
 // for one another: 96 x 50257 fp32 with counts, a bias, masks and noise, 58 MB, 32 us (1.8 TB/s) with 46 % of the issue slots taken by 24 warps an SM.  Without the weights, where
-// no log-probability is asked for, draws were 0 to 4 % shorter, and with one 1 to 3 % longer.
+// no log-probability is asked for, draws were 0 to 4 % shorter, and with one 1 to 3 % longer.  From Philox states and without rules, noise given in brackets: 96 x 50257 bf16 28.0
+// (27.2), 64 x 50304 bf16 18.9 (19.4), 16 x 32000 bf16 10.2 (9.3), with a top-k of 200 18.9 (16.7).
 #include "philox.cuh"
 
 namespace b200 {
@@ -801,7 +804,7 @@ cudaError_t launch_draw_as(const Rules& r, const DrawArgs& a, int ctas, cudaStre
 
 template <typename LT>
 cudaError_t launch_draw(const Rules& r, DrawArgs a, cudaStream_t st) {
-  // The cluster's CTAs, each with 1024 tokens at least, and their threads: the shortest of draw_time.  us, k = 50, of clusters of 1, 2, 3, 4, 6, 8 CTAs of 512 threads, of 256:
+  // The cluster's CTAs, each with 1024 tokens at least, and their threads: the shortest of draw_time.  us, bf16 from Philox states, k = 50, of clusters of 1, 2, 3, 4, 6, 8 CTAs of 512 threads, of 256:
   //   1 x 32000   25.5 17.7 15.6 14.3 13.1 12.7, 37.4 23.2 18.7 17.0 15.4 14.1;     38 x 50304   25.6 25.5 24.2 21.9 19.6 27.9, 35.8 35.8 28.5 26.1 23.4 22.1
   //   96 x 50257  47.2 47.4 38.0 38.6 42.6 47.8, 65.9 65.8 49.7 30.3 39.9 42.0;     200 x 32000  51.7 38.5 46.7 47.4 59.1 72.8, 77.1 51.6 42.9 41.9 52.7 62.5
   const int sizes = r.vocab / 1024, most = sizes < 1 ? 1 : sizes < kSaCtas ? sizes : kSaCtas, least = (r.vocab + kSaMaxSlice - 1) / kSaMaxSlice;

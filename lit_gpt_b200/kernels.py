@@ -740,7 +740,8 @@ def sample_rows_(logits: torch.Tensor, token_out: torch.Tensor, temperature: Per
 
 
 def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], lengths: Optional[Sequence[int]] = None) -> None:
-    """t[dst[i]] = t[src[i]] for every i and every tensor t (slots, ...) of caches and states, in one launch for all of them: a live sequence forked, or moved to another slot.
+    """t[dst[i]] = t[src[i]] for every i and every tensor t (slots, ...) of caches and states: a live sequence forked, or moved to another slot.  A launch takes up to 128 tensors,
+    and up to 256 copies from 64 sources (neighbouring copies of one source and length count as one).
     ``lengths``: copy i takes only the leading lengths[i] positions (the second dimension) of caches by position.  A slot may be the source of several copies;
     one that is written may be neither the source nor the destination of another."""
     if len(src) != len(dst) or (lengths is not None and len(lengths) != len(src)):
