@@ -349,3 +349,72 @@ def test_batches_of_samples_and_rules(kind):
     with pytest.raises(ValueError, match="one token at least"):
         generate_batch(model, [[], prompts[0]], 5, num_samples=2, session=session)
     assert not session.live
+
+
+# ---- the command line ---------------------------------------------------------------------------------------------------------------
+def command(directory, *args):
+    import pathlib
+    import subprocess
+    import sys
+
+    root = pathlib.Path(__file__).resolve().parent.parent
+    res = subprocess.run([sys.executable, "-m", "lit_gpt_b200.generate.base", *args, "--checkpoint_dir", str(directory)], cwd=root, capture_output=True, text=True, timeout=600)
+    assert res.returncode == 0, res.stderr[-2000:]
+    return res.stdout.strip().splitlines(), res.stderr
+
+
+@pytest.mark.parametrize("quantize", [["--quantize", "bnb.nf4"], []])
+def test_command_line(tmp_path, golden, quantize):
+    """Answers as a batch from a checkpoint directory with a tokenizer, whose prompts are 32-bit tokens."""
+    import json
+
+    from tokenizers import Tokenizer, models, pre_tokenizers
+    from test_gpu_model import cfg_from_golden
+
+    from lit_gpt_b200 import Config
+
+    cfgd, kw = cfg_from_golden(golden("llama_gqa_hs64"))
+    kw["block_size"] = max(kw["block_size"], 128)
+    V = Config(**kw).padded_vocab_size
+    torch.save({k: v.to(torch.bfloat16) for k, v in M.init_weights(M.RefConfig.from_any(cfgd), seed=1234).items()}, tmp_path / "lit_model.pth")
+    (tmp_path / "lit_config.json").write_text(json.dumps(kw))
+    words = Tokenizer(models.WordLevel({f"t{i}": i for i in range(V)}, unk_token="t0"))
+    words.pre_tokenizer = pre_tokenizers.WhitespaceSplit()
+    words.save(str(tmp_path / "tokenizer.json"))
+    (tmp_path / "tokenizer_config.json").write_text("{}")
+    prompt = [f"t{i}" for i in (5, 17, 3, 88, 41, 7)]
+    ask = lambda *args: command(tmp_path, " ".join(prompt), "--max_new_tokens", "30", *quantize, *args)
+    plain, _ = ask("--temperature", "0")
+    lines, said = ask("--temperature", "0", "--num_samples", "5", "--batch_samples", "true")
+    assert len(lines) == 5 and len(set(lines)) == 1 and "Time for inference of 5" in said
+    assert lines[0].split()[:7] == plain[0].split()[:7] and len(lines[0].split()) == len(plain[0].split()) == 36
+    lines, _ = ask("--num_samples", "3", "--presence_penalty", "10000")
+    assert len(set(lines)) == 3
+    for line in lines:
+        assert line.split()[:6] == prompt and len(line.split()) == 36 and len(set(line.split()[6:])) == 30
+
+
+def test_command_line_of_a_slot_served_model(tmp_path):
+    import test_gpu_fizadra as F
+
+    w = F.checkpoint(F.CFG_ODD, 111)
+    F._write_checkpoint(tmp_path, F.CFG_ODD, w)
+    prompt = F.tokens_for(F.CFG_ODD, 6, 112)
+    want = F.O.greedy(F.CFG_ODD, w, prompt, 9)
+    lines, _ = command(tmp_path, " ".join(map(str, prompt)), "--precision", "32-true", "--temperature", "0", "--max_new_tokens", "9", "--num_samples", "3", "--batch_samples", "true")
+    assert [list(map(int, line.split())) for line in lines] == [want] * 3
+    lines, _ = command(tmp_path, " ".join(map(str, prompt)), "--precision", "32-true", "--max_new_tokens", "20", "--frequency_penalty", "10000")
+    assert len(lines) == 1 and len(set(lines[0].split()[6:])) == 20 and len(lines[0].split()) == 26
+
+
+@pytest.mark.parametrize("mode", ["nf4", None])
+@torch.inference_mode()
+def test_prompts_of_32_bit_tokens(golden, mode):
+    import lit_gpt_b200.generate.base as gb
+
+    model, *_, prompt = toy(golden, mode)
+    T = len(prompt)
+    kw = dict(temperature=0.0, presence_penalty=2.0, count_prompt=True, logprobs=True, eos_id=3)
+    want, scores = gb.generate_samples(model, prompt.long().cuda(), T + 20, 3, **kw)
+    got, scores32 = gb.generate_samples(model, prompt.int().cuda(), T + 20, 3, **kw)
+    assert all(a.dtype == torch.int32 and torch.equal(a.long(), b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(scores32, scores))
