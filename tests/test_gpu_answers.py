@@ -418,3 +418,28 @@ def test_prompts_of_32_bit_tokens(golden, mode):
     want, scores = gb.generate_samples(model, prompt.long().cuda(), T + 20, 3, **kw)
     got, scores32 = gb.generate_samples(model, prompt.int().cuda(), T + 20, 3, **kw)
     assert all(a.dtype == torch.int32 and torch.equal(a.long(), b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(scores32, scores))
+
+
+@torch.inference_mode()
+def test_the_last_group_of_rows_takes_the_place_of_the_others(golden, monkeypatch):
+    """A last, smaller group of rows whose caches find no place beside the step of the groups before: that one is let go."""
+    import weakref
+
+    import lit_gpt_b200.generate.base as gb
+
+    model, *_, prompt = toy(golden)
+    p, T = prompt.cuda(), len(prompt)
+    want = gb.generate_samples(model, p, T + 20, 19, temperature=0.0)
+    model.__dict__.pop("_sample_graphs")
+    there = []
+
+    class Step(gb.SampleGraph):
+        def __init__(self, model, *key):
+            if any(step() is not None for step in there):
+                raise torch.OutOfMemoryError("full")
+            super().__init__(model, *key)
+            there.append(weakref.ref(self))
+
+    monkeypatch.setattr(gb, "SampleGraph", Step)
+    got = gb.generate_samples(model, p, T + 20, 19, temperature=0.0)
+    assert len(got) == 19 and all(torch.equal(a, b) for a, b in zip(got, want)) and [step() is None for step in there] == [True, False]
