@@ -311,6 +311,53 @@ int b200_attn_decode_shared(const b200_attn_decode_shared_args* args, b200_strea
  * the setting at the time. */
 int b200_attn_decode_shared_tune(int path);
 
+/* One ragged step over a paged key-value cache: every sequence brings one token or a chunk of them; their rotated keys and values join its pages, and each row attends to its
+ * sequence's keys up to its own.
+ *   qkv        (rows, (n_head + 2 n_groups) * head_size) bf16, interleaved per group as in b200_attn_decode
+ *   row_pos    position of every row, its row of the tables (clamped); apart from the keys' places, since a cache may hold fewer keys than a sequence has positions
+ *   row_seq    int32, the sequence of every row; a row of none (-1, or outside its sequence's rows) takes no part, its result is zero
+ *   seqs       int32 (n_seqs, 4) on a 16-byte boundary: first row, rows, keys in the cache before the step, row of the page table.  Sequences of no rows take no part.
+ *   pages      int32 (table_seqs, max_pages), rows pages_ld apart: entry i of a sequence's row is the page of its keys [i * page, (i + 1) * page).  Where the entry is no page (outside
+ *              0 .. pool - 1) there are no keys: new ones are dropped, the rest take no part.  A row that sees no key has a result of zero.
+ *   k_pages, v_pages   (pool, n_groups, page, head_size) bf16, rows head_size apart, pages and groups at the given distances (elements, multiples of 8); page 16, 32, 64, 128 or 256.
+ *              What lies in a page behind a sequence's last key is not read.
+ *   key_weights        (pool, n_groups, page) fp32 or NULL: what attention weight every key has received.  New keys begin at zero; every key gains the sum of its softmax
+ *              weights over the step's rows and its group's heads.
+ *   max_rows, max_length   bounds of a sequence's rows and of its keys behind the step: they size the work; keys from max_length on are dropped
+ *   cos, sin   (table_rows, rope_n_elem), row = position; table_preselected: row = row of qkv
+ * head_size 64 or 128.  No page belongs to two sequences that bring rows into it.  The workspace needs no initial contents; two calls that run at the same time need one each. */
+typedef struct b200_attn_paged_args {
+  const void* qkv;
+  const void* cos; const void* sin; int table_dtype, table_rows, table_preselected, rope_n_elem;
+  const void* row_pos; int pos_is_int64;
+  const int32_t* row_seq; const int32_t* seqs; int n_seqs;
+  const int32_t* pages; int64_t pages_ld; int table_seqs, max_pages, pool, page;
+  void* k_pages; void* v_pages; int64_t k_page_stride, k_group_stride, v_page_stride, v_group_stride;
+  float* key_weights;
+  void* out;                  /* (rows, n_head * head_size) bf16 */
+  int64_t rows, max_rows, max_length; int n_head, n_groups, head_size;
+  void* workspace; size_t workspace_bytes;
+} b200_attn_paged_args;
+size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int n_groups, int head_size, int64_t max_rows, int64_t max_length, int key_weights);
+int b200_attn_paged(const b200_attn_paged_args* args, b200_stream_t stream);
+
+/* Sequences of a paged cache cut down to `keep` keys each, every group by itself: the first `first` keys, the last `recent` and, of those between, the ones with the largest
+ * key_weights (equal ones: the lower index; NaN counts as the largest) stay; they move to the front of the sequence's pages in order -- keys, values and weights; what lies behind
+ * them stays as it was.
+ *   lengths    int32 (n_seqs): keys of each sequence; lengths_out: keys it has behind the call, in a place of its own
+ *   rows       int32 (n_seqs): its row of the page table; NULL: row i
+ * A sequence of at most `keep` keys, of more than max_length, or with an entry that is no page among its own stays as it is.  No page belongs to two sequences of the call. */
+typedef struct b200_evict_paged_args {
+  void* k_pages; void* v_pages; int64_t k_page_stride, k_group_stride, v_page_stride, v_group_stride;
+  float* key_weights;
+  const int32_t* pages; int64_t pages_ld; int table_seqs, max_pages, pool, page;
+  const int32_t* lengths; const int32_t* rows; int32_t* lengths_out; int n_seqs;
+  int n_groups, head_size; int64_t keep, first, recent, max_length;
+  void* workspace; size_t workspace_bytes;
+} b200_evict_paged_args;
+size_t b200_evict_paged_workspace_bytes(int n_seqs, int n_groups, int64_t keep);
+int b200_evict_paged(const b200_evict_paged_args* args, b200_stream_t stream);
+
 /* ---- prefill helper: RoPE + KV-cache write for T > 1 tokens at positions pos[0..T) (lit_gpt/model.py:624-649).
  * table_preselected = 1: cos/sin are (T, rope_n_elem) rows already gathered by input_pos; 0: full tables.
  * Writes roped q to q_out (batch, n_head, T, head_size) and the roped k / v rows into the GQA-native caches. */

@@ -160,6 +160,23 @@ class AttnDecodeSharedArgs(ctypes.Structure):  # mirrors b200_attn_decode_shared
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+class AttnPagedArgs(ctypes.Structure):  # mirrors b200_attn_paged_args
+    _fields_ = [("qkv", c_void_p), ("cos", c_void_p), ("sin", c_void_p), ("table_dtype", c_int), ("table_rows", c_int), ("table_preselected", c_int),
+                ("rope_n_elem", c_int), ("row_pos", c_void_p), ("pos_is_int64", c_int), ("row_seq", c_void_p), ("seqs", c_void_p), ("n_seqs", c_int),
+                ("pages", c_void_p), ("pages_ld", c_int64), ("table_seqs", c_int), ("max_pages", c_int), ("pool", c_int), ("page", c_int), ("k_pages", c_void_p),
+                ("v_pages", c_void_p), ("k_page_stride", c_int64), ("k_group_stride", c_int64), ("v_page_stride", c_int64), ("v_group_stride", c_int64),
+                ("key_weights", c_void_p), ("out", c_void_p), ("rows", c_int64), ("max_rows", c_int64), ("max_length", c_int64), ("n_head", c_int),
+                ("n_groups", c_int), ("head_size", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class EvictPagedArgs(ctypes.Structure):  # mirrors b200_evict_paged_args
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_page_stride", c_int64), ("k_group_stride", c_int64), ("v_page_stride", c_int64),
+                ("v_group_stride", c_int64), ("key_weights", c_void_p), ("pages", c_void_p), ("pages_ld", c_int64), ("table_seqs", c_int), ("max_pages", c_int),
+                ("pool", c_int), ("page", c_int), ("lengths", c_void_p), ("rows", c_void_p), ("lengths_out", c_void_p), ("n_seqs", c_int), ("n_groups", c_int),
+                ("head_size", c_int), ("keep", c_int64), ("first", c_int64), ("recent", c_int64), ("max_length", c_int64), ("workspace", c_void_p),
+                ("workspace_bytes", c_size_t)]
+
+
 class LogitRules(ctypes.Structure):  # mirrors b200_logit_rules
     _fields_ = [("logits", c_void_p), ("logits_dtype", c_int), ("ld", c_int64), ("rows", c_int64), ("vocab", c_int64), ("counts", c_void_p), ("counts_ld", c_int64),
                 ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p), ("repetition_all", c_float), ("frequency_all", c_float),
@@ -308,6 +325,10 @@ _SIGNATURES = {
     "b200_attn_decode_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "b200_attn_decode_shared_tune": (c_int, [c_int]),
     "b200_attn_decode_shared": (c_int, [ctypes.POINTER(AttnDecodeSharedArgs), c_void_p]),
+    "b200_attn_paged_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]),
+    "b200_attn_paged": (c_int, [ctypes.POINTER(AttnPagedArgs), c_void_p]),
+    "b200_evict_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int64]),
+    "b200_evict_paged": (c_int, [ctypes.POINTER(EvictPagedArgs), c_void_p]),
     "b200_rope_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "b200_attn_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -1,0 +1,618 @@
+// A ragged step over a paged key-value cache: every sequence brings one token or a chunk of them, whose rotated keys and values join its pages, and
+//   o_i = sum_j softmax_j(q_i . k_j / sqrt(hs)) v_j   over the keys j <= cached + i of its sequence that have a page.
+// The rounding points are those of the model's step (lit_gpt/model.py:624-653, 767-773): q and k are bf16 after the rotation, the softmax is fp32 with a running maximum,
+// the result is rounded once.  A row that sees no key has a result of zero.
+//
+// Three launches: queries and new keys are turned and the new rows stored in their pages; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys;
+// a head's partial results are joined.  No counter or flag is left between calls, and two calls at a time share nothing.
+//
+// An item is a tile of queries of one sequence and group -- rows times heads of the group, row after row, so that the heads of a group share the keys that they read -- against the
+// sequence's keys.  The tiles of all items are one list, cut evenly over the warps of all SMs (attn_list.cuh): requests of unequal lengths leave no SM without work.
+//
+// The weight that a key receives, sum over the step's rows and the group's heads of its softmax weights, is computed from the rows' maxima and sums: a warp takes a tile of 32 keys and
+// goes through the queries that see it, S^T = K Q^T, the keys as rows: a key's sum stays with the lanes that hold its row.  No atomics: one order of additions.
+#include "attn_list.cuh"
+#include "paged.cuh"
+
+namespace b200 {
+
+using namespace list;
+
+namespace {
+
+constexpr int kMaxTiles = 1 << 29;          // of a step
+constexpr int kUnits = 3;                   // a warp's ring: units of 32 keys or 32 values
+
+__device__ __forceinline__ int64_t paged_pos(const PagedParams& p, int row) {
+  const int64_t at = p.table_presel ? row : p.pos64 ? reinterpret_cast<const int64_t*>(p.row_pos)[row] : (int64_t)reinterpret_cast<const int32_t*>(p.row_pos)[row];
+  return at < 0 ? 0 : (at >= p.table_rows ? p.table_rows - 1 : at);
+}
+
+// ---- the queries and the new keys turned, the new rows stored: a head a warp ----
+template <int HS>
+__global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) {
+  constexpr int V = HS / 32;
+  griddep_wait();     // (before the launch of what follows: the kernels behind read the step's description and the older keys ahead of their own wait)
+  griddep_launch();
+  const int lane = threadIdx.x & 31, heads = p.n_groups * (p.per + 2);
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int row = (int)(at / heads), i = (int)(at - (int64_t)row * heads), gi = i / (p.per + 2), h = i - gi * (p.per + 2);
+  if (row >= p.rows) return;
+  const int which = p.row_seq[row];
+  PagedSeq s = {};
+  if (which >= 0 && which < p.n_seqs) s = paged_seq(p, which);
+  const int mine = row - s.first, key = s.cached + mine;
+  if (mine < 0 || mine >= s.rows) {   // a row of no sequence
+    if (h < p.per) {
+      __nv_bfloat16* const to = p.out + ((int64_t)row * p.n_head + gi * p.per + h) * HS;
+      for (int j = 0; j < V; ++j) to[lane * V + j] = __float2bfloat16_rn(0.f);
+    }
+    return;
+  }
+  const __nv_bfloat16* const x = p.qkv + at * HS;
+  uint32_t v[HS / 64];
+  if (h <= p.per) {
+    turned_part<HS>(p, x, paged_pos(p, row), lane, v);
+  } else {
+    const uint16_t* const u = reinterpret_cast<const uint16_t*>(x + lane * V);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = (uint32_t)u[2 * j] | ((uint32_t)u[2 * j + 1] << 16);
+  }
+  __nv_bfloat16* to;
+  if (h < p.per) {
+    to = p.q + (((int64_t)gi * p.rows + row) * p.per + h) * HS;
+  } else {
+    if (key >= s.n) return;           // no room behind max_length
+    const int id = page_at(p, s.table, key >> p.shift), in = key & ((1 << p.shift) - 1);
+    if (id < 0) return;
+    to = (h == p.per ? p.k + (int64_t)id * p.k_page + (int64_t)gi * p.k_group : p.v + (int64_t)id * p.v_page + (int64_t)gi * p.v_group) + (int64_t)in * HS;
+    if (p.kw && h == p.per && lane == 0) p.kw[(((int64_t)id * p.n_groups + gi) << p.shift) + in] = 0.f;
+  }
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(to + lane * V) = make_uint2(v[0], v[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t*>(to + lane * V) = v[0];
+}
+
+// Workers take runs of the list's tiles, sequence after sequence, there group after group and tile of queries after tile of queries.  The result of item i by worker w goes to slot
+// i + w, which no other pair has, since either grows with the tiles.
+struct Split {
+  int all, workers;      // tiles; workers
+  int each, more;        // every worker has `each` tiles, the first `more` of them one more
+};
+__device__ __forceinline__ int worker_of(int tile, const Split& s) {
+  const int wide = s.more * (s.each + 1);
+  return tile < wide ? tile / (s.each + 1) : s.more + (tile - wide) / s.each;
+}
+__device__ __forceinline__ int first_tile(int w, const Split& s) { return w * s.each + min(w, s.more); }
+
+__device__ __forceinline__ int seq_items(const PagedParams& p, const PagedSeq& s) { return s.rows > 0 ? (s.rows * p.per + p.tile_rows - 1) / p.tile_rows : 0; }   // of a group
+__device__ __forceinline__ int seq_tiles(const PagedSeq& s) { return (s.n + kShTile - 1) / kShTile; }
+
+// Sequences are summed in runs of one per thread: sums[t] = tiles and items (of one group) of the sequences before run t, sums[THREADS] of all.
+template <int THREADS>
+__device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, int2* s_warp, bool note) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = (p.n_seqs + THREADS - 1) / THREADS;
+  // (a description whose sequences overlap can hold more tiles than fit the step's limits: then none is done)
+  auto capped = [](int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); };
+  int2 here = make_int2(0, 0);
+  for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
+    const PagedSeq s = paged_seq(p, i);
+    const int items = seq_items(p, s);
+    here.x = capped(here.x + (int64_t)items * seq_tiles(s));
+    here.y = capped((int64_t)here.y + items);
+  }
+  int2 inc = here;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
+    if (lane >= o) { inc.x = capped((int64_t)inc.x + x); inc.y = capped((int64_t)inc.y + y); }
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int2 before = make_int2(inc.x - here.x, inc.y - here.y);
+  for (int w = 0; w < warp; ++w) { before.x = capped((int64_t)before.x + s_warp[w].x); before.y = capped((int64_t)before.y + s_warp[w].y); }
+  sums[tid] = before;
+  if (tid == THREADS - 1) sums[THREADS] = make_int2(capped((int64_t)before.x + here.x), capped((int64_t)before.y + here.y));
+  if (note) {                            // who joins the results learns where a sequence's items begin
+    int items = before.y * p.n_groups;
+    for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
+      __stcg(p.item_base + i, items);
+      items += seq_items(p, paged_seq(p, i)) * p.n_groups;
+    }
+  }
+  __syncthreads();
+  Split s;
+  const int64_t all = (int64_t)sums[THREADS].x * p.n_groups, items = (int64_t)sums[THREADS].y * p.n_groups;
+  s.all = all < kMaxTiles && items <= p.items ? (int)all : 0;
+  // two tiles a worker at least, unless that leaves SMs without one
+  s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
+  s.each = s.workers ? s.all / s.workers : 0;
+  s.more = s.all - s.each * s.workers;
+  return s;
+}
+
+// A tile of a worker's range, and the item that it belongs to.
+struct Tile {
+  int index;                         // in the order of all tiles
+  int s, gi, part;                   // sequence, group, tile of queries
+  PagedSeq seq;
+  int tile, tiles;                   // of the item
+  int item;
+  int id0, id1;                      // pages of its first and last sixteen keys
+  __device__ __forceinline__ int left() const { return tiles - 1 - tile; }
+  __device__ __forceinline__ int key0() const { return tile * kShTile; }
+  __device__ __forceinline__ uint32_t bits() const {   // its keys that are there
+    const int rest = seq.n - key0();
+    const uint32_t in = rest >= 32 ? 0xffffffffu : (1u << rest) - 1u;
+    return in & ((id0 >= 0 ? 0xffffu : 0u) | (id1 >= 0 ? 0xffff0000u : 0u));
+  }
+};
+
+struct Walk {
+  const PagedParams& p;
+  const int2* sums;
+  int run, threads;
+
+  __device__ __forceinline__ void locate(Tile& t) const {
+    const int i = t.key0() >> p.shift;
+    t.id0 = page_at(p, t.seq.table, i);
+    t.id1 = p.shift == 4 && t.key0() + 16 < t.seq.n ? page_at(p, t.seq.table, i + 1) : t.id0;
+  }
+  __device__ __forceinline__ Tile find(int index) const {
+    Tile t;
+    t.index = index;
+    int lo = 0, hi = threads;        // the run whose sequences hold it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (sums[mid].x * p.n_groups <= index) lo = mid; else hi = mid;
+    }
+    int rest = index - sums[lo].x * p.n_groups;
+    t.item = sums[lo].y * p.n_groups;
+    t.s = lo * run;
+    for (;;) {                       // (one sequence a run unless there are many)
+      t.seq = paged_seq(p, t.s);
+      t.tiles = seq_tiles(t.seq);
+      const int items = seq_items(p, t.seq), here = items * t.tiles * p.n_groups;
+      if (rest < here) {
+        const int item = rest / t.tiles;
+        t.tile = rest - item * t.tiles;
+        t.item += item;
+        t.gi = item / items;
+        t.part = item - t.gi * items;
+        break;
+      }
+      rest -= here;
+      t.item += items * p.n_groups;
+      ++t.s;
+    }
+    locate(t);
+    return t;
+  }
+  // the tile behind it (there is one)
+  __device__ __forceinline__ void next(Tile& t) const {
+    ++t.index;
+    if (++t.tile == t.tiles) {
+      t.tile = 0;
+      ++t.item;
+      if (++t.part == seq_items(p, t.seq)) {
+        t.part = 0;
+        if (++t.gi == p.n_groups) {
+          t.gi = 0;
+          do t.seq = paged_seq(p, ++t.s); while (t.seq.n == 0);
+          t.tiles = seq_tiles(t.seq);
+        }
+      }
+    }
+    locate(t);
+  }
+  __device__ __forceinline__ int queries(const Tile& t) const { return min(p.tile_rows, t.seq.rows * p.per - t.part * p.tile_rows); }
+  __device__ __forceinline__ int64_t query_row(const Tile& t) const { return ((int64_t)t.gi * p.rows + t.seq.first) * p.per + t.part * p.tile_rows; }
+};
+
+// 32 rows of a tile, zeros where there is no key: a weight of zero times whatever lies there must be zero
+template <int HS>
+__device__ __forceinline__ void load_tile(const PagedParams& p, const Tile& t, const __nv_bfloat16* base, int64_t page, int64_t group, uint32_t dst, int lane) {
+  constexpr int CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
+  const uint32_t bits = t.bits();
+  const int c = lane % CH, in = t.key0() & ((1 << p.shift) - 1);
+  const __nv_bfloat16* const g = base + (int64_t)t.gi * group + c * 8;
+  const __nv_bfloat16* const a = g + (int64_t)max(t.id0, 0) * page + (int64_t)in * HS;
+  const __nv_bfloat16* const b = p.shift == 4 ? g + (int64_t)max(t.id1, 0) * page - (int64_t)16 * HS : a;
+#pragma unroll
+  for (int j = 0; j < kShTile / RP; ++j) {
+    const int r = j * RP + lane / CH;
+    const bool ok = (bits >> r) & 1u;
+    const __nv_bfloat16* const src = j * RP < 16 ? a : b;
+    pf_cp16(dst + sw<HS>(r, c), ok ? src + r * HS : g, ok);
+  }
+}
+
+// A warp's shared memory: a ring of units, the queries of two items.  One CTA an SM.  Queries come in eights, NQ of them.
+template <int HS, int NQ>
+struct PgSmem {
+  static constexpr int kUnit = kShTile * HS * 2, kQ = 8 * NQ * HS * 2;
+  static constexpr int kWarp = kUnits * kUnit + 2 * kQ;
+  static constexpr int kWarps = HS == 64 ? (NQ == 4 ? 10 : 12) : (NQ == 4 ? 5 : 7);
+  static constexpr int kBytes = kWarps * kWarp;
+};
+
+template <int HS, int NQ>
+__global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_kernel(const PagedParams p) {
+  using C = PgSmem<HS, NQ>;
+  constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;
+  extern __shared__ __align__(128) uint8_t pg_smem[];
+  __shared__ int2 s_sums[T + 1], s_warp[C::kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tq = lane & 3;
+  griddep_launch();
+  const Split s = make_split<T>(p, s_sums, s_warp, blockIdx.x == 0);
+  const int w = warp * (int)gridDim.x + (int)blockIdx.x;   // (workers beside each other on different SMs)
+  if (w >= s.workers) {
+    griddep_wait();
+    return;
+  }
+  const Walk walk{p, s_sums, (p.n_seqs + T - 1) / T, T};
+  const uint32_t ring = pf_smem(pg_smem) + warp * C::kWarp, sq = ring + kUnits * C::kUnit;
+
+  auto load_k = [&](uint32_t dst, const Tile& t) { load_tile<HS>(p, t, p.k, p.k_page, p.k_group, dst, lane); };
+  auto load_v = [&](uint32_t dst, const Tile& t) { load_tile<HS>(p, t, p.v, p.v_page, p.v_group, dst, lane); };
+  auto load_queries = [&](uint32_t dst, const Tile& t) {
+    const __nv_bfloat16* const src = p.q + walk.query_row(t) * HS;
+    const int valid = walk.queries(t);
+#pragma unroll
+    for (int j = 0; j < 8 * NQ / RP; ++j) {
+      const int r = j * RP + lane / CH, c = lane % CH;
+      const bool ok = r < valid;
+      pf_cp16(dst + sw<HS>(r, c), src + (ok ? r * HS : 0) + c * 8, ok);
+    }
+  };
+  const int first = first_tile(w, s), end = first_tile(w + 1, s);
+  Tile cur = walk.find(first);
+  Tile coming = cur;                                       // the tile behind it: its values are loaded next
+  const bool two = cur.index + 1 < end;
+  if (two) walk.next(coming);
+  // What the append kernel writes, queries and new keys, is read behind the wait; everything else was there before.
+  auto early = [&](bool now) {
+    const bool c = now == (cur.key0() + kShTile <= cur.seq.cached), n = two && now == (coming.key0() + kShTile <= coming.seq.cached);
+    if (c) {
+      load_k(ring, cur);
+      load_v(ring + C::kUnit, cur);
+    }
+    if (n) load_k(ring + 2 * C::kUnit, coming);
+  };
+  early(true);
+  griddep_wait();
+  early(false);
+  load_queries(sq, cur);
+  int qb = 0, next_qb = 0;                                 // the query buffers of either
+  if (two && cur.left() == 0) load_queries(sq + (next_qb = 1) * C::kQ, coming);
+  pf_commit();
+  pf_commit();
+  pf_commit();
+
+  Sums<HS, NQ> a;
+  auto clear = [&]() {
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+#pragma unroll
+      for (int i = 0; i < HS / 16; ++i) a.o[i][t][0] = a.o[i][t][1] = a.o[i][t][2] = a.o[i][t][3] = 0.f;
+      a.m[t][0] = a.m[t][1] = -INFINITY;
+      a.l[t][0] = a.l[t][1] = 0.f;
+    }
+  };
+  clear();
+  int unit = 0;                                            // of the current tile's keys
+  for (;;) {
+    const uint32_t kb = ring + unit * C::kUnit;
+    unit = unit == kUnits - 1 ? 0 : unit + 1;
+    const uint32_t vb = ring + unit * C::kUnit;
+    unit = unit == kUnits - 1 ? 0 : unit + 1;
+    const bool more = cur.index + 1 < end;
+    pf_wait<2>();
+    __syncwarp();
+    auto values = [&]() {
+      __syncwarp();                                        // the keys have been read: the values of the next tile take their place
+      if (more) load_v(kb, coming);
+      pf_commit();
+      pf_wait<2>();
+      __syncwarp();
+      return vb;
+    };
+    const uint32_t bits = cur.bits();
+    const int key0 = cur.key0(), count = walk.queries(cur);
+    if (key0 + kShTile > cur.seq.cached + 1 && cur.seq.rows > 1) {   // a chunk's own keys: every row sees those up to its own
+      int lim[NQ][2];
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) lim[t][c] = cur.seq.cached + (cur.part * p.tile_rows + t * 8 + 2 * tq + c) / p.per - key0;
+      attend_tile<HS, NQ, NQ>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, [&](int key, int t, int c) { return ((bits >> key) & 1u) && key <= lim[t][c]; }, values);
+    } else {
+      auto seen = [bits](int key, int, int) { return ((bits >> key) & 1u) != 0u; };
+      if (NQ == 1 || count > 8) attend_tile<HS, NQ, NQ>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, values);
+      else attend_tile<HS, NQ, 1>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, values);
+    }
+    __syncwarp();                                          // the values have been read: the keys of the tile after the next take their place
+    const bool ends = cur.left() == 0 || !more;
+    const Tile was = cur;
+    cur = coming;
+    qb = next_qb;
+    if (cur.index + 1 < end) {
+      walk.next(coming);
+      load_k(vb, coming);
+      if (cur.left() == 0) load_queries(sq + (next_qb = qb ^ 1) * C::kQ, coming);
+    }
+    pf_commit();
+    if (ends) {
+      // ---- the item, or this worker's part of it, ends ----
+      const int64_t slot = (int64_t)was.item + w;
+      if (lane == 0 && was.index - was.tile >= first)      // it began here: who joins its results learns where they are
+        __stcg(p.where + was.item, make_int2(w, worker_of(was.index + was.left(), s) - w + 1));
+      store_sums<HS, NQ>(a, p.acc + slot * p.tile_rows * HS, p.ml + slot * p.tile_rows, walk.queries(was), lane);
+      if (!more) break;
+      clear();
+    }
+  }
+  pf_wait<0>();
+}
+
+// A head's results joined: `ways` warps a head, HS / 32 numbers a lane.
+template <int HS>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  constexpr int V = HS / 32;
+  __shared__ float s_acc[8][HS];
+  __shared__ float2 s_ml[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = 8 / p.ways, blocks = (p.n_head + heads - 1) / heads;
+  const int row = blockIdx.x / blocks, h = (blockIdx.x - row * blocks) * heads + warp / p.ways, way = warp % p.ways;
+  griddep_launch();
+  const int which = p.row_seq[row];
+  PagedSeq s = {};
+  if (which >= 0 && which < p.n_seqs) s = paged_seq(p, which);
+  const bool idle = row < s.first || row - s.first >= s.rows;
+  griddep_wait();
+  float top = -INFINITY, sum = 0.f, a[V] = {};
+  const int gi = h / p.per, m = (row - s.first) * p.per + h - gi * p.per;
+  int item = -1;
+  if (h < p.n_head && !idle && s.n > 0) item = __ldcg(p.item_base + which) + gi * seq_items(p, s) + m / p.tile_rows;
+  if (item >= 0 && item < p.items) {
+    const int at = m % p.tile_rows;
+    const int2 at_w = __ldcg(p.where + item);
+    join_results<V>(way, p.ways, at_w.y, lane, top, sum, a, [&](int i, const float2*& ml, const float*& acc) {
+      const int64_t slot = ((int64_t)item + at_w.x + i) * p.tile_rows + at;
+      ml = p.ml + slot;
+      acc = p.acc + slot * HS;
+    });
+  }
+  if (p.ways > 1) {
+    if (way > 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) s_acc[warp][lane * V + j] = a[j];
+      if (lane == 0) s_ml[warp] = make_float2(top, sum);
+    }
+    __syncthreads();
+    if (way == 0) join_warps<HS>(s_acc[warp], s_ml + warp, p.ways, lane, top, sum, a);
+  }
+  if (way > 0 || h >= p.n_head || idle) return;
+  store_result<HS>(p.out + ((int64_t)row * p.n_head + h) * HS, a, sum > 0.f ? 1.f / sum : 0.f, lane);
+  if (p.lse && lane == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h - gi * p.per] = sum > 0.f ? top + log2f(sum) : INFINITY;
+}
+
+// ---- the weight that every key receives ----
+template <int HS>
+struct KwSmem {
+  static constexpr int kKeys = kShTile * HS * 2, kQ = 16 * HS * 2, kWarp = kKeys + 2 * kQ, kWarps = 4, kBytes = kWarps * kWarp;
+};
+
+template <int HS>
+__global__ void __launch_bounds__(KwSmem<HS>::kWarps * 32) paged_weights_kernel(const PagedParams p) {
+  using C = KwSmem<HS>;
+  constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;
+  extern __shared__ __align__(128) uint8_t kw_smem[];
+  __shared__ int2 s_sums[T + 1], s_warp[C::kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
+  griddep_wait();
+  griddep_launch();
+  const int all = make_split<T>(p, s_sums, s_warp, false).all;
+  const Walk walk{p, s_sums, (p.n_seqs + T - 1) / T, T};
+  const uint32_t sk = pf_smem(kw_smem) + warp * C::kWarp, sq = sk + C::kKeys;
+  for (int index = blockIdx.x * C::kWarps + warp; index < all; index += gridDim.x * C::kWarps) {
+    const Tile t = walk.find(index);
+    const uint32_t bits = t.bits();
+    const int key0 = t.key0(), m0 = max(0, key0 - t.seq.cached) * p.per & ~15, count = t.seq.rows * p.per;   // (earlier rows see none of these keys)
+    const int64_t q0 = ((int64_t)t.gi * p.rows + t.seq.first) * p.per;
+    auto load_queries = [&](int m, int buf) {
+#pragma unroll
+      for (int j = 0; j < 16 / RP; ++j) {
+        const int r = j * RP + lane / CH, c = lane % CH;
+        const bool ok = m + r < count;
+        pf_cp16(sq + buf * C::kQ + sw<HS>(r, c), p.q + (q0 + (ok ? m + r : 0)) * HS + c * 8, ok);
+      }
+      pf_commit();
+    };
+    load_tile<HS>(p, t, p.k, p.k_page, p.k_group, sk, lane);
+    load_queries(m0, 0);
+    float sum[2][2] = {};                      // keys 16 i + 8 h + g
+    for (int m = m0, buf = 0; m < count; m += 16, buf ^= 1) {
+      float lse[2][2];
+      int lim[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int mm = m + u * 8 + 2 * tq + c;
+          lse[u][c] = mm < count ? __ldcg(p.lse + q0 + mm) : INFINITY;
+          lim[u][c] = mm < count ? t.seq.cached + mm / p.per - key0 : -1;
+        }
+      if (m + 16 < count) { load_queries(m + 16, buf ^ 1); pf_wait<1>(); } else { pf_wait<0>(); }
+      __syncwarp();
+      float s[2][2][4] = {};
+#pragma unroll
+      for (int kp = 0; kp < HS / 32; ++kp) {
+        uint32_t qf[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) ldsm_x4(qf[u], sq + buf * C::kQ + sw<HS>(u * 8 + (lane & 7), kp * 4 + (lane >> 3)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t kf[4];
+            ldsm_x4(kf, sk + sw<HS>(i * 16 + (lane & 15), kp * 4 + h * 2 + (lane >> 4)));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) pf_mma(s[i][u], kf, qf[u][2 * h], qf[u][2 * h + 1]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = i * 16 + (e >> 1) * 8 + g;
+            sum[i][e >> 1] += key <= lim[u][e & 1] ? ex2(fmaf(s[i][u][e], p.scale_log2, -lse[u][e & 1])) : 0.f;
+          }
+      __syncwarp();                            // the queries have been read
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = sum[i][h];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        const int key = i * 16 + h * 8 + g;
+        if (tq == 0 && ((bits >> key) & 1u)) {
+          const int id = key < 16 ? t.id0 : t.id1, in = (key0 + key) & ((1 << p.shift) - 1);
+          p.kw[(((int64_t)id * p.n_groups + t.gi) << p.shift) + in] += x;
+        }
+      }
+    pf_wait<0>();
+    __syncwarp();
+  }
+}
+
+// ---- host ----
+struct PagedPlan {
+  int nq, ctas, workers, ways;
+  int64_t items, slots, q;
+  size_t bytes;
+};
+
+PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, int64_t max_rows, int64_t max_length, bool kw) {
+  PagedPlan s;
+  const int64_t most = max_rows * per;
+  s.nq = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+  s.items = (int64_t)n_groups * ((rows * per + 8 * s.nq - 1) / (8 * s.nq) + n_seqs);
+  const int warps = hs == 64 ? (s.nq == 4 ? PgSmem<64, 4>::kWarps : PgSmem<64, 1>::kWarps) : (s.nq == 4 ? PgSmem<128, 4>::kWarps : PgSmem<128, 1>::kWarps);
+  const int64_t tiles = s.items * ((max_length + kShTile - 1) / kShTile);
+  s.ctas = sm_count();
+  if (s.ctas > tiles) s.ctas = (int)tiles;
+  s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
+  s.slots = (s.items + s.workers) * 8 * s.nq;
+  s.q = rows * per * n_groups * hs;
+  s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * sizeof(int) +
+            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0);
+  const int64_t results = 2 + (int64_t)s.workers / s.items;
+  s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
+  while (s.ways < 8 && results > 4 * s.ways && rows * n_groups * per * s.ways < 24 * sm_count()) s.ways *= 2;
+  return s;
+}
+
+template <int HS, int NQ>
+cudaError_t launch_list(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
+  using C = PgSmem<HS, NQ>;
+  static PerDeviceOnce once;
+  if (once.need()) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_list_kernel<HS, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (e != cudaSuccess) return e;
+    once.done();
+  }
+  return launch(paged_list_kernel<HS, NQ>, dim3((unsigned)s.ctas), dim3(C::kWarps * 32), (size_t)C::kBytes, st, p);
+}
+
+template <int HS>
+cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
+  const int64_t warps = (int64_t)p.rows * p.n_groups * (p.per + 2);
+  cudaError_t e = launch(paged_append_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
+  if (e != cudaSuccess) return e;
+  e = s.nq == 4 ? launch_list<HS, 4>(p, s, st) : s.nq == 2 ? launch_list<HS, 2>(p, s, st) : launch_list<HS, 1>(p, s, st);
+  if (e != cudaSuccess) return e;
+  const int heads = 8 / s.ways;
+  e = launch(paged_join_kernel<HS>, dim3((unsigned)(p.rows * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
+  if (e != cudaSuccess || !p.kw) return e;
+  using C = KwSmem<HS>;
+  static PerDeviceOnce once;
+  if (once.need()) {
+    e = cudaFuncSetAttribute(paged_weights_kernel<HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (e != cudaSuccess) return e;
+    once.done();
+  }
+  PagedParams one = p;             // the queries of a sequence and group as one tile: the list is that of the key tiles
+  one.tile_rows = 0x3fffffff;
+  return launch(paged_weights_kernel<HS>, dim3((unsigned)(4 * p.sms)), dim3(C::kWarps * 32), (size_t)C::kBytes, st, one);
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int n_groups, int head_size, int64_t max_rows, int64_t max_length, int key_weights) {
+  if (rows <= 0 || n_seqs <= 0 || n_groups <= 0 || n_head <= 0 || n_head % n_groups || max_rows <= 0 || max_rows > rows || max_length <= 0 || (head_size != 64 && head_size != 128) ||
+      rows * n_head >= (1 << 24) || n_seqs > (1 << 20) || max_length >= (1 << 30))
+    return 0;
+  return paged_plan(rows, n_seqs, n_groups, n_head / n_groups, head_size, max_rows, max_length, key_weights != 0).bytes;
+}
+
+int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
+  B200_CHECK_ARG(a, "b200_attn_paged: null argument");
+  B200_CHECK_ARG(a->head_size == 64 || a->head_size == 128, "b200_attn_paged: head size %d (64 or 128)", a->head_size);
+  B200_CHECK_ARG(a->rows > 0 && a->n_seqs > 0 && a->n_groups > 0 && a->n_head > 0 && a->n_head % a->n_groups == 0, "b200_attn_paged: bad rows, sequences, heads %d or groups %d",
+                 a->n_head, a->n_groups);
+  B200_CHECK_ARG(a->rows < (1 << 24) && a->rows * a->n_head < (1 << 24) && a->n_seqs <= (1 << 20), "b200_attn_paged: too many rows or sequences in a step");
+  B200_CHECK_ARG(a->max_rows > 0 && a->max_rows <= a->rows, "b200_attn_paged: sequences of up to %lld rows, of %lld", (long long)a->max_rows, (long long)a->rows);
+  B200_CHECK_ARG(a->page >= 16 && a->page <= 256 && (a->page & (a->page - 1)) == 0, "b200_attn_paged: pages of %d keys (16, 32, 64, 128 or 256)", a->page);
+  B200_CHECK_ARG(a->pool > 0 && a->table_seqs > 0 && a->max_pages > 0 && a->pages_ld >= a->max_pages, "b200_attn_paged: no pages, or a bad page table");
+  B200_CHECK_ARG(a->max_length > 0 && a->max_length <= (int64_t)a->max_pages * a->page && a->max_length < (1 << 30), "b200_attn_paged: %lld keys in %d pages of %d",
+                 (long long)a->max_length, a->max_pages, a->page);
+  B200_CHECK_ARG(a->qkv && a->row_pos && a->row_seq && a->seqs && a->pages && a->k_pages && a->v_pages && a->out && a->workspace, "b200_attn_paged: null pointer");
+  B200_CHECK_ARG(a->rope_n_elem >= 0 && a->rope_n_elem <= a->head_size && a->rope_n_elem % 2 == 0, "b200_attn_paged: bad rope_n_elem %d", a->rope_n_elem);
+  B200_CHECK_ARG(a->rope_n_elem == 0 || (a->cos && a->sin && a->table_rows > 0), "b200_attn_paged: no tables");
+  B200_CHECK_ARG(!a->table_preselected || a->rope_n_elem == 0 || a->table_rows >= a->rows, "b200_attn_paged: %d preselected table rows for %lld rows", a->table_rows, (long long)a->rows);
+  B200_CHECK_ARG(a->table_dtype == B200_F32 || a->table_dtype == B200_BF16, "b200_attn_paged: tables must be fp32 or bf16");
+  const uintptr_t at = (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)a->workspace | (uintptr_t)a->seqs;
+  const int64_t strides = a->k_page_stride | a->k_group_stride | a->v_page_stride | a->v_group_stride;
+  B200_CHECK_ARG((at & 15) == 0 && (strides & 7) == 0 && ((uintptr_t)a->out & 7) == 0 && ((uintptr_t)a->key_weights & 3) == 0,
+                 "b200_attn_paged: pages, workspace and the sequences' description must lie on 16-byte boundaries");
+  const int per = a->n_head / a->n_groups;
+  const PagedPlan s = paged_plan(a->rows, a->n_seqs, a->n_groups, per, a->head_size, a->max_rows, a->max_length, a->key_weights != nullptr);
+  B200_CHECK_ARG(s.items * ((a->max_length + kShTile - 1) / kShTile) < kMaxTiles, "b200_attn_paged: too many keys in a step");
+  B200_CHECK_ARG(a->workspace_bytes >= s.bytes, "b200_attn_paged: workspace too small");
+  PagedParams p = {};
+  p.qkv = (const __nv_bfloat16*)a->qkv;
+  p.cos = a->cos; p.sin = a->sin; p.table_bf16 = a->table_dtype == B200_BF16; p.table_rows = a->table_rows; p.table_presel = a->table_preselected; p.rope_n = a->rope_n_elem;
+  const int n = a->rope_n_elem, part = a->head_size / 32;
+  p.wide = ((uintptr_t)a->qkv & 15) == 0 && n % (2 * part) == 0 && (a->table_dtype == B200_BF16 || (((uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0);
+  p.row_pos = a->row_pos; p.pos64 = a->pos_is_int64; p.row_seq = a->row_seq;
+  p.seqs = (const int4*)a->seqs; p.n_seqs = a->n_seqs;
+  p.pages = a->pages; p.pages_ld = a->pages_ld; p.page_rows = a->table_seqs; p.max_pages = a->max_pages; p.pool = a->pool;
+  for (p.shift = 4; (1 << p.shift) < a->page; ++p.shift) {}
+  p.k = (__nv_bfloat16*)a->k_pages; p.v = (__nv_bfloat16*)a->v_pages;
+  p.k_page = a->k_page_stride; p.k_group = a->k_group_stride; p.v_page = a->v_page_stride; p.v_group = a->v_group_stride;
+  p.kw = a->key_weights;
+  p.out = (__nv_bfloat16*)a->out;
+  p.rows = (int)a->rows; p.n_head = a->n_head; p.n_groups = a->n_groups; p.per = per; p.max_length = (int)a->max_length;
+  p.tile_rows = 8 * s.nq; p.items = (int)s.items; p.workers = s.workers; p.sms = sm_count(); p.ways = s.ways;
+  // (every part of wide accesses begins on a 16-byte boundary: they come first)
+  p.q = (__nv_bfloat16*)a->workspace;
+  p.acc = (float*)(p.q + s.q);
+  p.ml = (float2*)(p.acc + s.slots * a->head_size);
+  p.where = (int2*)(p.ml + s.slots);
+  p.item_base = (int*)(p.where + s.items);
+  p.lse = p.kw ? (float*)(p.item_base + a->n_seqs) : nullptr;
+  p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
+  const cudaStream_t st = (cudaStream_t)stream;
+  B200_CUDA((a->head_size == 128 ? launch_paged<128>(p, s, st) : launch_paged<64>(p, s, st)));
+  return B200_OK;
+}
+
+}  // extern "C"

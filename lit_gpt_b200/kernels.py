@@ -887,6 +887,124 @@ def _shared_workspace_bytes(device: int, batch: int, n_head: int, n_groups: int,
     return int(C.load().b200_attn_decode_shared_workspace_bytes(batch, n_head, n_groups, head_size, prefix_rows, own_rows))
 
 
+def _pages_of(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, key_weights: Optional[torch.Tensor], table: torch.Tensor, n_groups: int,
+              head_size: int) -> Tuple[int, int, int, int, int, int]:
+    """The paged cache checked -> its pages, keys of a page, and the distances of pages and groups of keys and of values."""
+    shape, bf16 = k_pages.shape, torch.bfloat16
+    if len(shape) != 4 or shape != v_pages.shape or shape[1] != n_groups or shape[3] != head_size or k_pages.dtype is not bf16 or v_pages.dtype is not bf16:
+        raise C.B200Error(f"{what}: pages must be bfloat16 (pages, {n_groups}, page, {head_size}) (got {k_pages.dtype}, {tuple(shape)}, {v_pages.dtype}, {tuple(v_pages.shape)})")
+    pool, G, page, hs = shape
+    kp, kg, kr, ke = k_pages.stride()
+    vp, vg, vr, ve = v_pages.stride()
+    if ke != 1 or ve != 1 or kr != hs or vr != hs:
+        raise C.B200Error(f"{what}: the rows of a page must lie next to each other")
+    for a, b in ((kp, kg), (vp, vg)):   # (a tensor of one page or group may have any distance)
+        if (G > 1 and b < page * hs) or (pool > 1 and a < page * hs) or (G > 1 and pool > 1 and a < (G - 1) * b + page * hs and b < (pool - 1) * a + page * hs):
+            raise C.B200Error(f"{what}: pages or groups overlap")
+    if key_weights is not None and (key_weights.dtype is not torch.float32 or key_weights.shape != (pool, G, page) or not key_weights.is_contiguous()):
+        raise C.B200Error(f"{what}: key_weights must be contiguous fp32 ({pool}, {G}, {page}) (got {key_weights.dtype}, {tuple(key_weights.shape)})")
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.numel() == 0 or (table.shape[1] > 1 and table.stride(1) != 1) or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+        raise C.B200Error(f"{what}: the page table must be int32 (sequences, pages), the entries of a sequence next to each other (got {table.dtype}, {tuple(table.shape)})")
+    return pool, page, kp if pool > 1 else 0, kg if G > 1 else 0, vp if pool > 1 else 0, vg if G > 1 else 0
+
+
+def attn_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor, seqs: torch.Tensor, table: torch.Tensor,
+               k_pages: torch.Tensor, v_pages: torch.Tensor, n_head: int, n_groups: int, head_size: int, rope_n_elem: int, *, max_rows: int, max_length: int,
+               key_weights: Optional[torch.Tensor] = None, table_preselected: bool = False) -> torch.Tensor:
+    """Rotation, cache append and causal attention of a ragged step over a paged cache: any mix of sequences that bring one token and sequences that bring a chunk.
+
+    qkv (rows, (H+2G)*hs) bf16 (further leading dimensions are rows, too); cos/sin: the model's FULL tables (positions, rope_n_elem), with ``table_preselected`` one row per row of qkv;
+    row_pos int32/int64 (rows,): positions for the rotation (a cache that was cut down holds fewer keys than the sequence has positions); row_seq int32 (rows,): index of
+    each row's sequence in seqs, -1 for a row of none, whose result is zero; seqs int32 (S, 4) per sequence: first row, rows, keys in the cache before the step, row of the page
+    table (``ragged.state_batch`` makes row_seq and seqs).  table int32 (sequences, pages): entry i of a row is the page of keys i * page and on; where an entry is no page, there are
+    no keys -- new ones are dropped, the rest take no part.  k_pages / v_pages (pages, G, page, hs) bf16, updated in place, pages of 16, 32, 64, 128 or 256 keys, any distance between pages
+    and groups that is a multiple of 8 numbers.  key_weights fp32 (pages, G, page): new keys begin at zero, every key gains the sum of its softmax weights over the step's rows and
+    its group's heads.  max_rows, max_length: bounds (on the host) of a sequence's rows and of its keys behind the step; keys from max_length on are dropped.
+    No page belongs to two sequences that bring rows into it.  Returns (rows, H*hs)."""
+    device, bf16 = qkv.get_device(), torch.bfloat16
+    if (device < 0 or cos.get_device() != device or sin.get_device() != device or row_pos.get_device() != device or row_seq.get_device() != device or seqs.get_device() != device
+            or table.get_device() != device or k_pages.get_device() != device or v_pages.get_device() != device or (key_weights is not None and key_weights.get_device() != device)):
+        C.require_cuda(qkv)
+        _one_device("attn_paged", device, cos, sin, row_pos, row_seq, seqs, table, k_pages, v_pages, key_weights)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return attn_paged(qkv, cos, sin, row_pos, row_seq, seqs, table, k_pages, v_pages, n_head, n_groups, head_size, rope_n_elem, max_rows=max_rows, max_length=max_length,
+                              key_weights=key_weights, table_preselected=table_preselected)
+    if qkv.dtype is not bf16 or not qkv.is_contiguous():
+        qkv = _bf16c(qkv, "qkv")
+    pool, page, kp, kg, vp, vg = _pages_of("attn_paged", k_pages, v_pages, key_weights, table, n_groups, head_size)
+    width = (n_head + 2 * n_groups) * head_size
+    rows = qkv.numel() // max(width, 1)
+    if rows * width != qkv.numel() or qkv.shape[-1] != width:
+        raise C.B200Error(f"attn_paged: qkv must be (rows, {width}) (got {tuple(qkv.shape)})")
+    kind = row_pos.dtype
+    if (kind is not torch.int32 and kind is not torch.int64) or row_pos.numel() != rows or row_seq.dtype is not torch.int32 or row_seq.numel() != rows:
+        raise C.B200Error(f"attn_paged: row_pos (int32 or int64) and row_seq (int32) must have one entry per row (got {row_pos.numel()}, {row_seq.numel()} for {rows} rows)")
+    if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4:
+        raise C.B200Error(f"attn_paged: seqs must be int32 (sequences, 4) (got {seqs.dtype}, {tuple(seqs.shape)})")
+    out = qkv.new_empty((rows, n_head * head_size))
+    if rows == 0 or seqs.shape[0] == 0:
+        return out.zero_()
+    shape = cos.shape
+    if shape != sin.shape or shape[-1] != rope_n_elem or cos.dtype is not sin.dtype:
+        raise C.B200Error(f"attn_paged: cos and sin must be (positions, {rope_n_elem}) of one dtype")
+    if not (cos.is_contiguous() and sin.is_contiguous() and row_pos.is_contiguous() and row_seq.is_contiguous() and seqs.is_contiguous()):
+        cos, sin, row_pos, row_seq, seqs = cos.contiguous(), sin.contiguous(), row_pos.contiguous(), row_seq.contiguous(), seqs.contiguous()
+    if seqs.data_ptr() % 16:
+        seqs = seqs.clone()
+    table_rows = cos.numel() // max(rope_n_elem, 1)
+    nbytes = _paged_workspace_bytes(device, rows, seqs.shape[0], n_head, n_groups, head_size, max_rows, max_length, key_weights is not None)
+    ws = qkv.new_empty(max(nbytes // 2, 8))   # of this call: calls on two streams, or in two graphs, have one each
+    args = C.AttnPagedArgs(
+        qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, row_pos.data_ptr(), kind is torch.int64, row_seq.data_ptr(),
+        seqs.data_ptr(), seqs.shape[0], table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[0], table.shape[1], pool, page, k_pages.data_ptr(),
+        v_pages.data_ptr(), kp, kg, vp, vg, None if key_weights is None else key_weights.data_ptr(), out.data_ptr(), rows, max_rows, max_length, n_head, n_groups, head_size,
+        ws.data_ptr(), nbytes)
+    C.check(C.load().b200_attn_paged(ctypes.byref(args), _raw_stream(device)), "attn_paged")
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace_bytes(device: int, rows: int, n_seqs: int, n_head: int, n_groups: int, head_size: int, max_rows: int, max_length: int, key_weights: bool) -> int:
+    return int(C.load().b200_attn_paged_workspace_bytes(rows, n_seqs, n_head, n_groups, head_size, max_rows, max_length, key_weights))
+
+
+def evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, key_weights: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, keep: int, *, max_length: int, first: int = 0,
+                recent: int = 0, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sequences of a paged cache (``attn_paged``) cut down to ``keep`` keys each, every group by itself: the ``first`` first keys, the ``recent`` last and, of those between, the ones with
+    the largest key_weights (equal ones: the lower index; NaN counts as the largest) stay and move to the front of the sequence's pages in order -- keys, values and weights, in
+    place; what lies behind them stays as it was.  lengths int32 (S,): keys of each sequence, at most max_length; rows int32 (S,): its row of the page table (None: row i).  A sequence of at
+    most ``keep`` keys, of more than max_length, or with an entry that is no page among its own stays as it is.  No page belongs to two sequences of the call.
+    Returns the keys of each sequence behind the call, int32 (S,)."""
+    device = k_pages.get_device()
+    if (device < 0 or v_pages.get_device() != device or key_weights.get_device() != device or table.get_device() != device or lengths.get_device() != device
+            or (rows is not None and rows.get_device() != device)):
+        C.require_cuda(k_pages)
+        _one_device("evict_paged", device, v_pages, key_weights, table, lengths, rows)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return evict_paged(k_pages, v_pages, key_weights, table, lengths, keep, max_length=max_length, first=first, recent=recent, rows=rows)
+    if k_pages.dim() != 4:
+        raise C.B200Error(f"evict_paged: pages must be bfloat16 (pages, groups, page, head_size) (got {tuple(k_pages.shape)})")
+    G, hs = k_pages.shape[1], k_pages.shape[3]
+    pool, page, kp, kg, vp, vg = _pages_of("evict_paged", k_pages, v_pages, key_weights, table, G, hs)
+    for t, name in ((lengths, "lengths"), (rows, "rows")):
+        if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != lengths.numel()):
+            raise C.B200Error(f"evict_paged: {name} must be int32, one per sequence (got {t.dtype}, {tuple(t.shape)})")
+    out = torch.empty_like(lengths, memory_format=torch.contiguous_format)
+    S = lengths.numel()
+    if S == 0:
+        return out
+    lengths, rows = lengths.contiguous(), None if rows is None else rows.contiguous()
+    nbytes = int(C.load().b200_evict_paged_workspace_bytes(S, G, keep))
+    ws = k_pages.new_empty(max(nbytes // 2, 8))
+    args = C.EvictPagedArgs(k_pages.data_ptr(), v_pages.data_ptr(), kp, kg, vp, vg, key_weights.data_ptr(), table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1],
+                            table.shape[0], table.shape[1], pool, page, lengths.data_ptr(), None if rows is None else rows.data_ptr(), out.data_ptr(), S, G, hs, keep, first, recent,
+                            max_length, ws.data_ptr(), nbytes)
+    C.check(C.load().b200_evict_paged(ctypes.byref(args), _raw_stream(device)), "evict_paged")
+    return out
+
+
 def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,
                    v_cache: torch.Tensor, n_head: int, n_groups: int, head_size: int, rope_n_elem: int,
                    table_preselected: bool = False) -> torch.Tensor:
