@@ -325,7 +325,7 @@ int b200_attn_decode_shared_tune(int path);
  *              weights over the step's rows and its group's heads.
  *   max_rows, max_length   bounds of a sequence's rows and of its keys behind the step: they size the work; keys from max_length on are dropped
  *   cos, sin   (table_rows, rope_n_elem), row = position; table_preselected: row = row of qkv
- * head_size 64 or 128.  No page belongs to two sequences that bring rows into it.  The workspace needs no initial contents; two calls that run at the same time need one each. */
+ * head_size 64 or 128.  out on a 16-byte boundary.  No page belongs to two sequences that bring rows into it.  The workspace needs no initial contents; two calls that run at the same time need one each. */
 typedef struct b200_attn_paged_args {
   const void* qkv;
   const void* cos; const void* sin; int table_dtype, table_rows, table_preselected, rope_n_elem;
@@ -340,6 +340,9 @@ typedef struct b200_attn_paged_args {
 } b200_attn_paged_args;
 size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int n_groups, int head_size, int64_t max_rows, int64_t max_length, int key_weights);
 int b200_attn_paged(const b200_attn_paged_args* args, b200_stream_t stream);
+/* development / test knob: every sequence in the list of tiles (1), every one on the tensor memory (2; not with more than 128 heads a group), by size (0); returns the previous
+ * setting.  Workspaces are sized for the setting at the time. */
+int b200_attn_paged_tune(int path);
 
 /* Sequences of a paged cache cut down to `keep` keys each, every group by itself: the first `first` keys, the last `recent` and, of those between, the ones with the largest
  * key_weights (equal ones: the lower index; NaN counts as the largest) stay; they move to the front of the sequence's pages in order -- keys, values and weights; what lies behind

@@ -327,6 +327,7 @@ _SIGNATURES = {
     "b200_attn_decode_shared": (c_int, [ctypes.POINTER(AttnDecodeSharedArgs), c_void_p]),
     "b200_attn_paged_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]),
     "b200_attn_paged": (c_int, [ctypes.POINTER(AttnPagedArgs), c_void_p]),
+    "b200_attn_paged_tune": (c_int, [c_int]),
     "b200_evict_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int64]),
     "b200_evict_paged": (c_int, [ctypes.POINTER(EvictPagedArgs), c_void_p]),
     "b200_rope_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,

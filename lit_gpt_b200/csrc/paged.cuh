@@ -4,6 +4,13 @@
 
 namespace b200 {
 
+constexpr int kMaxTiles = 1 << 29;          // of a step
+
+struct PagedCut {                                           // what a CTA of paged_attn_tc05.cu goes on with that others began
+  int first, last;                                          // the CTAs that have segments of it; last -1: it begins with an item of its own
+  int count, row, gi;                                       // its queries, its first row, its group
+};
+
 struct PagedParams {
   const __nv_bfloat16* qkv;
   const void* cos; const void* sin;
@@ -23,6 +30,9 @@ struct PagedParams {
   int workers, sms;                                         // warps that share the tiles, at most
   float* acc; float2* ml;                                   // results of key ranges: slots of tile_rows queries
   int2* where;                                              // per item: the first worker that has tiles of it, and how many workers have
+  int list_max;                                             // sequences of more queries a group are left to the tensor memory (paged_attn_tc05.cu)
+  int tc_workers;                                           // CTAs that share their tiles, at most
+  float* tc_acc; float2* tc_ml; PagedCut* cuts;             // their results: two slots of 256 queries a CTA
   int* item_base;                                           // per sequence: its first item
   int ways;                                                 // warps that join a head's results
   float scale_log2;
@@ -51,5 +61,7 @@ __device__ __forceinline__ int page_at(const PagedParams& p, int table, int inde
   const int id = p.pages[(int64_t)table * p.pages_ld + index];
   return id >= 0 && id < p.pool ? id : -1;
 }
+
+cudaError_t launch_paged_tc05(const PagedParams& p, int head_size, cudaStream_t st);   // rows of sequences of more than list_max queries a group
 
 }  // namespace b200

@@ -13,6 +13,7 @@
 // goes through the queries that see it, S^T = K Q^T, the keys as rows: a key's sum stays with the lanes that hold its row.  No atomics: one order of additions.
 #include "attn_list.cuh"
 #include "paged.cuh"
+#include "tc05.cuh"
 
 namespace b200 {
 
@@ -20,7 +21,6 @@ using namespace list;
 
 namespace {
 
-constexpr int kMaxTiles = 1 << 29;          // of a step
 constexpr int kUnits = 3;                   // a warp's ring: units of 32 keys or 32 values
 
 __device__ __forceinline__ int64_t paged_pos(const PagedParams& p, int row) {
@@ -84,7 +84,9 @@ __device__ __forceinline__ int worker_of(int tile, const Split& s) {
 }
 __device__ __forceinline__ int first_tile(int w, const Split& s) { return w * s.each + min(w, s.more); }
 
-__device__ __forceinline__ int seq_items(const PagedParams& p, const PagedSeq& s) { return s.rows > 0 ? (s.rows * p.per + p.tile_rows - 1) / p.tile_rows : 0; }   // of a group
+__device__ __forceinline__ int seq_items(const PagedParams& p, const PagedSeq& s) {   // of a group
+  return s.rows > 0 && s.rows * p.per <= p.list_max ? (s.rows * p.per + p.tile_rows - 1) / p.tile_rows : 0;
+}
 __device__ __forceinline__ int seq_tiles(const PagedSeq& s) { return (s.n + kShTile - 1) / kShTile; }
 
 // Sequences are summed in runs of one per thread: sums[t] = tiles and items (of one group) of the sequences before run t, sums[THREADS] of all.
@@ -197,7 +199,7 @@ struct Walk {
         t.part = 0;
         if (++t.gi == p.n_groups) {
           t.gi = 0;
-          do t.seq = paged_seq(p, ++t.s); while (t.seq.n == 0);
+          do t.seq = paged_seq(p, ++t.s); while (seq_items(p, t.seq) == 0);
           t.tiles = seq_tiles(t.seq);
         }
       }
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   const int which = p.row_seq[row];
   PagedSeq s = {};
   if (which >= 0 && which < p.n_seqs) s = paged_seq(p, which);
-  const bool idle = row < s.first || row - s.first >= s.rows;
+  const bool idle = row < s.first || row - s.first >= s.rows || s.rows * p.per > p.list_max;   // (or the tensor memory's)
   griddep_wait();
   float top = -INFINITY, sum = 0.f, a[V] = {};
   const int gi = h / p.per, m = (row - s.first) * p.per + h - gi * p.per;
@@ -491,13 +493,23 @@ __global__ void __launch_bounds__(KwSmem<HS>::kWarps * 32) paged_weights_kernel(
 // ---- host ----
 struct PagedPlan {
   int nq, ctas, workers, ways;
+  bool list, tensor;               // which kernels there is work for
+  int list_max, tc_workers;
   int64_t items, slots, q;
   size_t bytes;
 };
 
+std::atomic<int> g_paged_path{0};
+constexpr int kListMax = 32;       // queries of a sequence and group that the list of tiles takes
+
 PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, int64_t max_rows, int64_t max_length, bool kw) {
   PagedPlan s;
-  const int64_t most = max_rows * per;
+  const int path = g_paged_path.load(std::memory_order_relaxed);
+  // chunks of one length only: all go to the tensor memory (some of them may turn out shorter, or not there)
+  s.list_max = path == 1 || per > 128 ? 0x3fffffff : path == 2 || (max_rows * per > kListMax && rows == (int64_t)n_seqs * max_rows) ? 0 : kListMax;
+  s.tensor = max_rows * per > s.list_max;
+  s.list = s.list_max > 0;
+  const int64_t most = max_rows * per < s.list_max ? max_rows * per : s.list_max;   // queries of an item
   s.nq = most <= 8 ? 1 : most <= 16 ? 2 : 4;
   s.items = (int64_t)n_groups * ((rows * per + 8 * s.nq - 1) / (8 * s.nq) + n_seqs);
   const int warps = hs == 64 ? (s.nq == 4 ? PgSmem<64, 4>::kWarps : PgSmem<64, 1>::kWarps) : (s.nq == 4 ? PgSmem<128, 4>::kWarps : PgSmem<128, 1>::kWarps);
@@ -505,10 +517,13 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   s.ctas = sm_count();
   if (s.ctas > tiles) s.ctas = (int)tiles;
   s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
-  s.slots = (s.items + s.workers) * 8 * s.nq;
+  s.slots = s.list ? (s.items + s.workers) * 8 * s.nq : 0;
+  const int64_t blocks = s.tensor ? (int64_t)n_groups * (rows / (256 / per) + n_seqs) * ((max_length + 127) / 128) : 0;
+  s.tc_workers = blocks < sm_count() ? (int)blocks : sm_count();
+  const int64_t tc_slots = (int64_t)s.tc_workers * 2 * 256;
   s.q = rows * per * n_groups * hs;
   s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * sizeof(int) +
-            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0);
+            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
   const int64_t results = 2 + (int64_t)s.workers / s.items;
   s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
   while (s.ways < 8 && results > 4 * s.ways && rows * n_groups * per * s.ways < 24 * sm_count()) s.ways *= 2;
@@ -532,11 +547,15 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t 
   const int64_t warps = (int64_t)p.rows * p.n_groups * (p.per + 2);
   cudaError_t e = launch(paged_append_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
-  e = s.nq == 4 ? launch_list<HS, 4>(p, s, st) : s.nq == 2 ? launch_list<HS, 2>(p, s, st) : launch_list<HS, 1>(p, s, st);
-  if (e != cudaSuccess) return e;
-  const int heads = 8 / s.ways;
-  e = launch(paged_join_kernel<HS>, dim3((unsigned)(p.rows * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
-  if (e != cudaSuccess || !p.kw) return e;
+  if (s.tensor && (e = launch_paged_tc05(p, HS, st)) != cudaSuccess) return e;
+  if (s.list) {
+    e = s.nq == 4 ? launch_list<HS, 4>(p, s, st) : s.nq == 2 ? launch_list<HS, 2>(p, s, st) : launch_list<HS, 1>(p, s, st);
+    if (e != cudaSuccess) return e;
+    const int heads = 8 / s.ways;
+    e = launch(paged_join_kernel<HS>, dim3((unsigned)(p.rows * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
+    if (e != cudaSuccess) return e;
+  }
+  if (!p.kw) return e;
   using C = KwSmem<HS>;
   static PerDeviceOnce once;
   if (once.need()) {
@@ -545,7 +564,7 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t 
     once.done();
   }
   PagedParams one = p;             // the queries of a sequence and group as one tile: the list is that of the key tiles
-  one.tile_rows = 0x3fffffff;
+  one.tile_rows = one.list_max = 0x3fffffff;
   return launch(paged_weights_kernel<HS>, dim3((unsigned)(4 * p.sms)), dim3(C::kWarps * 32), (size_t)C::kBytes, st, one);
 }
 
@@ -562,6 +581,8 @@ size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int
     return 0;
   return paged_plan(rows, n_seqs, n_groups, n_head / n_groups, head_size, max_rows, max_length, key_weights != 0).bytes;
 }
+
+int b200_attn_paged_tune(int path) { return g_paged_path.exchange(path == 1 || path == 2 ? path : 0); }
 
 int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a, "b200_attn_paged: null argument");
@@ -581,12 +602,13 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a->table_dtype == B200_F32 || a->table_dtype == B200_BF16, "b200_attn_paged: tables must be fp32 or bf16");
   const uintptr_t at = (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)a->workspace | (uintptr_t)a->seqs;
   const int64_t strides = a->k_page_stride | a->k_group_stride | a->v_page_stride | a->v_group_stride;
-  B200_CHECK_ARG((at & 15) == 0 && (strides & 7) == 0 && ((uintptr_t)a->out & 7) == 0 && ((uintptr_t)a->key_weights & 3) == 0,
-                 "b200_attn_paged: pages, workspace and the sequences' description must lie on 16-byte boundaries");
+  B200_CHECK_ARG((at & 15) == 0 && (strides & 7) == 0 && ((uintptr_t)a->out & 15) == 0 && ((uintptr_t)a->key_weights & 3) == 0,
+                 "b200_attn_paged: pages, result, workspace and the sequences' description must lie on 16-byte boundaries");
   const int per = a->n_head / a->n_groups;
   const PagedPlan s = paged_plan(a->rows, a->n_seqs, a->n_groups, per, a->head_size, a->max_rows, a->max_length, a->key_weights != nullptr);
   B200_CHECK_ARG(s.items * ((a->max_length + kShTile - 1) / kShTile) < kMaxTiles, "b200_attn_paged: too many keys in a step");
   B200_CHECK_ARG(a->workspace_bytes >= s.bytes, "b200_attn_paged: workspace too small");
+  if (s.tensor) B200_CHECK_WAITS("b200_attn_paged");
   PagedParams p = {};
   p.qkv = (const __nv_bfloat16*)a->qkv;
   p.cos = a->cos; p.sin = a->sin; p.table_bf16 = a->table_dtype == B200_BF16; p.table_rows = a->table_rows; p.table_presel = a->table_preselected; p.rope_n = a->rope_n_elem;
@@ -606,8 +628,12 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.q = (__nv_bfloat16*)a->workspace;
   p.acc = (float*)(p.q + s.q);
   p.ml = (float2*)(p.acc + s.slots * a->head_size);
-  p.where = (int2*)(p.ml + s.slots);
-  p.item_base = (int*)(p.where + s.items);
+  p.list_max = s.list_max; p.tc_workers = s.tc_workers;
+  p.tc_acc = (float*)(p.ml + s.slots);
+  p.tc_ml = (float2*)(p.tc_acc + (int64_t)s.tc_workers * 512 * a->head_size);
+  p.where = (int2*)(p.tc_ml + (int64_t)s.tc_workers * 512);
+  p.cuts = (PagedCut*)(p.where + s.items);
+  p.item_base = (int*)(p.cuts + s.tc_workers);
   p.lse = p.kw ? (float*)(p.item_base + a->n_seqs) : nullptr;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
   const cudaStream_t st = (cudaStream_t)stream;

@@ -1,0 +1,641 @@
+// Chunks of new tokens over a paged key-value cache on the 5th-generation tensor cores (paged_attn.cu has the step, and says which sequences come here).
+//
+// An item is a block of up to 256 queries of one sequence and group -- whole rows, every head of the group -- against the keys that its last row sees, in tiles of 128.  The key tiles of
+// all items are one list, cut evenly over the CTAs, one an SM: neither few rows over many keys nor chunks of unequal lengths leave SMs without work.  A CTA's part of an item is a segment.
+// The result of an item that is one CTA's is stored at once; else every segment leaves maxima, sums and unscaled outputs, and a second launch joins them.
+//   * warps 0-3 and 4-7: the softmax of the block's first and second 128 queries, one per thread.  S (128 columns of tensor memory) is read into registers, the
+//     probabilities go back over it as bf16, the left operand of P V, in two halves so that P V starts on the first (attn_tc05.cu says what was tried);
+//   * warps 8-11: when a row's maximum grew, they shrink its O in tensor memory while its exponentials are still being taken;
+//   * warp 12: one thread issues S = Q K^T and O += P V, 128 x 128 x 16 each, S of a tile's next step right behind its P V;
+//   * warp 13 brings the keys and the queries, warp 14 the values, two stages each, 128-byte-swizzled: a page, or what of it lies in the tile, is one TMA box; values of a tile that
+//     ends past the sequence's last key, or has no page somewhere, come row by row with cp.async, zeros where there is nothing.
+// A masked key has weight 0, and 0 times an infinite or NaN value is NaN: a value of the chunk that is not finite reaches the rows before its own, within its
+// tile of 128 keys and 128 queries.
+// Probabilities are rounded to bf16 as they multiply V; the running maximum is exact, so that the largest probability is 1 and loses nothing.  They are summed before the rounding: the
+// keys' weights are taken from these sums (of rounded ones a result's error against 64 bits is 0.1 to 0.4 % smaller, a weight's thousands of times larger).
+#include "attn_list.cuh"
+#include "attn_tmem.cuh"
+#include "paged.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kPtThreads = 480, kPtSegs = 16;
+
+template <int HS>
+struct PtTile {
+  static constexpr int kPanels = HS / 64;                  // 128-byte-wide panels of a tile of 128 rows
+  static constexpr int kBytes = kPanels * 128 * 128;       // one operand tile
+  static constexpr int kSmem = 6 * kBytes + 1024;          // Q0 Q1 | K x 2 | V x 2
+  static constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static constexpr uint32_t kS = 0, kO = 256;              // tensor-memory columns: S0 S1 (P over them) | O0 O1
+};
+
+__device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(group), "r"(page), "r"(bar) : "memory");
+}
+
+// ---- the list of key tiles ----
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {   // sum over i < n of (a i + b) / m, rounded down
+  int64_t s = 0;
+  while (n > 0) {
+    s += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return s;
+}
+struct Blocks {            // of a sequence
+  int rows_each, count;    // rows of a block; blocks of a group
+  int cached, rows, n;
+  __device__ __forceinline__ int tiles(int block) const { return (min(cached + min((block + 1) * rows_each, rows), n) + 127) >> 7; }
+  __device__ __forceinline__ int64_t before(int block) const {   // tiles of the blocks before it
+    // blocks whose last row is below n
+    const int whole = n - cached >= rows_each ? min(block, (n - cached) / rows_each) : 0, clear = min(whole, rows / rows_each);
+    int64_t s = floor_sum(clear, 128, rows_each, (int64_t)cached + rows_each + 127);
+    return s + (int64_t)(block - clear) * ((n + 127) >> 7);
+  }
+};
+__device__ __forceinline__ Blocks blocks_of(const PagedParams& p, const PagedSeq& s) {
+  Blocks b;
+  b.rows_each = 256 / p.per;
+  b.count = s.rows * p.per > p.list_max ? (s.rows + b.rows_each - 1) / b.rows_each : 0;
+  b.cached = s.cached; b.rows = s.rows; b.n = s.n;
+  return b;
+}
+
+struct Seg {
+  int q0, count;           // first query in the workspace's order, queries
+  int m0, first;           // its number within the sequence and group; the sequence's first row
+  int cached, n, table, gi;
+  int lo, hi, hi0;         // key tiles; those of the first 128 queries end at hi0
+  int slot;                // place of its results; -1: the item is done here
+};
+
+template <int HS>
+__global__ void __launch_bounds__(kPtThreads, 1)
+paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, unsigned* err) {
+  using C = PtTile<HS>;
+  extern __shared__ __align__(1024) uint8_t pt_smem[];
+  __shared__ __align__(8) uint64_t s_bars[27];
+  __shared__ float s_shrink[256];         // per query: what its O and sum shrink by in this step
+  __shared__ __align__(16) uint32_t s_bits[4][4];        // keys of a tile that have a page, of the last four tiles
+  __shared__ Seg s_seg[kPtSegs];
+  __shared__ int s_segs, s_more;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_sums[kPtThreads + 1], s_warp[kPtThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const uint32_t smem = (tc::smem_u32(pt_smem) + 1023u) & ~1023u;
+  const uint32_t sq_ = smem, sk_ = smem + 2 * C::kBytes, sv_ = smem + 4 * C::kBytes;
+  const uint32_t bars = tc::smem_u32(s_bars);
+  const uint32_t k_full = bars, v_full = bars + 16, k_empty = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_half = bars + 80, p_full = bars + 96,
+                 o_done = bars + 112, q_full = bars + 128, shrink = bars + 136, idle = bars + 200;   // shrink: one per softmax warp; idle: products that gave up
+
+  griddep_launch();
+  griddep_wait();
+  // ---- this CTA's part of the list ----
+  auto capped = [](int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); };
+  const int run = (p.n_seqs + kPtThreads - 1) / kPtThreads;
+  int here = 0;
+  for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
+    const Blocks b = blocks_of(p, paged_seq(p, i));
+    here = capped(here + (b.count ? b.before(b.count) : 0));
+  }
+  int inc = here;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc = capped((int64_t)inc + x);
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  if (tid == 0) {
+    tc::mbar_init(q_full, 1);
+    tc::mbar_init(idle, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(k_full + 8 * i, 1);
+      tc::mbar_init(v_full + 8 * i, 1);
+      tc::mbar_init(k_empty + 8 * i, 1);
+      tc::mbar_init(v_empty + 8 * i, 1);
+      tc::mbar_init(s_full + 8 * i, 1);
+      tc::mbar_init(p_half + 8 * i, 8);   // the softmax and the shrinking warps
+      tc::mbar_init(p_full + 8 * i, 4);
+      tc::mbar_init(o_done + 8 * i, 1);
+    }
+    for (int i = 0; i < 8; ++i) tc::mbar_init(shrink + 8 * i, 1);
+    tc::mbar_init_fence();
+  }
+  __syncthreads();
+  int before = inc - here;
+  for (int w = 0; w < warp; ++w) before = capped((int64_t)before + s_warp[w]);
+  s_sums[tid] = before;
+  if (tid == kPtThreads - 1) s_sums[kPtThreads] = capped((int64_t)before + here);
+  if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = s_tmem;
+  const int64_t all64 = (int64_t)s_sums[kPtThreads] * p.n_groups;
+  const int all = all64 < kMaxTiles ? (int)all64 : 0;      // (a description whose sequences overlap can hold more: then none is done)
+  const int workers = min(max(all / 2, min(all, p.sms)), p.tc_workers), w = blockIdx.x;
+  const int each = workers ? all / workers : 0, more = all - each * workers;
+  const int first = w * each + min(w, more), end = w < workers ? first + each + (w < more ? 1 : 0) : first;
+  auto worker_of = [&](int tile) {
+    const int wide = more * (each + 1);
+    return tile < wide ? tile / (each + 1) : more + (tile - wide) / each;
+  };
+
+  // where the list goes on, kept by the thread that lists the segments
+  int at_tile = first, at_s = 0, at_gi = 0, at_block = 0, at_lo = 0;
+  PagedSeq seq = {};
+  Blocks blk = {};
+  if (tid == 0 && first < end) {
+    int lo = 0, hi = kPtThreads;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if ((int64_t)s_sums[mid] * p.n_groups <= first) lo = mid; else hi = mid;
+    }
+    int rest = first - s_sums[lo] * p.n_groups;
+    for (at_s = lo * run;; ++at_s) {
+      seq = paged_seq(p, at_s);
+      blk = blocks_of(p, seq);
+      const int of_group = blk.count ? (int)blk.before(blk.count) : 0;
+      if (rest < of_group * p.n_groups) {
+        at_gi = rest / of_group;
+        rest -= at_gi * of_group;
+        int a = 0, b = blk.count;       // the block that holds it
+        while (b - a > 1) {
+          const int mid = (a + b) / 2;
+          if (blk.before(mid) <= rest) a = mid; else b = mid;
+        }
+        at_block = a;
+        at_lo = rest - (int)blk.before(a);
+        break;
+      }
+      rest -= of_group * p.n_groups;
+    }
+  }
+  if (tid == 0) {                       // for the launch that joins: the item that this CTA goes on with
+    PagedCut c = {};
+    c.last = -1;
+    if (first < end && at_lo > 0) {
+      const int m0 = at_block * blk.rows_each * p.per;
+      c.first = worker_of(first - at_lo);
+      c.last = worker_of(first - at_lo + blk.tiles(at_block) - 1);
+      c.count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
+      c.row = seq.first + at_block * blk.rows_each;
+      c.gi = at_gi;
+    }
+    p.cuts[w] = c;
+  }
+  bool ok = true;
+  // counted over all segments, so that every barrier's phase is known
+  int tiles_done = 0, segs_done = 0;                       // loads and products
+  uint32_t n[2] = {0u, 0u};                                // steps of either 128 queries
+
+  for (;;) {
+    if (tid == 0) {
+      int c = 0;
+      for (; c < kPtSegs && at_tile < end; ++c) {
+        const int tiles = blk.tiles(at_block), m0 = at_block * blk.rows_each * p.per, count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
+        Seg& g = s_seg[c];
+        g.q0 = (at_gi * p.rows + seq.first) * p.per + m0;
+        g.count = count;
+        g.m0 = m0;
+        g.first = seq.first;
+        g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at_gi;
+        g.lo = at_lo;
+        g.hi = min(tiles, at_lo + end - at_tile);
+        g.hi0 = min(g.hi, (min(seq.cached + (m0 + min(count, 128) - 1) / p.per + 1, seq.n) + 127) >> 7);
+        g.slot = g.lo == 0 && g.hi == tiles ? -1 : 2 * w + (g.lo == 0);   // (of a CTA's segments only the first begins, only the last ends within an item)
+        at_tile += g.hi - g.lo;
+        if (at_tile >= end) continue;
+        at_lo = 0;
+        if (++at_block == blk.count) {
+          at_block = 0;
+          if (++at_gi == p.n_groups) {
+            at_gi = 0;
+            do {
+              seq = paged_seq(p, ++at_s);
+              blk = blocks_of(p, seq);
+            } while (blk.count == 0);
+          }
+        }
+      }
+      s_segs = c;
+      s_more = at_tile < end;
+    }
+    __syncthreads();
+    const int segs = s_segs;
+
+    if (warp >= 13) {
+      // ================================ loads ================================
+      const bool keys = warp == 13;
+      const uint32_t dst = keys ? sk_ : sv_, full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
+      const CUtensorMap* const map = keys ? &map_k : &map_v;
+      const int parts = p.shift >= 7 ? 1 : 128 >> p.shift, part_rows = min(128, 1 << p.shift);
+      for (int c = 0; c < segs && ok; ++c) {
+        const Seg& g = s_seg[c];
+        const int lo = g.lo, hi = g.hi, total = g.n, table = g.table, gi = g.gi;
+        auto page_of = [&](int j) { return lane < parts ? page_at(p, table, ((j * 128) >> p.shift) + lane) : -1; };
+        int id = page_of(lo);
+        for (int j = lo; j < hi; ++j, ++tiles_done) {
+          const int s = tiles_done & 1;
+          const int next = j + 1 < hi ? page_of(j + 1) : -1;
+          ok = __all_sync(0xffffffffu, tc::mbar_wait(empty + 8 * s, ((uint32_t)(tiles_done >> 1) & 1u) ^ 1u));
+          if (!ok) break;
+          const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+          const bool whole = have == (1u << parts) - 1u;
+          if (keys && lane < 4) {       // word l: keys 32 l and on
+            uint32_t bits = 0u;
+            if (p.shift >= 5) bits = (have >> ((lane * 32) >> min(p.shift, 7))) & 1u ? 0xffffffffu : 0u;
+            else bits = ((have >> (2 * lane)) & 1u ? 0xffffu : 0u) | ((have >> (2 * lane + 1)) & 1u ? 0xffff0000u : 0u);
+            s_bits[tiles_done & 3][lane] = bits;
+          }
+          const int row = p.shift >= 7 ? (j * 128) & ((1 << p.shift) - 1) : 0;
+          if (keys || (whole && (j + 1) * 128 <= total)) {
+            __syncwarp();               // (the words are written before the barrier that hands them over is arrived on)
+            if (lane == 0) tc::mbar_expect_tx(full + 8 * s, (uint32_t)(__popc(have) * part_rows * HS * 2));
+            __syncwarp();
+            if (id >= 0) {
+#pragma unroll
+              for (int e = 0; e < C::kPanels; ++e)
+                load_page(dst + s * C::kBytes + e * 16384u + (uint32_t)(lane * part_rows) * 128u, map, e * 64, row, gi, id, full + 8 * s);
+            }
+          } else {
+            constexpr int CH = HS / 8, RP = 32 / CH;   // 16-byte pieces per row, rows per pass
+            const int cc = lane % CH;
+            const __nv_bfloat16* const base = p.v + (int64_t)gi * p.v_group + cc * 8;
+            const uint32_t to = dst + s * C::kBytes + (uint32_t)(cc >> 3) * 16384u;
+#pragma unroll 8
+            for (int i = 0; i < 128 / RP; ++i) {
+              const int r = i * RP + lane / CH, of = __shfl_sync(0xffffffffu, id, p.shift >= 7 ? 0 : r >> p.shift);
+              const bool in = of >= 0 && j * 128 + r < total;
+              cp16(to + (uint32_t)(r * 128 + (((cc & 7) ^ (r & 7)) << 4)), in ? base + (int64_t)of * p.v_page + (int64_t)((row + r) & ((1 << p.shift) - 1)) * HS : base, in);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            tc::fence_smem_async();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(full + 8 * s);
+          }
+          if (keys && j == lo) {        // the queries, once the segment before has done its last product with the ones there
+            if (tiles_done > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + 8 * (s ^ 1), (uint32_t)((tiles_done - 1) >> 1) & 1u));
+            if (!ok) break;
+            const int halves = g.count > 128 ? 2 : 1;
+            if (lane == 0) {
+              tc::mbar_expect_tx(q_full, halves * C::kBytes);
+              for (int h = 0; h < halves; ++h)
+#pragma unroll
+                for (int e = 0; e < C::kPanels; ++e) tc::tma_load_2d(sq_ + h * C::kBytes + e * 16384u, &map_q, e * 64, g.q0 + h * 128, q_full);
+            }
+            __syncwarp();
+          }
+          id = next;
+        }
+        ++segs_done;
+      }
+    } else if (warp == 12) {
+      // ================================ products ================================
+      if (tc::elect()) {
+        const uint32_t q_low = tc::desc_sw128_low(sq_), k_low = tc::desc_sw128_low(sk_), v_low = desc_v_low(sv_);
+        auto scores = [&](int t, int s) {                    // S of query tile t with the keys of stage s
+          const uint32_t q = q_low + t * (C::kBytes >> 4), k = k_low + s * (C::kBytes >> 4);
+#pragma unroll
+          for (int e = 0; e < HS / 16; ++e) {
+            const uint32_t off = ((uint32_t)(e >> 2) * 16384u + (uint32_t)(e & 3) * 32u) >> 4;
+            mma_ss(tmem + C::kS + t * 128, tc::desc_of(q + off, tc::kDescSw128High), tc::desc_of(k + off, tc::kDescSw128High), C::kIdescS, e != 0);
+          }
+          tc::commit(s_full + 8 * t);
+        };
+        for (int c = 0; c < segs && ok; ++c) {
+          const Seg& g = s_seg[c];
+          const int lo = g.lo, hi = g.hi, hi0 = g.hi0, hi1 = g.count > 128 ? hi : lo;
+          ok = tc::mbar_wait_here(q_full, (uint32_t)segs_done & 1u) && tc::mbar_wait_here(k_full + 8 * (tiles_done & 1), (uint32_t)(tiles_done >> 1) & 1u);
+          if (!ok) break;
+          tc::fence_after();
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (lo < (t ? hi1 : hi0)) scores(t, tiles_done & 1);
+          tc::commit(k_empty + 8 * (tiles_done & 1));
+          bool fresh[2] = {true, true};
+          for (int j = lo; j < hi; ++j, ++tiles_done) {
+            const int i = tiles_done, s = i & 1, s1 = s ^ 1;
+            const bool more_keys = j + 1 < hi;
+            ok = tc::mbar_wait_here(v_full + 8 * s, (uint32_t)(i >> 1) & 1u) && (!more_keys || tc::mbar_wait_here(k_full + 8 * s1, (uint32_t)((i + 1) >> 1) & 1u));
+            if (!ok) break;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int stop = t ? hi1 : hi0;
+              if (j < stop) {
+                const uint32_t dv = v_low + s * (C::kBytes >> 4);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  ok = ok && tc::mbar_wait_here((half ? p_full : p_half) + 8 * t, n[t] & 1u);
+                  if (!ok) break;
+                  tc::fence_after();
+#pragma unroll
+                  for (int e = 4 * half; e < 4 * half + 4; ++e)
+                    mma_ts(tmem + C::kO + t * HS, tmem + C::kS + t * 128 + e * 8, tc::desc_of(dv + 128 * e, tc::kDescSw128High), C::kIdescO, !fresh[t] || e != 0);
+                }
+                if (!ok) break;
+                fresh[t] = false;
+                tc::commit(o_done + 8 * t);
+                ++n[t];
+              }
+              if (more_keys && j + 1 < stop) scores(t, s1);
+            }
+            if (!ok) break;
+            tc::commit(v_empty + 8 * s);
+            if (more_keys) tc::commit(k_empty + 8 * s1);
+          }
+          ++segs_done;
+        }
+        if (!ok) {
+          tc::commit(idle);
+          tc::mbar_wait(idle, 0);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+    } else if (warp >= 8) {
+      // ================================ shrinking O ================================
+      const int v = warp - 8;
+      for (int c = 0; c < segs && ok; ++c) {
+        const Seg& g = s_seg[c];
+        const int lo = g.lo, hi = g.hi, hi0 = g.hi0, hi1 = g.count > 128 ? hi : lo;
+        for (int j = lo; j < hi && ok; ++j) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= (t ? hi1 : hi0)) continue;
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(shrink + 8 * (4 * t + v), n[t] & 1u));
+            if (!ok) break;
+            const float f = s_shrink[t * 128 + v * 32 + lane];
+            if (__any_sync(0xffffffffu, f != 1.0f)) {   // (S of this step is there, so P V of the last one is done; a segment's first step has f = 1)
+              tc::fence_after();
+              const uint32_t to = tmem + ((uint32_t)(v * 32) << 16) + C::kO + t * HS;
+#pragma unroll 1
+              for (int cc = 0; cc < HS; cc += 32) {
+                uint32_t o[32];
+                tc::ld32(o, to + cc);
+                tc::wait_ld(o);
+                uint32_t a[16], bb[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  a[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  bb[e] = __float_as_uint(__uint_as_float(o[16 + e]) * f);
+                }
+                st16(to + cc, a);
+                st16(to + cc + 16, bb);
+              }
+              wait_st();
+              tc::fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(p_half + 8 * t);
+            ++n[t];
+          }
+        }
+      }
+    } else {
+      // ================================ softmax: a query per thread ================================
+      const int t = warp >> 2;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + lanes + C::kS + t * 128, to = tmem + lanes + C::kO + t * HS;
+      const float sl = p.scale_log2;
+      int tiles_before = tiles_done;                       // of this batch's segments before the current one
+      for (int c = 0; c < segs && ok; ++c) {
+        const Seg& g = s_seg[c];
+        const int count = g.count, lo = g.lo, hi = t ? (count > 128 ? g.hi : lo) : g.hi0;
+        const int row = (g.m0 + tid) / p.per;              // of the sequence
+        const int lim = tid < count ? min(g.cached + row, g.n - 1) : -1;
+        const int w_lim = __reduce_min_sync(0xffffffffu, lim < 0 ? 0x7fffffff : lim);
+        float m = -INFINITY;
+        f2 l2[2] = {0ull, 0ull};
+        const uint32_t n0 = n[0];
+        for (int j = lo; j < hi; ++j, ++n[0]) {
+          ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * t, n[0] & 1u));
+          if (!ok) break;
+          tc::fence_after();
+          const int j0 = j * 128;
+          const uint4 bits = *reinterpret_cast<const uint4*>(s_bits[(tiles_before + j - lo) & 3]);
+          const bool holes = (bits.x & bits.y & bits.z & bits.w) != 0xffffffffu;
+          const bool masked = j0 + 127 > w_lim || holes;   // (queries past the segment's are computed and not stored)
+          auto mask = [&](uint32_t (&s)[32], int i) {
+            if (masked) {
+              const uint32_t there = i == 0 ? bits.x : i == 1 ? bits.y : i == 2 ? bits.z : bits.w;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int key = j0 + i * 32 + e;
+                if (key > lim || !((there >> e) & 1u)) s[e] = 0xff800000u;
+              }
+            }
+          };
+          auto most = [](const uint32_t (&s)[32], float mx) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            return mx;
+          };
+          uint32_t s0[32], s1[32];
+          float mx[4];
+          tc::ld32(s0, ts + 64);
+          tc::ld32(s1, ts + 96);
+          tc::wait_ld(s0);
+          tc::wait_ld(s1);
+          mask(s0, 2);
+          mask(s1, 3);
+          mx[2] = most(s0, -INFINITY);
+          mx[3] = most(s1, -INFINITY);
+          tc::ld32(s0, ts);
+          tc::ld32(s1, ts + 32);
+          tc::wait_ld(s0);
+          tc::wait_ld(s1);
+          mask(s0, 0);
+          mask(s1, 1);
+          mx[0] = most(s0, -INFINITY);
+          mx[1] = most(s1, -INFINITY);
+          const float nm = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          const float f = m == -INFINITY ? 1.0f : ex2((m - nm) * sl);   // nothing seen so far: O and the sum are zero
+          m = nm;
+          s_shrink[tid] = f;
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(shrink + 8 * warp);
+          const f2 ff = pk2(f, f);
+          l2[0] = fma2(l2[0], ff, 0ull);
+          l2[1] = fma2(l2[1], ff, 0ull);
+          const float org = m == -INFINITY ? 0.f : m * sl;   // queries with nothing visible yet: exp2(-inf) = 0
+          const f2 sl2 = pk2(sl, sl), org2 = pk2(-org, -org);
+          auto exps = [&](const uint32_t (&s)[32], int i) {
+            uint32_t q[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float a, b;
+              un2(fma2(pk2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl2, org2), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              q[e] = pack_bf16(a, b);
+              l2[e & 1] = add2(l2[e & 1], pk2(a, b));
+            }
+            st16(ts + i * 16, q);
+          };
+          auto hand_over = [&](uint32_t bar) {
+            wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(bar + 8 * t);
+          };
+          exps(s0, 0);
+          tc::ld32(s0, ts + 64);   // (P so far lies in columns 0 .. 31, at most 0 .. 63: scores 64 .. 127 are still there)
+          exps(s1, 1);
+          tc::wait_ld(s0);
+          tc::ld32(s1, ts + 96);
+          hand_over(p_half);
+          mask(s0, 2);
+          exps(s0, 2);
+          tc::wait_ld(s1);
+          mask(s1, 3);
+          exps(s1, 3);
+          hand_over(p_full);
+        }
+        tiles_before += g.hi - lo;
+        const bool any = n[0] != n0;
+        if (any && ok) {
+          ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * t, (n[0] - 1) & 1u));
+          tc::fence_after();
+        }
+        if (!ok) break;
+        if (t * 128 < count) {
+          float a, b, d, e;
+          un2(l2[0], a, b);
+          un2(l2[1], d, e);
+          const float l = (a + b) + (d + e);
+          const int slot = g.slot;
+          const int hh = g.m0 + tid - row * p.per;
+          if (slot < 0) {
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            __nv_bfloat16* const yr = p.out + ((int64_t)(g.first + row) * p.n_head + g.gi * p.per + hh) * HS;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HS; c0 += 32) {
+              uint32_t o[32], x[16];
+              tc::ld32(o, to + c0);
+              tc::wait_ld(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = any ? pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
+              if (tid < count) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(yr + c0 + 2 * i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+              }
+            }
+            if (p.lse && tid < count) p.lse[g.q0 + tid] = l > 0.f ? m * sl + log2f(l) : INFINITY;
+          } else {
+            float* const at = p.tc_acc + ((int64_t)slot * 256 + tid) * HS;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HS; c0 += 32) {
+              uint32_t o[32];
+              tc::ld32(o, to + c0);
+              tc::wait_ld(o);
+              if (tid < count) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) __stcg(reinterpret_cast<uint4*>(at + c0 + i), make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+              }
+            }
+            if (tid < count) __stcg(p.tc_ml + (int64_t)slot * 256 + tid, make_float2(m == -INFINITY ? m : m * sl, any ? l : 0.f));
+          }
+          tc::fence_before();
+        }
+      }
+      tiles_done = tiles_before;
+    }
+    ok = __syncthreads_and(ok);
+    if (!ok || !s_more) break;
+    __syncthreads();                                       // (everyone has read s_more)
+  }
+  if (!ok) {
+    // copies on their way: neither stage may be written once this CTA has left
+    if (warp >= 13) {
+      const uint32_t full = warp == 13 ? k_full : v_full;
+      for (int e = max(tiles_done - 2, 0); e < tiles_done; ++e) tc::mbar_wait(full + 8 * (e & 1), (uint32_t)(e >> 1) & 1u);
+      if (warp == 13 && segs_done > 0) tc::mbar_wait(q_full, (uint32_t)(segs_done - 1) & 1u);
+    }
+    *err = 1u;
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    __syncwarp();
+    tc::tmem_free<512>(tmem);
+  }
+}
+
+// An item that several CTAs had segments of: CTA (w, part) of this launch joins a share of its queries, for the w-th worker's beginning within it.  A query a warp.
+template <int HS>
+__global__ void __launch_bounds__(256) paged_tc05_join_kernel(const PagedParams p, int parts) {
+  constexpr int V = HS / 32;
+  griddep_launch();
+  griddep_wait();
+  const int w = blockIdx.x / parts, part = blockIdx.x - w * parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const PagedCut c = p.cuts[w];
+  if (c.last < 0) return;
+  const int shares = (c.last - c.first) * parts, share = (w - c.first - 1) * parts + part;
+  const int end = (int)((int64_t)c.count * (share + 1) / shares);
+  for (int m = (int)((int64_t)c.count * share / shares) + warp; m < end; m += 8) {
+    float top = -INFINITY, sum = 0.f, a[V] = {};
+    list::join_results<V>(0, 1, c.last - c.first + 1, lane, top, sum, a, [&](int i, const float2*& ml, const float*& acc) {
+      const int64_t at = (int64_t)(2 * (c.first + i) + (i == 0)) * 256 + m;
+      ml = p.tc_ml + at;
+      acc = p.tc_acc + at * HS;
+    });
+    const int row = m / p.per, hh = m - row * p.per;
+    list::store_result<HS>(p.out + ((int64_t)(c.row + row) * p.n_head + c.gi * p.per + hh) * HS, a, sum > 0.f ? 1.f / sum : 0.f, lane);
+    if (p.lse && lane == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
+  }
+}
+
+bool page_map(CUtensorMap* map, const void* base, int hs, int page, int groups, int pool, int64_t group, int64_t apart) {
+  const TensorMapEncodeFn enc = tensor_map_encoder();
+  if (!enc) return false;
+  // (a single group's, or a single page's, distance is not used, but has to be one)
+  if (group == 0) group = (int64_t)page * hs;
+  if (apart == 0) apart = (int64_t)page * hs;
+  const cuuint64_t dim[4] = {(cuuint64_t)hs, (cuuint64_t)page, (cuuint64_t)groups, (cuuint64_t)pool};
+  const cuuint64_t stride[3] = {(cuuint64_t)hs * 2, (cuuint64_t)group * 2, (cuuint64_t)apart * 2};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)(page < 128 ? page : 128), 1u, 1u};
+  const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HS>
+cudaError_t launch_hs(const PagedParams& p, cudaStream_t st) {
+  constexpr int smem = PtTile<HS>::kSmem;
+  static PerDeviceOnce once;
+  if (once.need()) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_tc05_kernel<HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    once.done();
+  }
+  alignas(64) CUtensorMap mq, mk, mv;
+  const int page = 1 << p.shift;
+  if (!tensor_map_2d(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.q, (int64_t)p.n_groups * p.rows * p.per, HS, HS * 2, 128) ||
+      !page_map(&mk, p.k, HS, page, p.n_groups, p.pool, p.k_group, p.k_page) || !page_map(&mv, p.v, HS, page, p.n_groups, p.pool, p.v_group, p.v_page))
+    return cudaErrorInvalidValue;
+  unsigned* const err = wait_error_word();
+  if (!err) return cudaErrorMemoryAllocation;
+  cudaError_t e = launch(paged_tc05_kernel<HS>, dim3((unsigned)p.tc_workers), dim3(kPtThreads), (size_t)smem, st, p, mq, mk, mv, err);
+  if (e != cudaSuccess) return e;
+  constexpr int parts = 8;
+  return launch(paged_tc05_join_kernel<HS>, dim3((unsigned)(p.tc_workers * parts)), dim3(256), 0, st, p, parts);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_tc05(const PagedParams& p, int head_size, cudaStream_t st) { return head_size == 128 ? launch_hs<128>(p, st) : launch_hs<64>(p, st); }
+
+}  // namespace b200

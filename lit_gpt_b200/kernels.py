@@ -1050,6 +1050,12 @@ def attn_decode_shared_tune(path: int = 0) -> int:
     return int(C.load().b200_attn_decode_shared_tune(int(path)))
 
 
+def attn_paged_tune(path: int = 0) -> int:
+    """Test knob: every sequence of ``attn_paged`` in the list of tiles (1), every one on the tensor memory (2), by size (0); returns the previous setting."""
+    _paged_workspace_bytes.cache_clear()
+    return int(C.load().b200_attn_paged_tune(int(path)))
+
+
 def attn_decode_tune(force_scalar: bool = False) -> bool:
     """Test knob: route grouped-query shapes through the scalar decode-attention kernel; returns the previous setting."""
     return bool(C.load().b200_attn_decode_tune(int(force_scalar)))

@@ -47,10 +47,10 @@ def step(d, rounded=0.0):
     A result's bound: weights that are off by a factor 1 +- off make 2 off sum_j w_j |v_j|, with off the sum of
       * the error of a score: hs + 2 roundings of 2^-24 of sum |q k| / sqrt(hs), in the exponent and once more in the row's maximum;
       * the rounding of the exponent's argument, 2^-23 of the largest score's distance (at most 2 max |s|), and of ex2, 2^-22;
-      * a probability in two bf16 numbers: 2^-16 -- or in one: `rounded`, 2^-8;
+      * a probability in two bf16 numbers: 2^-16 -- or in one: `rounded`, 2^-8 (of that the sums know nothing: once and not twice);
       * sums of n products in fp32: (n + 64) 2^-24, n keys at most.
-    A key's weight: the same without the probability's rounding (the sums of exponentials are of unrounded ones, unless `rounded`), of the step's part, and a rounding of 2^-24 for
-    every one of its additions."""
+    A key's weight: the same without the probability's rounding (the sums of exponentials are of unrounded ones), of the step's part, and a rounding of 2^-24 for every one of its
+    additions."""
     G, per, hs, page = d["groups"], d["per"], d["hs"], d["k"].shape[2]
     n = d["qkv"].shape[0]
     heads = d["qkv"].view(n, G, per + 2, hs)
@@ -96,9 +96,9 @@ def step(d, rounded=0.0):
             out[first + r] = w @ vs
             size = (q.abs() @ ks.abs().transpose(1, 2)).amax() / math.sqrt(hs)
             off = 2 * (hs + 2) * 2 ** -24 * size + 2 ** -23 * 2 * score.abs().amax() + 2 ** -22 + (ks.shape[1] + 64) * 2 ** -24
-            slack[first + r] = 2 * (off + max(rounded, 2 ** -16)) * (w @ vs.abs())
+            slack[first + r] = (2 * off + max(rounded, 2 ** -15)) * (w @ vs.abs())
             got[:, seen] += w.sum(1)
-            err[:, seen] += (2 * off + rounded) * w.sum(1)
+            err[:, seen] += 2 * off * w.sum(1)
         if kw is not None:
             before = kw[ids, :, os_].T
             kw[ids, :, os_] = (before + got).T

@@ -11,8 +11,31 @@ from paged_oracle import F64, make
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(params=["list", "tensor memory", "by size"])
+def path(request):
+    return request.param
+
+
 @pytest.fixture
-def K():
+def K(path):
+    """The kernels with every sequence in the list of tiles, on the tensor memory, or where its size puts it."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from lit_gpt_b200 import kernels
+
+    before = kernels.attn_paged_tune({"list": 1, "tensor memory": 2, "by size": 0}[path])
+    yield kernels
+    kernels.attn_paged_tune(before)
+
+
+@pytest.fixture
+def formula(path):
+    """The step in 64 bits; on the tensor memory probabilities are rounded to bf16."""
+    return lambda d: oracle.step(d, 0.0 if path == "list" else 2 ** -8)
+
+
+@pytest.fixture
+def E():
     if not torch.cuda.is_available():
         pytest.skip("needs a CUDA device")
     from lit_gpt_b200 import kernels
@@ -60,56 +83,56 @@ MIXED = [(1, 40), (5, 0), (0, 7), (17, 33), (1, 0), (40, 129), (2, 300)]
 @pytest.mark.parametrize("groups,per", [(1, 1), (3, 1), (2, 4), (1, 7), (2, 16), (1, 20)])
 @pytest.mark.parametrize("page", [16, 32, 64, 256])
 @pytest.mark.parametrize("steps", [SINGLES, MIXED, [(70, 0)], [(33, 90), (64, 0)]], ids=["singles", "mixed", "prompt", "chunks"])
-def test_formula(K, hs, groups, per, page, steps):
+def test_formula(K, formula, hs, groups, per, page, steps):
     d = make(steps, groups, per, hs, page, seed=page + per)
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 65, 127, 128, 129, 200, 257])
-def test_chunk_lengths(K, rows):
+def test_chunk_lengths(K, formula, rows):
     d = make([(rows, rows * 3 % 50)], 2, 4, 128, 64, seed=rows)
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
 @pytest.mark.parametrize("steps", [[(1, 5000)], [(1, 3), (1, 4097), (1, 900)], [(1, 17 * i) for i in range(70)], [(130, 1500)]])
 @pytest.mark.parametrize("per,hs", [(4, 128), (1, 64)])
-def test_long(K, steps, per, hs):
+def test_long(K, formula, steps, per, hs):
     d = make(steps, 2, per, hs, 64, seed=3)
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
-def test_many_sequences(K):
+def test_many_sequences(K, formula):
     """More sequences than a CTA has threads."""
     d = make([(1 if i % 3 else 0, i % 50) for i in range(1500)], 1, 2, 64, 16, seed=4)
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
 @pytest.mark.parametrize("table", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rope", [0, 2, 16, 32, 64])
-def test_rotated_part(K, table, rope):
+def test_rotated_part(K, formula, table, rope):
     d = make([(1, 9), (20, 13)], 2, 2, 64, 16, rope=rope, table=table, seed=rope)
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
-def test_without_weights(K):
+def test_without_weights(K, formula):
     d = make(MIXED, 2, 2, 128, 32, weights=False)
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
-def test_positions_apart_from_places(K):
+def test_positions_apart_from_places(K, formula):
     """A cache that was cut down: rows are rotated at their positions, which are not their places in the cache; positions in 64 bits; tables gathered before the call."""
     d = make([(1, 9), (20, 13)], 2, 2, 64, 16, seed=9)
     d["cos"], d["sin"] = (torch.cat([t] * 9) for t in (d["cos"], d["sin"]))
     d["row_pos"] = (d["row_pos"].long() * 7 + 3) % len(d["cos"])
-    want = oracle.step(d)
+    want = formula(d)
     check(call(K, d), want)
     d["cos"], d["sin"] = d["cos"][d["row_pos"]], d["sin"][d["row_pos"]]
     check(call(K, d, table_preselected=True), want)
 
 
-def test_leading_dimensions_and_strided_rows(K):
+def test_leading_dimensions_and_strided_rows(K, formula):
     d = make([(1, 9), (21, 13)], 2, 2, 64, 16, seed=9)
-    want = oracle.step(d)
+    want = formula(d)
     t = on_gpu(d)
     wide = torch.zeros(2, 11, 600, device="cuda", dtype=torch.bfloat16)
     wide[..., :512] = t["qkv"].view(2, 11, 512)
@@ -123,9 +146,9 @@ def test_leading_dimensions_and_strided_rows(K):
 
 
 @pytest.mark.parametrize("layout", ["keys beside values", "group by group", "apart"])
-def test_page_layouts(K, layout):
+def test_page_layouts(K, formula, layout):
     d = make(MIXED, 3, 2, 128, 32, seed=12)
-    want = oracle.step(d)
+    want = formula(d)
     t = on_gpu(d)
     P, G, page, hs = d["k"].shape
     if layout == "keys beside values":
@@ -143,7 +166,7 @@ def test_page_layouts(K, layout):
     check((out, k.contiguous(), v.contiguous(), t["kw"]), want)
 
 
-def test_missing_pages(K):
+def test_missing_pages(K, formula):
     """No page: no keys there, new ones are dropped; a row without any key has a result of zero.  Page numbers outside the pool are none."""
     d = make([(1, 100), (1, 100), (30, 50), (3, 20), (1, 16)], 2, 4, 128, 16, seed=5)
     at = d["seqs"][:, 3].tolist()
@@ -153,22 +176,22 @@ def test_missing_pages(K):
     d["pages"][at[2], 0] = 2 ** 31 - 1
     d["pages"][at[3]] = -1                      # all of them
     d["pages"][at[4], 0] = -1
-    want = oracle.step(d)
+    want = formula(d)
     got = call(K, d)
     check(got, want)
     assert not got[0][32:35].any()
 
 
-def test_bounds_drop_keys(K):
+def test_bounds_drop_keys(K, formula):
     """Keys from max_length on are dropped; the rows behind see those before."""
     d = make([(1, 60), (20, 50)], 2, 2, 64, 16, seed=6)
     d["max_length"] = 60
-    check(call(K, d), oracle.step(d))
+    check(call(K, d), formula(d))
 
 
-def test_rows_of_no_sequence(K):
+def test_rows_of_no_sequence(K, formula):
     d = make([(1, 20), (6, 10), (1, 5)], 2, 2, 64, 16, seed=7)
-    want = [t.clone() if torch.is_tensor(t) else t for t in oracle.step({**d, "seqs": torch.cat((d["seqs"][:2], d["seqs"][2:] * torch.tensor([1, 0, 1, 1], dtype=torch.int32)))})]
+    want = [t.clone() if torch.is_tensor(t) else t for t in formula({**d, "seqs": torch.cat((d["seqs"][:2], d["seqs"][2:] * torch.tensor([1, 0, 1, 1], dtype=torch.int32)))})]
     d["row_seq"][7] = -1
     bad = d["seqs"].clone()
     bad[2] = torch.tensor([0, 0, 5, 0])
@@ -179,10 +202,10 @@ def test_rows_of_no_sequence(K):
 
 
 @pytest.mark.parametrize("seq", [(0, 500, 3, 0), (-1, 2, 3, 0), (7, 1, -2, 0), (7, 1, 3, 99), (7, 1, 3, -1), (2 ** 31 - 1, 2 ** 31 - 1, 5, 0), (7, 1, 2 ** 31 - 1, 0)])
-def test_sequences_that_do_not_fit_take_no_part(K, seq):
+def test_sequences_that_do_not_fit_take_no_part(K, formula, seq):
     """A description that reaches beyond the rows or the page table: nothing of it is read or written."""
     d = make([(1, 20), (6, 10), (1, 5)], 2, 2, 64, 16, seed=7)
-    want = oracle.step({**d, "seqs": torch.cat((d["seqs"][:2], torch.zeros(1, 4, dtype=torch.int32)))})
+    want = formula({**d, "seqs": torch.cat((d["seqs"][:2], torch.zeros(1, 4, dtype=torch.int32)))})
     d["seqs"][2] = torch.tensor(seq, dtype=torch.int32)
     got = call(K, d)
     if seq[2] < 2 ** 31 - 1:
@@ -191,24 +214,24 @@ def test_sequences_that_do_not_fit_take_no_part(K, seq):
         assert torch.isfinite(got[0].float()).all() and same(got[1].cpu(), want[2])
 
 
-def test_what_lies_behind_the_last_key_is_not_read(K):
+def test_what_lies_behind_the_last_key_is_not_read(K, formula):
     for steps in (SINGLES, [(20, 33), (1, 70)]):
         d = make(steps, 2, 4, 128, 64, seed=8)
-        want = oracle.step(d)
+        want = formula(d)
         used = torch.zeros(d["k"].shape[0], d["k"].shape[2], dtype=torch.bool)
         for first, rows, cached, at in d["seqs"].tolist():
             for j in range(cached + rows):
                 used[d["pages"][at, j // 64], j % 64] = True
         for x, bad in ((d["k"], float("nan")), (d["v"], float("inf"))):
             x.permute(0, 2, 1, 3)[~used] = bad
-        want = (want[0], want[1], *oracle.step(d)[2:4], want[4], want[5])
+        want = (want[0], want[1], *formula(d)[2:4], want[4], want[5])
         check(call(K, d), want)
 
 
-def test_offsets_past_32_bits(K):
+def test_offsets_past_32_bits(K, formula):
     """Pages more than 2^31 numbers into the pool."""
     d = make([(1, 40), (20, 70)], 1, 2, 128, 256, seed=10)
-    want = oracle.step(d)
+    want = formula(d)
     t = on_gpu(d)
     P, far = len(d["k"]), 2 ** 31 // (256 * 128) + 5
     k, v = (torch.empty(far + P, 1, 256, 128, device="cuda", dtype=torch.bfloat16) for _ in range(2))
@@ -219,7 +242,7 @@ def test_offsets_past_32_bits(K):
     check((out, k[far:], v[far:], kw[far:]), want)
 
 
-def test_same_bits_every_time(K):
+def test_same_bits_every_time(K, formula):
     d = make([(1, 700), (64, 300), (1, 90), (200, 0)], 2, 4, 128, 64, seed=11)
     first = call(K, d)
     for _ in range(3):
@@ -227,10 +250,10 @@ def test_same_bits_every_time(K):
             assert same(a, b)
 
 
-def test_two_streams(K):
+def test_two_streams(K, formula):
     """Two calls at a time share nothing."""
     ds = [make([(1, 300 + 50 * i), (1 + 30 * i, 20)], 2, 4, 128, 32, seed=20 + i) for i in range(2)]
-    wants = [oracle.step(d) for d in ds]
+    wants = [formula(d) for d in ds]
     ts = [on_gpu(d) for d in ds]
     streams = [torch.cuda.Stream() for _ in ds]
     torch.cuda.synchronize()
@@ -244,7 +267,7 @@ def test_two_streams(K):
         check((out, t["k"], t["v"], t["kw"]), want)
 
 
-def test_captured_steps(K):
+def test_captured_steps(K, formula):
     """A captured step follows its description, page table and positions as they change; two captured steps at a time have a workspace each."""
     first = make([(1, 40), (1, 100), (1, 9)], 2, 4, 128, 16, seed=30)
     second = make([(1, 250), (0, 3), (1, 77)], 2, 4, 128, 16, seed=31, spare=2)
@@ -260,7 +283,7 @@ def test_captured_steps(K):
     second["row_pos"] = torch.tensor([250, 0, 77], dtype=torch.int32)
     second["seqs"] = torch.tensor([[0, 1, 250, second["seqs"][0, 3]], [1, 0, 3, second["seqs"][1, 3]], [2, 1, 77, second["seqs"][2, 3]]], dtype=torch.int32)
     first["cos"], first["sin"] = second["cos"], second["sin"]
-    want = [oracle.step(d) for d in (first, second)]
+    want = [formula(d) for d in (first, second)]
     t = on_gpu(first)
     launch(K, t)
     torch.cuda.synchronize()
@@ -287,10 +310,10 @@ def cache(lengths, groups, hs, page, seed=0, spare=2):
     return d, [int(at) for at in d["seqs"][:, 3]]
 
 
-def evict_check(K, d, lengths, keep, rows, **kw):
+def evict_check(E, d, lengths, keep, rows, **kw):
     want = oracle.evict(d["k"], d["v"], d["kw"], d["pages"], lengths, keep, rows=rows, **kw)
     t = on_gpu(d)
-    left = K.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths, dtype=torch.int32, device="cuda"), keep, max_length=max(max(lengths), 1),
+    left = E.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths, dtype=torch.int32, device="cuda"), keep, max_length=max(max(lengths), 1),
                          rows=None if rows is None else torch.tensor(rows, dtype=torch.int32, device="cuda"), **kw)
     assert same(t["k"].cpu(), want[0]) and same(t["v"].cpu(), want[1]) and same(t["kw"].cpu(), want[2]) and left.tolist() == want[3]
 
@@ -298,19 +321,19 @@ def evict_check(K, d, lengths, keep, rows, **kw):
 @pytest.mark.parametrize("hs,groups,page", [(64, 1, 16), (128, 3, 64), (64, 2, 256), (128, 2, 32)])
 @pytest.mark.parametrize("lengths,keep,first,recent", [([2], 1, 0, 0), ([100], 99, 0, 0), ([100], 1, 1, 0), ([100, 7, 300], 50, 4, 16), ([1025, 2, 1024, 1023], 64, 0, 64),
                                                        ([1500], 1400, 64, 300), ([513, 40, 41], 40, 0, 7), ([2100, 2049], 700, 1, 0), ([33], 32, 16, 16)])
-def test_evict(K, hs, groups, page, lengths, keep, first, recent):
+def test_evict(E, hs, groups, page, lengths, keep, first, recent):
     d, rows = cache(lengths, groups, hs, page, seed=keep)
-    evict_check(K, d, lengths, keep, rows, first=first, recent=recent)
+    evict_check(E, d, lengths, keep, rows, first=first, recent=recent)
 
 
-def test_evict_long(K):
+def test_evict_long(E):
     lengths = [9000, 5000]
     d, rows = cache(lengths, 1, 64, 16, seed=3)
-    evict_check(K, d, lengths, 4097, rows, first=5, recent=1000)
+    evict_check(E, d, lengths, 4097, rows, first=5, recent=1000)
 
 
 @pytest.mark.parametrize("kind", ["zeros", "few values", "signs", "infinite", "not a number", "neighbours", "tiny"])
-def test_evict_ties_and_odd_weights(K, kind):
+def test_evict_ties_and_odd_weights(E, kind):
     """Equal weights: the lower index; the two zeros are equal; NaN above all."""
     lengths = [700, 300]
     d, rows = cache(lengths, 2, 64, 32, seed=17)
@@ -321,10 +344,10 @@ def test_evict_ties_and_odd_weights(K, kind):
                "infinite": lambda: pick(inf, -inf, 0.0, 3.0), "not a number": lambda: pick(nan, inf, 1.0, -nan, -2.0),
                "neighbours": lambda: 1.0 + torch.randint(0, 600, d["kw"].shape, generator=r) * 2 ** -23, "tiny": lambda: torch.randint(0, 300, d["kw"].shape, generator=r) * 2.0 ** -149}[kind]().float()
     for keep in (299, 128, 57):
-        evict_check(K, d, lengths, keep, rows, first=3, recent=20)
+        evict_check(E, d, lengths, keep, rows, first=3, recent=20)
 
 
-def test_evict_leaves_what_it_must(K):
+def test_evict_leaves_what_it_must(E):
     """Sequences that are short, longer than max_length, or with an entry that is no page, stay as they are; as do those that are in no row of the page table."""
     lengths = [300, 40, 300, 500, 90]
     d, rows = cache(lengths, 2, 64, 16, seed=18)
@@ -332,22 +355,22 @@ def test_evict_leaves_what_it_must(K):
     want = oracle.evict(d["k"], d["v"], d["kw"], d["pages"], lengths, 64, rows=rows)
     k, v, kw, _ = oracle.evict(d["k"], d["v"], d["kw"], d["pages"], lengths[:3] + lengths[4:], 64, rows=rows[:3] + rows[4:])
     t = on_gpu(d)
-    left = K.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths + [300], dtype=torch.int32, device="cuda"), 64, max_length=400,
+    left = E.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths + [300], dtype=torch.int32, device="cuda"), 64, max_length=400,
                          rows=torch.tensor(rows + [77], dtype=torch.int32, device="cuda"))
     assert left.tolist() == [64, 40, 300, 500, 64, 300] and want[3] == [64, 40, 300, 64, 64]
     assert same(t["k"].cpu(), k) and same(t["v"].cpu(), v) and same(t["kw"].cpu(), kw)
     before = [x.clone() for x in (t["k"], t["v"], t["kw"])]
-    left = K.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths, dtype=torch.int32, device="cuda"), 512, max_length=500)
+    left = E.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths, dtype=torch.int32, device="cuda"), 512, max_length=500)
     assert left.tolist() == lengths and all(same(a, b) for a, b in zip(before, (t["k"], t["v"], t["kw"])))
 
 
-def test_evict_captured_and_on_another_stream(K):
+def test_evict_captured_and_on_another_stream(E):
     lengths = [200, 150]
     d, rows = cache(lengths, 2, 64, 16, seed=19)
     want = oracle.evict(d["k"], d["v"], d["kw"], d["pages"], lengths, 100, first=2, recent=9, rows=rows)
     t = on_gpu(d)
     n, r = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, rows))
-    run = lambda: K.evict_paged(t["k"], t["v"], t["kw"], t["pages"], n, 100, first=2, recent=9, max_length=200, rows=r)
+    run = lambda: E.evict_paged(t["k"], t["v"], t["kw"], t["pages"], n, 100, first=2, recent=9, max_length=200, rows=r)
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
@@ -364,7 +387,7 @@ def test_evict_captured_and_on_another_stream(K):
 
 
 # ---- the operators together ------------------------------------------------------------------------------------------------------------
-def test_a_sequence_of_steps(K):
+def test_a_sequence_of_steps(K, formula):
     """A prompt in portions, tokens one by one, an eviction, more tokens: as a server uses them.  The choice of an eviction is made from the kernels' own weights."""
     G, per, hs, page = 2, 4, 64, 16
     r = random.Random(3)
@@ -393,7 +416,7 @@ def test_a_sequence_of_steps(K):
         i32 = lambda x: torch.tensor(x, dtype=torch.int32)
         d = dict(base, **pool, qkv=torch.randn(len(row_seq), (per + 2) * G * hs, generator=g).bfloat16(), row_seq=i32(row_seq), row_pos=i32(row_pos), seqs=i32(seqs), pages=pages,
                  max_rows=max(step), max_length=192)
-        want = oracle.step(d)
+        want = formula(d)
         t = dict(on_gpu(d), **gpu)
         out = launch(K, t)
         check((out, gpu["k"], gpu["v"], gpu["kw"]), want)

@@ -25,7 +25,7 @@ def test_attention_arguments_are_checked():
                      (dict(pool=0), "no pages"), (dict(max_pages=0), "no pages"), (dict(pages_ld=7), "page table"), (dict(max_length=129), "129 keys"), (dict(max_length=0), "0 keys"),
                      (dict(qkv=None), "null"), (dict(row_seq=None), "null"), (dict(pages=None), "null"), (dict(v_pages=None), "null"), (dict(out=None), "null"), (dict(rope_n_elem=66), "rope"),
                      (dict(rope_n_elem=3), "rope"), (dict(cos=None), "tables"), (dict(table_rows=0), "tables"), (dict(table_preselected=1, table_rows=4), "preselected"),
-                     (dict(table_dtype=C.F16), "tables"), (dict(k_pages=FAKE + 2), "16-byte"), (dict(v_group_stride=1028), "16-byte"), (dict(seqs=FAKE + 4), "16-byte"),
+                     (dict(table_dtype=C.F16), "tables"), (dict(k_pages=FAKE + 2), "16-byte"), (dict(v_group_stride=1028), "16-byte"), (dict(seqs=FAKE + 4), "16-byte"), (dict(out=FAKE + 8), "16-byte"),
                      (dict(key_weights=FAKE + 2), "16-byte"), (dict(workspace_bytes=16), "workspace")):
         refused(call(**kw), text)
     refused(lib.b200_attn_paged(None, None), "null")
