@@ -31,6 +31,7 @@ struct PagedParams {
   float* acc; float2* ml;                                   // results of key ranges: slots of tile_rows queries
   int2* where;                                              // per item: the first worker that has tiles of it, and how many workers have
   int list_max;                                             // sequences of more queries a group are left to the tensor memory (paged_attn_tc05.cu)
+  int tc_rows;                                              // rows of a block of theirs: 256 queries at most
   int tc_workers;                                           // CTAs that share their tiles, at most
   float* tc_acc; float2* tc_ml; PagedCut* cuts;             // their results: two slots of 256 queries a CTA
   int* item_base;                                           // per sequence: its first item

@@ -28,11 +28,85 @@ __device__ __forceinline__ int64_t paged_pos(const PagedParams& p, int row) {
   return at < 0 ? 0 : (at >= p.table_rows ? p.table_rows - 1 : at);
 }
 
-// ---- the queries and the new keys turned, the new rows stored: a head a warp ----
+// ---- the queries and the new keys turned, the new rows stored ----
+// A CTA takes a row, or some heads of one: HS / 16 threads a head, each with sixteen numbers of it, eight and the eight that they turn with (or, where nothing is turned, any sixteen), whose cosines
+// and sines it keeps from head to head.  Needs rows of heads and tables for accesses of 16 bytes, and halves of the rotation that are multiples of eight numbers (or no rotation).
+template <int HS>
+__global__ void __launch_bounds__(256) paged_append_wide_kernel(const PagedParams p) {
+  constexpr int TH = HS / 16, HEADS = 256 / TH;    // threads of a head; heads at once
+  griddep_wait();     // (before the launch of what follows: the kernels behind read the step's description and the older keys ahead of their own wait)
+  griddep_launch();
+  const int row = blockIdx.x, heads = p.n_groups * (p.per + 2), n = p.rope_n, half = n >> 1;
+  const int piece = threadIdx.x % TH;
+  // numbers a .. a + 7 and b .. b + 7: pairs of the rotation first, then what it leaves
+  const int turning = half >> 3, a = piece < turning ? piece * 8 : n + (piece - turning) * 16, b = piece < turning ? a + half : a + 8;
+  const __nv_bfloat16* const x = p.qkv + (int64_t)row * heads * HS;
+  int i = blockIdx.y * HEADS + threadIdx.x / TH;
+  uint4 ra = {}, rb = {};
+  auto load = [&](int h) {
+    if (h < heads) {
+      ra = *reinterpret_cast<const uint4*>(x + (int64_t)h * HS + a);
+      rb = *reinterpret_cast<const uint4*>(x + (int64_t)h * HS + b);
+    }
+  };
+  load(i);
+  const int which = p.row_seq[row];
+  float ca[8], sa[8], cb[8], sb[8];
+  if (piece < turning) {
+    const int64_t at = paged_pos(p, row) * n;
+    auto get = [&](const void* t, int d, float (&f)[8]) {
+      if (p.table_bf16) load8(reinterpret_cast<const __nv_bfloat16*>(t) + at + d, f);
+      else load8(reinterpret_cast<const float*>(t) + at + d, f);
+    };
+    get(p.cos, a, ca);
+    get(p.sin, a, sa);
+    get(p.cos, b, cb);
+    get(p.sin, b, sb);
+  }
+  PagedSeq s = {};
+  if (which >= 0 && which < p.n_seqs) s = paged_seq(p, which);
+  const int mine = row - s.first, key = s.cached + mine;
+  const bool none = mine < 0 || mine >= s.rows;    // a row of no sequence
+  const int id = none || key >= s.n ? -1 : page_at(p, s.table, key >> p.shift), in = key & ((1 << p.shift) - 1);   // (no room behind max_length)
+  for (; i < heads; i += gridDim.y * HEADS) {
+    const uint4 ua = ra, ub = rb;
+    load(i + gridDim.y * HEADS);
+    const int gi = i / (p.per + 2), h = i - gi * (p.per + 2);
+    if (none) {
+      if (h < p.per) {
+        __nv_bfloat16* const to = p.out + ((int64_t)row * p.n_head + gi * p.per + h) * HS;
+        *reinterpret_cast<uint4*>(to + a) = *reinterpret_cast<uint4*>(to + b) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      continue;
+    }
+    if (h >= p.per && id < 0) continue;
+    __nv_bfloat16* const to = h < p.per    ? p.q + (((int64_t)gi * p.rows + row) * p.per + h) * HS
+                              : h == p.per ? p.k + (int64_t)id * p.k_page + (int64_t)gi * p.k_group + (int64_t)in * HS
+                                           : p.v + (int64_t)id * p.v_page + (int64_t)gi * p.v_group + (int64_t)in * HS;
+    uint4 wa = ua, wb = ub;
+    if (piece < turning && h <= p.per) {
+      const uint32_t xa[4] = {ua.x, ua.y, ua.z, ua.w}, xb[4] = {ub.x, ub.y, ub.z, ub.w};
+      uint32_t ya[4], yb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float al = bf16lo(xa[j]), ah = bf16hi(xa[j]), bl = bf16lo(xb[j]), bh = bf16hi(xb[j]);
+        ya[j] = pack_bf16(turned(al, bl, true, ca[2 * j], sa[2 * j], p.table_bf16), turned(ah, bh, true, ca[2 * j + 1], sa[2 * j + 1], p.table_bf16));
+        yb[j] = pack_bf16(turned(bl, al, false, cb[2 * j], sb[2 * j], p.table_bf16), turned(bh, ah, false, cb[2 * j + 1], sb[2 * j + 1], p.table_bf16));
+      }
+      wa = make_uint4(ya[0], ya[1], ya[2], ya[3]);
+      wb = make_uint4(yb[0], yb[1], yb[2], yb[3]);
+    }
+    *reinterpret_cast<uint4*>(to + a) = wa;
+    *reinterpret_cast<uint4*>(to + b) = wb;
+    if (p.kw && h == p.per && piece == 0) p.kw[(((int64_t)id * p.n_groups + gi) << p.shift) + in] = 0.f;
+  }
+}
+
+// Any rotation and alignment: a head a warp.
 template <int HS>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) {
   constexpr int V = HS / 32;
-  griddep_wait();     // (before the launch of what follows: the kernels behind read the step's description and the older keys ahead of their own wait)
+  griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31, heads = p.n_groups * (p.per + 2);
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -506,7 +580,8 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   PagedPlan s;
   const int path = g_paged_path.load(std::memory_order_relaxed);
   // chunks of one length only: all go to the tensor memory (some of them may turn out shorter, or not there)
-  s.list_max = path == 1 || per > 128 ? 0x3fffffff : path == 2 || (max_rows * per > kListMax && rows == (int64_t)n_seqs * max_rows) ? 0 : kListMax;
+  const int singles = per <= 8 ? 8 : per <= 16 ? 16 : kListMax;   // beside chunks the list takes single tokens, in items as small as they are
+  s.list_max = path == 1 || per > 128 ? 0x3fffffff : path == 2 ? 0 : max_rows * per <= kListMax ? kListMax : rows == (int64_t)n_seqs * max_rows ? 0 : singles;
   s.tensor = max_rows * per > s.list_max;
   s.list = s.list_max > 0;
   const int64_t most = max_rows * per < s.list_max ? max_rows * per : s.list_max;   // queries of an item
@@ -545,7 +620,13 @@ cudaError_t launch_list(const PagedParams& p, const PagedPlan& s, cudaStream_t s
 template <int HS>
 cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
   const int64_t warps = (int64_t)p.rows * p.n_groups * (p.per + 2);
-  cudaError_t e = launch(paged_append_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
+  cudaError_t e;
+  if (p.wide) {                    // few rows: a row's heads on several CTAs, as many as are at once
+    const int turns = (p.n_groups * (p.per + 2) * (HS / 16) + 255) / 256, ctas = p.sms * 4 / p.rows;
+    e = launch(paged_append_wide_kernel<HS>, dim3((unsigned)p.rows, (unsigned)(ctas < 1 ? 1 : ctas < turns ? ctas : turns)), dim3(256), 0, st, p);
+  } else {
+    e = launch(paged_append_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
+  }
   if (e != cudaSuccess) return e;
   if (s.tensor && (e = launch_paged_tc05(p, HS, st)) != cudaSuccess) return e;
   if (s.list) {
@@ -612,8 +693,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   PagedParams p = {};
   p.qkv = (const __nv_bfloat16*)a->qkv;
   p.cos = a->cos; p.sin = a->sin; p.table_bf16 = a->table_dtype == B200_BF16; p.table_rows = a->table_rows; p.table_presel = a->table_preselected; p.rope_n = a->rope_n_elem;
-  const int n = a->rope_n_elem, part = a->head_size / 32;
-  p.wide = ((uintptr_t)a->qkv & 15) == 0 && n % (2 * part) == 0 && (a->table_dtype == B200_BF16 || (((uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0);
+  p.wide = (((uintptr_t)a->qkv | (uintptr_t)a->cos | (uintptr_t)a->sin) & 15) == 0 && a->rope_n_elem % 16 == 0;
   p.row_pos = a->row_pos; p.pos64 = a->pos_is_int64; p.row_seq = a->row_seq;
   p.seqs = (const int4*)a->seqs; p.n_seqs = a->n_seqs;
   p.pages = a->pages; p.pages_ld = a->pages_ld; p.page_rows = a->table_seqs; p.max_pages = a->max_pages; p.pool = a->pool;
@@ -628,7 +708,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.q = (__nv_bfloat16*)a->workspace;
   p.acc = (float*)(p.q + s.q);
   p.ml = (float2*)(p.acc + s.slots * a->head_size);
-  p.list_max = s.list_max; p.tc_workers = s.tc_workers;
+  p.list_max = s.list_max; p.tc_workers = s.tc_workers; p.tc_rows = per <= 256 ? 256 / per : 1;
   p.tc_acc = (float*)(p.ml + s.slots);
   p.tc_ml = (float2*)(p.tc_acc + (int64_t)s.tc_workers * 512 * a->head_size);
   p.where = (int2*)(p.tc_ml + (int64_t)s.tc_workers * 512);

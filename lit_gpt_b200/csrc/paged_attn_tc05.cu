@@ -13,7 +13,6 @@
 // tile of 128 keys and 128 queries.
 // Probabilities are rounded to bf16 as they multiply V; the running maximum is exact, so that the largest probability is 1 and loses nothing.  They are summed before the rounding: the
 // keys' weights are taken from these sums (of rounded ones a result's error against 64 bits is 0.1 to 0.4 % smaller, a weight's thousands of times larger).
-#include "attn_list.cuh"
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
@@ -39,39 +38,29 @@ __device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap* map, 
 }
 
 // ---- the list of key tiles ----
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {   // sum over i < n of (a i + b) / m, rounded down
-  int64_t s = 0;
-  while (n > 0) {
-    s += n * (n - 1) / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const int64_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const int64_t t = m;
-    m = a;
-    a = t;
-  }
-  return s;
-}
+// The list is cut by steps: an item counts as its key tiles and kLead more, the time that its queries' way in and its results' way out take (4 to 5 us where a tile takes 2.2).
+constexpr int kLead = 2;
 struct Blocks {            // of a sequence
-  int rows_each, count;    // rows of a block; blocks of a group
-  int cached, rows, n;
-  __device__ __forceinline__ int tiles(int block) const { return (min(cached + min((block + 1) * rows_each, rows), n) + 127) >> 7; }
-  __device__ __forceinline__ int64_t before(int block) const {   // tiles of the blocks before it
-    // blocks whose last row is below n
-    const int whole = n - cached >= rows_each ? min(block, (n - cached) / rows_each) : 0, clear = min(whole, rows / rows_each);
-    int64_t s = floor_sum(clear, 128, rows_each, (int64_t)cached + rows_each + 127);
-    return s + (int64_t)(block - clear) * ((n + 127) >> 7);
-  }
+  int count;               // of a group; none where the sequence is the list's
+  int rows_each, cached, rows, n;
+  __device__ __forceinline__ int steps(int block) const { return block < count ? kLead + ((min(cached + min((block + 1) * rows_each, rows), n) + 127) >> 7) : 0; }
 };
 __device__ __forceinline__ Blocks blocks_of(const PagedParams& p, const PagedSeq& s) {
   Blocks b;
-  b.rows_each = 256 / p.per;
+  b.rows_each = p.tc_rows;
   b.count = s.rows * p.per > p.list_max ? (s.rows + b.rows_each - 1) / b.rows_each : 0;
   b.cached = s.cached; b.rows = s.rows; b.n = s.n;
   return b;
+}
+__device__ __forceinline__ int capped(int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); }
+// The steps of a group, by a whole warp.
+__device__ __forceinline__ int steps_of(const Blocks& b, int lane) {
+  int64_t s = 0;
+  for (int i = lane; i < b.count; i += 32) s += b.steps(i);
+  int c = capped(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) c = capped((int64_t)c + __shfl_xor_sync(0xffffffffu, c, o));
+  return c;
 }
 
 struct Seg {
@@ -80,6 +69,11 @@ struct Seg {
   int cached, n, table, gi;
   int lo, hi, hi0;         // key tiles; those of the first 128 queries end at hi0
   int slot;                // place of its results; -1: the item is done here
+};
+
+struct ListAt {            // where the list of segments goes on
+  int tile, end;
+  int s, gi, block, lo;    // sequence, group, block, first key tile
 };
 
 template <int HS>
@@ -91,6 +85,8 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   __shared__ float s_shrink[256];         // per query: what its O and sum shrink by in this step
   __shared__ __align__(16) uint32_t s_bits[4][4];        // keys of a tile that have a page, of the last four tiles
   __shared__ Seg s_seg[kPtSegs];
+  __shared__ ListAt s_at;
+  __shared__ PagedCut s_cut;
   __shared__ int s_segs, s_more;
   __shared__ uint32_t s_tmem;
   __shared__ int s_sums[kPtThreads + 1], s_warp[kPtThreads / 32];
@@ -102,14 +98,27 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
                  o_done = bars + 112, q_full = bars + 128, shrink = bars + 136, idle = bars + 200;   // shrink: one per softmax warp; idle: products that gave up
 
   griddep_launch();
-  griddep_wait();
-  // ---- this CTA's part of the list ----
-  auto capped = [](int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); };
+  // ---- this CTA's part of the list: from the step's description, which was there before the append kernel ----
   const int run = (p.n_seqs + kPtThreads - 1) / kPtThreads;
   int here = 0;
-  for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
-    const Blocks b = blocks_of(p, paged_seq(p, i));
-    here = capped(here + (b.count ? b.before(b.count) : 0));
+  for (int k = 0; k < run; ++k) {
+    const int i = tid * run + k;
+    Blocks mine = {};
+    if (i < p.n_seqs) mine = blocks_of(p, paged_seq(p, i));
+    if (mine.count <= 16) {
+      for (int e = 0; e < mine.count; ++e) here = capped((int64_t)here + mine.steps(e));
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, mine.count > 16); left; left &= left - 1) {   // long ones: by all lanes, one after the other
+      const int of = __ffs(left) - 1;
+      Blocks b;
+      b.rows_each = p.tc_rows;
+      b.count = __shfl_sync(0xffffffffu, mine.count, of);
+      b.cached = __shfl_sync(0xffffffffu, mine.cached, of);
+      b.rows = __shfl_sync(0xffffffffu, mine.rows, of);
+      b.n = __shfl_sync(0xffffffffu, mine.n, of);
+      const int sum = steps_of(b, lane);
+      if (lane == of) here = capped((int64_t)here + sum);
+    }
   }
   int inc = here;
 #pragma unroll
@@ -139,102 +148,122 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   for (int w = 0; w < warp; ++w) before = capped((int64_t)before + s_warp[w]);
   s_sums[tid] = before;
   if (tid == kPtThreads - 1) s_sums[kPtThreads] = capped((int64_t)before + here);
-  if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
-  tc::fence_before();
   __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = s_tmem;
   const int64_t all64 = (int64_t)s_sums[kPtThreads] * p.n_groups;
   const int all = all64 < kMaxTiles ? (int)all64 : 0;      // (a description whose sequences overlap can hold more: then none is done)
-  const int workers = min(max(all / 2, min(all, p.sms)), p.tc_workers), w = blockIdx.x;
-  const int each = workers ? all / workers : 0, more = all - each * workers;
-  const int first = w * each + min(w, more), end = w < workers ? first + each + (w < more ? 1 : 0) : first;
-  auto worker_of = [&](int tile) {
-    const int wide = more * (each + 1);
-    return tile < wide ? tile / (each + 1) : more + (tile - wide) / each;
-  };
-
-  // where the list goes on, kept by the thread that lists the segments
-  int at_tile = first, at_s = 0, at_gi = 0, at_block = 0, at_lo = 0;
-  PagedSeq seq = {};
-  Blocks blk = {};
-  if (tid == 0 && first < end) {
-    int lo = 0, hi = kPtThreads;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if ((int64_t)s_sums[mid] * p.n_groups <= first) lo = mid; else hi = mid;
-    }
-    int rest = first - s_sums[lo] * p.n_groups;
-    for (at_s = lo * run;; ++at_s) {
-      seq = paged_seq(p, at_s);
-      blk = blocks_of(p, seq);
-      const int of_group = blk.count ? (int)blk.before(blk.count) : 0;
-      if (rest < of_group * p.n_groups) {
-        at_gi = rest / of_group;
-        rest -= at_gi * of_group;
-        int a = 0, b = blk.count;       // the block that holds it
-        while (b - a > 1) {
-          const int mid = (a + b) / 2;
-          if (blk.before(mid) <= rest) a = mid; else b = mid;
-        }
-        at_block = a;
-        at_lo = rest - (int)blk.before(a);
-        break;
-      }
-      rest -= of_group * p.n_groups;
-    }
-  }
-  if (tid == 0) {                       // for the launch that joins: the item that this CTA goes on with
-    PagedCut c = {};
+  if (warp == 0) {
+    const int workers = min(max(all / 2, min(all, p.sms)), p.tc_workers), w = blockIdx.x;
+    const int each = workers ? all / workers : 0, more = all - each * workers;
+    const int first = w * each + min(w, more), end = w < workers ? first + each + (w < more ? 1 : 0) : first;
+    ListAt at = {};
+    at.tile = first;
+    at.end = end;
+    PagedCut c = {};                    // for the launch that joins: the item that this CTA goes on with
     c.last = -1;
-    if (first < end && at_lo > 0) {
-      const int m0 = at_block * blk.rows_each * p.per;
-      c.first = worker_of(first - at_lo);
-      c.last = worker_of(first - at_lo + blk.tiles(at_block) - 1);
-      c.count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
-      c.row = seq.first + at_block * blk.rows_each;
-      c.gi = at_gi;
+    if (first < end) {
+      int lo = 0, hi = kPtThreads;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if ((int64_t)s_sums[mid] * p.n_groups <= first) lo = mid; else hi = mid;
+      }
+      int rest = first - s_sums[lo] * p.n_groups, of_group;
+      PagedSeq seq;
+      Blocks blk;
+      for (at.s = lo * run;; ++at.s) {
+        seq = paged_seq(p, at.s);
+        blk = blocks_of(p, seq);
+        of_group = steps_of(blk, lane);
+        if (rest < of_group * p.n_groups) break;
+        rest -= of_group * p.n_groups;
+      }
+      at.gi = rest / of_group;
+      rest -= at.gi * of_group;
+      for (int b0 = 0;; b0 += 32) {     // the block that holds it
+        const int t = blk.steps(b0 + lane);
+        int sum = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += x; }
+        const unsigned behind = __ballot_sync(0xffffffffu, sum > rest);
+        if (behind) {
+          const int of = __ffs(behind) - 1;
+          at.block = b0 + of;
+          at.lo = rest - __shfl_sync(0xffffffffu, sum - t, of);
+          break;
+        }
+        rest -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (at.lo > kLead) {
+        const int m0 = at.block * blk.rows_each * p.per, wide = more * (each + 1);
+        auto worker_of = [&](int tile) { return tile < wide ? tile / (each + 1) : more + (tile - wide) / each; };
+        c.first = worker_of(first - at.lo + kLead);   // (whose part holds the first key tile)
+        c.last = worker_of(first - at.lo + blk.steps(at.block) - 1);
+        c.count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
+        c.row = seq.first + at.block * blk.rows_each;
+        c.gi = at.gi;
+      }
     }
-    p.cuts[w] = c;
+    if (lane == 0) {
+      s_cut = c;
+      s_at = at;
+    }
   }
-  bool ok = true;
+  uint32_t tmem = 0;
+  bool ok = true, began = false;
   // counted over all segments, so that every barrier's phase is known
   int tiles_done = 0, segs_done = 0;                       // loads and products
   uint32_t n[2] = {0u, 0u};                                // steps of either 128 queries
 
   for (;;) {
     if (tid == 0) {
+      ListAt at = s_at;
       int c = 0;
-      for (; c < kPtSegs && at_tile < end; ++c) {
-        const int tiles = blk.tiles(at_block), m0 = at_block * blk.rows_each * p.per, count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
-        Seg& g = s_seg[c];
-        g.q0 = (at_gi * p.rows + seq.first) * p.per + m0;
-        g.count = count;
-        g.m0 = m0;
-        g.first = seq.first;
-        g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at_gi;
-        g.lo = at_lo;
-        g.hi = min(tiles, at_lo + end - at_tile);
-        g.hi0 = min(g.hi, (min(seq.cached + (m0 + min(count, 128) - 1) / p.per + 1, seq.n) + 127) >> 7);
-        g.slot = g.lo == 0 && g.hi == tiles ? -1 : 2 * w + (g.lo == 0);   // (of a CTA's segments only the first begins, only the last ends within an item)
-        at_tile += g.hi - g.lo;
-        if (at_tile >= end) continue;
-        at_lo = 0;
-        if (++at_block == blk.count) {
-          at_block = 0;
-          if (++at_gi == p.n_groups) {
-            at_gi = 0;
-            do {
-              seq = paged_seq(p, ++at_s);
-              blk = blocks_of(p, seq);
-            } while (blk.count == 0);
+      if (at.tile < at.end) {
+        PagedSeq seq = paged_seq(p, at.s);
+        Blocks blk = blocks_of(p, seq);
+        for (; c < kPtSegs && at.tile < at.end; c += s_seg[c].hi > s_seg[c].lo) {   // (a part without a key tile is none)
+          const int steps = blk.steps(at.block), m0 = at.block * blk.rows_each * p.per, count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
+          Seg& g = s_seg[c];
+          g.q0 = (at.gi * p.rows + seq.first) * p.per + m0;
+          g.count = count;
+          g.m0 = m0;
+          g.first = seq.first;
+          g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at.gi;
+          const int stop = min(steps, at.lo + at.end - at.tile);
+          g.lo = max(at.lo - kLead, 0);
+          g.hi = max(stop - kLead, 0);
+          g.hi0 = min(g.hi, (min(seq.cached + (m0 + min(count, 128) - 1) / p.per + 1, seq.n) + 127) >> 7);
+          g.slot = g.lo == 0 && stop == steps ? -1 : 2 * (int)blockIdx.x + (g.lo == 0);   // (of a CTA's segments only the first begins, only the last ends within an item)
+          at.tile += stop - at.lo;
+          if (at.tile >= at.end) continue;
+          at.lo = 0;
+          if (++at.block == blk.count) {
+            at.block = 0;
+            if (++at.gi == p.n_groups) {
+              at.gi = 0;
+              do {
+                seq = paged_seq(p, ++at.s);
+                blk = blocks_of(p, seq);
+              } while (blk.count == 0);
+            }
           }
         }
       }
+      s_at = at;                                           // (in shared memory: the softmax has no registers for it)
       s_segs = c;
-      s_more = at_tile < end;
+      s_more = at.tile < at.end;
+    }
+    if (!began) {                                          // (tensor memory is taken behind the wait only)
+      griddep_wait();
+      if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+      if (tid == 0) p.cuts[blockIdx.x] = s_cut;
+      tc::fence_before();
     }
     __syncthreads();
+    if (!began) {
+      tc::fence_after();
+      tmem = s_tmem;
+      began = true;
+    }
     const int segs = s_segs;
 
     if (warp >= 13) {
@@ -520,7 +549,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           const int hh = g.m0 + tid - row * p.per;
           if (slot < 0) {
             const float inv = l > 0.f ? 1.0f / l : 0.f;
-            __nv_bfloat16* const yr = p.out + ((int64_t)(g.first + row) * p.n_head + g.gi * p.per + hh) * HS;
+            const int64_t y_at = tid < count ? ((int64_t)(g.first + row) * p.n_head + g.gi * p.per + hh) * HS : -1;
 #pragma unroll 1
             for (int c0 = 0; c0 < HS; c0 += 32) {
               uint32_t o[32], x[16];
@@ -528,14 +557,31 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
               tc::wait_ld(o);
 #pragma unroll
               for (int i = 0; i < 16; ++i) x[i] = any ? pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
-              if (tid < count) {
+              // Four neighbouring lanes have 64 bytes of four rows, and swap so that each store has 64 bytes of eight rows and not sixteen of 32: piece i of lane l becomes piece l of the
+              // row of lane i (the four stores of 16 bytes at one address a lane took 2.2 us a segment).
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(yr + c0 + 2 * i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+              for (int d = 1; d < 4; d <<= 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if (i & d) continue;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const bool high = lane & d;
+                    const uint32_t give = high ? x[4 * i + e] : x[4 * (i + d) + e];
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
+                    if (high) x[4 * i + e] = got; else x[4 * (i + d) + e] = got;
+                  }
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int64_t to_row = __shfl_sync(0xffffffffu, y_at, (lane & ~3) + i);
+                if (to_row >= 0) *reinterpret_cast<uint4*>(p.out + to_row + c0 + (lane & 3) * 8) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
               }
             }
             if (p.lse && tid < count) p.lse[g.q0 + tid] = l > 0.f ? m * sl + log2f(l) : INFINITY;
           } else {
-            float* const at = p.tc_acc + ((int64_t)slot * 256 + tid) * HS;
+            float* const at = p.tc_acc + (int64_t)slot * 256 * HS + tid * 4;   // four numbers of every query side by side: a warp's stores are whole lines (a query's all together: 4 us a segment)
 #pragma unroll 1
             for (int c0 = 0; c0 < HS; c0 += 32) {
               uint32_t o[32];
@@ -543,7 +589,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
               tc::wait_ld(o);
               if (tid < count) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) __stcg(reinterpret_cast<uint4*>(at + c0 + i), make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                for (int i = 0; i < 32; i += 4) __stcg(reinterpret_cast<uint4*>(at + (int64_t)(c0 + i) * 256), make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
               }
             }
             if (tid < count) __stcg(p.tc_ml + (int64_t)slot * 256 + tid, make_float2(m == -INFINITY ? m : m * sl, any ? l : 0.f));
@@ -574,27 +620,64 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   }
 }
 
-// An item that several CTAs had segments of: CTA (w, part) of this launch joins a share of its queries, for the w-th worker's beginning within it.  A query a warp.
+// An item that several CTAs had segments of: CTA (w, part) of this launch joins a share of its queries, 32 at a time, for the w-th worker's beginning within it.  A query a lane, HS / 8
+// numbers a warp.
 template <int HS>
 __global__ void __launch_bounds__(256) paged_tc05_join_kernel(const PagedParams p, int parts) {
-  constexpr int V = HS / 32;
+  constexpr int V = HS / 8;
   griddep_launch();
   griddep_wait();
   const int w = blockIdx.x / parts, part = blockIdx.x - w * parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PagedCut c = p.cuts[w];
   if (c.last < 0) return;
   const int shares = (c.last - c.first) * parts, share = (w - c.first - 1) * parts + part;
-  const int end = (int)((int64_t)c.count * (share + 1) / shares);
-  for (int m = (int)((int64_t)c.count * share / shares) + warp; m < end; m += 8) {
+  for (int m0 = share * 32; m0 < c.count; m0 += shares * 32) {
+    const int m = m0 + lane;
     float top = -INFINITY, sum = 0.f, a[V] = {};
-    list::join_results<V>(0, 1, c.last - c.first + 1, lane, top, sum, a, [&](int i, const float2*& ml, const float*& acc) {
-      const int64_t at = (int64_t)(2 * (c.first + i) + (i == 0)) * 256 + m;
-      ml = p.tc_ml + at;
-      acc = p.tc_acc + at * HS;
-    });
+    for (int i0 = c.first; i0 <= c.last; i0 += 2) {
+      float2 e[2];
+      float4 v[2][V / 4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        e[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) v[u][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + u <= c.last && m < c.count) {
+          const int64_t slot = 2 * (i0 + u) + (i0 + u == c.first);
+          e[u] = __ldcg(p.tc_ml + slot * 256 + m);
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) v[u][j] = __ldcg(reinterpret_cast<const float4*>(p.tc_acc + slot * 256 * HS + (int64_t)(warp * V + 4 * j) * 256 + m * 4));
+        }
+      }
+      const float now = fmaxf(top, fmaxf(e[0].x, e[1].x)), org = now == -INFINITY ? 0.f : now, shrink = ex2(top - org);
+      top = now;
+      sum *= shrink;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] *= shrink;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float f = ex2(e[u].x - org);
+        sum += e[u].y * f;
+        if (e[u].y != 0.f) {            // (a range that saw nothing has no result)
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) {
+            a[4 * j] += v[u][j].x * f;
+            a[4 * j + 1] += v[u][j].y * f;
+            a[4 * j + 2] += v[u][j].z * f;
+            a[4 * j + 3] += v[u][j].w * f;
+          }
+        }
+      }
+    }
+    if (m >= c.count) continue;
     const int row = m / p.per, hh = m - row * p.per;
-    list::store_result<HS>(p.out + ((int64_t)(c.row + row) * p.n_head + c.gi * p.per + hh) * HS, a, sum > 0.f ? 1.f / sum : 0.f, lane);
-    if (p.lse && lane == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    __nv_bfloat16* const to = p.out + ((int64_t)(c.row + row) * p.n_head + c.gi * p.per + hh) * HS + warp * V;
+#pragma unroll
+    for (int j = 0; j < V; j += 8)
+      *reinterpret_cast<uint4*>(to + j) = make_uint4(pack_bf16(a[j] * inv, a[j + 1] * inv), pack_bf16(a[j + 2] * inv, a[j + 3] * inv), pack_bf16(a[j + 4] * inv, a[j + 5] * inv),
+                                                     pack_bf16(a[j + 6] * inv, a[j + 7] * inv));
+    if (p.lse && warp == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
   }
 }
 
