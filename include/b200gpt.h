@@ -316,7 +316,8 @@ int b200_attn_decode_shared_tune(int path);
  *   qkv        (rows, (n_head + 2 n_groups) * head_size) bf16, interleaved per group as in b200_attn_decode
  *   row_pos    position of every row, its row of the tables (clamped); apart from the keys' places, since a cache may hold fewer keys than a sequence has positions
  *   row_seq    int32, the sequence of every row; a row of none (-1, or outside its sequence's rows) takes no part, its result is zero
- *   seqs       int32 (n_seqs, 4) on a 16-byte boundary: first row, rows, keys in the cache before the step, row of the page table.  Sequences of no rows take no part.
+ *   seqs       int32 (n_seqs, 4) on a 16-byte boundary: first row, rows, keys in the cache before the step, row of the page table.  Sequences of no rows, of more
+ *              than max_rows, or that reach beyond rows or table_seqs take no part.
  *   pages      int32 (table_seqs, max_pages), rows pages_ld apart: entry i of a sequence's row is the page of its keys [i * page, (i + 1) * page).  Where the entry is no page (outside
  *              0 .. pool - 1) there are no keys: new ones are dropped, the rest take no part.  A row that sees no key has a result of zero.
  *   k_pages, v_pages   (pool, n_groups, page, head_size) bf16, rows head_size apart, pages and groups at the given distances (elements, multiples of 8); page 16, 32, 64, 128 or 256.
@@ -340,8 +341,8 @@ typedef struct b200_attn_paged_args {
 } b200_attn_paged_args;
 size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int n_groups, int head_size, int64_t max_rows, int64_t max_length, int key_weights);
 int b200_attn_paged(const b200_attn_paged_args* args, b200_stream_t stream);
-/* development / test knob: every sequence in the list of tiles (1), every one on the tensor memory (2; not with more than 128 heads a group), by size (0); returns the previous
- * setting.  Workspaces are sized for the setting at the time. */
+/* development / test knob: every sequence in the list of tiles (1), every one on the tensor memory (2; not with more than 128 heads a group), the list without
+ * keeping its scores (3), by size (0); returns the previous setting.  Workspaces are sized for the setting at the time. */
 int b200_attn_paged_tune(int path);
 
 /* Sequences of a paged cache cut down to `keep` keys each, every group by itself: the first `first` keys, the last `recent` and, of those between, the ones with the largest

@@ -92,9 +92,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8 x 8 matri
 }
 
 // 8 N queries, from row q0 of `q` on, and a tile of keys: S^T = K Q^T and O^T += V^T P^T, keys and dimensions as the rows of the products, so that few queries cost few of them.  seen(key,
-// t, c): whether query 8 t + 2 tq + c sees that key of the tile.  `vb` of the values is what `values` gives, which waits for them.
-template <int HS, int NQ, int N, typename Seen, typename Values>
-__device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, int q0, uint32_t kb, float scale_log2, int lane, Seen seen, Values values) {
+// t, c): whether query 8 t + 2 tq + c sees that key of the tile; keep(key, t, c, s): for a
+// use of its score times log2(e), -inf where it does not.  `vb` of the values is what `values` gives, which waits for them.
+template <int HS, int NQ, int N, typename Seen, typename Keep, typename Values>
+__device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, int q0, uint32_t kb, float scale_log2, int lane, Seen seen, Keep keep, Values values) {
   const int g = lane >> 2;
   float s[kShTile / 16][N][4];
 #pragma unroll
@@ -125,6 +126,7 @@ __device__ __forceinline__ void attend_tile(Sums<HS, NQ>& a, uint32_t q, int q0,
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[i][t][e] = seen(i * 16 + (e >> 1) * 8 + g, t, e & 1) ? s[i][t][e] * scale_log2 : -INFINITY;
+        keep(i * 16 + (e >> 1) * 8 + g, t, e & 1, s[i][t][e]);
         top[e & 1] = fmaxf(top[e & 1], s[i][t][e]);
       }
 #pragma unroll

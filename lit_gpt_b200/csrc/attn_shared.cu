@@ -27,6 +27,7 @@ using namespace list;
 
 namespace {
 
+struct NoUse { __device__ __forceinline__ void operator()(int, int, int, float) const {} };   // of the scores
 constexpr int kShUnits = 3;                 // a warp's ring: units of 32 keys or 32 values
 
 // index of a row's new key in its own cache; -1: the row takes no part
@@ -337,8 +338,8 @@ __global__ void __launch_bounds__(ShSmem<HS, NP>::kWarps * 32, 1) attn_shared_ke
     };
     const int valid = cur.valid;
     auto seen = [valid](int key, int, int) { return key < valid; };
-    if (NP == NO || cur.own) attend_tile<HS, NQ, NO>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, values);
-    else attend_tile<HS, NQ, NP>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, values);
+    if (NP == NO || cur.own) attend_tile<HS, NQ, NO>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, NoUse{}, values);
+    else attend_tile<HS, NQ, NP>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, NoUse{}, values);
     __syncwarp();                                          // the values have been read: the keys of the tile after the next take their place
     const bool ends = cur.left == 0 || !more;
     Tile was = cur;
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(ClSmem<HS, NP>::kWarps * 32, 1) attn_shared_cl
       };
       const int valid = cur.valid;
       auto seen = [valid](int key, int, int) { return key < valid; };
-      attend_tile<HS, NP, NP>(a, sq, cur.own ? cur.b * p.per : 0, kb, p.scale_log2, lane, seen, values);   // (own keys with as many columns: the code of fewer is fetched, too)
+      attend_tile<HS, NP, NP>(a, sq, cur.own ? cur.b * p.per : 0, kb, p.scale_log2, lane, seen, NoUse{}, values);   // (own keys with as many columns: the code of fewer is fetched, too)
       __syncwarp();                                        // the values have been read: the keys of the tile after the next take their place
       const bool ends = cur.last || !more;
       const int own = cur.own, b = cur.b;

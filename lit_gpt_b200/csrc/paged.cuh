@@ -1,6 +1,6 @@
 // A ragged step over a paged key-value cache: what its kernels (paged_attn.cu) are given.
 #pragma once
-#include "common.cuh"
+#include "tc05.cuh"
 
 namespace b200 {
 
@@ -9,6 +9,11 @@ constexpr int kMaxTiles = 1 << 29;          // of a step
 struct PagedCut {                                           // what a CTA of paged_attn_tc05.cu goes on with that others began
   int first, last;                                          // the CTAs that have segments of it; last -1: it begins with an item of its own
   int count, row, gi;                                       // its queries, its first row, its group
+};
+
+struct PagedWeightCut {                                     // a block of 128 keys that several CTAs of paged_weights.cu have parts of
+  int first, last;                                          // those CTAs; last -1: none to join
+  int table, n, gi, block;
 };
 
 struct PagedParams {
@@ -22,7 +27,7 @@ struct PagedParams {
   __nv_bfloat16* k; __nv_bfloat16* v; int64_t k_page, k_group, v_page, v_group;
   float* kw;                                                // [pool][n_groups][page] attention weight that every key has received; null: not wanted
   __nv_bfloat16* out;
-  int rows, n_head, n_groups, per, max_length;
+  int rows, n_head, n_groups, per, max_rows, max_length;
   __nv_bfloat16* q;                                         // the queries, turned: [n_groups][rows * per][HS]
   float* lse;                                               // [n_groups][rows * per] log2 of the sum of exponentials of a query's scores (with kw)
   int tile_rows;                                            // queries of an item
@@ -34,6 +39,8 @@ struct PagedParams {
   int tc_rows;                                              // rows of a block of theirs: 256 queries at most
   int tc_workers;                                           // CTAs that share their tiles, at most
   float* tc_acc; float2* tc_ml; PagedCut* cuts;             // their results: two slots of 256 queries a CTA
+  float* scores; int score_rows, kept_max;                  // scores of the list's tiles, that many queries each; of sequences of up to kept_max queries a group (0: none are kept)
+  int kw_workers; float* kw_part; PagedWeightCut* kw_cuts;  // CTAs that compute the others' again, their sums: two slots of 128 keys a CTA
   int* item_base;                                           // per sequence: its first item
   int ways;                                                 // warps that join a head's results
   float scale_log2;
@@ -50,7 +57,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int s) {
   PagedSeq q;
   q.first = v.x;
   q.table = v.w;
-  const bool fits = v.y > 0 && v.x >= 0 && v.x < p.rows && v.y <= p.rows - v.x && v.z >= 0 && v.w >= 0 && v.w < p.page_rows;
+  const bool fits = v.y > 0 && v.x >= 0 && v.x < p.rows && v.y <= p.rows - v.x && v.y <= p.max_rows && v.z >= 0 && v.w >= 0 && v.w < p.page_rows;
   q.rows = fits ? v.y : 0;
   q.cached = min(max(v.z, 0), p.max_length);
   q.n = fits ? min(q.cached + q.rows, p.max_length) : 0;
@@ -63,6 +70,28 @@ __device__ __forceinline__ int page_at(const PagedParams& p, int table, int inde
   return id >= 0 && id < p.pool ? id : -1;
 }
 
+__device__ __forceinline__ int capped(int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); }
+
+// A box of 64 numbers of min(page, 128) keys, 128-byte-swizzled
+__device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(group), "r"(page), "r"(bar) : "memory");
+}
+inline bool page_map(CUtensorMap* map, const void* base, int hs, int page, int groups, int pool, int64_t group, int64_t apart) {
+  const TensorMapEncodeFn enc = tensor_map_encoder();
+  if (!enc) return false;
+  // (a single group's, or a single page's, distance is not used, but has to be one)
+  if (group == 0) group = (int64_t)page * hs;
+  if (apart == 0) apart = (int64_t)page * hs;
+  const cuuint64_t dim[4] = {(cuuint64_t)hs, (cuuint64_t)page, (cuuint64_t)groups, (cuuint64_t)pool};
+  const cuuint64_t stride[3] = {(cuuint64_t)hs * 2, (cuuint64_t)group * 2, (cuuint64_t)apart * 2};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)(page < 128 ? page : 128), 1u, 1u};
+  const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaError_t launch_paged_weights(const PagedParams& p, int head_size, cudaStream_t st);   // what the keys of sequences of more than kept_max queries a group receive
 cudaError_t launch_paged_tc05(const PagedParams& p, int head_size, cudaStream_t st);   // rows of sequences of more than list_max queries a group
 
 }  // namespace b200

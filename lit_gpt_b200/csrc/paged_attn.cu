@@ -9,11 +9,9 @@
 // An item is a tile of queries of one sequence and group -- rows times heads of the group, row after row, so that the heads of a group share the keys that they read -- against the
 // sequence's keys.  The tiles of all items are one list, cut evenly over the warps of all SMs (attn_list.cuh): requests of unequal lengths leave no SM without work.
 //
-// The weight that a key receives, sum over the step's rows and the group's heads of its softmax weights, is computed from the rows' maxima and sums: a warp takes a tile of 32 keys and
-// goes through the queries that see it, S^T = K Q^T, the keys as rows: a key's sum stays with the lanes that hold its row.  No atomics: one order of additions.
+// With the weights of keys wanted (paged_weights.cu), the list keeps its scores beside the results, and a launch behind the join adds up what every key received: no key is read again.
 #include "attn_list.cuh"
 #include "paged.cuh"
-#include "tc05.cuh"
 
 namespace b200 {
 
@@ -168,7 +166,6 @@ template <int THREADS>
 __device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, int2* s_warp, bool note) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = (p.n_seqs + THREADS - 1) / THREADS;
   // (a description whose sequences overlap can hold more tiles than fit the step's limits: then none is done)
-  auto capped = [](int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); };
   int2 here = make_int2(0, 0);
   for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
     const PagedSeq s = paged_seq(p, i);
@@ -311,7 +308,7 @@ struct PgSmem {
   static constexpr int kBytes = kWarps * kWarp;
 };
 
-template <int HS, int NQ>
+template <int HS, int NQ, bool KEEP>
 __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_kernel(const PagedParams p) {
   using C = PgSmem<HS, NQ>;
   constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;
@@ -394,17 +391,24 @@ __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_ker
     };
     const uint32_t bits = cur.bits();
     const int key0 = cur.key0(), count = walk.queries(cur);
+    float* const kept = KEEP ? p.scores + (int64_t)cur.index * p.score_rows * kShTile : nullptr;
+    auto keep = [&](int key, int t, int c, float s) {
+      if constexpr (KEEP) {
+        const int m = t * 8 + 2 * tq + c;
+        if (m < count) __stcg(kept + m * kShTile + key, s);
+      }
+    };
     if (key0 + kShTile > cur.seq.cached + 1 && cur.seq.rows > 1) {   // a chunk's own keys: every row sees those up to its own
       int lim[NQ][2];
 #pragma unroll
       for (int t = 0; t < NQ; ++t)
 #pragma unroll
         for (int c = 0; c < 2; ++c) lim[t][c] = cur.seq.cached + (cur.part * p.tile_rows + t * 8 + 2 * tq + c) / p.per - key0;
-      attend_tile<HS, NQ, NQ>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, [&](int key, int t, int c) { return ((bits >> key) & 1u) && key <= lim[t][c]; }, values);
+      attend_tile<HS, NQ, NQ>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, [&](int key, int t, int c) { return ((bits >> key) & 1u) && key <= lim[t][c]; }, keep, values);
     } else {
       auto seen = [bits](int key, int, int) { return ((bits >> key) & 1u) != 0u; };
-      if (NQ == 1 || count > 8) attend_tile<HS, NQ, NQ>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, values);
-      else attend_tile<HS, NQ, 1>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, values);
+      if (NQ == 1 || count > 8) attend_tile<HS, NQ, NQ>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, keep, values);
+      else attend_tile<HS, NQ, 1>(a, sq + qb * C::kQ, 0, kb, p.scale_log2, lane, seen, keep, values);
     }
     __syncwarp();                                          // the values have been read: the keys of the tile after the next take their place
     const bool ends = cur.left() == 0 || !more;
@@ -471,96 +475,40 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   if (p.lse && lane == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h - gi * p.per] = sum > 0.f ? top + log2f(sum) : INFINITY;
 }
 
-// ---- the weight that every key receives ----
-template <int HS>
-struct KwSmem {
-  static constexpr int kKeys = kShTile * HS * 2, kQ = 16 * HS * 2, kWarp = kKeys + 2 * kQ, kWarps = 4, kBytes = kWarps * kWarp;
-};
-
-template <int HS>
-__global__ void __launch_bounds__(KwSmem<HS>::kWarps * 32) paged_weights_kernel(const PagedParams p) {
-  using C = KwSmem<HS>;
-  constexpr int T = C::kWarps * 32, CH = HS / 8, RP = 32 / CH;
-  extern __shared__ __align__(128) uint8_t kw_smem[];
-  __shared__ int2 s_sums[T + 1], s_warp[C::kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
-  griddep_wait();
+// ---- the weight that the keys of the list's sequences receive: a tile of 32 keys a warp, a key a lane, from the scores that were kept ----
+__global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
+  constexpr int T = 256;
+  __shared__ int2 s_sums[T + 1], s_warp[T / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_launch();
-  const int all = make_split<T>(p, s_sums, s_warp, false).all;
+  const Split s = make_split<T>(p, s_sums, s_warp, false);
+  const int w = warp * (int)gridDim.x + (int)blockIdx.x;
   const Walk walk{p, s_sums, (p.n_seqs + T - 1) / T, T};
-  const uint32_t sk = pf_smem(kw_smem) + warp * C::kWarp, sq = sk + C::kKeys;
-  for (int index = blockIdx.x * C::kWarps + warp; index < all; index += gridDim.x * C::kWarps) {
-    const Tile t = walk.find(index);
-    const uint32_t bits = t.bits();
-    const int key0 = t.key0(), m0 = max(0, key0 - t.seq.cached) * p.per & ~15, count = t.seq.rows * p.per;   // (earlier rows see none of these keys)
-    const int64_t q0 = ((int64_t)t.gi * p.rows + t.seq.first) * p.per;
-    auto load_queries = [&](int m, int buf) {
-#pragma unroll
-      for (int j = 0; j < 16 / RP; ++j) {
-        const int r = j * RP + lane / CH, c = lane % CH;
-        const bool ok = m + r < count;
-        pf_cp16(sq + buf * C::kQ + sw<HS>(r, c), p.q + (q0 + (ok ? m + r : 0)) * HS + c * 8, ok);
+  const int first = first_tile(w, s), end = first_tile(w + 1, s);
+  Tile t = {};
+  if (w < s.workers) t = walk.find(first);
+  griddep_wait();
+  if (w >= s.workers) return;
+  for (;;) {
+    if (t.part == 0) {                     // (the tile of all tiles of queries)
+      const uint32_t bits = t.bits();
+      const int key0 = t.key0(), id = lane < 16 ? t.id0 : t.id1;
+      const bool there = (bits >> lane) & 1u;
+      float* const at = p.kw + (((int64_t)max(id, 0) * p.n_groups + t.gi) << p.shift) + ((key0 + lane) & ((1 << p.shift) - 1));
+      float sum = 0.f;
+      const float before = there ? *at : 0.f;
+      const int count = t.seq.rows * p.per;
+      const float* const lse = p.lse + ((int64_t)t.gi * p.rows + t.seq.first) * p.per;
+      for (int m0 = 0, index = t.index; m0 < count; m0 += p.tile_rows, index += t.tiles) {
+        const float* const kept = p.scores + (int64_t)index * p.score_rows * kShTile + lane;
+        const int n = min(p.tile_rows, count - m0);
+#pragma unroll 4
+        for (int m = 0; m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
       }
-      pf_commit();
-    };
-    load_tile<HS>(p, t, p.k, p.k_page, p.k_group, sk, lane);
-    load_queries(m0, 0);
-    float sum[2][2] = {};                      // keys 16 i + 8 h + g
-    for (int m = m0, buf = 0; m < count; m += 16, buf ^= 1) {
-      float lse[2][2];
-      int lim[2][2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int mm = m + u * 8 + 2 * tq + c;
-          lse[u][c] = mm < count ? __ldcg(p.lse + q0 + mm) : INFINITY;
-          lim[u][c] = mm < count ? t.seq.cached + mm / p.per - key0 : -1;
-        }
-      if (m + 16 < count) { load_queries(m + 16, buf ^ 1); pf_wait<1>(); } else { pf_wait<0>(); }
-      __syncwarp();
-      float s[2][2][4] = {};
-#pragma unroll
-      for (int kp = 0; kp < HS / 32; ++kp) {
-        uint32_t qf[2][4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) ldsm_x4(qf[u], sq + buf * C::kQ + sw<HS>(u * 8 + (lane & 7), kp * 4 + (lane >> 3)));
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t kf[4];
-            ldsm_x4(kf, sk + sw<HS>(i * 16 + (lane & 15), kp * 4 + h * 2 + (lane >> 4)));
-#pragma unroll
-            for (int u = 0; u < 2; ++u) pf_mma(s[i][u], kf, qf[u][2 * h], qf[u][2 * h + 1]);
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = i * 16 + (e >> 1) * 8 + g;
-            sum[i][e >> 1] += key <= lim[u][e & 1] ? ex2(fmaf(s[i][u][e], p.scale_log2, -lse[u][e & 1])) : 0.f;
-          }
-      __syncwarp();                            // the queries have been read
+      if (there) *at = before + sum;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = sum[i][h];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        const int key = i * 16 + h * 8 + g;
-        if (tq == 0 && ((bits >> key) & 1u)) {
-          const int id = key < 16 ? t.id0 : t.id1, in = (key0 + key) & ((1 << p.shift) - 1);
-          p.kw[(((int64_t)id * p.n_groups + t.gi) << p.shift) + in] += x;
-        }
-      }
-    pf_wait<0>();
-    __syncwarp();
+    if (t.index + 1 >= end) break;
+    walk.next(t);
   }
 }
 
@@ -570,8 +518,11 @@ struct PagedPlan {
   bool list, tensor;               // which kernels there is work for
   int list_max, tc_workers;
   int64_t items, slots, q;
+  int score_rows, kept_max, kw_workers;
+  int64_t scores;
   size_t bytes;
 };
+constexpr int64_t kScoresMax = (int64_t)1 << 28;   // scores that a step may keep: 1 GB
 
 std::atomic<int> g_paged_path{0};
 constexpr int kListMax = 32;       // queries of a sequence and group that the list of tiles takes
@@ -581,7 +532,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   const int path = g_paged_path.load(std::memory_order_relaxed);
   // chunks of one length only: all go to the tensor memory (some of them may turn out shorter, or not there)
   const int singles = per <= 8 ? 8 : per <= 16 ? 16 : kListMax;   // beside chunks the list takes single tokens, in items as small as they are
-  s.list_max = path == 1 || per > 128 ? 0x3fffffff : path == 2 ? 0 : max_rows * per <= kListMax ? kListMax : rows == (int64_t)n_seqs * max_rows ? 0 : singles;
+  s.list_max = path == 1 || path == 3 || per > 128 ? 0x3fffffff : path == 2 ? 0 : max_rows * per <= kListMax ? kListMax : rows == (int64_t)n_seqs * max_rows ? 0 : singles;
   s.tensor = max_rows * per > s.list_max;
   s.list = s.list_max > 0;
   const int64_t most = max_rows * per < s.list_max ? max_rows * per : s.list_max;   // queries of an item
@@ -597,25 +548,41 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   s.tc_workers = blocks < sm_count() ? (int)blocks : sm_count();
   const int64_t tc_slots = (int64_t)s.tc_workers * 2 * 256;
   s.q = rows * per * n_groups * hs;
+  s.score_rows = s.kept_max = s.kw_workers = 0;
+  s.scores = 0;
+  if (kw) {
+    s.score_rows = (int)(most < 8 * s.nq ? most : 8 * s.nq);
+    if (s.list && path != 3 && tiles * s.score_rows * kShTile <= kScoresMax) {
+      s.scores = tiles * s.score_rows * kShTile;
+      s.kept_max = s.list_max;
+    }
+    if (s.tensor || s.kept_max == 0) {
+      const int64_t blocks = (int64_t)n_groups * n_seqs * ((max_length + 127) / 128) * ((max_rows * per + 127) / 128);
+      s.kw_workers = blocks < sm_count() ? (int)blocks : sm_count();
+    }
+  }
   s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * sizeof(int) +
-            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
+            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)s.scores * sizeof(float) + (size_t)s.kw_workers * (256 * sizeof(float) + sizeof(PagedWeightCut)) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
   const int64_t results = 2 + (int64_t)s.workers / s.items;
   s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
   while (s.ways < 8 && results > 4 * s.ways && rows * n_groups * per * s.ways < 24 * sm_count()) s.ways *= 2;
   return s;
 }
 
-template <int HS, int NQ>
-cudaError_t launch_list(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
+template <int HS, int NQ, bool KEEP>
+cudaError_t launch_list_of(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
   using C = PgSmem<HS, NQ>;
   static PerDeviceOnce once;
   if (once.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_list_kernel<HS, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    const cudaError_t e = cudaFuncSetAttribute(paged_list_kernel<HS, NQ, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
     if (e != cudaSuccess) return e;
     once.done();
   }
-  return launch(paged_list_kernel<HS, NQ>, dim3((unsigned)s.ctas), dim3(C::kWarps * 32), (size_t)C::kBytes, st, p);
+  return launch(paged_list_kernel<HS, NQ, KEEP>, dim3((unsigned)s.ctas), dim3(C::kWarps * 32), (size_t)C::kBytes, st, p);
 }
+
+template <int HS, int NQ>
+cudaError_t launch_list(const PagedParams& p, const PagedPlan& s, cudaStream_t st) { return p.scores ? launch_list_of<HS, NQ, true>(p, s, st) : launch_list_of<HS, NQ, false>(p, s, st); }
 
 template <int HS>
 cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
@@ -636,17 +603,13 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t 
     e = launch(paged_join_kernel<HS>, dim3((unsigned)(p.rows * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
     if (e != cudaSuccess) return e;
   }
-  if (!p.kw) return e;
-  using C = KwSmem<HS>;
-  static PerDeviceOnce once;
-  if (once.need()) {
-    e = cudaFuncSetAttribute(paged_weights_kernel<HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
-    if (e != cudaSuccess) return e;
-    once.done();
+  if (p.scores) {
+    PagedParams k = p;
+    const int ctas = 8 * p.sms;      // a warp's tiles are a chain of loads each: as many warps as are at once
+    k.workers = 8 * ctas;
+    if ((e = launch(paged_kept_kernel, dim3((unsigned)ctas), dim3(256), 0, st, k)) != cudaSuccess) return e;
   }
-  PagedParams one = p;             // the queries of a sequence and group as one tile: the list is that of the key tiles
-  one.tile_rows = one.list_max = 0x3fffffff;
-  return launch(paged_weights_kernel<HS>, dim3((unsigned)(4 * p.sms)), dim3(C::kWarps * 32), (size_t)C::kBytes, st, one);
+  return s.kw_workers > 0 ? launch_paged_weights(p, HS, st) : e;
 }
 
 }  // namespace
@@ -663,7 +626,7 @@ size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int
   return paged_plan(rows, n_seqs, n_groups, n_head / n_groups, head_size, max_rows, max_length, key_weights != 0).bytes;
 }
 
-int b200_attn_paged_tune(int path) { return g_paged_path.exchange(path == 1 || path == 2 ? path : 0); }
+int b200_attn_paged_tune(int path) { return g_paged_path.exchange(path >= 1 && path <= 3 ? path : 0); }
 
 int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a, "b200_attn_paged: null argument");
@@ -689,7 +652,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   const PagedPlan s = paged_plan(a->rows, a->n_seqs, a->n_groups, per, a->head_size, a->max_rows, a->max_length, a->key_weights != nullptr);
   B200_CHECK_ARG(s.items * ((a->max_length + kShTile - 1) / kShTile) < kMaxTiles, "b200_attn_paged: too many keys in a step");
   B200_CHECK_ARG(a->workspace_bytes >= s.bytes, "b200_attn_paged: workspace too small");
-  if (s.tensor) B200_CHECK_WAITS("b200_attn_paged");
+  if (s.tensor || s.kw_workers > 0) B200_CHECK_WAITS("b200_attn_paged");
   PagedParams p = {};
   p.qkv = (const __nv_bfloat16*)a->qkv;
   p.cos = a->cos; p.sin = a->sin; p.table_bf16 = a->table_dtype == B200_BF16; p.table_rows = a->table_rows; p.table_presel = a->table_preselected; p.rope_n = a->rope_n_elem;
@@ -702,7 +665,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.k_page = a->k_page_stride; p.k_group = a->k_group_stride; p.v_page = a->v_page_stride; p.v_group = a->v_group_stride;
   p.kw = a->key_weights;
   p.out = (__nv_bfloat16*)a->out;
-  p.rows = (int)a->rows; p.n_head = a->n_head; p.n_groups = a->n_groups; p.per = per; p.max_length = (int)a->max_length;
+  p.rows = (int)a->rows; p.n_head = a->n_head; p.n_groups = a->n_groups; p.per = per; p.max_rows = (int)a->max_rows; p.max_length = (int)a->max_length;
   p.tile_rows = 8 * s.nq; p.items = (int)s.items; p.workers = s.workers; p.sms = sm_count(); p.ways = s.ways;
   // (every part of wide accesses begins on a 16-byte boundary: they come first)
   p.q = (__nv_bfloat16*)a->workspace;
@@ -714,7 +677,11 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.where = (int2*)(p.tc_ml + (int64_t)s.tc_workers * 512);
   p.cuts = (PagedCut*)(p.where + s.items);
   p.item_base = (int*)(p.cuts + s.tc_workers);
-  p.lse = p.kw ? (float*)(p.item_base + a->n_seqs) : nullptr;
+  p.score_rows = s.score_rows; p.kept_max = s.kept_max; p.kw_workers = s.kw_workers;
+  p.kw_cuts = (PagedWeightCut*)(p.item_base + a->n_seqs);
+  p.kw_part = (float*)(p.kw_cuts + s.kw_workers);
+  p.lse = p.kw ? p.kw_part + (int64_t)s.kw_workers * 256 : nullptr;
+  p.scores = s.scores ? p.lse + (int64_t)p.rows * p.per * p.n_groups : nullptr;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_size);
   const cudaStream_t st = (cudaStream_t)stream;
   B200_CUDA((a->head_size == 128 ? launch_paged<128>(p, s, st) : launch_paged<64>(p, s, st)));

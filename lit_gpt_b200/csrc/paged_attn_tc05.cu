@@ -32,11 +32,6 @@ struct PtTile {
   static constexpr uint32_t kS = 0, kO = 256;              // tensor-memory columns: S0 S1 (P over them) | O0 O1
 };
 
-__device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int page, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(group), "r"(page), "r"(bar) : "memory");
-}
-
 // ---- the list of key tiles ----
 // The list is cut by steps: an item counts as its key tiles and kLead more, the time that its queries' way in and its results' way out take (4 to 5 us where a tile takes 2.2).
 constexpr int kLead = 2;
@@ -52,7 +47,6 @@ __device__ __forceinline__ Blocks blocks_of(const PagedParams& p, const PagedSeq
   b.cached = s.cached; b.rows = s.rows; b.n = s.n;
   return b;
 }
-__device__ __forceinline__ int capped(int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); }
 // The steps of a group, by a whole warp.
 __device__ __forceinline__ int steps_of(const Blocks& b, int lane) {
   int64_t s = 0;
@@ -679,20 +673,6 @@ __global__ void __launch_bounds__(256) paged_tc05_join_kernel(const PagedParams 
                                                      pack_bf16(a[j + 6] * inv, a[j + 7] * inv));
     if (p.lse && warp == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
   }
-}
-
-bool page_map(CUtensorMap* map, const void* base, int hs, int page, int groups, int pool, int64_t group, int64_t apart) {
-  const TensorMapEncodeFn enc = tensor_map_encoder();
-  if (!enc) return false;
-  // (a single group's, or a single page's, distance is not used, but has to be one)
-  if (group == 0) group = (int64_t)page * hs;
-  if (apart == 0) apart = (int64_t)page * hs;
-  const cuuint64_t dim[4] = {(cuuint64_t)hs, (cuuint64_t)page, (cuuint64_t)groups, (cuuint64_t)pool};
-  const cuuint64_t stride[3] = {(cuuint64_t)hs * 2, (cuuint64_t)group * 2, (cuuint64_t)apart * 2};
-  const cuuint32_t box[4] = {64u, (cuuint32_t)(page < 128 ? page : 128), 1u, 1u};
-  const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int HS>

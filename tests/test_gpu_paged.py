@@ -11,7 +11,7 @@ from paged_oracle import F64, make
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(params=["list", "tensor memory", "by size"])
+@pytest.fixture(params=["list", "tensor memory", "list without scores", "by size"])
 def path(request):
     return request.param
 
@@ -23,7 +23,7 @@ def K(path):
         pytest.skip("needs a CUDA device")
     from lit_gpt_b200 import kernels
 
-    before = kernels.attn_paged_tune({"list": 1, "tensor memory": 2, "by size": 0}[path])
+    before = kernels.attn_paged_tune({"list": 1, "tensor memory": 2, "list without scores": 3, "by size": 0}[path])
     yield kernels
     kernels.attn_paged_tune(before)
 
@@ -31,7 +31,7 @@ def K(path):
 @pytest.fixture
 def formula(path):
     """The step in 64 bits; on the tensor memory probabilities are rounded to bf16."""
-    return lambda d: oracle.step(d, 0.0 if path == "list" else 2 ** -8)
+    return lambda d: oracle.step(d, 0.0 if path.startswith("list") else 2 ** -8)
 
 
 @pytest.fixture
