@@ -1,10 +1,11 @@
 // Sequences of a paged key-value cache cut down by the attention weight that their keys have received: per sequence and group the first, the last and the heaviest keys stay, in order, at
 // the front of the sequence's pages.
 //
-// Two launches.  paged_choose_kernel, a CTA per sequence and group: the smallest weight that stays by radix selection over the weights as ordered whole numbers, eight bits at a time; then
-// the indices that stay, in order, by a scan, and their weights moved.  paged_move_kernel: keys and values moved in place, a CTA per sequence, group, tensor and slice of the columns.
-// A key moves to a lower index or stays, and slices of columns share nothing: a CTA that goes through its rows in order, reads a tile of them before it writes them, and has a
-// barrier between, never writes what is still to be read.
+// Two launches.  paged_choose_kernel, a CTA per sequence and group: the smallest weight that stays by radix selection over the weights as ordered whole numbers; then the indices that
+// stay, in order, by a scan, and their weights moved.  Weights that fit are held in shared memory: read once, eleven bits a digit, one scan of a run of keys a thread; longer sequences'
+// are read for every digit, eight bits each, and scanned in rounds.  paged_move_kernel: keys and values moved in place, a cluster of CTAs per sequence, group and tensor.
+// A key moves to a lower index or stays: a cluster that goes through its rows in order, reads a tile of them before it writes them, and has a barrier between, never writes what is still
+// to be read.
 //
 // Bound: bytes of the rows that stay, read and written.
 #include "common.cuh"
@@ -117,36 +118,165 @@ __global__ void __launch_bounds__(kChThreads) paged_choose_kernel(const EvictPar
   }
 }
 
-// LANES lanes of 16 bytes each a row
-template <int LANES>
-__global__ void __launch_bounds__(kMvThreads) paged_move_kernel(const EvictParams p) {
-  constexpr int ROWS = kMvThreads / LANES;        // at once
-  griddep_launch();
-  griddep_wait();
-  const int s = blockIdx.x / p.n_groups, g = blockIdx.x - s * p.n_groups, page = 1 << p.shift;
-  const int keep = p.moved[s];
-  if (keep == 0) return;
-  const int hs = (int)gridDim.z * LANES * 8;
-  const int* const table = p.pages + (int64_t)(p.rows ? p.rows[s] : s) * p.pages_ld;
-  const int* const from = p.from + (int64_t)blockIdx.x * p.keep;
-  const int64_t apart = blockIdx.y ? p.v_page : p.k_page;
-  __nv_bfloat16* const base = (blockIdx.y ? p.v + (int64_t)g * p.v_group : p.k + (int64_t)g * p.k_group) + blockIdx.z * LANES * 8 + threadIdx.x % LANES * 8;
-  auto at = [&](int i) { return reinterpret_cast<uint4*>(base + (int64_t)table[i >> p.shift] * apart + (int64_t)(i & (page - 1)) * hs); };
-  for (int d0 = (int)threadIdx.x / LANES; d0 < keep + (int)threadIdx.x / LANES; d0 += ROWS * kMvUnroll) {   // (as many rounds in every thread)
-    uint4 x[kMvUnroll];
+// ---- the same with the sequence's weights, and the places that stay, in shared memory ----
+constexpr int kBins = 2048, kBinCopies = 2;
+
+// a's sum over the threads before this one; `all`: over all of them
+__device__ __forceinline__ int block_before(int a, int* s_warp, int& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = a;
 #pragma unroll
-    for (int j = 0; j < kMvUnroll; ++j) {
-      const int d = d0 + j * ROWS;
-      if (d < keep) x[j] = *at(from[d]);
+  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+  __syncthreads();                                 // (s_warp has been read)
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int w = s_warp[lane];                            // (as many warps as lanes)
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += t; }
+  all = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  return inc - a + (warp ? before : 0);
+}
+
+__global__ void __launch_bounds__(kChThreads) paged_choose_smem_kernel(const EvictParams p) {
+  extern __shared__ __align__(16) float ch_smem[];
+  float* const s_w = ch_smem;                                       // [max_length]
+  int* const s_from = reinterpret_cast<int*>(ch_smem + p.max_length);   // [keep]
+  int* const s_table = s_from + p.keep;                             // the sequence's pages
+  __shared__ int s_hist[kBinCopies * kBins];
+  __shared__ int s_warp[kChWarps], s_pick[2];
+  griddep_wait();
+  griddep_launch();
+  const int tid = threadIdx.x, warp = tid >> 5, s = blockIdx.x / p.n_groups, g = blockIdx.x - s * p.n_groups, page = 1 << p.shift;
+  const int n = p.lengths[s], row = p.rows ? p.rows[s] : s;
+  bool cut = n > p.keep && n <= p.max_length && row >= 0 && row < p.table_seqs;
+  const int* const table = p.pages + (int64_t)(cut ? row : 0) * p.pages_ld;
+  if (cut) {
+    bool all = true;
+    for (int i = tid; i < (n + page - 1) >> p.shift; i += kChThreads) {
+      const int id = table[i];
+      s_table[i] = id;
+      all = all && id >= 0 && id < p.pool;
+    }
+    cut = __syncthreads_and(all);
+  }
+  if (g == 0 && tid == 0) {
+    p.lengths_out[s] = cut ? p.keep : n;
+    p.moved[s] = cut ? p.keep : 0;
+  }
+  if (!cut) return;
+  auto at = [&](int i) -> float* { return p.kw + (((int64_t)s_table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1)); };
+#pragma unroll 8
+  for (int i = tid; i < n; i += kChThreads) s_w[i] = *at(i);
+  const int lo = p.first, hi = n - p.recent;
+  int need = p.keep - p.first - p.recent;
+  const bool any = need > 0;
+  uint32_t high = 0;
+  // digits of 11, 11 and 10 bits
+  for (int digit = 0; digit < 3 && any; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+    for (int i = tid; i < kBinCopies * kBins; i += kChThreads) s_hist[i] = 0;
+    __syncthreads();                               // (and: the weights are there)
+    for (int i = lo + tid; i < hi; i += kChThreads) {
+      const uint32_t u = ordered(s_w[i]);
+      if (digit == 0 || u >> (shift + bits) == high) atomicAdd(&s_hist[warp % kBinCopies * kBins + ((u >> shift) & ((1u << bits) - 1u))], 1);
     }
     __syncthreads();
+    // a thread has two digits, the greater ones first
+    const int top = kBins - 1 - 2 * tid;
+    int c[2] = {0, 0}, all;
+#pragma unroll
+    for (int k = 0; k < kBinCopies; ++k) { c[0] += s_hist[k * kBins + top]; c[1] += s_hist[k * kBins + top - 1]; }
+    int before = block_before(c[0] + c[1], s_warp, all);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (before < need && need <= before + c[j]) { s_pick[0] = top - j; s_pick[1] = need - before; }
+      before += c[j];
+    }
+    __syncthreads();
+    high = (high << bits) | (uint32_t)s_pick[0];
+    need = s_pick[1];
+    __syncthreads();
+  }
+  // a run of keys a thread: those above, and the first `need` of those that equal it
+  const int run = (n + kChThreads - 1) / kChThreads, begin = min(n, tid * run), end = min(n, begin + run);
+  int above = 0, ties = 0, all;
+  for (int i = begin; i < end; ++i) {
+    const uint32_t u = ordered(s_w[i]);
+    const bool mid = i >= lo && i < hi;
+    above += !mid || (any && u > high);
+    ties += mid && any && u == high;
+  }
+  const int above_before = block_before(above, s_warp, all);
+  int equal = block_before(ties, s_warp, all), place = above_before + min(equal, need);
+  for (int i = begin; i < end; ++i) {
+    const uint32_t u = ordered(s_w[i]);
+    const bool mid = i >= lo && i < hi, tie = mid && any && u == high;
+    if (!mid || (any && u > high) || (tie && equal < need)) s_from[place++] = i;
+    equal += tie;
+  }
+  __syncthreads();
+  int* const from = p.from + (int64_t)blockIdx.x * p.keep;
+#pragma unroll 8
+  for (int d = tid; d < p.keep; d += kChThreads) {
+    const int i = s_from[d];
+    from[d] = i;
+    *at(d) = s_w[i];
+  }
+}
+
+// LANES lanes of 16 bytes each a row; the CTAs of a cluster share the rows of a sequence, group and tensor, a tile each at a time.  A tile is read while the one before it is still in
+// registers: its rows lie behind all places of that one.
+template <int LANES>
+__global__ void __launch_bounds__(kMvThreads) paged_move_kernel(const EvictParams p, int ctas) {
+  constexpr int ROWS = kMvThreads / LANES, TILE = ROWS * kMvUnroll;        // at once; of a tile
+  griddep_launch();
+  griddep_wait();
+  const int rank = blockIdx.x % ctas, item = blockIdx.x / ctas, s = item / p.n_groups, g = item - s * p.n_groups, page = 1 << p.shift;
+  const int keep = p.moved[s];
+  if (keep == 0) return;
+  const int hs = LANES * 8, row = rank * TILE + (int)threadIdx.x / LANES;
+  const int* const table = p.pages + (int64_t)(p.rows ? p.rows[s] : s) * p.pages_ld;
+  const int* const from = p.from + (int64_t)item * p.keep;
+  const int64_t apart = blockIdx.y ? p.v_page : p.k_page;
+  __nv_bfloat16* const base = (blockIdx.y ? p.v + (int64_t)g * p.v_group : p.k + (int64_t)g * p.k_group) + threadIdx.x % LANES * 8;
+  auto at = [&](int i) { return reinterpret_cast<uint4*>(base + (int64_t)table[i >> p.shift] * apart + (int64_t)(i & (page - 1)) * hs); };
+  uint4 x[kMvUnroll];
+  int f[kMvUnroll];
+  auto indices = [&](int d0) {
 #pragma unroll
     for (int j = 0; j < kMvUnroll; ++j) {
-      const int d = d0 + j * ROWS;
-      if (d < keep) *at(d) = x[j];
+      const int d = d0 + row + j * ROWS;
+      f[j] = d < keep ? from[d] : -1;
+    }
+  };
+  auto load = [&]() {
+#pragma unroll
+    for (int j = 0; j < kMvUnroll; ++j)
+      if (f[j] >= 0) x[j] = *at(f[j]);
+  };
+  const int step = ctas * TILE;
+  indices(0);
+  load();
+  indices(step);
+  for (int d0 = 0; d0 < keep; d0 += step) {        // (as many rounds in every thread)
+    uint4 y[kMvUnroll];
+#pragma unroll
+    for (int j = 0; j < kMvUnroll; ++j) y[j] = x[j];
+    load();                                        // of the next tile
+    indices(d0 + 2 * step);
+    // this tile has been read by all
+    if (ctas == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < kMvUnroll; ++j) {
+      const int d = d0 + row + j * ROWS;
+      if (d < keep) *at(d) = y[j];
     }
   }
 }
+
+constexpr int kHeldMax = 200 * 1024;              // shared memory for weights, places and pages
 
 size_t evict_bytes(int n_seqs, int n_groups, int64_t keep) { return ((size_t)n_seqs * n_groups * keep + n_seqs) * sizeof(int); }
 
@@ -195,8 +325,22 @@ int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
   p.moved = p.from + (int64_t)a->n_seqs * a->n_groups * a->keep;
   const cudaStream_t st = (cudaStream_t)stream;
   const unsigned items = (unsigned)(a->n_seqs * a->n_groups);
-  B200_CUDA(launch(paged_choose_kernel, dim3(items), dim3(kChThreads), 0, st, p));
-  B200_CUDA(launch(paged_move_kernel<2>, dim3(items, 2, (unsigned)(a->head_size / 16)), dim3(kMvThreads), 0, st, p));
+  const int64_t held = (a->max_length + a->keep + (a->max_length + a->page - 1) / a->page) * 4;
+  if (held <= kHeldMax) {
+    static PerDeviceOnce once;
+    if (once.need()) {
+      B200_CUDA(cudaFuncSetAttribute(paged_choose_smem_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
+      once.done();
+    }
+    B200_CUDA(launch(paged_choose_smem_kernel, dim3(items), dim3(kChThreads), (size_t)held, st, p));
+  } else {
+    B200_CUDA(launch(paged_choose_kernel, dim3(items), dim3(kChThreads), 0, st, p));
+  }
+  // as many CTAs for the rows of one tensor as leave none of the SMs without, no more than they have tiles
+  const int lanes = a->head_size / 8, tile = kMvThreads / lanes * kMvUnroll;
+  int ctas = 1;
+  while (ctas < 8 && (int64_t)items * 2 * ctas < sm_count() && ctas * tile < a->keep) ctas *= 2;
+  B200_CUDA(launch_cluster(lanes == 8 ? paged_move_kernel<8> : paged_move_kernel<16>, dim3(items * ctas, 2), dim3(kMvThreads), ctas, 0, st, p, ctas));
   return B200_OK;
 }
 
