@@ -25,11 +25,13 @@ import torch.nn.functional as F
 from . import kernels as K
 from .config import Config
 from .quant import QLinear, prefill_pair, short_pair
+from .ragged import PagedStep
 
 # batched decode with more rows than this runs RMSNorm as its own launch instead of in the GEMV prologue (see GPT._fused_decode)
 SPLIT_NORM_ROWS = int(os.environ.get("B200_SPLIT_NORM_ROWS", "8"))
 
 FUSED_HEAD_SIZES = (64, 128)
+FUSED_ROWS = 16   # rows of a step that the fused decode chain's GEMVs take
 
 
 class GPT(nn.Module):
@@ -91,6 +93,8 @@ class GPT(nn.Module):
                 raise TypeError("You need to call `gpt.set_kv_cache()`")
             if T > 1 and isinstance(self.transformer.h[0].attn.kv_cache, SharedKVCache):
                 raise RuntimeError("rows that share a prefix take one token each per step")
+            if isinstance(self.transformer.h[0].attn.kv_cache, PagedKVCache):
+                raise RuntimeError("a paged cache runs ragged steps: `gpt.paged_step`")
             # (a traced forward takes the module path: its kernels are registered custom ops, the fused chain is raw C-ABI calls)
             if T == 1 and input_pos.numel() == 1 and not torch.compiler.is_compiling() and self.fused_decode_ready(idx):
                 return self._fused_decode(idx, input_pos)
@@ -110,6 +114,37 @@ class GPT(nn.Module):
             x = block(x, cos, sin, mask, input_pos)
         x = self.transformer.ln_f(x)
         return self.lm_head(x)
+
+    @property
+    def device(self) -> torch.device:
+        return self.transformer.wte.weight.device
+
+    @torch.inference_mode()
+    def paged_step(self, tokens: torch.Tensor, step: PagedStep, want: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One ragged step over paged caches (``PagedKVCache`` in every block): `tokens` (rows,) are the new tokens of all sequences, `step` says whose they are.  Returns the
+        logits (rows, vocab) of the rows `want` (indices; None: all of them)."""
+        caches = [b.attn.kv_cache for b in self.transformer.h]
+        if not all(isinstance(c, PagedKVCache) for c in caches):
+            raise TypeError("a paged step needs a PagedKVCache in every block")
+        n = tokens.numel()
+        for c in caches:
+            c.step = step
+        try:
+            if self.fused_decode_ready(tokens.view(1, n)):
+                if n <= FUSED_ROWS:
+                    logits = self._fused_decode(tokens.view(n, 1), step.row_pos)[:, 0]
+                    return logits if want is None else logits.index_select(0, want)
+                if self.config.intermediate_size % 8 == 0:
+                    return self._fused_prefill(tokens.view(1, n), step.row_pos, want)[0]
+            x = self.transformer.wte(tokens.view(1, n))
+            for block in self.transformer.h:
+                x = block(x, self.cos, self.sin, None, step.row_pos)
+            if want is not None:
+                x = x.index_select(1, want)
+            return self.lm_head(self.transformer.ln_f(x))[0]
+        finally:
+            for c in caches:
+                c.step = None
 
     @classmethod
     def from_name(cls, name: str, **kwargs: Any) -> "GPT":
@@ -261,11 +296,12 @@ class GPT(nn.Module):
             hit = tabs[dev] = (self.cos.to(dev), self.sin.to(dev), self.cos.data_ptr())
         return hit[0], hit[1]
 
-    def _fused_prefill(self, idx: torch.Tensor, input_pos: torch.Tensor) -> torch.Tensor:
+    def _fused_prefill(self, idx: torch.Tensor, input_pos: torch.Tensor, want: Optional[torch.Tensor] = None) -> torch.Tensor:
         """T > 1 tokens over the cache with this library's kernels only (reference: model.py:499-519, 572-593, 609-665, 712-716): the
         embedding, the residual adds fused into the RMSNorm that follows them (b200_rmsnorm delta / sum_out), SwiGLU as one kernel,
         RoPE + cache append + causal attention straight from the full cos / sin tables and input_pos -- no table or mask
-        `index_select` (the 16 MB mask gather at T = 4096 fed nothing: the attention kernel derives the mask row from input_pos)."""
+        `index_select` (the 16 MB mask gather at T = 4096 fed nothing: the attention kernel derives the mask row from input_pos).  `want`: only these of the B * T rows go
+        on to the head."""
         c = self.config
         B, T = idx.shape
         eps = c.norm_eps
@@ -284,9 +320,12 @@ class GPT(nn.Module):
                 n1 = K.rmsnorm(x, block.norm_1.weight, eps, delta=delta, sum_out=x_new)
                 x = x_new
             qkv = a.attn(n1.view(B, T, -1))
-            q = K.rope_kv_append(qkv, self.cos, self.sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size,
-                                 c.rope_n_elem, table_preselected=False)
-            y = K.attn_prefill(q, cache.k, cache.v, input_pos, scale)
+            if isinstance(cache, PagedKVCache):
+                y = cache.attend(c, qkv, self.cos, self.sin).view(B, T, -1)
+            else:
+                q = K.rope_kv_append(qkv, self.cos, self.sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size,
+                                     c.rope_n_elem, table_preselected=False)
+                y = K.attn_prefill(q, cache.k, cache.v, input_pos, scale)
             h = a.proj(y)
             if tp:
                 h = self._all_reduce(h.contiguous())
@@ -295,8 +334,10 @@ class GPT(nn.Module):
             x = x_new
             n2 = n2.view(B, T, -1)
             delta = m(n2).view(B * T, -1)   # LLaMAMLP.forward: fused SwiGLU (b200_swiglu, or the epilogue of the GEMV for <= 16 rows, of the GEMM for long prompts); its tensor-parallel hook sums the ranks' partials
+        if want is not None:
+            x, delta = x.index_select(0, want), None if delta is None else delta.index_select(0, want)
         xf = K.rmsnorm(x, self.transformer.ln_f.weight, eps, delta=delta)
-        return self.lm_head(xf.view(B, T, -1))
+        return self.lm_head(xf.view(B, T, -1) if want is None else xf.view(1, len(want), -1))
 
     def _fused_prefill_multi(self, idx: torch.Tensor, input_pos: torch.Tensor) -> torch.Tensor:
         """_fused_prefill for blocks placed on several devices (generate/sequentially.py): the residual stream and the pending
@@ -458,7 +499,7 @@ class GPT(nn.Module):
         # launches per token fewer, but measured SLOWER on B200 (632 vs 676 tok/s): in-kernel the
         # attention tail runs on one SM per head at the GEMV's register budget, 5.5 - 7.5 us against ~6 us for the stand-alone
         # cluster kernel INCLUDING its launch boundary
-        fuse_attn = (not tp and B == 1 and a0 is not None and not isinstance(blocks[0].attn.kv_cache, SharedKVCache) and self.max_seq_length <= int(os.environ.get("B200_FUSE_ATTN_MAX_SEQ", "0"))
+        fuse_attn = (not tp and B == 1 and a0 is not None and not isinstance(blocks[0].attn.kv_cache, (SharedKVCache, PagedKVCache)) and self.max_seq_length <= int(os.environ.get("B200_FUSE_ATTN_MAX_SEQ", "0"))
                      and a0.fold == 1 and a0.streams(1) and input_pos.numel() == 1
                      and K.qgemv_attn_fusable(a0.out_features, a0.in_features, a0.quant_type, c.n_head, c.n_query_groups, c.head_size,
                                               c.rope_n_elem, self.max_seq_length))
@@ -468,8 +509,8 @@ class GPT(nn.Module):
         for li, block in enumerate(blocks):
             a, m, cache = block.attn, block.mlp, block.attn.kv_cache
             nxt_qkv = blocks[li + 1].attn.attn if li + 1 < len(blocks) else self.lm_head
-            # L2 hint: the filled K / V rows this block's attention reads next (positions of a row's own cache behind a shared prefix count from another zero)
-            hint = None if isinstance(cache, SharedKVCache) else (cache.k, cache.v, input_pos)
+            # L2 hint: the filled K / V rows this block's attention reads next (positions of a row's own cache behind a shared prefix count from another zero, pages lie anywhere)
+            hint = None if isinstance(cache, (SharedKVCache, PagedKVCache)) else (cache.k, cache.v, input_pos)
             if fuse_attn:
                 # the attention step runs inside the QKV GEMV's kernel (b200_qgemv_tiled_args::attn): one launch boundary less
                 y = torch.empty((B, c.n_head * c.head_size), dtype=torch.bfloat16, device=x.device)
@@ -605,6 +646,8 @@ class CausalSelfAttention(nn.Module):
         if T == 1:
             y = _decode_attention(c, cache, qkv, cos, sin, input_pos, table_preselected=True)
             return y.view(B, 1, c.n_head * c.head_size)
+        if isinstance(cache, PagedKVCache):
+            return cache.attend(c, qkv, cos, sin).view(B, T, c.n_head * c.head_size)
         q = K.rope_kv_append(qkv, cos, sin, input_pos, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size,
                              c.rope_n_elem, table_preselected=True)
         # the mask row of token t (model.py:509) is "cache positions <= input_pos[t]": the kernel takes input_pos directly
@@ -746,8 +789,29 @@ class SharedKVCache(KVCache):
         self.prefix_len = prefix_len   # int32 (1,) on the device: how much of the prompt's cache is the prompt
 
 
+class PagedKVCache(KVCache):
+    """Keys and values of many sequences, in pages of one pool: sequences of any lengths share it, and hold pages as they grow (``generate.serve.PagedSession``).  With `weights` every
+    key's share of the attention is recorded, by which ``kernels.evict_paged`` cuts sequences down."""
+
+    def __init__(self, config: Config, pages: int, page: int, device: Optional[torch.device] = None, weights: bool = False) -> None:
+        shape = (pages, config.n_query_groups, page, config.head_size)
+        super().__init__(shape, shape, device=device, dtype=torch.bfloat16, gqa_native=True)
+        self.register_buffer("key_weights", torch.zeros(shape[:3], device=device) if weights else None, persistent=False)
+        self.step: Optional[PagedStep] = None   # whose rows the current step's are
+
+    def attend(self, c: Config, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        """Rotation (by the full tables), append and attention of the current step's rows."""
+        s = self.step
+        if s is None:
+            raise RuntimeError("a paged cache runs ragged steps: `gpt.paged_step`")
+        return K.attn_paged(qkv, cos, sin, s.row_pos, s.row_seq, s.seqs, s.table, self.k, self.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem, max_rows=s.max_rows,
+                            max_length=s.max_length, key_weights=self.key_weights)
+
+
 def _decode_attention(c: Config, cache: KVCache, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, table_preselected: bool = False) -> torch.Tensor:
     """Rotation, cache append and attention of one token per row, over the kind of cache that there is."""
+    if isinstance(cache, PagedKVCache):
+        return cache.attend(c, qkv, cos, sin)
     if isinstance(cache, SharedKVCache):
         return K.attn_decode_shared(qkv, cos, sin, pos, cache.k, cache.v, cache.k_prefix, cache.v_prefix, cache.prefix_len, c.n_head, c.n_query_groups, c.head_size,
                                     c.rope_n_elem, table_preselected=table_preselected)

@@ -85,6 +85,21 @@ def _(qkv, cos, sin, pos, k_cache, v_cache, k_prefix, v_prefix, prefix_len, n_he
     return qkv.new_empty((k_cache.shape[0], n_head * head_size), dtype=torch.bfloat16)
 
 
+# ---- a ragged step over a paged cache -----------------------------------------------------------------------------
+@torch.library.custom_op(f"{NS}::attn_paged", mutates_args=("k_pages", "v_pages", "key_weights"))
+def attn_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor, seqs: torch.Tensor, table: torch.Tensor,
+               k_pages: torch.Tensor, v_pages: torch.Tensor, n_head: int, n_groups: int, head_size: int, rope_n_elem: int, max_rows: int, max_length: int,
+               key_weights: Optional[torch.Tensor] = None, table_preselected: bool = False) -> torch.Tensor:
+    return K.attn_paged(qkv, cos, sin, row_pos, row_seq, seqs, table, k_pages, v_pages, n_head, n_groups, head_size, rope_n_elem, max_rows=max_rows, max_length=max_length,
+                        key_weights=key_weights, table_preselected=table_preselected)
+
+
+@attn_paged.register_fake
+def _(qkv, cos, sin, row_pos, row_seq, seqs, table, k_pages, v_pages, n_head, n_groups, head_size, rope_n_elem, max_rows, max_length, key_weights=None,
+      table_preselected=False):
+    return qkv.new_empty((row_seq.shape[0], n_head * head_size), dtype=torch.bfloat16)
+
+
 # ---- prefill: RoPE + cache write, then causal attention over the cache (model.py:624-665) -------------------------
 @torch.library.custom_op(f"{NS}::rope_kv_append", mutates_args=("k_cache", "v_cache"))
 def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,

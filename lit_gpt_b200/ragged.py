@@ -28,6 +28,18 @@ class RaggedBatch:
     identity_ctx: bool = False       # every sequence starts at position 0: the context rows ARE the step's rows, in order
 
 
+@dataclass
+class PagedStep:
+    """Device-side description of one ragged step over paged caches (``kernels.attn_paged``), the same for every layer."""
+
+    seqs: torch.Tensor       # int32 (S, 4): first row, rows, keys in the cache before the step, row of the page table
+    row_pos: torch.Tensor    # int32 (n,)   position of each row (the rotation's; a cache that was cut down holds fewer keys)
+    row_seq: torch.Tensor    # int32 (n,)   index of each row's sequence in seqs, -1: a row of none
+    table: torch.Tensor      # int32 (S, pages)
+    max_rows: int            # bounds of a sequence's rows and of its keys behind the step
+    max_length: int
+
+
 def state_batch(seqs: Sequence[Tuple[int, int, int]], device: torch.device, extra: Sequence[int] = (),
                 positions: bool = False) -> Tuple[RaggedBatch, torch.Tensor]:
     """The description of a step for models that keep a state per slot.  `seqs`: per sequence (state slot, position of its first
