@@ -342,7 +342,7 @@ typedef struct b200_attn_paged_args {
 size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int n_groups, int head_size, int64_t max_rows, int64_t max_length, int key_weights);
 int b200_attn_paged(const b200_attn_paged_args* args, b200_stream_t stream);
 /* development / test knob: every sequence in the list of tiles (1), every one on the tensor memory (2; not with more than 128 heads a group), the list without
- * keeping its scores (3), by size (0); returns the previous setting.  Workspaces are sized for the setting at the time. */
+ * keeping its scores (3), single tokens without key_weights by clusters (4; up to 16 heads a group), by size (0); returns the previous setting.  Workspaces are sized for the setting at the time. */
 int b200_attn_paged_tune(int path);
 
 /* Sequences of a paged cache cut down to `keep` keys each, every group by itself: the first `first` keys, the last `recent` and, of those between, the ones with the largest

@@ -3,7 +3,7 @@
 // The rounding points are those of the model's step (lit_gpt/model.py:624-653, 767-773): q and k are bf16 after the rotation, the softmax is fp32 with a running maximum,
 // the result is rounded once.  A row that sees no key has a result of zero.
 //
-// Three launches: queries and new keys are turned and the new rows stored in their pages; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys;
+// Few single tokens: one launch, a cluster of CTAs for a sequence and group.  Else three: queries and new keys are turned and the new rows stored in their pages; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys;
 // a head's partial results are joined.  No counter or flag is left between calls, and two calls at a time share nothing.
 //
 // An item is a tile of queries of one sequence and group -- rows times heads of the group, row after row, so that the heads of a group share the keys that they read -- against the
@@ -475,6 +475,191 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   if (p.lse && lane == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h - gi * p.per] = sum > 0.f ? top + log2f(sum) : INFINITY;
 }
 
+// ---- few single tokens: a sequence and group's whole step by a cluster of CTAs, in one launch ----
+// Every CTA turns the group's heads itself; the cluster's warps share the tiles, the new key and value come into their tile from shared memory; behind the cluster's barrier its CTAs
+// join the results, a head at a time each.
+template <int HS, int NQ>
+struct ClSmem {
+  static constexpr int kWarps = 4, kUnit = kShTile * HS * 2, kWarp = 2 * kUnit, kQ = 8 * NQ * HS * 2;   // keys and values of a tile; a warp's results in their place
+  static constexpr int kBytes = kWarps * kWarp + kQ + 2 * HS * 2;
+  static_assert(8 * NQ * HS * 4 <= kWarp, "a warp's results");
+};
+
+template <int HS, int NQ>
+__global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_kernel(const PagedParams p, int ctas) {
+  using C = ClSmem<HS, NQ>;
+  constexpr int W = C::kWarps, V = HS / 32;
+  extern __shared__ __align__(128) uint8_t cl_smem[];
+  __shared__ float2 s_ml[W][8 * NQ], s_cta[8 * NQ];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x % ctas, item = blockIdx.x / ctas, gi = item % p.n_groups;
+  uint8_t* const s_q = cl_smem + W * C::kWarp;
+  uint8_t* const s_new = s_q + C::kQ;              // the new key, the new value
+  griddep_launch();
+  griddep_wait();
+  Tile t;
+  t.seq = paged_seq(p, item / p.n_groups);
+  // rows of no sequence
+  for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const int which = p.row_seq[row];
+    PagedSeq s = {};
+    if (which >= 0 && which < p.n_seqs) s = paged_seq(p, which);
+    if (row >= s.first && row - s.first < s.rows) continue;
+    for (int i = threadIdx.x; i < p.n_head * HS / 8; i += W * 32) reinterpret_cast<uint4*>(p.out + (int64_t)row * p.n_head * HS)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (t.seq.rows == 0) return;                     // (the whole cluster)
+  const int row = t.seq.first, key = t.seq.cached, step = ctas * W;
+  const Walk walk{p, nullptr, 0, 0};
+  t.gi = gi;
+  t.tiles = seq_tiles(t.seq);
+  t.tile = rank * W + warp;
+  const uint32_t kb = pf_smem(cl_smem) + warp * C::kWarp, vb = kb + C::kUnit;
+  // the new key is not read from its page: it comes from shared memory
+  const int fresh = key < t.seq.n && page_at(p, t.seq.table, key >> p.shift) >= 0 ? key : -1;
+  auto load = [&](const Tile& x, const __nv_bfloat16* base, int64_t page, int64_t group, uint32_t dst) {
+    Tile y = x;
+    y.seq.n = min(y.seq.n, key);
+    load_tile<HS>(p, y, base, page, group, dst, lane);
+    pf_commit();
+  };
+  if (t.tile < t.tiles) {
+    walk.locate(t);
+    load(t, p.k, p.k_page, p.k_group, kb);
+    load(t, p.v, p.v_page, p.v_group, vb);
+  }
+  const int64_t trow = paged_pos(p, row);
+  for (int h = warp; h < 8 * NQ + 2; h += W) {     // the queries (zeros behind them), the new key, the new value
+    uint32_t v[HS / 64];
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = 0u;
+    const int head = h < 8 * NQ ? h : p.per + h - 8 * NQ;
+    const __nv_bfloat16* const x = p.qkv + (((int64_t)row * p.n_groups + gi) * (p.per + 2) + head) * HS;
+    if (h < p.per || h == 8 * NQ) {
+      turned_part<HS>(p, x, trow, lane, v);
+    } else if (h == 8 * NQ + 1) {
+      const uint16_t* const u = reinterpret_cast<const uint16_t*>(x + lane * V);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) v[j] = (uint32_t)u[2 * j] | ((uint32_t)u[2 * j + 1] << 16);
+    }
+    auto store = [&](void* at) {
+      if constexpr (V == 4) *reinterpret_cast<uint2*>(at) = make_uint2(v[0], v[V / 2 - 1]);
+      else *reinterpret_cast<uint32_t*>(at) = v[0];
+    };
+    store(h < 8 * NQ ? s_q + sw<HS>(h, lane * V / 8) + lane * V % 8 * 2 : s_new + (h - 8 * NQ) * HS * 2 + lane * V * 2);
+    if (h >= 8 * NQ && rank == 0 && fresh >= 0) {
+      const int64_t id = page_at(p, t.seq.table, key >> p.shift), in = key & ((1 << p.shift) - 1);
+      store((h == 8 * NQ ? p.k + id * p.k_page + (int64_t)gi * p.k_group : p.v + id * p.v_page + (int64_t)gi * p.v_group) + in * HS + lane * V);
+    }
+  }
+  __syncthreads();
+  Sums<HS, NQ> a;
+#pragma unroll
+  for (int u = 0; u < NQ; ++u) {
+#pragma unroll
+    for (int i = 0; i < HS / 16; ++i) a.o[i][u][0] = a.o[i][u][1] = a.o[i][u][2] = a.o[i][u][3] = 0.f;
+    a.m[u][0] = a.m[u][1] = -INFINITY;
+    a.l[u][0] = a.l[u][1] = 0.f;
+  }
+  while (t.tile < t.tiles) {
+    Tile next = t;
+    next.tile += step;
+    const bool more = next.tile < t.tiles;
+    if (more) walk.locate(next);
+    const int at = fresh - t.key0();               // the new key's place in this tile
+    auto patch = [&](uint32_t dst, int which) {
+      if (at >= 0 && at < kShTile) {
+        if (lane < HS / 8) {
+          const uint4 x = *reinterpret_cast<const uint4*>(s_new + which * HS * 2 + lane * 16);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + sw<HS>(at, lane)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+        }
+        __syncwarp();
+      }
+    };
+    pf_wait<1>();
+    __syncwarp();
+    patch(kb, 0);
+    const uint32_t bits = t.bits();
+    attend_tile<HS, NQ, NQ>(a, pf_smem(s_q), 0, kb, p.scale_log2, lane, [bits](int k, int, int) { return ((bits >> k) & 1u) != 0u; }, [](int, int, int, float) {}, [&]() {
+      __syncwarp();
+      if (more) load(next, p.k, p.k_page, p.k_group, kb); else pf_commit();
+      pf_wait<1>();
+      __syncwarp();
+      patch(vb, 1);
+      return vb;
+    });
+    __syncwarp();
+    if (more) load(next, p.v, p.v_page, p.v_group, vb); else pf_commit();
+    t = next;
+  }
+  pf_wait<0>();
+  __syncwarp();
+  // ---- the CTA's results, then the cluster's ----
+  float* const mine = reinterpret_cast<float*>(cl_smem + warp * C::kWarp);
+  const int g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int u = 0; u < NQ; ++u)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = a.l[u][c];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const int h = u * 8 + 2 * tq + c;
+#pragma unroll
+      for (int i = 0; i < HS / 16; ++i) {
+        mine[h * HS + i * 16 + g] = a.o[i][u][c];
+        mine[h * HS + i * 16 + 8 + g] = a.o[i][u][2 + c];
+      }
+      if (g == 0) s_ml[warp][h] = make_float2(a.m[u][c], l);
+    }
+  __syncthreads();
+  float* const first = reinterpret_cast<float*>(cl_smem);
+  for (int i = threadIdx.x; i < p.per * HS; i += W * 32) {
+    const int h = i / HS;
+    float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][h].x);
+    const float org = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = ex2(s_ml[w][h].x - org);
+      sum += s_ml[w][h].y * f;
+      x += s_ml[w][h].y == 0.f ? 0.f : reinterpret_cast<const float*>(cl_smem + w * C::kWarp)[i] * f;   // (a warp that saw nothing has no result)
+    }
+    first[i] = x;                                  // (read by this thread alone)
+    if (i % HS == 0) s_cta[h] = make_float2(top, sum);
+  }
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+  auto remote = [](const void* at, int of) {
+    uint32_t ra;
+    float x;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(pf_smem(at)), "r"(of));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(ra) : "memory");
+    return x;
+  };
+  for (int i = rank * W * 32 + threadIdx.x; i < p.per * HS; i += ctas * W * 32) {
+    const int h = i / HS;
+    float m[8], l[8], x[8], top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool in = u < ctas;
+      m[u] = in ? remote(&s_cta[h].x, u) : -INFINITY;
+      l[u] = in ? remote(&s_cta[h].y, u) : 0.f;
+      x[u] = in ? remote(first + i, u) : 0.f;
+      top = fmaxf(top, m[u]);
+    }
+    const float org = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float f = ex2(m[u] - org);
+      sum += l[u] * f;
+      y += l[u] == 0.f ? 0.f : x[u] * f;
+    }
+    p.out[((int64_t)row * p.n_head + gi * p.per + h) * HS + i % HS] = __float2bfloat16_rn(sum > 0.f ? y / sum : 0.f);
+  }
+  // no CTA leaves, and frees its shared memory, before the others have read it
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // ---- the weight that the keys of the list's sequences receive: a tile of 32 keys a warp, a key a lane, from the scores that were kept ----
 __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
   constexpr int T = 256;
@@ -516,6 +701,7 @@ __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
 struct PagedPlan {
   int nq, ctas, workers, ways;
   bool list, tensor;               // which kernels there is work for
+  int cluster;                     // CTAs that a sequence and group's step takes in one launch; 0: the launches above
   int list_max, tc_workers;
   int64_t items, slots, q;
   int score_rows, kept_max, kw_workers;
@@ -531,8 +717,10 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   PagedPlan s;
   const int path = g_paged_path.load(std::memory_order_relaxed);
   // chunks of one length only: all go to the tensor memory (some of them may turn out shorter, or not there)
+  // 17 to 32 queries: 8 groups of 4 heads, us of the list and of the tensor memory: 8 rows behind 500 keys 13.7, 17.4, behind 16000 38, 32; 16 times 8 rows behind 300 22, 24, behind 3000 82, 61
+  const bool short_ = (int64_t)n_seqs * n_groups * max_length <= 60000;
   const int singles = per <= 8 ? 8 : per <= 16 ? 16 : kListMax;   // beside chunks the list takes single tokens, in items as small as they are
-  s.list_max = path == 1 || path == 3 || per > 128 ? 0x3fffffff : path == 2 ? 0 : max_rows * per <= kListMax ? kListMax : rows == (int64_t)n_seqs * max_rows ? 0 : singles;
+  s.list_max = path == 1 || path == 3 || per > 128 ? 0x3fffffff : path == 2 ? 0 : max_rows * per <= (short_ ? kListMax : 16) ? kListMax : rows == (int64_t)n_seqs * max_rows ? 0 : singles;
   s.tensor = max_rows * per > s.list_max;
   s.list = s.list_max > 0;
   const int64_t most = max_rows * per < s.list_max ? max_rows * per : s.list_max;   // queries of an item
@@ -563,6 +751,16 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   }
   s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * sizeof(int) +
             (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)s.scores * sizeof(float) + (size_t)s.kw_workers * (256 * sizeof(float) + sizeof(PagedWeightCut)) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
+  // A cluster where its warps have four tiles each at most, and all clusters run at once.  us of the list and of clusters: 1 token of 32 groups, 128 numbers a head, over 300 keys 12.9, 7.5, over
+  // 2000 13.6, 10.4, over 8000 30.6, 28.1; of 8 groups of 4 heads over 8000 16.6, 17.2; 16 tokens of 32 groups over 300 18.5, 19.5; 64 of 8 groups over 100 14.4, 15.4; of 12 groups, 64 numbers
+  // a head, over 500 22.5, 17.9; 16 of them over 1000 16.4, 17.9.
+  s.cluster = 0;
+  if (max_rows == 1 && !kw && most <= 16 && (path == 0 || path == 4)) {
+    const int64_t key_tiles = (max_length + kShTile - 1) / kShTile, pairs = (int64_t)n_seqs * n_groups;
+    int ctas = 1;
+    while (ctas < 8 && (ctas * 4 < key_tiles || ctas * 4 < per) && pairs * 2 * ctas <= 2 * sm_count()) ctas *= 2;   // (its CTAs share the heads' joins, too)
+    if (path == 4 || (key_tiles <= 16 * ctas && pairs * ctas <= (hs == 64 ? 6 : 3) * sm_count())) s.cluster = ctas;
+  }
   const int64_t results = 2 + (int64_t)s.workers / s.items;
   s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
   while (s.ways < 8 && results > 4 * s.ways && rows * n_groups * per * s.ways < 24 * sm_count()) s.ways *= 2;
@@ -584,8 +782,21 @@ cudaError_t launch_list_of(const PagedParams& p, const PagedPlan& s, cudaStream_
 template <int HS, int NQ>
 cudaError_t launch_list(const PagedParams& p, const PagedPlan& s, cudaStream_t st) { return p.scores ? launch_list_of<HS, NQ, true>(p, s, st) : launch_list_of<HS, NQ, false>(p, s, st); }
 
+template <int HS, int NQ>
+cudaError_t launch_clusters(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
+  using C = ClSmem<HS, NQ>;
+  static PerDeviceOnce once;
+  if (once.need()) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_cluster_kernel<HS, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (e != cudaSuccess) return e;
+    once.done();
+  }
+  return launch_cluster(paged_cluster_kernel<HS, NQ>, dim3((unsigned)(p.n_seqs * p.n_groups * s.cluster)), dim3(C::kWarps * 32), s.cluster, (size_t)C::kBytes, st, p, s.cluster);
+}
+
 template <int HS>
 cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
+  if (s.cluster) return s.nq == 1 ? launch_clusters<HS, 1>(p, s, st) : launch_clusters<HS, 2>(p, s, st);
   const int64_t warps = (int64_t)p.rows * p.n_groups * (p.per + 2);
   cudaError_t e;
   if (p.wide) {                    // few rows: a row's heads on several CTAs, as many as are at once
@@ -626,7 +837,7 @@ size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int
   return paged_plan(rows, n_seqs, n_groups, n_head / n_groups, head_size, max_rows, max_length, key_weights != 0).bytes;
 }
 
-int b200_attn_paged_tune(int path) { return g_paged_path.exchange(path >= 1 && path <= 3 ? path : 0); }
+int b200_attn_paged_tune(int path) { return g_paged_path.exchange(path >= 1 && path <= 4 ? path : 0); }
 
 int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a, "b200_attn_paged: null argument");

@@ -1052,7 +1052,7 @@ def attn_decode_shared_tune(path: int = 0) -> int:
 
 def attn_paged_tune(path: int = 0) -> int:
     """Test knob: every sequence of ``attn_paged`` in the list of tiles (1), every one on the tensor memory (2), the list without keeping its scores (3),
-    by size (0); returns the previous setting."""
+    single tokens without key_weights by clusters (4), by size (0); returns the previous setting."""
     _paged_workspace_bytes.cache_clear()
     return int(C.load().b200_attn_paged_tune(int(path)))
 

@@ -11,7 +11,7 @@ from paged_oracle import F64, make
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(params=["list", "tensor memory", "list without scores", "by size"])
+@pytest.fixture(params=["list", "tensor memory", "list without scores", "clusters", "by size"])
 def path(request):
     return request.param
 
@@ -23,7 +23,7 @@ def K(path):
         pytest.skip("needs a CUDA device")
     from lit_gpt_b200 import kernels
 
-    before = kernels.attn_paged_tune({"list": 1, "tensor memory": 2, "list without scores": 3, "by size": 0}[path])
+    before = kernels.attn_paged_tune({"list": 1, "tensor memory": 2, "list without scores": 3, "clusters": 4, "by size": 0}[path])
     yield kernels
     kernels.attn_paged_tune(before)
 
@@ -86,6 +86,21 @@ MIXED = [(1, 40), (5, 0), (0, 7), (17, 33), (1, 0), (40, 129), (2, 300)]
 def test_formula(K, formula, hs, groups, per, page, steps):
     d = make(steps, groups, per, hs, page, seed=page + per)
     check(call(K, d), formula(d))
+
+
+@pytest.mark.parametrize("hs,groups,per", [(64, 1, 1), (128, 3, 4), (64, 2, 8), (128, 2, 9), (64, 1, 16), (128, 2, 1)])
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("cached", [[0], [1, 31, 32], [500], [900, 0, 63, 1300, 64], [127] * 9])
+def test_single_tokens_without_weights(K, formula, hs, groups, per, page, cached):
+    d = make([(1, n) for n in cached], groups, per, hs, page, weights=False, seed=len(cached))
+    check(call(K, d), formula(d))
+    d["seqs"][0, 1] = 0                         # a sequence without a row, a row without a sequence
+    d["row_seq"][0] = -1
+    check(call(K, d), formula(d))
+    if len(cached) > 1:
+        d["pages"][d["seqs"][1, 3], 0] = -1     # a missing page
+        d["pages"][d["seqs"][-1, 3], (cached[-1]) // page] = 2 ** 30   # the new key's
+        check(call(K, d), formula(d))
 
 
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 65, 127, 128, 129, 200, 257])
