@@ -326,7 +326,8 @@ int b200_attn_decode_shared_tune(int path);
  *              weights over the step's rows and its group's heads.
  *   max_rows, max_length   bounds of a sequence's rows and of its keys behind the step: they size the work; keys from max_length on are dropped
  *   cos, sin   (table_rows, rope_n_elem), row = position; table_preselected: row = row of qkv
- * head_size 64 or 128.  out on a 16-byte boundary.  No page belongs to two sequences that bring rows into it.  The workspace needs no initial contents; two calls that run at the same time need one each. */
+ * head_size 64 or 128.  out on a 16-byte boundary.  No page belongs to two sequences that bring rows into it.  The workspace needs no initial contents; two calls that run at the same time need one each
+ * (small steps need none: 0 bytes). */
 typedef struct b200_attn_paged_args {
   const void* qkv;
   const void* cos; const void* sin; int table_dtype, table_rows, table_preselected, rope_n_elem;
@@ -359,7 +360,7 @@ typedef struct b200_evict_paged_args {
   int n_groups, head_size; int64_t keep, first, recent, max_length;
   void* workspace; size_t workspace_bytes;
 } b200_evict_paged_args;
-size_t b200_evict_paged_workspace_bytes(int n_seqs, int n_groups, int64_t keep);
+size_t b200_evict_paged_workspace_bytes(int n_seqs, int n_groups, int64_t keep, int64_t max_length, int page);   /* 0: none is needed */
 int b200_evict_paged(const b200_evict_paged_args* args, b200_stream_t stream);
 
 /* ---- prefill helper: RoPE + KV-cache write for T > 1 tokens at positions pos[0..T) (lit_gpt/model.py:624-649).

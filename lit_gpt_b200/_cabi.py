@@ -169,12 +169,18 @@ class AttnPagedArgs(ctypes.Structure):  # mirrors b200_attn_paged_args
                 ("n_groups", c_int), ("head_size", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+ATTN_PAGED_PACKED = "@PPPiiiiPiPPiPqiiiiPPqqqqPPqqqiiiPN"   # the same fields for struct.pack: a third of the time that the structure takes
+
+
 class EvictPagedArgs(ctypes.Structure):  # mirrors b200_evict_paged_args
     _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_page_stride", c_int64), ("k_group_stride", c_int64), ("v_page_stride", c_int64),
                 ("v_group_stride", c_int64), ("key_weights", c_void_p), ("pages", c_void_p), ("pages_ld", c_int64), ("table_seqs", c_int), ("max_pages", c_int),
                 ("pool", c_int), ("page", c_int), ("lengths", c_void_p), ("rows", c_void_p), ("lengths_out", c_void_p), ("n_seqs", c_int), ("n_groups", c_int),
                 ("head_size", c_int), ("keep", c_int64), ("first", c_int64), ("recent", c_int64), ("max_length", c_int64), ("workspace", c_void_p),
                 ("workspace_bytes", c_size_t)]
+
+
+EVICT_PAGED_PACKED = "@PPqqqqPPqiiiiPPPiiiqqqqPN"
 
 
 class LogitRules(ctypes.Structure):  # mirrors b200_logit_rules
@@ -326,10 +332,10 @@ _SIGNATURES = {
     "b200_attn_decode_shared_tune": (c_int, [c_int]),
     "b200_attn_decode_shared": (c_int, [ctypes.POINTER(AttnDecodeSharedArgs), c_void_p]),
     "b200_attn_paged_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]),
-    "b200_attn_paged": (c_int, [ctypes.POINTER(AttnPagedArgs), c_void_p]),
+    "b200_attn_paged": (c_int, [c_void_p, c_void_p]),   # AttnPagedArgs, by reference or packed
     "b200_attn_paged_tune": (c_int, [c_int]),
-    "b200_evict_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int64]),
-    "b200_evict_paged": (c_int, [ctypes.POINTER(EvictPagedArgs), c_void_p]),
+    "b200_evict_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64, c_int]),
+    "b200_evict_paged": (c_int, [c_void_p, c_void_p]),  # EvictPagedArgs, likewise
     "b200_rope_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "b200_attn_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -761,6 +761,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
     while (ctas < 8 && (ctas * 4 < key_tiles || ctas * 4 < per) && pairs * 2 * ctas <= 2 * sm_count()) ctas *= 2;   // (its CTAs share the heads' joins, too)
     if (path == 4 || (key_tiles <= 16 * ctas && pairs * ctas <= (hs == 64 ? 6 : 3) * sm_count())) s.cluster = ctas;
   }
+  if (s.cluster) s.bytes = 0;
   const int64_t results = 2 + (int64_t)s.workers / s.items;
   s.ways = 1;                      // four results a warp are one round; no more warps than the GPU has at once
   while (s.ways < 8 && results > 4 * s.ways && rows * n_groups * per * s.ways < 24 * sm_count()) s.ways *= 2;
@@ -850,7 +851,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a->pool > 0 && a->table_seqs > 0 && a->max_pages > 0 && a->pages_ld >= a->max_pages, "b200_attn_paged: no pages, or a bad page table");
   B200_CHECK_ARG(a->max_length > 0 && a->max_length <= (int64_t)a->max_pages * a->page && a->max_length < (1 << 30), "b200_attn_paged: %lld keys in %d pages of %d",
                  (long long)a->max_length, a->max_pages, a->page);
-  B200_CHECK_ARG(a->qkv && a->row_pos && a->row_seq && a->seqs && a->pages && a->k_pages && a->v_pages && a->out && a->workspace, "b200_attn_paged: null pointer");
+  B200_CHECK_ARG(a->qkv && a->row_pos && a->row_seq && a->seqs && a->pages && a->k_pages && a->v_pages && a->out, "b200_attn_paged: null pointer");
   B200_CHECK_ARG(a->rope_n_elem >= 0 && a->rope_n_elem <= a->head_size && a->rope_n_elem % 2 == 0, "b200_attn_paged: bad rope_n_elem %d", a->rope_n_elem);
   B200_CHECK_ARG(a->rope_n_elem == 0 || (a->cos && a->sin && a->table_rows > 0), "b200_attn_paged: no tables");
   B200_CHECK_ARG(!a->table_preselected || a->rope_n_elem == 0 || a->table_rows >= a->rows, "b200_attn_paged: %d preselected table rows for %lld rows", a->table_rows, (long long)a->rows);
@@ -862,7 +863,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   const int per = a->n_head / a->n_groups;
   const PagedPlan s = paged_plan(a->rows, a->n_seqs, a->n_groups, per, a->head_size, a->max_rows, a->max_length, a->key_weights != nullptr);
   B200_CHECK_ARG(s.items * ((a->max_length + kShTile - 1) / kShTile) < kMaxTiles, "b200_attn_paged: too many keys in a step");
-  B200_CHECK_ARG(a->workspace_bytes >= s.bytes, "b200_attn_paged: workspace too small");
+  B200_CHECK_ARG(a->workspace_bytes >= s.bytes && (a->workspace || s.bytes == 0), "b200_attn_paged: workspace too small");
   if (s.tensor || s.kw_workers > 0) B200_CHECK_WAITS("b200_attn_paged");
   PagedParams p = {};
   p.qkv = (const __nv_bfloat16*)a->qkv;

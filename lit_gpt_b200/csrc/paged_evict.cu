@@ -1,13 +1,14 @@
 // Sequences of a paged key-value cache cut down by the attention weight that their keys have received: per sequence and group the first, the last and the heaviest keys stay, in order, at
 // the front of the sequence's pages.
 //
-// Two launches.  paged_choose_kernel, a CTA per sequence and group: the smallest weight that stays by radix selection over the weights as ordered whole numbers; then the indices that
-// stay, in order, by a scan, and their weights moved.  Weights that fit are held in shared memory: read once, eleven bits a digit, one scan of a run of keys a thread; longer sequences'
-// are read for every digit, eight bits each, and scanned in rounds.  paged_move_kernel: keys and values moved in place, a cluster of CTAs per sequence, group and tensor.
-// A key moves to a lower index or stays: a cluster that goes through its rows in order, reads a tile of them before it writes them, and has a barrier between, never writes what is still
-// to be read.
+// One launch where a sequence's weights, places and pages fit into shared memory: a cluster of CTAs per sequence and group.  Every CTA finds the smallest weight that stays by radix
+// selection over the weights as ordered whole numbers (11, 11 and 10 bits) and the places that stay by a scan, a run of keys a thread; then the cluster moves keys, values and
+// weights in place.  A key moves to a lower index or stays: a cluster that goes through its rows in order, reads a tile of them before it writes them, and has a barrier between, never
+// writes what is still to be read.  Longer sequences: a launch that chooses (weights read for every digit, eight bits each, and scanned in rounds), a launch that moves.
 //
-// Bound: bytes of the rows that stay, read and written.
+// Bound: bytes of the rows that stay, read and written, behind the choice, which is a chain on one SM.  us in a captured graph: 1 sequence of 32 groups cut from 576 keys to 512 9.4 (choice and
+// move in two launches 14.3); 16 of 8 groups from 3001 - 8001 to 2048 59, 4.6 TB/s (two launches 77; pieces of 32 bytes of a row a CTA 119); 1 of 12 groups, 64 numbers a head,
+// from 30001 to 8191 38, about 22 of them the choice (weights not held 151).  512 threads with twice the rows each: 62 and 50.
 #include "common.cuh"
 
 namespace b200 {
@@ -121,8 +122,10 @@ __global__ void __launch_bounds__(kChThreads) paged_choose_kernel(const EvictPar
 // ---- the same with the sequence's weights, and the places that stay, in shared memory ----
 constexpr int kBins = 2048, kBinCopies = 2;
 
-// a's sum over the threads before this one; `all`: over all of them
-__device__ __forceinline__ int block_before(int a, int* s_warp, int& all) {
+// a's sum over the threads before this one
+template <int THREADS>
+__device__ __forceinline__ int block_before(int a, int* s_warp) {
+  constexpr int WARPS = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = a;
 #pragma unroll
@@ -130,44 +133,40 @@ __device__ __forceinline__ int block_before(int a, int* s_warp, int& all) {
   __syncthreads();                                 // (s_warp has been read)
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
-  int w = s_warp[lane];                            // (as many warps as lanes)
+  int w = lane < WARPS ? s_warp[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += t; }
-  all = __shfl_sync(0xffffffffu, w, 31);
+  for (int o = 1; o < WARPS; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += t; }
   const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
   return inc - a + (warp ? before : 0);
 }
 
-__global__ void __launch_bounds__(kChThreads) paged_choose_smem_kernel(const EvictParams p) {
-  extern __shared__ __align__(16) float ch_smem[];
-  float* const s_w = ch_smem;                                       // [max_length]
-  int* const s_from = reinterpret_cast<int*>(ch_smem + p.max_length);   // [keep]
-  int* const s_table = s_from + p.keep;                             // the sequence's pages
+struct Held {                                      // in dynamic shared memory
+  float* w;                                        // [max_length] weights
+  int* from;                                       // [keep] where what moves to each place comes from
+  int* table;                                      // the sequence's pages
+};
+
+// By a whole CTA: whether the sequence is cut down; if so, its pages, its weights and the places that stay.
+template <int THREADS>
+__device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const Held& h) {
   __shared__ int s_hist[kBinCopies * kBins];
-  __shared__ int s_warp[kChWarps], s_pick[2];
-  griddep_wait();
-  griddep_launch();
-  const int tid = threadIdx.x, warp = tid >> 5, s = blockIdx.x / p.n_groups, g = blockIdx.x - s * p.n_groups, page = 1 << p.shift;
+  __shared__ int s_warp[THREADS / 32], s_pick[2];
+  const int tid = threadIdx.x, warp = tid >> 5, page = 1 << p.shift;
   const int n = p.lengths[s], row = p.rows ? p.rows[s] : s;
   bool cut = n > p.keep && n <= p.max_length && row >= 0 && row < p.table_seqs;
-  const int* const table = p.pages + (int64_t)(cut ? row : 0) * p.pages_ld;
-  if (cut) {
-    bool all = true;
-    for (int i = tid; i < (n + page - 1) >> p.shift; i += kChThreads) {
-      const int id = table[i];
-      s_table[i] = id;
-      all = all && id >= 0 && id < p.pool;
-    }
-    cut = __syncthreads_and(all);
+  if (!cut) return false;
+  const int* const table = p.pages + (int64_t)row * p.pages_ld;
+  bool all = true;
+#pragma unroll 4
+  for (int i = tid; i < (n + page - 1) >> p.shift; i += THREADS) {
+    const int id = table[i];
+    h.table[i] = id;
+    all = all && id >= 0 && id < p.pool;
   }
-  if (g == 0 && tid == 0) {
-    p.lengths_out[s] = cut ? p.keep : n;
-    p.moved[s] = cut ? p.keep : 0;
-  }
-  if (!cut) return;
-  auto at = [&](int i) -> float* { return p.kw + (((int64_t)s_table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1)); };
+  cut = __syncthreads_and(all);
+  if (!cut) return false;
 #pragma unroll 8
-  for (int i = tid; i < n; i += kChThreads) s_w[i] = *at(i);
+  for (int i = tid; i < n; i += THREADS) h.w[i] = p.kw[(((int64_t)h.table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1))];
   const int lo = p.first, hi = n - p.recent;
   int need = p.keep - p.first - p.recent;
   const bool any = need > 0;
@@ -175,21 +174,28 @@ __global__ void __launch_bounds__(kChThreads) paged_choose_smem_kernel(const Evi
   // digits of 11, 11 and 10 bits
   for (int digit = 0; digit < 3 && any; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-    for (int i = tid; i < kBinCopies * kBins; i += kChThreads) s_hist[i] = 0;
+    for (int i = tid; i < kBinCopies * kBins; i += THREADS) s_hist[i] = 0;
     __syncthreads();                               // (and: the weights are there)
-    for (int i = lo + tid; i < hi; i += kChThreads) {
-      const uint32_t u = ordered(s_w[i]);
+#pragma unroll 4
+    for (int i = lo + tid; i < hi; i += THREADS) {
+      const uint32_t u = ordered(h.w[i]);
       if (digit == 0 || u >> (shift + bits) == high) atomicAdd(&s_hist[warp % kBinCopies * kBins + ((u >> shift) & ((1u << bits) - 1u))], 1);
     }
     __syncthreads();
-    // a thread has two digits, the greater ones first
-    const int top = kBins - 1 - 2 * tid;
-    int c[2] = {0, 0}, all;
+    // a thread has some digits next to each other, the greater ones first
+    constexpr int D = kBins / THREADS;
+    const int top = kBins - 1 - D * tid;
+    int c[D], sum = 0;
 #pragma unroll
-    for (int k = 0; k < kBinCopies; ++k) { c[0] += s_hist[k * kBins + top]; c[1] += s_hist[k * kBins + top - 1]; }
-    int before = block_before(c[0] + c[1], s_warp, all);
+    for (int j = 0; j < D; ++j) {
+      c[j] = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+      for (int k = 0; k < kBinCopies; ++k) c[j] += s_hist[k * kBins + top - j];
+      sum += c[j];
+    }
+    int before = block_before<THREADS>(sum, s_warp);
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
       if (before < need && need <= before + c[j]) { s_pick[0] = top - j; s_pick[1] = need - before; }
       before += c[j];
     }
@@ -198,30 +204,93 @@ __global__ void __launch_bounds__(kChThreads) paged_choose_smem_kernel(const Evi
     need = s_pick[1];
     __syncthreads();
   }
+  if (!any) __syncthreads();                       // (the weights are there)
   // a run of keys a thread: those above, and the first `need` of those that equal it
-  const int run = (n + kChThreads - 1) / kChThreads, begin = min(n, tid * run), end = min(n, begin + run);
-  int above = 0, ties = 0, all;
+  const int run = (n + THREADS - 1) / THREADS, begin = min(n, tid * run), end = min(n, begin + run);
+  int above = 0, ties = 0;
   for (int i = begin; i < end; ++i) {
-    const uint32_t u = ordered(s_w[i]);
+    const uint32_t u = ordered(h.w[i]);
     const bool mid = i >= lo && i < hi;
     above += !mid || (any && u > high);
     ties += mid && any && u == high;
   }
-  const int above_before = block_before(above, s_warp, all);
-  int equal = block_before(ties, s_warp, all), place = above_before + min(equal, need);
+  const int above_before = block_before<THREADS>(above, s_warp);
+  int equal = block_before<THREADS>(ties, s_warp), place = above_before + min(equal, need);
   for (int i = begin; i < end; ++i) {
-    const uint32_t u = ordered(s_w[i]);
+    const uint32_t u = ordered(h.w[i]);
     const bool mid = i >= lo && i < hi, tie = mid && any && u == high;
-    if (!mid || (any && u > high) || (tie && equal < need)) s_from[place++] = i;
+    if (!mid || (any && u > high) || (tie && equal < need)) h.from[place++] = i;
     equal += tie;
   }
   __syncthreads();
-  int* const from = p.from + (int64_t)blockIdx.x * p.keep;
-#pragma unroll 8
-  for (int d = tid; d < p.keep; d += kChThreads) {
-    const int i = s_from[d];
-    from[d] = i;
-    *at(d) = s_w[i];
+  return true;
+}
+__device__ __forceinline__ Held held_of(const EvictParams& p, float* smem) {
+  Held h;
+  h.w = smem;
+  h.from = reinterpret_cast<int*>(smem + p.max_length);
+  h.table = h.from + p.keep;
+  return h;
+}
+
+// ---- the whole of it in one launch ----
+// A cluster of CTAs per sequence and group: each of them chooses for itself, from weights that all have read before the first is written; then they share the rows.
+constexpr int kEvThreads = 1024, kEvUnroll = 2;
+
+template <int LANES>
+__global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const EvictParams p, int ctas) {
+  extern __shared__ __align__(16) float ev_smem[];
+  griddep_launch();
+  griddep_wait();
+  const int tid = threadIdx.x, rank = blockIdx.x % ctas, item = blockIdx.x / ctas, s = item / p.n_groups, g = item - s * p.n_groups, page = 1 << p.shift;
+  const Held h = held_of(p, ev_smem);
+  const bool cut = choose<kEvThreads>(p, s, g, h);
+  if (g == 0 && rank == 0 && tid == 0) p.lengths_out[s] = cut ? p.keep : p.lengths[s];
+  if (!cut) return;                                // (the whole cluster)
+  const float* const s_w = h.w;
+  const int* const s_from = h.from;
+  const int* const s_table = h.table;
+  auto at = [&](int i) -> float* { return p.kw + (((int64_t)s_table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1)); };
+  // ---- the rows.  A tile is read while the one before it is still in registers: its rows lie behind all places of that one ----
+  constexpr int ROWS = kEvThreads / LANES, TILE = ROWS * kEvUnroll;   // at once; of a tile
+  const int keep = p.keep, hs = LANES * 8, first = rank * TILE + tid / LANES, step = ctas * TILE, lane8 = tid % LANES * 8;
+  __nv_bfloat16* const kg = p.k + (int64_t)g * p.k_group + lane8;
+  __nv_bfloat16* const vg = p.v + (int64_t)g * p.v_group + lane8;
+  auto key_at = [&](int i) { return reinterpret_cast<uint4*>(kg + (int64_t)s_table[i >> p.shift] * p.k_page + (i & (page - 1)) * hs); };
+  auto value_at = [&](int i) { return reinterpret_cast<uint4*>(vg + (int64_t)s_table[i >> p.shift] * p.v_page + (i & (page - 1)) * hs); };
+  uint4 kx[kEvUnroll], vx[kEvUnroll];
+  auto load = [&](int d0) {
+#pragma unroll
+    for (int j = 0; j < kEvUnroll; ++j) {
+      const int d = d0 + first + j * ROWS;
+      if (d < keep) {
+        const int f = s_from[d];
+        kx[j] = *key_at(f);
+        vx[j] = *value_at(f);
+      }
+    }
+  };
+  load(0);
+  for (int d0 = 0; d0 < keep; d0 += step) {        // (as many rounds in every thread)
+    uint4 ky[kEvUnroll], vy[kEvUnroll];
+#pragma unroll
+    for (int j = 0; j < kEvUnroll; ++j) { ky[j] = kx[j]; vy[j] = vx[j]; }
+    load(d0 + step);
+    // this tile, and the first time the weights, have been read by all
+    if (ctas == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (d0 == 0) {
+#pragma unroll 4
+      for (int d = rank * kEvThreads + tid; d < keep; d += ctas * kEvThreads) *at(d) = s_w[s_from[d]];
+    }
+#pragma unroll
+    for (int j = 0; j < kEvUnroll; ++j) {
+      const int d = d0 + first + j * ROWS;
+      if (d < keep) {
+        *key_at(d) = ky[j];
+        *value_at(d) = vy[j];
+      }
+    }
   }
 }
 
@@ -278,7 +347,10 @@ __global__ void __launch_bounds__(kMvThreads) paged_move_kernel(const EvictParam
 
 constexpr int kHeldMax = 200 * 1024;              // shared memory for weights, places and pages
 
-size_t evict_bytes(int n_seqs, int n_groups, int64_t keep) { return ((size_t)n_seqs * n_groups * keep + n_seqs) * sizeof(int); }
+int64_t evict_held(int64_t max_length, int64_t keep, int page) { return (max_length + keep + (max_length + page - 1) / page) * 4; }
+size_t evict_bytes(int n_seqs, int n_groups, int64_t keep, int64_t max_length, int page) {
+  return evict_held(max_length, keep, page) <= kHeldMax ? 0 : ((size_t)n_seqs * n_groups * keep + n_seqs) * sizeof(int);
+}
 
 }  // namespace
 }  // namespace b200
@@ -287,9 +359,9 @@ using namespace b200;
 
 extern "C" {
 
-size_t b200_evict_paged_workspace_bytes(int n_seqs, int n_groups, int64_t keep) {
-  if (n_seqs <= 0 || n_groups <= 0 || keep <= 0 || keep >= (1 << 30)) return 0;
-  return evict_bytes(n_seqs, n_groups, keep);
+size_t b200_evict_paged_workspace_bytes(int n_seqs, int n_groups, int64_t keep, int64_t max_length, int page) {
+  if (n_seqs <= 0 || n_groups <= 0 || keep <= 0 || keep >= max_length || max_length >= (1 << 30) || page <= 0) return 0;
+  return evict_bytes(n_seqs, n_groups, keep, max_length, page);
 }
 
 int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
@@ -303,7 +375,7 @@ int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
                  (long long)a->max_length, a->max_pages, a->page);
   B200_CHECK_ARG(a->keep > 0 && a->first >= 0 && a->recent >= 0 && a->first <= a->keep && a->recent <= a->keep - a->first, "b200_evict_paged: %lld first and %lld recent keys of %lld to keep",
                  (long long)a->first, (long long)a->recent, (long long)a->keep);
-  B200_CHECK_ARG(a->k_pages && a->v_pages && a->key_weights && a->pages && a->lengths && a->lengths_out && a->workspace, "b200_evict_paged: null pointer");
+  B200_CHECK_ARG(a->k_pages && a->v_pages && a->key_weights && a->pages && a->lengths && a->lengths_out, "b200_evict_paged: null pointer");
   B200_CHECK_ARG(a->lengths != a->lengths_out, "b200_evict_paged: lengths_out in the place of lengths");
   B200_CHECK_ARG((((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0 && ((a->k_page_stride | a->k_group_stride | a->v_page_stride | a->v_group_stride) & 7) == 0 &&
                      (((uintptr_t)a->key_weights | (uintptr_t)a->workspace) & 3) == 0,
@@ -312,7 +384,8 @@ int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
     B200_CUDA(cudaMemcpyAsync(a->lengths_out, a->lengths, sizeof(int) * (size_t)a->n_seqs, cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
     return B200_OK;
   }
-  B200_CHECK_ARG(a->workspace_bytes >= evict_bytes(a->n_seqs, a->n_groups, a->keep), "b200_evict_paged: workspace too small");
+  const size_t need = evict_bytes(a->n_seqs, a->n_groups, a->keep, a->max_length, a->page);
+  B200_CHECK_ARG(a->workspace_bytes >= need && (a->workspace || need == 0), "b200_evict_paged: workspace too small");
   EvictParams p = {};
   p.k = (__nv_bfloat16*)a->k_pages; p.v = (__nv_bfloat16*)a->v_pages;
   p.k_page = a->k_page_stride; p.k_group = a->k_group_stride; p.v_page = a->v_page_stride; p.v_group = a->v_group_stride;
@@ -325,19 +398,25 @@ int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
   p.moved = p.from + (int64_t)a->n_seqs * a->n_groups * a->keep;
   const cudaStream_t st = (cudaStream_t)stream;
   const unsigned items = (unsigned)(a->n_seqs * a->n_groups);
-  const int64_t held = (a->max_length + a->keep + (a->max_length + a->page - 1) / a->page) * 4;
+  const int lanes = a->head_size / 8;
+  const int64_t held = evict_held(a->max_length, a->keep, a->page);
   if (held <= kHeldMax) {
     static PerDeviceOnce once;
     if (once.need()) {
-      B200_CUDA(cudaFuncSetAttribute(paged_choose_smem_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
+      B200_CUDA(cudaFuncSetAttribute(paged_evict_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
+      B200_CUDA(cudaFuncSetAttribute(paged_evict_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
       once.done();
     }
-    B200_CUDA(launch(paged_choose_smem_kernel, dim3(items), dim3(kChThreads), (size_t)held, st, p));
-  } else {
-    B200_CUDA(launch(paged_choose_kernel, dim3(items), dim3(kChThreads), 0, st, p));
+    // as many CTAs for a sequence and group as the SMs take at once, no more than they have tiles
+    const int tile = kEvThreads / lanes * kEvUnroll;
+    int ctas = 1;
+    while (ctas < 8 && (int64_t)items * ctas * 2 <= sm_count() && ctas * tile < a->keep) ctas *= 2;
+    B200_CUDA(launch_cluster(lanes == 8 ? paged_evict_kernel<8> : paged_evict_kernel<16>, dim3(items * ctas), dim3(kEvThreads), ctas, (size_t)held, st, p, ctas));
+    return B200_OK;
   }
+  B200_CUDA(launch(paged_choose_kernel, dim3(items), dim3(kChThreads), 0, st, p));
   // as many CTAs for the rows of one tensor as leave none of the SMs without, no more than they have tiles
-  const int lanes = a->head_size / 8, tile = kMvThreads / lanes * kMvUnroll;
+  const int tile = kMvThreads / lanes * kMvUnroll;
   int ctas = 1;
   while (ctas < 8 && (int64_t)items * 2 * ctas < sm_count() && ctas * tile < a->keep) ctas *= 2;
   B200_CUDA(launch_cluster(lanes == 8 ? paged_move_kernel<8> : paged_move_kernel<16>, dim3(items * ctas, 2), dim3(kMvThreads), ctas, 0, st, p, ctas));

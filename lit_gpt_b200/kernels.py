@@ -894,17 +894,19 @@ def _pages_of(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, key_weigh
     if len(shape) != 4 or shape != v_pages.shape or shape[1] != n_groups or shape[3] != head_size or k_pages.dtype is not bf16 or v_pages.dtype is not bf16:
         raise C.B200Error(f"{what}: pages must be bfloat16 (pages, {n_groups}, page, {head_size}) (got {k_pages.dtype}, {tuple(shape)}, {v_pages.dtype}, {tuple(v_pages.shape)})")
     pool, G, page, hs = shape
-    kp, kg, kr, ke = k_pages.stride()
-    vp, vg, vr, ve = v_pages.stride()
-    if ke != 1 or ve != 1 or kr != hs or vr != hs:
-        raise C.B200Error(f"{what}: the rows of a page must lie next to each other")
-    for a, b in ((kp, kg), (vp, vg)):   # (a tensor of one page or group may have any distance)
-        if (G > 1 and b < page * hs) or (pool > 1 and a < page * hs) or (G > 1 and pool > 1 and a < (G - 1) * b + page * hs and b < (pool - 1) * a + page * hs):
+    strides = k_pages.stride()
+    values = v_pages.stride()
+    for kp, kg, kr, ke in (strides,) if values == strides else (strides, values):
+        if ke != 1 or kr != hs:
+            raise C.B200Error(f"{what}: the rows of a page must lie next to each other")
+        # (a tensor of one page or group may have any distance)
+        if (G > 1 and kg < page * hs) or (pool > 1 and kp < page * hs) or (G > 1 and pool > 1 and kp < (G - 1) * kg + page * hs and kg < (pool - 1) * kp + page * hs):
             raise C.B200Error(f"{what}: pages or groups overlap")
     if key_weights is not None and (key_weights.dtype is not torch.float32 or key_weights.shape != (pool, G, page) or not key_weights.is_contiguous()):
         raise C.B200Error(f"{what}: key_weights must be contiguous fp32 ({pool}, {G}, {page}) (got {key_weights.dtype}, {tuple(key_weights.shape)})")
     if table.dtype is not torch.int32 or table.dim() != 2 or table.numel() == 0 or (table.shape[1] > 1 and table.stride(1) != 1) or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
         raise C.B200Error(f"{what}: the page table must be int32 (sequences, pages), the entries of a sequence next to each other (got {table.dtype}, {tuple(table.shape)})")
+    (kp, kg, _, _), (vp, vg, _, _) = strides, values
     return pool, page, kp if pool > 1 else 0, kg if G > 1 else 0, vp if pool > 1 else 0, vg if G > 1 else 0
 
 
@@ -953,14 +955,14 @@ def attn_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, row_pos:
     if seqs.data_ptr() % 16:
         seqs = seqs.clone()
     table_rows = cos.numel() // max(rope_n_elem, 1)
-    nbytes = _paged_workspace_bytes(device, rows, seqs.shape[0], n_head, n_groups, head_size, max_rows, max_length, key_weights is not None)
-    ws = qkv.new_empty(max(nbytes // 2, 8))   # of this call: calls on two streams, or in two graphs, have one each
-    args = C.AttnPagedArgs(
-        qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, row_pos.data_ptr(), kind is torch.int64, row_seq.data_ptr(),
-        seqs.data_ptr(), seqs.shape[0], table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[0], table.shape[1], pool, page, k_pages.data_ptr(),
-        v_pages.data_ptr(), kp, kg, vp, vg, None if key_weights is None else key_weights.data_ptr(), out.data_ptr(), rows, max_rows, max_length, n_head, n_groups, head_size,
-        ws.data_ptr(), nbytes)
-    C.check(C.load().b200_attn_paged(ctypes.byref(args), _raw_stream(device)), "attn_paged")
+    n_seqs, (table_seqs, max_pages) = seqs.shape[0], table.shape
+    nbytes = _paged_workspace_bytes(device, rows, n_seqs, n_head, n_groups, head_size, max_rows, max_length, key_weights is not None)
+    ws = qkv.new_empty(nbytes // 2) if nbytes else None   # of this call: calls on two streams, or in two graphs, have one each
+    args = struct.pack(C.ATTN_PAGED_PACKED, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), _table_code(cos), table_rows, table_preselected, rope_n_elem, row_pos.data_ptr(),
+                       kind is torch.int64, row_seq.data_ptr(), seqs.data_ptr(), n_seqs, table.data_ptr(), table.stride(0) if table_seqs > 1 else max_pages, table_seqs, max_pages, pool,
+                       page, k_pages.data_ptr(), v_pages.data_ptr(), kp, kg, vp, vg, 0 if key_weights is None else key_weights.data_ptr(), out.data_ptr(), rows, max_rows, max_length,
+                       n_head, n_groups, head_size, 0 if ws is None else ws.data_ptr(), nbytes)
+    C.check(C.load().b200_attn_paged(args, _raw_stream(device)), "attn_paged")
     return out
 
 
@@ -996,12 +998,14 @@ def evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, key_weights: torch
     if S == 0:
         return out
     lengths, rows = lengths.contiguous(), None if rows is None else rows.contiguous()
-    nbytes = int(C.load().b200_evict_paged_workspace_bytes(S, G, keep))
-    ws = k_pages.new_empty(max(nbytes // 2, 8))
-    args = C.EvictPagedArgs(k_pages.data_ptr(), v_pages.data_ptr(), kp, kg, vp, vg, key_weights.data_ptr(), table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1],
-                            table.shape[0], table.shape[1], pool, page, lengths.data_ptr(), None if rows is None else rows.data_ptr(), out.data_ptr(), S, G, hs, keep, first, recent,
-                            max_length, ws.data_ptr(), nbytes)
-    C.check(C.load().b200_evict_paged(ctypes.byref(args), _raw_stream(device)), "evict_paged")
+    lib = C.load()
+    nbytes = lib.b200_evict_paged_workspace_bytes(S, G, keep, max_length, page)
+    ws = k_pages.new_empty(nbytes // 2) if nbytes else None   # of this call
+    table_seqs, max_pages = table.shape
+    args = struct.pack(C.EVICT_PAGED_PACKED, k_pages.data_ptr(), v_pages.data_ptr(), kp, kg, vp, vg, key_weights.data_ptr(), table.data_ptr(),
+                       table.stride(0) if table_seqs > 1 else max_pages, table_seqs, max_pages, pool, page, lengths.data_ptr(), 0 if rows is None else rows.data_ptr(), out.data_ptr(), S, G,
+                       hs, keep, first, recent, max_length, 0 if ws is None else ws.data_ptr(), nbytes)
+    C.check(lib.b200_evict_paged(args, _raw_stream(device)), "evict_paged")
     return out
 
 

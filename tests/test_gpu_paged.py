@@ -341,10 +341,12 @@ def test_evict(E, hs, groups, page, lengths, keep, first, recent):
     evict_check(E, d, lengths, keep, rows, first=first, recent=recent)
 
 
-def test_evict_long(E):
-    lengths = [9000, 5000]
+@pytest.mark.parametrize("lengths,keep,first,recent", [([9000, 5000], 4097, 5, 1000), ([60000, 500, 41000], 33333, 5, 100), ([60000], 100, 0, 0)])
+def test_evict_long(E, lengths, keep, first, recent):
+    """Weights that fit into shared memory and such that do not."""
     d, rows = cache(lengths, 1, 64, 16, seed=3)
-    evict_check(E, d, lengths, 4097, rows, first=5, recent=1000)
+    d["kw"] = (d["kw"] * 1000).round() / 1000          # (equal ones among them)
+    evict_check(E, d, lengths, keep, rows, first=first, recent=recent)
 
 
 @pytest.mark.parametrize("kind", ["zeros", "few values", "signs", "infinite", "not a number", "neighbours", "tiny"])

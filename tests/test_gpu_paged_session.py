@@ -1,4 +1,6 @@
 """GPT models served from a paged cache through the public entry points: generate.serve.PagedSession and generate_batch."""
+import dataclasses
+
 import pytest
 import torch
 
@@ -126,7 +128,7 @@ def test_caches_that_are_cut_down(golden, mode):
     """With room for all keys nothing changes; cut down, a request holds its first, its last and its heaviest keys, in order, goes on at its positions and gives its pages back."""
     from lit_gpt_b200.generate.serve import PagedSession
 
-    model, *_ = toy(golden, mode)
+    model, rc, pw, _ = toy(golden, mode)
     g = torch.Generator().manual_seed(6)
     tokens = {r: torch.randint(1, 500, (150,), generator=g).tolist() for r in "ab"}
 
@@ -137,13 +139,16 @@ def test_caches_that_are_cut_down(golden, mode):
             out.append(s.step([("a", [tokens["a"][90 + k]], None), ("b", [tokens["b"][20 + k]], None)]))
         return s, torch.cat(out)
 
+    # steps that record weights may run other kernels than those that do not: either side's logits are within `tol` of the oracle's, so within 2 tol of each other
+    rc = dataclasses.replace(rc, block_size=200)
+    tol = max(along(model, rc, pw, torch.tensor(t), 1)[1] for t in tokens.values())
     plain, want = run()
     same, got = run(keep=1000)
-    assert torch.equal(got, want) and same.live["a"].cached == 150
+    assert (got - want).abs().max() <= 2 * tol and same.live["a"].cached == 150
     cut, got = run(keep=48, first=3, recent=10, portion=30)
     again, got2 = run(keep=48, first=3, recent=10, portion=30)
     assert torch.equal(got, got2) and torch.isfinite(got).all()
-    assert torch.allclose(got[:30], want[:30], atol=0.05 * want.abs().max().item())   # (nothing had been cut yet)
+    assert (got[:30] - want[:30]).abs().max() <= 2 * tol   # (nothing had been cut yet)
     for r, n in (("a", 150), ("b", 80)):
         now = cut.live[r]
         assert now.position == n and 48 <= now.cached < 48 + 16 and len(now.pages) == -(-now.cached // 16)

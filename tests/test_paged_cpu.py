@@ -44,10 +44,19 @@ def test_eviction_arguments_are_checked():
     for kw, text in ((dict(head_size=80), "head size"), (dict(n_seqs=0), "0 sequences"), (dict(n_groups=1 << 23), "groups"), (dict(page=24), "pages of 24"), (dict(pool=0), "no pages"),
                      (dict(n_seqs=5), "page table of 4 rows"), (dict(max_length=129), "129 keys"), (dict(keep=0), "to keep"), (dict(first=-1), "to keep"), (dict(recent=47), "to keep"),
                      (dict(key_weights=None), "null"), (dict(lengths=None), "null"), (dict(lengths_out=None), "null"), (dict(lengths_out=FAKE), "in the place"),
-                     (dict(k_pages=FAKE + 8), "16-byte"), (dict(k_page_stride=2050), "16-byte"), (dict(workspace_bytes=8), "workspace")):
+                     (dict(k_pages=FAKE + 8), "16-byte"), (dict(k_page_stride=2050), "16-byte"), (dict(workspace_bytes=8, keep=30000, max_length=60000, max_pages=8000, pages_ld=8000), "workspace")):
         refused(call(**kw), text)
     refused(lib.b200_evict_paged(None, None), "null")
-    assert lib.b200_evict_paged_workspace_bytes(3, 2, 50) == (3 * 2 * 50 + 3) * 4 and lib.b200_evict_paged_workspace_bytes(3, 2, 0) == 0
+    need = lib.b200_evict_paged_workspace_bytes
+    assert need(3, 2, 30000, 60000, 16) == (3 * 2 * 30000 + 3) * 4 and need(3, 2, 50, 128, 16) == 0 and need(3, 2, 0, 128, 16) == 0
+
+
+def test_packed_arguments_are_the_structures():
+    import struct
+
+    for cls, fmt in ((C.AttnPagedArgs, C.ATTN_PAGED_PACKED), (C.EvictPagedArgs, C.EVICT_PAGED_PACKED)):
+        n = len(cls._fields_)
+        assert struct.calcsize(fmt) == ctypes.sizeof(cls) and struct.pack(fmt, *range(1, n + 1)) == bytes(cls(*range(1, n + 1)))
 
 
 def test_tensors_on_the_cpu_are_refused():
