@@ -20,7 +20,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kPtThreads = 480, kPtSegs = 16;
+constexpr int kPtThreads = 512, kPtSegs = 16;
 
 template <int HS>
 struct PtTile {
@@ -202,65 +202,70 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     }
   }
   uint32_t tmem = 0;
-  bool ok = true, began = false;
+  bool ok = true;
   // counted over all segments, so that every barrier's phase is known
   int tiles_done = 0, segs_done = 0;                       // loads and products
   uint32_t n[2] = {0u, 0u};                                // steps of either 128 queries
 
-  for (;;) {
-    if (tid == 0) {
-      ListAt at = s_at;
-      int c = 0;
-      if (at.tile < at.end) {
-        PagedSeq seq = paged_seq(p, at.s);
-        Blocks blk = blocks_of(p, seq);
-        for (; c < kPtSegs && at.tile < at.end; c += s_seg[c].hi > s_seg[c].lo) {   // (a part without a key tile is none)
-          const int steps = blk.steps(at.block), m0 = at.block * blk.rows_each * p.per, count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
-          Seg& g = s_seg[c];
-          g.q0 = (at.gi * p.rows + seq.first) * p.per + m0;
-          g.count = count;
-          g.m0 = m0;
-          g.first = seq.first;
-          g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at.gi;
-          const int stop = min(steps, at.lo + at.end - at.tile);
-          g.lo = max(at.lo - kLead, 0);
-          g.hi = max(stop - kLead, 0);
-          g.hi0 = min(g.hi, (min(seq.cached + (m0 + min(count, 128) - 1) / p.per + 1, seq.n) + 127) >> 7);
-          g.slot = g.lo == 0 && stop == steps ? -1 : 2 * (int)blockIdx.x + (g.lo == 0);   // (of a CTA's segments only the first begins, only the last ends within an item)
-          at.tile += stop - at.lo;
-          if (at.tile >= at.end) continue;
-          at.lo = 0;
-          if (++at.block == blk.count) {
-            at.block = 0;
-            if (++at.gi == p.n_groups) {
-              at.gi = 0;
-              do {
-                seq = paged_seq(p, ++at.s);
-                blk = blocks_of(p, seq);
-              } while (blk.count == 0);
-            }
+  auto list_segments = [&]() {            // by thread 0
+    ListAt at = s_at;
+    int c = 0;
+    if (at.tile < at.end) {
+      PagedSeq seq = paged_seq(p, at.s);
+      Blocks blk = blocks_of(p, seq);
+      for (; c < kPtSegs && at.tile < at.end; c += s_seg[c].hi > s_seg[c].lo) {   // (a part without a key tile is none)
+        const int steps = blk.steps(at.block), m0 = at.block * blk.rows_each * p.per, count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
+        Seg& g = s_seg[c];
+        g.q0 = (at.gi * p.rows + seq.first) * p.per + m0;
+        g.count = count;
+        g.m0 = m0;
+        g.first = seq.first;
+        g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at.gi;
+        const int stop = min(steps, at.lo + at.end - at.tile);
+        g.lo = max(at.lo - kLead, 0);
+        g.hi = max(stop - kLead, 0);
+        g.hi0 = min(g.hi, (min(seq.cached + (m0 + min(count, 128) - 1) / p.per + 1, seq.n) + 127) >> 7);
+        g.slot = g.lo == 0 && stop == steps ? -1 : 2 * (int)blockIdx.x + (g.lo == 0);   // (of a CTA's segments only the first begins, only the last ends within an item)
+        at.tile += stop - at.lo;
+        if (at.tile >= at.end) continue;
+        at.lo = 0;
+        if (++at.block == blk.count) {
+          at.block = 0;
+          if (++at.gi == p.n_groups) {
+            at.gi = 0;
+            do {
+              seq = paged_seq(p, ++at.s);
+              blk = blocks_of(p, seq);
+            } while (blk.count == 0);
           }
         }
       }
-      s_at = at;                                           // (in shared memory: the softmax has no registers for it)
-      s_segs = c;
-      s_more = at.tile < at.end;
     }
-    if (!began) {                                          // (tensor memory is taken behind the wait only)
-      griddep_wait();
-      if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
-      if (tid == 0) p.cuts[blockIdx.x] = s_cut;
-      tc::fence_before();
-    }
-    __syncthreads();
-    if (!began) {
-      tc::fence_after();
-      tmem = s_tmem;
-      began = true;
-    }
-    const int segs = s_segs;
-
-    if (warp >= 13) {
+    s_at = at;                                           // (in shared memory: the softmax has no registers for it)
+    s_segs = c;
+    s_more = at.tile < at.end;
+  };
+  if (tid == 0) list_segments();
+  griddep_wait();                         // (tensor memory is taken behind the wait only)
+  if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+  if (tid == 0) p.cuts[blockIdx.x] = s_cut;
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  tmem = s_tmem;
+  auto more_segments = [&]() {            // by all, behind a batch's segments
+    ok = __syncthreads_and(ok);
+    const bool more = ok && s_more;
+    __syncthreads();                      // (everyone has read s_more)
+    return more;
+  };
+  // A role has its loop over batches of segments to itself, so that its registers are its own: the softmax warps hold a query's 128 scores, and registers go from the others to them
+  // (256 x 192 + 256 x 56 of the launch's 512 x 128).
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp >= 13 && warp < 15) {
+      for (;;) {
+        const int segs = s_segs;
       // ================================ loads ================================
       const bool keys = warp == 13;
       const uint32_t dst = keys ? sk_ : sv_, full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
@@ -274,7 +279,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         for (int j = lo; j < hi; ++j, ++tiles_done) {
           const int s = tiles_done & 1;
           const int next = j + 1 < hi ? page_of(j + 1) : -1;
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(empty + 8 * s, ((uint32_t)(tiles_done >> 1) & 1u) ^ 1u));
+          ok = __all_sync(0xffffffffu, tc::mbar_wait_here(empty + 8 * s, ((uint32_t)(tiles_done >> 1) & 1u) ^ 1u));
           if (!ok) break;
           const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
           const bool whole = have == (1u << parts) - 1u;
@@ -311,7 +316,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
             if (lane == 0) tc::mbar_arrive(full + 8 * s);
           }
           if (keys && j == lo) {        // the queries, once the segment before has done its last product with the ones there
-            if (tiles_done > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + 8 * (s ^ 1), (uint32_t)((tiles_done - 1) >> 1) & 1u));
+            if (tiles_done > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait_here(k_empty + 8 * (s ^ 1), (uint32_t)((tiles_done - 1) >> 1) & 1u));
             if (!ok) break;
             const int halves = g.count > 128 ? 2 : 1;
             if (lane == 0) {
@@ -326,7 +331,12 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         }
         ++segs_done;
       }
+        if (!more_segments()) break;
+        __syncthreads();
+      }
     } else if (warp == 12) {
+      for (;;) {
+        const int segs = s_segs;
       // ================================ products ================================
       if (tc::elect()) {
         const uint32_t q_low = tc::desc_sw128_low(sq_), k_low = tc::desc_sw128_low(sk_), v_low = desc_v_low(sv_);
@@ -384,11 +394,20 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         }
         if (!ok) {
           tc::commit(idle);
-          tc::mbar_wait(idle, 0);
+          tc::mbar_wait_here(idle, 0);
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-    } else if (warp >= 8) {
+        if (!more_segments()) break;
+        __syncthreads();
+      }
+    } else {
+      while (more_segments()) __syncthreads();
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    for (;;) {
+      const int segs = s_segs;
       // ================================ shrinking O ================================
       const int v = warp - 8;
       for (int c = 0; c < segs && ok; ++c) {
@@ -398,25 +417,20 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (j >= (t ? hi1 : hi0)) continue;
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(shrink + 8 * (4 * t + v), n[t] & 1u));
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait_here(shrink + 8 * (4 * t + v), n[t] & 1u));
             if (!ok) break;
             const float f = s_shrink[t * 128 + v * 32 + lane];
             if (__any_sync(0xffffffffu, f != 1.0f)) {   // (S of this step is there, so P V of the last one is done; a segment's first step has f = 1)
               tc::fence_after();
               const uint32_t to = tmem + ((uint32_t)(v * 32) << 16) + C::kO + t * HS;
 #pragma unroll 1
-              for (int cc = 0; cc < HS; cc += 32) {
-                uint32_t o[32];
-                tc::ld32(o, to + cc);
+              for (int cc = 0; cc < HS; cc += 16) {
+                uint32_t o[16];
+                tc::ld16(o, to + cc);
                 tc::wait_ld(o);
-                uint32_t a[16], bb[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  a[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  bb[e] = __float_as_uint(__uint_as_float(o[16 + e]) * f);
-                }
-                st16(to + cc, a);
-                st16(to + cc + 16, bb);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                st16(to + cc, o);
               }
               wait_st();
               tc::fence_before();
@@ -427,7 +441,13 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           }
         }
       }
-    } else {
+      if (!more_segments()) break;
+      __syncthreads();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    for (;;) {
+      const int segs = s_segs;
       // ================================ softmax: a query per thread ================================
       const int t = warp >> 2;
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -444,7 +464,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         f2 l2[2] = {0ull, 0ull};
         const uint32_t n0 = n[0];
         for (int j = lo; j < hi; ++j, ++n[0]) {
-          ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * t, n[0] & 1u));
+          ok = ok && __all_sync(0xffffffffu, tc::mbar_wait_here(s_full + 8 * t, n[0] & 1u));
           if (!ok) break;
           tc::fence_after();
           const int j0 = j * 128;
@@ -466,24 +486,16 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
             for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
             return mx;
           };
-          uint32_t s0[32], s1[32];
+          uint32_t v[4][32];
           float mx[4];
-          tc::ld32(s0, ts + 64);
-          tc::ld32(s1, ts + 96);
-          tc::wait_ld(s0);
-          tc::wait_ld(s1);
-          mask(s0, 2);
-          mask(s1, 3);
-          mx[2] = most(s0, -INFINITY);
-          mx[3] = most(s1, -INFINITY);
-          tc::ld32(s0, ts);
-          tc::ld32(s1, ts + 32);
-          tc::wait_ld(s0);
-          tc::wait_ld(s1);
-          mask(s0, 0);
-          mask(s1, 1);
-          mx[0] = most(s0, -INFINITY);
-          mx[1] = most(s1, -INFINITY);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tc::ld32(v[i], ts + 32 * i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            tc::wait_ld(v[i]);
+            mask(v[i], i);
+            mx[i] = most(v[i], -INFINITY);
+          }
           const float nm = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           const float f = m == -INFINITY ? 1.0f : ex2((m - nm) * sl);   // nothing seen so far: O and the sum are zero
           m = nm;
@@ -514,23 +526,17 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(bar + 8 * t);
           };
-          exps(s0, 0);
-          tc::ld32(s0, ts + 64);   // (P so far lies in columns 0 .. 31, at most 0 .. 63: scores 64 .. 127 are still there)
-          exps(s1, 1);
-          tc::wait_ld(s0);
-          tc::ld32(s1, ts + 96);
+          exps(v[0], 0);
+          exps(v[1], 1);
           hand_over(p_half);
-          mask(s0, 2);
-          exps(s0, 2);
-          tc::wait_ld(s1);
-          mask(s1, 3);
-          exps(s1, 3);
+          exps(v[2], 2);
+          exps(v[3], 3);
           hand_over(p_full);
         }
         tiles_before += g.hi - lo;
         const bool any = n[0] != n0;
         if (any && ok) {
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * t, (n[0] - 1) & 1u));
+          ok = __all_sync(0xffffffffu, tc::mbar_wait_here(o_done + 8 * t, (n[0] - 1) & 1u));
           tc::fence_after();
         }
         if (!ok) break;
@@ -592,17 +598,17 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         }
       }
       tiles_done = tiles_before;
+      if (!more_segments()) break;
+      if (tid == 0) list_segments();
+      __syncthreads();
     }
-    ok = __syncthreads_and(ok);
-    if (!ok || !s_more) break;
-    __syncthreads();                                       // (everyone has read s_more)
   }
   if (!ok) {
     // copies on their way: neither stage may be written once this CTA has left
-    if (warp >= 13) {
+    if (warp == 13 || warp == 14) {
       const uint32_t full = warp == 13 ? k_full : v_full;
-      for (int e = max(tiles_done - 2, 0); e < tiles_done; ++e) tc::mbar_wait(full + 8 * (e & 1), (uint32_t)(e >> 1) & 1u);
-      if (warp == 13 && segs_done > 0) tc::mbar_wait(q_full, (uint32_t)(segs_done - 1) & 1u);
+      for (int e = max(tiles_done - 2, 0); e < tiles_done; ++e) tc::mbar_wait_here(full + 8 * (e & 1), (uint32_t)(e >> 1) & 1u);
+      if (warp == 13 && segs_done > 0) tc::mbar_wait_here(q_full, (uint32_t)(segs_done - 1) & 1u);
     }
     *err = 1u;
   }
