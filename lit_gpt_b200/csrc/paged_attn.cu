@@ -30,7 +30,7 @@ __device__ __forceinline__ int64_t paged_pos(const PagedParams& p, int row) {
 // A CTA takes a row, or some heads of one: HS / 16 threads a head, each with sixteen numbers of it, eight and the eight that they turn with (or, where nothing is turned, any sixteen), whose cosines
 // and sines it keeps from head to head.  Needs rows of heads and tables for accesses of 16 bytes, and halves of the rotation that are multiples of eight numbers (or no rotation).
 template <int HS>
-__global__ void __launch_bounds__(256) paged_append_wide_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(256, 4) paged_append_wide_kernel(const PagedParams p) {
   constexpr int TH = HS / 16, HEADS = 256 / TH;    // threads of a head; heads at once
   griddep_wait();     // (before the launch of what follows: the kernels behind read the step's description and the older keys ahead of their own wait)
   griddep_launch();
@@ -185,16 +185,20 @@ __device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, in
   for (int w = 0; w < warp; ++w) { before.x = capped((int64_t)before.x + s_warp[w].x); before.y = capped((int64_t)before.y + s_warp[w].y); }
   sums[tid] = before;
   if (tid == THREADS - 1) sums[THREADS] = make_int2(capped((int64_t)before.x + here.x), capped((int64_t)before.y + here.y));
-  if (note) {                            // who joins the results learns where a sequence's items begin
-    int items = before.y * p.n_groups;
-    for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
-      __stcg(p.item_base + i, items);
-      items += seq_items(p, paged_seq(p, i)) * p.n_groups;
-    }
-  }
   __syncthreads();
   Split s;
   const int64_t all = (int64_t)sums[THREADS].x * p.n_groups, items = (int64_t)sums[THREADS].y * p.n_groups;
+  if (note) {                            // who joins the results, and who adds up the keys' weights, learns where a sequence's items and tiles begin
+    const bool fits = all < kMaxTiles && items <= p.items;
+    for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
+      const PagedSeq q = paged_seq(p, i);
+      const int n = seq_items(p, q);
+      __stcg(p.item_base + i, before.y * p.n_groups);
+      __stcg(p.tile_base + i, fits ? before.x * p.n_groups : -1);
+      before.x += n * seq_tiles(q);
+      before.y += n;
+    }
+  }
   s.all = all < kMaxTiles && items <= p.items ? (int)all : 0;
   // two tiles a worker at least, unless that leaves SMs without one
   s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
@@ -660,40 +664,35 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// ---- the weight that the keys of the list's sequences receive: a tile of 32 keys a warp, a key a lane, from the scores that were kept ----
+// ---- the weight that the keys of the list's sequences receive: a key a thread, from the scores that were kept ----
 __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
-  constexpr int T = 256;
-  __shared__ int2 s_sums[T + 1], s_warp[T / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_launch();
-  const Split s = make_split<T>(p, s_sums, s_warp, false);
-  const int w = warp * (int)gridDim.x + (int)blockIdx.x;
-  const Walk walk{p, s_sums, (p.n_seqs + T - 1) / T, T};
-  const int first = first_tile(w, s), end = first_tile(w + 1, s);
-  Tile t = {};
-  if (w < s.workers) t = walk.find(first);
+  const int which = blockIdx.x / p.n_groups, gi = blockIdx.x - which * p.n_groups;
+  const PagedSeq s = paged_seq(p, which);
+  const int items = seq_items(p, s);
+  auto place = [&](int key) -> float* {
+    const int id = key < s.n ? page_at(p, s.table, key >> p.shift) : -1;
+    return id < 0 ? nullptr : p.kw + (((int64_t)id * p.n_groups + gi) << p.shift) + (key & ((1 << p.shift) - 1));
+  };
+  int key = blockIdx.y * 256 + threadIdx.x;
+  float* at = items > 0 ? place(key) : nullptr;
   griddep_wait();
-  if (w >= s.workers) return;
-  for (;;) {
-    if (t.part == 0) {                     // (the tile of all tiles of queries)
-      const uint32_t bits = t.bits();
-      const int key0 = t.key0(), id = lane < 16 ? t.id0 : t.id1;
-      const bool there = (bits >> lane) & 1u;
-      float* const at = p.kw + (((int64_t)max(id, 0) * p.n_groups + t.gi) << p.shift) + ((key0 + lane) & ((1 << p.shift) - 1));
-      float sum = 0.f;
-      const float before = there ? *at : 0.f;
-      const int count = t.seq.rows * p.per;
-      const float* const lse = p.lse + ((int64_t)t.gi * p.rows + t.seq.first) * p.per;
-      for (int m0 = 0, index = t.index; m0 < count; m0 += p.tile_rows, index += t.tiles) {
-        const float* const kept = p.scores + (int64_t)index * p.score_rows * kShTile + lane;
-        const int n = min(p.tile_rows, count - m0);
-#pragma unroll 4
-        for (int m = 0; m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
-      }
-      if (there) *at = before + sum;
+  if (items == 0) return;
+  const int tiles = seq_tiles(s), count = s.rows * p.per;
+  const int first = __ldcg(p.tile_base + which);
+  if (first < 0) return;                           // (more than fits a step's limits: nothing was done)
+  const float* const lse = p.lse + ((int64_t)gi * p.rows + s.first) * p.per;
+  for (; key < s.n; key += gridDim.y * 256, at = place(key)) {
+    if (!at) continue;
+    float sum = 0.f;
+    const float before = *at;
+    for (int m0 = 0, index = first + gi * items * tiles + key / kShTile; m0 < count; m0 += p.tile_rows, index += tiles) {
+      const float* const kept = p.scores + (int64_t)index * p.score_rows * kShTile + key % kShTile;
+      const int n = min(p.tile_rows, count - m0);
+#pragma unroll 8
+      for (int m = 0; m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
     }
-    if (t.index + 1 >= end) break;
-    walk.next(t);
+    *at = before + sum;
   }
 }
 
@@ -749,7 +748,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
       s.kw_workers = blocks < sm_count() ? (int)blocks : sm_count();
     }
   }
-  s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * sizeof(int) +
+  s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * 2 * sizeof(int) +
             (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)s.scores * sizeof(float) + (size_t)s.kw_workers * (256 * sizeof(float) + sizeof(PagedWeightCut)) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
   // A cluster where its warps have four tiles each at most, and all clusters run at once.  us of the list and of clusters: 1 token of 32 groups, 128 numbers a head, over 300 keys 12.9, 7.5, over
   // 2000 13.6, 10.4, over 8000 30.6, 28.1; of 8 groups of 4 heads over 8000 16.6, 17.2; 16 tokens of 32 groups over 300 18.5, 19.5; 64 of 8 groups over 100 14.4, 15.4; of 12 groups, 64 numbers
@@ -816,10 +815,8 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t 
     if (e != cudaSuccess) return e;
   }
   if (p.scores) {
-    PagedParams k = p;
-    const int ctas = 8 * p.sms;      // a warp's tiles are a chain of loads each: as many warps as are at once
-    k.workers = 8 * ctas;
-    if ((e = launch(paged_kept_kernel, dim3((unsigned)ctas), dim3(256), 0, st, k)) != cudaSuccess) return e;
+    const int64_t pairs = (int64_t)p.n_seqs * p.n_groups, runs = (p.max_length + 255) / 256, most = 16 * p.sms / pairs + 1;   // (a few rounds of CTAs at most)
+    if ((e = launch(paged_kept_kernel, dim3((unsigned)pairs, (unsigned)(runs < most ? runs : most)), dim3(256), 0, st, p)) != cudaSuccess) return e;
   }
   return s.kw_workers > 0 ? launch_paged_weights(p, HS, st) : e;
 }
@@ -890,7 +887,8 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.cuts = (PagedCut*)(p.where + s.items);
   p.item_base = (int*)(p.cuts + s.tc_workers);
   p.score_rows = s.score_rows; p.kept_max = s.kept_max; p.kw_workers = s.kw_workers;
-  p.kw_cuts = (PagedWeightCut*)(p.item_base + a->n_seqs);
+  p.tile_base = p.item_base + a->n_seqs;
+  p.kw_cuts = (PagedWeightCut*)(p.tile_base + a->n_seqs);
   p.kw_part = (float*)(p.kw_cuts + s.kw_workers);
   p.lse = p.kw ? p.kw_part + (int64_t)s.kw_workers * 256 : nullptr;
   p.scores = s.scores ? p.lse + (int64_t)p.rows * p.per * p.n_groups : nullptr;
