@@ -438,14 +438,81 @@ __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_ker
   pf_wait<0>();
 }
 
-// A head's results joined: `ways` warps a head, HS / 32 numbers a lane.
+// An item of the tensor memory's that several CTAs had segments of (paged_attn_tc05.cu): CTA (w, part) joins a share of its queries, 32 at a time, for the w-th worker's beginning within it.  A query a lane, HS / 8
+// numbers a warp.
+template <int HS>
+__device__ __forceinline__ void join_cut(const PagedParams& p, int index, int parts) {
+  constexpr int V = HS / 8;
+  const int w = index / parts, part = index - w * parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const PagedCut c = p.cuts[w];
+  if (c.last < 0) return;
+  const int shares = (c.last - c.first) * parts, share = (w - c.first - 1) * parts + part;
+  for (int m0 = share * 32; m0 < c.count; m0 += shares * 32) {
+    const int m = m0 + lane;
+    float top = -INFINITY, sum = 0.f, a[V] = {};
+    for (int i0 = c.first; i0 <= c.last; i0 += 2) {
+      float2 e[2];
+      float4 v[2][V / 4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        e[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) v[u][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + u <= c.last && m < c.count) {
+          const int64_t slot = 2 * (i0 + u) + (i0 + u == c.first);
+          e[u] = __ldcg(p.tc_ml + slot * 256 + m);
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) v[u][j] = __ldcg(reinterpret_cast<const float4*>(p.tc_acc + slot * 256 * HS + (int64_t)(warp * V + 4 * j) * 256 + m * 4));
+        }
+      }
+      const float now = fmaxf(top, fmaxf(e[0].x, e[1].x)), org = now == -INFINITY ? 0.f : now, shrink = ex2(top - org);
+      top = now;
+      sum *= shrink;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] *= shrink;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float f = ex2(e[u].x - org);
+        sum += e[u].y * f;
+        if (e[u].y != 0.f) {            // (a range that saw nothing has no result)
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) {
+            a[4 * j] += v[u][j].x * f;
+            a[4 * j + 1] += v[u][j].y * f;
+            a[4 * j + 2] += v[u][j].z * f;
+            a[4 * j + 3] += v[u][j].w * f;
+          }
+        }
+      }
+    }
+    if (m >= c.count) continue;
+    const int row = m / p.per, hh = m - row * p.per;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    __nv_bfloat16* const to = p.out + ((int64_t)(c.row + row) * p.n_head + c.gi * p.per + hh) * HS + warp * V;
+#pragma unroll
+    for (int j = 0; j < V; j += 8)
+      *reinterpret_cast<uint4*>(to + j) = make_uint4(pack_bf16(a[j] * inv, a[j + 1] * inv), pack_bf16(a[j + 2] * inv, a[j + 3] * inv), pack_bf16(a[j + 4] * inv, a[j + 5] * inv),
+                                                     pack_bf16(a[j + 6] * inv, a[j + 7] * inv));
+    if (p.lse && warp == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
+  }
+}
+
+// The first CTAs join the tensor memory's cut items, kCutParts a worker; the others the list's results, `ways` warps a head, HS / 32 numbers a lane.
+constexpr int kCutParts = 8;
 template <int HS>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  if ((int)blockIdx.x < p.tc_workers * kCutParts) {
+    griddep_launch();
+    griddep_wait();
+    join_cut<HS>(p, blockIdx.x, kCutParts);
+    return;
+  }
+  const int block = blockIdx.x - p.tc_workers * kCutParts;
   constexpr int V = HS / 32;
   __shared__ float s_acc[8][HS];
   __shared__ float2 s_ml[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = 8 / p.ways, blocks = (p.n_head + heads - 1) / heads;
-  const int row = blockIdx.x / blocks, h = (blockIdx.x - row * blocks) * heads + warp / p.ways, way = warp % p.ways;
+  const int row = block / blocks, h = (block - row * blocks) * heads + warp / p.ways, way = warp % p.ways;
   griddep_launch();
   const int which = p.row_seq[row];
   PagedSeq s = {};
@@ -664,10 +731,22 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// ---- the weight that the keys of the list's sequences receive: a key a thread, from the scores that were kept ----
+// ---- the weight that keys receive: blocks of keys that several CTAs of paged_weights.cu had parts of, in the CTAs' order; and the list's sequences', a key a thread, from the scores
+// that were kept ----
 __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
   griddep_launch();
-  const int which = blockIdx.x / p.n_groups, gi = blockIdx.x - which * p.n_groups;
+  if ((int)blockIdx.x < p.kw_workers) {
+    griddep_wait();
+    const PagedWeightCut c = p.kw_cuts[blockIdx.x];
+    if (c.last < 0 || blockIdx.y > 0 || threadIdx.x >= 128) return;
+    const int key = c.block * 128 + (int)threadIdx.x;
+    float sum = 0.f;
+    for (int w = c.first; w <= c.last; ++w) sum += __ldcg(p.kw_part + (2 * w + (w == c.first)) * 128 + threadIdx.x);
+    const int id = key < c.n ? page_at(p, c.table, key >> p.shift) : -1;
+    if (id >= 0) p.kw[(((int64_t)id * p.n_groups + c.gi) << p.shift) + (key & ((1 << p.shift) - 1))] += sum;
+    return;
+  }
+  const int pair = blockIdx.x - p.kw_workers, which = pair / p.n_groups, gi = pair - which * p.n_groups;
   const PagedSeq s = paged_seq(p, which);
   const int items = seq_items(p, s);
   auto place = [&](int key) -> float* {
@@ -810,15 +889,14 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t 
   if (s.list) {
     e = s.nq == 4 ? launch_list<HS, 4>(p, s, st) : s.nq == 2 ? launch_list<HS, 2>(p, s, st) : launch_list<HS, 1>(p, s, st);
     if (e != cudaSuccess) return e;
-    const int heads = 8 / s.ways;
-    e = launch(paged_join_kernel<HS>, dim3((unsigned)(p.rows * ((p.n_head + heads - 1) / heads))), dim3(256), 0, st, p);
-    if (e != cudaSuccess) return e;
   }
-  if (p.scores) {
-    const int64_t pairs = (int64_t)p.n_seqs * p.n_groups, runs = (p.max_length + 255) / 256, most = 16 * p.sms / pairs + 1;   // (a few rounds of CTAs at most)
-    if ((e = launch(paged_kept_kernel, dim3((unsigned)pairs, (unsigned)(runs < most ? runs : most)), dim3(256), 0, st, p)) != cudaSuccess) return e;
-  }
-  return s.kw_workers > 0 ? launch_paged_weights(p, HS, st) : e;
+  const int heads = 8 / s.ways, joins = s.list ? p.rows * ((p.n_head + heads - 1) / heads) : 0;
+  e = launch(paged_join_kernel<HS>, dim3((unsigned)(p.tc_workers * kCutParts + joins)), dim3(256), 0, st, p);
+  if (e != cudaSuccess || !p.kw) return e;
+  if (s.kw_workers > 0 && (e = launch_paged_weights(p, HS, st)) != cudaSuccess) return e;
+  const int64_t pairs = p.scores ? (int64_t)p.n_seqs * p.n_groups : 0;
+  const int64_t runs = p.scores ? (p.max_length + 255) / 256 : 1, most = 16 * p.sms / (pairs + 1) + 1;   // (a few rounds of CTAs at most)
+  return launch(paged_kept_kernel, dim3((unsigned)(p.kw_workers + pairs), (unsigned)(runs < most ? runs : most)), dim3(256), 0, st, p);
 }
 
 }  // namespace

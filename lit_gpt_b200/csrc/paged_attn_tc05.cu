@@ -2,7 +2,7 @@
 //
 // An item is a block of up to 256 queries of one sequence and group -- whole rows, every head of the group -- against the keys that its last row sees, in tiles of 128.  The key tiles of
 // all items are one list, cut evenly over the CTAs, one an SM: neither few rows over many keys nor chunks of unequal lengths leave SMs without work.  A CTA's part of an item is a segment.
-// The result of an item that is one CTA's is stored at once; else every segment leaves maxima, sums and unscaled outputs, and a second launch joins them.
+// The result of an item that is one CTA's is stored at once; else every segment leaves maxima, sums and unscaled outputs, and the step's join (paged_attn.cu) puts them together.
 //   * warps 0-3 and 4-7: the softmax of the block's first and second 128 queries, one per thread.  S (128 columns of tensor memory) is read into registers, the
 //     probabilities go back over it as bf16, the left operand of P V, in two halves so that P V starts on the first (attn_tc05.cu says what was tried);
 //   * warps 8-11: when a row's maximum grew, they shrink its O in tensor memory while its exponentials are still being taken;
@@ -620,67 +620,6 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   }
 }
 
-// An item that several CTAs had segments of: CTA (w, part) of this launch joins a share of its queries, 32 at a time, for the w-th worker's beginning within it.  A query a lane, HS / 8
-// numbers a warp.
-template <int HS>
-__global__ void __launch_bounds__(256) paged_tc05_join_kernel(const PagedParams p, int parts) {
-  constexpr int V = HS / 8;
-  griddep_launch();
-  griddep_wait();
-  const int w = blockIdx.x / parts, part = blockIdx.x - w * parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const PagedCut c = p.cuts[w];
-  if (c.last < 0) return;
-  const int shares = (c.last - c.first) * parts, share = (w - c.first - 1) * parts + part;
-  for (int m0 = share * 32; m0 < c.count; m0 += shares * 32) {
-    const int m = m0 + lane;
-    float top = -INFINITY, sum = 0.f, a[V] = {};
-    for (int i0 = c.first; i0 <= c.last; i0 += 2) {
-      float2 e[2];
-      float4 v[2][V / 4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        e[u] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int j = 0; j < V / 4; ++j) v[u][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i0 + u <= c.last && m < c.count) {
-          const int64_t slot = 2 * (i0 + u) + (i0 + u == c.first);
-          e[u] = __ldcg(p.tc_ml + slot * 256 + m);
-#pragma unroll
-          for (int j = 0; j < V / 4; ++j) v[u][j] = __ldcg(reinterpret_cast<const float4*>(p.tc_acc + slot * 256 * HS + (int64_t)(warp * V + 4 * j) * 256 + m * 4));
-        }
-      }
-      const float now = fmaxf(top, fmaxf(e[0].x, e[1].x)), org = now == -INFINITY ? 0.f : now, shrink = ex2(top - org);
-      top = now;
-      sum *= shrink;
-#pragma unroll
-      for (int j = 0; j < V; ++j) a[j] *= shrink;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float f = ex2(e[u].x - org);
-        sum += e[u].y * f;
-        if (e[u].y != 0.f) {            // (a range that saw nothing has no result)
-#pragma unroll
-          for (int j = 0; j < V / 4; ++j) {
-            a[4 * j] += v[u][j].x * f;
-            a[4 * j + 1] += v[u][j].y * f;
-            a[4 * j + 2] += v[u][j].z * f;
-            a[4 * j + 3] += v[u][j].w * f;
-          }
-        }
-      }
-    }
-    if (m >= c.count) continue;
-    const int row = m / p.per, hh = m - row * p.per;
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    __nv_bfloat16* const to = p.out + ((int64_t)(c.row + row) * p.n_head + c.gi * p.per + hh) * HS + warp * V;
-#pragma unroll
-    for (int j = 0; j < V; j += 8)
-      *reinterpret_cast<uint4*>(to + j) = make_uint4(pack_bf16(a[j] * inv, a[j + 1] * inv), pack_bf16(a[j + 2] * inv, a[j + 3] * inv), pack_bf16(a[j + 4] * inv, a[j + 5] * inv),
-                                                     pack_bf16(a[j + 6] * inv, a[j + 7] * inv));
-    if (p.lse && warp == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
-  }
-}
-
 template <int HS>
 cudaError_t launch_hs(const PagedParams& p, cudaStream_t st) {
   constexpr int smem = PtTile<HS>::kSmem;
@@ -697,10 +636,7 @@ cudaError_t launch_hs(const PagedParams& p, cudaStream_t st) {
     return cudaErrorInvalidValue;
   unsigned* const err = wait_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  cudaError_t e = launch(paged_tc05_kernel<HS>, dim3((unsigned)p.tc_workers), dim3(kPtThreads), (size_t)smem, st, p, mq, mk, mv, err);
-  if (e != cudaSuccess) return e;
-  constexpr int parts = 8;
-  return launch(paged_tc05_join_kernel<HS>, dim3((unsigned)(p.tc_workers * parts)), dim3(256), 0, st, p, parts);
+  return launch(paged_tc05_kernel<HS>, dim3((unsigned)p.tc_workers), dim3(kPtThreads), (size_t)smem, st, p, mq, mk, mv, err);
 }
 
 }  // namespace

@@ -1,11 +1,11 @@
 // The attention weight that the keys of a paged cache receive in a step (paged_attn.cu): per key and group the sum, over the step's rows and the group's heads, of
 //   exp2(s - lse),   s the score and lse the logarithm of the row's sum of exponentials, both times log2(e).
 //
-// Sequences of the list of tiles leave their scores behind (a hundredth to a sixth of their keys' bytes); paged_kept_kernel reads them, a tile of 32 keys a warp, a key a lane.
+// Sequences of the list of tiles leave their scores behind (a hundredth to a sixth of their keys' bytes); paged_kept_kernel (paged_attn.cu) adds up what they give, a key a thread.
 //
 // The others' are computed again on the 5th-generation tensor cores, paged_weights_kernel: S^T = K Q^T, 128 keys as the rows of tensor memory and 128 queries as its columns, so that a
 // thread has a key, its sum stays in registers and nothing is reduced across threads.  An item is a block of 128 keys of a sequence and group against the tiles of queries that see it; the
-// tiles of all items are one list, cut evenly over the CTAs.  The sums of an item that several CTAs have parts of are added by paged_weights_join_kernel, in the order of the CTAs.
+// tiles of all items are one list, cut evenly over the CTAs.  The sums of an item that several CTAs have parts of are added by the same kernel, in the order of the CTAs.
 //   * warps 0-3 and 4-7: the even and the odd tiles of queries, a key a thread: s in registers, a query's lse from shared memory (one address for all lanes), an exponential and an addition
 //   * warp 8: one thread issues the products, four tiles of scores in tensor memory
 //   * warp 9 brings keys (a page, or what of it lies in the block, is one TMA box), queries (four stages) and the queries' lse
@@ -418,19 +418,6 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
   }
 }
 
-// A block of keys that several CTAs had parts of: a CTA of this launch for each of theirs that was the first to go on with one
-__global__ void __launch_bounds__(128) paged_weights_join_kernel(const PagedParams p) {
-  griddep_launch();
-  griddep_wait();
-  const PagedWeightCut c = p.kw_cuts[blockIdx.x];
-  if (c.last < 0) return;
-  const int key = c.block * 128 + (int)threadIdx.x;
-  float sum = 0.f;
-  for (int w = c.first; w <= c.last; ++w) sum += __ldcg(p.kw_part + (2 * w + (w == c.first)) * 128 + threadIdx.x);
-  const int id = key < c.n ? page_at(p, c.table, key >> p.shift) : -1;
-  if (id >= 0) p.kw[(((int64_t)id * p.n_groups + c.gi) << p.shift) + (key & ((1 << p.shift) - 1))] += sum;
-}
-
 template <int HS>
 cudaError_t launch_hs(const PagedParams& p, cudaStream_t st) {
   constexpr int smem = KwTile<HS>::kSmem;
@@ -446,9 +433,7 @@ cudaError_t launch_hs(const PagedParams& p, cudaStream_t st) {
     return cudaErrorInvalidValue;
   unsigned* const err = wait_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  const cudaError_t e = launch(paged_weights_kernel<HS>, dim3((unsigned)p.kw_workers), dim3(kKwThreads), (size_t)smem, st, p, mq, mk, err);
-  if (e != cudaSuccess) return e;
-  return launch(paged_weights_join_kernel, dim3((unsigned)p.kw_workers), dim3(128), 0, st, p);
+  return launch(paged_weights_kernel<HS>, dim3((unsigned)p.kw_workers), dim3(kKwThreads), (size_t)smem, st, p, mq, mk, err);
 }
 
 }  // namespace
