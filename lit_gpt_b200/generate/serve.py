@@ -392,10 +392,10 @@ def generate_batch(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens:
     if num_samples < 1:
         raise ValueError(f"num_samples must be at least 1 (got {num_samples})")
     penalties = (float(repetition_penalty), float(frequency_penalty), float(presence_penalty))
-    if num_samples > 1 or penalties != (1.0, 0.0, 0.0) or logit_bias or allowed is not None:
+    if num_samples > 1 or penalties != (1.0, 0.0, 0.0) or logit_bias or allowed is not None or isinstance(model, GPT):   # (all rows draw in one launch)
         session = session if session is not None else _session_for(model, prompts, max_new_tokens, num_samples)
         return _generate_ruled(model, prompts, max_new_tokens, temperature, top_k, eos_id, session, num_samples, penalties, count_prompt, logit_bias, allowed)
-    session = session if session is not None else _session_for(model, prompts, max_new_tokens, 1)
+    session = session if session is not None else Session(model, slots=len(prompts))
     dev = model.device
     out = [list(p) for p in prompts]
     ids = [("gen", i) for i in range(len(prompts))]
@@ -412,24 +412,20 @@ def generate_batch(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens:
 
     live = list(range(len(prompts)))
     budget = [max_new_tokens] * len(prompts)
-    try:
-        nxt = draw(session.step([(ids[i], out[i], [len(out[i]) - 1]) for i in live])) if max_new_tokens > 0 else []
-        while live:
-            done = []
-            for i, t in zip(live, nxt):
-                out[i].append(t)
-                budget[i] -= 1
-                if budget[i] <= 0 or t == eos_id or len(out[i]) >= model.max_seq_length:
-                    done.append(i)
-            live = [i for i in live if i not in done]
-            if not live:
-                session.step([], end=[ids[i] for i in done])
-                break
-            logits = session.step([(ids[i], [out[i][-1]], None) for i in live], end=[ids[i] for i in done])
-            nxt = draw(logits)
-    except Exception:
-        session.step([], end=ids)   # (a pool without a page left, say: what these requests hold is the session's again)
-        raise
+    nxt = draw(session.step([(ids[i], out[i], [len(out[i]) - 1]) for i in live])) if max_new_tokens > 0 else []
+    while live:
+        done = []
+        for i, t in zip(live, nxt):
+            out[i].append(t)
+            budget[i] -= 1
+            if budget[i] <= 0 or t == eos_id or len(out[i]) >= model.max_seq_length:
+                done.append(i)
+        live = [i for i in live if i not in done]
+        if not live:
+            session.step([], end=[ids[i] for i in done])
+            break
+        logits = session.step([(ids[i], [out[i][-1]], None) for i in live], end=[ids[i] for i in done])
+        nxt = draw(logits)
     return out
 
 
