@@ -326,7 +326,8 @@ int b200_attn_decode_shared_tune(int path);
  *              weights over the step's rows and its group's heads.
  *   max_rows, max_length   bounds of a sequence's rows and of its keys behind the step: they size the work; keys from max_length on are dropped
  *   cos, sin   (table_rows, rope_n_elem), row = position; table_preselected: row = row of qkv
- * head_size 64 or 128.  out on a 16-byte boundary.  No page belongs to two sequences that bring rows into it.  The workspace needs no initial contents; two calls that run at the same time need one each
+ * head_size 64 or 128.  out on a 16-byte boundary.  No page belongs to two sequences that bring rows into it (with key_weights: to two sequences at all), or twice to one.  A
+ * chunk's value that is not finite can reach rows of the chunk before it, whose weight for it is zero.  The workspace needs no initial contents; two calls that run at the same time need one each
  * (small steps need none: 0 bytes). */
 typedef struct b200_attn_paged_args {
   const void* qkv;

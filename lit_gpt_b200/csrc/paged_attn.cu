@@ -784,6 +784,7 @@ struct PagedPlan {
   int64_t items, slots, q;
   int score_rows, kept_max, kw_workers;
   int64_t scores;
+  int64_t steps;                   // bound of what any kernel counts in its list
   size_t bytes;
 };
 constexpr int64_t kScoresMax = (int64_t)1 << 28;   // scores that a step may keep: 1 GB
@@ -816,14 +817,19 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   s.q = rows * per * n_groups * hs;
   s.score_rows = s.kept_max = s.kw_workers = 0;
   s.scores = 0;
+  s.steps = s.list ? tiles : 0;
+  const int64_t steps = (int64_t)n_groups * (rows / (per <= 256 ? 256 / per : 1) + n_seqs) * ((max_length + 127) / 128 + 2);
+  if (s.tensor && steps > s.steps) s.steps = steps;
   if (kw) {
+    const int64_t again = (int64_t)n_groups * ((max_length + 127) / 128) * ((rows * per + 127) / 128 + 2 * (int64_t)n_seqs);
+    if (again > s.steps) s.steps = again;
     s.score_rows = (int)(most < 8 * s.nq ? most : 8 * s.nq);
     if (s.list && path != 3 && tiles * s.score_rows * kShTile <= kScoresMax) {
       s.scores = tiles * s.score_rows * kShTile;
       s.kept_max = s.list_max;
     }
     if (s.tensor || s.kept_max == 0) {
-      const int64_t blocks = (int64_t)n_groups * n_seqs * ((max_length + 127) / 128) * ((max_rows * per + 127) / 128);
+      const double blocks = (double)n_groups * n_seqs * ((max_length + 127) / 128) * ((max_rows * per + 127) / 128);
       s.kw_workers = blocks < sm_count() ? (int)blocks : sm_count();
     }
   }
@@ -908,7 +914,7 @@ extern "C" {
 
 size_t b200_attn_paged_workspace_bytes(int64_t rows, int n_seqs, int n_head, int n_groups, int head_size, int64_t max_rows, int64_t max_length, int key_weights) {
   if (rows <= 0 || n_seqs <= 0 || n_groups <= 0 || n_head <= 0 || n_head % n_groups || max_rows <= 0 || max_rows > rows || max_length <= 0 || (head_size != 64 && head_size != 128) ||
-      rows * n_head >= (1 << 24) || n_seqs > (1 << 20) || max_length >= (1 << 30))
+      rows * n_head >= (1 << 24) || (int64_t)n_seqs * n_groups >= (1 << 24) || max_length >= (1 << 30))
     return 0;
   return paged_plan(rows, n_seqs, n_groups, n_head / n_groups, head_size, max_rows, max_length, key_weights != 0).bytes;
 }
@@ -920,7 +926,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   B200_CHECK_ARG(a->head_size == 64 || a->head_size == 128, "b200_attn_paged: head size %d (64 or 128)", a->head_size);
   B200_CHECK_ARG(a->rows > 0 && a->n_seqs > 0 && a->n_groups > 0 && a->n_head > 0 && a->n_head % a->n_groups == 0, "b200_attn_paged: bad rows, sequences, heads %d or groups %d",
                  a->n_head, a->n_groups);
-  B200_CHECK_ARG(a->rows < (1 << 24) && a->rows * a->n_head < (1 << 24) && a->n_seqs <= (1 << 20), "b200_attn_paged: too many rows or sequences in a step");
+  B200_CHECK_ARG(a->rows < (1 << 24) && a->rows * a->n_head < (1 << 24) && (int64_t)a->n_seqs * a->n_groups < (1 << 24), "b200_attn_paged: too many rows or sequences in a step");
   B200_CHECK_ARG(a->max_rows > 0 && a->max_rows <= a->rows, "b200_attn_paged: sequences of up to %lld rows, of %lld", (long long)a->max_rows, (long long)a->rows);
   B200_CHECK_ARG(a->page >= 16 && a->page <= 256 && (a->page & (a->page - 1)) == 0, "b200_attn_paged: pages of %d keys (16, 32, 64, 128 or 256)", a->page);
   B200_CHECK_ARG(a->pool > 0 && a->table_seqs > 0 && a->max_pages > 0 && a->pages_ld >= a->max_pages, "b200_attn_paged: no pages, or a bad page table");
@@ -937,7 +943,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
                  "b200_attn_paged: pages, result, workspace and the sequences' description must lie on 16-byte boundaries");
   const int per = a->n_head / a->n_groups;
   const PagedPlan s = paged_plan(a->rows, a->n_seqs, a->n_groups, per, a->head_size, a->max_rows, a->max_length, a->key_weights != nullptr);
-  B200_CHECK_ARG(s.items * ((a->max_length + kShTile - 1) / kShTile) < kMaxTiles, "b200_attn_paged: too many keys in a step");
+  B200_CHECK_ARG(s.steps < kMaxTiles, "b200_attn_paged: too many keys in a step");
   B200_CHECK_ARG(a->workspace_bytes >= s.bytes && (a->workspace || s.bytes == 0), "b200_attn_paged: workspace too small");
   if (s.tensor || s.kw_workers > 0) B200_CHECK_WAITS("b200_attn_paged");
   PagedParams p = {};

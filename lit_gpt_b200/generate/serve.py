@@ -501,6 +501,8 @@ def _generate_ruled(model: Any, prompts: Sequence[Sequence[int]], max_new_tokens
             nxt = draw(logits, live)
     finally:
         session.step([], end=ids)   # (also when the grammar raises: the slots are the session's again)
+        if isinstance(model, GPT):
+            K.check_gemv_errors(dev)
 
 
 class Replayer:

@@ -922,7 +922,8 @@ def attn_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, row_pos:
     no keys -- new ones are dropped, the rest take no part.  k_pages / v_pages (pages, G, page, hs) bf16, updated in place, pages of 16, 32, 64, 128 or 256 keys, any distance between pages
     and groups that is a multiple of 8 numbers.  key_weights fp32 (pages, G, page): new keys begin at zero, every key gains the sum of its softmax weights over the step's rows and
     its group's heads.  max_rows, max_length: bounds (on the host) of a sequence's rows and of its keys behind the step; keys from max_length on are dropped.
-    No page belongs to two sequences that bring rows into it.  Returns (rows, H*hs)."""
+    No page belongs to two sequences that bring rows into it (with key_weights: to two sequences at all), or twice to one.  A chunk's value that is not finite can reach rows of
+    the chunk before it, whose weight for it is zero.  Returns (rows, H*hs)."""
     device, bf16 = qkv.get_device(), torch.bfloat16
     if (device < 0 or cos.get_device() != device or sin.get_device() != device or row_pos.get_device() != device or row_seq.get_device() != device or seqs.get_device() != device
             or table.get_device() != device or k_pages.get_device() != device or v_pages.get_device() != device or (key_weights is not None and key_weights.get_device() != device)):
@@ -955,6 +956,7 @@ def attn_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, row_pos:
     if seqs.data_ptr() % 16:
         seqs = seqs.clone()
     table_rows = cos.numel() // max(rope_n_elem, 1)
+    max_rows = min(max_rows, rows)
     n_seqs, (table_seqs, max_pages) = seqs.shape[0], table.shape
     nbytes = _paged_workspace_bytes(device, rows, n_seqs, n_head, n_groups, head_size, max_rows, max_length, key_weights is not None)
     ws = qkv.new_empty(nbytes // 2) if nbytes else None   # of this call: calls on two streams, or in two graphs, have one each

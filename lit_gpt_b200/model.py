@@ -130,7 +130,7 @@ class GPT(nn.Module):
         for c in caches:
             c.step = step
         try:
-            if self.fused_decode_ready(tokens.view(1, n)):
+            if not torch.compiler.is_compiling() and self.fused_decode_ready(tokens.view(1, n)):
                 if n <= FUSED_ROWS:
                     logits = self._fused_decode(tokens.view(n, 1), step.row_pos)[:, 0]
                     return logits if want is None else logits.index_select(0, want)
@@ -634,6 +634,11 @@ class CausalSelfAttention(nn.Module):
             from . import ops  # noqa: F401
 
             o = torch.ops.b200gpt
+            if isinstance(cache, PagedKVCache):
+                s = cache.step
+                y = o.attn_paged(qkv, cos, sin, s.row_pos, s.row_seq, s.seqs, s.table, cache.k, cache.v, c.n_head, c.n_query_groups, c.head_size, c.rope_n_elem, s.max_rows,
+                                 s.max_length, cache.key_weights)
+                return y.view(B, T, c.n_head * c.head_size)
             if T == 1:
                 if isinstance(cache, SharedKVCache):
                     y = o.attn_decode_shared(qkv, cos, sin, input_pos, cache.k, cache.v, cache.k_prefix, cache.v_prefix, cache.prefix_len, c.n_head, c.n_query_groups,

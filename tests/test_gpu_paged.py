@@ -88,6 +88,21 @@ def test_formula(K, formula, hs, groups, per, page, steps):
     check(call(K, d), formula(d))
 
 
+@pytest.mark.parametrize("per,hs", [(70, 64), (130, 128)])
+def test_many_heads_a_group(K, formula, per, hs):
+    d = make([(1, 50), (3, 0), (1, 200)], 1, per, hs, 32, seed=per)
+    check(call(K, d), formula(d))
+
+
+def test_registered_operator(K, formula):
+    from lit_gpt_b200 import ops  # noqa: F401
+
+    d = make([(1, 50), (30, 7)], 2, 2, 64, 16)
+    t = on_gpu(d)
+    out = torch.ops.b200gpt.attn_paged(t["qkv"], t["cos"], t["sin"], t["row_pos"], t["row_seq"], t["seqs"], t["pages"], t["k"], t["v"], 4, 2, 64, 64, t["max_rows"], t["max_length"], t["kw"])
+    check((out, t["k"], t["v"], t["kw"]), formula(d))
+
+
 @pytest.mark.parametrize("hs,groups,per", [(64, 1, 1), (128, 3, 4), (64, 2, 8), (128, 2, 9), (64, 1, 16), (128, 2, 1)])
 @pytest.mark.parametrize("page", [16, 128])
 @pytest.mark.parametrize("cached", [[0], [1, 31, 32], [500], [900, 0, 63, 1300, 64], [127] * 9])

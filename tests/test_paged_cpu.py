@@ -26,7 +26,9 @@ def test_attention_arguments_are_checked():
                      (dict(qkv=None), "null"), (dict(row_seq=None), "null"), (dict(pages=None), "null"), (dict(v_pages=None), "null"), (dict(out=None), "null"), (dict(rope_n_elem=66), "rope"),
                      (dict(rope_n_elem=3), "rope"), (dict(cos=None), "tables"), (dict(table_rows=0), "tables"), (dict(table_preselected=1, table_rows=4), "preselected"),
                      (dict(table_dtype=C.F16), "tables"), (dict(k_pages=FAKE + 2), "16-byte"), (dict(v_group_stride=1028), "16-byte"), (dict(seqs=FAKE + 4), "16-byte"), (dict(out=FAKE + 8), "16-byte"),
-                     (dict(key_weights=FAKE + 2), "16-byte"), (dict(workspace_bytes=16), "workspace")):
+                     (dict(key_weights=FAKE + 2), "16-byte"), (dict(workspace_bytes=16), "workspace"),
+                     (dict(rows=1 << 20, max_rows=1 << 20, max_length=1 << 29, max_pages=1 << 25, pages_ld=1 << 25), "too many keys"),
+                     (dict(rows=1 << 20, max_rows=1, max_length=1 << 29, max_pages=1 << 25, pages_ld=1 << 25), "too many keys")):
         refused(call(**kw), text)
     refused(lib.b200_attn_paged(None, None), "null")
     need = lib.b200_attn_paged_workspace_bytes
