@@ -35,6 +35,7 @@ struct PagedParams {
   int workers, sms;                                         // warps that share the tiles, at most
   float* acc; float2* ml;                                   // results of key ranges: slots of tile_rows queries
   int2* where;                                              // per item: the first worker that has tiles of it, and how many workers have
+  int mixed, list_ns, tensor_ns;                            // the list beside the tensor memory; what a tile of either takes
   int list_max;                                             // sequences of more queries a group are left to the tensor memory (paged_attn_tc05.cu)
   int tc_rows;                                              // rows of a block of theirs: 256 queries at most
   int tc_workers;                                           // CTAs that share their tiles, at most
@@ -64,6 +65,30 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int s) {
   q.n = fits ? min(q.cached + q.rows, p.max_length) : 0;
   return q;
 }
+__device__ __forceinline__ int seq_items(const PagedParams& p, const PagedSeq& s) {   // of the list, of a group
+  return s.rows > 0 && s.rows * p.per <= p.list_max ? (s.rows * p.per + p.tile_rows - 1) / p.tile_rows : 0;
+}
+__device__ __forceinline__ int seq_tiles(const PagedSeq& s) { return (s.n + 31) / 32; }
+
+// Single tokens beside chunks: the list and the tensor memory run at the same time, on SMs of their own, as many as their work (in ns, of a group) asks for.  Both kernels come to the same
+// numbers, whole ones, each from its own look at the sequences.  What a step of either costs an SM: 16 KB of keys and values at 45 GB/s, 128 keys of 256 queries 3.4 us (beside the list; 2.1 alone); half heads 0.5 and
+// 0.75 of it.  us in a captured graph, one after the other and so: 32 tokens over 100 - 3001 keys beside 512 rows, 8 groups of 4 heads, 89, 75; 3 over 16000 beside 512 81, 78; 8 over 300 beside
+// 64, 32 groups, 32, 26; 64 over 500 beside 1000 rows behind 3000 131, 134; 2 over 100 beside 2048 103, 102.  (With 2.1 us 88, 98, 28, 142, 102; with 4.2 73, 73, 26, 150, 102.)
+struct Shares { unsigned long long list, tensor; };
+__device__ __forceinline__ void add_work(const PagedParams& p, const PagedSeq& s, Shares& w) {
+  w.list += (unsigned long long)seq_items(p, s) * seq_tiles(s) * p.list_ns;
+  if (s.rows > 0 && s.rows * p.per > p.list_max) {
+    const int blocks = (s.rows + p.tc_rows - 1) / p.tc_rows;
+    w.tensor += (unsigned long long)blocks * (2 + (s.n - s.rows / 2 + 127) / 128) * p.tensor_ns;
+  }
+}
+__device__ __forceinline__ int tensor_share(const PagedParams& p, const Shares& w) {   // of the SMs
+  if (w.list == 0) return p.sms;
+  if (w.tensor == 0) return 0;
+  const double f = (double)w.tensor / ((double)w.tensor + (double)w.list);
+  return min(max((int)(f * p.sms + 0.5), 1), p.sms - 1);
+}
+
 // the page of keys [index << shift, ...) of a row of the page table; -1: there is none
 __device__ __forceinline__ int page_at(const PagedParams& p, int table, int index) {
   if (index >= p.max_pages) return -1;

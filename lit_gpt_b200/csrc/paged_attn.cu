@@ -156,20 +156,19 @@ __device__ __forceinline__ int worker_of(int tile, const Split& s) {
 }
 __device__ __forceinline__ int first_tile(int w, const Split& s) { return w * s.each + min(w, s.more); }
 
-__device__ __forceinline__ int seq_items(const PagedParams& p, const PagedSeq& s) {   // of a group
-  return s.rows > 0 && s.rows * p.per <= p.list_max ? (s.rows * p.per + p.tile_rows - 1) / p.tile_rows : 0;
-}
-__device__ __forceinline__ int seq_tiles(const PagedSeq& s) { return (s.n + kShTile - 1) / kShTile; }
-
 // Sequences are summed in runs of one per thread: sums[t] = tiles and items (of one group) of the sequences before run t, sums[THREADS] of all.
+// `ctas`: the CTAs that take part.
 template <int THREADS>
-__device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, int2* s_warp, bool note) {
+__device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, int2* s_warp, bool note, int& ctas) {
+  __shared__ Shares s_shares[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = (p.n_seqs + THREADS - 1) / THREADS;
   // (a description whose sequences overlap can hold more tiles than fit the step's limits: then none is done)
   int2 here = make_int2(0, 0);
+  Shares work = {0ull, 0ull};
   for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
     const PagedSeq s = paged_seq(p, i);
     const int items = seq_items(p, s);
+    if (p.mixed) add_work(p, s, work);
     here.x = capped(here.x + (int64_t)items * seq_tiles(s));
     here.y = capped((int64_t)here.y + items);
   }
@@ -180,7 +179,20 @@ __device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, in
     if (lane >= o) { inc.x = capped((int64_t)inc.x + x); inc.y = capped((int64_t)inc.y + y); }
   }
   if (lane == 31) s_warp[warp] = inc;
+  if (p.mixed) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      work.list += __shfl_xor_sync(0xffffffffu, work.list, o);
+      work.tensor += __shfl_xor_sync(0xffffffffu, work.tensor, o);
+    }
+    if (lane == 0) s_shares[warp] = work;
+  }
   __syncthreads();
+  if (p.mixed) {
+    work = {0ull, 0ull};
+    for (int w = 0; w < THREADS / 32; ++w) { work.list += s_shares[w].list; work.tensor += s_shares[w].tensor; }
+    ctas = max(p.sms - tensor_share(p, work), 1);
+  }
   int2 before = make_int2(inc.x - here.x, inc.y - here.y);
   for (int w = 0; w < warp; ++w) { before.x = capped((int64_t)before.x + s_warp[w].x); before.y = capped((int64_t)before.y + s_warp[w].y); }
   sums[tid] = before;
@@ -201,7 +213,7 @@ __device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, in
   }
   s.all = all < kMaxTiles && items <= p.items ? (int)all : 0;
   // two tiles a worker at least, unless that leaves SMs without one
-  s.workers = min(max(s.all / 2, min(s.all, p.sms)), p.workers);
+  s.workers = min(max(s.all / 2, min(s.all, ctas)), p.workers / (int)gridDim.x * ctas);
   s.each = s.workers ? s.all / s.workers : 0;
   s.more = s.all - s.each * s.workers;
   return s;
@@ -320,9 +332,12 @@ __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_ker
   __shared__ int2 s_sums[T + 1], s_warp[C::kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tq = lane & 3;
   griddep_launch();
-  const Split s = make_split<T>(p, s_sums, s_warp, blockIdx.x == 0);
-  const int w = warp * (int)gridDim.x + (int)blockIdx.x;   // (workers beside each other on different SMs)
-  if (w >= s.workers) {
+  int ctas = gridDim.x;
+  const Split s = make_split<T>(p, s_sums, s_warp, blockIdx.x == 0, ctas);
+  const int w = warp * ctas + (int)blockIdx.x;             // (workers beside each other on different SMs)
+  // Beside the tensor memory's kernel, which lets this one begin once the append kernel has ended, the wait is for that kernel: at the end, so that what comes next finds both done.
+  const bool late = p.mixed;
+  if (w >= s.workers || (int)blockIdx.x >= ctas) {
     griddep_wait();
     return;
   }
@@ -356,7 +371,7 @@ __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_ker
     if (n) load_k(ring + 2 * C::kUnit, coming);
   };
   early(true);
-  griddep_wait();
+  if (!late) griddep_wait();
   early(false);
   load_queries(sq, cur);
   int qb = 0, next_qb = 0;                                 // the query buffers of either
@@ -436,6 +451,7 @@ __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_ker
     }
   }
   pf_wait<0>();
+  if (late) griddep_wait();
 }
 
 // An item of the tensor memory's that several CTAs had segments of (paged_attn_tc05.cu): CTA (w, part) joins a share of its queries, 32 at a time, for the w-th worker's beginning within it.  A query a lane, HS / 8
@@ -808,11 +824,12 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   const int warps = hs == 64 ? (s.nq == 4 ? PgSmem<64, 4>::kWarps : PgSmem<64, 1>::kWarps) : (s.nq == 4 ? PgSmem<128, 4>::kWarps : PgSmem<128, 1>::kWarps);
   const int64_t tiles = s.items * ((max_length + kShTile - 1) / kShTile);
   s.ctas = sm_count();
-  if (s.ctas > tiles) s.ctas = (int)tiles;
-  s.workers = s.ctas * warps < tiles ? s.ctas * warps : (int)tiles;
+  if (s.ctas > tiles && !(s.tensor && s.list)) s.ctas = (int)tiles;
+  s.workers = s.ctas * warps;
   s.slots = s.list ? (s.items + s.workers) * 8 * s.nq : 0;
   const int64_t blocks = s.tensor ? (int64_t)n_groups * (rows / (256 / per) + n_seqs) * ((max_length + 127) / 128) : 0;
-  s.tc_workers = blocks < sm_count() ? (int)blocks : sm_count();
+  s.tc_workers = blocks < sm_count() && !(s.tensor && s.list) ? (int)blocks : sm_count();
+  if (!s.tensor) s.tc_workers = 0;
   const int64_t tc_slots = (int64_t)s.tc_workers * 2 * 256;
   s.q = rows * per * n_groups * hs;
   s.score_rows = s.kept_max = s.kw_workers = 0;
@@ -964,6 +981,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.q = (__nv_bfloat16*)a->workspace;
   p.acc = (float*)(p.q + s.q);
   p.ml = (float2*)(p.acc + s.slots * a->head_size);
+  p.mixed = s.tensor && s.list; p.list_ns = a->head_size == 64 ? 182 : 364; p.tensor_ns = a->head_size == 64 ? 2550 : 3400;
   p.list_max = s.list_max; p.tc_workers = s.tc_workers; p.tc_rows = per <= 256 ? 256 / per : 1;
   p.tc_acc = (float*)(p.ml + s.slots);
   p.tc_ml = (float2*)(p.tc_acc + (int64_t)s.tc_workers * 512 * a->head_size);

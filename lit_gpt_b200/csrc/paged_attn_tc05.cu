@@ -84,6 +84,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   __shared__ int s_segs, s_more;
   __shared__ uint32_t s_tmem;
   __shared__ int s_sums[kPtThreads + 1], s_warp[kPtThreads / 32];
+  __shared__ Shares s_shares[kPtThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t smem = (tc::smem_u32(pt_smem) + 1023u) & ~1023u;
   const uint32_t sq_ = smem, sk_ = smem + 2 * C::kBytes, sv_ = smem + 4 * C::kBytes;
@@ -91,14 +92,19 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   const uint32_t k_full = bars, v_full = bars + 16, k_empty = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_half = bars + 80, p_full = bars + 96,
                  o_done = bars + 112, q_full = bars + 128, shrink = bars + 136, idle = bars + 200;   // shrink: one per softmax warp; idle: products that gave up
 
-  griddep_launch();
+  if (!p.mixed) griddep_launch();
   // ---- this CTA's part of the list: from the step's description, which was there before the append kernel ----
   const int run = (p.n_seqs + kPtThreads - 1) / kPtThreads;
   int here = 0;
+  Shares work = {0ull, 0ull};
   for (int k = 0; k < run; ++k) {
     const int i = tid * run + k;
     Blocks mine = {};
-    if (i < p.n_seqs) mine = blocks_of(p, paged_seq(p, i));
+    if (i < p.n_seqs) {
+      const PagedSeq s = paged_seq(p, i);
+      mine = blocks_of(p, s);
+      if (p.mixed) add_work(p, s, work);
+    }
     if (mine.count <= 16) {
       for (int e = 0; e < mine.count; ++e) here = capped((int64_t)here + mine.steps(e));
     }
@@ -121,6 +127,14 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     if (lane >= o) inc = capped((int64_t)inc + x);
   }
   if (lane == 31) s_warp[warp] = inc;
+  if (p.mixed) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      work.list += __shfl_xor_sync(0xffffffffu, work.list, o);
+      work.tensor += __shfl_xor_sync(0xffffffffu, work.tensor, o);
+    }
+    if (lane == 0) s_shares[warp] = work;
+  }
   if (tid == 0) {
     tc::mbar_init(q_full, 1);
     tc::mbar_init(idle, 1);
@@ -145,8 +159,24 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   __syncthreads();
   const int64_t all64 = (int64_t)s_sums[kPtThreads] * p.n_groups;
   const int all = all64 < kMaxTiles ? (int)all64 : 0;      // (a description whose sequences overlap can hold more: then none is done)
+  int ctas = gridDim.x;
+  if (p.mixed) {                        // the list's kernel takes the other SMs: it may begin once the append kernel has ended
+    work = {0ull, 0ull};
+    for (int w = 0; w < kPtThreads / 32; ++w) { work.list += s_shares[w].list; work.tensor += s_shares[w].tensor; }
+    ctas = tensor_share(p, work);
+    if ((int)blockIdx.x >= ctas) {
+      griddep_wait();
+      griddep_launch();
+      if (tid == 0) {
+        PagedCut c = {};
+        c.last = -1;
+        p.cuts[blockIdx.x] = c;
+      }
+      return;
+    }
+  }
   if (warp == 0) {
-    const int workers = min(max(all / 2, min(all, p.sms)), p.tc_workers), w = blockIdx.x;
+    const int workers = min(max(all / 2, min(all, ctas)), ctas), w = blockIdx.x;
     const int each = workers ? all / workers : 0, more = all - each * workers;
     const int first = w * each + min(w, more), end = w < workers ? first + each + (w < more ? 1 : 0) : first;
     ListAt at = {};
@@ -247,6 +277,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   };
   if (tid == 0) list_segments();
   griddep_wait();                         // (tensor memory is taken behind the wait only)
+  if (p.mixed) griddep_launch();
   if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
   if (tid == 0) p.cuts[blockIdx.x] = s_cut;
   tc::fence_before();
