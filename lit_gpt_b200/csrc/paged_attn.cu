@@ -213,7 +213,7 @@ __device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, in
   }
   s.all = all < kMaxTiles && items <= p.items ? (int)all : 0;
   // two tiles a worker at least, unless that leaves SMs without one
-  s.workers = min(max(s.all / 2, min(s.all, ctas)), p.workers / (int)gridDim.x * ctas);
+  s.workers = min(max(s.all / 2, min(s.all, ctas)), p.mixed ? p.workers / (int)gridDim.x * ctas : p.workers);
   s.each = s.workers ? s.all / s.workers : 0;
   s.more = s.all - s.each * s.workers;
   return s;
@@ -825,7 +825,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   const int64_t tiles = s.items * ((max_length + kShTile - 1) / kShTile);
   s.ctas = sm_count();
   if (s.ctas > tiles && !(s.tensor && s.list)) s.ctas = (int)tiles;
-  s.workers = s.ctas * warps;
+  s.workers = s.ctas * warps < tiles || (s.tensor && s.list) ? s.ctas * warps : (int)tiles;
   s.slots = s.list ? (s.items + s.workers) * 8 * s.nq : 0;
   const int64_t blocks = s.tensor ? (int64_t)n_groups * (rows / (256 / per) + n_seqs) * ((max_length + 127) / 128) : 0;
   s.tc_workers = blocks < sm_count() && !(s.tensor && s.list) ? (int)blocks : sm_count();
