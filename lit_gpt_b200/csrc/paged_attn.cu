@@ -3,13 +3,19 @@
 // The rounding points are those of the model's step (lit_gpt/model.py:624-653, 767-773): q and k are bf16 after the rotation, the softmax is fp32 with a running maximum,
 // the result is rounded once.  A row that sees no key has a result of zero.
 //
-// Few single tokens: one launch, a cluster of CTAs for a sequence and group.  Else three: queries and new keys are turned and the new rows stored in their pages; warps compute partial results (maximum, sum, unscaled output) over tiles of 32 keys;
-// a head's partial results are joined.  No counter or flag is left between calls, and two calls at a time share nothing.
+// Few single tokens: one launch, a cluster of CTAs for a sequence and group (paged_cluster_kernel).  Else queries and new keys are turned and the new rows stored in their pages
+// (paged_append_wide_kernel); sequences of few queries a group -- single tokens -- are the list's (paged_list_kernel), the others the tensor memory's (paged_attn_tc05.cu), at the same time where a
+// step has both; their partial results are joined (paged_join_kernel).  No counter or flag is left between calls, and two calls at a time share nothing.
 //
-// An item is a tile of queries of one sequence and group -- rows times heads of the group, row after row, so that the heads of a group share the keys that they read -- against the
-// sequence's keys.  The tiles of all items are one list, cut evenly over the warps of all SMs (attn_list.cuh): requests of unequal lengths leave no SM without work.
+// The list: an item is a tile of queries of one sequence and group -- rows times heads of the group, row after row, so that the heads of a group share the keys that they read -- against
+// the sequence's keys, in tiles of 32.  The tiles of all items are one list, cut evenly over the warps of all SMs (attn_list.cuh): requests of unequal lengths leave no SM without work.
 //
-// With the weights of keys wanted (paged_weights.cu), the list keeps its scores beside the results, and a launch behind the join adds up what every key received: no key is read again.
+// With the weights of keys wanted, the list keeps its scores beside the results, and a launch behind the join adds up what every key received: no key is read again.  What chunks' keys
+// receive is computed from the joined sums (paged_weights.cu).
+//
+// Bound: single tokens by the bytes of their keys and values: 64 of 8 groups of 4 heads over 5 - 16000 keys, 2.1 GB, 325 us, 6.45 TB/s; 16 of 32 groups over 2047 with weights, 546 MB, 104 us, 83 of
+// them the bytes: the rest the append's and the join's launches and the scores (with the keys read again for them 190).  Few of them by latency: 1 token of 32 groups over 300 keys 7.5 us (12.5 in
+// three launches).  Beside chunks: 32 tokens over 100 - 3001 keys and 512 rows behind 1024 75 us, where either alone takes 40 and 30.
 #include "attn_list.cuh"
 #include "paged.cuh"
 
@@ -29,6 +35,8 @@ __device__ __forceinline__ int64_t paged_pos(const PagedParams& p, int row) {
 // ---- the queries and the new keys turned, the new rows stored ----
 // A CTA takes a row, or some heads of one: HS / 16 threads a head, each with sixteen numbers of it, eight and the eight that they turn with (or, where nothing is turned, any sixteen), whose cosines
 // and sines it keeps from head to head.  Needs rows of heads and tables for accesses of 16 bytes, and halves of the rotation that are multiples of eight numbers (or no rotation).
+// Bound: bytes in flight behind the look-up of the row's place, three loads one after the other: 4096 rows of 32 groups of 1 head, 200 MB, 44 us, 4.6 TB/s (a head a warp 112; three
+// CTAs an SM 48; three heads a thread on their way at a time, two CTAs an SM, 52).
 template <int HS>
 __global__ void __launch_bounds__(256, 4) paged_append_wide_kernel(const PagedParams p) {
   constexpr int TH = HS / 16, HEADS = 256 / TH;    // threads of a head; heads at once

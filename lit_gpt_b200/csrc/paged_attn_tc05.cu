@@ -3,8 +3,8 @@
 // An item is a block of up to 256 queries of one sequence and group -- whole rows, every head of the group -- against the keys that its last row sees, in tiles of 128.  The key tiles of
 // all items are one list, cut evenly over the CTAs, one an SM: neither few rows over many keys nor chunks of unequal lengths leave SMs without work.  A CTA's part of an item is a segment.
 // The result of an item that is one CTA's is stored at once; else every segment leaves maxima, sums and unscaled outputs, and the step's join (paged_attn.cu) puts them together.
-//   * warps 0-3 and 4-7: the softmax of the block's first and second 128 queries, one per thread.  S (128 columns of tensor memory) is read into registers, the
-//     probabilities go back over it as bf16, the left operand of P V, in two halves so that P V starts on the first (attn_tc05.cu says what was tried);
+//   * warps 0-3 and 4-7: the softmax of the block's first and second 128 queries, one per thread.  S (128 columns of tensor memory) is read into registers once, as many as the
+//     other warps give up; the probabilities go back over it as bf16, the left operand of P V, in two halves so that P V starts on the first;
 //   * warps 8-11: when a row's maximum grew, they shrink its O in tensor memory while its exponentials are still being taken;
 //   * warp 12: one thread issues S = Q K^T and O += P V, 128 x 128 x 16 each, S of a tile's next step right behind its P V;
 //   * warp 13 brings the keys and the queries, warp 14 the values, two stages each, 128-byte-swizzled: a page, or what of it lies in the tile, is one TMA box; values of a tile that
@@ -13,6 +13,11 @@
 // tile of 128 keys and 128 queries.
 // Probabilities are rounded to bf16 as they multiply V; the running maximum is exact, so that the largest probability is 1 and loses nothing.  They are summed before the rounding: the
 // keys' weights are taken from these sums (of rounded ones a result's error against 64 bits is 0.1 to 0.4 % smaller, a weight's thousands of times larger).
+//
+// Bound: a stream's chain of scores, maximum, exponentials and output, which the other stream fills in part: a tile of 256 queries takes 3800 clocks where its products and its exponentials take
+// 2048 each.  4096 rows of 32 groups of 1 head 163 us, 0.84 PFLOP/s of the causal half (half of S read twice: 178); 613 rows behind 1500 keys, 8 groups of 4 heads, 33 us, 5 of them the way to the
+// first tile.  Not taken: half of a query's scores a thread, sixteen softmax warps at 80 registers: the step with 4096 rows 223 -> 275 us.  A segment's results stored a query a thread in whole rows:
+// 4 us each; four numbers of 128 queries side by side: 2.
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
