@@ -70,7 +70,8 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
   using C = KwTile<HS>;
   extern __shared__ __align__(1024) uint8_t kw_smem[];
   __shared__ __align__(8) uint64_t s_bars[29];
-  __shared__ __align__(16) float s_lse[8][128];            // of the last eight tiles of queries, negative
+  __shared__ __align__(16) float s_lse[8][128];            // of the last eight tiles of queries, negative: tile i + 8's are written once the products of tile i + 4 are done, whose scores
+                                                           // take the place of tile i's
   __shared__ float s_sum[128];
   __shared__ KwSeg s_seg[kKwSegs];
   __shared__ KwAt s_at;
@@ -366,10 +367,10 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
           tc::ld32(y, at + 96);
           add(x, 2);
           tc::wait_ld(y);
+          add(y, 3);
           tc::fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(s_empty + 8 * s);
-          add(y, 3);
+          if (lane == 0) tc::mbar_arrive(s_empty + 8 * s);   // (behind the last look at the queries' lse: their place is taken again four tiles after the scores')
         }
         if (!ok) break;
         float a, b, d, h;

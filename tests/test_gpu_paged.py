@@ -131,6 +131,38 @@ def test_long(K, formula, steps, per, hs):
     check(call(K, d), formula(d))
 
 
+@pytest.mark.parametrize("rows,cached,per,hs", [(3000, 4100, 3, 64), (1300, 2000, 8, 128), (4000, 0, 1, 128)])
+def test_weights_of_long_chunks(E, rows, cached, per, hs):
+    """Many tiles of queries for every key.  The formula on the GPU in 64 bits, from the keys that the step has stored; the bound as in paged_oracle."""
+    G, page = 2, 64
+    d = make([(rows, cached)], G, per, hs, page, seed=rows)
+    t = on_gpu(d)
+    before = t["kw"].clone()
+    out = launch(E, t)
+    at = t["pages"][d["seqs"][0, 3]].long()
+    n = rows + cached
+    ids, slots = at[torch.arange(n, device="cuda") // page], torch.arange(n, device="cuda") % page
+    keys = t["k"][ids, :, slots].to(F64)                                   # (n, G, hs)
+    heads = t["qkv"].view(rows, G, per + 2, hs)
+    q = oracle.turn(heads[:, :, :per], t["cos"][cached:][:, None, None], t["sin"][cached:][:, None, None], hs).to(F64)
+    got, err = torch.zeros(n, G, dtype=F64, device="cuda"), torch.zeros(n, G, dtype=F64, device="cuda")
+    for lo in range(0, rows, 250):
+        hi = min(lo + 250, rows)
+        s = torch.einsum("igph,jgh->gpij", q[lo:hi], keys) / hs ** 0.5
+        size = torch.einsum("igph,jgh->gpij", q[lo:hi].abs(), keys.abs()).amax() / hs ** 0.5
+        s = s.masked_fill(torch.arange(n, device="cuda") > cached + torch.arange(lo, hi, device="cuda")[:, None], float("-inf"))
+        w = torch.softmax(s, -1).sum((1, 2)).T
+        off = 2 * (hs + 2) * 2 ** -24 * size + 2 ** -23 * 2 * s[s > float("-inf")].abs().amax() + 2 ** -22 + (n + 64) * 2 ** -24
+        got += w
+        err += 2 * off * w
+    old = before[ids, :, slots].to(F64)
+    old[cached:] = 0
+    over = (t["kw"][ids, :, slots].to(F64) - (old + got)).abs() - err - (rows * per + 8) * 2 ** -24 * (old + got)
+    assert over.max().item() <= 0, over.max().item()
+    again = on_gpu(d)
+    assert same(out, launch(E, again)) and same(t["kw"], again["kw"])
+
+
 def test_many_sequences(K, formula):
     """More sequences than a CTA has threads."""
     d = make([(1 if i % 3 else 0, i % 50) for i in range(1500)], 1, 2, 64, 16, seed=4)
