@@ -205,9 +205,10 @@ __device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const
     __syncthreads();
   }
   if (!any) __syncthreads();                       // (the weights are there)
-  // a run of keys a thread: those above, and the first `need` of those that equal it
-  const int run = (n + THREADS - 1) / THREADS, begin = min(n, tid * run), end = min(n, begin + run);
+  // a run of keys a thread, an odd number of them so that the threads meet all banks: those above, and the first `need` of those that equal it
+  const int run = ((n + THREADS - 1) / THREADS) | 1, begin = min(n, tid * run), end = min(n, begin + run);
   int above = 0, ties = 0;
+#pragma unroll 4
   for (int i = begin; i < end; ++i) {
     const uint32_t u = ordered(h.w[i]);
     const bool mid = i >= lo && i < hi;
