@@ -2,13 +2,14 @@
 // the front of the sequence's pages.
 //
 // One launch where a sequence's weights, places and pages fit into shared memory: a cluster of CTAs per sequence and group.  Every CTA finds the smallest weight that stays by radix
-// selection over the weights as ordered whole numbers (11, 11 and 10 bits) and the places that stay by a scan, a run of keys a thread; then the cluster moves keys, values and
-// weights in place.  A key moves to a lower index or stays: a cluster that goes through its rows in order, reads a tile of them before it writes them, and has a barrier between, never
-// writes what is still to be read.  Longer sequences: a launch that chooses (weights read for every digit, eight bits each, and scanned in rounds), a launch that moves.
+// selection over the weights as ordered whole numbers (11, 11 and 10 bits) and the places that stay by a scan, a run of keys a thread (of long sequences the cluster's CTAs each have a part of
+// the keys); then the cluster moves keys, values and weights in place.  A key moves to a lower index or stays: a cluster that goes through its rows in order, reads a tile of them before it
+// writes them, and has a barrier between, never writes what is still to be read.  What does not fit: a launch that chooses (weights read for every digit, eight bits each, and scanned in
+// rounds), a launch that moves.
 //
-// Bound: bytes of the rows that stay, read and written, behind the choice, which is a chain on one SM.  us in a captured graph: 1 sequence of 32 groups cut from 576 keys to 512 9.4 (choice and
-// move in two launches 14.3); 16 of 8 groups from 3001 - 8001 to 2048 59, 4.6 TB/s (two launches 77; pieces of 32 bytes of a row a CTA 119); 1 of 12 groups, 64 numbers a head,
-// from 30001 to 8191 38, about 22 of them the choice (weights not held 151).  512 threads with twice the rows each: 62 and 50.
+// Bound: bytes of the rows that stay, read and written, behind the choice, which is a chain.  us in a captured graph: 1 sequence of 32 groups cut from 576 keys to 512 9.3 (choice and
+// move in two launches 14.3); 16 of 8 groups from 3001 - 8001 to 2048 58, 4.7 TB/s (two launches 77; pieces of 32 bytes of a row a CTA 119); 1 of 12 groups, 64 numbers a head,
+// from 30001 to 8191 33 (two launches 151).  512 threads with twice the rows each: 62 and 50 (of 38, each CTA choosing for itself).
 #include "common.cuh"
 
 namespace b200 {
@@ -141,15 +142,32 @@ __device__ __forceinline__ int block_before(int a, int* s_warp) {
 }
 
 struct Held {                                      // in dynamic shared memory
-  float* w;                                        // [max_length] weights
+  float* w;                                        // weights: of all keys, or of this CTA's
   int* from;                                       // [keep] where what moves to each place comes from
   int* table;                                      // the sequence's pages
 };
 
-// By a whole CTA: whether the sequence is cut down; if so, its pages, its weights and the places that stay.
-template <int THREADS>
-__device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const Held& h) {
-  __shared__ int s_hist[kBinCopies * kBins];
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t smem_of(const void* at, int rank) {   // the same place in another CTA of the cluster
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ int2 other_pair(const int* at, int rank) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_of(at, rank)) : "memory");
+  return v;
+}
+
+// Whether the sequence is cut down; if so, its pages, its weights and the places that stay.  By every CTA for itself; or, SPLIT, by the cluster: each CTA has as many keys' weights, one part behind
+// the other, and counts their digits, all add up the counts; what comes to a place is told the CTA that moves it (places go round by `tile`), and the weights move at once.
+template <int THREADS, bool SPLIT>
+__device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const Held& h, int rank, int ctas, int tile) {
+  __shared__ __align__(8) int s_hist[kBinCopies * kBins];   // copies; SPLIT: this digit's and the one's before
+  __shared__ __align__(8) int s_counts[2];                  // of this CTA's keys: above, equal
   __shared__ int s_warp[THREADS / 32], s_pick[2];
   const int tid = threadIdx.x, warp = tid >> 5, page = 1 << p.shift;
   const int n = p.lengths[s], row = p.rows ? p.rows[s] : s;
@@ -165,8 +183,10 @@ __device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const
   }
   cut = __syncthreads_and(all);
   if (!cut) return false;
+  const int each = SPLIT ? (n + ctas - 1) / ctas : n, k0 = SPLIT ? min(rank * each, n) : 0, k1 = SPLIT ? min(k0 + each, n) : n;   // keys that this CTA looks at
+  auto at = [&](int i) -> float* { return p.kw + (((int64_t)h.table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1)); };
 #pragma unroll 8
-  for (int i = tid; i < n; i += THREADS) h.w[i] = p.kw[(((int64_t)h.table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1))];
+  for (int i = k0 + tid; i < k1; i += THREADS) h.w[i - k0] = *at(i);
   const int lo = p.first, hi = n - p.recent;
   int need = p.keep - p.first - p.recent;
   const bool any = need > 0;
@@ -174,28 +194,38 @@ __device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const
   // digits of 11, 11 and 10 bits
   for (int digit = 0; digit < 3 && any; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-    for (int i = tid; i < kBinCopies * kBins; i += THREADS) s_hist[i] = 0;
+    int* const hist = SPLIT ? s_hist + (digit & 1) * kBins : s_hist;
+    for (int i = tid; i < (SPLIT ? 1 : kBinCopies) * kBins; i += THREADS) hist[i] = 0;
     __syncthreads();                               // (and: the weights are there)
+    int* const mine = SPLIT ? hist : hist + warp % kBinCopies * kBins;
 #pragma unroll 4
-    for (int i = lo + tid; i < hi; i += THREADS) {
-      const uint32_t u = ordered(h.w[i]);
-      if (digit == 0 || u >> (shift + bits) == high) atomicAdd(&s_hist[warp % kBinCopies * kBins + ((u >> shift) & ((1u << bits) - 1u))], 1);
+    for (int i = max(lo, k0) + tid; i < min(hi, k1); i += THREADS) {
+      const uint32_t u = ordered(h.w[i - k0]);
+      if (digit == 0 || u >> (shift + bits) == high) atomicAdd(&mine[(u >> shift) & ((1u << bits) - 1u)], 1);
     }
-    __syncthreads();
-    // a thread has some digits next to each other, the greater ones first
-    constexpr int D = kBins / THREADS;
-    const int top = kBins - 1 - D * tid;
-    int c[D], sum = 0;
+    if (SPLIT) cluster_sync();                     // (who is past it has read the counts of the digit before)
+    else __syncthreads();
+    // a thread has two digits next to each other, the greater one first
+    static_assert(kBins == 2 * THREADS, "two digits a thread");
+    const int top = kBins - 1 - 2 * tid;
+    int c[2] = {0, 0};
+    if (SPLIT) {
+#pragma unroll 8
+      for (int k = 0; k < ctas; ++k) {
+        const int2 v = other_pair(hist + top - 1, k);
+        c[0] += v.y;
+        c[1] += v.x;
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < D; ++j) {
-      c[j] = 0;
-#pragma unroll
-      for (int k = 0; k < kBinCopies; ++k) c[j] += s_hist[k * kBins + top - j];
-      sum += c[j];
+      for (int k = 0; k < kBinCopies; ++k) {
+        c[0] += hist[k * kBins + top];
+        c[1] += hist[k * kBins + top - 1];
+      }
     }
-    int before = block_before<THREADS>(sum, s_warp);
+    int before = block_before<THREADS>(c[0] + c[1], s_warp);
 #pragma unroll
-    for (int j = 0; j < D; ++j) {
+    for (int j = 0; j < 2; ++j) {
       if (before < need && need <= before + c[j]) { s_pick[0] = top - j; s_pick[1] = need - before; }
       before += c[j];
     }
@@ -206,46 +236,67 @@ __device__ __forceinline__ bool choose(const EvictParams& p, int s, int g, const
   }
   if (!any) __syncthreads();                       // (the weights are there)
   // a run of keys a thread, an odd number of them so that the threads meet all banks: those above, and the first `need` of those that equal it
-  const int run = ((n + THREADS - 1) / THREADS) | 1, begin = min(n, tid * run), end = min(n, begin + run);
+  const int run = ((k1 - k0 + THREADS - 1) / THREADS) | 1, begin = min(k1, k0 + tid * run), end = min(k1, begin + run);
   int above = 0, ties = 0;
 #pragma unroll 4
   for (int i = begin; i < end; ++i) {
-    const uint32_t u = ordered(h.w[i]);
+    const uint32_t u = ordered(h.w[i - k0]);
     const bool mid = i >= lo && i < hi;
     above += !mid || (any && u > high);
     ties += mid && any && u == high;
   }
-  const int above_before = block_before<THREADS>(above, s_warp);
-  int equal = block_before<THREADS>(ties, s_warp), place = above_before + min(equal, need);
+  int above_before = block_before<THREADS>(above, s_warp);
+  int equal = block_before<THREADS>(ties, s_warp);
+  if (SPLIT) {
+    if (tid == THREADS - 1) { s_counts[0] = above_before + above; s_counts[1] = equal + ties; }
+    cluster_sync();                                // (and: every weight has been read)
+    for (int k = 0; k < rank; ++k) {
+      const int2 v = other_pair(s_counts, k);
+      above_before += v.x;
+      equal += v.y;
+    }
+  }
+  int place = above_before + min(equal, need);
   for (int i = begin; i < end; ++i) {
-    const uint32_t u = ordered(h.w[i]);
+    const float w = h.w[i - k0];
+    const uint32_t u = ordered(w);
     const bool mid = i >= lo && i < hi, tie = mid && any && u == high;
-    if (!mid || (any && u > high) || (tie && equal < need)) h.from[place++] = i;
+    if (!mid || (any && u > high) || (tie && equal < need)) {
+      if (SPLIT) {
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(smem_of(h.from + place, place / tile % ctas)), "r"(i) : "memory");
+        *at(place) = w;
+      } else {
+        h.from[place] = i;
+      }
+      ++place;
+    }
     equal += tie;
   }
-  __syncthreads();
+  if (SPLIT) cluster_sync();
+  else __syncthreads();
   return true;
 }
-__device__ __forceinline__ Held held_of(const EvictParams& p, float* smem) {
+__device__ __forceinline__ Held held_of(const EvictParams& p, float* smem, int parts) {
   Held h;
   h.w = smem;
-  h.from = reinterpret_cast<int*>(smem + p.max_length);
+  h.from = reinterpret_cast<int*>(smem + (p.max_length + parts - 1) / parts);
   h.table = h.from + p.keep;
   return h;
 }
 
 // ---- the whole of it in one launch ----
-// A cluster of CTAs per sequence and group: each of them chooses for itself, from weights that all have read before the first is written; then they share the rows.
+// A cluster of CTAs per sequence and group: each of them chooses for itself, from weights that all have read before the first is written, or they choose together; then they share the rows.
 constexpr int kEvThreads = 1024, kEvUnroll = 2;
 
-template <int LANES>
+template <int LANES, bool SPLIT>
 __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const EvictParams p, int ctas) {
   extern __shared__ __align__(16) float ev_smem[];
   griddep_launch();
   griddep_wait();
   const int tid = threadIdx.x, rank = blockIdx.x % ctas, item = blockIdx.x / ctas, s = item / p.n_groups, g = item - s * p.n_groups, page = 1 << p.shift;
-  const Held h = held_of(p, ev_smem);
-  const bool cut = choose<kEvThreads>(p, s, g, h);
+  constexpr int ROWS = kEvThreads / LANES, TILE = ROWS * kEvUnroll;   // at once; of a tile
+  const Held h = held_of(p, ev_smem, SPLIT ? ctas : 1);
+  const bool cut = choose<kEvThreads, SPLIT>(p, s, g, h, rank, ctas, TILE);
   if (g == 0 && rank == 0 && tid == 0) p.lengths_out[s] = cut ? p.keep : p.lengths[s];
   if (!cut) return;                                // (the whole cluster)
   const float* const s_w = h.w;
@@ -253,7 +304,6 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const EvictPara
   const int* const s_table = h.table;
   auto at = [&](int i) -> float* { return p.kw + (((int64_t)s_table[i >> p.shift] * p.n_groups + g) << p.shift) + (i & (page - 1)); };
   // ---- the rows.  A tile is read while the one before it is still in registers: its rows lie behind all places of that one ----
-  constexpr int ROWS = kEvThreads / LANES, TILE = ROWS * kEvUnroll;   // at once; of a tile
   const int keep = p.keep, hs = LANES * 8, first = rank * TILE + tid / LANES, step = ctas * TILE, lane8 = tid % LANES * 8;
   __nv_bfloat16* const kg = p.k + (int64_t)g * p.k_group + lane8;
   __nv_bfloat16* const vg = p.v + (int64_t)g * p.v_group + lane8;
@@ -279,8 +329,8 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const EvictPara
     load(d0 + step);
     // this tile, and the first time the weights, have been read by all
     if (ctas == 1) __syncthreads();
-    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (d0 == 0) {
+    else cluster_sync();
+    if (!SPLIT && d0 == 0) {
 #pragma unroll 4
       for (int d = rank * kEvThreads + tid; d < keep; d += ctas * kEvThreads) *at(d) = s_w[s_from[d]];
     }
@@ -337,7 +387,7 @@ __global__ void __launch_bounds__(kMvThreads) paged_move_kernel(const EvictParam
     indices(d0 + 2 * step);
     // this tile has been read by all
     if (ctas == 1) __syncthreads();
-    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else cluster_sync();
 #pragma unroll
     for (int j = 0; j < kMvUnroll; ++j) {
       const int d = d0 + row + j * ROWS;
@@ -347,10 +397,13 @@ __global__ void __launch_bounds__(kMvThreads) paged_move_kernel(const EvictParam
 }
 
 constexpr int kHeldMax = 200 * 1024;              // shared memory for weights, places and pages
+// Of more keys a cluster chooses together: its barriers and the counts' way between SMs are 10 us, a CTA's own choice of 30000 keys 22.  us, alone and together: 1 sequence of 8 groups from 8000 to
+// 2000 17.7, 22.0; from 16384 to 4096 28.1, 28.3; 12 groups, 64 numbers a head, from 30001 to 8191 38.6, 32.9; 4 groups from 100000 to 4000 350 (two launches), 31.
+constexpr int kSplitMin = 16384;
 
-int64_t evict_held(int64_t max_length, int64_t keep, int page) { return (max_length + keep + (max_length + page - 1) / page) * 4; }
-size_t evict_bytes(int n_seqs, int n_groups, int64_t keep, int64_t max_length, int page) {
-  return evict_held(max_length, keep, page) <= kHeldMax ? 0 : ((size_t)n_seqs * n_groups * keep + n_seqs) * sizeof(int);
+int64_t evict_held(int64_t max_length, int64_t keep, int page, int parts) { return ((max_length + parts - 1) / parts + keep + (max_length + page - 1) / page) * 4; }
+size_t evict_bytes(int n_seqs, int n_groups, int64_t keep, int64_t max_length, int page) {   // (more than a cluster needs that holds the weights together)
+  return evict_held(max_length, keep, page, 1) <= kHeldMax ? 0 : ((size_t)n_seqs * n_groups * keep + n_seqs) * sizeof(int);
 }
 
 }  // namespace
@@ -400,26 +453,28 @@ int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
   const cudaStream_t st = (cudaStream_t)stream;
   const unsigned items = (unsigned)(a->n_seqs * a->n_groups);
   const int lanes = a->head_size / 8;
-  const int64_t held = evict_held(a->max_length, a->keep, a->page);
+  // as many CTAs for a sequence and group as the SMs take at once, no more than they have tiles unless they choose together
+  const int tile = kEvThreads / lanes * kEvUnroll;
+  int ctas = 1;
+  while (ctas < 8 && (int64_t)items * ctas * 2 <= sm_count() && (ctas * tile < a->keep || a->max_length > kSplitMin)) ctas *= 2;
+  const bool split = ctas > 1 && a->max_length > kSplitMin;
+  const int64_t held = evict_held(a->max_length, a->keep, a->page, split ? ctas : 1);
   if (held <= kHeldMax) {
     static PerDeviceOnce once;
     if (once.need()) {
-      B200_CUDA(cudaFuncSetAttribute(paged_evict_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
-      B200_CUDA(cudaFuncSetAttribute(paged_evict_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
+      for (auto* k : {paged_evict_kernel<8, false>, paged_evict_kernel<8, true>, paged_evict_kernel<16, false>, paged_evict_kernel<16, true>})
+        B200_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
       once.done();
     }
-    // as many CTAs for a sequence and group as the SMs take at once, no more than they have tiles
-    const int tile = kEvThreads / lanes * kEvUnroll;
-    int ctas = 1;
-    while (ctas < 8 && (int64_t)items * ctas * 2 <= sm_count() && ctas * tile < a->keep) ctas *= 2;
-    B200_CUDA(launch_cluster(lanes == 8 ? paged_evict_kernel<8> : paged_evict_kernel<16>, dim3(items * ctas), dim3(kEvThreads), ctas, (size_t)held, st, p, ctas));
+    auto* const kernel = lanes == 8 ? (split ? paged_evict_kernel<8, true> : paged_evict_kernel<8, false>) : split ? paged_evict_kernel<16, true> : paged_evict_kernel<16, false>;
+    B200_CUDA(launch_cluster(kernel, dim3(items * ctas), dim3(kEvThreads), ctas, (size_t)held, st, p, ctas));
     return B200_OK;
   }
   B200_CUDA(launch(paged_choose_kernel, dim3(items), dim3(kChThreads), 0, st, p));
   // as many CTAs for the rows of one tensor as leave none of the SMs without, no more than they have tiles
-  const int tile = kMvThreads / lanes * kMvUnroll;
-  int ctas = 1;
-  while (ctas < 8 && (int64_t)items * 2 * ctas < sm_count() && ctas * tile < a->keep) ctas *= 2;
+  const int rows = kMvThreads / lanes * kMvUnroll;
+  ctas = 1;
+  while (ctas < 8 && (int64_t)items * 2 * ctas < sm_count() && ctas * rows < a->keep) ctas *= 2;
   B200_CUDA(launch_cluster(lanes == 8 ? paged_move_kernel<8> : paged_move_kernel<16>, dim3(items * ctas, 2), dim3(kMvThreads), ctas, 0, st, p, ctas));
   return B200_OK;
 }

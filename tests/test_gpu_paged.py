@@ -396,6 +396,56 @@ def test_evict_long(E, lengths, keep, first, recent):
     evict_check(E, d, lengths, keep, rows, first=first, recent=recent)
 
 
+@pytest.mark.parametrize("hs,groups,page,lengths,keep,first,recent",
+                         [(64, 1, 16, [16385], 16384, 0, 0), (128, 1, 16, [17001, 2, 17], 1, 0, 0), (64, 2, 16, [20003], 77, 70, 7), (128, 2, 256, [16411, 2100, 1999], 1999, 1500, 400),
+                          (64, 1, 32, [18191, 300], 299, 0, 299), (128, 1, 64, [7, 17777, 9], 6, 2, 1), (64, 18, 64, [17000, 30], 1000, 1, 30), (64, 19, 64, [17000, 30], 1000, 1, 30),
+                          (64, 38, 64, [17000, 30], 1000, 1, 30)])
+def test_evict_chosen_together(E, hs, groups, page, lengths, keep, first, recent):
+    """Few sequences of more keys than a thread block chooses from by itself; some of them are so short that parts of the cluster have none of their keys."""
+    d, rows = cache(lengths, groups, hs, page, seed=keep)
+    d["kw"] = (d["kw"] * 100).round() / 100            # (equal ones among them, on both sides of a part's end)
+    evict_check(E, d, lengths, keep, rows, first=first, recent=recent)
+
+
+@pytest.mark.parametrize("kind", ["zeros", "few values", "not a number", "neighbours"])
+def test_evict_chosen_together_ties(E, kind):
+    lengths = [17300, 900]
+    d, rows = cache(lengths, 1, 64, 32, seed=23)
+    r = torch.Generator().manual_seed(2)
+    pick = lambda *values: torch.tensor(values)[torch.randint(len(values), d["kw"].shape, generator=r)]
+    nan, inf = float("nan"), float("inf")
+    d["kw"] = {"zeros": lambda: torch.zeros_like(d["kw"]), "few values": lambda: pick(0.0, 1.0, 2.5), "not a number": lambda: pick(nan, inf, 1.0, -nan, -2.0),
+               "neighbours": lambda: 1.0 + torch.randint(0, 600, d["kw"].shape, generator=r) * 2 ** -23}[kind]().float()
+    for keep in (17299, 899, 40):
+        evict_check(E, d, lengths, keep, rows, first=3, recent=20)
+
+
+def test_evict_chosen_together_leaves_what_it_must(E):
+    """An entry that is no page, a length of more than max_length, a row outside the table: in clusters too the sequence stays."""
+    lengths = [2200, 2100, 20400]
+    d, rows = cache(lengths, 2, 64, 64, seed=25)
+    d["pages"][rows[1], 30] = len(d["k"])
+    want = oracle.evict(d["k"], d["v"], d["kw"], d["pages"], lengths[:2], 600, rows=rows[:2])
+    t = on_gpu(d)
+    left = E.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths + [2200, 0, -5], dtype=torch.int32, device="cuda"), 600, max_length=20000,
+                         rows=torch.tensor(rows + [-1, rows[0], rows[0]], dtype=torch.int32, device="cuda"))
+    assert left.tolist() == [600, 2100, 20400, 2200, 0, -5]
+    assert same(t["k"].cpu(), want[0]) and same(t["v"].cpu(), want[1]) and same(t["kw"].cpu(), want[2])
+
+
+@pytest.mark.parametrize("lengths,groups,keep,max_length", [([2100, 40, 900, 1500] + [33] * 34, 2, 700, 60000), ([60000], 1, 49000, 60000)])
+def test_evict_in_two_launches(E, lengths, groups, keep, max_length):
+    """Weights that fit into no thread block's shared memory, nor into a cluster's beside the places."""
+    d, rows = cache(lengths, groups, 64, 16, seed=29)
+    d["kw"] = (d["kw"] * 100).round() / 100
+    d["pages"] = torch.nn.functional.pad(d["pages"], (0, max(0, max_length // 16 - d["pages"].shape[1])), value=-1)
+    want = oracle.evict(d["k"], d["v"], d["kw"], d["pages"], lengths, keep, rows=rows, first=5, recent=50)
+    t = on_gpu(d)
+    left = E.evict_paged(t["k"], t["v"], t["kw"], t["pages"], torch.tensor(lengths, dtype=torch.int32, device="cuda"), keep, max_length=max_length, first=5, recent=50,
+                         rows=torch.tensor(rows, dtype=torch.int32, device="cuda"))
+    assert same(t["k"].cpu(), want[0]) and same(t["v"].cpu(), want[1]) and same(t["kw"].cpu(), want[2]) and left.tolist() == want[3]
+
+
 @pytest.mark.parametrize("kind", ["zeros", "few values", "signs", "infinite", "not a number", "neighbours", "tiny"])
 def test_evict_ties_and_odd_weights(E, kind):
     """Equal weights: the lower index; the two zeros are equal; NaN above all."""
