@@ -401,6 +401,43 @@ constexpr int kHeldMax = 200 * 1024;              // shared memory for weights, 
 // 2000 17.7, 22.0; from 16384 to 4096 28.1, 28.3; 12 groups, 64 numbers a head, from 30001 to 8191 38.6, 32.9; 4 groups from 100000 to 4000 350 (two launches), 31.
 constexpr int kSplitMin = 16384;
 
+// Clusters of 2, 4, 8 CTAs that this device runs at once: what its SMs come in leaves some of them without (B200: 74, 33, 15 with a CTA an SM, and not 74, 37, 18; a cluster more and all wait for a
+// second round: 36 groups cut from 3000 to 2000 in clusters of 4 35.9 us, of 2 27.5; 16 in clusters of 8 26.4, of 4 18.5).
+constexpr int kDevices = 64;
+std::atomic<int> g_clusters[kDevices][3];
+cudaError_t evict_configure() {
+  static PerDeviceOnce once;
+  if (!once.need()) return cudaSuccess;
+  for (auto* k : {paged_evict_kernel<8, false>, paged_evict_kernel<8, true>, paged_evict_kernel<16, false>, paged_evict_kernel<16, true>}) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax);
+    if (e != cudaSuccess) return e;
+  }
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  for (int i = 0; e == cudaSuccess && i < 3; ++i) {
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2u << i;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2u << i);
+    cfg.blockDim = dim3(kEvThreads);
+    cfg.dynamicSmemBytes = kHeldMax;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    e = cudaOccupancyMaxActiveClusters(&n, paged_evict_kernel<16, false>, &cfg);
+    if (device < kDevices) g_clusters[device][i].store(n, std::memory_order_relaxed);
+  }
+  if (e == cudaSuccess) once.done();
+  return e;
+}
+int clusters_at_once(int ctas) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= kDevices) return 0;
+  return g_clusters[device][ctas == 2 ? 0 : ctas == 4 ? 1 : 2].load(std::memory_order_relaxed);
+}
+
 int64_t evict_held(int64_t max_length, int64_t keep, int page, int parts) { return ((max_length + parts - 1) / parts + keep + (max_length + page - 1) / page) * 4; }
 size_t evict_bytes(int n_seqs, int n_groups, int64_t keep, int64_t max_length, int page) {   // (more than a cluster needs that holds the weights together)
   return evict_held(max_length, keep, page, 1) <= kHeldMax ? 0 : ((size_t)n_seqs * n_groups * keep + n_seqs) * sizeof(int);
@@ -453,19 +490,14 @@ int b200_evict_paged(const b200_evict_paged_args* a, b200_stream_t stream) {
   const cudaStream_t st = (cudaStream_t)stream;
   const unsigned items = (unsigned)(a->n_seqs * a->n_groups);
   const int lanes = a->head_size / 8;
-  // as many CTAs for a sequence and group as the SMs take at once, no more than they have tiles unless they choose together
+  B200_CUDA(evict_configure());
+  // as many CTAs for a sequence and group as run at once, no more than they have tiles unless they choose together
   const int tile = kEvThreads / lanes * kEvUnroll;
   int ctas = 1;
-  while (ctas < 8 && (int64_t)items * ctas * 2 <= sm_count() && (ctas * tile < a->keep || a->max_length > kSplitMin)) ctas *= 2;
+  while (ctas < 8 && items <= (unsigned)clusters_at_once(2 * ctas) && (ctas * tile < a->keep || a->max_length > kSplitMin)) ctas *= 2;
   const bool split = ctas > 1 && a->max_length > kSplitMin;
   const int64_t held = evict_held(a->max_length, a->keep, a->page, split ? ctas : 1);
   if (held <= kHeldMax) {
-    static PerDeviceOnce once;
-    if (once.need()) {
-      for (auto* k : {paged_evict_kernel<8, false>, paged_evict_kernel<8, true>, paged_evict_kernel<16, false>, paged_evict_kernel<16, true>})
-        B200_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMax));
-      once.done();
-    }
     auto* const kernel = lanes == 8 ? (split ? paged_evict_kernel<8, true> : paged_evict_kernel<8, false>) : split ? paged_evict_kernel<16, true> : paged_evict_kernel<16, false>;
     B200_CUDA(launch_cluster(kernel, dim3(items * ctas), dim3(kEvThreads), ctas, (size_t)held, st, p, ctas));
     return B200_OK;
