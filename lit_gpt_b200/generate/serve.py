@@ -267,6 +267,8 @@ class PagedSession:
             position, cached, held = (r.position, r.cached, len(r.pages)) if r is not None else (0, 0, 0)
             if position + len(toks) > self.model.max_seq_length:
                 raise ValueError(f"request {rid!r}: position {position} and {len(toks)} tokens, max seq length is only {self.model.max_seq_length}")
+            if min(toks) < 0 or max(toks) >= self.model.config.padded_vocab_size:
+                raise ValueError(f"request {rid!r}: tokens outside 0 .. {self.model.config.padded_vocab_size - 1}")
             if any(not 0 <= p < len(toks) for p in places):
                 raise ValueError(f"request {rid!r}: logits of places outside its {len(toks)} tokens are wanted")
             most = cached + len(toks) if self.keep is None else min(cached + len(toks), max(cached, self.keep + self.page) + self.portion)

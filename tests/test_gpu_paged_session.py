@@ -193,3 +193,19 @@ def test_refusals(golden):
     assert model(torch.tensor([[1, 2]], device="cuda"), torch.arange(2, device="cuda")).shape[1] == 2   # the model's own caches are in place again
     with pytest.raises(TypeError, match="PagedKVCache"):
         model.paged_step(torch.tensor([1], device="cuda"), None)
+
+
+@torch.inference_mode()
+def test_tokens_outside_the_vocabulary_are_refused(golden):
+    from lit_gpt_b200.generate.serve import PagedSession, generate_batch
+
+    model, *_ = toy(golden)
+    V = model.config.padded_vocab_size
+    s = PagedSession(model, 8, 16)
+    for bad in ([V], [1, -1], [3] * 20 + [1 << 40]):
+        with pytest.raises(ValueError, match="tokens outside"):
+            s.step([("a", [1, 2], None), ("b", bad, None)])
+        with pytest.raises(ValueError, match="tokens outside"):
+            generate_batch(model, [[1, 2], bad], 4)
+    assert not s.live and s.free_pages == 8
+    assert s.step([("a", [0, V - 1], None)]).shape == (2, V)
