@@ -11,11 +11,6 @@ struct PagedCut {                                           // what a CTA of pag
   int count, row, gi;                                       // its queries, its first row, its group
 };
 
-struct __align__(16) PagedPart {                            // a CTA's part of their list
-  int tile, end;                                            // steps; tile == end: none
-  int s, gi, block, lo;                                     // where it begins: sequence, group, block of queries, step of the block
-};
-
 struct PagedWeightCut {                                     // a block of 128 keys that several CTAs of paged_weights.cu have parts of
   int first, last;                                          // those CTAs; last -1: none to join
   int table, n, gi, block;
@@ -45,7 +40,6 @@ struct PagedParams {
   int tc_rows;                                              // rows of a block of theirs: 256 queries at most
   int tc_workers;                                           // CTAs that share their tiles, at most
   float* tc_acc; float2* tc_ml; PagedCut* cuts;             // their results: two slots of 256 queries a CTA
-  PagedPart* parts;                                         // written by the append kernel, as the cuts are
   float* scores; int score_rows, kept_max;                  // scores of the list's tiles, that many queries each; of sequences of up to kept_max queries a group (0: none are kept)
   int kw_workers; float* kw_part; PagedWeightCut* kw_cuts;  // CTAs that compute the others' again, their sums: two slots of 128 keys a CTA
   int* tile_base;                                           // per sequence: its first tile in the list; -1: nothing was done
@@ -103,22 +97,6 @@ __device__ __forceinline__ int page_at(const PagedParams& p, int table, int inde
 }
 
 __device__ __forceinline__ int capped(int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); }
-
-// ---- the tensor memory's list of key tiles ----
-// The list is cut by steps: an item counts as its key tiles and kLead more, the time that its queries' way in and its results' way out take (4 to 5 us where a tile takes 2.2).
-constexpr int kLead = 2;
-struct Blocks {            // of a sequence
-  int count;               // of a group; none where the sequence is the list's
-  int rows_each, cached, rows, n;
-  __device__ __forceinline__ int steps(int block) const { return block < count ? kLead + ((min(cached + min((block + 1) * rows_each, rows), n) + 127) >> 7) : 0; }
-};
-__device__ __forceinline__ Blocks blocks_of(const PagedParams& p, const PagedSeq& s) {
-  Blocks b;
-  b.rows_each = p.tc_rows;
-  b.count = s.rows * p.per > p.list_max ? (s.rows + b.rows_each - 1) / b.rows_each : 0;
-  b.cached = s.cached; b.rows = s.rows; b.n = s.n;
-  return b;
-}
 
 // A box of 64 numbers of min(page, 128) keys, 128-byte-swizzled
 __device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int page, uint32_t bar) {

@@ -32,121 +32,6 @@ __device__ __forceinline__ int64_t paged_pos(const PagedParams& p, int row) {
   return at < 0 ? 0 : (at >= p.table_rows ? p.table_rows - 1 : at);
 }
 
-// ---- the tensor memory's list, cut: by one CTA of the append kernel ----
-// Every one of its CTAs would come to the same by itself, at the beginning of the launch behind (3.3 to 4.2 us a step).
-template <int THREADS>
-__device__ __forceinline__ void cut_list(const PagedParams& p) {
-  __shared__ int s_sums[THREADS + 1], s_warp[THREADS / 32];
-  __shared__ Shares s_shares[THREADS / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int run = (p.n_seqs + THREADS - 1) / THREADS;
-  int here = 0;                           // steps of a group of this thread's sequences
-  Shares work = {0ull, 0ull};
-  for (int k = 0; k < run; ++k) {
-    const int i = tid * run + k;
-    Blocks mine = {};
-    if (i < p.n_seqs) {
-      const PagedSeq s = paged_seq(p, i);
-      mine = blocks_of(p, s);
-      if (p.mixed) add_work(p, s, work);
-    }
-    if (mine.count <= 16) {
-      for (int e = 0; e < mine.count; ++e) here = capped((int64_t)here + mine.steps(e));
-    }
-    for (unsigned left = __ballot_sync(0xffffffffu, mine.count > 16); left; left &= left - 1) {   // long ones: by all lanes, one after the other
-      const int of = __ffs(left) - 1;
-      Blocks b;
-      b.rows_each = p.tc_rows;
-      b.count = __shfl_sync(0xffffffffu, mine.count, of);
-      b.cached = __shfl_sync(0xffffffffu, mine.cached, of);
-      b.rows = __shfl_sync(0xffffffffu, mine.rows, of);
-      b.n = __shfl_sync(0xffffffffu, mine.n, of);
-      int64_t part = 0;
-      for (int e = lane; e < b.count; e += 32) part += b.steps(e);
-      int sum = capped(part);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum = capped((int64_t)sum + __shfl_xor_sync(0xffffffffu, sum, o));
-      if (lane == of) here = capped((int64_t)here + sum);
-    }
-  }
-  int inc = here;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc = capped((int64_t)inc + x);
-  }
-  if (lane == 31) s_warp[warp] = inc;
-  if (p.mixed) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      work.list += __shfl_xor_sync(0xffffffffu, work.list, o);
-      work.tensor += __shfl_xor_sync(0xffffffffu, work.tensor, o);
-    }
-    if (lane == 0) s_shares[warp] = work;
-  }
-  __syncthreads();
-  int before = inc - here;
-  for (int w = 0; w < warp; ++w) before = capped((int64_t)before + s_warp[w]);
-  s_sums[tid] = before;
-  if (tid == THREADS - 1) s_sums[THREADS] = capped((int64_t)before + here);
-  __syncthreads();
-  const int64_t all64 = (int64_t)s_sums[THREADS] * p.n_groups;
-  const int all = all64 < kMaxTiles ? (int)all64 : 0;      // (a description whose sequences overlap can hold more: then none is done)
-  int ctas = p.tc_workers;
-  if (p.mixed) {                          // the list's kernel takes the other SMs
-    work = {0ull, 0ull};
-    for (int w = 0; w < THREADS / 32; ++w) { work.list += s_shares[w].list; work.tensor += s_shares[w].tensor; }
-    ctas = tensor_share(p, work);
-  }
-  const int workers = min(all, ctas), each = workers ? all / workers : 0, more = all - each * workers, wide = more * (each + 1);
-  for (int w = tid; w < p.tc_workers; w += THREADS) {
-    PagedPart at = {};
-    PagedCut c = {};                      // for the launch that joins: the item that this part goes on with
-    c.last = -1;
-    if (w < workers) {
-      const int first = w * each + min(w, more);
-      at.tile = first;
-      at.end = first + each + (w < more ? 1 : 0);
-      int lo = 0, hi = THREADS;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if ((int64_t)s_sums[mid] * p.n_groups <= first) lo = mid; else hi = mid;
-      }
-      int rest = first - s_sums[lo] * p.n_groups, of_group;
-      PagedSeq seq;
-      Blocks blk;
-      for (at.s = lo * run;; ++at.s) {
-        seq = paged_seq(p, at.s);
-        blk = blocks_of(p, seq);
-        of_group = 0;
-        if (run == 1) of_group = s_sums[lo + 1] - s_sums[lo];
-        else for (int e = 0; e < blk.count; ++e) of_group += blk.steps(e);
-        if (rest < of_group * p.n_groups) break;
-        rest -= of_group * p.n_groups;
-      }
-      at.gi = rest / of_group;
-      rest -= at.gi * of_group;
-      for (;; ++at.block) {               // the block that holds it
-        const int steps = blk.steps(at.block);
-        if (rest < steps) break;
-        rest -= steps;
-      }
-      at.lo = rest;
-      if (at.lo > kLead) {
-        const int m0 = at.block * blk.rows_each * p.per;
-        auto worker_of = [&](int tile) { return tile < wide ? tile / (each + 1) : more + (tile - wide) / each; };
-        c.first = worker_of(first - at.lo + kLead);   // (whose part holds the first key tile)
-        c.last = worker_of(first - at.lo + blk.steps(at.block) - 1);
-        c.count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
-        c.row = seq.first + at.block * blk.rows_each;
-        c.gi = at.gi;
-      }
-    }
-    p.parts[w] = at;
-    p.cuts[w] = c;
-  }
-}
-
 // ---- the queries and the new keys turned, the new rows stored ----
 // A CTA takes a row, or some heads of one: HS / 16 threads a head, each with sixteen numbers of it, eight and the eight that they turn with (or, where nothing is turned, any sixteen), whose cosines
 // and sines it keeps from head to head.  Needs rows of heads and tables for accesses of 16 bytes, and halves of the rotation that are multiples of eight numbers (or no rotation).
@@ -157,12 +42,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_wide_kernel(const PagedPa
   constexpr int TH = HS / 16, HEADS = 256 / TH;    // threads of a head; heads at once
   griddep_wait();     // (before the launch of what follows: the kernels behind read the step's description and the older keys ahead of their own wait)
   griddep_launch();
-  int row = blockIdx.x;
-  if (p.tc_workers > 0 && --row < 0) {             // the first CTAs of a step with chunks
-    if (blockIdx.y == 0) cut_list<256>(p);
-    return;
-  }
-  const int heads = p.n_groups * (p.per + 2), n = p.rope_n, half = n >> 1;
+  const int row = blockIdx.x, heads = p.n_groups * (p.per + 2), n = p.rope_n, half = n >> 1;
   const int piece = threadIdx.x % TH;
   // numbers a .. a + 7 and b .. b + 7: pairs of the rotation first, then what it leaves
   const int turning = half >> 3, a = piece < turning ? piece * 8 : n + (piece - turning) * 16, b = piece < turning ? a + half : a + 8;
@@ -234,12 +114,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) 
   constexpr int V = HS / 32;
   griddep_wait();
   griddep_launch();
-  if (p.tc_workers > 0 && blockIdx.x == 0) {
-    cut_list<256>(p);
-    return;
-  }
   const int lane = threadIdx.x & 31, heads = p.n_groups * (p.per + 2);
-  const int64_t at = (int64_t)(blockIdx.x - (p.tc_workers > 0)) * 8 + (threadIdx.x >> 5);
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int row = (int)(at / heads), i = (int)(at - (int64_t)row * heads), gi = i / (p.per + 2), h = i - gi * (p.per + 2);
   if (row >= p.rows) return;
   const int which = p.row_seq[row];
@@ -983,7 +859,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
     }
   }
   s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * 2 * sizeof(int) +
-            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)s.scores * sizeof(float) + (size_t)s.kw_workers * (256 * sizeof(float) + sizeof(PagedWeightCut)) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * (sizeof(PagedPart) + sizeof(PagedCut));
+            (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)s.scores * sizeof(float) + (size_t)s.kw_workers * (256 * sizeof(float) + sizeof(PagedWeightCut)) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
   // A cluster where its warps have four tiles each at most, and all clusters run at once.  us of the list and of clusters: 1 token of 32 groups, 128 numbers a head, over 300 keys 12.9, 7.5, over
   // 2000 13.6, 10.4, over 8000 30.6, 28.1; of 8 groups of 4 heads over 8000 16.6, 17.2; 16 tokens of 32 groups over 300 18.5, 19.5; 64 of 8 groups over 100 14.4, 15.4; of 12 groups, 64 numbers
   // a head, over 500 22.5, 17.9; 16 of them over 1000 16.4, 17.9.
@@ -1032,13 +908,12 @@ template <int HS>
 cudaError_t launch_paged(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
   if (s.cluster) return s.nq == 1 ? launch_clusters<HS, 1>(p, s, st) : launch_clusters<HS, 2>(p, s, st);
   const int64_t warps = (int64_t)p.rows * p.n_groups * (p.per + 2);
-  const unsigned cutting = p.tc_workers > 0;
   cudaError_t e;
   if (p.wide) {                    // few rows: a row's heads on several CTAs, as many as are at once
     const int turns = (p.n_groups * (p.per + 2) * (HS / 16) + 255) / 256, ctas = p.sms * 4 / p.rows;
-    e = launch(paged_append_wide_kernel<HS>, dim3((unsigned)p.rows + cutting, (unsigned)(ctas < 1 ? 1 : ctas < turns ? ctas : turns)), dim3(256), 0, st, p);
+    e = launch(paged_append_wide_kernel<HS>, dim3((unsigned)p.rows, (unsigned)(ctas < 1 ? 1 : ctas < turns ? ctas : turns)), dim3(256), 0, st, p);
   } else {
-    e = launch(paged_append_kernel<HS>, dim3((unsigned)((warps + 7) / 8) + cutting), dim3(256), 0, st, p);
+    e = launch(paged_append_kernel<HS>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, p);
   }
   if (e != cudaSuccess) return e;
   if (s.tensor && (e = launch_paged_tc05(p, HS, st)) != cudaSuccess) return e;
@@ -1118,8 +993,7 @@ int b200_attn_paged(const b200_attn_paged_args* a, b200_stream_t stream) {
   p.list_max = s.list_max; p.tc_workers = s.tc_workers; p.tc_rows = per <= 256 ? 256 / per : 1;
   p.tc_acc = (float*)(p.ml + s.slots);
   p.tc_ml = (float2*)(p.tc_acc + (int64_t)s.tc_workers * 512 * a->head_size);
-  p.parts = (PagedPart*)(p.tc_ml + (int64_t)s.tc_workers * 512);
-  p.where = (int2*)(p.parts + s.tc_workers);
+  p.where = (int2*)(p.tc_ml + (int64_t)s.tc_workers * 512);
   p.cuts = (PagedCut*)(p.where + s.items);
   p.item_base = (int*)(p.cuts + s.tc_workers);
   p.score_rows = s.score_rows; p.kept_max = s.kept_max; p.kw_workers = s.kw_workers;

@@ -38,12 +38,42 @@ struct PtTile {
   static constexpr uint32_t kS = 0, kO = 256;              // tensor-memory columns: S0 S1 (P over them) | O0 O1
 };
 
+// ---- the list of key tiles ----
+// The list is cut by steps: an item counts as its key tiles and kLead more, the time that its queries' way in and its results' way out take (4 to 5 us where a tile takes 2.2).
+constexpr int kLead = 2;
+struct Blocks {            // of a sequence
+  int count;               // of a group; none where the sequence is the list's
+  int rows_each, cached, rows, n;
+  __device__ __forceinline__ int steps(int block) const { return block < count ? kLead + ((min(cached + min((block + 1) * rows_each, rows), n) + 127) >> 7) : 0; }
+};
+__device__ __forceinline__ Blocks blocks_of(const PagedParams& p, const PagedSeq& s) {
+  Blocks b;
+  b.rows_each = p.tc_rows;
+  b.count = s.rows * p.per > p.list_max ? (s.rows + b.rows_each - 1) / b.rows_each : 0;
+  b.cached = s.cached; b.rows = s.rows; b.n = s.n;
+  return b;
+}
+// The steps of a group, by a whole warp.
+__device__ __forceinline__ int steps_of(const Blocks& b, int lane) {
+  int64_t s = 0;
+  for (int i = lane; i < b.count; i += 32) s += b.steps(i);
+  int c = capped(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) c = capped((int64_t)c + __shfl_xor_sync(0xffffffffu, c, o));
+  return c;
+}
+
 struct Seg {
   int q0, count;           // first query in the workspace's order, queries
   int m0, first;           // its number within the sequence and group; the sequence's first row
   int cached, n, table, gi;
   int lo, hi, hi0;         // key tiles; those of the first 128 queries end at hi0
   int slot;                // place of its results; -1: the item is done here
+};
+
+struct ListAt {            // where the list of segments goes on
+  int tile, end;
+  int s, gi, block, lo;    // sequence, group, block, first key tile
 };
 
 template <int HS>
@@ -55,9 +85,12 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   __shared__ float s_shrink[256];         // per query: what its O and sum shrink by in this step
   __shared__ __align__(16) uint32_t s_bits[4][4];        // keys of a tile that have a page, of the last four tiles
   __shared__ Seg s_seg[kPtSegs];
-  __shared__ PagedPart s_at;
+  __shared__ ListAt s_at;
+  __shared__ PagedCut s_cut;
   __shared__ int s_segs, s_more;
   __shared__ uint32_t s_tmem;
+  __shared__ int s_sums[kPtThreads + 1], s_warp[kPtThreads / 32];
+  __shared__ Shares s_shares[kPtThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t smem = (tc::smem_u32(pt_smem) + 1023u) & ~1023u;
   const uint32_t sq_ = smem, sk_ = smem + 2 * C::kBytes, sv_ = smem + 4 * C::kBytes;
@@ -66,6 +99,48 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
                  o_done = bars + 112, q_full = bars + 128, shrink = bars + 136, idle = bars + 200;   // shrink: one per softmax warp; idle: products that gave up
 
   if (!p.mixed) griddep_launch();
+  // ---- this CTA's part of the list: from the step's description, which was there before the append kernel ----
+  const int run = (p.n_seqs + kPtThreads - 1) / kPtThreads;
+  int here = 0;
+  Shares work = {0ull, 0ull};
+  for (int k = 0; k < run; ++k) {
+    const int i = tid * run + k;
+    Blocks mine = {};
+    if (i < p.n_seqs) {
+      const PagedSeq s = paged_seq(p, i);
+      mine = blocks_of(p, s);
+      if (p.mixed) add_work(p, s, work);
+    }
+    if (mine.count <= 16) {
+      for (int e = 0; e < mine.count; ++e) here = capped((int64_t)here + mine.steps(e));
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, mine.count > 16); left; left &= left - 1) {   // long ones: by all lanes, one after the other
+      const int of = __ffs(left) - 1;
+      Blocks b;
+      b.rows_each = p.tc_rows;
+      b.count = __shfl_sync(0xffffffffu, mine.count, of);
+      b.cached = __shfl_sync(0xffffffffu, mine.cached, of);
+      b.rows = __shfl_sync(0xffffffffu, mine.rows, of);
+      b.n = __shfl_sync(0xffffffffu, mine.n, of);
+      const int sum = steps_of(b, lane);
+      if (lane == of) here = capped((int64_t)here + sum);
+    }
+  }
+  int inc = here;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc = capped((int64_t)inc + x);
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  if (p.mixed) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      work.list += __shfl_xor_sync(0xffffffffu, work.list, o);
+      work.tensor += __shfl_xor_sync(0xffffffffu, work.tensor, o);
+    }
+    if (lane == 0) s_shares[warp] = work;
+  }
   if (tid == 0) {
     tc::mbar_init(q_full, 1);
     tc::mbar_init(idle, 1);
@@ -82,10 +157,86 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     for (int i = 0; i < 8; ++i) tc::mbar_init(shrink + 8 * i, 1);
     tc::mbar_init_fence();
   }
-  griddep_wait();                         // (tensor memory is taken behind the wait only)
-  if (p.mixed) griddep_launch();          // (the list's kernel takes the other SMs)
-  const PagedPart part = p.parts[blockIdx.x];
-  if (part.tile >= part.end) return;
+  __syncthreads();
+  int before = inc - here;
+  for (int w = 0; w < warp; ++w) before = capped((int64_t)before + s_warp[w]);
+  s_sums[tid] = before;
+  if (tid == kPtThreads - 1) s_sums[kPtThreads] = capped((int64_t)before + here);
+  __syncthreads();
+  const int64_t all64 = (int64_t)s_sums[kPtThreads] * p.n_groups;
+  const int all = all64 < kMaxTiles ? (int)all64 : 0;      // (a description whose sequences overlap can hold more: then none is done)
+  int ctas = gridDim.x;
+  if (p.mixed) {                        // the list's kernel takes the other SMs: it may begin once the append kernel has ended
+    work = {0ull, 0ull};
+    for (int w = 0; w < kPtThreads / 32; ++w) { work.list += s_shares[w].list; work.tensor += s_shares[w].tensor; }
+    ctas = tensor_share(p, work);
+    if ((int)blockIdx.x >= ctas) {
+      griddep_wait();
+      griddep_launch();
+      if (tid == 0) {
+        PagedCut c = {};
+        c.last = -1;
+        p.cuts[blockIdx.x] = c;
+      }
+      return;
+    }
+  }
+  if (warp == 0) {
+    const int workers = min(max(all / 2, min(all, ctas)), ctas), w = blockIdx.x;
+    const int each = workers ? all / workers : 0, more = all - each * workers;
+    const int first = w * each + min(w, more), end = w < workers ? first + each + (w < more ? 1 : 0) : first;
+    ListAt at = {};
+    at.tile = first;
+    at.end = end;
+    PagedCut c = {};                    // for the launch that joins: the item that this CTA goes on with
+    c.last = -1;
+    if (first < end) {
+      int lo = 0, hi = kPtThreads;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if ((int64_t)s_sums[mid] * p.n_groups <= first) lo = mid; else hi = mid;
+      }
+      int rest = first - s_sums[lo] * p.n_groups, of_group;
+      PagedSeq seq;
+      Blocks blk;
+      for (at.s = lo * run;; ++at.s) {
+        seq = paged_seq(p, at.s);
+        blk = blocks_of(p, seq);
+        of_group = steps_of(blk, lane);
+        if (rest < of_group * p.n_groups) break;
+        rest -= of_group * p.n_groups;
+      }
+      at.gi = rest / of_group;
+      rest -= at.gi * of_group;
+      for (int b0 = 0;; b0 += 32) {     // the block that holds it
+        const int t = blk.steps(b0 + lane);
+        int sum = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += x; }
+        const unsigned behind = __ballot_sync(0xffffffffu, sum > rest);
+        if (behind) {
+          const int of = __ffs(behind) - 1;
+          at.block = b0 + of;
+          at.lo = rest - __shfl_sync(0xffffffffu, sum - t, of);
+          break;
+        }
+        rest -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (at.lo > kLead) {
+        const int m0 = at.block * blk.rows_each * p.per, wide = more * (each + 1);
+        auto worker_of = [&](int tile) { return tile < wide ? tile / (each + 1) : more + (tile - wide) / each; };
+        c.first = worker_of(first - at.lo + kLead);   // (whose part holds the first key tile)
+        c.last = worker_of(first - at.lo + blk.steps(at.block) - 1);
+        c.count = min(blk.rows_each * p.per, seq.rows * p.per - m0);
+        c.row = seq.first + at.block * blk.rows_each;
+        c.gi = at.gi;
+      }
+    }
+    if (lane == 0) {
+      s_cut = c;
+      s_at = at;
+    }
+  }
   uint32_t tmem = 0;
   bool ok = true;
   // counted over all segments, so that every barrier's phase is known
@@ -93,7 +244,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   uint32_t n[2] = {0u, 0u};                                // steps of either 128 queries
 
   auto list_segments = [&]() {            // by thread 0
-    PagedPart at = s_at;
+    ListAt at = s_at;
     int c = 0;
     if (at.tile < at.end) {
       PagedSeq seq = paged_seq(p, at.s);
@@ -130,11 +281,11 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     s_segs = c;
     s_more = at.tile < at.end;
   };
-  if (tid == 0) {
-    s_at = part;
-    list_segments();
-  }
+  if (tid == 0) list_segments();
+  griddep_wait();                         // (tensor memory is taken behind the wait only)
+  if (p.mixed) griddep_launch();
   if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+  if (tid == 0) p.cuts[blockIdx.x] = s_cut;
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
