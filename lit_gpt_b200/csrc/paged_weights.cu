@@ -85,9 +85,10 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
 
   griddep_launch();
   // ---- this CTA's part of the list: from the step's description ----
-  const int run = (p.n_seqs + kKwThreads - 1) / kKwThreads;
+  const bool few = p.n_seqs <= 32;        // by one warp
+  const int run = (p.n_seqs + kKwThreads - 1) / kKwThreads, turns = few && warp > 0 ? 0 : run;
   int here = 0;
-  for (int k = 0; k < run; ++k) {
+  for (int k = 0; k < turns; ++k) {
     const int i = tid * run + k;
     KeyBlocks mine = {};
     if (i < p.n_seqs) mine = key_blocks(p, paged_seq(p, i));
@@ -111,8 +112,15 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
     const int x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc = capped((int64_t)inc + x);
   }
-  if (lane == 31) s_warp[warp] = inc;
-  if (tid == 0) {
+  if (few) {
+    if (warp == 0) {
+      s_sums[lane] = inc - here;
+      if (lane == 31) s_sums[32] = s_sums[kKwThreads] = inc;
+    }
+  } else if (lane == 31) {
+    s_warp[warp] = inc;
+  }
+  if (tid == kKwThreads - 32) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(k_full + 8 * i, 1);
       tc::mbar_init(k_empty + 8 * i, 1);
@@ -129,11 +137,13 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
     tc::mbar_init_fence();
   }
   __syncthreads();
-  int before = inc - here;
-  for (int w = 0; w < warp; ++w) before = capped((int64_t)before + s_warp[w]);
-  s_sums[tid] = before;
-  if (tid == kKwThreads - 1) s_sums[kKwThreads] = capped((int64_t)before + here);
-  __syncthreads();
+  if (!few) {
+    int before = inc - here;
+    for (int w = 0; w < warp; ++w) before = capped((int64_t)before + s_warp[w]);
+    s_sums[tid] = before;
+    if (tid == kKwThreads - 1) s_sums[kKwThreads] = capped((int64_t)before + here);
+    __syncthreads();
+  }
   if (warp == 0) {
     const int64_t all64 = (int64_t)s_sums[kKwThreads] * p.n_groups;
     const int all = all64 < kMaxTiles ? (int)all64 : 0;
@@ -146,7 +156,7 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
     PagedWeightCut c = {};
     c.last = -1;
     if (first < end) {
-      int lo = 0, hi = kKwThreads;
+      int lo = 0, hi = few ? 32 : kKwThreads;
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if ((int64_t)s_sums[mid] * p.n_groups <= first) lo = mid; else hi = mid;
@@ -157,7 +167,7 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
       for (at.s = lo * run;; ++at.s) {
         seq = paged_seq(p, at.s);
         blk = key_blocks(p, seq);
-        of_group = steps_of(blk, lane);
+        of_group = run == 1 ? s_sums[lo + 1] - s_sums[lo] : steps_of(blk, lane);
         if (rest < of_group * p.n_groups) break;
         rest -= of_group * p.n_groups;
       }
