@@ -169,6 +169,13 @@ def test_many_sequences(K, formula):
     check(call(K, d), formula(d))
 
 
+@pytest.mark.parametrize("n", [31, 32, 33, 319, 321, 513])
+def test_as_many_sequences_as_a_list_is_cut_by(K, formula, n):
+    """A warp's number of sequences, a CTA's, one more: chunks and tokens, some without rows, the longest last."""
+    d = make([(0 if i % 5 == 2 else 1 + i % 4 * 3, i * 7 % 40) for i in range(n - 1)] + [(70, 90)], 2, 4, 64, 16, seed=n)
+    check(call(K, d), formula(d))
+
+
 @pytest.mark.parametrize("table", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rope", [0, 2, 16, 32, 64])
 def test_rotated_part(K, formula, table, rope):
