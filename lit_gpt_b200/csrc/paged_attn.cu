@@ -864,7 +864,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   // 2000 13.6, 10.4, over 8000 30.6, 28.1; of 8 groups of 4 heads over 8000 16.6, 17.2; 16 tokens of 32 groups over 300 18.5, 19.5; 64 of 8 groups over 100 14.4, 15.4; of 12 groups, 64 numbers
   // a head, over 500 22.5, 17.9; 16 of them over 1000 16.4, 17.9.
   s.cluster = 0;
-  if (max_rows == 1 && !kw && most <= 16 && (path == 0 || path == 4)) {
+  if (max_rows == 1 && !kw && per <= 16 && (path == 0 || path == 4)) {   // (then the list takes every sequence, and nq queries hold a group's heads)
     const int64_t key_tiles = (max_length + kShTile - 1) / kShTile, pairs = (int64_t)n_seqs * n_groups;
     int ctas = 1;
     while (ctas < 8 && (ctas * 4 < key_tiles || ctas * 4 < per) && pairs * 2 * ctas <= 2 * sm_count()) ctas *= 2;   // (its CTAs share the heads' joins, too)
@@ -895,6 +895,7 @@ cudaError_t launch_list(const PagedParams& p, const PagedPlan& s, cudaStream_t s
 template <int HS, int NQ>
 cudaError_t launch_clusters(const PagedParams& p, const PagedPlan& s, cudaStream_t st) {
   using C = ClSmem<HS, NQ>;
+  if (p.per > 8 * NQ) return cudaErrorInvalidValue;
   static PerDeviceOnce once;
   if (once.need()) {
     const cudaError_t e = cudaFuncSetAttribute(paged_cluster_kernel<HS, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
