@@ -317,7 +317,8 @@ int b200_attn_decode_shared_tune(int path);
  *   row_pos    position of every row, its row of the tables (clamped); apart from the keys' places, since a cache may hold fewer keys than a sequence has positions
  *   row_seq    int32, the sequence of every row; a row of none (-1, or outside its sequence's rows) takes no part, its result is zero
  *   seqs       int32 (n_seqs, 4) on a 16-byte boundary: first row, rows, keys in the cache before the step, row of the page table.  Sequences of no rows, of more
- *              than max_rows, or that reach beyond rows or table_seqs take no part.
+ *              than max_rows, or that reach beyond rows or table_seqs take no part.  Sequences share no rows: of some that do, and come to more work than the step's rows can, nothing
+ *              is done, and their results are zero.
  *   pages      int32 (table_seqs, max_pages), rows pages_ld apart: entry i of a sequence's row is the page of its keys [i * page, (i + 1) * page).  Where the entry is no page (outside
  *              0 .. pool - 1) there are no keys: new ones are dropped, the rest take no part.  A row that sees no key has a result of zero.
  *   k_pages, v_pages   (pool, n_groups, page, head_size) bf16, rows head_size apart, pages and groups at the given distances (elements, multiples of 8); page 16, 32, 64, 128 or 256.

@@ -43,7 +43,7 @@ struct PagedParams {
   float* scores; int score_rows, kept_max;                  // scores of the list's tiles, that many queries each; of sequences of up to kept_max queries a group (0: none are kept)
   int kw_workers; float* kw_part; PagedWeightCut* kw_cuts;  // CTAs that compute the others' again, their sums: two slots of 128 keys a CTA
   int* tile_base;                                           // per sequence: its first tile in the list; -1: nothing was done
-  int* item_base;                                           // per sequence: its first item
+  int* item_base;                                           // per sequence: its first item; -1 likewise
   int ways;                                                 // warps that join a head's results
   float scale_log2;
 };

@@ -213,7 +213,7 @@ __device__ __forceinline__ Split make_split(const PagedParams& p, int2* sums, in
     for (int i = tid * run; i < min(p.n_seqs, (tid + 1) * run); ++i) {
       const PagedSeq q = paged_seq(p, i);
       const int n = seq_items(p, q);
-      __stcg(p.item_base + i, before.y * p.n_groups);
+      __stcg(p.item_base + i, fits ? before.y * p.n_groups : -1);
       __stcg(p.tile_base + i, fits ? before.x * p.n_groups : -1);
       before.x += n * seq_tiles(q);
       before.y += n;
@@ -546,8 +546,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   float top = -INFINITY, sum = 0.f, a[V] = {};
   const int gi = h / p.per, m = (row - s.first) * p.per + h - gi * p.per;
   int item = -1;
-  if (h < p.n_head && !idle && s.n > 0) item = __ldcg(p.item_base + which) + gi * seq_items(p, s) + m / p.tile_rows;
-  if (item >= 0 && item < p.items) {
+  if (h < p.n_head && !idle && s.n > 0) item = __ldcg(p.item_base + which);
+  if (item >= 0) {                 // (less where nothing was done: there is no result to read)
+    item += gi * seq_items(p, s) + m / p.tile_rows;
     const int at = m % p.tile_rows;
     const int2 at_w = __ldcg(p.where + item);
     join_results<V>(way, p.ways, at_w.y, lane, top, sum, a, [&](int i, const float2*& ml, const float*& acc) {
