@@ -6,8 +6,9 @@ namespace b200 {
 
 constexpr int kMaxTiles = 1 << 29;          // of a step
 
+constexpr int kCutNothing = -2;
 struct PagedCut {                                           // what a CTA of paged_attn_tc05.cu goes on with that others began
-  int first, last;                                          // the CTAs that have segments of it; last -1: it begins with an item of its own
+  int first, last;                                          // the CTAs that have segments of it; last -1: it begins with an item of its own, kCutNothing: nothing was done
   int count, row, gi;                                       // its queries, its first row, its group
 };
 

@@ -469,6 +469,14 @@ __device__ __forceinline__ void join_cut(const PagedParams& p, int index, int pa
   constexpr int V = HS / 8;
   const int w = index / parts, part = index - w * parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PagedCut c = p.cuts[w];
+  if (c.last == kCutNothing && w == 0) {           // rows that were the tensor memory's see no key
+    for (int row = part; row < p.rows; row += parts) {
+      const int which = p.row_seq[row];
+      if (which < 0 || which >= p.n_seqs || paged_seq(p, which).rows * p.per <= p.list_max) continue;
+      for (int i = threadIdx.x; i < p.n_head * HS / 8; i += blockDim.x) reinterpret_cast<uint4*>(p.out + (int64_t)row * p.n_head * HS)[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = threadIdx.x; p.lse && i < p.n_head; i += blockDim.x) p.lse[((int64_t)(i / p.per) * p.rows + row) * p.per + i % p.per] = INFINITY;
+    }
+  }
   if (c.last < 0) return;
   const int shares = (c.last - c.first) * parts, share = (w - c.first - 1) * parts + part;
   for (int m0 = share * 32; m0 < c.count; m0 += shares * 32) {

@@ -200,7 +200,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     at.tile = first;
     at.end = end;
     PagedCut c = {};                    // for the launch that joins: the item that this CTA goes on with
-    c.last = -1;
+    c.last = all64 < kMaxTiles ? -1 : kCutNothing;
     if (first < end) {
       int lo = 0, hi = few ? 32 : kPtThreads;
       while (hi - lo > 1) {
@@ -295,11 +295,6 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   if (tid == 0) list_segments();
   griddep_wait();                         // (tensor memory is taken behind the wait only)
   if (p.mixed) griddep_launch();
-  if (all64 >= kMaxTiles) {               // nothing is done: no row sees a key
-    const int64_t from = (int64_t)blockIdx.x * kPtThreads + tid, step = (int64_t)ctas * kPtThreads, heads = (int64_t)p.rows * p.n_head;
-    for (int64_t i = from; i < heads * (HS / 8); i += step) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int64_t i = from; p.lse && i < heads; i += step) p.lse[i] = INFINITY;
-  }
   if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
   if (tid == 0) p.cuts[blockIdx.x] = s_cut;
   tc::fence_before();
