@@ -30,7 +30,7 @@ struct PagedParams {
   __nv_bfloat16* out;
   int rows, n_head, n_groups, per, max_rows, max_length;
   __nv_bfloat16* q;                                         // the queries, turned: [n_groups][rows * per][HS]
-  float* lse;                                               // [n_groups][rows * per] log2 of the sum of exponentials of a query's scores (with kw)
+  float* lse;                                               // [n_groups][rows * per] log2 of the sum of exponentials of a query's scores (with kw); inf: it sees no key; NaN: a score is
   int tile_rows;                                            // queries of an item
   int items;                                                // at most
   int workers, sms;                                         // warps that share the tiles, at most

@@ -519,13 +519,13 @@ __device__ __forceinline__ void join_cut(const PagedParams& p, int index, int pa
     }
     if (m >= c.count) continue;
     const int row = m / p.per, hh = m - row * p.per;
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;   // (a sum that is NaN stays one)
     __nv_bfloat16* const to = p.out + ((int64_t)(c.row + row) * p.n_head + c.gi * p.per + hh) * HS + warp * V;
 #pragma unroll
     for (int j = 0; j < V; j += 8)
       *reinterpret_cast<uint4*>(to + j) = make_uint4(pack_bf16(a[j] * inv, a[j + 1] * inv), pack_bf16(a[j + 2] * inv, a[j + 3] * inv), pack_bf16(a[j + 4] * inv, a[j + 5] * inv),
                                                      pack_bf16(a[j + 6] * inv, a[j + 7] * inv));
-    if (p.lse && warp == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum > 0.f ? top + log2f(sum) : INFINITY;
+    if (p.lse && warp == 0) p.lse[((int64_t)c.gi * p.rows + c.row) * p.per + m] = sum == 0.f ? INFINITY : top + log2f(sum);
   }
 }
 
@@ -575,8 +575,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
     if (way == 0) join_warps<HS>(s_acc[warp], s_ml + warp, p.ways, lane, top, sum, a);
   }
   if (way > 0 || h >= p.n_head || idle) return;
-  store_result<HS>(p.out + ((int64_t)row * p.n_head + h) * HS, a, sum > 0.f ? 1.f / sum : 0.f, lane);
-  if (p.lse && lane == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h - gi * p.per] = sum > 0.f ? top + log2f(sum) : INFINITY;
+  store_result<HS>(p.out + ((int64_t)row * p.n_head + h) * HS, a, sum == 0.f ? 0.f : 1.f / sum, lane);
+  if (p.lse && lane == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h - gi * p.per] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
 
 // ---- few single tokens: a sequence and group's whole step by a cluster of CTAs, in one launch ----
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
       sum += l[u] * f;
       y += l[u] == 0.f ? 0.f : x[u] * f;
     }
-    p.out[((int64_t)row * p.n_head + gi * p.per + h) * HS + i % HS] = __float2bfloat16_rn(sum > 0.f ? y / sum : 0.f);
+    p.out[((int64_t)row * p.n_head + gi * p.per + h) * HS + i % HS] = __float2bfloat16_rn(sum == 0.f ? 0.f : y / sum);
   }
   // no CTA leaves, and frees its shared memory, before the others have read it
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -798,11 +798,17 @@ __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
     if (!at) continue;
     float sum = 0.f;
     const float before = *at;
-    for (int m0 = 0, index = first + gi * items * tiles + key / kShTile; m0 < count; m0 += p.tile_rows, index += tiles) {
+    int low = 0, m0 = 0, index = first + gi * items * tiles + key / kShTile;
+    if (key > s.cached) {                          // a chunk's own: queries before this one do not see the key, whatever their sums are
+      low = (key - s.cached) * p.per;
+      m0 = low / p.tile_rows * p.tile_rows;
+      index += low / p.tile_rows * tiles;
+    }
+    for (; m0 < count; m0 += p.tile_rows, index += tiles) {
       const float* const kept = p.scores + (int64_t)index * p.score_rows * kShTile + key % kShTile;
       const int n = min(p.tile_rows, count - m0);
 #pragma unroll 8
-      for (int m = 0; m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
+      for (int m = max(low - m0, 0); m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
     }
     *at = before + sum;
   }

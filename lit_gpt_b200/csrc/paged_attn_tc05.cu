@@ -596,7 +596,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           const int slot = g.slot;
           const int hh = g.m0 + tid - row * p.per;
           if (slot < 0) {
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
             const int64_t y_at = tid < count ? ((int64_t)(g.first + row) * p.n_head + g.gi * p.per + hh) * HS : -1;
 #pragma unroll 1
             for (int c0 = 0; c0 < HS; c0 += 32) {
@@ -627,7 +627,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
                 if (to_row >= 0) *reinterpret_cast<uint4*>(p.out + to_row + c0 + (lane & 3) * 8) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
               }
             }
-            if (p.lse && tid < count) p.lse[g.q0 + tid] = l > 0.f ? m * sl + log2f(l) : INFINITY;
+            if (p.lse && tid < count) p.lse[g.q0 + tid] = l == 0.f ? INFINITY : m * sl + log2f(l);
           } else {
             float* const at = p.tc_acc + (int64_t)slot * 256 * HS + tid * 4;   // four numbers of every query side by side: a warp's stores are whole lines (a query's all together: 4 us a segment)
 #pragma unroll 1

@@ -16,6 +16,8 @@
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
+#include <type_traits>
+
 namespace b200 {
 
 namespace {
@@ -72,6 +74,7 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
   __shared__ __align__(8) uint64_t s_bars[29];
   __shared__ __align__(16) float s_lse[8][128];            // of the last eight tiles of queries, negative: tile i + 8's are written once the products of tile i + 4 are done, whose scores
                                                            // take the place of tile i's
+  __shared__ int s_blind[8];                               // whether a query of theirs sees no key, or there are fewer than 128
   __shared__ float s_sum[128];
   __shared__ KwSeg s_seg[kKwSegs];
   __shared__ KwAt s_at;
@@ -285,6 +288,8 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
           ok = __all_sync(0xffffffffu, tc::mbar_wait(q_empty + 8 * s, ((uint32_t)(tiles_done >> 2) & 1u) ^ 1u));
           if (!ok) break;
           *reinterpret_cast<float4*>(&s_lse[tiles_done & 7][lane * 4]) = make_float4(f[0], f[1], f[2], f[3]);
+          const int blind = __any_sync(0xffffffffu, f[0] == -INFINITY || f[1] == -INFINITY || f[2] == -INFINITY || f[3] == -INFINITY);
+          if (lane == 0) s_blind[tiles_done & 7] = blind;
           __syncwarp();                   // (written before the barrier that hands them over is arrived on)
           if (lane == 0) {
             tc::mbar_expect_tx(q_full + 8 * s, C::kBytes);
@@ -345,39 +350,47 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
           if (!ok) break;
           tc::fence_after();
           const int m0 = j * 128;
-          const bool masked = m0 < w_low || m0 + 128 > g.m;
           const float* const lse = s_lse[tiles_done & 7];
           uint32_t x[32], y[32];
-          auto add = [&](uint32_t (&v)[32], int i) {
-            if (masked) {
-              const int a = low - m0 - i * 32, b = g.m - m0 - i * 32;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (e < a || e >= b) v[e] = 0xff800000u;
-            }
+          auto add = [&](uint32_t (&v)[32], int i, auto masked) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const float4 l = *reinterpret_cast<const float4*>(lse + i * 32 + e);
               float a, b, d, h;
               un2(fma2(pk2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sl2, pk2(l.x, l.y)), a, b);
               un2(fma2(pk2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), sl2, pk2(l.z, l.w)), d, h);
-              sum[0] = add2(sum[0], pk2(ex2(a), ex2(b)));
-              sum[1] = add2(sum[1], pk2(ex2(d), ex2(h)));
+              a = ex2(a);
+              b = ex2(b);
+              d = ex2(d);
+              h = ex2(h);
+              if constexpr (masked.value) {   // (behind the exponentials: what a query gives a key that it does not see is zero even where its sum is NaN)
+                const int from = low - m0 - i * 32;
+                if (e < from || l.x == -INFINITY) a = 0.f;
+                if (e + 1 < from || l.y == -INFINITY) b = 0.f;
+                if (e + 2 < from || l.z == -INFINITY) d = 0.f;
+                if (e + 3 < from || l.w == -INFINITY) h = 0.f;
+              }
+              sum[0] = add2(sum[0], pk2(a, b));
+              sum[1] = add2(sum[1], pk2(d, h));
             }
           };
           const uint32_t at = tmem + lanes + s * 128;
-          tc::ld32(x, at);
-          tc::wait_ld(x);
-          tc::ld32(y, at + 32);
-          add(x, 0);
-          tc::wait_ld(y);
-          tc::ld32(x, at + 64);
-          add(y, 1);
-          tc::wait_ld(x);
-          tc::ld32(y, at + 96);
-          add(x, 2);
-          tc::wait_ld(y);
-          add(y, 3);
+          auto add_all = [&](auto masked) {
+            tc::ld32(x, at);
+            tc::wait_ld(x);
+            tc::ld32(y, at + 32);
+            add(x, 0, masked);
+            tc::wait_ld(y);
+            tc::ld32(x, at + 64);
+            add(y, 1, masked);
+            tc::wait_ld(x);
+            tc::ld32(y, at + 96);
+            add(x, 2, masked);
+            tc::wait_ld(y);
+            add(y, 3, masked);
+          };
+          if (m0 < w_low || s_blind[tiles_done & 7]) add_all(std::true_type{});
+          else add_all(std::false_type{});
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(s_empty + 8 * s);   // (behind the last look at the queries' lse: their place is taken again four tiles after the scores')

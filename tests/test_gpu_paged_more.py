@@ -62,3 +62,44 @@ def test_sequences_that_share_rows_on_the_tensor_memory(E, weights):
     out = E.attn_paged(qkv, cos, sin, torch.arange(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda"), i32(0, rows, length - rows, 0).expand(n, 4).contiguous(),
                        table, k, v, G, G, hs, hs, max_rows=rows, max_length=length, key_weights=kw)
     assert not out.any() and (k == 1).all() and (v == 1).all() and (kw is None or (kw == 1).all())
+
+
+def check_with_nan(got, bad, clean):
+    """What the formula of the spoilt inputs says is NaN is; everything else is what it is without them."""
+    out, kw = got[0].cpu().to(F64), None if got[3] is None else got[3].cpu().to(F64)
+    wrong = torch.isnan(bad[0])
+    assert wrong.any() and torch.equal(torch.isnan(out), wrong)
+    over = ((out - clean[0]).abs() - (2 ** -8 * clean[0].abs() + clean[1]))[~wrong]
+    assert over.numel() == 0 or over.max().item() <= 0, over.max().item()
+    if kw is not None:
+        wrong = torch.isnan(bad[4])
+        assert wrong.any() and torch.equal(torch.isnan(kw), wrong)
+        over = ((kw - clean[4]).abs() - clean[5])[~wrong]
+        assert over.max().item() <= 0, over.max().item()
+
+
+@pytest.mark.parametrize("hs,groups,per,page", [(64, 2, 4, 16), (128, 3, 1, 64), (128, 1, 16, 32)])
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("steps", [[(1, 0)], [(1, 300)], [(1, 40), (1, 700), (1, 9)], [(1, 5000)], [(1, 40), (5, 3), (1, 9)], [(200, 100)], [(1, 60), (130, 700), (3, 0)]],
+                         ids=["first", "token", "tokens", "long", "short chunk", "chunk", "mixed"])
+@pytest.mark.parametrize("where", ["query", "key", "infinite query"])
+def test_what_is_not_a_number_stays_so(K, formula, hs, groups, per, page, weights, steps, where):
+    """A query that holds NaN, a key that does: results of the heads that see it are NaN, and so is the weight of every key that they see; no other's."""
+    d = make(steps, groups, per, hs, page, rope=0 if where == "infinite query" else None, weights=weights, seed=len(steps) + per)
+    s = len(steps) // 2
+    first, rows, cached, at = d["seqs"][s].tolist()
+    g = groups - 1
+    row = (first + rows // 2, g, per - 1, 3)
+    heads = lambda of: of["qkv"].view(-1, groups, per + 2, hs)
+    if where == "infinite query":                    # scores of +inf
+        d["k"][..., 3] = heads(d)[:, :, per, 3] = 1.0
+    clean = formula(d)
+    spoilt = {k: v.clone() if torch.is_tensor(v) else v for k, v in d.items()}
+    if where == "key" and cached > 0:                # an older one
+        j = cached * 2 // 3
+        spoilt["k"][d["pages"][at, j // page], g, j % page, 5] = float("nan")
+    elif where == "key":                             # the step's own
+        heads(spoilt)[first + rows // 2, g, per, hs - 1] = float("nan")
+    else:
+        heads(spoilt)[row] = float("nan" if where == "query" else "inf")
+    check_with_nan(call(K, spoilt), formula(spoilt), clean)
