@@ -327,7 +327,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         for (int j = lo; j < hi; ++j, ++tiles_done) {
           const int s = tiles_done & 1;
           const int next = j + 1 < hi ? page_of(j + 1) : -1;
-          ok = __all_sync(0xffffffffu, tc::mbar_wait_here(empty + 8 * s, ((uint32_t)(tiles_done >> 1) & 1u) ^ 1u));
+          ok = __all_sync(0xffffffffu, tc::mbar_wait_loop(empty + 8 * s, ((uint32_t)(tiles_done >> 1) & 1u) ^ 1u));
           if (!ok) break;
           const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
           const bool whole = have == (1u << parts) - 1u;
@@ -364,7 +364,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
             if (lane == 0) tc::mbar_arrive(full + 8 * s);
           }
           if (keys && j == lo) {        // the queries, once the segment before has done its last product with the ones there
-            if (tiles_done > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait_here(k_empty + 8 * (s ^ 1), (uint32_t)((tiles_done - 1) >> 1) & 1u));
+            if (tiles_done > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait_loop(k_empty + 8 * (s ^ 1), (uint32_t)((tiles_done - 1) >> 1) & 1u));
             if (!ok) break;
             const int halves = g.count > 128 ? 2 : 1;
             if (lane == 0) {
@@ -400,7 +400,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         for (int c = 0; c < segs && ok; ++c) {
           const Seg& g = s_seg[c];
           const int lo = g.lo, hi = g.hi, hi0 = g.hi0, hi1 = g.count > 128 ? hi : lo;
-          ok = tc::mbar_wait_here(q_full, (uint32_t)segs_done & 1u) && tc::mbar_wait_here(k_full + 8 * (tiles_done & 1), (uint32_t)(tiles_done >> 1) & 1u);
+          ok = tc::mbar_wait_loop(q_full, (uint32_t)segs_done & 1u) && tc::mbar_wait_loop(k_full + 8 * (tiles_done & 1), (uint32_t)(tiles_done >> 1) & 1u);
           if (!ok) break;
           tc::fence_after();
 #pragma unroll
@@ -411,7 +411,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           for (int j = lo; j < hi; ++j, ++tiles_done) {
             const int i = tiles_done, s = i & 1, s1 = s ^ 1;
             const bool more_keys = j + 1 < hi;
-            ok = tc::mbar_wait_here(v_full + 8 * s, (uint32_t)(i >> 1) & 1u) && (!more_keys || tc::mbar_wait_here(k_full + 8 * s1, (uint32_t)((i + 1) >> 1) & 1u));
+            ok = tc::mbar_wait_loop(v_full + 8 * s, (uint32_t)(i >> 1) & 1u) && (!more_keys || tc::mbar_wait_loop(k_full + 8 * s1, (uint32_t)((i + 1) >> 1) & 1u));
             if (!ok) break;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -420,7 +420,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
                 const uint32_t dv = v_low + s * (C::kBytes >> 4);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                  ok = ok && tc::mbar_wait_here((half ? p_full : p_half) + 8 * t, n[t] & 1u);
+                  ok = ok && tc::mbar_wait_loop((half ? p_full : p_half) + 8 * t, n[t] & 1u);
                   if (!ok) break;
                   tc::fence_after();
 #pragma unroll
@@ -442,7 +442,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         }
         if (!ok) {
           tc::commit(idle);
-          tc::mbar_wait_here(idle, 0);
+          tc::mbar_wait_loop(idle, 0);
         }
       }
       ok = __all_sync(0xffffffffu, ok);
@@ -465,7 +465,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (j >= (t ? hi1 : hi0)) continue;
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait_here(shrink + 8 * (4 * t + v), n[t] & 1u));
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait_loop(shrink + 8 * (4 * t + v), n[t] & 1u));
             if (!ok) break;
             const float f = s_shrink[t * 128 + v * 32 + lane];
             if (__any_sync(0xffffffffu, f != 1.0f)) {   // (S of this step is there, so P V of the last one is done; a segment's first step has f = 1)
@@ -512,7 +512,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         f2 l2[2] = {0ull, 0ull};
         const uint32_t n0 = n[0];
         for (int j = lo; j < hi; ++j, ++n[0]) {
-          ok = ok && __all_sync(0xffffffffu, tc::mbar_wait_here(s_full + 8 * t, n[0] & 1u));
+          ok = ok && __all_sync(0xffffffffu, tc::mbar_wait_loop(s_full + 8 * t, n[0] & 1u));
           if (!ok) break;
           tc::fence_after();
           const int j0 = j * 128;
@@ -584,7 +584,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         tiles_before += g.hi - lo;
         const bool any = n[0] != n0;
         if (any && ok) {
-          ok = __all_sync(0xffffffffu, tc::mbar_wait_here(o_done + 8 * t, (n[0] - 1) & 1u));
+          ok = __all_sync(0xffffffffu, tc::mbar_wait_loop(o_done + 8 * t, (n[0] - 1) & 1u));
           tc::fence_after();
         }
         if (!ok) break;
@@ -655,8 +655,8 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     // copies on their way: neither stage may be written once this CTA has left
     if (warp == 13 || warp == 14) {
       const uint32_t full = warp == 13 ? k_full : v_full;
-      for (int e = max(tiles_done - 2, 0); e < tiles_done; ++e) tc::mbar_wait_here(full + 8 * (e & 1), (uint32_t)(e >> 1) & 1u);
-      if (warp == 13 && segs_done > 0) tc::mbar_wait_here(q_full, (uint32_t)(segs_done - 1) & 1u);
+      for (int e = max(tiles_done - 2, 0); e < tiles_done; ++e) tc::mbar_wait_loop(full + 8 * (e & 1), (uint32_t)(e >> 1) & 1u);
+      if (warp == 13 && segs_done > 0) tc::mbar_wait_loop(q_full, (uint32_t)(segs_done - 1) & 1u);
     }
     *err = 1u;
   }
