@@ -315,7 +315,8 @@ int b200_attn_decode_shared_tune(int path);
  * sequence's keys up to its own.
  *   qkv        (rows, (n_head + 2 n_groups) * head_size) bf16, interleaved per group as in b200_attn_decode
  *   row_pos    position of every row, its row of the tables (clamped); apart from the keys' places, since a cache may hold fewer keys than a sequence has positions
- *   row_seq    int32, the sequence of every row; a row of none (-1, or outside its sequence's rows) takes no part, its result is zero
+ *   row_seq    int32, the sequence of every row; a row of none (-1, or outside its sequence's rows) takes no part, its result is zero.  Where a sequence's range holds such a row (the padded end of a chunk), it
+ *              has no query there, nothing is stored in its place, and there is no key
  *   seqs       int32 (n_seqs, 4) on a 16-byte boundary: first row, rows, keys in the cache before the step, row of the page table.  Sequences of no rows, of more
  *              than max_rows, or that reach beyond rows or table_seqs take no part.  Sequences share no rows: of some that do, and come to more work than the step's rows can, nothing
  *              is done, and their results are zero.

@@ -14,7 +14,7 @@ struct PagedCut {                                           // what a CTA of pag
 
 struct PagedWeightCut {                                     // a block of 128 keys that several CTAs of paged_weights.cu have parts of
   int first, last;                                          // those CTAs; last -1: none to join
-  int table, n, gi, block;
+  int s, table, cached, n, row, gi, block;                  // its sequence, and that one's first row
 };
 
 struct PagedParams {
@@ -22,7 +22,7 @@ struct PagedParams {
   const void* cos; const void* sin;
   int table_bf16, table_rows, table_presel, rope_n, wide;   // wide: rows of heads and tables allow accesses of HS / 32 numbers
   const void* row_pos; int pos64;                           // position of every row in the rotation's tables
-  const int* row_seq;                                       // sequence of every row
+  const int* row_seq;                                       // sequence of every row: one that is not the sequence's whose range holds it takes no part
   const int4* seqs; int n_seqs;                             // first row, rows, keys in the cache before the step, row of the page table
   const int* pages; int64_t pages_ld; int page_rows, max_pages, pool, shift;   // page table (page_rows, max_pages), pages there are, log2 of a page's keys
   __nv_bfloat16* k; __nv_bfloat16* v; int64_t k_page, k_group, v_page, v_group;
@@ -95,6 +95,14 @@ __device__ __forceinline__ int page_at(const PagedParams& p, int table, int inde
   if (index >= p.max_pages) return -1;
   const int id = p.pages[(int64_t)table * p.pages_ld + index];
   return id >= 0 && id < p.pool ? id : -1;
+}
+
+// The page of key `key` of sequence s; -1: there is no such key, since it has no page or, of the step's own, its row is not the sequence's
+__device__ __forceinline__ int whose_key(const PagedParams& p, int s, int cached, int first_row, int key) { return key < cached ? s : p.row_seq[first_row + key - cached]; }
+__device__ __forceinline__ int key_page(const PagedParams& p, int s, int table, int cached, int first_row, int n, int key) {
+  if (key >= n) return -1;
+  const int whose = whose_key(p, s, cached, first_row, key), id = page_at(p, table, key >> p.shift);   // (both on their way at once)
+  return whose == s ? id : -1;
 }
 
 __device__ __forceinline__ int capped(int64_t x) { return (int)(x < kMaxTiles ? x : kMaxTiles); }

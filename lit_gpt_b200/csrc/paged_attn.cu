@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_wide_kernel(const PagedPa
       if (h < p.per) {
         __nv_bfloat16* const to = p.out + ((int64_t)row * p.n_head + gi * p.per + h) * HS;
         *reinterpret_cast<uint4*>(to + a) = *reinterpret_cast<uint4*>(to + b) = make_uint4(0u, 0u, 0u, 0u);
+        if (p.lse && piece == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h] = INFINITY;
       }
       continue;
     }
@@ -126,6 +127,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) 
     if (h < p.per) {
       __nv_bfloat16* const to = p.out + ((int64_t)row * p.n_head + gi * p.per + h) * HS;
       for (int j = 0; j < V; ++j) to[lane * V + j] = __float2bfloat16_rn(0.f);
+      if (p.lse && lane == 0) p.lse[((int64_t)gi * p.rows + row) * p.per + h] = INFINITY;
     }
     return;
   }
@@ -235,13 +237,9 @@ struct Tile {
   int tile, tiles;                   // of the item
   int item;
   int id0, id1;                      // pages of its first and last sixteen keys
+  uint32_t bits;                     // its keys that are there
   __device__ __forceinline__ int left() const { return tiles - 1 - tile; }
   __device__ __forceinline__ int key0() const { return tile * kShTile; }
-  __device__ __forceinline__ uint32_t bits() const {   // its keys that are there
-    const int rest = seq.n - key0();
-    const uint32_t in = rest >= 32 ? 0xffffffffu : (1u << rest) - 1u;
-    return in & ((id0 >= 0 ? 0xffffu : 0u) | (id1 >= 0 ? 0xffff0000u : 0u));
-  }
 };
 
 struct Walk {
@@ -249,10 +247,19 @@ struct Walk {
   const int2* sums;
   int run, threads;
 
-  __device__ __forceinline__ void locate(Tile& t) const {
+  __device__ __forceinline__ void pages(Tile& t) const {
     const int i = t.key0() >> p.shift;
     t.id0 = page_at(p, t.seq.table, i);
     t.id1 = p.shift == 4 && t.key0() + 16 < t.seq.n ? page_at(p, t.seq.table, i + 1) : t.id0;
+    const int rest = t.seq.n - t.key0();
+    t.bits = (rest >= 32 ? 0xffffffffu : (1u << rest) - 1u) & ((t.id0 >= 0 ? 0xffffu : 0u) | (t.id1 >= 0 ? 0xffff0000u : 0u));
+  }
+  __device__ __forceinline__ void locate(Tile& t) const {   // by a warp
+    pages(t);
+    if (t.seq.rows > 1 && t.key0() + kShTile > t.seq.cached) {   // (of a single token's key nobody asks whose it is: a result that is not the sequence's goes nowhere)
+      const int key = t.key0() + (threadIdx.x & 31);
+      t.bits &= __ballot_sync(0xffffffffu, key < t.seq.n && whose_key(p, t.s, t.seq.cached, t.seq.first, key) == t.s);
+    }
   }
   __device__ __forceinline__ Tile find(int index) const {
     Tile t;
@@ -309,7 +316,7 @@ struct Walk {
 template <int HS>
 __device__ __forceinline__ void load_tile(const PagedParams& p, const Tile& t, const __nv_bfloat16* base, int64_t page, int64_t group, uint32_t dst, int lane) {
   constexpr int CH = HS / 8, RP = 32 / CH;   // 16-byte pieces of a row, rows a warp copies at once
-  const uint32_t bits = t.bits();
+  const uint32_t bits = t.bits;
   const int c = lane % CH, in = t.key0() & ((1 << p.shift) - 1);
   const __nv_bfloat16* const g = base + (int64_t)t.gi * group + c * 8;
   const __nv_bfloat16* const a = g + (int64_t)max(t.id0, 0) * page + (int64_t)in * HS;
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(PgSmem<HS, NQ>::kWarps * 32, 1) paged_list_ker
       __syncwarp();
       return vb;
     };
-    const uint32_t bits = cur.bits();
+    const uint32_t bits = cur.bits;
     const int key0 = cur.key0(), count = walk.queries(cur);
     float* const kept = KEEP ? p.scores + (int64_t)cur.index * p.score_rows * kShTile : nullptr;
     auto keep = [&](int key, int t, int c, float s) {
@@ -618,15 +625,17 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
   t.tile = rank * W + warp;
   const uint32_t kb = pf_smem(cl_smem) + warp * C::kWarp, vb = kb + C::kUnit;
   // the new key is not read from its page: it comes from shared memory
+  const int whose = p.row_seq[row];                // (where the row is another's, or none's, nothing of it is stored)
   const int fresh = key < t.seq.n && page_at(p, t.seq.table, key >> p.shift) >= 0 ? key : -1;
   auto load = [&](const Tile& x, const __nv_bfloat16* base, int64_t page, int64_t group, uint32_t dst) {
     Tile y = x;
-    y.seq.n = min(y.seq.n, key);
+    const int at = key - x.key0();
+    if (at >= 0 && at < kShTile) y.bits &= ~(1u << at);
     load_tile<HS>(p, y, base, page, group, dst, lane);
     pf_commit();
   };
   if (t.tile < t.tiles) {
-    walk.locate(t);
+    walk.pages(t);
     load(t, p.k, p.k_page, p.k_group, kb);
     load(t, p.v, p.v_page, p.v_group, vb);
   }
@@ -649,7 +658,7 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
       else *reinterpret_cast<uint32_t*>(at) = v[0];
     };
     store(h < 8 * NQ ? s_q + sw<HS>(h, lane * V / 8) + lane * V % 8 * 2 : s_new + (h - 8 * NQ) * HS * 2 + lane * V * 2);
-    if (h >= 8 * NQ && rank == 0 && fresh >= 0) {
+    if (h >= 8 * NQ && rank == 0 && fresh >= 0 && whose == item / p.n_groups) {
       const int64_t id = page_at(p, t.seq.table, key >> p.shift), in = key & ((1 << p.shift) - 1);
       store((h == 8 * NQ ? p.k + id * p.k_page + (int64_t)gi * p.k_group : p.v + id * p.v_page + (int64_t)gi * p.v_group) + in * HS + lane * V);
     }
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
     Tile next = t;
     next.tile += step;
     const bool more = next.tile < t.tiles;
-    if (more) walk.locate(next);
+    if (more) walk.pages(next);
     const int at = fresh - t.key0();               // the new key's place in this tile
     auto patch = [&](uint32_t dst, int which) {
       if (at >= 0 && at < kShTile) {
@@ -681,7 +690,7 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
     pf_wait<1>();
     __syncwarp();
     patch(kb, 0);
-    const uint32_t bits = t.bits();
+    const uint32_t bits = t.bits;
     attend_tile<HS, NQ, NQ>(a, pf_smem(s_q), 0, kb, p.scale_log2, lane, [bits](int k, int, int) { return ((bits >> k) & 1u) != 0u; }, [](int, int, int, float) {}, [&]() {
       __syncwarp();
       if (more) load(next, p.k, p.k_page, p.k_group, kb); else pf_commit();
@@ -758,7 +767,7 @@ __global__ void __launch_bounds__(ClSmem<HS, NQ>::kWarps * 32) paged_cluster_ker
       sum += l[u] * f;
       y += l[u] == 0.f ? 0.f : x[u] * f;
     }
-    p.out[((int64_t)row * p.n_head + gi * p.per + h) * HS + i % HS] = __float2bfloat16_rn(sum == 0.f ? 0.f : y / sum);
+    if (whose == item / p.n_groups) p.out[((int64_t)row * p.n_head + gi * p.per + h) * HS + i % HS] = __float2bfloat16_rn(sum == 0.f ? 0.f : y / sum);
   }
   // no CTA leaves, and frees its shared memory, before the others have read it
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -775,7 +784,7 @@ __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
     const int key = c.block * 128 + (int)threadIdx.x;
     float sum = 0.f;
     for (int w = c.first; w <= c.last; ++w) sum += __ldcg(p.kw_part + (2 * w + (w == c.first)) * 128 + threadIdx.x);
-    const int id = key < c.n ? page_at(p, c.table, key >> p.shift) : -1;
+    const int id = key_page(p, c.s, c.table, c.cached, c.row, c.n, key);
     if (id >= 0) p.kw[(((int64_t)id * p.n_groups + c.gi) << p.shift) + (key & ((1 << p.shift) - 1))] += sum;
     return;
   }
@@ -783,7 +792,7 @@ __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
   const PagedSeq s = paged_seq(p, which);
   const int items = seq_items(p, s);
   auto place = [&](int key) -> float* {
-    const int id = key < s.n ? page_at(p, s.table, key >> p.shift) : -1;
+    const int id = key_page(p, which, s.table, s.cached, s.first, s.n, key);
     return id < 0 ? nullptr : p.kw + (((int64_t)id * p.n_groups + gi) << p.shift) + (key & ((1 << p.shift) - 1));
   };
   int key = blockIdx.y * 256 + threadIdx.x;
@@ -796,20 +805,27 @@ __global__ void __launch_bounds__(256) paged_kept_kernel(const PagedParams p) {
   const float* const lse = p.lse + ((int64_t)gi * p.rows + s.first) * p.per;
   for (; key < s.n; key += gridDim.y * 256, at = place(key)) {
     if (!at) continue;
-    float sum = 0.f;
     const float before = *at;
-    int low = 0, m0 = 0, index = first + gi * items * tiles + key / kShTile;
-    if (key > s.cached) {                          // a chunk's own: queries before this one do not see the key, whatever their sums are
-      low = (key - s.cached) * p.per;
-      m0 = low / p.tile_rows * p.tile_rows;
-      index += low / p.tile_rows * tiles;
-    }
-    for (; m0 < count; m0 += p.tile_rows, index += tiles) {
-      const float* const kept = p.scores + (int64_t)index * p.score_rows * kShTile + key % kShTile;
-      const int n = min(p.tile_rows, count - m0);
+    auto gains = [&](bool rare) {
+      float sum = 0.f;
+      for (int m0 = 0, index = first + gi * items * tiles + key / kShTile; m0 < count; m0 += p.tile_rows, index += tiles) {
+        const float* const kept = p.scores + (int64_t)index * p.score_rows * kShTile + key % kShTile;
+        const int n = min(p.tile_rows, count - m0);
+        if (!rare) {
 #pragma unroll 8
-      for (int m = max(low - m0, 0); m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
-    }
+          for (int m = 0; m < n; ++m) sum += ex2(__ldcg(kept + m * kShTile) - __ldcg(lse + m0 + m));
+        } else {
+#pragma unroll 1
+          for (int m = 0; m < n; ++m) {
+            const float l = __ldcg(lse + m0 + m), x = ex2(__ldcg(kept + m * kShTile) - l);
+            sum += l == INFINITY || m0 + m < max(key - s.cached, 0) * p.per ? 0.f : x;
+          }
+        }
+      }
+      return sum;
+    };
+    float sum = gains(false);
+    if (sum != sum) sum = gains(true);             // of what is not a number only that counts which a row of the sequence that sees the key gives it
     *at = before + sum;
   }
 }

@@ -9,6 +9,7 @@
 //   * warp 12: one thread issues S = Q K^T and O += P V, 128 x 128 x 16 each, S of a tile's next step right behind its P V;
 //   * warp 13 brings the keys and the queries, warp 14 the values, two stages each, 128-byte-swizzled: a page, or what of it lies in the tile, is one TMA box; values of a tile that
 //     ends past the sequence's last key, or has no page somewhere, come row by row with cp.async, zeros where there is nothing.
+// A row that is not the sequence's whose range holds it (row_seq) is computed from whatever lies in its place and not stored; there is no key in its place.
 // A masked key has weight 0, and 0 times an infinite or NaN value is NaN: a value of the chunk that is not finite reaches the rows before its own, within its
 // tile of 128 keys and 128 queries.
 // Probabilities are rounded to bf16 as they multiply V; the running maximum is exact, so that the largest probability is 1 and loses nothing.  They are summed before the rounding: the
@@ -21,6 +22,8 @@
 // 4 us each; four numbers of 128 queries side by side: 2.
 #include "attn_tmem.cuh"
 #include "paged.cuh"
+
+#include <type_traits>
 
 namespace b200 {
 
@@ -66,7 +69,7 @@ __device__ __forceinline__ int steps_of(const Blocks& b, int lane) {
 struct Seg {
   int q0, count;           // first query in the workspace's order, queries
   int m0, first;           // its number within the sequence and group; the sequence's first row
-  int cached, n, table, gi;
+  int s, cached, n, table, gi;
   int lo, hi, hi0;         // key tiles; those of the first 128 queries end at hi0
   int slot;                // place of its results; -1: the item is done here
 };
@@ -91,6 +94,8 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   __shared__ uint32_t s_tmem;
   __shared__ int s_sums[kPtThreads + 1], s_warp[kPtThreads / 32];
   __shared__ Shares s_shares[kPtThreads / 32];
+  __shared__ long long s_held[kPtThreads / 32];          // rows that the sequences hold, by warps
+  __shared__ int s_owned[kPtThreads / 32];               // and those that are the sequence's which holds them: as many unless rows are taken out of a sequence's range
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t smem = (tc::smem_u32(pt_smem) + 1023u) & ~1023u;
   const uint32_t sq_ = smem, sk_ = smem + 2 * C::kBytes, sv_ = smem + 4 * C::kBytes;
@@ -103,14 +108,23 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
   // (of up to 32 sequences by one warp: without the other warps' sums 1 to 2 us less)
   const bool few = p.n_seqs <= 32;
   const int run = (p.n_seqs + kPtThreads - 1) / kPtThreads, turns = few && warp > 0 ? 0 : run;
-  int here = 0;
+  int here = 0, owned = 0;
+  long long held = 0;
   Shares work = {0ull, 0ull};
+#pragma unroll 4
+  for (int row = tid; row < p.rows; row += kPtThreads) {
+    const int of = p.row_seq[row];
+    const bool any = of >= 0 && of < p.n_seqs;
+    const PagedSeq s = paged_seq(p, any ? of : 0);
+    owned += any && row >= s.first && row - s.first < s.rows;
+  }
   for (int k = 0; k < turns; ++k) {
     const int i = tid * run + k;
     Blocks mine = {};
     if (i < p.n_seqs) {
       const PagedSeq s = paged_seq(p, i);
       mine = blocks_of(p, s);
+      held += s.rows;
       if (p.mixed) add_work(p, s, work);
     }
     if (mine.count <= 16) {
@@ -149,6 +163,13 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
       work.tensor += __shfl_xor_sync(0xffffffffu, work.tensor, o);
     }
     if (lane == 0) s_shares[warp] = work;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) held += __shfl_xor_sync(0xffffffffu, held, o);
+  owned = __reduce_add_sync(0xffffffffu, owned);
+  if (lane == 0) {
+    s_held[warp] = held;
+    s_owned[warp] = owned;
   }
   if (tid == kPtThreads - 32) {
     tc::mbar_init(q_full, 1);
@@ -267,7 +288,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         g.count = count;
         g.m0 = m0;
         g.first = seq.first;
-        g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at.gi;
+        g.s = at.s; g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at.gi;
         const int stop = min(steps, at.lo + at.end - at.tile);
         g.lo = max(at.lo - kLead, 0);
         g.hi = max(stop - kLead, 0);
@@ -307,11 +328,17 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
     __syncthreads();                      // (everyone has read s_more)
     return more;
   };
+  auto strangers = [&]() {                // whether a row is not the sequence's whose range holds it
+    long long held = 0, owned = 0;
+    for (int w = 0; w < kPtThreads / 32; ++w) { held += s_held[w]; owned += s_owned[w]; }
+    return held != owned;
+  };
   // A role has its loop over batches of segments to itself, so that its registers are its own: the softmax warps hold a query's 128 scores, and registers go from the others to them
   // (256 x 192 + 256 x 56 of the launch's 512 x 128).
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp >= 13 && warp < 15) {
+    // (whose rows a tile's keys are is looked up only where some are not the sequence's: 613 rows behind 1500 42.6 us, with the look in every loop 42.9, a prompt of 4096 186, 192)
+    auto loads = [&](auto strangers) {
       for (;;) {
         const int segs = s_segs;
       // ================================ loads ================================
@@ -330,12 +357,22 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           ok = __all_sync(0xffffffffu, tc::mbar_wait_loop(empty + 8 * s, ((uint32_t)(tiles_done >> 1) & 1u) ^ 1u));
           if (!ok) break;
           const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
-          const bool whole = have == (1u << parts) - 1u;
+          bool whole = have == (1u << parts) - 1u;
+          uint32_t own = 0xffffffffu;   // lane l < 4: keys 32 l and on, but those of rows that are not the sequence's
+          if constexpr (strangers.value) {
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+              const int key = j * 128 + 32 * e + lane;
+              const uint32_t word = __ballot_sync(0xffffffffu, key >= total || whose_key(p, g.s, g.cached, g.first, key) == g.s);
+              if (lane == e) own = word;
+            }
+            whole = whole && __all_sync(0xffffffffu, own == 0xffffffffu);
+          }
           if (keys && lane < 4) {       // word l: keys 32 l and on
             uint32_t bits = 0u;
             if (p.shift >= 5) bits = (have >> ((lane * 32) >> min(p.shift, 7))) & 1u ? 0xffffffffu : 0u;
             else bits = ((have >> (2 * lane)) & 1u ? 0xffffu : 0u) | ((have >> (2 * lane + 1)) & 1u ? 0xffff0000u : 0u);
-            s_bits[tiles_done & 3][lane] = bits;
+            s_bits[tiles_done & 3][lane] = strangers.value ? bits & own : bits;
           }
           const int row = p.shift >= 7 ? (j * 128) & ((1 << p.shift) - 1) : 0;
           if (keys || (whole && (j + 1) * 128 <= total)) {
@@ -354,9 +391,10 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
             const uint32_t to = dst + s * C::kBytes + (uint32_t)(cc >> 3) * 16384u;
 #pragma unroll 8
             for (int i = 0; i < 128 / RP; ++i) {
-              const int r = i * RP + lane / CH, of = __shfl_sync(0xffffffffu, id, p.shift >= 7 ? 0 : r >> p.shift);
-              const bool in = of >= 0 && j * 128 + r < total;
-              cp16(to + (uint32_t)(r * 128 + (((cc & 7) ^ (r & 7)) << 4)), in ? base + (int64_t)of * p.v_page + (int64_t)((row + r) & ((1 << p.shift) - 1)) * HS : base, in);
+              const int r = i * RP + lane / CH, at = __shfl_sync(0xffffffffu, id, p.shift >= 7 ? 0 : r >> p.shift);
+              bool in = at >= 0 && j * 128 + r < total;
+              if constexpr (strangers.value) in = (__shfl_sync(0xffffffffu, own, r >> 5) >> (r & 31) & 1u) && in;
+              cp16(to + (uint32_t)(r * 128 + (((cc & 7) ^ (r & 7)) << 4)), in ? base + (int64_t)at * p.v_page + (int64_t)((row + r) & ((1 << p.shift) - 1)) * HS : base, in);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             tc::fence_smem_async();
@@ -382,6 +420,10 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         if (!more_segments()) break;
         __syncthreads();
       }
+    };
+    const bool loading = warp == 13 || warp == 14, checked = loading && strangers();
+    if (loading && !checked) {
+      loads(std::false_type{});
     } else if (warp == 12) {
       for (;;) {
         const int segs = s_segs;
@@ -449,6 +491,8 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
         if (!more_segments()) break;
         __syncthreads();
       }
+    } else if (checked) {
+      loads(std::true_type{});
     } else {
       while (more_segments()) __syncthreads();
     }
@@ -582,6 +626,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           hand_over(p_full);
         }
         tiles_before += g.hi - lo;
+        const int whose = tid < count ? p.row_seq[g.first + row] : -1;   // (of a row that is not the sequence's the queries are whatever lay there)
         const bool any = n[0] != n0;
         if (any && ok) {
           ok = __all_sync(0xffffffffu, tc::mbar_wait_loop(o_done + 8 * t, (n[0] - 1) & 1u));
@@ -596,8 +641,8 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
           const int slot = g.slot;
           const int hh = g.m0 + tid - row * p.per;
           if (slot < 0) {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
-            const int64_t y_at = tid < count ? ((int64_t)(g.first + row) * p.n_head + g.gi * p.per + hh) * HS : -1;
+            const float inv = l > 0.f ? 1.0f / l : 0.f;   // (NaN: the output is NaN itself)
+            const int64_t y_at = whose == g.s ? ((int64_t)(g.first + row) * p.n_head + g.gi * p.per + hh) * HS : -1;
 #pragma unroll 1
             for (int c0 = 0; c0 < HS; c0 += 32) {
               uint32_t o[32], x[16];
@@ -627,7 +672,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
                 if (to_row >= 0) *reinterpret_cast<uint4*>(p.out + to_row + c0 + (lane & 3) * 8) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
               }
             }
-            if (p.lse && tid < count) p.lse[g.q0 + tid] = l == 0.f ? INFINITY : m * sl + log2f(l);
+            if (p.lse && whose == g.s) p.lse[g.q0 + tid] = l == 0.f ? INFINITY : m * sl + log2f(l);
           } else {
             float* const at = p.tc_acc + (int64_t)slot * 256 * HS + tid * 4;   // four numbers of every query side by side: a warp's stores are whole lines (a query's all together: 4 us a segment)
 #pragma unroll 1
@@ -640,7 +685,7 @@ paged_tc05_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_q
                 for (int i = 0; i < 32; i += 4) __stcg(reinterpret_cast<uint4*>(at + (int64_t)(c0 + i) * 256), make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
               }
             }
-            if (tid < count) __stcg(p.tc_ml + (int64_t)slot * 256 + tid, make_float2(m == -INFINITY ? m : m * sl, any ? l : 0.f));
+            if (tid < count) __stcg(p.tc_ml + (int64_t)slot * 256 + tid, whose != g.s ? make_float2(-INFINITY, 0.f) : make_float2(m == -INFINITY ? m : m * sl, any ? l : 0.f));
           }
           tc::fence_before();
         }

@@ -56,6 +56,7 @@ __device__ __forceinline__ int steps_of(const KeyBlocks& b, int lane) {
 }
 
 struct KwSeg {
+  int s, row;                             // the sequence, its first row
   int q0, m;                              // the sequence's and group's first query in the workspace's order; queries
   int cached, n, table, gi;
   int block, lo, hi;                      // tiles of queries
@@ -195,6 +196,7 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
       if (at.lo > kKwLead && worker_of(first - at.lo + kKwLead) == w - 1) {   // (the first of those that go on with it joins it)
         c.first = w - 1;
         c.last = worker_of(first - at.lo + blk.steps(at.block) - 1);
+        c.s = at.s; c.row = seq.first; c.cached = seq.cached;
         c.table = seq.table; c.n = seq.n; c.gi = at.gi; c.block = at.block;
       }
     }
@@ -217,6 +219,7 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
         for (; c < kKwSegs && at.tile < at.end; c += s_seg[c].hi > s_seg[c].lo) {   // (a part without a tile is none)
           const int steps = blk.steps(at.block), stop = min(steps, at.lo + at.end - at.tile), from = blk.from(at.block);
           KwSeg& g = s_seg[c];
+          g.s = at.s; g.row = seq.first;
           g.q0 = (at.gi * p.rows + seq.first) * p.per;
           g.m = blk.m;
           g.cached = seq.cached; g.n = seq.n; g.table = seq.table; g.gi = at.gi;
@@ -416,8 +419,8 @@ paged_weights_kernel(const PagedParams p, const __grid_constant__ CUtensorMap ma
           if (lane == 0) tc::mbar_arrive(x_empty + 8 * w);
           if (g.slot >= 0) {
             __stcg(p.kw_part + g.slot * 128 + mine, both);
-          } else if (key < g.n) {
-            const int id = page_at(p, g.table, key >> p.shift);
+          } else {
+            const int id = key_page(p, g.s, g.table, g.cached, g.row, g.n, key);
             if (id >= 0) p.kw[(((int64_t)id * p.n_groups + g.gi) << p.shift) + (key & ((1 << p.shift) - 1))] += both;
           }
         }

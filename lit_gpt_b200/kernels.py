@@ -917,7 +917,7 @@ def attn_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, row_pos:
 
     qkv (rows, (H+2G)*hs) bf16 (further leading dimensions are rows, too); cos/sin: the model's FULL tables (positions, rope_n_elem), with ``table_preselected`` one row per row of qkv;
     row_pos int32/int64 (rows,): positions for the rotation (a cache that was cut down holds fewer keys than the sequence has positions); row_seq int32 (rows,): index of
-    each row's sequence in seqs, -1 for a row of none, whose result is zero; seqs int32 (S, 4) per sequence: first row, rows, keys in the cache before the step, row of the page
+    each row's sequence in seqs, -1 for a row of none, whose result is zero (one that a sequence's range holds, as the padded end of a chunk, has no query and leaves no key in its place); seqs int32 (S, 4) per sequence: first row, rows, keys in the cache before the step, row of the page
     table (``ragged.state_batch`` makes row_seq and seqs).  table int32 (sequences, pages): entry i of a row is the page of keys i * page and on; where an entry is no page, there are
     no keys -- new ones are dropped, the rest take no part.  k_pages / v_pages (pages, G, page, hs) bf16, updated in place, pages of 16, 32, 64, 128 or 256 keys, any distance between pages
     and groups that is a multiple of 8 numbers.  key_weights fp32 (pages, G, page): new keys begin at zero, every key gains the sum of its softmax weights over the step's rows and

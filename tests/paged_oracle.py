@@ -67,8 +67,13 @@ def step(d, rounded=0.0):
             id_ = int(d["pages"][at, j // page]) if j // page < d["pages"].shape[1] else -1
             place.append((id_, j % page) if 0 <= id_ < len(k) else None)
         turned = {}
+        mine = [int(x) == i for x in d["row_seq"][first : first + rows]]   # (a row of no sequence, or of another: no query, and no key in its place)
         for r in range(rows):
             row = first + r
+            if not mine[r]:
+                if cached + r < total:
+                    place[cached + r] = None
+                continue
             p = int(d["row_pos"][row])
             c, s = d["cos"][p], d["sin"][p]
             turned[r] = turn(heads[row, :, : per + 1], c, s, d["rope"])
@@ -87,7 +92,7 @@ def step(d, rounded=0.0):
         got, err = torch.zeros(G, len(there), dtype=F64), torch.zeros(G, len(there), dtype=F64)
         for r in range(rows):
             seen = index <= cached + r
-            if not seen.any():
+            if not seen.any() or not mine[r]:
                 continue
             q = turned[r][:, :per].to(F64)
             ks, vs = keys[:, seen], values[:, seen]

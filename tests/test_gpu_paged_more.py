@@ -12,12 +12,10 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("weights", [False, True])
 @pytest.mark.parametrize("per,hs", [(17, 64), (20, 128), (32, 64), (33, 128), (48, 128), (71, 64), (128, 64), (129, 128)])
-@pytest.mark.parametrize("cached", [[300], [4100] * 16, [5, 0, 2000]], ids=["one", "many", "unequal"])
-def test_single_tokens_of_wide_groups(K, formula, weights, per, hs, cached):
-    if per > 32:   # (they go to the tensor memory however few the keys are)
-        cached = cached[:4]
-    d = make([(1, n) for n in cached], 1, per, hs, 64, weights=weights, seed=per)
-    check(call(K, d), formula(d))
+def test_single_tokens_of_wide_groups(K, formula, weights, per, hs):
+    for cached in ([300], [4100] * (16 if per <= 32 else 4), [5, 0, 2000]):   # (wider ones go to the tensor memory however few the keys are)
+        d = make([(1, n) for n in cached], 1, per, hs, 64, weights=weights, seed=per)
+        check(call(K, d), formula(d))
 
 
 @pytest.mark.parametrize("tune,per,rows,n", [(1, 4, 100, 40), (3, 4, 100, 40), (0, 130, 9, 60), (1, 1, 4096, 200)])
@@ -30,7 +28,7 @@ def test_sequences_that_share_rows(E, tune, per, rows, n, weights):
     d["seqs"] = torch.tensor([first] * n, dtype=torch.int32)
     d["row_seq"] = torch.arange(rows, dtype=torch.int32) % n
     d["max_rows"] = rows
-    ref = oracle.step({**d, "seqs": d["seqs"][:1]})
+    ref = oracle.step({**d, "seqs": d["seqs"][:1], "row_seq": torch.zeros(rows, dtype=torch.int32)})   # (for the pages)
     before = E.attn_paged_tune(tune)
     try:
         junk = torch.full((1 << 26,), float("nan"), device="cuda")   # what a workspace may find in its place
@@ -78,13 +76,7 @@ def check_with_nan(got, bad, clean):
         assert over.max().item() <= 0, over.max().item()
 
 
-@pytest.mark.parametrize("hs,groups,per,page", [(64, 2, 4, 16), (128, 3, 1, 64), (128, 1, 16, 32)])
-@pytest.mark.parametrize("weights", [False, True])
-@pytest.mark.parametrize("steps", [[(1, 0)], [(1, 300)], [(1, 40), (1, 700), (1, 9)], [(1, 5000)], [(1, 40), (5, 3), (1, 9)], [(200, 100)], [(1, 60), (130, 700), (3, 0)]],
-                         ids=["first", "token", "tokens", "long", "short chunk", "chunk", "mixed"])
-@pytest.mark.parametrize("where", ["query", "key", "infinite query"])
-def test_what_is_not_a_number_stays_so(K, formula, hs, groups, per, page, weights, steps, where):
-    """A query that holds NaN, a key that does: results of the heads that see it are NaN, and so is the weight of every key that they see; no other's."""
+def one_of_nan(K, formula, weights, steps, where, hs, groups, per, page):
     d = make(steps, groups, per, hs, page, rope=0 if where == "infinite query" else None, weights=weights, seed=len(steps) + per)
     s = len(steps) // 2
     first, rows, cached, at = d["seqs"][s].tolist()
@@ -103,3 +95,55 @@ def test_what_is_not_a_number_stays_so(K, formula, hs, groups, per, page, weight
     else:
         heads(spoilt)[row] = float("nan" if where == "query" else "inf")
     check_with_nan(call(K, spoilt), formula(spoilt), clean)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("steps", [[(1, 0)], [(1, 300)], [(1, 40), (1, 700), (1, 9)], [(1, 5000)], [(1, 40), (5, 3), (1, 9)], [(200, 100)], [(1, 60), (130, 700), (3, 0)]],
+                         ids=["first", "token", "tokens", "long", "short chunk", "chunk", "mixed"])
+def test_what_is_not_a_number_stays_so(K, formula, weights, steps):
+    """A query that holds NaN, a key that does: results of the heads that see it are NaN, and so is the weight of every key that they see; no other's."""
+    for where in ("query", "key", "infinite query"):
+        for hs, groups, per, page in ((64, 2, 4, 16), (128, 3, 1, 64), (128, 1, 16, 32)):
+            one_of_nan(K, formula, weights, steps, where, hs, groups, per, page)
+
+
+def poison():
+    """What a workspace may find in its place."""
+    junk = [torch.full((1 << n,), float("nan"), device="cuda") for n in range(7, 27) for _ in range(2)]
+    del junk
+
+
+def one_of_strangers(K, formula, weights, steps, which, hs, groups, per, page):
+    d = make(steps, groups, per, hs, page, weights=weights, seed=len(steps) + per)
+    n = len(d["row_seq"])
+    for s, (first, rows, cached, at) in enumerate(d["seqs"].tolist()):
+        if s % 3 == 1 and which != "all":
+            continue
+        out = {"the end": range(rows - max(rows // 3, 1), rows), "the beginning": range(max(rows // 3, 1)), "every third": range(0, rows, 3), "all": range(rows), "another's": range(rows // 2, rows)}[which]
+        for r in out:
+            d["row_seq"][first + r] = (s + 1) % len(steps) if which == "another's" and len(steps) > 1 else (-1, len(steps), -(2 ** 31), 2 ** 31 - 1)[r % 4]
+            j = cached + r
+            d["k"][d["pages"][at, j // page], :, j % page], d["v"][d["pages"][at, j // page], :, j % page] = float("nan"), float("inf")
+    want = formula(d)
+    poison()
+    t = on_gpu(d)
+    got = launch(K, t), t["k"], t["v"], t["kw"]
+    check(got, want)
+    for row in range(n):
+        s = int(d["row_seq"][row])
+        if not 0 <= s < len(steps) or not d["seqs"][s, 0] <= row < d["seqs"][s, 0] + d["seqs"][s, 1]:
+            assert not got[0][row].any()
+    poison()
+    t = on_gpu(d)
+    assert same(got[0], launch(K, t)) and (not weights or same(got[3], t["kw"]))
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("steps", [[(1, 0), (1, 40), (1, 70)], [(1, 300)], [(40, 25)], [(5, 0), (7, 90), (3, 31), (8, 2)], [(300, 200)], [(1, 60), (170, 333), (2, 0), (90, 7)]],
+                         ids=["tokens", "token", "prompt", "short chunks", "chunk", "mixed"])
+def test_rows_within_a_range_that_are_not_the_sequence_s(K, formula, weights, steps):
+    """They have no query and no key, whatever lies in their places: results of zero, weights and pages as they were, nothing of them in the other rows."""
+    layouts = ((64, 2, 4, 16), (128, 3, 1, 64), (128, 1, 20, 32), (64, 1, 130, 256))
+    for i, which in enumerate(("the end", "the beginning", "every third", "all", "another's")):
+        for layout in (layouts[i % 4], layouts[(i + 1) % 4]):
+            one_of_strangers(K, formula, weights, steps, which, *layout)
