@@ -859,7 +859,8 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   s.list = s.list_max > 0;
   const int64_t most = max_rows * per < s.list_max ? max_rows * per : s.list_max;   // queries of an item
   s.nq = most <= 8 ? 1 : most <= 16 ? 2 : 4;
-  s.items = (int64_t)n_groups * ((rows * per + 8 * s.nq - 1) / (8 * s.nq) + n_seqs);
+  // (beside chunks, whose rows are none of the list's, an item holds the queries of any sequence and group that is)
+  s.items = (int64_t)n_groups * (s.tensor && most <= 8 * s.nq ? n_seqs : (rows * per + 8 * s.nq - 1) / (8 * s.nq) + n_seqs);
   const int warps = hs == 64 ? (s.nq == 4 ? PgSmem<64, 4>::kWarps : PgSmem<64, 1>::kWarps) : (s.nq == 4 ? PgSmem<128, 4>::kWarps : PgSmem<128, 1>::kWarps);
   const int64_t tiles = s.items * ((max_length + kShTile - 1) / kShTile);
   s.ctas = sm_count();
