@@ -10,6 +10,7 @@ shorter requests leaving the batch early); ``Replayer`` feeds it recorded steps 
 from __future__ import annotations
 
 import contextlib
+from collections import Counter
 from pathlib import Path
 from typing import Any, Callable, Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
@@ -256,9 +257,10 @@ class PagedSession:
 
     def step(self, entries: Sequence[Tuple[Any, Sequence[int], Optional[Sequence[int]]]], end: Iterable[Any] = ()) -> Optional[torch.Tensor]:
         """As ``Session.step``: entries (request id, its next tokens, places among them whose logits are wanted or None for all); returns the wanted logits, fp32 (rows, vocab),
-        in the order of the entries -- None when nothing is wanted."""
+        in the order of the entries -- None when nothing is wanted.  Other than there an entry's rows come in the order of its tokens, whatever that of `places` is (a place that is
+        named twice comes twice)."""
         K.raise_wait_errors()   # of the steps whose logits the caller has read since
-        todo = [(rid, list(toks), set(range(len(toks)) if places is None else (int(p) for p in places))) for rid, toks, places in entries if toks]
+        todo = [(rid, list(toks), Counter(range(len(toks)) if places is None else (int(p) for p in places))) for rid, toks, places in entries if toks]
         if len({rid for rid, _, _ in todo}) != len(todo):
             raise ValueError("a request has one entry in a step")
         need = 0
@@ -288,7 +290,7 @@ class PagedSession:
                     part.append((i, self.live[rid], toks[done[i] : done[i] + n]))
                     left -= n
             rows = [(i, done[i] + k) for i, _, toks in part for k in range(len(toks))]
-            want = [k for k, (i, place) in enumerate(rows) if place in todo[i][2]]
+            want = [k for k, (i, place) in enumerate(rows) for _ in range(todo[i][2][place])]
             for _, r, toks in part:
                 self._take(r, r.cached + len(toks))
             logits = self._run([r for _, r, _ in part], [toks for _, _, toks in part], want)
@@ -319,7 +321,7 @@ class PagedSession:
                 g = self._graph(len(requests), max(len(r.pages) for r in requests))
                 g.fill([t[0] for t in tokens], requests)
                 g.graph.replay()
-                return g.logits[: len(requests)].clone() if len(want) == len(requests) else g.logits[torch.tensor(want, device=dev)] if want else None
+                return g.logits[: len(requests)].clone() if want == list(range(len(requests))) else g.logits[torch.tensor(want, device=dev)] if want else None
             n, width = sum(len(t) for t in tokens), max(len(r.pages) for r in requests)
             seqs, row_seq, row_pos = [], [], []
             for i, (r, t) in enumerate(zip(requests, tokens)):
