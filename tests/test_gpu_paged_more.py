@@ -147,3 +147,134 @@ def test_rows_within_a_range_that_are_not_the_sequence_s(K, formula, weights, st
     for i, which in enumerate(("the end", "the beginning", "every third", "all", "another's")):
         for layout in (layouts[i % 4], layouts[(i + 1) % 4]):
             one_of_strangers(K, formula, weights, steps, which, *layout)
+
+
+# ---- single tokens without weights, every sequence and group by a cluster in one launch -------------------------------------------------
+TOKENS = [(1, 0), (1, 31), (1, 300), (1, 64)]
+
+
+@pytest.fixture
+def one_launch(E):
+    before = E.attn_paged_tune(4)
+    yield lambda d, **kw: call(E, d, **kw)
+    E.attn_paged_tune(before)
+
+
+def tokens(groups=2, per=4, hs=128, page=32, **kw):
+    d = make(TOKENS, groups, per, hs, page, weights=False, **kw)
+    assert d["max_rows"] == 1
+    return d
+
+
+def test_one_launch_rotations(one_launch):
+    for table in (torch.float32, torch.bfloat16):
+        for rope in (0, 2, 16, 48, 64):
+            d = tokens(hs=64, rope=rope, table=table, seed=rope)
+            check(one_launch(d), oracle.step(d))
+
+
+def test_one_launch_positions_apart_from_places(one_launch):
+    d = tokens(seed=9)
+    d["cos"], d["sin"] = (torch.cat([t] * 3) for t in (d["cos"], d["sin"]))
+    d["row_pos"] = (d["row_pos"].long() * 7 + 3) % len(d["cos"])
+    want = oracle.step(d)
+    check(one_launch(d), want)
+    d["cos"], d["sin"] = d["cos"][d["row_pos"]], d["sin"][d["row_pos"]]
+    check(one_launch(d, table_preselected=True), want)
+    d["qkv"] = d["qkv"].view(2, 2, -1)                       # leading dimensions
+    check(one_launch(d, table_preselected=True), want)
+
+
+def test_one_launch_strided_rows_and_a_wider_page_table(E, one_launch):
+    d = tokens(seed=10)
+    want = oracle.step(d)
+    t = on_gpu(d)
+    n, width = d["qkv"].shape
+    wide = torch.zeros(n, width + 72, device="cuda", dtype=torch.bfloat16)
+    wide[:, :width] = t["qkv"]
+    apart = torch.full((len(d["pages"]), 50), 77, device="cuda", dtype=torch.int32)
+    apart[:, : d["pages"].shape[1]] = t["pages"]
+    t["qkv"], t["pages"] = wide[:, :width], apart[:, : d["pages"].shape[1]]
+    check((launch(E, t), t["k"], t["v"], t["kw"]), want)
+
+
+@pytest.mark.parametrize("layout", ["keys beside values", "group by group", "apart"])
+def test_one_launch_page_layouts(E, one_launch, layout):
+    d = tokens(groups=3, per=2, seed=12)
+    t = on_gpu(d)
+    P, G, page, hs = d["k"].shape
+    if layout == "keys beside values":
+        both = torch.empty(P, 2, G, page, hs, device="cuda", dtype=torch.bfloat16)
+        k, v = both[:, 0], both[:, 1]
+    elif layout == "group by group":
+        k, v = (torch.empty(G, P, page, hs, device="cuda", dtype=torch.bfloat16).transpose(0, 1) for _ in range(2))
+    else:
+        k, v = (torch.empty(P * (G * (page * hs + 8) + 64), device="cuda", dtype=torch.bfloat16).as_strided((P, G, page, hs), (G * (page * hs + 8) + 64, page * hs + 8, hs, 1)) for _ in range(2))
+    k.copy_(t["k"])
+    v.copy_(t["v"])
+    t["k"], t["v"] = k, v
+    check((launch(E, t), k.contiguous(), v.contiguous(), None), oracle.step(d))
+
+
+def test_one_launch_offsets_past_32_bits(E, one_launch):
+    d = tokens(groups=1, per=2, page=256, seed=13)
+    t = on_gpu(d)
+    P, far = len(d["k"]), 2 ** 31 // (256 * 128) + 5
+    k, v = (torch.empty(far + P, 1, 256, 128, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    k[far:], v[far:] = t["k"], t["v"]
+    t.update(k=k, v=v, pages=torch.where(t["pages"] >= 0, t["pages"] + far, -1).int())
+    check((launch(E, t), k[far:], v[far:], None), oracle.step(d))
+
+
+def test_one_launch_reads_nothing_behind_the_last_key(one_launch):
+    d = tokens(seed=14)
+    page, want = d["k"].shape[2], oracle.step(d)
+    used = torch.zeros(d["k"].shape[0], page, dtype=torch.bool)
+    for first, rows, cached, at in d["seqs"].tolist():
+        for j in range(cached + rows):
+            used[d["pages"][at, j // page], j % page] = True
+    for x, bad in ((d["k"], float("nan")), (d["v"], float("inf"))):
+        x.permute(0, 2, 1, 3)[~used] = bad
+    check(one_launch(d), (*want[:2], *oracle.step(d)[2:]))
+
+
+def test_one_launch_bounds_and_sequences_that_do_not_fit(one_launch):
+    d = tokens(seed=15)
+    d["max_length"] = 60                                     # keys from here on are dropped: the new ones of the two longest among them
+    check(one_launch(d), oracle.step(d))
+    for seq in ((2, 1, 300, 99), (2, 1, 300, -1), (4, 1, 0, 0), (-1, 1, 0, 0), (2, 2, 300, 0), (2, 1, -3, 0)):
+        d = tokens(seed=15)
+        want = oracle.step({**d, "seqs": torch.cat((d["seqs"][:2], torch.zeros(1, 4, dtype=torch.int32), d["seqs"][3:]))})
+        d["seqs"][2] = torch.tensor(seq, dtype=torch.int32)
+        got = one_launch(d)
+        check(got, want)
+        assert not got[0][2].any()
+
+
+def test_one_launch_same_bits_two_streams_and_graphs(E, one_launch):
+    ds = [tokens(seed=20), tokens(hs=64, per=16, seed=21)]
+    wants, ts = [oracle.step(d) for d in ds], [on_gpu(d) for d in ds]
+    first = [launch(E, t) for t in ts]
+    for _ in range(3):
+        assert all(same(a, launch(E, t)) for a, t in zip(first, ts))
+    torch.cuda.synchronize()
+    outs, streams = [], [torch.cuda.Stream() for _ in ts]
+    for t, s in zip(ts, streams):
+        with torch.cuda.stream(s):
+            outs.append(launch(E, t))
+    torch.cuda.synchronize()
+    for t, out, want in zip(ts, outs, wants):
+        check((out, t["k"], t["v"], None), want)
+    graphs = []
+    for t in ts:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            graphs.append((g, launch(E, t)))
+    for d, t in zip(ds, ts):
+        t["k"].copy_(d["k"])
+        t["v"].copy_(d["v"])
+    for g, _ in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for (_, out), t, want in zip(graphs, ts, wants):
+        check((out, t["k"], t["v"], None), want)
