@@ -126,6 +126,8 @@ class GPT(nn.Module):
         caches = [b.attn.kv_cache for b in self.transformer.h]
         if not all(isinstance(c, PagedKVCache) for c in caches):
             raise TypeError("a paged step needs a PagedKVCache in every block")
+        if self.spans_devices():
+            raise NotImplementedError("a paged step runs on one GPU, this model's blocks are on several")
         n = tokens.numel()
         for c in caches:
             c.step = step

@@ -44,3 +44,22 @@ def test_a_token_beside_a_long_chunk_over_many_keys_is_not_refused():
                 v_group_stride=1024, out=0x10000, rows=16385, max_rows=16384, max_length=1 << 20, n_head=32, n_groups=32, head_size=64, workspace=0x10000, workspace_bytes=16)
     assert C.load().b200_attn_paged(ctypes.byref(C.AttnPagedArgs(**args)), None) == 1
     assert "workspace too small" in C.load().b200_last_error().decode()   # (what the call gets to: it has nothing against the step's size)
+
+
+def test_a_paged_step_over_several_devices_is_refused():
+    import torch
+
+    from lit_gpt_b200 import GPT, Config
+    from lit_gpt_b200.model import PagedKVCache
+    from lit_gpt_b200.ragged import PagedStep
+
+    config = Config(n_layer=2, n_head=2, n_embd=128, vocab_size=50, block_size=32)
+    model = GPT(config)
+    model.transformer.h[1].to("meta")
+    for b in model.transformer.h:
+        b.attn.kv_cache = PagedKVCache(config, 4, 16)
+    z = torch.zeros(1, dtype=torch.int32)
+    step = PagedStep(seqs=z.expand(1, 4), row_pos=z, row_seq=z, table=z[None], max_rows=1, max_length=16)
+    with pytest.raises(NotImplementedError, match="one GPU"):
+        model.paged_step(z, step)
+    assert all(b.attn.kv_cache.step is None for b in model.transformer.h)
