@@ -73,8 +73,9 @@ __device__ __forceinline__ int seq_tiles(const PagedSeq& s) { return (s.n + 31) 
 
 // Single tokens beside chunks: the list and the tensor memory run at the same time, on SMs of their own, as many as their work (in ns, of a group) asks for.  Both kernels come to the same
 // numbers, whole ones, each from its own look at the sequences.  What a step of either costs an SM: 16 KB of keys and values at 45 GB/s, 128 keys of 256 queries 3.4 us (beside the list; 2.1 alone); half heads 0.5 and
-// 0.75 of it.  us in a captured graph, one after the other and so: 32 tokens over 100 - 3001 keys beside 512 rows, 8 groups of 4 heads, 89, 75; 3 over 16000 beside 512 81, 78; 8 over 300 beside
-// 64, 32 groups, 32, 26; 64 over 500 beside 1000 rows behind 3000 131, 134; 2 over 100 beside 2048 103, 102.  (With 2.1 us 88, 98, 28, 142, 102; with 4.2 73, 73, 26, 150, 102.)
+// 0.75 of it.  us in a captured graph, when this was chosen, one after the other and so: 32 tokens over 100 - 3001 keys beside 512 rows, 8 groups of 4 heads, 89, 75; 3 over 16000 beside 512 81, 78; 8
+// over 300 beside 64, 32 groups, 32, 26; 64 over 500 beside 1000 rows behind 3000 131, 134; 2 over 100 beside 2048 103, 102.  (With 2.1 us 88, 98, 28, 142, 102; with 4.2 73, 73, 26, 150, 102.)  Since the
+// tensor memory's waits are shorter code: 74, 75, 27, 125, 96.
 struct Shares { unsigned long long list, tensor; };
 __device__ __forceinline__ void add_work(const PagedParams& p, const PagedSeq& s, Shares& w) {
   w.list += (unsigned long long)seq_items(p, s) * seq_tiles(s) * p.list_ns;

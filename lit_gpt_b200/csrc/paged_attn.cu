@@ -13,9 +13,9 @@
 // With the weights of keys wanted, the list keeps its scores beside the results, and a launch behind the join adds up what every key received: no key is read again.  What chunks' keys
 // receive is computed from the joined sums (paged_weights.cu).
 //
-// Bound: single tokens by the bytes of their keys and values: 64 of 8 groups of 4 heads over 5 - 16000 keys, 2.1 GB, 325 us, 6.45 TB/s; 16 of 32 groups over 2047 with weights, 546 MB, 104 us, 83 of
-// them the bytes: the rest the append's and the join's launches and the scores (with the keys read again for them 190).  Few of them by latency: 1 token of 32 groups over 300 keys 7.5 us (12.5 in
-// three launches).  Beside chunks: 32 tokens over 100 - 3001 keys and 512 rows behind 1024 75 us, where either alone takes 40 and 30.
+// Bound: single tokens by the bytes of their keys and values: 64 of 8 groups of 4 heads over 5 - 16000 keys, 2.1 GB, 325 us, 6.45 TB/s; 16 of 32 groups over 2047 with weights, 546 MB, 105 us, 83 of
+// them the bytes: the rest the append's and the join's launches and the scores (with the keys read again for them 190).  Few of them by latency: 1 token of 32 groups over 300 keys 7.7 us (13.5 in
+// three launches).  Beside chunks: 32 tokens over 100 - 3001 keys and 512 rows behind 1024 74 us, where either alone takes 40 and 30.
 #include "attn_list.cuh"
 #include "paged.cuh"
 
@@ -851,7 +851,7 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   PagedPlan s;
   const int path = g_paged_path.load(std::memory_order_relaxed);
   // chunks of one length only: all go to the tensor memory (some of them may turn out shorter, or not there)
-  // 17 to 32 queries: 8 groups of 4 heads, us of the list and of the tensor memory: 8 rows behind 500 keys 13.7, 17.4, behind 16000 38, 32; 16 times 8 rows behind 300 22, 24, behind 3000 82, 61
+  // 17 to 32 queries: 8 groups of 4 heads, us of the list and of the tensor memory: 8 rows behind 500 keys 13.5, 16.2, behind 16000 40, 29; 16 times 8 rows behind 300 23, 22, behind 3000 86, 55
   const bool short_ = (int64_t)n_seqs * n_groups * max_length <= 60000;
   const int singles = per <= 8 ? 8 : per <= 16 ? 16 : kListMax;   // beside chunks the list takes single tokens, in items as small as they are
   s.list_max = path == 1 || path == 3 || per > 128 ? 0x3fffffff : path == 2 ? 0 : max_rows * per <= (short_ ? kListMax : 16) ? kListMax : rows == (int64_t)n_seqs * max_rows ? 0 : singles;
@@ -892,9 +892,9 @@ PagedPlan paged_plan(int64_t rows, int n_seqs, int n_groups, int per, int hs, in
   }
   s.bytes = (size_t)s.slots * (hs + 2) * sizeof(float) + (size_t)s.q * 2 + (size_t)s.items * sizeof(int2) + (size_t)n_seqs * 2 * sizeof(int) +
             (kw ? (size_t)rows * per * n_groups * sizeof(float) : 0) + (size_t)s.scores * sizeof(float) + (size_t)s.kw_workers * (256 * sizeof(float) + sizeof(PagedWeightCut)) + (size_t)tc_slots * (hs + 2) * sizeof(float) + (size_t)s.tc_workers * sizeof(PagedCut);
-  // A cluster where its warps have four tiles each at most, and all clusters run at once.  us of the list and of clusters: 1 token of 32 groups, 128 numbers a head, over 300 keys 12.9, 7.5, over
-  // 2000 13.6, 10.4, over 8000 30.6, 28.1; of 8 groups of 4 heads over 8000 16.6, 17.2; 16 tokens of 32 groups over 300 18.5, 19.5; 64 of 8 groups over 100 14.4, 15.4; of 12 groups, 64 numbers
-  // a head, over 500 22.5, 17.9; 16 of them over 1000 16.4, 17.9.
+  // A cluster where its warps have four tiles each at most, and all clusters run at once.  us of the list and of clusters: 1 token of 32 groups, 128 numbers a head, over 300 keys 13.5, 7.7, over
+  // 2000 14.1, 10.7, over 8000 30.4, 28.3 (the list's all the same: more than four tiles a warp); of 8 groups of 4 heads over 8000 16.2, 16.8; 16 tokens of 32 groups over 300 18.3, 19.9; 64 of 8
+  // groups over 100 15.1, 16.2; 7 of 12 groups, 64 numbers a head, over 500 12.3, 8.3; 16 of them over 1000 16.0, 18.0.
   s.cluster = 0;
   if (max_rows == 1 && !kw && per <= 16 && (path == 0 || path == 4)) {   // (then the list takes every sequence, and nq queries hold a group's heads)
     const int64_t key_tiles = (max_length + kShTile - 1) / kShTile, pairs = (int64_t)n_seqs * n_groups;

@@ -15,11 +15,12 @@
 // Probabilities are rounded to bf16 as they multiply V; the running maximum is exact, so that the largest probability is 1 and loses nothing.  They are summed before the rounding: the
 // keys' weights are taken from these sums (of rounded ones a result's error against 64 bits is 0.1 to 0.4 % smaller, a weight's thousands of times larger).
 //
-// Bound: a stream's chain of scores, maximum, exponentials and output, which the other stream fills in part: a tile of 256 queries takes 3800 clocks where its products and its exponentials take
-// 2048 each.  4096 rows of 32 groups of 1 head 163 us, 0.84 PFLOP/s of the causal half (half of S read twice: 178); 613 rows behind 1500 keys, 8 groups of 4 heads, 33 us, 4 of them the way to the
-// first tile.  Not taken: half of a query's scores a thread, sixteen softmax warps at 80 registers: the step with 4096 rows 223 -> 275 us; the scores of the
-// next tile's keys 64 .. 127, whose place is free early, ahead of P V: 200 -> 222 (products of 64 columns cost shared memory nearly what those of 128 do).  A segment's results stored a query a thread in whole rows:
-// 4 us each; four numbers of 128 queries side by side: 2.
+// Bound: a stream's chain of scores, maximum, exponentials and output, which the other stream fills in part: a tile of 256 queries takes 3300 clocks where its products and its exponentials take
+// 2048 each.  4096 rows of 32 groups of 1 head 143 us, 0.96 PFLOP/s of the causal half; 613 rows behind 1500 keys, 8 groups of 4 heads, 32 us, 4 of them the way to the
+// first tile.  The instruction cache takes part: the roles walk different code, and each wait that was unrolled 64 times cost them all (tc05.cuh, mbar_wait_loop).
+// Not taken, measured while they were and the step with 4096 rows took 200 us and more: half of S read twice: products 163 -> 178; half of a query's scores a thread, sixteen softmax warps at 80
+// registers: the step 223 -> 275; the scores of the next tile's keys 64 .. 127, whose place is free early, ahead of P V: 200 -> 222 (products of 64 columns cost shared memory nearly what those of 128
+// do).  A segment's results stored a query a thread in whole rows: 4 us each; four numbers of 128 queries side by side: 2.
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 

@@ -11,7 +11,7 @@
 //   * warp 9 brings keys (a page, or what of it lies in the block, is one TMA box), queries (four stages) and the queries' lse
 // No atomics: one order of additions.
 //
-// Bound: the exponentials, 16 a clock and SM: 2048 clocks for two tiles of queries.  512 rows behind 2000 keys, 8 groups of 4 heads: 25 us, 10 of them the exponentials; the rest the way to the
+// Bound: the exponentials, 16 a clock and SM: 2048 clocks for two tiles of queries.  512 rows behind 2000 keys, 8 groups of 4 heads: 24 us, 10 of them the exponentials; the rest the way to the
 // first tile (6), and the sums' way out (on mma.sync, a tile of 32 keys a warp, 137).
 #include "attn_tmem.cuh"
 #include "paged.cuh"

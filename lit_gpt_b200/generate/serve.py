@@ -165,7 +165,9 @@ class PagedSession:
 
     pages, page: how many pages the pool has, and keys of a page (16, 32, 64, 128 or 256).  keep: a request's cache is cut down to that many keys whenever it holds a page more, every group of
     heads by itself: the first `first` keys and the last `recent` stay, and of the others those that received most attention (``kernels.evict_paged``); positions go on.  portion: rows of
-    one pass; longer prompts run in several, and are cut down between them."""
+    one pass; longer prompts run in several, and are cut down between them: while one runs a request holds up to `portion` keys more.
+
+    While a step runs the pool stands in the place of the model's own caches: one thread at a time works with a model, whether in its sessions or without."""
 
     GRAPHS = 8   # captured steps that are kept
 
